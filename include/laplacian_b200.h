@@ -41,7 +41,17 @@ enum lf_dtype {
     LF_F32 = 0,
     LF_F64 = 1,
     LF_F16 = 2,
-    LF_BF16 = 3
+    LF_BF16 = 3,
+    LF_F8E4M3 = 4 /* 8-bit operands of lf_linear_quant_fwd */
+};
+
+/* Activations of the block operators. */
+enum lf_activation {
+    LF_ACT_NONE = 0,
+    LF_ACT_RELU = 1,
+    LF_ACT_GELU = 2,      /* z Phi(z), by erf */
+    LF_ACT_GELU_TANH = 3, /* its tanh approximation */
+    LF_ACT_SILU = 4       /* z / (1 + exp(-z)) */
 };
 
 /* Status codes. */
@@ -344,6 +354,105 @@ LF_API int lf_laplace_sub_bwd_peers(const void* g, const void* q, const void* kT
                                     void* dq, void* dkT, void* const* dq_peers, int npeer,
                                     int64_t bh, int64_t n, int64_t m, int64_t d, int dtype,
                                     void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+   Block operators: what a transformer block needs around the attention.  The
+   reference has none of them (its callers use framework modules).  Sums,
+   statistics and accumulators are fp32; every output is rounded once.
+   Results do not depend on timing (no atomics).  Workspaces need no
+   initialisation; concurrent calls need distinct ones.
+   ------------------------------------------------------------------------- */
+
+/* y = s * rstd * weight with s = x + residual and rstd = 1/sqrt(mean(s^2) + eps)
+   per row of `cols`.  dtype F32, F16 or BF16.  residual and s (the sum, written
+   for the next block) are given together or both NULL (s = x).  rstd: NULL, or
+   `rows` floats, kept for lf_rms_norm_bwd. */
+LF_API int lf_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y, void* s, float* rstd,
+                           int64_t rows, int64_t cols, int dtype, double eps, lf_stream_t stream);
+
+/* Gradients of lf_rms_norm_fwd from dy and (NULL, or) the gradient ds of its
+   second output: dx = rstd (a - xhat mean(a xhat)) + ds with a = dy weight and
+   xhat = s rstd, which is the residual's gradient too, and
+   dw = sum over rows of dy xhat.  dx or dw may be NULL; dw needs
+   lf_rms_norm_bwd_workspace_size bytes of 16-byte aligned workspace. */
+LF_API size_t lf_rms_norm_bwd_workspace_size(int64_t rows, int64_t cols);
+LF_API int lf_rms_norm_bwd(const void* dy, const void* ds, const void* s, const float* rstd, const void* weight,
+                           void* dx, void* dw, int64_t rows, int64_t cols, int dtype, void* workspace,
+                           size_t workspace_bytes, lf_stream_t stream);
+
+/* lf_rms_norm_fwd with its output in 8 bits: per row scale = max|y| / 448 (1 for
+   a row of zeros) and q = e4m3(y / scale), from the unrounded y. */
+LF_API int lf_rms_norm_quant_fwd(const void* x, const void* residual, const void* weight, void* q, float* scale, void* s,
+                                 int64_t rows, int64_t cols, int dtype, double eps, lf_stream_t stream);
+
+/* The same quantisation of x itself (weights for lf_linear_quant_fwd). */
+LF_API int lf_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int dtype,
+                            lf_stream_t stream);
+
+/* y[m,n] = act(x[m,k] w[n,k]^T + bias[n]) + residual[m,n].  dtype F16 or BF16 for
+   every tensor; in lf_linear_quant_fwd x and w are e4m3 and the product is
+   scaled by x_scale[m] and w_scale[n] before the bias.  ldx, ldw, ldr, lddy:
+   elements between rows.  y, dx, dw and db are dense.  Zero-initialise the
+   struct; NULL leaves an operand or a gradient out. */
+typedef struct lf_linear {
+    const void *x, *w, *bias, *residual;
+    const float *x_scale, *w_scale;
+    void* y;
+    const void* dy;
+    void *dx, *dw, *db;
+    int64_t ldx, ldw, ldr, lddy;
+    int64_t m, n, k;
+    int32_t activation, dtype;
+} lf_linear_t;
+
+LF_API size_t lf_linear_fwd_workspace_size(const lf_linear_t* args);
+LF_API int lf_linear_fwd(const lf_linear_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
+LF_API size_t lf_linear_quant_fwd_workspace_size(const lf_linear_t* args);
+LF_API int lf_linear_quant_fwd(const lf_linear_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
+/* Gradients of lf_linear_fwd: with z = x w^T + bias recomputed where there is
+   an activation, dz = dy act'(z) (rounded to dtype as an operand of the
+   products that follow), dx = dz w, dw = dz^T x, db = sum of dz's rows.  The
+   residual's gradient is dy.  The workspace sizes of this and the other
+   struct entry points depend on the sizes, the strides, the alignment of the
+   pointers and which gradients are asked for: ask with the struct that will
+   run.  Workspaces are 256-byte aligned. */
+LF_API size_t lf_linear_bwd_workspace_size(const lf_linear_t* args);
+LF_API int lf_linear_bwd(const lf_linear_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
+/* Gated feed-forward block on m tokens of c channels, hidden width f:
+   [g|u] = x w_in^T + b_in with w_in [2f, c] (gate rows, then up rows),
+   h = act(g) u (rounded to dtype as an operand), y = h w_out^T + b_out + residual
+   with w_out [c, f].  Weights, y and the gradients are dense. */
+typedef struct lf_gated_ffn {
+    const void *x, *w_in, *b_in, *w_out, *b_out, *residual;
+    void* y;
+    const void* dy;
+    void *dx, *dw_in, *db_in, *dw_out, *db_out;
+    int64_t ldx, ldr, lddy;
+    int64_t m, c, f;
+    int32_t activation, dtype;
+} lf_gated_ffn_t;
+
+LF_API size_t lf_gated_ffn_fwd_workspace_size(const lf_gated_ffn_t* args);
+LF_API int lf_gated_ffn_fwd(const lf_gated_ffn_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
+/* Gradients of lf_gated_ffn_fwd; g, u and h are recomputed from x (nothing but
+   the inputs is kept between the passes).  The residual's gradient is dy. */
+LF_API size_t lf_gated_ffn_bwd_workspace_size(const lf_gated_ffn_t* args);
+LF_API int lf_gated_ffn_bwd(const lf_gated_ffn_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
+/* norm = sqrt of the sum of squares over all `count` tensors, and
+   outs[i] = min(1, max_norm / (norm + 1e-6)) * grads[i].  Tensor i has sizes[i]
+   elements of type dtypes[i] (F32, F16 or BF16, mixed freely); outs[i] may be
+   grads[i].  A norm that is not finite gives what the formula gives (NaN
+   gradients).  The tables are host arrays, read before the call returns;
+   norm is one device float. */
+LF_API size_t lf_clip_grad_norm_workspace_size(const int64_t* sizes, int64_t count);
+LF_API int lf_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes,
+                             int64_t count, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                             lf_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "liblfb200.so")
 
-LF_F32, LF_F64, LF_F16, LF_BF16 = 0, 1, 2, 3
+LF_F32, LF_F64, LF_F16, LF_BF16, LF_F8E4M3 = 0, 1, 2, 3, 4
 LF_OK, LF_ERR_INVALID, LF_ERR_DTYPE, LF_ERR_UNSUPPORTED, LF_ERR_CUDA, LF_ERR_TIMEOUT = range(6)
 INIT_REFERENCE, INIT_SCALED_TRANSPOSE = 0, 1
 PREC_SPLIT3, PREC_MIXED, PREC_FP32_SIMT = 0, 1, 2
@@ -26,6 +26,27 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _D = ctypes.c_double
+
+
+
+class Linear(ctypes.Structure):
+    """lf_linear_t: one matrix product with its epilogue and gradients."""
+
+    _fields_ = ([(n, _P) for n in ("x", "w", "bias", "residual", "x_scale", "w_scale", "y", "dy", "dx", "dw", "db")]
+                + [(n, _I64) for n in ("ldx", "ldw", "ldr", "lddy", "m", "n", "k")]
+                + [(n, ctypes.c_int32) for n in ("activation", "dtype")])
+
+
+class GatedFfn(ctypes.Structure):
+    """lf_gated_ffn_t: one gated feed-forward block and its gradients."""
+
+    _fields_ = ([(n, _P) for n in ("x", "w_in", "b_in", "w_out", "b_out", "residual", "y", "dy", "dx", "dw_in", "db_in",
+                                   "dw_out", "db_out")]
+                + [(n, _I64) for n in ("ldx", "ldr", "lddy", "m", "c", "f")]
+                + [(n, ctypes.c_int32) for n in ("activation", "dtype")])
+
+
+_LIN, _FFN, _SZ = ctypes.POINTER(Linear), ctypes.POINTER(GatedFfn), ctypes.c_size_t
 
 # name -> (restype, argtypes); the exported symbol set of include/laplacian_b200.h
 SIGNATURES = {
@@ -62,6 +83,23 @@ SIGNATURES = {
     "lf_peer_barrier": (_I, [_P, _I, _I, ctypes.c_uint32, _I, _P]),
     "lf_laplace_sub_bwd_peers": (_I, [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I, _P, ctypes.c_size_t,
                                       _P]),
+    "lf_rms_norm_fwd": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I, _D, _P]),
+    "lf_rms_norm_bwd_workspace_size": (_SZ, [_I64, _I64]),
+    "lf_rms_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I, _P, _SZ, _P]),
+    "lf_rms_norm_quant_fwd": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I, _D, _P]),
+    "lf_quantize_rows": (_I, [_P, _P, _P, _I64, _I64, _I, _P]),
+    "lf_linear_fwd_workspace_size": (_SZ, [_LIN]),
+    "lf_linear_fwd": (_I, [_LIN, _P, _SZ, _P]),
+    "lf_linear_quant_fwd_workspace_size": (_SZ, [_LIN]),
+    "lf_linear_quant_fwd": (_I, [_LIN, _P, _SZ, _P]),
+    "lf_linear_bwd_workspace_size": (_SZ, [_LIN]),
+    "lf_linear_bwd": (_I, [_LIN, _P, _SZ, _P]),
+    "lf_gated_ffn_fwd_workspace_size": (_SZ, [_FFN]),
+    "lf_gated_ffn_fwd": (_I, [_FFN, _P, _SZ, _P]),
+    "lf_gated_ffn_bwd_workspace_size": (_SZ, [_FFN]),
+    "lf_gated_ffn_bwd": (_I, [_FFN, _P, _SZ, _P]),
+    "lf_clip_grad_norm_workspace_size": (_SZ, [_P, _I64]),
+    "lf_clip_grad_norm": (_I, [_P, _P, _P, _P, _I64, _D, _P, _P, _SZ, _P]),
 }
 
 LF_MAX_PEERS = 8

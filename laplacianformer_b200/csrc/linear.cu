@@ -1,0 +1,1312 @@
+// Matrix products with fused epilogues on the tcgen05 tensor cores, and the
+// operators made of them:
+//
+//   linear      z = x W^T + b,  y = act(z) + r
+//               dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum dz
+//   8-bit form  z = sx sw (q qw^T) + b on e4m3 operands
+//   gated FFN   [g|u] = x Win^T + bin,  h = act(g) u,  y = h Wout^T + bout + r
+//               dh = dy Wout,  dg = dh u act'(g),  du = dh act(g)
+//               dx = [dg|du] Win,  dWin = [dg|du]^T x,  dWout = dy^T h
+//
+// One persistent kernel (tc_gemm_kernel) runs every product: operands come
+// through TMA into a ring of 128-byte-swizzled stages, one warp issues the
+// tcgen05 products into accumulators in tensor memory, and eight warps turn
+// finished accumulators into outputs while the next tile's products run.
+// Either operand may be stored K-major or transposed (MN-major), so no
+// product needs a transposed copy.  The backward passes recompute z, g, u and
+// h from x in 32 bits instead of reading rounded copies of them back.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "tc_ptx.cuh"
+
+namespace lfb {
+
+// Set by a kernel whose bounded wait expired (merged into lf_device_status).
+__device__ int g_gemm_status = 0;
+
+int gemm_status(bool clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int)) != cudaSuccess) return LF_ERR_CUDA;
+    if (clear) {
+        int z = 0;
+        if (cudaMemcpyToSymbol(g_gemm_status, &z, sizeof(int)) != cudaSuccess) return LF_ERR_CUDA;
+    }
+    return v;
+}
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Activations
+// ---------------------------------------------------------------------------
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+    if constexpr (ACT == LF_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps NaN
+    if constexpr (ACT == LF_ACT_SILU) return z * __fdividef(1.f, 1.f + __expf(-z));
+    if constexpr (ACT == LF_ACT_GELU) return z * (0.5f + 0.5f * erff(z * 0.70710678118654752f));
+    if constexpr (ACT == LF_ACT_GELU_TANH) {
+        const float t = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+        return z * (1.f - __fdividef(1.f, 1.f + __expf(2.f * t)));  // (1 + tanh t)/2
+    }
+    return z;
+}
+
+// The activation's value and derivative.
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float& a, float& slope) {
+    if constexpr (ACT == LF_ACT_RELU) {
+        a = z < 0.f ? 0.f : z;
+        slope = z > 0.f ? 1.f : 0.f;
+    } else if constexpr (ACT == LF_ACT_SILU) {
+        const float p = __fdividef(1.f, 1.f + __expf(-z));
+        a = z * p;
+        slope = p * (1.f + z * (1.f - p));
+    } else if constexpr (ACT == LF_ACT_GELU) {
+        const float p = 0.5f + 0.5f * erff(z * 0.70710678118654752f);
+        a = z * p;
+        slope = p + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    } else if constexpr (ACT == LF_ACT_GELU_TANH) {
+        const float k = 0.79788456080286536f, c = 0.044715f;
+        const float q = 1.f - __fdividef(1.f, 1.f + __expf(2.f * k * (z + c * z * z * z)));  // (1 + tanh)/2
+        a = z * q;
+        slope = q + 2.f * z * q * (1.f - q) * k * (1.f + 3.f * c * z * z);
+    } else {
+        a = z;
+        slope = 1.f;
+    }
+}
+
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+    switch (act) {
+        case LF_ACT_RELU: f(std::integral_constant<int, LF_ACT_RELU>()); break;
+        case LF_ACT_GELU: f(std::integral_constant<int, LF_ACT_GELU>()); break;
+        case LF_ACT_GELU_TANH: f(std::integral_constant<int, LF_ACT_GELU_TANH>()); break;
+        case LF_ACT_SILU: f(std::integral_constant<int, LF_ACT_SILU>()); break;
+        default: f(std::integral_constant<int, LF_ACT_NONE>()); break;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit pairs
+// ---------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+
+// Four consecutive elements of a row of n at p (column c); beyond the row: 0.
+template <typename T>
+__device__ __forceinline__ uint2 load4(const T* p, int c, int n, bool vec) {
+    if (vec && c + 4 <= n) return *reinterpret_cast<const uint2*>(p + c);
+    uint2 u = make_uint2(0u, 0u);
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (c + j < n) e[j] = p[c + j];
+    return u;
+}
+template <typename T>
+__device__ __forceinline__ float4 widen4(uint2 u) {
+    const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int c, int n, bool vec, float4 v) {
+    const uint2 u = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+    if (vec && c + 4 <= n) {
+        *reinterpret_cast<uint2*>(p + c) = u;
+        return;
+    }
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (c + j < n) p[c + j] = e[j];
+}
+
+// What follows the product of one output: bias, activation, residual; or,
+// for the backward, the activation's derivative times the upstream gradient.
+struct Epilogue {
+    void* out;
+    const void *bias, *res;  // res: the residual, or dy when act_bwd
+    const float *sa, *sb;    // row and column scales of the 8-bit form
+    int64_t ldo, ldr;
+    int act;
+    bool act_bwd, vec_out, vec_res;
+};
+
+template <int ACT>
+__device__ __forceinline__ float4 finish4(float4 z, float4 bias, float4 r, bool act_bwd) {
+    z.x += bias.x, z.y += bias.y, z.z += bias.z, z.w += bias.w;
+    if (act_bwd) {
+        float a, s;
+        act_both<ACT>(z.x, a, s), z.x = r.x * s;
+        act_both<ACT>(z.y, a, s), z.y = r.y * s;
+        act_both<ACT>(z.z, a, s), z.z = r.z * s;
+        act_both<ACT>(z.w, a, s), z.w = r.w * s;
+        return z;
+    }
+    return make_float4(act_value<ACT>(z.x) + r.x, act_value<ACT>(z.y) + r.y, act_value<ACT>(z.z) + r.z,
+                       act_value<ACT>(z.w) + r.w);
+}
+
+// ---------------------------------------------------------------------------
+// The product kernel
+// ---------------------------------------------------------------------------
+enum Mode { kLinear, kGated, kGatedBwd };
+
+constexpr int kBM = 128;                  // rows of a tile (tcgen05 M)
+constexpr int kRowBytes = 128;            // a stage holds 128 bytes of K: 64 16-bit or 128 8-bit elements
+constexpr int kEpiWarps = 8;              // two per 32-lane quarter of the tensor memory
+constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
+constexpr int kStageOut = 4096;           // output staging per epilogue warp
+constexpr int kMaxStages = 8;
+constexpr int kTmemAll = 512;
+constexpr int kBarrierBytes = 256;
+constexpr int kSmemLimit = 227 * 1024;
+constexpr int kGroupM = 16;               // row tiles that are walked together, so that their operands stay in L2
+
+struct alignas(64) GemmArgs {
+    CUtensorMap a, b, a2, b2;  // a2, b2: dy and Wout of the gated backward
+    Epilogue e;
+    float* part;               // split K: raw sums [split][rows][ldp]
+    int64_t ldp, plane;        // plane: elements between dg, du and h (gated backward)
+    int m, n;                  // rows of one row segment; output columns (hidden columns of the gated modes)
+    int msegs, tiles_m, tiles_n, splits;
+    int iters, split_iters, seg_iters;  // K steps in all, per split, per K segment
+    int bn, stages, nbuf;      // columns of the first product; ring depth; accumulator buffers
+    uint32_t idesc, idesc2;
+    bool a_mn, b_mn;
+};
+
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t go) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(go)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+struct Tile {
+    int seg, m0, n0, split, it0, it1;
+};
+// Work units: for each split of K, row tiles in groups of kGroupM, within a
+// group all row tiles of one column tile before the next column tile.
+__device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out) {
+    const int rows = p.msegs * p.tiles_m, tiles = rows * p.tiles_n;
+    Tile t;
+    t.split = unit / tiles;
+    int r = unit - t.split * tiles;
+    const int group = r / (kGroupM * p.tiles_n), first = group * kGroupM;
+    const int gm = min(kGroupM, rows - first);
+    r -= group * kGroupM * p.tiles_n;
+    const int mi = first + r % gm;
+    t.n0 = (r / gm) * bn_out;
+    t.seg = mi / p.tiles_m;
+    t.m0 = (mi - t.seg * p.tiles_m) * kBM;
+    t.it0 = t.split * p.split_iters;
+    t.it1 = min(p.iters, t.it0 + p.split_iters);
+    return t;
+}
+
+// 32 rows x 32 16-bit columns of one warp, staged in shared memory (64-byte
+// rows, 16-byte chunks swizzled so that neither side has bank conflicts) and
+// written as 64-byte row segments.  v: the calling lane's row.
+template <typename T>
+__device__ __forceinline__ void stage16(uint8_t* st, int lane, const float (&v)[32]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint4 u = make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
+                                   pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+        *reinterpret_cast<uint4*>(st + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = u;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void unstage16(const uint8_t* st, int lane, T* out, int64_t ld, int row0, int rows, int col0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2), c = lane & 3;
+        if (row0 + row < rows && col0 + c * 8 < ld)
+            *reinterpret_cast<uint4*>(out + (row0 + row) * ld + col0 + c * 8) =
+                *reinterpret_cast<const uint4*>(st + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+    }
+}
+
+// Reads 32 bias values of columns col0.. into per-warp shared memory.
+template <typename T>
+__device__ __forceinline__ void bias_to_smem(float* sb, const T* bias, int lane, int col0, int n) {
+    sb[lane] = bias && col0 + lane < n ? Elem<T>::load(bias[col0 + lane]) : 0.f;
+}
+
+template <typename T, int MODE, bool FP8>
+__global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs p) {
+    extern __shared__ __align__(1024) uint8_t smem[];  // stages, output staging, barriers
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int BK = FP8 ? 128 : 64;
+    const int bh = p.bn / 2;                                   // hidden columns of a gated tile
+    const int bn_out = MODE == kLinear ? p.bn : bh;
+    const int cols = MODE == kGatedBwd ? 3 * bh : p.bn;        // accumulator columns
+    constexpr int kABytes = kBM * kRowBytes * (MODE == kGatedBwd ? 2 : 1);
+    const int stage_bytes = kABytes + (MODE == kGatedBwd ? 3 * bh : p.bn) * kRowBytes;
+    uint8_t* out_stage = smem + p.stages * stage_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * kStageOut);
+    uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *drain = tempty + 2;
+    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps);
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(tmem_ptr, kTmemAll);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    const int units = p.splits * p.msegs * p.tiles_m * p.tiles_n;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
+                const Tile t = tile_of(p, unit, bn_out);
+                for (int it = t.it0; it < t.it1; ++it) {
+                    if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
+                    const int ks = it / p.seg_iters, k0 = (it - ks * p.seg_iters) * BK;
+                    uint8_t* sa = smem + s * stage_bytes;
+                    uint8_t* sb = sa + kABytes;
+                    mbar_expect(&full[s], stage_bytes);
+                    if (!p.a_mn) tma_load(sa, &p.a, &full[s], k0, t.m0, ks);
+                    else
+                        for (int j = 0; j < kBM / 64; ++j) tma_load(sa + j * 8192, &p.a, &full[s], t.m0 + 64 * j, k0, t.seg);
+                    if (MODE == kLinear) {
+                        if (!p.b_mn) tma_load(sb, &p.b, &full[s], k0, t.n0, ks);
+                        else
+                            for (int j = 0; j < p.bn / 64; ++j)
+                                tma_load(sb + j * 8192, &p.b, &full[s], t.n0 + 64 * j, k0, ks);
+                    } else {
+                        tma_load(sb, &p.b, &full[s], k0, t.n0, 0);
+                        tma_load(sb + bh * kRowBytes, &p.b, &full[s], k0, t.n0, 1);
+                    }
+                    if (MODE == kGatedBwd) {
+                        tma_load(sa + kBM * kRowBytes, &p.a2, &full[s], k0, t.m0, 0);
+                        for (int j = 0; j < bh / 64; ++j)
+                            tma_load(sb + p.bn * kRowBytes + j * 8192, &p.b2, &full[s], t.n0 + 64 * j, k0, 0);
+                    }
+                    ++issued;
+                    if (++s == p.stages) s = 0, ph ^= 1;
+                }
+            }
+            // A wait ran out: let the copies in flight land before the block ends.
+            if (!ok)
+                for (int k = max(0, issued - p.stages); k < issued; ++k)
+                    mbar_wait(&full[k % p.stages], (k / p.stages) & 1, 100000000ull);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t go = elect_one() ? 1u : 0u;
+        const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
+        const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
+        int s = 0, buf = 0;
+        uint32_t ph = 0, bph = 0;
+        for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
+            const Tile t = tile_of(p, unit, bn_out);
+            if (!(ok = mbar_wait(&tempty[buf], bph ^ 1))) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * cols;
+            for (int it = t.it0; it < t.it1; ++it) {
+                if (!(ok = mbar_wait(&full[s], ph))) break;
+                tc_fence_after();
+                const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + kABytes;
+                const uint64_t da = make_desc(sa, a_lbo, 1024), db = make_desc(sb, b_lbo, 1024);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t add = it > t.it0 || k > 0 ? 1u : 0u;
+                    if (FP8) mma_f8(acc, da + k * a_step, db + k * b_step, p.idesc, add, go);
+                    else mma_f16(acc, da + k * a_step, db + k * b_step, p.idesc, add, go);
+                }
+                if (MODE == kGatedBwd) {
+                    const uint64_t da2 = make_desc(sa + kBM * kRowBytes, 16, 1024);
+                    const uint64_t db2 = make_desc(sb + p.bn * kRowBytes, 8192, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f16(acc + p.bn, da2 + k * 2, db2 + k * 128, p.idesc2, it > t.it0 || k > 0 ? 1u : 0u, go);
+                }
+                if (go) mma_commit(&empty[s]);
+                if (++s == p.stages) s = 0, ph ^= 1;
+            }
+            if (!ok) break;
+            if (go) mma_commit(&tfull[buf]);
+            if (++buf == p.nbuf) buf = 0, bph ^= 1;
+        }
+        if (!ok) {  // products in flight end before the tensor memory is freed
+            if (go) mma_commit(drain);
+            mbar_wait(drain, 0, 100000000ull);
+        }
+    } else {
+        const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+        uint8_t* st = out_stage + ew * kStageOut;
+        int buf = 0;
+        uint32_t bph = 0;
+        const Epilogue& e = p.e;
+        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+            const Tile t = tile_of(p, unit, bn_out);
+            if (!(ok = mbar_wait(&tfull[buf], bph))) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * cols + ((uint32_t)(quad * 32) << 16);
+            const int row0 = t.m0 + quad * 32;
+            for (int c0 = half * 32; c0 < bn_out; c0 += 64) {
+                if (t.n0 + c0 >= p.n) break;
+                const int col0 = t.n0 + c0;
+                if constexpr (MODE == kLinear) {
+                    // Raw sums through shared memory, so that a lane has four
+                    // columns and residual, bias and output are row segments.
+                    const int col = col0 + (lane & 7) * 4;
+                    const int64_t seg_row = (int64_t)t.seg * p.m;
+                    uint2 r[8];
+                    if (e.res && !p.part) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int row = row0 + i * 4 + (lane >> 3);
+                            r[i] = row < p.m ? load4((const T*)e.res + (seg_row + row) * e.ldr, col, p.n, e.vec_res)
+                                             : make_uint2(0u, 0u);
+                        }
+                    }
+                    float v[32];
+                    tmem_ld32(acc + c0, v);
+                    tmem_wait_ld();
+                    reg_fence(v);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                    __syncwarp();
+                    auto staged = [&](int i) {
+                        const int row = i * 4 + (lane >> 3);
+                        return *reinterpret_cast<const float4*>(st + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+                    };
+                    if (p.part) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int row = row0 + i * 4 + (lane >> 3);
+                            if (row < p.m && col < p.ldp)
+                                *reinterpret_cast<float4*>(
+                                    p.part + ((int64_t)t.split * p.msegs * p.m + seg_row + row) * p.ldp + col) = staged(i);
+                        }
+                    } else {
+                        float4 b = make_float4(0.f, 0.f, 0.f, 0.f), sb = make_float4(1.f, 1.f, 1.f, 1.f);
+                        if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, p.n, false));
+                        if (FP8) {
+                            float* q = reinterpret_cast<float*>(&sb);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) q[j] = col + j < p.n ? e.sb[col + j] : 0.f;
+                        }
+                        with_act(e.act, [&](auto act) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int row = row0 + i * 4 + (lane >> 3);
+                                if (row < p.m) {
+                                    float4 z = staged(i);
+                                    if (FP8) {
+                                        const float s = e.sa[seg_row + row];
+                                        z.x *= s * sb.x, z.y *= s * sb.y, z.z *= s * sb.z, z.w *= s * sb.w;
+                                    }
+                                    const float4 x = e.res ? widen4<T>(r[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                    store4((T*)e.out + (seg_row + row) * e.ldo, col, p.n, e.vec_out,
+                                           finish4<decltype(act)::value>(z, b, x, e.act_bwd));
+                                }
+                            }
+                        });
+                    }
+                    __syncwarp();
+                } else if constexpr (MODE == kGated) {
+                    float g[32], u[32];
+                    float* sb = reinterpret_cast<float*>(st + 2048);
+                    if (e.bias) {
+                        bias_to_smem(sb, (const T*)e.bias, lane, col0, p.n);
+                        bias_to_smem(sb + 32, (const T*)e.bias + p.n, lane, col0, p.n);
+                    }
+                    tmem_ld32(acc + c0, g);
+                    tmem_ld32(acc + bh + c0, u);
+                    tmem_wait_ld();
+                    reg_fence(g);
+                    reg_fence(u);
+                    __syncwarp();
+                    if (e.bias) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) g[j] += sb[j], u[j] += sb[32 + j];
+                    }
+                    with_act(e.act, [&](auto act) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
+                    });
+                    stage16<T>(st, lane, u);
+                    __syncwarp();
+                    unstage16(st, lane, (T*)e.out, e.ldo, row0, p.m, col0);
+                    __syncwarp();
+                } else {
+                    float g[32], u[32], d[32];
+                    float* sb = reinterpret_cast<float*>(st);
+                    if (e.bias) {
+                        bias_to_smem(sb, (const T*)e.bias, lane, col0, p.n);
+                        bias_to_smem(sb + 32, (const T*)e.bias + p.n, lane, col0, p.n);
+                    }
+                    tmem_ld32(acc + c0, g);
+                    tmem_ld32(acc + bh + c0, u);
+                    tmem_wait_ld();
+                    reg_fence(g);
+                    reg_fence(u);
+                    __syncwarp();
+                    if (e.bias) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) g[j] += sb[j], u[j] += sb[32 + j];
+                        __syncwarp();
+                    }
+                    // g, u become h's two factors' products: h in d, act(g) in g, u act'(g) in u.
+                    with_act(e.act, [&](auto act) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            float a, slope;
+                            act_both<decltype(act)::value>(g[j], a, slope);
+                            d[j] = a * u[j];
+                            g[j] = a;
+                            u[j] *= slope;
+                        }
+                    });
+                    stage16<T>(st, lane, d);
+                    tmem_ld32(acc + 2 * bh + c0, d);
+                    __syncwarp();
+                    T* out = (T*)e.out;
+                    unstage16(st, lane, out + 2 * p.plane, e.ldo, row0, p.m, col0);
+                    tmem_wait_ld();
+                    reg_fence(d);
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) u[j] *= d[j], g[j] *= d[j];
+                    stage16<T>(st, lane, u);
+                    stage16<T>(st + 2048, lane, g);
+                    __syncwarp();
+                    unstage16(st, lane, out, e.ldo, row0, p.m, col0);
+                    unstage16(st + 2048, lane, out + p.plane, e.ldo, row0, p.m, col0);
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[buf]);
+            if (++buf == p.nbuf) buf = 0, bph ^= 1;
+        }
+    }
+    if (!ok && lane == 0) atomicExch(&g_gemm_status, (int)LF_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kTmemAll);
+}
+
+// Joins the splits of K in order and applies the epilogue.
+template <typename T>
+__global__ void __launch_bounds__(256) split_join_kernel(const float* part, int splits, int64_t rows, int n, int64_t ldp,
+                                                         const Epilogue e) {
+    const int64_t groups = ldp / 4, total = rows * groups;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / groups;
+        const int col = (int)(i - row * groups) * 4;
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < splits; ++s) {
+            const float4 v = *reinterpret_cast<const float4*>(part + ((int64_t)s * rows + row) * ldp + col);
+            z.x += v.x, z.y += v.y, z.z += v.z, z.w += v.w;
+        }
+        if (e.sa) {
+            const float s = e.sa[row];
+            float* q = reinterpret_cast<float*>(&z);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] *= s * (col + j < n ? e.sb[col + j] : 0.f);
+        }
+        float4 b = make_float4(0.f, 0.f, 0.f, 0.f), x = b;
+        if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, n, false));
+        if (e.res) x = widen4<T>(load4((const T*)e.res + row * e.ldr, col, n, e.vec_res));
+        with_act(e.act, [&](auto act) {
+            store4((T*)e.out + row * e.ldo, col, n, e.vec_out, finish4<decltype(act)::value>(z, b, x, e.act_bwd));
+        });
+    }
+}
+
+// Copies a matrix whose rows TMA cannot address (row pitch or base not a
+// multiple of 16 bytes) to rows of ldo elements.
+template <typename U>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const U* in, int64_t ldi, U* out, int64_t ldo, int64_t rows, int64_t cols) {
+    const int64_t total = rows * cols;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / cols, c = i - r * cols;
+        out[r * ldo + c] = in[r * ldi + c];
+    }
+}
+
+// Column sums, first step: part[slice][c] over the rows of a slice.  A thread
+// adds V neighbouring columns; the block's eight row walkers join in order.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) colsum_kernel(const T* in, int64_t ld, int64_t rows, int64_t cols, int64_t slice, float* part) {
+    __shared__ float sh[8][32 * V];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * V;
+    const int64_t r0 = (int64_t)blockIdx.y * slice, r1 = min(rows, r0 + slice);
+    float a[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] = 0.f;
+    if (c < cols)
+        for (int64_t r = r0 + w; r < r1; r += 8) {
+            if constexpr (V == 1) a[0] += Elem<T>::load(in[r * ld + c]);
+            else {
+                uint4 u;
+                if constexpr (V == 8) u = *reinterpret_cast<const uint4*>(in + r * ld + c);
+                else u.x = *reinterpret_cast<const uint32_t*>(in + r * ld + c);
+                const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+                for (int j = 0; j < V; ++j) a[j] += Elem<T>::load(e[j]);
+            }
+        }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sh[w][lane * V + j] = a[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+        const int64_t col = (int64_t)blockIdx.x * 32 * V + i;
+        if (col < cols) {
+            float t = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t += sh[k][i];
+            part[(int64_t)blockIdx.y * cols + col] = t;
+        }
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) colsum_join_kernel(const float* part, int slices, int64_t cols, T* out) {
+    __shared__ float sh[8][33];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    float t = 0.f;
+    if (c < cols)
+        for (int s = w; s < slices; s += 8) t += part[(int64_t)s * cols + c];
+    sh[w][lane] = t;
+    __syncthreads();
+    if (w == 0 && c < cols) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) t += sh[i][lane];
+        out[c] = Elem<T>::store(t);
+    }
+}
+
+// Products of a few rows (MT at most): bound by reading the weights once.
+// One to eight warps share a weight row, each lane has four 16-byte loads in
+// flight, the sums meet by shuffles and shared memory in a fixed order.
+template <typename T, bool GATED, int MT, bool VEC>
+__global__ void __launch_bounds__(256) few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int m, int n, int k,
+                                                       int wpr, const Epilogue e) {
+    __shared__ float sh[8][GATED ? 2 : 1][MT];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part = warp % wpr, col = blockIdx.x * (8 / wpr) + warp / wpr;
+    float a[GATED ? 2 : 1][MT];
+#pragma unroll
+    for (int q = 0; q < (GATED ? 2 : 1); ++q)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) a[q][i] = 0.f;
+    if (col < n) {
+        const T* wr[2] = {w + (int64_t)col * ldw, GATED ? w + (int64_t)(n + col) * ldw : nullptr};
+        if constexpr (VEC) {
+            const int nv = k / 8, step = wpr * 32;
+            for (int v0 = part * 32 + lane; v0 < nv; v0 += 4 * step) {
+                uint4 u[GATED ? 2 : 1][4];
+#pragma unroll
+                for (int q = 0; q < (GATED ? 2 : 1); ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (v0 + j * step < nv) u[q][j] = __ldg(reinterpret_cast<const uint4*>(wr[q]) + v0 + j * step);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int v = v0 + j * step;
+                    if (v >= nv) break;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        if (i >= m) break;
+                        const uint4 xv = *(reinterpret_cast<const uint4*>(x + i * ldx) + v);
+                        const uint32_t* xe = reinterpret_cast<const uint32_t*>(&xv);
+#pragma unroll
+                        for (int q = 0; q < (GATED ? 2 : 1); ++q) {
+                            const uint32_t* we = reinterpret_cast<const uint32_t*>(&u[q][j]);
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                const float2 xf = unpack2<T>(xe[h]), wf = unpack2<T>(we[h]);
+                                a[q][i] = __fmaf_rn(xf.x, wf.x, a[q][i]);
+                                a[q][i] = __fmaf_rn(xf.y, wf.y, a[q][i]);
+                            }
+                        }
+                    }
+                }
+            }
+        } else {
+            for (int v = part * 32 + lane; v < k; v += wpr * 32) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if (i >= m) break;
+                    const float xf = Elem<T>::load(x[i * ldx + v]);
+#pragma unroll
+                    for (int q = 0; q < (GATED ? 2 : 1); ++q) a[q][i] = __fmaf_rn(xf, Elem<T>::load(wr[q][v]), a[q][i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < (GATED ? 2 : 1); ++q)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) a[q][i] += __shfl_xor_sync(0xffffffffu, a[q][i], o);
+            if (lane == 0) sh[warp][q][i] = a[q][i];
+        }
+    __syncthreads();
+    if (part == 0 && col < n && lane < m) {
+        float z[2] = {0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < (GATED ? 2 : 1); ++q) {
+            for (int i = 0; i < wpr; ++i) z[q] += sh[warp + i][q][lane];
+            if (e.bias) z[q] += Elem<T>::load(((const T*)e.bias)[q * n + col]);
+        }
+        float y = 0.f;
+        with_act(e.act, [&](auto act) { y = act_value<decltype(act)::value>(z[0]); });
+        if (GATED) y *= z[1];
+        if (e.res) y += Elem<T>::load(((const T*)e.res)[lane * e.ldr + col]);
+        ((T*)e.out)[lane * e.ldo + col] = Elem<T>::store(y);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static std::once_flag once;
+    static EncodeFn fn = nullptr;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (EncodeFn)p;
+    });
+    return fn;
+}
+
+// A matrix in device memory as TMA sees it: `rows` rows of `inner` contiguous
+// elements, ld elements apart, in `planes` planes `plane` elements apart.
+struct Mat {
+    const void* p = nullptr;
+    int64_t inner = 0, rows = 0, ld = 0, planes = 1, plane = 0;
+};
+
+bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_rows) {
+    const int es = dtype == LF_F8E4M3 ? 1 : 2;
+    const CUtensorMapDataType ty = dtype == LF_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.inner, (cuuint64_t)a.rows, (cuuint64_t)a.planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)(a.ld * es), (cuuint64_t)((a.planes > 1 ? a.plane : a.rows * a.ld) * es)};
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    EncodeFn fn = encode_fn();
+    if (!fn) {
+        set_error("cuTensorMapEncodeTiled is not available");
+        return false;
+    }
+    const CUresult r = fn(map, ty, 3, const_cast<void*>(a.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return r == CUDA_SUCCESS;
+}
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Bump allocator over the caller's workspace; with base 0 it only counts.
+struct Arena {
+    uintptr_t base;
+    size_t used = 0;
+    void* take(size_t bytes) {
+        const size_t at = used;
+        used += up((int64_t)bytes, 256);
+        return base ? reinterpret_cast<void*>(base + at) : nullptr;
+    }
+};
+
+// One product out[m, n] = A B^T (+ epilogue), A and B in either major.
+struct Product {
+    Mat a, b;
+    bool a_mn = false, b_mn = false;
+    int64_t m = 0, n = 0, k = 0;   // rows of one row segment, columns, K of one K segment
+    int msegs = 1, ksegs = 1;
+    Epilogue e{};
+    int dtype = 0, op_dtype = 0;   // output type; operand type
+};
+
+struct Shape {
+    int bn, splits;
+};
+
+// Tile width and splits of K by an estimate in SM cycles: a K step costs bn
+// cycles of the tensor pipe (at least 128: a narrower product is bound by
+// reading A), an output column of a tile about 10 cycles of epilogue, which
+// overlaps the next tile's products; splitting costs writing and reading the
+// partial sums once more and another launch.
+Shape choose(const Product& q) {
+    const int bk = q.op_dtype == LF_F8E4M3 ? 128 : 64;
+    const int64_t iters = (q.k + bk - 1) / bk * q.ksegs, rows = (q.m + kBM - 1) / kBM * q.msegs, sms = num_sms();
+    Shape best{256, 1};
+    double least = 1e30;
+    for (int bn : {256, 128, 64}) {
+        const int64_t tiles = rows * ((q.n + bn - 1) / bn);
+        for (int s = 1; s <= 64; s *= 2) {
+            if (s > 1 && iters / s < 4) break;
+            const int64_t per = (iters + s - 1) / s, units = tiles * ((iters + per - 1) / per);
+            const int64_t waves = (units + sms - 1) / sms;
+            const double main = (double)per * std::max(bn, 128), epi = bn * 10.0;
+            double t = waves * std::max(main, epi) + std::min(main, epi) + 2000;
+            if (s > 1) t += 4000 + (double)s * q.m * q.msegs * q.n * 8 / 3400.0;
+            if (t < least) least = t, best = {bn, s};
+        }
+    }
+    return best;
+}
+
+size_t part_bytes(const Product& q, const Shape& s) {
+    return s.splits > 1 ? (size_t)s.splits * q.m * q.msegs * up(q.n, 4) * 4 : 0;
+}
+
+uint32_t idesc_of(int dtype, bool a_mn, bool b_mn, int n) {
+    const uint32_t f = dtype == LF_BF16 ? 1u : 0u;  // kind::f16: 0 fp16, 1 bf16; kind::f8f6f4: 0 e4m3
+    return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+}
+
+template <auto Kernel>
+int launch_gemm(GemmArgs& g, int stage_bytes, cudaStream_t st) {
+    constexpr int rest = kEpiWarps * kStageOut + kBarrierBytes;
+    g.stages = std::min(kMaxStages, (kSmemLimit - rest) / stage_bytes);
+    const int smem = g.stages * stage_bytes + rest;
+    static std::once_flag once[64];  // per kernel and device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
+    const int64_t units = (int64_t)g.splits * g.msegs * g.tiles_m * g.tiles_n;
+    Kernel<<<(unsigned)std::min<int64_t>(units, num_sms()), kGemmThreads, smem, st>>>(g);
+    return check_launch("tc_gemm_kernel");
+}
+
+int too_large(const char* what) {
+    set_error("%s: more than 2^31 tiles or rows", what);
+    return LF_ERR_UNSUPPORTED;
+}
+
+int join_splits(const Product& q, const float* part, int splits, cudaStream_t st) {
+    const int64_t rows = q.m * q.msegs, ldp = up(q.n, 4), groups = rows * (ldp / 4);
+    const unsigned grid = (unsigned)std::min<int64_t>((groups + 255) / 256, (int64_t)num_sms() * 16);
+    if (q.dtype == LF_F16) split_join_kernel<__half><<<grid, 256, 0, st>>>(part, splits, rows, (int)q.n, ldp, q.e);
+    else split_join_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(part, splits, rows, (int)q.n, ldp, q.e);
+    return check_launch("split_join_kernel");
+}
+
+int run_product(const Product& q, Arena& ws, cudaStream_t st) {
+    if (q.m == 0 || q.n == 0) return LF_OK;
+    if (q.k == 0) return ws.base ? join_splits(q, nullptr, 0, st) : LF_OK;  // an empty sum: the epilogue of zero
+    const Shape s = choose(q);
+    float* part = s.splits > 1 ? (float*)ws.take(part_bytes(q, s)) : nullptr;
+    if (!ws.base) return LF_OK;
+    const int bk = q.op_dtype == LF_F8E4M3 ? 128 : 64;
+    GemmArgs g{};
+    g.m = (int)q.m, g.n = (int)q.n;
+    g.msegs = q.msegs;
+    g.tiles_m = (int)((q.m + kBM - 1) / kBM);
+    g.tiles_n = (int)((q.n + s.bn - 1) / s.bn);
+    g.seg_iters = (int)((q.k + bk - 1) / bk);
+    g.iters = g.seg_iters * q.ksegs;
+    g.split_iters = (g.iters + s.splits - 1) / s.splits;
+    g.splits = (g.iters + g.split_iters - 1) / g.split_iters;
+    if (q.m > INT32_MAX - 256 || q.n > INT32_MAX - 256 || (int64_t)g.splits * g.msegs * g.tiles_m * g.tiles_n > INT32_MAX / 2)
+        return too_large("matrix product");
+    g.bn = s.bn;
+    g.nbuf = 2;
+    g.a_mn = q.a_mn, g.b_mn = q.b_mn;
+    g.idesc = idesc_of(q.op_dtype, q.a_mn, q.b_mn, s.bn);
+    g.e = q.e;
+    g.part = part;
+    g.ldp = up(q.n, 4);
+    if (!encode(&g.a, q.a, q.op_dtype, q.a_mn ? 64 : bk, q.a_mn ? bk : kBM)) return LF_ERR_CUDA;
+    if (!encode(&g.b, q.b, q.op_dtype, q.b_mn ? 64 : bk, q.b_mn ? bk : s.bn)) return LF_ERR_CUDA;
+    const int stage = (kBM + s.bn) * kRowBytes;
+    int rc;
+    if (q.op_dtype == LF_F8E4M3)
+        rc = q.dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kLinear, true>>(g, stage, st)
+                               : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kLinear, true>>(g, stage, st);
+    else
+        rc = q.dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kLinear, false>>(g, stage, st)
+                               : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kLinear, false>>(g, stage, st);
+    return rc || !part ? rc : join_splits(q, part, g.splits, st);
+}
+
+// A dense operand as TMA can read it: itself, or a copy with padded rows.
+bool tma_ok(const void* p, int64_t ld, int es) { return aligned(p, 16) && ld * es % 16 == 0; }
+
+Mat operand(const void* p, int64_t rows, int64_t cols, int64_t ld, int es, Arena& ws, cudaStream_t st) {
+    if (rows == 0 || cols == 0 || tma_ok(p, ld, es)) return {p, cols, rows, ld, 1, 0};
+    const int64_t ldo = up(cols, 16 / es);
+    void* out = ws.take((size_t)rows * ldo * es);
+    if (out) {
+        const unsigned grid = (unsigned)std::min<int64_t>((rows * cols + 255) / 256, (int64_t)num_sms() * 32);
+        if (es == 1) pack_rows_kernel<uint8_t><<<grid, 256, 0, st>>>((const uint8_t*)p, ld, (uint8_t*)out, ldo, rows, cols);
+        else pack_rows_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)p, ld, (uint16_t*)out, ldo, rows, cols);
+    }
+    return {out, cols, rows, ldo, 1, 0};
+}
+
+void set_out(Epilogue& e, void* out, int64_t ldo) {
+    e.out = out;
+    e.ldo = ldo;
+    e.vec_out = aligned(out, 8) && ldo % 4 == 0;
+}
+void set_res(Epilogue& e, const void* res, int64_t ldr) {
+    e.res = res;
+    e.ldr = ldr;
+    e.vec_res = aligned(res, 8) && ldr % 4 == 0;
+}
+
+int zero(void* p, int64_t rows, int64_t row_bytes, cudaStream_t st) {
+    if (p && rows * row_bytes && cudaMemsetAsync(p, 0, (size_t)(rows * row_bytes), st) != cudaSuccess) return check_launch("zero fill");
+    return LF_OK;
+}
+
+template <typename T>
+void launch_colsum(const T* in, int64_t ld, int64_t rows, int64_t cols, T* out, float* part, int64_t slice, int slices, cudaStream_t st) {
+    const bool v8 = cols >= 256 && cols % 8 == 0 && ld % 8 == 0 && aligned(in, 16);
+    const bool v2 = cols % 2 == 0 && ld % 2 == 0 && aligned(in, 4);
+    const int v = v8 ? 8 : v2 ? 2 : 1;
+    const dim3 grid((unsigned)((cols + 32 * v - 1) / (32 * v)), (unsigned)slices);
+    if (v8) colsum_kernel<T, 8><<<grid, 256, 0, st>>>(in, ld, rows, cols, slice, part);
+    else if (v2) colsum_kernel<T, 2><<<grid, 256, 0, st>>>(in, ld, rows, cols, slice, part);
+    else colsum_kernel<T, 1><<<grid, 256, 0, st>>>(in, ld, rows, cols, slice, part);
+    colsum_join_kernel<T><<<(unsigned)((cols + 31) / 32), 256, 0, st>>>(part, slices, cols, out);
+}
+
+// out[c] = sum of column c of in [rows, cols] (16-bit).
+int run_colsum(const void* in, int64_t ld, int64_t rows, int64_t cols, void* out, int dtype, Arena& ws, cudaStream_t st) {
+    if (rows == 0 || cols == 0) return ws.base ? zero(out, 1, cols * 2, st) : LF_OK;
+    const int64_t want = std::max<int64_t>(1, 4 * num_sms() * 64 / std::max<int64_t>(cols, 64));
+    const int64_t slice = std::max<int64_t>(64, (rows + want - 1) / want);
+    const int slices = (int)((rows + slice - 1) / slice);
+    float* part = (float*)ws.take((size_t)slices * cols * 4);
+    if (!ws.base) return LF_OK;
+    if (dtype == LF_F16) launch_colsum((const __half*)in, ld, rows, cols, (__half*)out, part, slice, slices, st);
+    else launch_colsum((const __nv_bfloat16*)in, ld, rows, cols, (__nv_bfloat16*)out, part, slice, slices, st);
+    return check_launch("colsum_kernel");
+}
+
+constexpr int kFewRows = 8;
+
+template <typename T, bool GATED>
+void launch_few(const void* x, int64_t ldx, const void* w, int64_t ldw, int m, int n, int k, const Epilogue& e, cudaStream_t st) {
+    const bool vec = k % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && aligned(x, 16) && aligned(w, 16);
+    int wpr = 1;  // warps per weight row: more where there are too few rows to fill the SMs
+    while (wpr < 8 && (int64_t)n * wpr < 32 * (int64_t)num_sms() && k / (256 * wpr) > 1) wpr *= 2;
+    const unsigned grid = (unsigned)((n + 8 / wpr - 1) / (8 / wpr));
+    const T *xp = (const T*)x, *wp = (const T*)w;
+#define LFB_FEW(MT)                                                                                          \
+    if (vec) few_rows_kernel<T, GATED, MT, true><<<grid, 256, 0, st>>>(xp, ldx, wp, ldw, m, n, k, wpr, e);   \
+    else few_rows_kernel<T, GATED, MT, false><<<grid, 256, 0, st>>>(xp, ldx, wp, ldw, m, n, k, wpr, e)
+    if (m == 1) { LFB_FEW(1); }
+    else if (m == 2) { LFB_FEW(2); }
+    else if (m <= 4) { LFB_FEW(4); }
+    else { LFB_FEW(8); }
+#undef LFB_FEW
+}
+template <bool GATED>
+int run_few(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k, const Epilogue& e,
+            int dtype, cudaStream_t st) {
+    if (dtype == LF_F16) launch_few<__half, GATED>(x, ldx, w, ldw, (int)m, (int)n, (int)k, e, st);
+    else launch_few<__nv_bfloat16, GATED>(x, ldx, w, ldw, (int)m, (int)n, (int)k, e, st);
+    return check_launch("few_rows_kernel");
+}
+
+int check_common(const char* what, int act, int dtype, std::initializer_list<int64_t> sizes) {
+    if (dtype != LF_F16 && dtype != LF_BF16) {
+        set_error("%s: unsupported dtype code %d (fp16 and bf16)", what, dtype);
+        return LF_ERR_DTYPE;
+    }
+    if (act < LF_ACT_NONE || act > LF_ACT_SILU) {
+        set_error("%s: unknown activation %d", what, act);
+        return LF_ERR_INVALID;
+    }
+    for (int64_t v : sizes)
+        if (v < 0) {
+            set_error("%s: negative size", what);
+            return LF_ERR_INVALID;
+        }
+    for (int64_t v : sizes)
+        if (v > INT32_MAX - 256) {
+            set_error("%s: a size passes 2^31", what);
+            return LF_ERR_UNSUPPORTED;
+        }
+    return LF_OK;
+}
+
+int missing(const char* what, const char* names) {
+    set_error("%s: %s required", what, names);
+    return LF_ERR_INVALID;
+}
+
+Product weight_product(const Mat& x, const Mat& w, int64_t m, int64_t n, int64_t k, int dtype, int op_dtype) {
+    Product q;
+    q.a = x, q.b = w;
+    q.m = m, q.n = n, q.k = k;
+    q.dtype = dtype, q.op_dtype = op_dtype;
+    return q;
+}
+
+// ---- linear ----------------------------------------------------------------
+int check_linear(const char* what, const lf_linear_t* a, bool quant) {
+    if (!a) return missing(what, "arguments are");
+    if (int rc = check_common(what, a->activation, a->dtype, {a->m, a->n, a->k})) return rc;
+    if (a->m == 0 || a->n == 0) return LF_OK;
+    if (!a->w || !a->x) return a->k == 0 ? LF_OK : missing(what, "x and w are");
+    if (a->ldx < a->k || a->ldw < a->k || (a->residual && a->ldr < a->n)) {
+        set_error("%s: a row stride is shorter than its row", what);
+        return LF_ERR_INVALID;
+    }
+    if (quant && (!a->x_scale || !a->w_scale)) return missing(what, "x_scale and w_scale are");
+    return LF_OK;
+}
+
+int linear_fwd(const lf_linear_t* a, bool quant, Arena& ws, cudaStream_t st) {
+    if (a->m == 0 || a->n == 0) return LF_OK;
+    Epilogue e{};
+    set_out(e, a->y, a->n);
+    e.bias = a->bias;
+    if (a->residual) set_res(e, a->residual, a->ldr);
+    e.act = a->activation;
+    if (quant) e.sa = (const float*)a->x_scale, e.sb = (const float*)a->w_scale;
+    if (!quant && a->k > 0 && a->m <= kFewRows) return ws.base ? run_few<false>(a->x, a->ldx, a->w, a->ldw, a->m, a->n, a->k, e, a->dtype, st) : LF_OK;
+    const int es = quant ? 1 : 2;
+    Mat x = operand(a->x, a->m, a->k, a->ldx, es, ws, st), w = operand(a->w, a->n, a->k, a->ldw, es, ws, st);
+    Product q = weight_product(x, w, a->m, a->n, a->k, a->dtype, quant ? LF_F8E4M3 : a->dtype);
+    q.e = e;
+    return run_product(q, ws, st);
+}
+
+int linear_bwd(const lf_linear_t* a, Arena& ws, cudaStream_t st) {
+    const int64_t m = a->m, n = a->n, k = a->k;
+    const bool need_z = a->activation != LF_ACT_NONE;
+    Mat x, w, dz;
+    if (need_z || a->dw) x = operand(a->x, m, k, a->ldx, 2, ws, st);
+    if (need_z || a->dx) w = operand(a->w, n, k, a->ldw, 2, ws, st);
+    if (need_z) {
+        const int64_t ld = up(n, 8);
+        dz = {ws.take((size_t)m * ld * 2), n, m, ld, 1, 0};
+        Product q = weight_product(x, w, m, n, k, a->dtype, a->dtype);
+        set_out(q.e, const_cast<void*>(dz.p), ld);
+        set_res(q.e, a->dy, a->lddy);
+        q.e.bias = a->bias;
+        q.e.act = a->activation;
+        q.e.act_bwd = true;
+        if (int rc = run_product(q, ws, st)) return rc;
+    } else {
+        dz = operand(a->dy, m, n, a->lddy, 2, ws, st);
+    }
+    if (a->dx) {  // dx = dz W: W is read with its k contiguous
+        Product q = weight_product(dz, w, m, k, n, a->dtype, a->dtype);
+        q.b_mn = true;
+        set_out(q.e, a->dx, k);
+        if (int rc = run_product(q, ws, st)) return rc;
+    }
+    if (a->dw) {  // dW = dz^T x: both operands transposed
+        Product q = weight_product(dz, x, n, k, m, a->dtype, a->dtype);
+        q.a_mn = q.b_mn = true;
+        set_out(q.e, a->dw, k);
+        if (int rc = run_product(q, ws, st)) return rc;
+    }
+    if (a->db) return run_colsum(dz.p, dz.ld, m, n, a->db, a->dtype, ws, st);
+    return LF_OK;
+}
+
+// ---- gated feed-forward block ----------------------------------------------
+int check_ffn(const char* what, const lf_gated_ffn_t* a) {
+    if (!a) return missing(what, "arguments are");
+    if (int rc = check_common(what, a->activation, a->dtype, {a->m, a->c, a->f})) return rc;
+    if (2 * a->f > INT32_MAX - 256) return too_large(what);
+    if (a->m == 0 || a->c == 0) return LF_OK;
+    if (!a->x || (a->f > 0 && (!a->w_in || !a->w_out))) return missing(what, "x, w_in and w_out are");
+    if (a->ldx < a->c || (a->residual && a->ldr < a->c)) {
+        set_error("%s: a row stride is shorter than its row", what);
+        return LF_ERR_INVALID;
+    }
+    return LF_OK;
+}
+
+// Win [2F, C] as two planes of F rows, so that a tile that passes F reads zeros.
+Mat gate_up(Mat w, int64_t f) { return {w.p, w.inner, f, w.ld, 2, f * w.ld}; }
+
+// Hidden columns per tile of the gated kernels by the same estimate as choose().
+int choose_gated(int64_t m, int64_t f, int64_t c, bool bwd) {
+    const int64_t rows = (m + kBM - 1) / kBM, iters = (c + 63) / 64, sms = num_sms();
+    int best = 64;
+    double least = 1e30;
+    for (int bh : {128, 64, 32}) {
+        if (bwd && bh != 64) continue;
+        const int64_t waves = (rows * ((f + bh - 1) / bh) + sms - 1) / sms;
+        const double main = (double)iters * std::max(bwd ? 3 * bh : 2 * bh, 128), epi = bh * (bwd ? 40.0 : 20.0);
+        const double t = waves * std::max(main, epi) + std::min(main, epi);
+        if (t < least) least = t, best = bh;
+    }
+    return best;
+}
+
+int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* dy, const Mat* wout, void* out, int64_t ldo,
+              int64_t plane, cudaStream_t st) {
+    const bool bwd = dy != nullptr;
+    const int bh = choose_gated(a->m, a->f, a->c, bwd);
+    GemmArgs g{};
+    g.m = (int)a->m, g.n = (int)a->f;
+    g.msegs = g.splits = 1;
+    g.tiles_m = (int)((a->m + kBM - 1) / kBM);
+    g.tiles_n = (int)((a->f + bh - 1) / bh);
+    if ((int64_t)g.tiles_m * g.tiles_n > INT32_MAX / 2) return too_large("gated feed-forward block");
+    g.iters = g.split_iters = g.seg_iters = (int)((a->c + 63) / 64);
+    g.bn = 2 * bh;
+    g.nbuf = 2;
+    g.idesc = idesc_of(a->dtype, false, false, 2 * bh);
+    g.idesc2 = idesc_of(a->dtype, false, true, bh);
+    g.e.out = out, g.e.ldo = ldo, g.e.bias = a->b_in, g.e.act = a->activation;
+    g.plane = plane;
+    if (!encode(&g.a, x, a->dtype, 64, kBM) || !encode(&g.b, gate_up(win, a->f), a->dtype, 64, bh)) return LF_ERR_CUDA;
+    if (bwd && (!encode(&g.a2, *dy, a->dtype, 64, kBM) || !encode(&g.b2, *wout, a->dtype, 64, 64))) return LF_ERR_CUDA;
+    const int stage = (bwd ? 2 * kBM + 3 * bh : kBM + 2 * bh) * kRowBytes;
+    if (bwd)
+        return a->dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kGatedBwd, false>>(g, stage, st)
+                                  : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kGatedBwd, false>>(g, stage, st);
+    return a->dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kGated, false>>(g, stage, st)
+                              : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kGated, false>>(g, stage, st);
+}
+
+int ffn_fwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
+    const int64_t m = a->m, c = a->c, f = a->f;
+    if (m == 0 || c == 0) return LF_OK;
+    const int64_t ldh = up(f, 8);
+    Mat h{ws.take((size_t)m * ldh * 2), f, m, ldh, 1, 0};
+    Epilogue e{};
+    set_out(e, a->y, c);
+    e.bias = a->b_out;
+    if (a->residual) set_res(e, a->residual, a->ldr);
+    if (m <= kFewRows && f > 0) {
+        if (!ws.base) return LF_OK;
+        Epilogue eh{};
+        set_out(eh, const_cast<void*>(h.p), ldh);
+        eh.bias = a->b_in, eh.act = a->activation;
+        if (int rc = run_few<true>(a->x, a->ldx, a->w_in, c, m, f, c, eh, a->dtype, st)) return rc;
+        return run_few<false>(h.p, ldh, a->w_out, f, m, c, f, e, a->dtype, st);
+    }
+    Mat x = operand(a->x, m, c, a->ldx, 2, ws, st), win = operand(a->w_in, 2 * f, c, c, 2, ws, st);
+    Mat wout = operand(a->w_out, c, f, f, 2, ws, st);
+    if (ws.base && f > 0)
+        if (int rc = run_gated(a, x, win, nullptr, nullptr, const_cast<void*>(h.p), ldh, 0, st)) return rc;
+    Product q = weight_product(h, wout, m, c, f, a->dtype, a->dtype);
+    q.e = e;
+    return run_product(q, ws, st);
+}
+
+int ffn_bwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
+    const int64_t m = a->m, c = a->c, f = a->f;
+    if (m == 0 || c == 0) return LF_OK;
+    const int64_t ld = up(f, 8), plane = m * ld;
+    uint16_t* dz = (uint16_t*)ws.take((size_t)3 * plane * 2);  // dg, du, h
+    Mat x = operand(a->x, m, c, a->ldx, 2, ws, st), win = operand(a->w_in, 2 * f, c, c, 2, ws, st);
+    Mat wout = operand(a->w_out, c, f, f, 2, ws, st), dy = operand(a->dy, m, c, a->lddy, 2, ws, st);
+    if (ws.base && f > 0)
+        if (int rc = run_gated(a, x, win, &dy, &wout, dz, ld, plane, st)) return rc;
+    const Mat both{dz, f, m, ld, 2, plane}, h{dz + 2 * plane, f, m, ld, 1, 0};
+    if (a->dx) {  // dx = [dg|du] Win: two K segments of F
+        Product q = weight_product(both, gate_up(win, f), m, c, f, a->dtype, a->dtype);
+        q.b_mn = true;
+        q.ksegs = 2;
+        set_out(q.e, a->dx, c);
+        if (int rc = run_product(q, ws, st)) return rc;
+    }
+    if (a->dw_in) {  // two row segments of F
+        Product q = weight_product(both, x, f, c, m, a->dtype, a->dtype);
+        q.a_mn = q.b_mn = true;
+        q.msegs = 2;
+        set_out(q.e, a->dw_in, c);
+        if (int rc = run_product(q, ws, st)) return rc;
+    }
+    if (a->dw_out) {
+        Product q = weight_product(dy, h, c, f, m, a->dtype, a->dtype);
+        q.a_mn = q.b_mn = true;
+        set_out(q.e, a->dw_out, f);
+        if (int rc = run_product(q, ws, st)) return rc;
+    }
+    if (a->db_in)
+        for (int s = 0; s < 2; ++s)
+            if (int rc = run_colsum(dz + s * plane, ld, m, f, (uint16_t*)a->db_in + s * f, a->dtype, ws, st)) return rc;
+    if (a->db_out) return run_colsum(a->dy, a->lddy, m, c, a->db_out, a->dtype, ws, st);
+    return LF_OK;
+}
+
+int check_ws(const char* what, const void* ws, size_t have, size_t need) {
+    if (need && (!ws || !aligned(ws, 256) || have < need)) {
+        set_error("%s: needs %zu bytes of 256-byte aligned workspace, got %zu", what, need, ws ? have : (size_t)0);
+        return LF_ERR_INVALID;
+    }
+    return LF_OK;
+}
+
+// With a counting arena the operators only add up what they would take.
+template <class F>
+size_t count_of(F&& f) {
+    Arena ws{0};
+    return f(ws) == LF_OK ? ws.used : 0;
+}
+constexpr uintptr_t kNoWorkspace = 256;  // stands for a workspace of no bytes
+
+template <class F>
+int run_with(const char* what, void* ws, size_t bytes, size_t need, F&& f) {
+    if (int rc = check_ws(what, ws, bytes, need)) return rc;
+    Arena arena{need ? reinterpret_cast<uintptr_t>(ws) : kNoWorkspace};
+    return f(arena);
+}
+
+}  // namespace
+}  // namespace lfb
+
+using namespace lfb;
+
+extern "C" size_t lf_linear_fwd_workspace_size(const lf_linear_t* a) {
+    if (check_linear("lf_linear_fwd", a, false)) return 0;
+    return count_of([&](Arena& w) { return linear_fwd(a, false, w, nullptr); });
+}
+
+extern "C" int lf_linear_fwd(const lf_linear_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
+    clear_error();
+    if (int rc = check_linear("lf_linear_fwd", a, false)) return rc;
+    if (a->m && a->n && !a->y) return missing("lf_linear_fwd", "y is");
+    return run_with("lf_linear_fwd", workspace, workspace_bytes, lf_linear_fwd_workspace_size(a),
+                    [&](Arena& w) { return linear_fwd(a, false, w, (cudaStream_t)stream); });
+}
+
+extern "C" size_t lf_linear_quant_fwd_workspace_size(const lf_linear_t* a) {
+    if (check_linear("lf_linear_quant_fwd", a, true)) return 0;
+    return count_of([&](Arena& w) { return linear_fwd(a, true, w, nullptr); });
+}
+
+extern "C" int lf_linear_quant_fwd(const lf_linear_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
+    clear_error();
+    if (int rc = check_linear("lf_linear_quant_fwd", a, true)) return rc;
+    if (a->m && a->n && !a->y) return missing("lf_linear_quant_fwd", "y is");
+    return run_with("lf_linear_quant_fwd", workspace, workspace_bytes, lf_linear_quant_fwd_workspace_size(a),
+                    [&](Arena& w) { return linear_fwd(a, true, w, (cudaStream_t)stream); });
+}
+
+extern "C" size_t lf_linear_bwd_workspace_size(const lf_linear_t* a) {
+    if (check_linear("lf_linear_bwd", a, false)) return 0;
+    return count_of([&](Arena& w) { return linear_bwd(a, w, nullptr); });
+}
+
+extern "C" int lf_linear_bwd(const lf_linear_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
+    clear_error();
+    if (int rc = check_linear("lf_linear_bwd", a, false)) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a->m && a->n && !a->dy) return missing("lf_linear_bwd", "dy is");
+    if (a->lddy < a->n) {
+        set_error("lf_linear_bwd: lddy is shorter than a row");
+        return LF_ERR_INVALID;
+    }
+    return run_with("lf_linear_bwd", workspace, workspace_bytes, lf_linear_bwd_workspace_size(a),
+                    [&](Arena& w) { return linear_bwd(a, w, st); });
+}
+
+extern "C" size_t lf_gated_ffn_fwd_workspace_size(const lf_gated_ffn_t* a) {
+    if (check_ffn("lf_gated_ffn_fwd", a)) return 0;
+    return count_of([&](Arena& w) { return ffn_fwd(a, w, nullptr); });
+}
+
+extern "C" int lf_gated_ffn_fwd(const lf_gated_ffn_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
+    clear_error();
+    if (int rc = check_ffn("lf_gated_ffn_fwd", a)) return rc;
+    if (a->m && a->c && !a->y) return missing("lf_gated_ffn_fwd", "y is");
+    return run_with("lf_gated_ffn_fwd", workspace, workspace_bytes, lf_gated_ffn_fwd_workspace_size(a),
+                    [&](Arena& w) { return ffn_fwd(a, w, (cudaStream_t)stream); });
+}
+
+extern "C" size_t lf_gated_ffn_bwd_workspace_size(const lf_gated_ffn_t* a) {
+    if (check_ffn("lf_gated_ffn_bwd", a)) return 0;
+    return count_of([&](Arena& w) { return ffn_bwd(a, w, nullptr); });
+}
+
+extern "C" int lf_gated_ffn_bwd(const lf_gated_ffn_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
+    clear_error();
+    if (int rc = check_ffn("lf_gated_ffn_bwd", a)) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a->m == 0 || a->c == 0) {  // no token or no channel: every gradient is empty or zero
+        if (int rc = zero(a->dw_in, 2 * a->f, a->c * 2, st)) return rc;
+        if (int rc = zero(a->dw_out, a->c, a->f * 2, st)) return rc;
+        if (int rc = zero(a->db_in, 2 * a->f, 2, st)) return rc;
+        return zero(a->db_out, 1, a->c * 2, st);
+    }
+    if (!a->dy) return missing("lf_gated_ffn_bwd", "dy is");
+    if (a->lddy < a->c) {
+        set_error("lf_gated_ffn_bwd: lddy is shorter than a row");
+        return LF_ERR_INVALID;
+    }
+    return run_with("lf_gated_ffn_bwd", workspace, workspace_bytes, lf_gated_ffn_bwd_workspace_size(a),
+                    [&](Arena& w) { return ffn_bwd(a, w, st); });
+}

@@ -4,6 +4,7 @@
 
 #include <string>
 
+#include "BlockOperators.h"
 #include "LaplaceSubtraction.h"
 #include "NewtonInverse.h"
 #include "laplacian_b200.h"
@@ -78,4 +79,60 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("iter"), py::arg("init_mode") = 0, py::arg("reg") = 0.01, py::arg("precision") = 0);
     m.def("NewtonInverse_residual", &NewtonInverse_residual,
           "NewtonInverse_residual (mat, inverse, residual, reg): ||(A + reg I) X - I||_F per matrix");
+
+    // Block operators (no counterpart in the reference module).
+    using T = c10::optional<at::Tensor>;
+    auto t = [](const T& v) { return v.has_value() ? *v : at::Tensor(); };
+    auto o = [](const at::Tensor& v) { return v.defined() ? T(v) : T(); };
+    m.def("RmsNorm_forward",
+          [=](const at::Tensor& x, const at::Tensor& w, const T& r, double eps, bool keep) {
+              auto [y, s, rstd] = RmsNorm_forward(x, w, t(r), eps, keep);
+              return std::make_tuple(y, o(s), o(rstd));
+          },
+          "RmsNorm_forward (x, weight, residual, eps, keep) -> (y, s, rstd)");
+    m.def("RmsNorm_backward",
+          [=](const at::Tensor& dy, const T& ds, const at::Tensor& s, const at::Tensor& rstd, const at::Tensor& w,
+              bool need_x, bool need_w) {
+              auto [dx, dw] = RmsNorm_backward(dy, t(ds), s, rstd, w, need_x, need_w);
+              return std::make_tuple(o(dx), o(dw));
+          },
+          "RmsNorm_backward (dy, ds, s, rstd, weight, need_x, need_w) -> (dx, dw)");
+    m.def("RmsNorm_quant_forward",
+          [=](const at::Tensor& x, const at::Tensor& w, const T& r, double eps) {
+              auto [q, scale, s] = RmsNorm_quant_forward(x, w, t(r), eps);
+              return std::make_tuple(q, scale, o(s));
+          },
+          "RmsNorm_quant_forward (x, weight, residual, eps) -> (q, scale, s)");
+    m.def("Quantize_rows", &Quantize_rows, "Quantize_rows (x) -> (q, scale)");
+    m.def("Linear_forward",
+          [=](const at::Tensor& x, const at::Tensor& w, const T& b, const T& r, int64_t act) {
+              return Linear_forward(x, w, t(b), t(r), act);
+          },
+          "Linear_forward (x, weight, bias, residual, activation) -> y");
+    m.def("Linear_quant_forward",
+          [=](const at::Tensor& q, const at::Tensor& scale, const at::Tensor& w, const at::Tensor& wscale, const T& b,
+              const T& r, int64_t act, bool bf16) {
+              return Linear_quant_forward(q, scale, w, wscale, t(b), t(r), act, bf16 ? at::kBFloat16 : at::kHalf);
+          },
+          "Linear_quant_forward (q, scale, weight, weight_scale, bias, residual, activation, bf16) -> y");
+    m.def("Linear_backward",
+          [=](const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const T& b, int64_t act, bool need_x,
+              bool need_w, bool need_b) {
+              auto [dx, dw, db] = Linear_backward(dy, x, w, t(b), act, need_x, need_w, need_b);
+              return std::make_tuple(o(dx), o(dw), o(db));
+          },
+          "Linear_backward (dy, x, weight, bias, activation, need_x, need_w, need_b) -> (dx, dw, db)");
+    m.def("GatedFeedForward_forward",
+          [=](const at::Tensor& x, const at::Tensor& wi, const at::Tensor& wo, const T& bi, const T& bo, const T& r,
+              int64_t act) { return GatedFeedForward_forward(x, wi, wo, t(bi), t(bo), t(r), act); },
+          "GatedFeedForward_forward (x, w_in, w_out, b_in, b_out, residual, activation) -> y");
+    m.def("GatedFeedForward_backward",
+          [=](const at::Tensor& dy, const at::Tensor& x, const at::Tensor& wi, const at::Tensor& wo, const T& bi,
+              int64_t act, bool nx, bool nwi, bool nwo, bool nbi, bool nbo) {
+              auto [dx, dwi, dwo, dbi, dbo] = GatedFeedForward_backward(dy, x, wi, wo, t(bi), act, nx, nwi, nwo, nbi, nbo);
+              return std::make_tuple(o(dx), o(dwi), o(dwo), o(dbi), o(dbo));
+          },
+          "GatedFeedForward_backward (dy, x, w_in, w_out, b_in, activation, need_x, need_w_in, need_w_out, need_b_in, "
+          "need_b_out) -> (dx, dw_in, dw_out, db_in, db_out)");
+    m.def("ClipGradNorm", &ClipGradNorm, "ClipGradNorm (grads, outs, max_norm) -> norm");
 }

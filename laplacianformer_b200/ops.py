@@ -10,6 +10,11 @@ These wrappers give that composition:
 * :func:`newton_inverse` — Newton–Schulz inverse; backward is the reference's
   analytic ``-V^T G V^T`` (src/NewtonInverse_cuda_kernel.cu:466-573).
 
+The rest of a transformer block (the reference has none of it): :func:`rms_norm`,
+:func:`linear` and :func:`gated_feed_forward` with their backward passes,
+:func:`rms_norm_quant`, :func:`quantize_rows` and :func:`linear_quant` for
+serving with 8-bit operands, and :func:`clip_grad_norm`.
+
 Every call goes to the ``Laplace_subtraction_cuda`` extension; there is no CPU
 fallback and a missing extension raises ImportError.
 """
@@ -167,3 +172,142 @@ def newton_residual(mat: torch.Tensor, inv: torch.Tensor, reg: float = 0.0) -> t
                       dtype=torch.float64 if mat.dtype == torch.float64 else torch.float32)
     ext().NewtonInverse_residual(mat.contiguous(), inv.contiguous(), res, float(reg))
     return res
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _act(name: str) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
+
+
+def _tracked(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class RmsNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, s, rstd = ext().RmsNorm_forward(x, weight, residual, eps, True)
+        ctx.save_for_backward(x if s is None else s, rstd, weight)
+        ctx.set_materialize_grads(False)
+        return y, s
+
+    @staticmethod
+    def backward(ctx, dy, ds):
+        s, rstd, weight = ctx.saved_tensors
+        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
+        if dy is None:  # only the sum was used: its gradient passes through
+            return ds, None, ds if ctx.needs_input_grad[2] else None, None
+        dx, dw = ext().RmsNorm_backward(dy, ds, s, rstd, weight, need_x, ctx.needs_input_grad[1])
+        return dx, dw, dx if ctx.needs_input_grad[2] else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
+    """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension, s = x + residual.
+
+    Returns y, or (y, s) when a residual is given (s continues the residual
+    stream).  fp32, fp16 and bf16; statistics in fp32."""
+    if _tracked(x, weight, residual):
+        y, s = RmsNormFn.apply(x, weight, residual, float(eps))
+    else:
+        y, s, _ = ext().RmsNorm_forward(x, weight, residual, float(eps), False)
+    return y if residual is None else (y, s)
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
+    """:func:`rms_norm` with its output in 8 bits, for :func:`linear_quant`: (q, scale), or (q, scale, s) with a
+    residual; y is about q * scale, q float8_e4m3fn, one fp32 scale per row (max|y| / 448).  No gradient."""
+    q, scale, s = ext().RmsNorm_quant_forward(x, weight, residual, float(eps))
+    return (q, scale) if residual is None else (q, scale, s)
+
+
+def quantize_rows(x: torch.Tensor):
+    """(q, scale) with x about q * scale, q float8_e4m3fn and one fp32 scale per row (weights for :func:`linear_quant`)."""
+    return ext().Quantize_rows(x)
+
+
+class LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        ctx.save_for_backward(x, weight, bias)
+        ctx.act = act
+        return ext().Linear_forward(x, weight, bias, residual, act)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, bias = ctx.saved_tensors
+        nx, nw, nb, nr = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if nx or nw or nb:
+            dx, dw, db = ext().Linear_backward(dy, x, weight, bias, ctx.act, nx, nw, nb)
+        return dx, dw, db, dy if nr else None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """activation(x @ weight.T + bias) + residual in one kernel, for fp16 and bf16.
+
+    x [..., K] (rows may be strided), weight [N, K] as torch.nn.Linear keeps it,
+    bias [N], residual [..., N].  activation: none, relu, gelu, gelu_tanh or
+    silu; the backward recomputes the pre-activation instead of keeping it."""
+    act = _act(activation)
+    if _tracked(x, weight, bias, residual):
+        return LinearFn.apply(x, weight, bias, residual, act)
+    return ext().Linear_forward(x, weight, bias, residual, act)
+
+
+def linear_quant(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                 bias: torch.Tensor | None = None, activation: str = "none", residual: torch.Tensor | None = None,
+                 dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """:func:`linear` on 8-bit operands: q [..., K] and weight [N, K] float8_e4m3fn with one fp32 scale per row
+    (:func:`rms_norm_quant`, :func:`quantize_rows`); bias, residual and output fp16 or bf16.  No gradient."""
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {dtype}: float16 or bfloat16")
+    return ext().Linear_quant_forward(q, scale, weight, weight_scale, bias, residual, _act(activation),
+                                      dtype == torch.bfloat16)
+
+
+class GatedFeedForwardFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_in, w_out, b_in, b_out, residual, act):
+        ctx.save_for_backward(x, w_in, w_out, b_in)
+        ctx.act = act
+        return ext().GatedFeedForward_forward(x, w_in, w_out, b_in, b_out, residual, act)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w_in, w_out, b_in = ctx.saved_tensors
+        needs, nr = ctx.needs_input_grad[:5], ctx.needs_input_grad[5]
+        grads = (None,) * 5
+        if any(needs):
+            grads = ext().GatedFeedForward_backward(dy, x, w_in, w_out, b_in, ctx.act, *needs)
+        return *grads, dy if nr else None, None
+
+
+def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: torch.Tensor | None = None,
+                       b_out: torch.Tensor | None = None, activation: str = "silu",
+                       residual: torch.Tensor | None = None) -> torch.Tensor:
+    """(activation(g) * u) @ w_out.T + b_out + residual with [g | u] = x @ w_in.T + b_in, for fp16 and bf16.
+
+    x [..., C], w_in [2F, C] (gate rows, then up rows), w_out [C, F].  Both
+    projections, the activation and the product run in one kernel; between the
+    passes only x is kept, the backward recomputes the projections."""
+    act = _act(activation)
+    if _tracked(x, w_in, w_out, b_in, b_out, residual):
+        return GatedFeedForwardFn.apply(x, w_in, w_out, b_in, b_out, residual, act)
+    return ext().GatedFeedForward_forward(x, w_in, w_out, b_in, b_out, residual, act)
+
+
+def clip_grad_norm(grads, max_norm: float, out=None):
+    """Global 2-norm of all tensors in `grads` and their copies scaled by min(1, max_norm / (norm + 1e-6)).
+
+    Returns (norm, out): norm a float32 device scalar (nothing is read back to
+    the host), out the clipped tensors.  `out` may be given, `grads` itself
+    included (in place).  fp32, fp16 and bf16 tensors may be mixed."""
+    grads = list(grads)
+    out = [torch.empty_like(g) for g in grads] if out is None else list(out)
+    return ext().ClipGradNorm(grads, out, float(max_norm)), out

@@ -27,6 +27,7 @@ setup(
             sources=[
                 os.path.join("laplacianformer_b200", "csrc", "wrapper.cpp"),
                 os.path.join("laplacianformer_b200", "csrc", "torch_ops.cpp"),
+                os.path.join("laplacianformer_b200", "csrc", "torch_block_ops.cpp"),
             ],
             include_dirs=[os.path.join(HERE, "include")],
             define_macros=[("WITH_CUDA", None)],
