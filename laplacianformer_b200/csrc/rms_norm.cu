@@ -12,6 +12,9 @@
 // of a group.  Statistics and sums are fp32 (row sums by shuffles in a fixed
 // order); dw is summed per thread, then per block, then over the blocks'
 // partials in block order, so results do not depend on timing.
+#include <initializer_list>
+#include <mutex>
+
 #include "lf_common.cuh"
 
 namespace lfb {
@@ -93,9 +96,18 @@ constexpr int block_of() {
     return G <= 32 ? 256 : G;
 }
 
+// Blocks per SM that the forward is compiled for.  Rows of two vectors per
+// thread run best with 16 (one warp per row) or 24 warps per SM resident:
+// bf16, width 1024, 131072 rows: 167 us at 24 warps, 201 at 32, where values
+// spill (171 without a bound); width 512: 96 us at 16, 115 at 24 (130 without).
+template <int NV, int G>
+constexpr int fwd_blocks() {
+    return NV != 2 ? 1 : G <= 32 ? 2 : G >= 512 ? 1 : 24 * 32 / G;
+}
+
 // Element j of vector i of thread g is column (i*G + g)*VEC + j.
 template <typename T, int VEC, int NV, int G, bool QUANT>
-__global__ void __launch_bounds__(block_of<G>()) rms_fwd_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(block_of<G>(), fwd_blocks<NV, G>()) rms_fwd_kernel(const NormArgs p) {
     constexpr int RPB = block_of<G>() / G;  // rows in flight per block
     __shared__ float red[32];
     const int g = threadIdx.x % G, sub = threadIdx.x / G;
@@ -343,79 +355,132 @@ __global__ void __launch_bounds__(512) rms_bwd_long_kernel(const NormBwdArgs p) 
     }
 }
 
-// dw[c] = sum over blocks of part[block][c]: 32 columns per block, 8 strided
+// dw[c] = sum over blocks of part[block][c]: 32 columns per block, 32 strided
 // partial sums per column joined in order.
 template <typename T>
-__global__ void __launch_bounds__(256) rms_dw_kernel(const float* part, T* dw, int blocks, int64_t cols) {
-    __shared__ float sh[8][33];
+__global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, T* dw, int blocks, int64_t cols) {
+    __shared__ float sh[32][33];
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     float t = 0.f;
     if (c < cols)
-        for (int b = k; b < blocks; b += 8) t += part[(int64_t)b * cols + c];
+#pragma unroll 4
+        for (int b = k; b < blocks; b += 32) t += part[(int64_t)b * cols + c];
     sh[k][lane] = t;
     __syncthreads();
     if (k == 0 && c < cols) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) t += sh[i][lane];
+        for (int i = 1; i < 32; ++i) t += sh[i][lane];
         dw[c] = Elem<T>::store(t);
     }
 }
 
-// Threads per row and vectors per thread.  A warp (or part of one) per row
-// up to 1024 16-bit columns keeps the reductions to shuffles; wider rows take
-// a block.  Rows whose width or base does not divide a 16-byte load use
-// scalar (still coalesced) accesses, eight per thread.
-#define LFB_NORM_SHAPES(T, V, cols, vec, CALL)                            \
-    if (vec) {                                                            \
-        if (cols <= 8 * V) { CALL(T, V, 1, 8); }                          \
-        else if (cols <= 32 * V) { CALL(T, V, 1, 32); }                   \
-        else if (cols <= 64 * V) { CALL(T, V, 2, 32); }                   \
-        else if (cols <= 128 * V) { CALL(T, V, 4, 32); }                  \
-        else if (cols <= 512 * V) { CALL(T, V, 4, 128); }                 \
-        else if (cols <= 2048 * V) { CALL(T, V, 4, 512); }                \
-        else long_rows = true;                                            \
-    } else {                                                              \
-        if (cols <= 256) { CALL(T, 1, 8, 32); }                           \
-        else if (cols <= 1024) { CALL(T, 1, 8, 128); }                    \
-        else if (cols <= 4096) { CALL(T, 1, 8, 512); }                    \
-        else long_rows = true;                                            \
+// Vectors per thread (NV) and threads per row (G).  Rows that divide into
+// 16-byte vectors: one or two vectors per thread in the forward and one in
+// the backward, whose running dw takes the registers of another; more
+// registers per thread cost more occupancy than the wider row groups' block
+// reductions (bf16 width 1024: forward (2,64) 167 us, (1,128) 209, (4,32) 277;
+// backward (1,128) 181, (2,64) 183, (4,32) 391; width 512 forward (2,32) 96,
+// (1,64) 103).  Other rows use scalar (still coalesced) accesses, four or
+// eight per thread.
+#define LFB_NORM_FWD(T, V, cols, vec, CALL)             \
+    if (vec) {                                          \
+        if (cols <= 8 * V) { CALL(T, V, 1, 8); }        \
+        else if (cols <= 16 * V) { CALL(T, V, 1, 16); } \
+        else if (cols <= 32 * V) { CALL(T, V, 1, 32); } \
+        else if (cols <= 64 * V) { CALL(T, V, 2, 32); } \
+        else if (cols <= 128 * V) { CALL(T, V, 2, 64); } \
+        else if (cols <= 256 * V) { CALL(T, V, 2, 128); } \
+        else if (cols <= 512 * V) { CALL(T, V, 2, 256); } \
+        else if (cols <= 1024 * V) { CALL(T, V, 2, 512); } \
+        else if (cols <= 2048 * V) { CALL(T, V, 4, 512); } \
+        else long_rows = true;                          \
+    } else LFB_NORM_SCALAR(T, cols, CALL)
+#define LFB_NORM_BWD(T, V, cols, vec, CALL)             \
+    if (vec) {                                          \
+        if (cols <= 8 * V) { CALL(T, V, 1, 8); }        \
+        else if (cols <= 16 * V) { CALL(T, V, 1, 16); } \
+        else if (cols <= 32 * V) { CALL(T, V, 1, 32); } \
+        else if (cols <= 64 * V) { CALL(T, V, 1, 64); } \
+        else if (cols <= 128 * V) { CALL(T, V, 1, 128); } \
+        else if (cols <= 256 * V) { CALL(T, V, 1, 256); } \
+        else if (cols <= 512 * V) { CALL(T, V, 1, 512); } \
+        else if (cols <= 1024 * V) { CALL(T, V, 2, 512); } \
+        else if (cols <= 2048 * V) { CALL(T, V, 4, 512); } \
+        else long_rows = true;                          \
+    } else LFB_NORM_SCALAR(T, cols, CALL)
+#define LFB_NORM_SCALAR(T, cols, CALL)              \
+    {                                               \
+        if (cols <= 128) { CALL(T, 1, 4, 32); }     \
+        else if (cols <= 512) { CALL(T, 1, 4, 128); } \
+        else if (cols <= 1024) { CALL(T, 1, 4, 256); } \
+        else if (cols <= 2048) { CALL(T, 1, 4, 512); } \
+        else if (cols <= 4096) { CALL(T, 1, 8, 512); } \
+        else long_rows = true;                      \
     }
 
-unsigned row_blocks(int64_t rows, int per_block, int block) {
-    const int64_t want = (rows + per_block - 1) / per_block, slots = (int64_t)num_sms() * (2048 / block);
+// Blocks that are resident at once: the kernels walk the rows in strides of
+// the grid, and one resident wave measured best (two: 1 % slower, one block
+// per row group: 6 %).
+template <auto Kernel>
+int resident_blocks(int block, size_t smem) {
+    static std::once_flag once[64];
+    static int per_sm[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    dev &= 63;
+    std::call_once(once[dev], [&] {
+        int v = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, Kernel, block, smem) != cudaSuccess || v < 1) v = 1;
+        per_sm[dev] = v;
+    });
+    return per_sm[dev] * num_sms();
+}
+
+unsigned row_blocks(int64_t rows, int per_block, int slots) {
+    const int64_t want = (rows + per_block - 1) / per_block;
     return (unsigned)(want < slots ? want : slots);
 }
 
-// Blocks of the backward: its partial sums are one row of `cols` per block,
-// so wide rows get fewer blocks.
-int bwd_blocks(int64_t rows, int64_t cols) {
-    const int64_t most = (int64_t)num_sms() * (cols <= 256 ? 4 : 2), want = (rows + 7) / 8;
-    return (int)(want < 1 ? 1 : want < most ? want : most);
+// Rows of partial sums in the backward's workspace: never fewer than its
+// blocks, of which there are at most 2048 threads' worth per SM.
+int64_t bwd_part_rows(int64_t rows, int64_t cols) {
+    const int64_t most = (int64_t)num_sms() * (cols <= 256 ? 8 : 32);
+    return rows < most ? rows : most;
 }
 
 template <typename T, bool QUANT>
 void launch_fwd(const NormArgs& a, bool vec, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     bool long_rows = false;
-#define LFB_CALL(TT, VV, NV, G)                                                                                   \
-    rms_fwd_kernel<TT, VV, NV, G, QUANT><<<row_blocks(a.rows, block_of<G>() / G, block_of<G>()), block_of<G>(), 0, st>>>(a)
-    LFB_NORM_SHAPES(T, V, a.cols, vec, LFB_CALL)
+#define LFB_CALL(TT, VV, NV, G)                                                                                    \
+    rms_fwd_kernel<TT, VV, NV, G, QUANT>                                                                           \
+        <<<row_blocks(a.rows, block_of<G>() / G, resident_blocks<rms_fwd_kernel<TT, VV, NV, G, QUANT>>(block_of<G>(), 0)), \
+           block_of<G>(), 0, st>>>(a)
+    LFB_NORM_FWD(T, V, a.cols, vec, LFB_CALL)
 #undef LFB_CALL
-    if (long_rows) rms_fwd_long_kernel<T, QUANT><<<row_blocks(a.rows, 1, 512), 512, 0, st>>>(a);
+    if (long_rows)
+        rms_fwd_long_kernel<T, QUANT><<<row_blocks(a.rows, 1, resident_blocks<rms_fwd_long_kernel<T, QUANT>>(512, 0)), 512, 0, st>>>(a);
 }
 
 template <typename T>
 void launch_bwd(const NormBwdArgs& a, void* dw, bool vec, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     bool long_rows = false;
-    const int blocks = bwd_blocks(a.rows, a.cols);
-    const size_t smem = a.part && a.cols <= 1024 ? (size_t)a.cols * 32 : 0;
-#define LFB_CALL(TT, VV, NV, G) rms_bwd_kernel<TT, VV, NV, G><<<blocks, block_of<G>(), G <= 32 ? smem : 0, st>>>(a)
-    LFB_NORM_SHAPES(T, V, a.cols, vec, LFB_CALL)
+    unsigned blocks = 1;
+    const int64_t most = bwd_part_rows(a.rows, a.cols);
+    auto grid = [&](int per_block, int slots) {
+        return blocks = row_blocks(a.rows, per_block, (int)(slots < most ? slots : most));
+    };
+    // Shared memory of the largest width that a warp-per-row group takes, so that residency does not depend on cols.
+#define LFB_CALL(TT, VV, NV, G)                                                                                  \
+    rms_bwd_kernel<TT, VV, NV, G>                                                                                \
+        <<<grid(block_of<G>() / G, resident_blocks<rms_bwd_kernel<TT, VV, NV, G>>(block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0)), \
+           block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0, st>>>(a)
+    LFB_NORM_BWD(T, V, a.cols, vec, LFB_CALL)
 #undef LFB_CALL
-    if (long_rows) rms_bwd_long_kernel<T><<<blocks, 512, 0, st>>>(a);
-    if (dw) rms_dw_kernel<T><<<(unsigned)((a.cols + 31) / 32), 256, 0, st>>>(a.part, (T*)dw, blocks, a.cols);
+    if (long_rows) rms_bwd_long_kernel<T><<<grid(1, resident_blocks<rms_bwd_long_kernel<T>>(512, 0)), 512, 0, st>>>(a);
+    if (dw) rms_dw_kernel<T><<<(unsigned)((a.cols + 31) / 32), 1024, 0, st>>>(a.part, (T*)dw, (int)blocks, a.cols);
 }
 
 int check_rows(const char* what, int64_t rows, int64_t cols, int dtype) {
@@ -498,7 +563,7 @@ extern "C" int lf_quantize_rows(const void* x, void* q, float* scale, int64_t ro
 
 extern "C" size_t lf_rms_norm_bwd_workspace_size(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return (size_t)bwd_blocks(rows, cols) * cols * sizeof(float);
+    return (size_t)bwd_part_rows(rows, cols) * cols * sizeof(float);
 }
 
 extern "C" int lf_rms_norm_bwd(const void* dy, const void* ds, const void* s, const float* rstd, const void* weight,
