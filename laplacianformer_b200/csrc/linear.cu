@@ -149,6 +149,7 @@ struct Epilogue {
     int64_t ldo, ldr;
     int act;
     bool act_bwd, vec_out, vec_res;
+    bool vec16;              // the product kernel may write whole 16-byte chunks (set by run_product)
 };
 
 template <int ACT>
@@ -171,7 +172,7 @@ __device__ __forceinline__ float4 finish4(float4 z, float4 bias, float4 r, bool 
 // ---------------------------------------------------------------------------
 enum Mode { kLinear, kGated, kGatedBwd };
 
-constexpr int kBM = 128;                  // rows of a tile (tcgen05 M)
+constexpr int kBM = 128;                  // rows of a tile per CTA
 constexpr int kRowBytes = 128;            // a stage holds 128 bytes of K: 64 16-bit or 128 8-bit elements
 constexpr int kEpiWarps = 8;              // two per 32-lane quarter of the tensor memory
 constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
@@ -180,7 +181,7 @@ constexpr int kMaxStages = 8;
 constexpr int kTmemAll = 512;
 constexpr int kBarrierBytes = 256;
 constexpr int kSmemLimit = 227 * 1024;
-constexpr int kGroupM = 16;               // row tiles that are walked together, so that their operands stay in L2
+constexpr int kGroupRows = 2048;          // rows that are walked together, so that their operands stay in L2
 
 struct alignas(64) GemmArgs {
     CUtensorMap a, b, a2, b2;  // a2, b2: dy and Wout of the gated backward
@@ -190,33 +191,90 @@ struct alignas(64) GemmArgs {
     int m, n;                  // rows of one row segment; output columns (hidden columns of the gated modes)
     int msegs, tiles_m, tiles_n, splits;
     int iters, split_iters, seg_iters;  // K steps in all, per split, per K segment
-    int bn, stages, nbuf;      // columns of the first product; ring depth; accumulator buffers
+    int bn, stages, stage_bytes;        // columns of a tile's (first) product; ring depth
     uint32_t idesc, idesc2;
     bool a_mn, b_mn;
 };
 
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {  // the same shared memory in CTA 0 of the cluster
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+// Copies into this CTA's shared memory.  A pair's copies all count on the
+// barrier of its first CTA, which issues the products.
+template <int CTAS>
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, "
+            "%5}], [%2];" ::"r"(smem_u32(dst)),
+            "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
 }
 __device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+    if constexpr (CTAS == 2)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+    else
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate, uint32_t go) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(go)
-        : "memory");
+#define LFB_MMA(CG, KIND)                                                                              \
+    asm volatile(                                                                                      \
+        "{\n\t.reg .pred p, q;\n\t"                                                                    \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                                    \
+        "setp.ne.b32 q, %5, 0;\n\t"                                                                    \
+        "@q tcgen05.mma.cta_group::" CG ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),   \
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(go)                                   \
+        : "memory")
+// D[tmem] (+)= A[smem] B[smem]; the whole warp executes it, the lane with go != 0 issues it.
+template <int CTAS, bool FP8>
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate,
+                                    uint32_t go) {
+    if constexpr (CTAS == 2 && FP8) LFB_MMA("2", "f8f6f4");
+    else if constexpr (CTAS == 2) LFB_MMA("2", "f16");
+    else if constexpr (FP8) LFB_MMA("1", "f8f6f4");
+    else LFB_MMA("1", "f16");
+}
+#undef LFB_MMA
+// Arrives on the barrier (of both CTAs of a pair) when the products issued so far are done.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else mma_commit(bar);
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_take(uint32_t* dst) {
+    if constexpr (CTAS == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(kTmemAll) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else tmem_alloc(dst, kTmemAll);
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t taddr) {
+    if constexpr (CTAS == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(kTmemAll) : "memory");
+    else tmem_dealloc(taddr, kTmemAll);
+}
+template <int CTAS>
+__device__ __forceinline__ void sync_all() {
+    if constexpr (CTAS == 2)
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -234,20 +292,22 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 struct Tile {
     int seg, m0, n0, split, it0, it1;
 };
-// Work units: for each split of K, row tiles in groups of kGroupM, within a
+// Work units: for each split of K, row tiles in groups of kGroupRows, within a
 // group all row tiles of one column tile before the next column tile.
-__device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out) {
+template <int CTAS>
+__device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out, int rank) {
+    constexpr int kGroup = kGroupRows / (kBM * CTAS);
     const int rows = p.msegs * p.tiles_m, tiles = rows * p.tiles_n;
     Tile t;
     t.split = unit / tiles;
     int r = unit - t.split * tiles;
-    const int group = r / (kGroupM * p.tiles_n), first = group * kGroupM;
-    const int gm = min(kGroupM, rows - first);
-    r -= group * kGroupM * p.tiles_n;
-    const int mi = first + r % gm;
-    t.n0 = (r / gm) * bn_out;
+    const int group = r / (kGroup * p.tiles_n), first = group * kGroup;
+    const int gm = min(kGroup, rows - first);
+    r -= group * kGroup * p.tiles_n;
+    const int ni = r / gm, mi = first + r - ni * gm;
+    t.n0 = ni * bn_out;
     t.seg = mi / p.tiles_m;
-    t.m0 = (mi - t.seg * p.tiles_m) * kBM;
+    t.m0 = ((mi - t.seg * p.tiles_m) * CTAS + rank) * kBM;
     t.it0 = t.split * p.split_iters;
     t.it1 = min(p.iters, t.it0 + p.split_iters);
     return t;
@@ -265,130 +325,162 @@ __device__ __forceinline__ void stage16(uint8_t* st, int lane, const float (&v)[
         *reinterpret_cast<uint4*>(st + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = u;
     }
 }
+// out: row 0 of the warp's rows, of which `rows` exist; ld and col0 are multiples of 8.
 template <typename T>
-__device__ __forceinline__ void unstage16(const uint8_t* st, int lane, T* out, int64_t ld, int row0, int rows, int col0) {
+__device__ __forceinline__ void unstage16(const uint8_t* st, int lane, T* out, int64_t ld, int rows, int col0) {
+    const int c = lane & 3;
+    if (col0 + c * 8 >= ld) return;
+    T* o = out + (lane >> 2) * ld + col0 + c * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = i * 8 + (lane >> 2), c = lane & 3;
-        if (row0 + row < rows && col0 + c * 8 < ld)
-            *reinterpret_cast<uint4*>(out + (row0 + row) * ld + col0 + c * 8) =
-                *reinterpret_cast<const uint4*>(st + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+    for (int i = 0; i < 4; ++i, o += 8 * ld) {
+        const int row = i * 8 + (lane >> 2);
+        if (row < rows) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(st + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
     }
 }
 
-// Reads 32 bias values of columns col0.. into per-warp shared memory.
 template <typename T>
-__device__ __forceinline__ void bias_to_smem(float* sb, const T* bias, int lane, int col0, int n) {
-    sb[lane] = bias && col0 + lane < n ? Elem<T>::load(bias[col0 + lane]) : 0.f;
+__device__ __forceinline__ float column_value(const T* p, int col, int n) {
+    return p && col < n ? Elem<T>::load(p[col]) : 0.f;
 }
 
-template <typename T, int MODE, bool FP8>
+// A CTA (CTAS = 1) or a pair of CTAs on two SMs (CTAS = 2) walks tiles of
+// 128 CTAS rows.  In a pair every CTA holds its own rows of A, half of B's
+// columns and the accumulators of its own rows; its first CTA issues the
+// products of both.
+//
+// kLinear: out = epilogue(A B^T), two accumulator buffers.
+// kGated: B's tile is bn/2 gate and bn/2 up rows of Win, the accumulator's
+// halves are g and u of the same hidden columns.
+// kGatedBwd: first dh = dy Wout (accumulators at 256 or 384, in turn), then
+// [g|u] = x Win^T at 0: while the epilogue reads a tile, the next tile's dh is
+// computed.
+template <typename T, int MODE, bool FP8, int CTAS>
 __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];  // stages, output staging, barriers
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int BK = FP8 ? 128 : 64;
-    const int bh = p.bn / 2;                                   // hidden columns of a gated tile
-    const int bn_out = MODE == kLinear ? p.bn : bh;
-    const int cols = MODE == kGatedBwd ? 3 * bh : p.bn;        // accumulator columns
-    constexpr int kABytes = kBM * kRowBytes * (MODE == kGatedBwd ? 2 : 1);
-    const int stage_bytes = kABytes + (MODE == kGatedBwd ? 3 * bh : p.bn) * kRowBytes;
-    uint8_t* out_stage = smem + p.stages * stage_bytes;
+    uint8_t* out_stage = smem + p.stages * p.stage_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * kStageOut);
     uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *drain = tempty + 2;
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0;
+    constexpr int BK = FP8 ? 128 : 64;
+    constexpr int kABytes = kBM * kRowBytes;
+    constexpr int kDh = 256;                                   // tensor memory columns of dh
+    const int bh = p.bn / 2;                                   // hidden columns of a gated tile
+    const int bn_out = MODE == kLinear ? p.bn : bh;
+    const int phases = MODE == kGatedBwd ? 2 : 1;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps);
+        for (int i = 0; i < 2; ++i) mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps * CTAS);
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tmem_alloc(tmem_ptr, kTmemAll);
+    if (warp == 1) tmem_take<CTAS>(tmem_ptr);
     tc_fence_before();
     __syncthreads();
+    sync_all<CTAS>();
     tc_fence_after();
     const uint32_t tmem = *tmem_ptr;
     const int units = p.splits * p.msegs * p.tiles_m * p.tiles_n;
+    const int unit0 = blockIdx.x / CTAS, unit_step = gridDim.x / CTAS;
     bool ok = true;
 
     if (warp == 0) {
         if (elect_one()) {
             int s = 0, issued = 0;
             uint32_t ph = 0;
-            for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
-                const Tile t = tile_of(p, unit, bn_out);
-                for (int it = t.it0; it < t.it1; ++it) {
-                    if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
-                    const int ks = it / p.seg_iters, k0 = (it - ks * p.seg_iters) * BK;
-                    uint8_t* sa = smem + s * stage_bytes;
-                    uint8_t* sb = sa + kABytes;
-                    mbar_expect(&full[s], stage_bytes);
-                    if (!p.a_mn) tma_load(sa, &p.a, &full[s], k0, t.m0, ks);
-                    else
-                        for (int j = 0; j < kBM / 64; ++j) tma_load(sa + j * 8192, &p.a, &full[s], t.m0 + 64 * j, k0, t.seg);
-                    if (MODE == kLinear) {
-                        if (!p.b_mn) tma_load(sb, &p.b, &full[s], k0, t.n0, ks);
-                        else
-                            for (int j = 0; j < p.bn / 64; ++j)
-                                tma_load(sb + j * 8192, &p.b, &full[s], t.n0 + 64 * j, k0, ks);
-                    } else {
-                        tma_load(sb, &p.b, &full[s], k0, t.n0, 0);
-                        tma_load(sb + bh * kRowBytes, &p.b, &full[s], k0, t.n0, 1);
+            const int bw = p.bn / CTAS;                        // B rows that this CTA holds
+            for (int unit = unit0; ok && unit < units; unit += unit_step) {
+                const Tile t = tile_of<CTAS>(p, unit, bn_out, rank);
+                for (int phase = 0; ok && phase < phases; ++phase) {
+                    const bool dh = MODE == kGatedBwd && phase == 0;
+                    const uint32_t bytes = kABytes + (dh ? bh / CTAS : bw) * kRowBytes;
+                    for (int it = t.it0; it < t.it1; ++it) {
+                        if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
+                        const int ks = it / p.seg_iters, k0 = (it - ks * p.seg_iters) * BK;
+                        uint8_t* sa = smem + s * p.stage_bytes;
+                        uint8_t* sb = sa + kABytes;
+                        const uint32_t bar = CTAS == 2 ? leader_addr(&full[s]) : smem_u32(&full[s]);
+                        if (rank == 0) mbar_expect(&full[s], bytes * CTAS);
+                        if (dh) {
+                            tma_load<CTAS>(sa, &p.a2, bar, k0, t.m0, 0);
+                            for (int j = 0; j < bh / CTAS / 64; ++j)
+                                tma_load<CTAS>(sb + j * 8192, &p.b2, bar, t.n0 + rank * (bh / CTAS) + 64 * j, k0, 0);
+                        } else {
+                            if (!p.a_mn) tma_load<CTAS>(sa, &p.a, bar, k0, t.m0, ks);
+                            else
+                                for (int j = 0; j < kBM / 64; ++j)
+                                    tma_load<CTAS>(sa + j * 8192, &p.a, bar, t.m0 + 64 * j, k0, t.seg);
+                            if (MODE == kLinear) {
+                                if (!p.b_mn) tma_load<CTAS>(sb, &p.b, bar, k0, t.n0 + rank * bw, ks);
+                                else
+                                    for (int j = 0; j < bw / 64; ++j)
+                                        tma_load<CTAS>(sb + j * 8192, &p.b, bar, t.n0 + rank * bw + 64 * j, k0, ks);
+                            } else if (CTAS == 2) {            // one CTA the gate rows, the other the up rows
+                                tma_load<CTAS>(sb, &p.b, bar, k0, t.n0, rank);
+                            } else {
+                                tma_load<CTAS>(sb, &p.b, bar, k0, t.n0, 0);
+                                tma_load<CTAS>(sb + bh * kRowBytes, &p.b, bar, k0, t.n0, 1);
+                            }
+                        }
+                        ++issued;
+                        if (++s == p.stages) s = 0, ph ^= 1;
                     }
-                    if (MODE == kGatedBwd) {
-                        tma_load(sa + kBM * kRowBytes, &p.a2, &full[s], k0, t.m0, 0);
-                        for (int j = 0; j < bh / 64; ++j)
-                            tma_load(sb + p.bn * kRowBytes + j * 8192, &p.b2, &full[s], t.n0 + 64 * j, k0, 0);
-                    }
-                    ++issued;
-                    if (++s == p.stages) s = 0, ph ^= 1;
                 }
             }
-            // A wait ran out: let the copies in flight land before the block ends.
-            if (!ok)
+            // A wait ran out: let the copies in flight land before the block
+            // ends (the leader's barriers count both CTAs' copies).
+            if (!ok && rank == 0)
                 for (int k = max(0, issued - p.stages); k < issued; ++k)
                     mbar_wait(&full[k % p.stages], (k / p.stages) & 1, 100000000ull);
         }
         __syncwarp();
     } else if (warp == 1) {
-        const uint32_t go = elect_one() ? 1u : 0u;
-        const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
-        const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
-        int s = 0, buf = 0;
-        uint32_t ph = 0, bph = 0;
-        for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
-            const Tile t = tile_of(p, unit, bn_out);
-            if (!(ok = mbar_wait(&tempty[buf], bph ^ 1))) break;
-            tc_fence_after();
-            const uint32_t acc = tmem + buf * cols;
-            for (int it = t.it0; it < t.it1; ++it) {
-                if (!(ok = mbar_wait(&full[s], ph))) break;
-                tc_fence_after();
-                const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + kABytes;
-                const uint64_t da = make_desc(sa, a_lbo, 1024), db = make_desc(sb, b_lbo, 1024);
+        if (rank == 0) {
+            const uint32_t go = elect_one() ? 1u : 0u;
+            const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
+            const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
+            int s = 0, buf = 0;
+            uint32_t ph = 0, bph = 0;
+            for (int unit = unit0; ok && unit < units; unit += unit_step) {
+                const Tile t = tile_of<CTAS>(p, unit, bn_out, 0);
+                for (int phase = 0; ok && phase < phases; ++phase) {
+                    const bool dh = MODE == kGatedBwd && phase == 0;
+                    // dh goes where the epilogue two tiles ago read, which had to end before the last tile's g and u.
+                    if (!dh) {
+                        if (!(ok = mbar_wait(&tempty[MODE == kGatedBwd ? 0 : buf], bph ^ 1))) break;
+                        tc_fence_after();
+                    }
+                    const uint32_t acc = tmem + (MODE != kGatedBwd ? buf * 256 : dh ? kDh + buf * 128 : 0);
+                    for (int it = t.it0; it < t.it1; ++it) {
+                        if (!(ok = mbar_wait(&full[s], ph))) break;
+                        tc_fence_after();
+                        const uint32_t sa = smem_u32(smem + s * p.stage_bytes), sb = sa + kABytes;
+                        if (dh) {
+                            const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sb, 8192, 1024);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t add = it > t.it0 || k > 0 ? 1u : 0u;
-                    if (FP8) mma_f8(acc, da + k * a_step, db + k * b_step, p.idesc, add, go);
-                    else mma_f16(acc, da + k * a_step, db + k * b_step, p.idesc, add, go);
-                }
-                if (MODE == kGatedBwd) {
-                    const uint64_t da2 = make_desc(sa + kBM * kRowBytes, 16, 1024);
-                    const uint64_t db2 = make_desc(sb + p.bn * kRowBytes, 8192, 1024);
+                            for (int k = 0; k < 4; ++k)
+                                mma<CTAS, FP8>(acc, da + k * 2, db + k * 128, p.idesc2, it > t.it0 || k > 0 ? 1u : 0u, go);
+                        } else {
+                            const uint64_t da = make_desc(sa, a_lbo, 1024), db = make_desc(sb, b_lbo, 1024);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_f16(acc + p.bn, da2 + k * 2, db2 + k * 128, p.idesc2, it > t.it0 || k > 0 ? 1u : 0u, go);
+                            for (int k = 0; k < 4; ++k)
+                                mma<CTAS, FP8>(acc, da + k * a_step, db + k * b_step, p.idesc, it > t.it0 || k > 0 ? 1u : 0u, go);
+                        }
+                        if (go) commit<CTAS>(&empty[s]);
+                        if (++s == p.stages) s = 0, ph ^= 1;
+                    }
                 }
-                if (go) mma_commit(&empty[s]);
-                if (++s == p.stages) s = 0, ph ^= 1;
+                if (!ok) break;
+                if (go) commit<CTAS>(&tfull[MODE == kGatedBwd ? 0 : buf]);
+                buf ^= 1;
+                if (MODE == kGatedBwd || buf == 0) bph ^= 1;
             }
-            if (!ok) break;
-            if (go) mma_commit(&tfull[buf]);
-            if (++buf == p.nbuf) buf = 0, bph ^= 1;
-        }
-        if (!ok) {  // products in flight end before the tensor memory is freed
-            if (go) mma_commit(drain);
-            mbar_wait(drain, 0, 100000000ull);
+            if (!ok) {  // products in flight end before the tensor memory is freed
+                if (go) commit<CTAS>(drain);
+                mbar_wait(drain, 0, 100000000ull);
+            }
         }
     } else {
         const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
@@ -396,159 +488,206 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
         int buf = 0;
         uint32_t bph = 0;
         const Epilogue& e = p.e;
-        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-            const Tile t = tile_of(p, unit, bn_out);
-            if (!(ok = mbar_wait(&tfull[buf], bph))) break;
-            tc_fence_after();
-            const uint32_t acc = tmem + buf * cols + ((uint32_t)(quad * 32) << 16);
-            const int row0 = t.m0 + quad * 32;
-            for (int c0 = half * 32; c0 < bn_out; c0 += 64) {
-                if (t.n0 + c0 >= p.n) break;
-                const int col0 = t.n0 + c0;
-                if constexpr (MODE == kLinear) {
-                    // Raw sums through shared memory, so that a lane has four
-                    // columns and residual, bias and output are row segments.
-                    const int col = col0 + (lane & 7) * 4;
-                    const int64_t seg_row = (int64_t)t.seg * p.m;
-                    uint2 r[8];
-                    if (e.res && !p.part) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int row = row0 + i * 4 + (lane >> 3);
-                            r[i] = row < p.m ? load4((const T*)e.res + (seg_row + row) * e.ldr, col, p.n, e.vec_res)
-                                             : make_uint2(0u, 0u);
+        for (int unit = unit0; unit < units; unit += unit_step) {
+            const Tile t = tile_of<CTAS>(p, unit, bn_out, rank);
+            const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+            const int rows = p.m - t.m0 - quad * 32;                           // rows that exist from the warp's first on
+            const int64_t row0 = (int64_t)t.seg * p.m + t.m0 + quad * 32;      // in the output
+            const int cend = min(bn_out, p.n - t.n0);
+            uint64_t* tf = &tfull[MODE == kGatedBwd ? 0 : buf];
+            if constexpr (MODE == kLinear) {
+                const uint32_t acc = tmem + buf * 256 + lanes;
+                const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
+                if (e.vec16) {
+                    // Whole 16-byte chunks and no residual: finished in the
+                    // accumulator's layout (a lane owns a row), column
+                    // values of the next 32 columns fetched ahead.
+                    float* cv = reinterpret_cast<float*>(st + 2048);
+                    float bias = column_value((const T*)e.bias, t.n0 + half * 32 + lane, p.n);
+                    float sb = FP8 && t.n0 + half * 32 + lane < p.n ? e.sb[t.n0 + half * 32 + lane] : 1.f;
+                    if (!(ok = mbar_wait(tf, bph))) break;
+                    tc_fence_after();
+                    for (int c0 = half * 32; c0 < cend; c0 += 64) {
+                        float v[32];
+                        tmem_ld32(acc + c0, v);
+                        if (FP8 || e.bias) {
+                            cv[lane] = bias;
+                            if (FP8) cv[32 + lane] = sb;
+                            const int next = t.n0 + c0 + 64 + lane;
+                            bias = column_value((const T*)e.bias, next, p.n);
+                            if (FP8) sb = next < p.n ? e.sb[next] : 1.f;
+                            __syncwarp();
                         }
+                        tmem_wait_ld();
+                        reg_fence(v);
+                        if (FP8) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(v[j], sa * cv[32 + j], cv[j]);
+                        } else if (e.bias) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] += cv[j];
+                        }
+                        if (e.act != LF_ACT_NONE)
+                            with_act(e.act, [&](auto act) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(act)::value>(v[j]);
+                            });
+                        stage16<T>(st, lane, v);
+                        __syncwarp();
+                        unstage16(st, lane, (T*)e.out + row0 * e.ldo, e.ldo, rows, t.n0 + c0);
+                        __syncwarp();
                     }
-                    float v[32];
-                    tmem_ld32(acc + c0, v);
-                    tmem_wait_ld();
-                    reg_fence(v);
+                } else {
+                    // Raw sums through shared memory, so that a lane has four
+                    // columns of eight rows and residual, bias and output are
+                    // row segments; the next 32 columns' residual and bias
+                    // are fetched ahead.
+                    uint2 r[8];
+                    float4 b, sb;
+                    auto fetch = [&](int c0) {
+                        const int col = t.n0 + c0 + (lane & 7) * 4;
+                        if (c0 >= cend || p.part) return;
+                        if (e.res) {
+                            const T* q = (const T*)e.res + (row0 + (lane >> 3)) * e.ldr;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                    __syncwarp();
-                    auto staged = [&](int i) {
-                        const int row = i * 4 + (lane >> 3);
-                        return *reinterpret_cast<const float4*>(st + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
-                    };
-                    if (p.part) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int row = row0 + i * 4 + (lane >> 3);
-                            if (row < p.m && col < p.ldp)
-                                *reinterpret_cast<float4*>(
-                                    p.part + ((int64_t)t.split * p.msegs * p.m + seg_row + row) * p.ldp + col) = staged(i);
+                            for (int i = 0; i < 8; ++i, q += 4 * e.ldr)
+                                r[i] = i * 4 + (lane >> 3) < rows ? load4(q, col, p.n, e.vec_res) : make_uint2(0u, 0u);
                         }
-                    } else {
-                        float4 b = make_float4(0.f, 0.f, 0.f, 0.f), sb = make_float4(1.f, 1.f, 1.f, 1.f);
                         if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, p.n, false));
                         if (FP8) {
                             float* q = reinterpret_cast<float*>(&sb);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) q[j] = col + j < p.n ? e.sb[col + j] : 0.f;
                         }
-                        with_act(e.act, [&](auto act) {
+                    };
+                    b = sb = make_float4(0.f, 0.f, 0.f, 0.f);
+                    fetch(half * 32);
+                    if (!(ok = mbar_wait(tf, bph))) break;
+                    tc_fence_after();
+                    for (int c0 = half * 32; c0 < cend; c0 += 64) {
+                        const int col = t.n0 + c0 + (lane & 7) * 4;
+                        float v[32];
+                        tmem_ld32(acc + c0, v);
+                        tmem_wait_ld();
+                        reg_fence(v);
+                        if (FP8) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int row = row0 + i * 4 + (lane >> 3);
-                                if (row < p.m) {
-                                    float4 z = staged(i);
-                                    if (FP8) {
-                                        const float s = e.sa[seg_row + row];
-                                        z.x *= s * sb.x, z.y *= s * sb.y, z.z *= s * sb.z, z.w *= s * sb.w;
+                            for (int j = 0; j < 32; ++j) v[j] *= sa;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                                make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                        __syncwarp();
+                        auto staged = [&](int i) {
+                            const int row = i * 4 + (lane >> 3);
+                            return *reinterpret_cast<const float4*>(st + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+                        };
+                        if (p.part) {
+                            float* q = p.part + ((int64_t)t.split * p.msegs * p.m + row0 + (lane >> 3)) * p.ldp + col;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i, q += 4 * p.ldp)
+                                if (i * 4 + (lane >> 3) < rows && col < p.ldp) *reinterpret_cast<float4*>(q) = staged(i);
+                        } else {
+                            T* out = (T*)e.out + (row0 + (lane >> 3)) * e.ldo;
+                            with_act(e.act, [&](auto act) {
+                                T* q = out;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i, q += 4 * e.ldo)
+                                    if (i * 4 + (lane >> 3) < rows) {
+                                        float4 z = staged(i);
+                                        if (FP8) z.x *= sb.x, z.y *= sb.y, z.z *= sb.z, z.w *= sb.w;
+                                        const float4 x = e.res ? widen4<T>(r[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                        store4(q, col, p.n, e.vec_out, finish4<decltype(act)::value>(z, b, x, e.act_bwd));
                                     }
-                                    const float4 x = e.res ? widen4<T>(r[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
-                                    store4((T*)e.out + (seg_row + row) * e.ldo, col, p.n, e.vec_out,
-                                           finish4<decltype(act)::value>(z, b, x, e.act_bwd));
-                                }
-                            }
-                        });
-                    }
-                    __syncwarp();
-                } else if constexpr (MODE == kGated) {
-                    float g[32], u[32];
-                    float* sb = reinterpret_cast<float*>(st + 2048);
-                    if (e.bias) {
-                        bias_to_smem(sb, (const T*)e.bias, lane, col0, p.n);
-                        bias_to_smem(sb + 32, (const T*)e.bias + p.n, lane, col0, p.n);
-                    }
-                    tmem_ld32(acc + c0, g);
-                    tmem_ld32(acc + bh + c0, u);
-                    tmem_wait_ld();
-                    reg_fence(g);
-                    reg_fence(u);
-                    __syncwarp();
-                    if (e.bias) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) g[j] += sb[j], u[j] += sb[32 + j];
-                    }
-                    with_act(e.act, [&](auto act) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
-                    });
-                    stage16<T>(st, lane, u);
-                    __syncwarp();
-                    unstage16(st, lane, (T*)e.out, e.ldo, row0, p.m, col0);
-                    __syncwarp();
-                } else {
-                    float g[32], u[32], d[32];
-                    float* sb = reinterpret_cast<float*>(st);
-                    if (e.bias) {
-                        bias_to_smem(sb, (const T*)e.bias, lane, col0, p.n);
-                        bias_to_smem(sb + 32, (const T*)e.bias + p.n, lane, col0, p.n);
-                    }
-                    tmem_ld32(acc + c0, g);
-                    tmem_ld32(acc + bh + c0, u);
-                    tmem_wait_ld();
-                    reg_fence(g);
-                    reg_fence(u);
-                    __syncwarp();
-                    if (e.bias) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) g[j] += sb[j], u[j] += sb[32 + j];
+                            });
+                            fetch(c0 + 64);
+                        }
                         __syncwarp();
                     }
-                    // g, u become h's two factors' products: h in d, act(g) in g, u act'(g) in u.
-                    with_act(e.act, [&](auto act) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float a, slope;
-                            act_both<decltype(act)::value>(g[j], a, slope);
-                            d[j] = a * u[j];
-                            g[j] = a;
-                            u[j] *= slope;
-                        }
-                    });
-                    stage16<T>(st, lane, d);
-                    tmem_ld32(acc + 2 * bh + c0, d);
-                    __syncwarp();
-                    T* out = (T*)e.out;
-                    unstage16(st, lane, out + 2 * p.plane, e.ldo, row0, p.m, col0);
+                }
+            } else {
+                const T* bias = (const T*)e.bias;
+                const uint32_t acc = tmem + (MODE == kGated ? buf * 256 : 0) + lanes;
+                const uint32_t acc_dh = tmem + kDh + buf * 128 + lanes;
+                T* out = (T*)e.out + row0 * e.ldo;
+                float* cv = reinterpret_cast<float*>(st + 2048);
+                float bg = column_value(bias, t.n0 + half * 32 + lane, p.n);
+                float bu = column_value(bias ? bias + p.n : bias, t.n0 + half * 32 + lane, p.n);
+                if (!(ok = mbar_wait(tf, bph))) break;
+                tc_fence_after();
+                for (int c0 = half * 32; c0 < cend; c0 += 64) {
+                    const int col0 = t.n0 + c0;
+                    float g[32], u[32];
+                    tmem_ld32(acc + c0, g);
+                    tmem_ld32(acc + bh + c0, u);
+                    if (bias) {
+                        cv[lane] = bg, cv[32 + lane] = bu;
+                        bg = column_value(bias, col0 + 64 + lane, p.n);
+                        bu = column_value(bias + p.n, col0 + 64 + lane, p.n);
+                        __syncwarp();
+                    }
                     tmem_wait_ld();
-                    reg_fence(d);
-                    __syncwarp();
+                    reg_fence(g);
+                    reg_fence(u);
+                    if (bias) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) u[j] *= d[j], g[j] *= d[j];
-                    stage16<T>(st, lane, u);
-                    stage16<T>(st + 2048, lane, g);
-                    __syncwarp();
-                    unstage16(st, lane, out, e.ldo, row0, p.m, col0);
-                    unstage16(st + 2048, lane, out + p.plane, e.ldo, row0, p.m, col0);
-                    __syncwarp();
+                        for (int j = 0; j < 32; ++j) g[j] += cv[j], u[j] += cv[32 + j];
+                        __syncwarp();
+                    }
+                    if constexpr (MODE == kGated) {
+                        with_act(e.act, [&](auto act) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
+                        });
+                        stage16<T>(st, lane, u);
+                        __syncwarp();
+                        unstage16(st, lane, out, e.ldo, rows, col0);
+                        __syncwarp();
+                    } else {
+                        float d[32];
+                        // g and u become what dh is multiplied by: g = act(g), u = u act'(g); h goes out first.
+                        with_act(e.act, [&](auto act) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                float a, slope;
+                                act_both<decltype(act)::value>(g[j], a, slope);
+                                d[j] = a * u[j];
+                                g[j] = a;
+                                u[j] *= slope;
+                            }
+                        });
+                        stage16<T>(st, lane, d);
+                        tmem_ld32(acc_dh + c0, d);
+                        __syncwarp();
+                        unstage16(st, lane, out + 2 * p.plane, e.ldo, rows, col0);
+                        tmem_wait_ld();
+                        reg_fence(d);
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) u[j] *= d[j], g[j] *= d[j];
+                        stage16<T>(st, lane, u);
+                        stage16<T>(st + 2048, lane, g);
+                        __syncwarp();
+                        unstage16(st, lane, out, e.ldo, rows, col0);
+                        unstage16(st + 2048, lane, out + p.plane, e.ldo, rows, col0);
+                        __syncwarp();
+                    }
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[buf]);
-            if (++buf == p.nbuf) buf = 0, bph ^= 1;
+            if (lane == 0) arrive_leader<CTAS>(&tempty[MODE == kGatedBwd ? 0 : buf]);
+            buf ^= 1;
+            if (MODE == kGatedBwd || buf == 0) bph ^= 1;
         }
     }
     if (!ok && lane == 0) atomicExch(&g_gemm_status, (int)LF_ERR_TIMEOUT);
     tc_fence_before();
     __syncthreads();
+    sync_all<CTAS>();  // no CTA of a pair leaves while the other's products read its operands
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, kTmemAll);
+    if (warp == 1) tmem_free<CTAS>(tmem);
 }
 
 // Joins the splits of K in order and applies the epilogue.
@@ -794,32 +933,37 @@ struct Product {
     int dtype = 0, op_dtype = 0;   // output type; operand type
 };
 
+// Tile of a launch: CTAs per tile, columns, splits of K.
 struct Shape {
-    int bn, splits;
+    int ctas, bn, splits;
 };
 
-// Tile width and splits of K by an estimate in SM cycles: a K step costs bn
-// cycles of the tensor pipe (at least 128: a narrower product is bound by
-// reading A), an output column of a tile about 10 cycles of epilogue, which
-// overlaps the next tile's products; splitting costs writing and reading the
-// partial sums once more and another launch.
+// SM cycles of one K step of a tile: the tensor pipe's (two per column), or
+// fetching the CTA's operands through L2 at about 60 bytes per cycle.
+double step_cycles(int ctas, int cols, int b_rows) { return std::max(2.0 * cols, (kBM + b_rows / ctas) * kRowBytes / 60.0); }
+
+// Tile shape and splits of K by an estimate in SM cycles: the epilogue of a
+// tile overlaps the next tile's products; a split costs writing and reading
+// the partial sums once more and another launch.
 Shape choose(const Product& q) {
     const int bk = q.op_dtype == LF_F8E4M3 ? 128 : 64;
-    const int64_t iters = (q.k + bk - 1) / bk * q.ksegs, rows = (q.m + kBM - 1) / kBM * q.msegs, sms = num_sms();
-    Shape best{256, 1};
+    const int64_t iters = (q.k + bk - 1) / bk * q.ksegs, sms = num_sms();
+    Shape best{1, 256, 1};
     double least = 1e30;
-    for (int bn : {256, 128, 64}) {
-        const int64_t tiles = rows * ((q.n + bn - 1) / bn);
-        for (int s = 1; s <= 64; s *= 2) {
-            if (s > 1 && iters / s < 4) break;
-            const int64_t per = (iters + s - 1) / s, units = tiles * ((iters + per - 1) / per);
-            const int64_t waves = (units + sms - 1) / sms;
-            const double main = (double)per * std::max(bn, 128), epi = bn * 10.0;
-            double t = waves * std::max(main, epi) + std::min(main, epi) + 2000;
-            if (s > 1) t += 4000 + (double)s * q.m * q.msegs * q.n * 8 / 3400.0;
-            if (t < least) least = t, best = {bn, s};
+    for (int ctas : {2, 1})
+        for (int bn : {256, 128, 64}) {
+            if (ctas == 2 && bn == 64) continue;
+            const int64_t tiles = (q.m + kBM * ctas - 1) / (kBM * ctas) * q.msegs * ((q.n + bn - 1) / bn);
+            for (int s = 1; s <= 64; s *= 2) {
+                if (s > 1 && iters / s < 4) break;
+                const int64_t per = (iters + s - 1) / s, units = tiles * ((iters + per - 1) / per);
+                const int64_t waves = (units * ctas + sms - 1) / sms;
+                const double main = per * step_cycles(ctas, bn, bn), epi = 500 + bn * 10.0;
+                double t = waves * std::max(main, epi) + std::min(main, epi) + 2000;
+                if (s > 1) t += 4000 + (double)s * q.m * q.msegs * q.n * 8 / 3400.0;
+                if (t < least) least = t, best = {ctas, bn, s};
+            }
         }
-    }
     return best;
 }
 
@@ -827,24 +971,43 @@ size_t part_bytes(const Product& q, const Shape& s) {
     return s.splits > 1 ? (size_t)s.splits * q.m * q.msegs * up(q.n, 4) * 4 : 0;
 }
 
-uint32_t idesc_of(int dtype, bool a_mn, bool b_mn, int n) {
+uint32_t idesc_of(int dtype, bool a_mn, bool b_mn, int ctas, int n) {
     const uint32_t f = dtype == LF_BF16 ? 1u : 0u;  // kind::f16: 0 fp16, 1 bf16; kind::f8f6f4: 0 e4m3
     return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kBM * ctas >> 4) << 24);
 }
 
 template <auto Kernel>
-int launch_gemm(GemmArgs& g, int stage_bytes, cudaStream_t st) {
+int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
     constexpr int rest = kEpiWarps * kStageOut + kBarrierBytes;
-    g.stages = std::min(kMaxStages, (kSmemLimit - rest) / stage_bytes);
-    const int smem = g.stages * stage_bytes + rest;
+    g.stages = std::min(kMaxStages, (kSmemLimit - rest) / g.stage_bytes);
     static std::once_flag once[64];  // per kernel and device
     int dev = 0;
     cudaGetDevice(&dev);
     std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
     const int64_t units = (int64_t)g.splits * g.msegs * g.tiles_m * g.tiles_n;
-    Kernel<<<(unsigned)std::min<int64_t>(units, num_sms()), kGemmThreads, smem, st>>>(g);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(units, num_sms() / ctas) * ctas));
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = (size_t)g.stages * g.stage_bytes + rest;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)ctas, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, Kernel, g);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        set_error("tc_gemm_kernel: %s", cudaGetErrorString(e));
+        return LF_ERR_CUDA;
+    }
     return check_launch("tc_gemm_kernel");
+}
+
+template <typename T, int MODE, bool FP8>
+int launch_ctas(GemmArgs& g, int ctas, cudaStream_t st) {
+    return ctas == 2 ? launch_gemm<tc_gemm_kernel<T, MODE, FP8, 2>>(g, 2, st) : launch_gemm<tc_gemm_kernel<T, MODE, FP8, 1>>(g, 1, st);
 }
 
 int too_large(const char* what) {
@@ -870,7 +1033,7 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
     GemmArgs g{};
     g.m = (int)q.m, g.n = (int)q.n;
     g.msegs = q.msegs;
-    g.tiles_m = (int)((q.m + kBM - 1) / kBM);
+    g.tiles_m = (int)((q.m + kBM * s.ctas - 1) / (kBM * s.ctas));
     g.tiles_n = (int)((q.n + s.bn - 1) / s.bn);
     g.seg_iters = (int)((q.k + bk - 1) / bk);
     g.iters = g.seg_iters * q.ksegs;
@@ -879,22 +1042,20 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
     if (q.m > INT32_MAX - 256 || q.n > INT32_MAX - 256 || (int64_t)g.splits * g.msegs * g.tiles_m * g.tiles_n > INT32_MAX / 2)
         return too_large("matrix product");
     g.bn = s.bn;
-    g.nbuf = 2;
+    g.stage_bytes = (kBM + s.bn / s.ctas) * kRowBytes;
     g.a_mn = q.a_mn, g.b_mn = q.b_mn;
-    g.idesc = idesc_of(q.op_dtype, q.a_mn, q.b_mn, s.bn);
+    g.idesc = idesc_of(q.op_dtype, q.a_mn, q.b_mn, s.ctas, s.bn);
     g.e = q.e;
+    g.e.vec16 = !part && !q.e.res && q.n % 8 == 0 && q.e.ldo % 8 == 0 && aligned(q.e.out, 16);
     g.part = part;
     g.ldp = up(q.n, 4);
     if (!encode(&g.a, q.a, q.op_dtype, q.a_mn ? 64 : bk, q.a_mn ? bk : kBM)) return LF_ERR_CUDA;
-    if (!encode(&g.b, q.b, q.op_dtype, q.b_mn ? 64 : bk, q.b_mn ? bk : s.bn)) return LF_ERR_CUDA;
-    const int stage = (kBM + s.bn) * kRowBytes;
+    if (!encode(&g.b, q.b, q.op_dtype, q.b_mn ? 64 : bk, q.b_mn ? bk : s.bn / s.ctas)) return LF_ERR_CUDA;
     int rc;
     if (q.op_dtype == LF_F8E4M3)
-        rc = q.dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kLinear, true>>(g, stage, st)
-                               : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kLinear, true>>(g, stage, st);
+        rc = q.dtype == LF_F16 ? launch_ctas<__half, kLinear, true>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, true>(g, s.ctas, st);
     else
-        rc = q.dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kLinear, false>>(g, stage, st)
-                               : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kLinear, false>>(g, stage, st);
+        rc = q.dtype == LF_F16 ? launch_ctas<__half, kLinear, false>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, false>(g, s.ctas, st);
     return rc || !part ? rc : join_splits(q, part, g.splits, st);
 }
 
@@ -1097,46 +1258,51 @@ int check_ffn(const char* what, const lf_gated_ffn_t* a) {
 // Win [2F, C] as two planes of F rows, so that a tile that passes F reads zeros.
 Mat gate_up(Mat w, int64_t f) { return {w.p, w.inner, f, w.ld, 2, f * w.ld}; }
 
-// Hidden columns per tile of the gated kernels by the same estimate as choose().
-int choose_gated(int64_t m, int64_t f, int64_t c, bool bwd) {
-    const int64_t rows = (m + kBM - 1) / kBM, iters = (c + 63) / 64, sms = num_sms();
-    int best = 64;
+// Tile of the gated kernels by the same estimate as choose(); bn counts gate
+// and up columns.  The backward's third product is as wide as one of them.
+Shape choose_gated(int64_t m, int64_t f, int64_t c, bool bwd) {
+    const int64_t iters = (c + 63) / 64, sms = num_sms();
+    Shape best{1, 128, 1};
     double least = 1e30;
-    for (int bh : {128, 64, 32}) {
-        if (bwd && bh != 64) continue;
-        const int64_t waves = (rows * ((f + bh - 1) / bh) + sms - 1) / sms;
-        const double main = (double)iters * std::max(bwd ? 3 * bh : 2 * bh, 128), epi = bh * (bwd ? 40.0 : 20.0);
-        const double t = waves * std::max(main, epi) + std::min(main, epi);
-        if (t < least) least = t, best = bh;
-    }
+    for (int ctas : {2, 1})
+        for (int bh : {128, 64, 32}) {
+            if (bh < (ctas == 2 ? 128 : bwd ? 64 : 32)) continue;
+            const int64_t tiles = (m + kBM * ctas - 1) / (kBM * ctas) * ((f + bh - 1) / bh), waves = (tiles * ctas + sms - 1) / sms;
+            const double first = iters * step_cycles(ctas, 2 * bh, 2 * bh), second = bwd ? iters * step_cycles(ctas, bh, bh) : 0;
+            const double epi = 500 + bh * (bwd ? 40.0 : 20.0);
+            // The backward's epilogue overlaps only the next tile's second product.
+            const double t = bwd ? waves * (first + std::max(second, epi)) + std::min(second, epi)
+                                 : waves * std::max(first, epi) + std::min(first, epi);
+            if (t < least) least = t, best = {ctas, 2 * bh, 1};
+        }
     return best;
 }
 
 int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* dy, const Mat* wout, void* out, int64_t ldo,
               int64_t plane, cudaStream_t st) {
     const bool bwd = dy != nullptr;
-    const int bh = choose_gated(a->m, a->f, a->c, bwd);
+    const Shape s = choose_gated(a->m, a->f, a->c, bwd);
+    const int bh = s.bn / 2;
     GemmArgs g{};
     g.m = (int)a->m, g.n = (int)a->f;
     g.msegs = g.splits = 1;
-    g.tiles_m = (int)((a->m + kBM - 1) / kBM);
+    g.tiles_m = (int)((a->m + kBM * s.ctas - 1) / (kBM * s.ctas));
     g.tiles_n = (int)((a->f + bh - 1) / bh);
     if ((int64_t)g.tiles_m * g.tiles_n > INT32_MAX / 2) return too_large("gated feed-forward block");
     g.iters = g.split_iters = g.seg_iters = (int)((a->c + 63) / 64);
-    g.bn = 2 * bh;
-    g.nbuf = 2;
-    g.idesc = idesc_of(a->dtype, false, false, 2 * bh);
-    g.idesc2 = idesc_of(a->dtype, false, true, bh);
+    g.bn = s.bn;
+    g.stage_bytes = (kBM + s.bn / s.ctas) * kRowBytes;
+    g.idesc = idesc_of(a->dtype, false, false, s.ctas, s.bn);
+    g.idesc2 = idesc_of(a->dtype, false, true, s.ctas, bh);
     g.e.out = out, g.e.ldo = ldo, g.e.bias = a->b_in, g.e.act = a->activation;
     g.plane = plane;
     if (!encode(&g.a, x, a->dtype, 64, kBM) || !encode(&g.b, gate_up(win, a->f), a->dtype, 64, bh)) return LF_ERR_CUDA;
     if (bwd && (!encode(&g.a2, *dy, a->dtype, 64, kBM) || !encode(&g.b2, *wout, a->dtype, 64, 64))) return LF_ERR_CUDA;
-    const int stage = (bwd ? 2 * kBM + 3 * bh : kBM + 2 * bh) * kRowBytes;
     if (bwd)
-        return a->dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kGatedBwd, false>>(g, stage, st)
-                                  : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kGatedBwd, false>>(g, stage, st);
-    return a->dtype == LF_F16 ? launch_gemm<tc_gemm_kernel<__half, kGated, false>>(g, stage, st)
-                              : launch_gemm<tc_gemm_kernel<__nv_bfloat16, kGated, false>>(g, stage, st);
+        return a->dtype == LF_F16 ? launch_ctas<__half, kGatedBwd, false>(g, s.ctas, st)
+                                  : launch_ctas<__nv_bfloat16, kGatedBwd, false>(g, s.ctas, st);
+    return a->dtype == LF_F16 ? launch_ctas<__half, kGated, false>(g, s.ctas, st)
+                              : launch_ctas<__nv_bfloat16, kGated, false>(g, s.ctas, st);
 }
 
 int ffn_fwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
