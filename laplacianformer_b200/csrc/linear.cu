@@ -43,15 +43,45 @@ namespace {
 // ---------------------------------------------------------------------------
 // Activations
 // ---------------------------------------------------------------------------
+// The epilogues are bound by instruction issue where K is short, so the
+// activations are written on the hardware's exponential and reciprocal (about
+// 2 units in the last place each, against results of 11 or 8 bits).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float sigmoid(float z) { return rcp_fast(1.f + exp2_fast(-1.44269504f * z)); }
+
+// Phi(z) and phi(z) of the normal distribution: erfc by Abramowitz and Stegun
+// 7.1.26 (absolute error 1.5e-7), whose exponential is the density's.
+__device__ __forceinline__ float normal_cdf(float z, float& density) {
+    const float x = fabsf(z) * 0.70710678f, t = rcp_fast(__fmaf_rn(0.3275911f, x, 1.f));
+    const float e = exp2_fast(-1.44269504f * x * x);
+    float q = __fmaf_rn(t, 1.061405429f, -1.453152027f);
+    q = __fmaf_rn(t, q, 1.421413741f);
+    q = __fmaf_rn(t, q, -0.284496736f);
+    q = __fmaf_rn(t, q, 0.254829592f) * (t * e) * 0.5f;  // Phi(-|z|)
+    density = e * 0.39894228f;
+    return z >= 0.f ? 1.f - q : q;
+}
+// (1 + tanh(k (z + c z^3))) / 2
+__device__ __forceinline__ float tanh_gate(float z) {
+    return sigmoid(1.59576912f * z * __fmaf_rn(0.044715f * z, z, 1.f));
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
+    float d;
     if constexpr (ACT == LF_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps NaN
-    if constexpr (ACT == LF_ACT_SILU) return z * __fdividef(1.f, 1.f + __expf(-z));
-    if constexpr (ACT == LF_ACT_GELU) return z * (0.5f + 0.5f * erff(z * 0.70710678118654752f));
-    if constexpr (ACT == LF_ACT_GELU_TANH) {
-        const float t = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-        return z * (1.f - __fdividef(1.f, 1.f + __expf(2.f * t)));  // (1 + tanh t)/2
-    }
+    if constexpr (ACT == LF_ACT_SILU) return z * sigmoid(z);
+    if constexpr (ACT == LF_ACT_GELU) return z * normal_cdf(z, d);
+    if constexpr (ACT == LF_ACT_GELU_TANH) return z * tanh_gate(z);
     return z;
 }
 
@@ -62,18 +92,18 @@ __device__ __forceinline__ void act_both(float z, float& a, float& slope) {
         a = z < 0.f ? 0.f : z;
         slope = z > 0.f ? 1.f : 0.f;
     } else if constexpr (ACT == LF_ACT_SILU) {
-        const float p = __fdividef(1.f, 1.f + __expf(-z));
+        const float p = sigmoid(z);
         a = z * p;
-        slope = p * (1.f + z * (1.f - p));
+        slope = __fmaf_rn(a, 1.f - p, p);
     } else if constexpr (ACT == LF_ACT_GELU) {
-        const float p = 0.5f + 0.5f * erff(z * 0.70710678118654752f);
+        float d;
+        const float p = normal_cdf(z, d);
         a = z * p;
-        slope = p + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+        slope = __fmaf_rn(z, d, p);
     } else if constexpr (ACT == LF_ACT_GELU_TANH) {
-        const float k = 0.79788456080286536f, c = 0.044715f;
-        const float q = 1.f - __fdividef(1.f, 1.f + __expf(2.f * k * (z + c * z * z * z)));  // (1 + tanh)/2
-        a = z * q;
-        slope = q + 2.f * z * q * (1.f - q) * k * (1.f + 3.f * c * z * z);
+        const float p = tanh_gate(z);
+        a = z * p;
+        slope = __fmaf_rn(a * (1.f - p), __fmaf_rn(0.214077774f * z, z, 1.59576912f), p);
     } else {
         a = z;
         slope = 1.f;
@@ -221,10 +251,13 @@ __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint
 __device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+// Tells the leader that this warp has read its accumulators (the tensor-memory
+// loads are done; nothing else is ordered, so stores in flight do not hold the
+// next products back).
 template <int CTAS>
 __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
     if constexpr (CTAS == 2)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
     else
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -352,14 +385,15 @@ __device__ __forceinline__ float column_value(const T* p, int col, int n) {
 // kGated: B's tile is bn/2 gate and bn/2 up rows of Win, the accumulator's
 // halves are g and u of the same hidden columns.
 // kGatedBwd: first dh = dy Wout (accumulators at 256 or 384, in turn), then
-// [g|u] = x Win^T at 0: while the epilogue reads a tile, the next tile's dh is
-// computed.
+// [g|u] = x Win^T at 0.  The epilogue takes all of a tile's g and u into
+// registers at once, while the next tile's dh is computed, so that neither
+// product waits for outputs.
 template <typename T, int MODE, bool FP8, int CTAS>
 __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];  // stages, output staging, barriers
     uint8_t* out_stage = smem + p.stages * p.stage_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * kStageOut);
-    uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *drain = tempty + 2;
+    uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *dempty = tempty + 2, *drain = dempty + 2;
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0;
@@ -372,7 +406,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps * CTAS);
+        for (int i = 0; i < 2; ++i)
+            mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps * CTAS), mbar_init(&dempty[i], kEpiWarps * CTAS);
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -442,16 +477,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
             const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
             int s = 0, buf = 0;
-            uint32_t ph = 0, bph = 0;
+            uint32_t ph = 0, bph = 0, dph = 0;
             for (int unit = unit0; ok && unit < units; unit += unit_step) {
                 const Tile t = tile_of<CTAS>(p, unit, bn_out, 0);
                 for (int phase = 0; ok && phase < phases; ++phase) {
                     const bool dh = MODE == kGatedBwd && phase == 0;
-                    // dh goes where the epilogue two tiles ago read, which had to end before the last tile's g and u.
-                    if (!dh) {
-                        if (!(ok = mbar_wait(&tempty[MODE == kGatedBwd ? 0 : buf], bph ^ 1))) break;
-                        tc_fence_after();
-                    }
+                    // Each accumulator's last reader: the previous tile for g and u, two tiles ago for the others.
+                    if (dh) ok = mbar_wait(&dempty[buf], dph ^ 1);
+                    else ok = mbar_wait(&tempty[MODE == kGatedBwd ? 0 : buf], bph ^ 1);
+                    if (!ok) break;
+                    tc_fence_after();
                     const uint32_t acc = tmem + (MODE != kGatedBwd ? buf * 256 : dh ? kDh + buf * 128 : 0);
                     for (int it = t.it0; it < t.it1; ++it) {
                         if (!(ok = mbar_wait(&full[s], ph))) break;
@@ -475,6 +510,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 if (!ok) break;
                 if (go) commit<CTAS>(&tfull[MODE == kGatedBwd ? 0 : buf]);
                 buf ^= 1;
+                if (buf == 0) dph ^= 1;
                 if (MODE == kGatedBwd || buf == 0) bph ^= 1;
             }
             if (!ok) {  // products in flight end before the tensor memory is freed
@@ -495,6 +531,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             const int64_t row0 = (int64_t)t.seg * p.m + t.m0 + quad * 32;      // in the output
             const int cend = min(bn_out, p.n - t.n0);
             uint64_t* tf = &tfull[MODE == kGatedBwd ? 0 : buf];
+            const int last = half * 32 + (cend - half * 32 - 1) / 64 * 64;     // this warp's last 32 columns (if it has any)
+            auto release = [&](uint64_t* bar) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader<CTAS>(bar);
+            };
+            if (half * 32 >= cend) {                                           // none: wait for the tile all the same
+                if (!(ok = mbar_wait(tf, bph))) break;
+                tc_fence_after();
+                release(&tempty[MODE == kGatedBwd ? 0 : buf]);
+                if (MODE == kGatedBwd) release(&dempty[buf]);
+            } else
             if constexpr (MODE == kLinear) {
                 const uint32_t acc = tmem + buf * 256 + lanes;
                 const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
@@ -520,6 +568,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         }
                         tmem_wait_ld();
                         reg_fence(v);
+                        if (c0 == last) release(&tempty[buf]);
                         if (FP8) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(v[j], sa * cv[32 + j], cv[j]);
@@ -570,6 +619,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         tmem_ld32(acc + c0, v);
                         tmem_wait_ld();
                         reg_fence(v);
+                        if (c0 == last) release(&tempty[buf]);
                         if (FP8) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] *= sa;
@@ -609,44 +659,61 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             } else {
                 const T* bias = (const T*)e.bias;
                 const uint32_t acc = tmem + (MODE == kGated ? buf * 256 : 0) + lanes;
-                const uint32_t acc_dh = tmem + kDh + buf * 128 + lanes;
                 T* out = (T*)e.out + row0 * e.ldo;
                 float* cv = reinterpret_cast<float*>(st + 2048);
                 float bg = column_value(bias, t.n0 + half * 32 + lane, p.n);
                 float bu = column_value(bias ? bias + p.n : bias, t.n0 + half * 32 + lane, p.n);
                 if (!(ok = mbar_wait(tf, bph))) break;
                 tc_fence_after();
-                for (int c0 = half * 32; c0 < cend; c0 += 64) {
-                    const int col0 = t.n0 + c0;
-                    float g[32], u[32];
-                    tmem_ld32(acc + c0, g);
-                    tmem_ld32(acc + bh + c0, u);
-                    if (bias) {
-                        cv[lane] = bg, cv[32 + lane] = bu;
-                        bg = column_value(bias, col0 + 64 + lane, p.n);
-                        bu = column_value(bias + p.n, col0 + 64 + lane, p.n);
-                        __syncwarp();
-                    }
-                    tmem_wait_ld();
-                    reg_fence(g);
-                    reg_fence(u);
-                    if (bias) {
+                auto add_bias = [&](float(&g)[32], float(&u)[32], int next) {
+                    if (!bias) return;
+                    cv[lane] = bg, cv[32 + lane] = bu;
+                    bg = column_value(bias, next + lane, p.n);
+                    bu = column_value(bias + p.n, next + lane, p.n);
+                    __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) g[j] += cv[j], u[j] += cv[32 + j];
-                        __syncwarp();
-                    }
-                    if constexpr (MODE == kGated) {
+                    for (int j = 0; j < 32; ++j) g[j] += cv[j], u[j] += cv[32 + j];
+                    __syncwarp();
+                };
+                if constexpr (MODE == kGated) {
+                    for (int c0 = half * 32; c0 < cend; c0 += 64) {
+                        float g[32], u[32];
+                        tmem_ld32(acc + c0, g);
+                        tmem_ld32(acc + bh + c0, u);
+                        tmem_wait_ld();
+                        reg_fence(g);
+                        reg_fence(u);
+                        if (c0 == last) release(&tempty[buf]);
+                        add_bias(g, u, t.n0 + c0 + 64);
                         with_act(e.act, [&](auto act) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
                         });
                         stage16<T>(st, lane, u);
                         __syncwarp();
-                        unstage16(st, lane, out, e.ldo, rows, col0);
+                        unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
                         __syncwarp();
-                    } else {
+                    }
+                } else {
+                    const uint32_t acc_dh = tmem + kDh + buf * 128 + lanes;
+                    float g0[32], u0[32], g1[32], u1[32];
+                    const int c0 = half * 32, c1 = c0 + 64;
+                    tmem_ld32(acc + c0, g0);
+                    tmem_ld32(acc + bh + c0, u0);
+                    if (last == c1) {
+                        tmem_ld32(acc + c1, g1);
+                        tmem_ld32(acc + bh + c1, u1);
+                    }
+                    tmem_wait_ld();
+                    reg_fence(g0);
+                    reg_fence(u0);
+                    reg_fence(g1);
+                    reg_fence(u1);
+                    release(&tempty[0]);
+                    // g and u become what dh is multiplied by: g = act(g), u = u act'(g); h goes out first.
+                    auto chunk = [&](float(&g)[32], float(&u)[32], int c) {
                         float d[32];
-                        // g and u become what dh is multiplied by: g = act(g), u = u act'(g); h goes out first.
+                        add_bias(g, u, t.n0 + c + 64);
                         with_act(e.act, [&](auto act) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
@@ -658,26 +725,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                             }
                         });
                         stage16<T>(st, lane, d);
-                        tmem_ld32(acc_dh + c0, d);
+                        tmem_ld32(acc_dh + c, d);
                         __syncwarp();
-                        unstage16(st, lane, out + 2 * p.plane, e.ldo, rows, col0);
+                        unstage16(st, lane, out + 2 * p.plane, e.ldo, rows, t.n0 + c);
                         tmem_wait_ld();
                         reg_fence(d);
+                        if (c == last) release(&dempty[buf]);
                         __syncwarp();
 #pragma unroll
                         for (int j = 0; j < 32; ++j) u[j] *= d[j], g[j] *= d[j];
                         stage16<T>(st, lane, u);
                         stage16<T>(st + 2048, lane, g);
                         __syncwarp();
-                        unstage16(st, lane, out, e.ldo, rows, col0);
-                        unstage16(st + 2048, lane, out + p.plane, e.ldo, rows, col0);
+                        unstage16(st, lane, out, e.ldo, rows, t.n0 + c);
+                        unstage16(st + 2048, lane, out + p.plane, e.ldo, rows, t.n0 + c);
                         __syncwarp();
-                    }
+                    };
+                    chunk(g0, u0, c0);
+                    if (last == c1) chunk(g1, u1, c1);
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_leader<CTAS>(&tempty[MODE == kGatedBwd ? 0 : buf]);
             buf ^= 1;
             if (MODE == kGatedBwd || buf == 0) bph ^= 1;
         }
@@ -904,8 +971,15 @@ bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_ro
         set_error("cuTensorMapEncodeTiled is not available");
         return false;
     }
-    const CUresult r = fn(map, ty, 3, const_cast<void*>(a.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto call = [&] {
+        return fn(map, ty, 3, const_cast<void*>(a.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = call();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {  // the first call of a host thread (an autograd worker): bind the device's context
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = call();
+    }
     if (r != CUDA_SUCCESS) set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
     return r == CUDA_SUCCESS;
 }

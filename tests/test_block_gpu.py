@@ -491,6 +491,23 @@ def test_other_stream_and_determinism():
     assert capi.device_status() == 0
 
 
+def test_first_call_of_a_host_thread():
+    """A thread that has made no CUDA call yet has no current context; its memory comes from the allocator's cache."""
+    import threading
+
+    g = gen("thread")
+    x, w = rand(g, torch.bfloat16, 200, 64), rand(g, torch.bfloat16, 64, 64, scale=0.1)
+    want = ops.linear(x, w)
+    spare = [torch.empty_like(want) for _ in range(4)]
+    torch.cuda.synchronize()
+    del spare
+    got = []
+    t = threading.Thread(target=lambda: got.append(ops.linear(x, w)))
+    t.start()
+    t.join()
+    assert got and torch.equal(got[0], want)
+
+
 def test_runs_in_a_cuda_graph():
     g = gen("graph")
     x, w = rand(g, torch.bfloat16, 200, 64), rand(g, torch.bfloat16, 64, 64, scale=0.1)
