@@ -204,14 +204,27 @@ enum Mode { kLinear, kGated, kGatedBwd };
 
 constexpr int kBM = 128;                  // rows of a tile per CTA
 constexpr int kRowBytes = 128;            // a stage holds 128 bytes of K: 64 16-bit or 128 8-bit elements
-constexpr int kEpiWarps = 8;              // two per 32-lane quarter of the tensor memory
-constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
-constexpr int kStageOut = 4096;           // output staging per epilogue warp
+constexpr int kEpiWarps = 16;             // four per 32-lane quarter of the tensor memory
+constexpr int kControlWarps = 3;          // copies of A, products, copies of B
+constexpr int kGemmThreads = 32 * (kControlWarps + kEpiWarps);
+constexpr int kStageOut = 2048;           // output staging per epilogue warp: 32 rows of 64 bytes
+constexpr int kEpiCols = kEpiWarps / 4 * 32;  // columns that the epilogue warps read at a time
 constexpr int kMaxStages = 8;
 constexpr int kTmemAll = 512;
 constexpr int kBarrierBytes = 256;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kGroupRows = 2048;          // rows that are walked together, so that their operands stay in L2
+
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery 1994).
+struct Divisor {
+    uint32_t d, mul, shift;
+    Divisor() = default;
+    explicit Divisor(uint32_t v) : d(v), shift(0) {
+        while ((1u << shift) < d) ++shift;
+        mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
 
 struct alignas(64) GemmArgs {
     CUtensorMap a, b, a2, b2;  // a2, b2: dy and Wout of the gated backward
@@ -220,6 +233,7 @@ struct alignas(64) GemmArgs {
     int64_t ldp, plane;        // plane: elements between dg, du and h (gated backward)
     int m, n;                  // rows of one row segment; output columns (hidden columns of the gated modes)
     int msegs, tiles_m, tiles_n, splits;
+    Divisor per_split, per_group, per_seg, group_rows, last_rows;  // tiles; row tiles of a whole and of the last group
     int iters, split_iters, seg_iters;  // K steps in all, per split, per K segment
     int bn, stages, stage_bytes;        // columns of a tile's (first) product; ring depth
     uint32_t idesc, idesc2;
@@ -325,49 +339,65 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 struct Tile {
     int seg, m0, n0, split, it0, it1;
 };
+// Order of the gated backward's 2 n steps: kLead steps of dh, while the
+// epilogue still reads the last tile's g and u, then g|u and dh in turn (dh
+// alone would fetch 96 bytes per cycle and SM), then what is left of g|u.
+constexpr int kLead = 4;
+struct Step {
+    bool dh;
+    int it;
+};
+__device__ __forceinline__ Step gated_step(int i, int n) {
+    const int lead = min(kLead, n), j = i - lead, both = 2 * (n - lead);
+    if (j < 0) return {true, i};
+    if (j < both) return {(j & 1) != 0, (j & 1) ? lead + (j >> 1) : j >> 1};
+    return {false, n - lead + (j - both)};
+}
 // Work units: for each split of K, row tiles in groups of kGroupRows, within a
 // group all row tiles of one column tile before the next column tile.
 template <int CTAS>
 __device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out, int rank) {
-    constexpr int kGroup = kGroupRows / (kBM * CTAS);
-    const int rows = p.msegs * p.tiles_m, tiles = rows * p.tiles_n;
     Tile t;
-    t.split = unit / tiles;
-    int r = unit - t.split * tiles;
-    const int group = r / (kGroup * p.tiles_n), first = group * kGroup;
-    const int gm = min(kGroup, rows - first);
-    r -= group * kGroup * p.tiles_n;
-    const int ni = r / gm, mi = first + r - ni * gm;
+    t.split = p.per_split.of(unit);
+    int r = unit - t.split * (int)p.per_split.d;
+    const int group = p.per_group.of(r);
+    r -= group * (int)p.per_group.d;
+    const bool whole = (group + 1) * (int)p.group_rows.d <= p.msegs * p.tiles_m;
+    const Divisor& gm = whole ? p.group_rows : p.last_rows;
+    const int ni = gm.of(r), mi = group * (int)p.group_rows.d + r - ni * (int)gm.d;
     t.n0 = ni * bn_out;
-    t.seg = mi / p.tiles_m;
+    t.seg = p.per_seg.of(mi);
     t.m0 = ((mi - t.seg * p.tiles_m) * CTAS + rank) * kBM;
     t.it0 = t.split * p.split_iters;
     t.it1 = min(p.iters, t.it0 + p.split_iters);
     return t;
 }
 
-// 32 rows x 32 16-bit columns of one warp, staged in shared memory (64-byte
-// rows, 16-byte chunks swizzled so that neither side has bank conflicts) and
-// written as 64-byte row segments.  v: the calling lane's row.
+// Staging of one warp: 32 rows of 64 bytes in shared memory whose 16-byte
+// chunks are swizzled so that neither a lane per row nor four lanes per row
+// meet bank conflicts.
+__device__ __forceinline__ uint8_t* stage_at(uint8_t* st, int row, int chunk) {
+    return st + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+// 32 16-bit columns: the calling lane's row in, 64-byte row segments out.
 template <typename T>
 __device__ __forceinline__ void stage16(uint8_t* st, int lane, const float (&v)[32]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const uint4 u = make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
-                                   pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
-        *reinterpret_cast<uint4*>(st + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = u;
-    }
+    for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(stage_at(st, lane, c)) =
+            make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
+                       pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
 }
 // out: row 0 of the warp's rows, of which `rows` exist; ld and col0 are multiples of 8.
 template <typename T>
-__device__ __forceinline__ void unstage16(const uint8_t* st, int lane, T* out, int64_t ld, int rows, int col0) {
+__device__ __forceinline__ void unstage16(uint8_t* st, int lane, T* out, int64_t ld, int rows, int col0) {
     const int c = lane & 3;
     if (col0 + c * 8 >= ld) return;
     T* o = out + (lane >> 2) * ld + col0 + c * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i, o += 8 * ld) {
         const int row = i * 8 + (lane >> 2);
-        if (row < rows) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(st + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+        if (row < rows) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(stage_at(st, row, c));
     }
 }
 
@@ -405,7 +435,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     const int phases = MODE == kGatedBwd ? 2 : 1;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 2), mbar_init(&empty[i], 1);
         for (int i = 0; i < 2; ++i)
             mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps * CTAS), mbar_init(&dempty[i], kEpiWarps * CTAS);
         mbar_init(drain, 1);
@@ -421,47 +451,46 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     const int unit0 = blockIdx.x / CTAS, unit_step = gridDim.x / CTAS;
     bool ok = true;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {
+        // One warp copies A, the other B: a copy takes its issuer a few
+        // hundred cycles, and one warp for both could not feed the products.
+        const bool is_a = warp == 0;
         if (elect_one()) {
             int s = 0, issued = 0;
             uint32_t ph = 0;
             const int bw = p.bn / CTAS;                        // B rows that this CTA holds
+            const uint32_t bars = CTAS == 2 ? leader_addr(full) : smem_u32(full);
             for (int unit = unit0; ok && unit < units; unit += unit_step) {
                 const Tile t = tile_of<CTAS>(p, unit, bn_out, rank);
-                for (int phase = 0; ok && phase < phases; ++phase) {
-                    const bool dh = MODE == kGatedBwd && phase == 0;
-                    const uint32_t bytes = kABytes + (dh ? bh / CTAS : bw) * kRowBytes;
-                    for (int it = t.it0; it < t.it1; ++it) {
-                        if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
-                        const int ks = it / p.seg_iters, k0 = (it - ks * p.seg_iters) * BK;
-                        uint8_t* sa = smem + s * p.stage_bytes;
-                        uint8_t* sb = sa + kABytes;
-                        const uint32_t bar = CTAS == 2 ? leader_addr(&full[s]) : smem_u32(&full[s]);
-                        if (rank == 0) mbar_expect(&full[s], bytes * CTAS);
-                        if (dh) {
-                            tma_load<CTAS>(sa, &p.a2, bar, k0, t.m0, 0);
-                            for (int j = 0; j < bh / CTAS / 64; ++j)
-                                tma_load<CTAS>(sb + j * 8192, &p.b2, bar, t.n0 + rank * (bh / CTAS) + 64 * j, k0, 0);
-                        } else {
-                            if (!p.a_mn) tma_load<CTAS>(sa, &p.a, bar, k0, t.m0, ks);
-                            else
-                                for (int j = 0; j < kBM / 64; ++j)
-                                    tma_load<CTAS>(sa + j * 8192, &p.a, bar, t.m0 + 64 * j, k0, t.seg);
-                            if (MODE == kLinear) {
-                                if (!p.b_mn) tma_load<CTAS>(sb, &p.b, bar, k0, t.n0 + rank * bw, ks);
-                                else
-                                    for (int j = 0; j < bw / 64; ++j)
-                                        tma_load<CTAS>(sb + j * 8192, &p.b, bar, t.n0 + rank * bw + 64 * j, k0, ks);
-                            } else if (CTAS == 2) {            // one CTA the gate rows, the other the up rows
-                                tma_load<CTAS>(sb, &p.b, bar, k0, t.n0, rank);
-                            } else {
-                                tma_load<CTAS>(sb, &p.b, bar, k0, t.n0, 0);
-                                tma_load<CTAS>(sb + bh * kRowBytes, &p.b, bar, k0, t.n0, 1);
-                            }
-                        }
-                        ++issued;
-                        if (++s == p.stages) s = 0, ph ^= 1;
+                const int steps = (t.it1 - t.it0) * phases;
+                int ks = t.it0 / p.seg_iters, in_seg = t.it0 - ks * p.seg_iters;
+                for (int i = 0; i < steps; ++i) {
+                    if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
+                    const Step step = MODE == kGatedBwd ? gated_step(i, steps / 2) : Step{false, i};
+                    const int k0 = (MODE == kLinear ? in_seg : step.it) * BK;
+                    uint8_t* dst = smem + s * p.stage_bytes + (is_a ? 0 : kABytes);
+                    const uint32_t bar = bars + 8 * s;
+                    if (rank == 0) mbar_expect(&full[s], (is_a ? kABytes : (step.dh ? bh / CTAS : bw) * kRowBytes) * CTAS);
+                    if (is_a) {
+                        if (step.dh) tma_load<CTAS>(dst, &p.a2, bar, k0, t.m0, 0);
+                        else if (!p.a_mn) tma_load<CTAS>(dst, &p.a, bar, k0, t.m0, ks);
+                        else
+                            for (int j = 0; j < kBM / 64; ++j) tma_load<CTAS>(dst + j * 8192, &p.a, bar, t.m0 + 64 * j, k0, t.seg);
+                    } else if (step.dh) {
+                        for (int j = 0; j < bh / CTAS / 64; ++j)
+                            tma_load<CTAS>(dst + j * 8192, &p.b2, bar, t.n0 + rank * (bh / CTAS) + 64 * j, k0, 0);
+                    } else if (MODE != kLinear) {
+                        if (CTAS == 2) tma_load<CTAS>(dst, &p.b, bar, k0, t.n0, rank);  // one CTA the gate rows, the other the up rows
+                        else
+                            for (int j = 0; j < 2; ++j) tma_load<CTAS>(dst + j * bh * kRowBytes, &p.b, bar, k0, t.n0, j);
+                    } else if (!p.b_mn) {
+                        tma_load<CTAS>(dst, &p.b, bar, k0, t.n0 + rank * bw, ks);
+                    } else {
+                        for (int j = 0; j < bw / 64; ++j) tma_load<CTAS>(dst + j * 8192, &p.b, bar, t.n0 + rank * bw + 64 * j, k0, ks);
                     }
+                    ++issued;
+                    if (MODE == kLinear && ++in_seg == p.seg_iters) in_seg = 0, ++ks;
+                    if (++s == p.stages) s = 0, ph ^= 1;
                 }
             }
             // A wait ran out: let the copies in flight land before the block
@@ -480,32 +509,34 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             uint32_t ph = 0, bph = 0, dph = 0;
             for (int unit = unit0; ok && unit < units; unit += unit_step) {
                 const Tile t = tile_of<CTAS>(p, unit, bn_out, 0);
-                for (int phase = 0; ok && phase < phases; ++phase) {
-                    const bool dh = MODE == kGatedBwd && phase == 0;
-                    // Each accumulator's last reader: the previous tile for g and u, two tiles ago for the others.
-                    if (dh) ok = mbar_wait(&dempty[buf], dph ^ 1);
-                    else ok = mbar_wait(&tempty[MODE == kGatedBwd ? 0 : buf], bph ^ 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t acc = tmem + (MODE != kGatedBwd ? buf * 256 : dh ? kDh + buf * 128 : 0);
-                    for (int it = t.it0; it < t.it1; ++it) {
-                        if (!(ok = mbar_wait(&full[s], ph))) break;
+                const int steps = (t.it1 - t.it0) * phases;
+                for (int i = 0; i < steps; ++i) {
+                    const Step step = MODE == kGatedBwd ? gated_step(i, steps / 2) : Step{false, i};
+                    const bool dh = step.dh;
+                    if (step.it == 0) {
+                        // Each accumulator's last reader: the previous tile for g and u, two tiles ago for the others.
+                        if (dh) ok = mbar_wait(&dempty[buf], dph ^ 1);
+                        else ok = mbar_wait(&tempty[MODE == kGatedBwd ? 0 : buf], bph ^ 1);
+                        if (!ok) break;
                         tc_fence_after();
-                        const uint32_t sa = smem_u32(smem + s * p.stage_bytes), sb = sa + kABytes;
-                        if (dh) {
-                            const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sb, 8192, 1024);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                mma<CTAS, FP8>(acc, da + k * 2, db + k * 128, p.idesc2, it > t.it0 || k > 0 ? 1u : 0u, go);
-                        } else {
-                            const uint64_t da = make_desc(sa, a_lbo, 1024), db = make_desc(sb, b_lbo, 1024);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                mma<CTAS, FP8>(acc, da + k * a_step, db + k * b_step, p.idesc, it > t.it0 || k > 0 ? 1u : 0u, go);
-                        }
-                        if (go) commit<CTAS>(&empty[s]);
-                        if (++s == p.stages) s = 0, ph ^= 1;
                     }
+                    const uint32_t acc = tmem + (MODE != kGatedBwd ? buf * 256 : dh ? kDh + buf * 128 : 0);
+                    if (!(ok = mbar_wait(&full[s], ph))) break;
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + s * p.stage_bytes), sb = sa + kABytes;
+                    if (dh) {
+                        const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sb, 8192, 1024);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma<CTAS, FP8>(acc, da + k * 2, db + k * 128, p.idesc2, step.it > 0 || k > 0 ? 1u : 0u, go);
+                    } else {
+                        const uint64_t da = make_desc(sa, a_lbo, 1024), db = make_desc(sb, b_lbo, 1024);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma<CTAS, FP8>(acc, da + k * a_step, db + k * b_step, p.idesc, step.it > 0 || k > 0 ? 1u : 0u, go);
+                    }
+                    if (go) commit<CTAS>(&empty[s]);
+                    if (++s == p.stages) s = 0, ph ^= 1;
                 }
                 if (!ok) break;
                 if (go) commit<CTAS>(&tfull[MODE == kGatedBwd ? 0 : buf]);
@@ -519,7 +550,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             }
         }
     } else {
-        const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+        const int ew = warp - kControlWarps, quad = warp & 3, cg = ew >> 2;  // lanes of the tensor memory, columns of a tile
         uint8_t* st = out_stage + ew * kStageOut;
         int buf = 0;
         uint32_t bph = 0;
@@ -531,13 +562,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             const int64_t row0 = (int64_t)t.seg * p.m + t.m0 + quad * 32;      // in the output
             const int cend = min(bn_out, p.n - t.n0);
             uint64_t* tf = &tfull[MODE == kGatedBwd ? 0 : buf];
-            const int last = half * 32 + (cend - half * 32 - 1) / 64 * 64;     // this warp's last 32 columns (if it has any)
+            const int last = cg * 32 + (cend - cg * 32 - 1) / kEpiCols * kEpiCols;  // this warp's last 32 columns (if it has any)
             auto release = [&](uint64_t* bar) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_leader<CTAS>(bar);
             };
-            if (half * 32 >= cend) {                                           // none: wait for the tile all the same
+            if (cg * 32 >= cend) {                                           // none: wait for the tile all the same
                 if (!(ok = mbar_wait(tf, bph))) break;
                 tc_fence_after();
                 release(&tempty[MODE == kGatedBwd ? 0 : buf]);
@@ -546,24 +577,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             if constexpr (MODE == kLinear) {
                 const uint32_t acc = tmem + buf * 256 + lanes;
                 const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
+                const int first = cg * 32;
+                float* cv = reinterpret_cast<float*>(st);
                 if (e.vec16) {
-                    // Whole 16-byte chunks and no residual: finished in the
-                    // accumulator's layout (a lane owns a row), column
-                    // values of the next 32 columns fetched ahead.
-                    float* cv = reinterpret_cast<float*>(st + 2048);
-                    float bias = column_value((const T*)e.bias, t.n0 + half * 32 + lane, p.n);
-                    float sb = FP8 && t.n0 + half * 32 + lane < p.n ? e.sb[t.n0 + half * 32 + lane] : 1.f;
+                    // Whole 16-byte chunks: finished in the accumulator's
+                    // layout (a lane owns a row); column values and the
+                    // residual of the next columns are fetched ahead.
+                    float bias, sb = 1.f;
+                    uint4 r[4];
+                    auto fetch = [&](int c0) {
+                        const int col = t.n0 + c0 + lane, col8 = t.n0 + c0 + (lane & 3) * 8;
+                        bias = column_value((const T*)e.bias, col, p.n);
+                        if (FP8) sb = col < p.n ? e.sb[col] : 1.f;
+                        if (!e.res) return;
+                        const T* q = (const T*)e.res + (row0 + (lane >> 2)) * e.ldr + col8;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i, q += 8 * e.ldr)
+                            r[i] = i * 8 + (lane >> 2) < rows && col8 < p.n ? *reinterpret_cast<const uint4*>(q) : make_uint4(0u, 0u, 0u, 0u);
+                    };
+                    fetch(first);
                     if (!(ok = mbar_wait(tf, bph))) break;
                     tc_fence_after();
-                    for (int c0 = half * 32; c0 < cend; c0 += 64) {
+                    for (int c0 = first; c0 < cend; c0 += kEpiCols) {
                         float v[32];
                         tmem_ld32(acc + c0, v);
                         if (FP8 || e.bias) {
                             cv[lane] = bias;
                             if (FP8) cv[32 + lane] = sb;
-                            const int next = t.n0 + c0 + 64 + lane;
-                            bias = column_value((const T*)e.bias, next, p.n);
-                            if (FP8) sb = next < p.n ? e.sb[next] : 1.f;
                             __syncwarp();
                         }
                         tmem_wait_ld();
@@ -576,174 +616,173 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] += cv[j];
                         }
+                        if (e.res) {  // to the lane that owns the row
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
+                            __syncwarp();
+                        }
                         if (e.act != LF_ACT_NONE)
                             with_act(e.act, [&](auto act) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(act)::value>(v[j]);
+                                for (int j = 0; j < 32; ++j) {
+                                    float a, slope;
+                                    if (e.act_bwd) act_both<decltype(act)::value>(v[j], a, slope);
+                                    else slope = act_value<decltype(act)::value>(v[j]);
+                                    v[j] = slope;
+                                }
                             });
+                        if (e.res) {  // added to the activation, or dy times its derivative
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                const uint4 u = *reinterpret_cast<const uint4*>(stage_at(st, lane, c));
+                                const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+                                for (int h = 0; h < 4; ++h) {
+                                    const float2 x = unpack2<T>(w[h]);
+                                    float &y0 = v[8 * c + 2 * h], &y1 = v[8 * c + 2 * h + 1];
+                                    y0 = e.act_bwd ? y0 * x.x : y0 + x.x;
+                                    y1 = e.act_bwd ? y1 * x.y : y1 + x.y;
+                                }
+                            }
+                        }
+                        __syncwarp();
                         stage16<T>(st, lane, v);
+                        fetch(c0 + kEpiCols);
                         __syncwarp();
                         unstage16(st, lane, (T*)e.out + row0 * e.ldo, e.ldo, rows, t.n0 + c0);
                         __syncwarp();
                     }
                 } else {
-                    // Raw sums through shared memory, so that a lane has four
-                    // columns of eight rows and residual, bias and output are
-                    // row segments; the next 32 columns' residual and bias
-                    // are fetched ahead.
-                    uint2 r[8];
-                    float4 b, sb;
-                    auto fetch = [&](int c0) {
-                        const int col = t.n0 + c0 + (lane & 7) * 4;
-                        if (c0 >= cend || p.part) return;
-                        if (e.res) {
-                            const T* q = (const T*)e.res + (row0 + (lane >> 3)) * e.ldr;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i, q += 4 * e.ldr)
-                                r[i] = i * 4 + (lane >> 3) < rows ? load4(q, col, p.n, e.vec_res) : make_uint2(0u, 0u);
-                        }
-                        if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, p.n, false));
-                        if (FP8) {
-                            float* q = reinterpret_cast<float*>(&sb);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) q[j] = col + j < p.n ? e.sb[col + j] : 0.f;
-                        }
-                    };
-                    b = sb = make_float4(0.f, 0.f, 0.f, 0.f);
-                    fetch(half * 32);
+                    // Any alignment, and split-K partials: raw sums through
+                    // shared memory, 16 columns at a time, so that a lane has
+                    // four columns of four rows.
                     if (!(ok = mbar_wait(tf, bph))) break;
                     tc_fence_after();
-                    for (int c0 = half * 32; c0 < cend; c0 += 64) {
-                        const int col = t.n0 + c0 + (lane & 7) * 4;
-                        float v[32];
-                        tmem_ld32(acc + c0, v);
-                        tmem_wait_ld();
-                        reg_fence(v);
-                        if (c0 == last) release(&tempty[buf]);
-                        if (FP8) {
+                    for (int c0 = first; c0 < cend; c0 += kEpiCols) {
+#pragma unroll 1
+                        for (int h = 0; h < 2; ++h) {
+                            const int col = t.n0 + c0 + h * 16 + (lane & 3) * 4;
+                            float v[16];
+                            tmem_ld16(acc + c0 + h * 16, v);
+                            tmem_wait_ld();
+                            reg_fence(v);
+                            if (c0 == last && h == 1) release(&tempty[buf]);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] *= sa;
+                            for (int c = 0; c < 4; ++c)
+                                *reinterpret_cast<float4*>(stage_at(st, lane, c)) =
+                                    make_float4(v[4 * c] * sa, v[4 * c + 1] * sa, v[4 * c + 2] * sa, v[4 * c + 3] * sa);
+                            __syncwarp();
+                            const int row = lane >> 2;
+                            if (p.part) {
+                                float* q = p.part + ((int64_t)t.split * p.msegs * p.m + row0 + row) * p.ldp + col;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i, q += 8 * p.ldp)
+                                    if (i * 8 + row < rows && col < p.ldp)
+                                        *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(stage_at(st, i * 8 + row, lane & 3));
+                            } else {
+                                uint2 r[4];
+                                float4 b = make_float4(0.f, 0.f, 0.f, 0.f), sb = b;
+                                if (e.res) {
+                                    const T* q = (const T*)e.res + (row0 + row) * e.ldr;
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i, q += 8 * e.ldr)
+                                        r[i] = i * 8 + row < rows ? load4(q, col, p.n, e.vec_res) : make_uint2(0u, 0u);
+                                }
+                                if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, p.n, false));
+                                if (FP8) {
+                                    float* q = reinterpret_cast<float*>(&sb);
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) q[j] = col + j < p.n ? e.sb[col + j] : 0.f;
+                                }
+                                T* out = (T*)e.out + (row0 + row) * e.ldo;
+                                with_act(e.act, [&](auto act) {
+                                    T* q = out;
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i, q += 8 * e.ldo)
+                                        if (i * 8 + row < rows) {
+                                            float4 z = *reinterpret_cast<const float4*>(stage_at(st, i * 8 + row, lane & 3));
+                                            if (FP8) z.x *= sb.x, z.y *= sb.y, z.z *= sb.z, z.w *= sb.w;
+                                            const float4 x = e.res ? widen4<T>(r[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                            store4(q, col, p.n, e.vec_out, finish4<decltype(act)::value>(z, b, x, e.act_bwd));
+                                        }
+                                });
+                            }
+                            __syncwarp();
                         }
-#pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                                make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                        __syncwarp();
-                        auto staged = [&](int i) {
-                            const int row = i * 4 + (lane >> 3);
-                            return *reinterpret_cast<const float4*>(st + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
-                        };
-                        if (p.part) {
-                            float* q = p.part + ((int64_t)t.split * p.msegs * p.m + row0 + (lane >> 3)) * p.ldp + col;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i, q += 4 * p.ldp)
-                                if (i * 4 + (lane >> 3) < rows && col < p.ldp) *reinterpret_cast<float4*>(q) = staged(i);
-                        } else {
-                            T* out = (T*)e.out + (row0 + (lane >> 3)) * e.ldo;
-                            with_act(e.act, [&](auto act) {
-                                T* q = out;
-#pragma unroll
-                                for (int i = 0; i < 8; ++i, q += 4 * e.ldo)
-                                    if (i * 4 + (lane >> 3) < rows) {
-                                        float4 z = staged(i);
-                                        if (FP8) z.x *= sb.x, z.y *= sb.y, z.z *= sb.z, z.w *= sb.w;
-                                        const float4 x = e.res ? widen4<T>(r[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
-                                        store4(q, col, p.n, e.vec_out, finish4<decltype(act)::value>(z, b, x, e.act_bwd));
-                                    }
-                            });
-                            fetch(c0 + 64);
-                        }
-                        __syncwarp();
                     }
                 }
             } else {
                 const T* bias = (const T*)e.bias;
                 const uint32_t acc = tmem + (MODE == kGated ? buf * 256 : 0) + lanes;
                 T* out = (T*)e.out + row0 * e.ldo;
-                float* cv = reinterpret_cast<float*>(st + 2048);
-                float bg = column_value(bias, t.n0 + half * 32 + lane, p.n);
-                float bu = column_value(bias ? bias + p.n : bias, t.n0 + half * 32 + lane, p.n);
+                float* cv = reinterpret_cast<float*>(st);
+                const int c0 = cg * 32;                                        // the warp's only columns
+                const float bg = column_value(bias, t.n0 + c0 + lane, p.n);
+                const float bu = column_value(bias ? bias + p.n : bias, t.n0 + c0 + lane, p.n);
                 if (!(ok = mbar_wait(tf, bph))) break;
                 tc_fence_after();
-                auto add_bias = [&](float(&g)[32], float(&u)[32], int next) {
-                    if (!bias) return;
-                    cv[lane] = bg, cv[32 + lane] = bu;
-                    bg = column_value(bias, next + lane, p.n);
-                    bu = column_value(bias + p.n, next + lane, p.n);
-                    __syncwarp();
+                float g[32], u[32];
+                tmem_ld32(acc + c0, g);
+                tmem_ld32(acc + bh + c0, u);
+                if (bias) cv[lane] = bg, cv[32 + lane] = bu;
+                tmem_wait_ld();
+                reg_fence(g);
+                reg_fence(u);
+                release(&tempty[MODE == kGatedBwd ? 0 : buf]);
+                if (bias) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) g[j] += cv[j], u[j] += cv[32 + j];
                     __syncwarp();
-                };
+                }
                 if constexpr (MODE == kGated) {
-                    for (int c0 = half * 32; c0 < cend; c0 += 64) {
-                        float g[32], u[32];
-                        tmem_ld32(acc + c0, g);
-                        tmem_ld32(acc + bh + c0, u);
-                        tmem_wait_ld();
-                        reg_fence(g);
-                        reg_fence(u);
-                        if (c0 == last) release(&tempty[buf]);
-                        add_bias(g, u, t.n0 + c0 + 64);
-                        with_act(e.act, [&](auto act) {
+                    with_act(e.act, [&](auto act) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
-                        });
-                        stage16<T>(st, lane, u);
-                        __syncwarp();
-                        unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
-                        __syncwarp();
-                    }
+                        for (int j = 0; j < 32; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
+                    });
+                    stage16<T>(st, lane, u);
+                    __syncwarp();
+                    unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
                 } else {
                     const uint32_t acc_dh = tmem + kDh + buf * 128 + lanes;
-                    float g0[32], u0[32], g1[32], u1[32];
-                    const int c0 = half * 32, c1 = c0 + 64;
-                    tmem_ld32(acc + c0, g0);
-                    tmem_ld32(acc + bh + c0, u0);
-                    if (last == c1) {
-                        tmem_ld32(acc + c1, g1);
-                        tmem_ld32(acc + bh + c1, u1);
-                    }
-                    tmem_wait_ld();
-                    reg_fence(g0);
-                    reg_fence(u0);
-                    reg_fence(g1);
-                    reg_fence(u1);
-                    release(&tempty[0]);
-                    // g and u become what dh is multiplied by: g = act(g), u = u act'(g); h goes out first.
-                    auto chunk = [&](float(&g)[32], float(&u)[32], int c) {
-                        float d[32];
-                        add_bias(g, u, t.n0 + c + 64);
-                        with_act(e.act, [&](auto act) {
+                    // h goes out; g and u become what dh is multiplied by: g = act(g), u = u act'(g).
+                    with_act(e.act, [&](auto act) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
+                        for (int c = 0; c < 4; ++c) {
+                            float h[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
                                 float a, slope;
-                                act_both<decltype(act)::value>(g[j], a, slope);
-                                d[j] = a * u[j];
-                                g[j] = a;
-                                u[j] *= slope;
+                                act_both<decltype(act)::value>(g[8 * c + j], a, slope);
+                                h[j] = a * u[8 * c + j];
+                                g[8 * c + j] = a;
+                                u[8 * c + j] *= slope;
                             }
-                        });
-                        stage16<T>(st, lane, d);
-                        tmem_ld32(acc_dh + c, d);
-                        __syncwarp();
-                        unstage16(st, lane, out + 2 * p.plane, e.ldo, rows, t.n0 + c);
+                            *reinterpret_cast<uint4*>(stage_at(st, lane, c)) =
+                                make_uint4(pack2<T>(h[0], h[1]), pack2<T>(h[2], h[3]), pack2<T>(h[4], h[5]), pack2<T>(h[6], h[7]));
+                        }
+                    });
+                    __syncwarp();
+                    unstage16(st, lane, out + 2 * p.plane, e.ldo, rows, t.n0 + c0);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float d[16];
+                        tmem_ld16(acc_dh + c0 + h * 16, d);
                         tmem_wait_ld();
                         reg_fence(d);
-                        if (c == last) release(&dempty[buf]);
-                        __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) u[j] *= d[j], g[j] *= d[j];
-                        stage16<T>(st, lane, u);
-                        stage16<T>(st + 2048, lane, g);
-                        __syncwarp();
-                        unstage16(st, lane, out, e.ldo, rows, t.n0 + c);
-                        unstage16(st + 2048, lane, out + p.plane, e.ldo, rows, t.n0 + c);
-                        __syncwarp();
-                    };
-                    chunk(g0, u0, c0);
-                    if (last == c1) chunk(g1, u1, c1);
+                        for (int j = 0; j < 16; ++j) u[h * 16 + j] *= d[j], g[h * 16 + j] *= d[j];
+                    }
+                    release(&dempty[buf]);
+                    stage16<T>(st, lane, u);
+                    __syncwarp();
+                    unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
+                    __syncwarp();
+                    stage16<T>(st, lane, g);
+                    __syncwarp();
+                    unstage16(st, lane, out + p.plane, e.ldo, rows, t.n0 + c0);
                 }
+                __syncwarp();
             }
             buf ^= 1;
             if (MODE == kGatedBwd || buf == 0) bph ^= 1;
@@ -1053,6 +1092,12 @@ uint32_t idesc_of(int dtype, bool a_mn, bool b_mn, int ctas, int n) {
 
 template <auto Kernel>
 int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
+    const int row_tiles = g.msegs * g.tiles_m, group = std::min(row_tiles, kGroupRows / (kBM * ctas));
+    g.per_split = Divisor(row_tiles * g.tiles_n);
+    g.per_group = Divisor(group * g.tiles_n);
+    g.per_seg = Divisor(g.tiles_m);
+    g.group_rows = Divisor(group);
+    g.last_rows = Divisor(row_tiles % group ? row_tiles % group : group);
     constexpr int rest = kEpiWarps * kStageOut + kBarrierBytes;
     g.stages = std::min(kMaxStages, (kSmemLimit - rest) / g.stage_bytes);
     static std::once_flag once[64];  // per kernel and device
@@ -1120,7 +1165,8 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
     g.a_mn = q.a_mn, g.b_mn = q.b_mn;
     g.idesc = idesc_of(q.op_dtype, q.a_mn, q.b_mn, s.ctas, s.bn);
     g.e = q.e;
-    g.e.vec16 = !part && !q.e.res && q.n % 8 == 0 && q.e.ldo % 8 == 0 && aligned(q.e.out, 16);
+    g.e.vec16 = !part && q.n % 8 == 0 && q.e.ldo % 8 == 0 && aligned(q.e.out, 16) &&
+                (!q.e.res || (q.e.ldr % 8 == 0 && aligned(q.e.res, 16)));
     g.part = part;
     g.ldp = up(q.n, 4);
     if (!encode(&g.a, q.a, q.op_dtype, q.a_mn ? 64 : bk, q.a_mn ? bk : kBM)) return LF_ERR_CUDA;
