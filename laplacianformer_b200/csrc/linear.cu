@@ -208,6 +208,7 @@ constexpr int kEpiWarps = 16;             // four per 32-lane quarter of the ten
 constexpr int kControlWarps = 3;          // copies of A, products, copies of B
 constexpr int kGemmThreads = 32 * (kControlWarps + kEpiWarps);
 constexpr int kStageOut = 2048;           // output staging per epilogue warp: 32 rows of 64 bytes
+constexpr int kColumnBytes = 128;         // and an fp32 value for each of 32 columns
 constexpr int kEpiCols = kEpiWarps / 4 * 32;  // columns that the epilogue warps read at a time
 constexpr int kMaxStages = 8;
 constexpr int kTmemAll = 512;
@@ -363,8 +364,8 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out,
     const int group = p.per_group.of(r);
     r -= group * (int)p.per_group.d;
     const bool whole = (group + 1) * (int)p.group_rows.d <= p.msegs * p.tiles_m;
-    const Divisor& gm = whole ? p.group_rows : p.last_rows;
-    const int ni = gm.of(r), mi = group * (int)p.group_rows.d + r - ni * (int)gm.d;
+    const int ni = whole ? p.group_rows.of(r) : p.last_rows.of(r);
+    const int mi = group * (int)p.group_rows.d + r - ni * (int)(whole ? p.group_rows.d : p.last_rows.d);
     t.n0 = ni * bn_out;
     t.seg = p.per_seg.of(mi);
     t.m0 = ((mi - t.seg * p.tiles_m) * CTAS + rank) * kBM;
@@ -379,14 +380,18 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out,
 __device__ __forceinline__ uint8_t* stage_at(uint8_t* st, int row, int chunk) {
     return st + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
-// 32 16-bit columns: the calling lane's row in, 64-byte row segments out.
+// Columns 16 half .. of the calling lane's row: in as 16-bit values, whole
+// 64-byte row segments out.
 template <typename T>
-__device__ __forceinline__ void stage16(uint8_t* st, int lane, const float (&v)[32]) {
+__device__ __forceinline__ void pack16(uint4 (&u)[2], const float (&v)[16]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<uint4*>(stage_at(st, lane, c)) =
-            make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
-                       pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+    for (int c = 0; c < 2; ++c)
+        u[c] = make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
+                          pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+}
+__device__ __forceinline__ void stage16(uint8_t* st, int lane, int half, const uint4 (&u)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) *reinterpret_cast<uint4*>(stage_at(st, lane, half * 2 + c)) = u[c];
 }
 // out: row 0 of the warp's rows, of which `rows` exist; ld and col0 are multiples of 8.
 template <typename T>
@@ -422,7 +427,7 @@ template <typename T, int MODE, bool FP8, int CTAS>
 __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];  // stages, output staging, barriers
     uint8_t* out_stage = smem + p.stages * p.stage_bytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * kStageOut);
+    uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * (kStageOut + kColumnBytes));
     uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *dempty = tempty + 2, *drain = dempty + 2;
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -552,6 +557,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     } else {
         const int ew = warp - kControlWarps, quad = warp & 3, cg = ew >> 2;  // lanes of the tensor memory, columns of a tile
         uint8_t* st = out_stage + ew * kStageOut;
+        float* cv = reinterpret_cast<float*>(out_stage + kEpiWarps * kStageOut + ew * kColumnBytes);
         int buf = 0;
         uint32_t bph = 0;
         const Epilogue& e = p.e;
@@ -578,7 +584,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 const uint32_t acc = tmem + buf * 256 + lanes;
                 const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
                 const int first = cg * 32;
-                float* cv = reinterpret_cast<float*>(st);
                 if (e.vec16) {
                     // Whole 16-byte chunks: finished in the accumulator's
                     // layout (a lane owns a row); column values and the
@@ -599,55 +604,59 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                     if (!(ok = mbar_wait(tf, bph))) break;
                     tc_fence_after();
                     for (int c0 = first; c0 < cend; c0 += kEpiCols) {
-                        float v[32];
-                        tmem_ld32(acc + c0, v);
                         if (FP8 || e.bias) {
                             cv[lane] = bias;
-                            if (FP8) cv[32 + lane] = sb;
                             __syncwarp();
-                        }
-                        tmem_wait_ld();
-                        reg_fence(v);
-                        if (c0 == last) release(&tempty[buf]);
-                        if (FP8) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(v[j], sa * cv[32 + j], cv[j]);
-                        } else if (e.bias) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] += cv[j];
                         }
                         if (e.res) {  // to the lane that owns the row
-                            __syncwarp();
 #pragma unroll
                             for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
                             __syncwarp();
                         }
-                        if (e.act != LF_ACT_NONE)
-                            with_act(e.act, [&](auto act) {
+                        uint4 o[2][2];
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) {
-                                    float a, slope;
-                                    if (e.act_bwd) act_both<decltype(act)::value>(v[j], a, slope);
-                                    else slope = act_value<decltype(act)::value>(v[j]);
-                                    v[j] = slope;
-                                }
-                            });
-                        if (e.res) {  // added to the activation, or dy times its derivative
+                        for (int h = 0; h < 2; ++h) {
+                            float v[16];
+                            tmem_ld16(acc + c0 + h * 16, v);
+                            tmem_wait_ld();
+                            reg_fence(v);
+                            if (h == 1 && c0 == last) release(&tempty[buf]);
+                            if (FP8) {
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                const uint4 u = *reinterpret_cast<const uint4*>(stage_at(st, lane, c));
-                                const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+                                for (int j = 0; j < 16; ++j) v[j] = __fmaf_rn(v[j], sa * __shfl_sync(0xffffffffu, sb, h * 16 + j), cv[h * 16 + j]);
+                            } else if (e.bias) {
 #pragma unroll
-                                for (int h = 0; h < 4; ++h) {
-                                    const float2 x = unpack2<T>(w[h]);
-                                    float &y0 = v[8 * c + 2 * h], &y1 = v[8 * c + 2 * h + 1];
-                                    y0 = e.act_bwd ? y0 * x.x : y0 + x.x;
-                                    y1 = e.act_bwd ? y1 * x.y : y1 + x.y;
+                                for (int j = 0; j < 16; ++j) v[j] += cv[h * 16 + j];
+                            }
+                            if (e.act != LF_ACT_NONE)
+                                with_act(e.act, [&](auto act) {
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) {
+                                        float a, slope;
+                                        if (e.act_bwd) act_both<decltype(act)::value>(v[j], a, slope);
+                                        else slope = act_value<decltype(act)::value>(v[j]);
+                                        v[j] = slope;
+                                    }
+                                });
+                            if (e.res) {  // added to the activation, or dy times its derivative
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    const uint4 u = *reinterpret_cast<const uint4*>(stage_at(st, lane, 2 * h + c));
+                                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) {
+                                        const float2 x = unpack2<T>(w[k]);
+                                        float &y0 = v[8 * c + 2 * k], &y1 = v[8 * c + 2 * k + 1];
+                                        y0 = e.act_bwd ? y0 * x.x : y0 + x.x;
+                                        y1 = e.act_bwd ? y1 * x.y : y1 + x.y;
+                                    }
                                 }
                             }
+                            pack16<T>(o[h], v);
                         }
                         __syncwarp();
-                        stage16<T>(st, lane, v);
+                        stage16(st, lane, 0, o[0]);
+                        stage16(st, lane, 1, o[1]);
                         fetch(c0 + kEpiCols);
                         __syncwarp();
                         unstage16(st, lane, (T*)e.out + row0 * e.ldo, e.ldo, rows, t.n0 + c0);
@@ -716,72 +725,82 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 const T* bias = (const T*)e.bias;
                 const uint32_t acc = tmem + (MODE == kGated ? buf * 256 : 0) + lanes;
                 T* out = (T*)e.out + row0 * e.ldo;
-                float* cv = reinterpret_cast<float*>(st);
                 const int c0 = cg * 32;                                        // the warp's only columns
                 const float bg = column_value(bias, t.n0 + c0 + lane, p.n);
                 const float bu = column_value(bias ? bias + p.n : bias, t.n0 + c0 + lane, p.n);
                 if (!(ok = mbar_wait(tf, bph))) break;
                 tc_fence_after();
-                float g[32], u[32];
-                tmem_ld32(acc + c0, g);
-                tmem_ld32(acc + bh + c0, u);
-                if (bias) cv[lane] = bg, cv[32 + lane] = bu;
-                tmem_wait_ld();
-                reg_fence(g);
-                reg_fence(u);
-                release(&tempty[MODE == kGatedBwd ? 0 : buf]);
                 if (bias) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) g[j] += cv[j], u[j] += cv[32 + j];
+                    cv[lane] = bg;
                     __syncwarp();
                 }
-                if constexpr (MODE == kGated) {
-                    with_act(e.act, [&](auto act) {
+                // 16 columns at a time; outputs wait as 16-bit pairs.
+                uint4 og[2][2], ou[2][2];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
-                    });
-                    stage16<T>(st, lane, u);
-                    __syncwarp();
-                    unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
-                } else {
-                    const uint32_t acc_dh = tmem + kDh + buf * 128 + lanes;
-                    // h goes out; g and u become what dh is multiplied by: g = act(g), u = u act'(g).
-                    with_act(e.act, [&](auto act) {
+                for (int h = 0; h < 2; ++h) {
+                    const int c = c0 + h * 16;
+                    float g[16], u[16];
+                    tmem_ld16(acc + c, g);
+                    tmem_ld16(acc + bh + c, u);
+                    if constexpr (MODE == kGated) {
+                        tmem_wait_ld();
+                        reg_fence(g);
+                        reg_fence(u);
+                        if (h == 1) release(&tempty[buf]);
+                        if (bias) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float h[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                float a, slope;
-                                act_both<decltype(act)::value>(g[8 * c + j], a, slope);
-                                h[j] = a * u[8 * c + j];
-                                g[8 * c + j] = a;
-                                u[8 * c + j] *= slope;
-                            }
-                            *reinterpret_cast<uint4*>(stage_at(st, lane, c)) =
-                                make_uint4(pack2<T>(h[0], h[1]), pack2<T>(h[2], h[3]), pack2<T>(h[4], h[5]), pack2<T>(h[6], h[7]));
+                            for (int j = 0; j < 16; ++j) g[j] += cv[h * 16 + j], u[j] += __shfl_sync(0xffffffffu, bu, h * 16 + j);
                         }
-                    });
+                        with_act(e.act, [&](auto act) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
+                        });
+                        pack16<T>(ou[h], u);
+                    } else {
+                        float d[16];
+                        tmem_ld16(tmem + kDh + buf * 128 + lanes + c, d);
+                        tmem_wait_ld();
+                        reg_fence(g);
+                        reg_fence(u);
+                        reg_fence(d);
+                        if (h == 1) release(&tempty[0]), release(&dempty[buf]);
+                        if (bias) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) g[j] += cv[h * 16 + j], u[j] += __shfl_sync(0xffffffffu, bu, h * 16 + j);
+                        }
+                        // h = act(g) u, du = dh act(g), dg = dh u act'(g), in d, g and u
+                        with_act(e.act, [&](auto act) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                float a, slope;
+                                act_both<decltype(act)::value>(g[j], a, slope);
+                                const float dh = d[j];
+                                d[j] = a * u[j];
+                                g[j] = a * dh;
+                                u[j] *= slope * dh;
+                            }
+                        });
+                        uint4 oh[2];
+                        pack16<T>(oh, d);
+                        pack16<T>(og[h], g);
+                        pack16<T>(ou[h], u);
+                        stage16(st, lane, h, oh);
+                    }
+                }
+                if constexpr (MODE == kGatedBwd) {
                     __syncwarp();
                     unstage16(st, lane, out + 2 * p.plane, e.ldo, rows, t.n0 + c0);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float d[16];
-                        tmem_ld16(acc_dh + c0 + h * 16, d);
-                        tmem_wait_ld();
-                        reg_fence(d);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) u[h * 16 + j] *= d[j], g[h * 16 + j] *= d[j];
-                    }
-                    release(&dempty[buf]);
-                    stage16<T>(st, lane, u);
                     __syncwarp();
-                    unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
-                    __syncwarp();
-                    stage16<T>(st, lane, g);
+                    stage16(st, lane, 0, og[0]);
+                    stage16(st, lane, 1, og[1]);
                     __syncwarp();
                     unstage16(st, lane, out + p.plane, e.ldo, rows, t.n0 + c0);
                 }
+                __syncwarp();
+                stage16(st, lane, 0, ou[0]);
+                stage16(st, lane, 1, ou[1]);
+                __syncwarp();
+                unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
                 __syncwarp();
             }
             buf ^= 1;
@@ -1098,7 +1117,7 @@ int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
     g.per_seg = Divisor(g.tiles_m);
     g.group_rows = Divisor(group);
     g.last_rows = Divisor(row_tiles % group ? row_tiles % group : group);
-    constexpr int rest = kEpiWarps * kStageOut + kBarrierBytes;
+    constexpr int rest = kEpiWarps * (kStageOut + kColumnBytes) + kBarrierBytes;
     g.stages = std::min(kMaxStages, (kSmemLimit - rest) / g.stage_bytes);
     static std::once_flag once[64];  // per kernel and device
     int dev = 0;
