@@ -48,4 +48,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> GatedFeed
 // Writes the clipped gradients to `outs` (which may be `grads`) and returns the norm (a float32 scalar).
 at::Tensor ClipGradNorm(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs, double max_norm);
 
+// The same operators as autograd nodes; without a tensor that requires a
+// gradient they are the _forward functions.  RmsNorm returns (y, s).
+std::tuple<at::Tensor, at::Tensor> RmsNorm(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& residual, double eps);
+at::Tensor Linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, const at::Tensor& residual,
+                  int64_t activation);
+at::Tensor GatedFeedForward(const at::Tensor& x, const at::Tensor& w_in, const at::Tensor& w_out, const at::Tensor& b_in,
+                            const at::Tensor& b_out, const at::Tensor& residual, int64_t activation);
+
 }  // namespace laplace

@@ -125,6 +125,8 @@ __device__ __forceinline__ V block_sum(V v, V* sh) {
 
 __global__ void __launch_bounds__(kThreads) grad_sq_kernel(const __grid_constant__ Table t, double* part) {
     __shared__ double sh[kThreads / 32];
+    grid_release();
+    grid_wait();
     const int chunks = t.first[t.count];
     for (int k = blockIdx.x; k < chunks; k += gridDim.x) {
         const int i = tensor_of(t, k);
@@ -142,6 +144,8 @@ __global__ void __launch_bounds__(kThreads) grad_sq_kernel(const __grid_constant
 __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_constant__ Table t, const double* part,
                                                               float max_norm, float* norm) {
     __shared__ double sh[kThreads / 32];
+    grid_release();
+    grid_wait();
     double s = 0.;
     for (int k = threadIdx.x; k < t.total; k += kThreads) s += part[k];
     const float n = (float)sqrt(block_sum<double>(s, sh));
@@ -242,8 +246,8 @@ extern "C" int lf_clip_grad_norm(const void* const* grads, void* const* outs, co
             base += chunks;
             const int slots = 8 * num_sms();
             const unsigned grid = (unsigned)(chunks < 1 ? 1 : chunks < slots ? chunks : slots);
-            if (pass == 0) grad_sq_kernel<<<grid, kThreads, 0, st>>>(t, (double*)workspace);
-            else grad_scale_kernel<<<grid, kThreads, 0, st>>>(t, (const double*)workspace, (float)max_norm, norm);
+            if (pass == 0) launch_early(grad_sq_kernel, grid, kThreads, 0, 1, st, t, (double*)workspace);
+            else launch_early(grad_scale_kernel, grid, kThreads, 0, 1, st, t, (const double*)workspace, (float)max_norm, norm);
             if (int rc = check_launch("lf_clip_grad_norm")) return rc;
         } while (i < count);
     }

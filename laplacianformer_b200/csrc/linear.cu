@@ -439,6 +439,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     const int bn_out = MODE == kLinear ? p.bn : bh;
     const int phases = MODE == kGatedBwd ? 2 : 1;
 
+    grid_release();
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 2), mbar_init(&empty[i], 1);
         for (int i = 0; i < 2; ++i)
@@ -451,6 +452,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     __syncthreads();
     sync_all<CTAS>();
     tc_fence_after();
+    grid_wait();
     const uint32_t tmem = *tmem_ptr;
     const int units = p.splits * p.msegs * p.tiles_m * p.tiles_n;
     const int unit0 = blockIdx.x / CTAS, unit_step = gridDim.x / CTAS;
@@ -819,6 +821,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
 template <typename T>
 __global__ void __launch_bounds__(256) split_join_kernel(const float* part, int splits, int64_t rows, int n, int64_t ldp,
                                                          const Epilogue e) {
+    grid_release();
+    grid_wait();
     const int64_t groups = ldp / 4, total = rows * groups;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / groups;
@@ -844,66 +848,92 @@ __global__ void __launch_bounds__(256) split_join_kernel(const float* part, int 
 }
 
 // Copies a matrix whose rows TMA cannot address (row pitch or base not a
-// multiple of 16 bytes) to rows of ldo elements.
+// multiple of 16 bytes) to rows of ldo elements: a warp per row, 16 bytes of
+// output per lane at a time (its scalar loads share cache lines).
 template <typename U>
 __global__ void __launch_bounds__(256) pack_rows_kernel(const U* in, int64_t ldi, U* out, int64_t ldo, int64_t rows, int64_t cols) {
-    const int64_t total = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        out[r * ldo + c] = in[r * ldi + c];
-    }
+    constexpr int V = 16 / sizeof(U);
+    grid_release();
+    grid_wait();
+    const int lane = threadIdx.x & 31;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8)
+        for (int64_t c = lane * V; c < ldo; c += 32 * V) {
+            U v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = c + j < cols ? in[r * ldi + c + j] : U(0);
+            *reinterpret_cast<uint4*>(out + r * ldo + c) = *reinterpret_cast<const uint4*>(v);
+        }
 }
 
-// Column sums, first step: part[slice][c] over the rows of a slice.  A thread
-// adds V neighbouring columns; the block's eight row walkers join in order.
+// Column sums of up to three matrices in one launch (blockIdx.z).  First step:
+// part[slice][c] over the rows of a slice.  A thread adds V neighbouring
+// columns; tx threads cover a row and 256/tx rows go side by side, whose sums
+// join in order.
+struct ColsumJob {
+    const void* in;
+    void* out;
+    float* part;
+    int64_t ld, cols;
+};
+struct ColsumJobs {
+    ColsumJob job[3];
+    int64_t rows, slice;
+    int slices, tx;
+};
 template <typename T, int V>
-__global__ void __launch_bounds__(256) colsum_kernel(const T* in, int64_t ld, int64_t rows, int64_t cols, int64_t slice, float* part) {
-    __shared__ float sh[8][32 * V];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * V;
-    const int64_t r0 = (int64_t)blockIdx.y * slice, r1 = min(rows, r0 + slice);
+__global__ void __launch_bounds__(256) colsum_kernel(const ColsumJobs p) {
+    __shared__ float sh[256 * V];
+    grid_release();
+    grid_wait();
+    const ColsumJob j = p.job[blockIdx.z];
+    const int walkers = 256 / p.tx, w = threadIdx.x / p.tx, width = p.tx * V, at = (threadIdx.x - w * p.tx) * V;
+    const int64_t c0 = (int64_t)blockIdx.x * width;
+    if (c0 >= j.cols) return;
+    const int64_t r0 = (int64_t)blockIdx.y * p.slice + w, r1 = min(p.rows, (int64_t)(blockIdx.y + 1) * p.slice);
     float a[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) a[j] = 0.f;
-    if (c < cols)
-        for (int64_t r = r0 + w; r < r1; r += 8) {
-            if constexpr (V == 1) a[0] += Elem<T>::load(in[r * ld + c]);
+    for (int k = 0; k < V; ++k) a[k] = 0.f;
+    if (c0 + at < j.cols) {
+        const T* q = (const T*)j.in + c0 + at;
+#pragma unroll 4
+        for (int64_t r = r0; r < r1; r += walkers) {
+            if constexpr (V == 1) a[0] += Elem<T>::load(q[r * j.ld]);
             else {
-                uint4 u;
-                if constexpr (V == 8) u = *reinterpret_cast<const uint4*>(in + r * ld + c);
-                else u.x = *reinterpret_cast<const uint32_t*>(in + r * ld + c);
+                const uint4 u = *reinterpret_cast<const uint4*>(q + r * j.ld);
                 const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-                for (int j = 0; j < V; ++j) a[j] += Elem<T>::load(e[j]);
+                for (int k = 0; k < V; ++k) a[k] += Elem<T>::load(e[k]);
             }
         }
-#pragma unroll
-    for (int j = 0; j < V; ++j) sh[w][lane * V + j] = a[j];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * V; i += 256) {
-        const int64_t col = (int64_t)blockIdx.x * 32 * V + i;
-        if (col < cols) {
-            float t = 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) t += sh[k][i];
-            part[(int64_t)blockIdx.y * cols + col] = t;
-        }
     }
+#pragma unroll
+    for (int k = 0; k < V; ++k) sh[w * width + at + k] = a[k];
+    __syncthreads();
+    for (int i = threadIdx.x; i < width; i += 256)
+        if (c0 + i < j.cols) {
+            float t = 0.f;
+            for (int k = 0; k < walkers; ++k) t += sh[k * width + i];
+            j.part[(int64_t)blockIdx.y * j.cols + c0 + i] = t;
+        }
 }
 template <typename T>
-__global__ void __launch_bounds__(256) colsum_join_kernel(const float* part, int slices, int64_t cols, T* out) {
-    __shared__ float sh[8][33];
+__global__ void __launch_bounds__(512) colsum_join_kernel(const ColsumJobs p) {
+    __shared__ float sh[16][33];
+    grid_release();
+    grid_wait();
+    const ColsumJob j = p.job[blockIdx.z];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     float t = 0.f;
-    if (c < cols)
-        for (int s = w; s < slices; s += 8) t += part[(int64_t)s * cols + c];
+    if (c < j.cols)
+#pragma unroll 4
+        for (int s = w; s < p.slices; s += 16) t += j.part[(int64_t)s * j.cols + c];
     sh[w][lane] = t;
     __syncthreads();
-    if (w == 0 && c < cols) {
+    if (w == 0 && c < j.cols) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) t += sh[i][lane];
-        out[c] = Elem<T>::store(t);
+        for (int i = 1; i < 16; ++i) t += sh[i][lane];
+        ((T*)j.out)[c] = Elem<T>::store(t);
     }
 }
 
@@ -914,6 +944,8 @@ template <typename T, bool GATED, int MT, bool VEC>
 __global__ void __launch_bounds__(256) few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int m, int n, int k,
                                                        int wpr, const Epilogue e) {
     __shared__ float sh[8][GATED ? 2 : 1][MT];
+    grid_release();
+    grid_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = warp % wpr, col = blockIdx.x * (8 / wpr) + warp / wpr;
     float a[GATED ? 2 : 1][MT];
@@ -1124,22 +1156,8 @@ int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
     cudaGetDevice(&dev);
     std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
     const int64_t units = (int64_t)g.splits * g.msegs * g.tiles_m * g.tiles_n;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(units, num_sms() / ctas) * ctas));
-    cfg.blockDim = dim3(kGemmThreads);
-    cfg.dynamicSmemBytes = (size_t)g.stages * g.stage_bytes + rest;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)ctas, at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, Kernel, g);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        set_error("tc_gemm_kernel: %s", cudaGetErrorString(e));
-        return LF_ERR_CUDA;
-    }
+    const unsigned grid = (unsigned)(std::min<int64_t>(units, num_sms() / ctas) * ctas);
+    launch_early(Kernel, grid, kGemmThreads, (size_t)g.stages * g.stage_bytes + rest, (unsigned)ctas, st, g);
     return check_launch("tc_gemm_kernel");
 }
 
@@ -1156,8 +1174,8 @@ int too_large(const char* what) {
 int join_splits(const Product& q, const float* part, int splits, cudaStream_t st) {
     const int64_t rows = q.m * q.msegs, ldp = up(q.n, 4), groups = rows * (ldp / 4);
     const unsigned grid = (unsigned)std::min<int64_t>((groups + 255) / 256, (int64_t)num_sms() * 16);
-    if (q.dtype == LF_F16) split_join_kernel<__half><<<grid, 256, 0, st>>>(part, splits, rows, (int)q.n, ldp, q.e);
-    else split_join_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(part, splits, rows, (int)q.n, ldp, q.e);
+    auto kernel = q.dtype == LF_F16 ? split_join_kernel<__half> : split_join_kernel<__nv_bfloat16>;
+    launch_early(kernel, grid, 256, 0, 1, st, part, splits, rows, (int)q.n, ldp, q.e);
     return check_launch("split_join_kernel");
 }
 
@@ -1206,9 +1224,9 @@ Mat operand(const void* p, int64_t rows, int64_t cols, int64_t ld, int es, Arena
     const int64_t ldo = up(cols, 16 / es);
     void* out = ws.take((size_t)rows * ldo * es);
     if (out) {
-        const unsigned grid = (unsigned)std::min<int64_t>((rows * cols + 255) / 256, (int64_t)num_sms() * 32);
-        if (es == 1) pack_rows_kernel<uint8_t><<<grid, 256, 0, st>>>((const uint8_t*)p, ld, (uint8_t*)out, ldo, rows, cols);
-        else pack_rows_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)p, ld, (uint16_t*)out, ldo, rows, cols);
+        const unsigned grid = (unsigned)std::min<int64_t>((rows + 7) / 8, (int64_t)num_sms() * 8);
+        if (es == 1) launch_early(pack_rows_kernel<uint8_t>, grid, 256, 0, 1, st, (const uint8_t*)p, ld, (uint8_t*)out, ldo, rows, cols);
+        else launch_early(pack_rows_kernel<uint16_t>, grid, 256, 0, 1, st, (const uint16_t*)p, ld, (uint16_t*)out, ldo, rows, cols);
     }
     return {out, cols, rows, ldo, 1, 0};
 }
@@ -1229,28 +1247,50 @@ int zero(void* p, int64_t rows, int64_t row_bytes, cudaStream_t st) {
     return LF_OK;
 }
 
-template <typename T>
-void launch_colsum(const T* in, int64_t ld, int64_t rows, int64_t cols, T* out, float* part, int64_t slice, int slices, cudaStream_t st) {
-    const bool v8 = cols >= 256 && cols % 8 == 0 && ld % 8 == 0 && aligned(in, 16);
-    const bool v2 = cols % 2 == 0 && ld % 2 == 0 && aligned(in, 4);
-    const int v = v8 ? 8 : v2 ? 2 : 1;
-    const dim3 grid((unsigned)((cols + 32 * v - 1) / (32 * v)), (unsigned)slices);
-    if (v8) colsum_kernel<T, 8><<<grid, 256, 0, st>>>(in, ld, rows, cols, slice, part);
-    else if (v2) colsum_kernel<T, 2><<<grid, 256, 0, st>>>(in, ld, rows, cols, slice, part);
-    else colsum_kernel<T, 1><<<grid, 256, 0, st>>>(in, ld, rows, cols, slice, part);
-    colsum_join_kernel<T><<<(unsigned)((cols + 31) / 32), 256, 0, st>>>(part, slices, cols, out);
-}
-
-// out[c] = sum of column c of in [rows, cols] (16-bit).
-int run_colsum(const void* in, int64_t ld, int64_t rows, int64_t cols, void* out, int dtype, Arena& ws, cudaStream_t st) {
-    if (rows == 0 || cols == 0) return ws.base ? zero(out, 1, cols * 2, st) : LF_OK;
-    const int64_t want = std::max<int64_t>(1, 4 * num_sms() * 64 / std::max<int64_t>(cols, 64));
-    const int64_t slice = std::max<int64_t>(64, (rows + want - 1) / want);
-    const int slices = (int)((rows + slice - 1) / slice);
-    float* part = (float*)ws.take((size_t)slices * cols * 4);
+// out[c] = sum of column c of in [rows, cols] (16-bit), for `count` matrices of
+// as many rows.  `padded`: whole vectors may be read past cols (our own buffers).
+struct Columns {
+    const void* in;
+    int64_t ld, cols;
+    void* out;
+    bool padded;
+};
+int run_colsum(const Columns* c, int count, int64_t rows, int dtype, Arena& ws, cudaStream_t st) {
+    ColsumJobs p{};
+    int64_t widest = 0;
+    bool vec = true;
+    int jobs = 0;
+    for (int i = 0; i < count; ++i) {
+        if (c[i].cols == 0 || !c[i].out) continue;
+        if (rows == 0) {
+            if (ws.base)
+                if (int rc = zero(c[i].out, 1, c[i].cols * 2, st)) return rc;
+            continue;
+        }
+        vec = vec && aligned(c[i].in, 16) && c[i].ld % 8 == 0 && (c[i].padded || c[i].cols % 8 == 0);
+        p.job[jobs++] = {c[i].in, c[i].out, nullptr, c[i].ld, c[i].cols};
+        widest = std::max(widest, c[i].cols);
+    }
+    if (!jobs) return LF_OK;
+    const int v = vec ? 8 : 1;
+    p.tx = 1;
+    while (p.tx < 32 && p.tx * v < widest) p.tx *= 2;
+    const int64_t wide = (widest + p.tx * v - 1) / (p.tx * v);
+    // About eight blocks per SM, each at least four rows per row walker.
+    const int64_t most = std::max<int64_t>(1, 8 * num_sms() / (wide * jobs)), least = 4 * 256 / p.tx;
+    p.rows = rows;
+    p.slice = std::max(least, (rows + most - 1) / most);
+    p.slices = (int)((rows + p.slice - 1) / p.slice);
+    for (int i = 0; i < jobs; ++i) p.job[i].part = (float*)ws.take((size_t)p.slices * p.job[i].cols * 4);
     if (!ws.base) return LF_OK;
-    if (dtype == LF_F16) launch_colsum((const __half*)in, ld, rows, cols, (__half*)out, part, slice, slices, st);
-    else launch_colsum((const __nv_bfloat16*)in, ld, rows, cols, (__nv_bfloat16*)out, part, slice, slices, st);
+    const dim3 grid((unsigned)wide, (unsigned)p.slices, (unsigned)jobs), join((unsigned)((widest + 31) / 32), 1, (unsigned)jobs);
+    if (dtype == LF_F16) {
+        launch_early(vec ? colsum_kernel<__half, 8> : colsum_kernel<__half, 1>, grid, 256, 0, 1, st, p);
+        launch_early(colsum_join_kernel<__half>, join, 512, 0, 1, st, p);
+    } else {
+        launch_early(vec ? colsum_kernel<__nv_bfloat16, 8> : colsum_kernel<__nv_bfloat16, 1>, grid, 256, 0, 1, st, p);
+        launch_early(colsum_join_kernel<__nv_bfloat16>, join, 512, 0, 1, st, p);
+    }
     return check_launch("colsum_kernel");
 }
 
@@ -1264,8 +1304,8 @@ void launch_few(const void* x, int64_t ldx, const void* w, int64_t ldw, int m, i
     const unsigned grid = (unsigned)((n + 8 / wpr - 1) / (8 / wpr));
     const T *xp = (const T*)x, *wp = (const T*)w;
 #define LFB_FEW(MT)                                                                                          \
-    if (vec) few_rows_kernel<T, GATED, MT, true><<<grid, 256, 0, st>>>(xp, ldx, wp, ldw, m, n, k, wpr, e);   \
-    else few_rows_kernel<T, GATED, MT, false><<<grid, 256, 0, st>>>(xp, ldx, wp, ldw, m, n, k, wpr, e)
+    launch_early(vec ? few_rows_kernel<T, GATED, MT, true> : few_rows_kernel<T, GATED, MT, false>, grid, 256, 0, 1, st, xp, ldx, \
+                 wp, ldw, m, n, k, wpr, e)
     if (m == 1) { LFB_FEW(1); }
     else if (m == 2) { LFB_FEW(2); }
     else if (m <= 4) { LFB_FEW(4); }
@@ -1376,8 +1416,8 @@ int linear_bwd(const lf_linear_t* a, Arena& ws, cudaStream_t st) {
         set_out(q.e, a->dw, k);
         if (int rc = run_product(q, ws, st)) return rc;
     }
-    if (a->db) return run_colsum(dz.p, dz.ld, m, n, a->db, a->dtype, ws, st);
-    return LF_OK;
+    const Columns c{dz.p, dz.ld, n, a->db, need_z};
+    return run_colsum(&c, 1, m, a->dtype, ws, st);
 }
 
 // ---- gated feed-forward block ----------------------------------------------
@@ -1500,11 +1540,9 @@ int ffn_bwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
         set_out(q.e, a->dw_out, f);
         if (int rc = run_product(q, ws, st)) return rc;
     }
-    if (a->db_in)
-        for (int s = 0; s < 2; ++s)
-            if (int rc = run_colsum(dz + s * plane, ld, m, f, (uint16_t*)a->db_in + s * f, a->dtype, ws, st)) return rc;
-    if (a->db_out) return run_colsum(a->dy, a->lddy, m, c, a->db_out, a->dtype, ws, st);
-    return LF_OK;
+    uint16_t* db_in = (uint16_t*)a->db_in;
+    const Columns cols[3] = {{dz, ld, f, db_in, true}, {dz + plane, ld, f, db_in ? db_in + f : nullptr, true}, {a->dy, a->lddy, c, a->db_out, false}};
+    return run_colsum(cols, 3, m, a->dtype, ws, st);
 }
 
 int check_ws(const char* what, const void* ws, size_t have, size_t need) {

@@ -110,6 +110,8 @@ template <typename T, int VEC, int NV, int G, bool QUANT>
 __global__ void __launch_bounds__(block_of<G>(), fwd_blocks<NV, G>()) rms_fwd_kernel(const NormArgs p) {
     constexpr int RPB = block_of<G>() / G;  // rows in flight per block
     __shared__ float red[32];
+    grid_release();
+    grid_wait();
     const int g = threadIdx.x % G, sub = threadIdx.x / G;
     const int cols = (int)p.cols;
     Pack<T, VEC> w[NV];
@@ -193,6 +195,8 @@ __global__ void __launch_bounds__(block_of<G>(), fwd_blocks<NV, G>()) rms_fwd_ke
 template <typename T, bool QUANT>
 __global__ void __launch_bounds__(512) rms_fwd_long_kernel(const NormArgs p) {
     __shared__ float red[32];
+    grid_release();
+    grid_wait();
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T* x = (const T*)p.x + row * p.cols;
         const T* r = p.res ? (const T*)p.res + row * p.cols : nullptr;
@@ -239,6 +243,8 @@ __global__ void __launch_bounds__(block_of<G>()) rms_bwd_kernel(const NormBwdArg
     constexpr int RPB = block_of<G>() / G;
     extern __shared__ float dwsum[];  // [warps][cols] when G <= 32
     __shared__ float red[32];
+    grid_release();
+    grid_wait();
     const int g = threadIdx.x % G, sub = threadIdx.x / G;
     const int cols = (int)p.cols;
     Pack<T, VEC> w[NV];
@@ -331,6 +337,8 @@ __global__ void __launch_bounds__(block_of<G>()) rms_bwd_kernel(const NormBwdArg
 template <typename T>
 __global__ void __launch_bounds__(512) rms_bwd_long_kernel(const NormBwdArgs p) {
     __shared__ float red[32];
+    grid_release();
+    grid_wait();
     float* part = p.part ? p.part + (int64_t)blockIdx.x * p.cols : nullptr;
     if (part)
         for (int64_t c = threadIdx.x; c < p.cols; c += 512) part[c] = 0.f;
@@ -360,6 +368,8 @@ __global__ void __launch_bounds__(512) rms_bwd_long_kernel(const NormBwdArgs p) 
 template <typename T>
 __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, T* dw, int blocks, int64_t cols) {
     __shared__ float sh[32][33];
+    grid_release();
+    grid_wait();
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     float t = 0.f;
@@ -453,14 +463,14 @@ template <typename T, bool QUANT>
 void launch_fwd(const NormArgs& a, bool vec, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     bool long_rows = false;
-#define LFB_CALL(TT, VV, NV, G)                                                                                    \
-    rms_fwd_kernel<TT, VV, NV, G, QUANT>                                                                           \
-        <<<row_blocks(a.rows, block_of<G>() / G, resident_blocks<rms_fwd_kernel<TT, VV, NV, G, QUANT>>(block_of<G>(), 0)), \
-           block_of<G>(), 0, st>>>(a)
+#define LFB_CALL(TT, VV, NV, G)                                                                                        \
+    launch_early(rms_fwd_kernel<TT, VV, NV, G, QUANT>,                                                                 \
+                 row_blocks(a.rows, block_of<G>() / G, resident_blocks<rms_fwd_kernel<TT, VV, NV, G, QUANT>>(block_of<G>(), 0)), \
+                 block_of<G>(), 0, 1, st, a)
     LFB_NORM_FWD(T, V, a.cols, vec, LFB_CALL)
 #undef LFB_CALL
     if (long_rows)
-        rms_fwd_long_kernel<T, QUANT><<<row_blocks(a.rows, 1, resident_blocks<rms_fwd_long_kernel<T, QUANT>>(512, 0)), 512, 0, st>>>(a);
+        launch_early(rms_fwd_long_kernel<T, QUANT>, row_blocks(a.rows, 1, resident_blocks<rms_fwd_long_kernel<T, QUANT>>(512, 0)), 512, 0, 1, st, a);
 }
 
 template <typename T>
@@ -473,14 +483,14 @@ void launch_bwd(const NormBwdArgs& a, void* dw, bool vec, cudaStream_t st) {
         return blocks = row_blocks(a.rows, per_block, (int)(slots < most ? slots : most));
     };
     // Shared memory of the largest width that a warp-per-row group takes, so that residency does not depend on cols.
-#define LFB_CALL(TT, VV, NV, G)                                                                                  \
-    rms_bwd_kernel<TT, VV, NV, G>                                                                                \
-        <<<grid(block_of<G>() / G, resident_blocks<rms_bwd_kernel<TT, VV, NV, G>>(block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0)), \
-           block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0, st>>>(a)
+#define LFB_CALL(TT, VV, NV, G)                                                                                   \
+    launch_early(rms_bwd_kernel<TT, VV, NV, G>,                                                                   \
+                 grid(block_of<G>() / G, resident_blocks<rms_bwd_kernel<TT, VV, NV, G>>(block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0)), \
+                 block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0, 1, st, a)
     LFB_NORM_BWD(T, V, a.cols, vec, LFB_CALL)
 #undef LFB_CALL
-    if (long_rows) rms_bwd_long_kernel<T><<<grid(1, resident_blocks<rms_bwd_long_kernel<T>>(512, 0)), 512, 0, st>>>(a);
-    if (dw) rms_dw_kernel<T><<<(unsigned)((a.cols + 31) / 32), 1024, 0, st>>>(a.part, (T*)dw, (int)blocks, a.cols);
+    if (long_rows) launch_early(rms_bwd_long_kernel<T>, grid(1, resident_blocks<rms_bwd_long_kernel<T>>(512, 0)), 512, 0, 1, st, a);
+    if (dw) launch_early(rms_dw_kernel<T>, (unsigned)((a.cols + 31) / 32), 1024, 0, 1, st, a.part, (T*)dw, (int)blocks, a.cols);
 }
 
 int check_rows(const char* what, int64_t rows, int64_t cols, int dtype) {

@@ -344,10 +344,12 @@ at::Tensor ClipGradNorm(const std::vector<at::Tensor>& grads, const std::vector<
     for (size_t i = 0; i < n; ++i) {
         need_cuda(grads[i], "gradient");
         TORCH_CHECK(grads[i].device() == grads[0].device(), "all gradients must be on one device");
-        TORCH_CHECK(grads[i].is_non_overlapping_and_dense(), "gradients must be dense");
         check_operand(outs[i], grads[i], "output");
-        TORCH_CHECK(outs[i].sizes() == grads[i].sizes() && outs[i].strides() == grads[i].strides(),
-                    "an output must have its gradient's shape and strides");
+        TORCH_CHECK(outs[i].sizes() == grads[i].sizes(), "an output must have its gradient's shape and strides");
+        if (!grads[i].is_contiguous() || !outs[i].is_contiguous()) {
+            TORCH_CHECK(grads[i].is_non_overlapping_and_dense(), "gradients must be dense");
+            TORCH_CHECK(outs[i].strides() == grads[i].strides(), "an output must have its gradient's shape and strides");
+        }
         in[i] = grads[i].data_ptr();
         out[i] = outs[i].data_ptr();
         sizes[i] = grads[i].numel();
@@ -361,6 +363,126 @@ at::Tensor ClipGradNorm(const std::vector<at::Tensor>& grads, const std::vector<
                                (float*)norm.data_ptr(), mut(ws), need, stream_of(grads[0])),
              "ClipGradNorm");
     return norm;
+}
+
+
+// ---------------------------------------------------------------------------
+// Autograd nodes.  They live here rather than in Python because a small
+// training step spends more time in Python nodes than in the kernels.
+// ---------------------------------------------------------------------------
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor opt(const c10::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
+c10::optional<at::Tensor> as_opt(const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; }
+
+void first_order(const char* op) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), std::string(op) + " has no second derivative (create_graph is not supported)");
+}
+
+struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                                 const c10::optional<at::Tensor>& residual, double eps) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [y, s, rstd] = RmsNorm_forward(x, weight, opt(residual), eps, true);
+        ctx->save_for_backward({s.defined() ? s : x, rstd, weight});
+        ctx->saved_data["residual"] = s.defined();
+        ctx->set_materialize_grads(false);
+        if (s.defined()) return {y, s};
+        return {y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        first_order("rms_norm");
+        const auto saved = ctx->get_saved_variables();
+        const bool residual = ctx->saved_data["residual"].toBool();
+        const at::Tensor ds = residual ? g[1] : at::Tensor();
+        // Inputs of the node: x, weight and, where given, the residual.
+        const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nr = residual && ctx->needs_input_grad(2);
+        at::Tensor dx, dw;
+        if (!g[0].defined()) dx = ds;  // only the sum was used: its gradient passes through
+        else std::tie(dx, dw) = RmsNorm_backward(g[0], ds, saved[0], saved[1], saved[2], nx || nr, nw);
+        return {nx ? dx : at::Tensor(), dw, nr ? dx : at::Tensor(), at::Tensor()};
+    }
+};
+
+struct LinearNode : torch::autograd::Function<LinearNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                              const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, int64_t act) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({x, weight, opt(bias)});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["residual"] = residual.has_value();
+        return Linear_forward(x, weight, opt(bias), opt(residual), act);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        first_order("linear");
+        const auto saved = ctx->get_saved_variables();
+        const bool bias = saved[2].defined(), residual = ctx->saved_data["residual"].toBool();
+        const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = bias && ctx->needs_input_grad(2);
+        const bool nr = residual && ctx->needs_input_grad(2 + bias);
+        at::Tensor dx, dw, db;
+        if (nx || nw || nb)
+            std::tie(dx, dw, db) = Linear_backward(g[0], saved[0], saved[1], saved[2], ctx->saved_data["act"].toInt(), nx, nw, nb);
+        return {dx, dw, db, nr ? g[0] : at::Tensor(), at::Tensor()};
+    }
+};
+
+struct GatedFeedForwardNode : torch::autograd::Function<GatedFeedForwardNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w_in, const at::Tensor& w_out,
+                              const c10::optional<at::Tensor>& b_in, const c10::optional<at::Tensor>& b_out,
+                              const c10::optional<at::Tensor>& residual, int64_t act) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({x, w_in, w_out, opt(b_in)});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["b_out"] = b_out.has_value();
+        ctx->saved_data["residual"] = residual.has_value();
+        return GatedFeedForward_forward(x, w_in, w_out, opt(b_in), opt(b_out), opt(residual), act);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        first_order("gated_feed_forward");
+        const auto saved = ctx->get_saved_variables();
+        const bool bi = saved[3].defined(), bo = ctx->saved_data["b_out"].toBool(), r = ctx->saved_data["residual"].toBool();
+        const bool n0 = ctx->needs_input_grad(0), n1 = ctx->needs_input_grad(1), n2 = ctx->needs_input_grad(2);
+        const bool n3 = bi && ctx->needs_input_grad(3), n4 = bo && ctx->needs_input_grad(3 + bi);
+        const bool n5 = r && ctx->needs_input_grad(3 + bi + bo);
+        at::Tensor dx, dwi, dwo, dbi, dbo;
+        if (n0 || n1 || n2 || n3 || n4)
+            std::tie(dx, dwi, dwo, dbi, dbo) = GatedFeedForward_backward(g[0], saved[0], saved[1], saved[2], saved[3],
+                                                                        ctx->saved_data["act"].toInt(), n0, n1, n2, n3, n4);
+        return {dx, dwi, dwo, dbi, dbo, n5 ? g[0] : at::Tensor(), at::Tensor()};
+    }
+};
+
+bool tracked(std::initializer_list<const at::Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor* t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> RmsNorm(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& residual, double eps) {
+    if (tracked({&x, &weight, &residual})) {
+        variable_list out = RmsNormNode::apply(x, weight, as_opt(residual), eps);
+        return {out[0], out.size() > 1 ? out[1] : at::Tensor()};
+    }
+    auto [y, s, rstd] = RmsNorm_forward(x, weight, residual, eps, false);
+    return {y, s};
+}
+
+at::Tensor Linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, const at::Tensor& residual, int64_t act) {
+    if (tracked({&x, &weight, &bias, &residual})) return LinearNode::apply(x, weight, as_opt(bias), as_opt(residual), act);
+    return Linear_forward(x, weight, bias, residual, act);
+}
+
+at::Tensor GatedFeedForward(const at::Tensor& x, const at::Tensor& w_in, const at::Tensor& w_out, const at::Tensor& b_in,
+                            const at::Tensor& b_out, const at::Tensor& residual, int64_t act) {
+    if (tracked({&x, &w_in, &w_out, &b_in, &b_out, &residual}))
+        return GatedFeedForwardNode::apply(x, w_in, w_out, as_opt(b_in), as_opt(b_out), as_opt(residual), act);
+    return GatedFeedForward_forward(x, w_in, w_out, b_in, b_out, residual, act);
 }
 
 }  // namespace laplace

@@ -134,5 +134,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           },
           "GatedFeedForward_backward (dy, x, w_in, w_out, b_in, activation, need_x, need_w_in, need_w_out, need_b_in, "
           "need_b_out) -> (dx, dw_in, dw_out, db_in, db_out)");
+    m.def("RmsNorm",
+          [=](const at::Tensor& x, const at::Tensor& w, const T& r, double eps) {
+              auto [y, s] = RmsNorm(x, w, t(r), eps);
+              return std::make_tuple(y, o(s));
+          },
+          "RmsNorm (x, weight, residual, eps) -> (y, s), with autograd");
+    m.def("Linear",
+          [=](const at::Tensor& x, const at::Tensor& w, const T& b, const T& r, int64_t act) { return Linear(x, w, t(b), t(r), act); },
+          "Linear (x, weight, bias, residual, activation) -> y, with autograd");
+    m.def("GatedFeedForward",
+          [=](const at::Tensor& x, const at::Tensor& wi, const at::Tensor& wo, const T& bi, const T& bo, const T& r,
+              int64_t act) { return GatedFeedForward(x, wi, wo, t(bi), t(bo), t(r), act); },
+          "GatedFeedForward (x, w_in, w_out, b_in, b_out, residual, activation) -> y, with autograd");
     m.def("ClipGradNorm", &ClipGradNorm, "ClipGradNorm (grads, outs, max_norm) -> norm");
 }

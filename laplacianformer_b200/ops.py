@@ -11,7 +11,8 @@ These wrappers give that composition:
   analytic ``-V^T G V^T`` (src/NewtonInverse_cuda_kernel.cu:466-573).
 
 The rest of a transformer block (the reference has none of it): :func:`rms_norm`,
-:func:`linear` and :func:`gated_feed_forward` with their backward passes,
+:func:`linear` and :func:`gated_feed_forward` with their backward passes (autograd
+nodes of the extension),
 :func:`rms_norm_quant`, :func:`quantize_rows` and :func:`linear_quant` for
 serving with 8-bit operands, and :func:`clip_grad_norm`.
 
@@ -184,67 +185,25 @@ def _act(name: str) -> int:
         raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
 
 
-def _tracked(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class RmsNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        y, s, rstd = ext().RmsNorm_forward(x, weight, residual, eps, True)
-        ctx.save_for_backward(x if s is None else s, rstd, weight)
-        ctx.set_materialize_grads(False)
-        return y, s
-
-    @staticmethod
-    def backward(ctx, dy, ds):
-        s, rstd, weight = ctx.saved_tensors
-        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
-        if dy is None:  # only the sum was used: its gradient passes through
-            return ds, None, ds if ctx.needs_input_grad[2] else None, None
-        dx, dw = ext().RmsNorm_backward(dy, ds, s, rstd, weight, need_x, ctx.needs_input_grad[1])
-        return dx, dw, dx if ctx.needs_input_grad[2] else None, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension, s = x + residual.
 
     Returns y, or (y, s) when a residual is given (s continues the residual
     stream).  fp32, fp16 and bf16; statistics in fp32."""
-    if _tracked(x, weight, residual):
-        y, s = RmsNormFn.apply(x, weight, residual, float(eps))
-    else:
-        y, s, _ = ext().RmsNorm_forward(x, weight, residual, float(eps), False)
+    y, s = ext().RmsNorm(x, weight, residual, eps)
     return y if residual is None else (y, s)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
     """:func:`rms_norm` with its output in 8 bits, for :func:`linear_quant`: (q, scale), or (q, scale, s) with a
     residual; y is about q * scale, q float8_e4m3fn, one fp32 scale per row (max|y| / 448).  No gradient."""
-    q, scale, s = ext().RmsNorm_quant_forward(x, weight, residual, float(eps))
+    q, scale, s = ext().RmsNorm_quant_forward(x, weight, residual, eps)
     return (q, scale) if residual is None else (q, scale, s)
 
 
 def quantize_rows(x: torch.Tensor):
     """(q, scale) with x about q * scale, q float8_e4m3fn and one fp32 scale per row (weights for :func:`linear_quant`)."""
     return ext().Quantize_rows(x)
-
-
-class LinearFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        ctx.save_for_backward(x, weight, bias)
-        ctx.act = act
-        return ext().Linear_forward(x, weight, bias, residual, act)
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors
-        nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if nx or nw or nb:
-            dx, dw, db = ext().Linear_backward(dy, x, weight, bias, ctx.act, nx, nw, nb)
-        return dx, dw, db, dy if nr else None, None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
@@ -254,10 +213,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     x [..., K] (rows may be strided), weight [N, K] as torch.nn.Linear keeps it,
     bias [N], residual [..., N].  activation: none, relu, gelu, gelu_tanh or
     silu; the backward recomputes the pre-activation instead of keeping it."""
-    act = _act(activation)
-    if _tracked(x, weight, bias, residual):
-        return LinearFn.apply(x, weight, bias, residual, act)
-    return ext().Linear_forward(x, weight, bias, residual, act)
+    return ext().Linear(x, weight, bias, residual, _act(activation))
 
 
 def linear_quant(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -271,23 +227,6 @@ def linear_quant(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, wei
                                       dtype == torch.bfloat16)
 
 
-class GatedFeedForwardFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_in, w_out, b_in, b_out, residual, act):
-        ctx.save_for_backward(x, w_in, w_out, b_in)
-        ctx.act = act
-        return ext().GatedFeedForward_forward(x, w_in, w_out, b_in, b_out, residual, act)
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, w_in, w_out, b_in = ctx.saved_tensors
-        needs, nr = ctx.needs_input_grad[:5], ctx.needs_input_grad[5]
-        grads = (None,) * 5
-        if any(needs):
-            grads = ext().GatedFeedForward_backward(dy, x, w_in, w_out, b_in, ctx.act, *needs)
-        return *grads, dy if nr else None, None
-
-
 def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: torch.Tensor | None = None,
                        b_out: torch.Tensor | None = None, activation: str = "silu",
                        residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -296,10 +235,7 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
     x [..., C], w_in [2F, C] (gate rows, then up rows), w_out [C, F].  Both
     projections, the activation and the product run in one kernel; between the
     passes only x is kept, the backward recomputes the projections."""
-    act = _act(activation)
-    if _tracked(x, w_in, w_out, b_in, b_out, residual):
-        return GatedFeedForwardFn.apply(x, w_in, w_out, b_in, b_out, residual, act)
-    return ext().GatedFeedForward_forward(x, w_in, w_out, b_in, b_out, residual, act)
+    return ext().GatedFeedForward(x, w_in, w_out, b_in, b_out, residual, _act(activation))
 
 
 def clip_grad_norm(grads, max_norm: float, out=None):
