@@ -179,7 +179,7 @@ struct Epilogue {
     int64_t ldo, ldr;
     int act;
     bool act_bwd, vec_out, vec_res;
-    bool vec16;              // the product kernel may write whole 16-byte chunks (set by run_product)
+    bool tma;                // the output's rows can be written by TMA (set by run_product)
 };
 
 template <int ACT>
@@ -208,7 +208,9 @@ constexpr int kEpiWarps = 16;             // four per 32-lane quarter of the ten
 constexpr int kControlWarps = 3;          // copies of A, products, copies of B
 constexpr int kGemmThreads = 32 * (kControlWarps + kEpiWarps);
 constexpr int kStageOut = 2048;           // output staging per epilogue warp: 32 rows of 64 bytes
-constexpr int kColumnBytes = 128;         // and an fp32 value for each of 32 columns
+// and the values of 32 columns: two 16-bit biases, or one and an fp32 scale
+template <bool FP8>
+constexpr int column_bytes() { return FP8 ? 256 : 128; }
 constexpr int kEpiCols = kEpiWarps / 4 * 32;  // columns that the epilogue warps read at a time
 constexpr int kMaxStages = 8;
 constexpr int kTmemAll = 512;
@@ -228,10 +230,10 @@ struct Divisor {
 };
 
 struct alignas(64) GemmArgs {
-    CUtensorMap a, b, a2, b2;  // a2, b2: dy and Wout of the gated backward
+    CUtensorMap a, b, a2, b2, out;  // a2, b2: dy and Wout of the gated backward
     Epilogue e;
     float* part;               // split K: raw sums [split][rows][ldp]
-    int64_t ldp, plane;        // plane: elements between dg, du and h (gated backward)
+    int64_t ldp;
     int m, n;                  // rows of one row segment; output columns (hidden columns of the gated modes)
     int msegs, tiles_m, tiles_n, splits;
     Divisor per_split, per_group, per_seg, group_rows, last_rows;  // tiles; row tiles of a whole and of the last group
@@ -262,6 +264,12 @@ __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint
                 smem_u32(dst)),
             "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
             : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, const void* src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)),
+                 "r"(x), "r"(y), "r"(z)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 __device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
@@ -375,13 +383,12 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out,
 }
 
 // Staging of one warp: 32 rows of 64 bytes in shared memory whose 16-byte
-// chunks are swizzled so that neither a lane per row nor four lanes per row
-// meet bank conflicts.
+// chunks are swizzled as TMA's 64-byte swizzle does, so that neither a lane per
+// row nor four lanes per row meet bank conflicts.
 __device__ __forceinline__ uint8_t* stage_at(uint8_t* st, int row, int chunk) {
     return st + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
-// Columns 16 half .. of the calling lane's row: in as 16-bit values, whole
-// 64-byte row segments out.
+// Columns 16 half .. of the calling lane's row, as 16-bit values.
 template <typename T>
 __device__ __forceinline__ void pack16(uint4 (&u)[2], const float (&v)[16]) {
 #pragma unroll
@@ -393,22 +400,24 @@ __device__ __forceinline__ void stage16(uint8_t* st, int lane, int half, const u
 #pragma unroll
     for (int c = 0; c < 2; ++c) *reinterpret_cast<uint4*>(stage_at(st, lane, half * 2 + c)) = u[c];
 }
-// out: row 0 of the warp's rows, of which `rows` exist; ld and col0 are multiples of 8.
+// Adds 16 column values to a row's.
 template <typename T>
-__device__ __forceinline__ void unstage16(uint8_t* st, int lane, T* out, int64_t ld, int rows, int col0) {
-    const int c = lane & 3;
-    if (col0 + c * 8 >= ld) return;
-    T* o = out + (lane >> 2) * ld + col0 + c * 8;
+__device__ __forceinline__ void add_columns(float (&v)[16], const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i, o += 8 * ld) {
-        const int row = i * 8 + (lane >> 2);
-        if (row < rows) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(stage_at(st, row, c));
+    for (int c = 0; c < 2; ++c) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[c];
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 x = unpack2<T>(w[k]);
+            v[8 * c + 2 * k] += x.x, v[8 * c + 2 * k + 1] += x.y;
+        }
     }
 }
 
 template <typename T>
-__device__ __forceinline__ float column_value(const T* p, int col, int n) {
-    return p && col < n ? Elem<T>::load(p[col]) : 0.f;
+__device__ __forceinline__ T column_value(const T* p, int col, int n) {
+    return p && col < n ? p[col] : Elem<T>::store(0.f);
 }
 
 // A CTA (CTAS = 1) or a pair of CTAs on two SMs (CTAS = 2) walks tiles of
@@ -427,7 +436,7 @@ template <typename T, int MODE, bool FP8, int CTAS>
 __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];  // stages, output staging, barriers
     uint8_t* out_stage = smem + p.stages * p.stage_bytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * (kStageOut + kColumnBytes));
+    uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * (kStageOut + column_bytes<FP8>()));
     uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *dempty = tempty + 2, *drain = dempty + 2;
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -559,7 +568,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     } else {
         const int ew = warp - kControlWarps, quad = warp & 3, cg = ew >> 2;  // lanes of the tensor memory, columns of a tile
         uint8_t* st = out_stage + ew * kStageOut;
-        float* cv = reinterpret_cast<float*>(out_stage + kEpiWarps * kStageOut + ew * kColumnBytes);
+        T* cv = reinterpret_cast<T*>(out_stage + kEpiWarps * kStageOut + ew * column_bytes<FP8>());
+        float* cs = reinterpret_cast<float*>(cv + 64);
+        // Writes the staged 32x32 outputs by TMA, and waits until they may be overwritten.
+        auto put = [&](int col, int row, int plane, bool some) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && some) tma_store(&p.out, st, col, row, plane);
+        };
+        auto reuse = [&] {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+        };
         int buf = 0;
         uint32_t bph = 0;
         const Epilogue& e = p.e;
@@ -586,11 +606,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 const uint32_t acc = tmem + buf * 256 + lanes;
                 const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
                 const int first = cg * 32;
-                if (e.vec16) {
-                    // Whole 16-byte chunks: finished in the accumulator's
-                    // layout (a lane owns a row); column values and the
-                    // residual of the next columns are fetched ahead.
-                    float bias, sb = 1.f;
+                if (e.tma) {
+                    // Finished in the accumulator's layout (a lane owns a
+                    // row); the column values and the residual of the next
+                    // columns are fetched ahead.
+                    T bias;
+                    float sb = 1.f;
                     uint4 r[4];
                     auto fetch = [&](int c0) {
                         const int col = t.n0 + c0 + lane, col8 = t.n0 + c0 + (lane & 3) * 8;
@@ -606,15 +627,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                     if (!(ok = mbar_wait(tf, bph))) break;
                     tc_fence_after();
                     for (int c0 = first; c0 < cend; c0 += kEpiCols) {
-                        if (FP8 || e.bias) {
-                            cv[lane] = bias;
-                            __syncwarp();
-                        }
+                        reuse();
+                        if (e.bias) cv[lane] = bias;
+                        if (FP8) cs[lane] = sb;
                         if (e.res) {  // to the lane that owns the row
 #pragma unroll
                             for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
-                            __syncwarp();
                         }
+                        fetch(c0 + kEpiCols);
+                        __syncwarp();
                         uint4 o[2][2];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -625,11 +646,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                             if (h == 1 && c0 == last) release(&tempty[buf]);
                             if (FP8) {
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] = __fmaf_rn(v[j], sa * __shfl_sync(0xffffffffu, sb, h * 16 + j), cv[h * 16 + j]);
-                            } else if (e.bias) {
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] += cv[h * 16 + j];
+                                for (int j = 0; j < 16; ++j) v[j] *= sa * cs[h * 16 + j];
                             }
+                            if (e.bias) add_columns(v, cv + h * 16);
                             if (e.act != LF_ACT_NONE)
                                 with_act(e.act, [&](auto act) {
 #pragma unroll
@@ -659,10 +678,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         __syncwarp();
                         stage16(st, lane, 0, o[0]);
                         stage16(st, lane, 1, o[1]);
-                        fetch(c0 + kEpiCols);
-                        __syncwarp();
-                        unstage16(st, lane, (T*)e.out + row0 * e.ldo, e.ldo, rows, t.n0 + c0);
-                        __syncwarp();
+                        put(t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
                     }
                 } else {
                     // Any alignment, and split-K partials: raw sums through
@@ -726,14 +742,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             } else {
                 const T* bias = (const T*)e.bias;
                 const uint32_t acc = tmem + (MODE == kGated ? buf * 256 : 0) + lanes;
-                T* out = (T*)e.out + row0 * e.ldo;
                 const int c0 = cg * 32;                                        // the warp's only columns
-                const float bg = column_value(bias, t.n0 + c0 + lane, p.n);
-                const float bu = column_value(bias ? bias + p.n : bias, t.n0 + c0 + lane, p.n);
+                const T bg = column_value(bias, t.n0 + c0 + lane, p.n);
+                const T bu = column_value(bias ? bias + p.n : bias, t.n0 + c0 + lane, p.n);
                 if (!(ok = mbar_wait(tf, bph))) break;
                 tc_fence_after();
+                reuse();
                 if (bias) {
-                    cv[lane] = bg;
+                    cv[lane] = bg, cv[32 + lane] = bu;
                     __syncwarp();
                 }
                 // 16 columns at a time; outputs wait as 16-bit pairs.
@@ -749,10 +765,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         reg_fence(g);
                         reg_fence(u);
                         if (h == 1) release(&tempty[buf]);
-                        if (bias) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) g[j] += cv[h * 16 + j], u[j] += __shfl_sync(0xffffffffu, bu, h * 16 + j);
-                        }
+                        if (bias) add_columns(g, cv + h * 16), add_columns(u, cv + 32 + h * 16);
                         with_act(e.act, [&](auto act) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
@@ -766,10 +779,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         reg_fence(u);
                         reg_fence(d);
                         if (h == 1) release(&tempty[0]), release(&dempty[buf]);
-                        if (bias) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) g[j] += cv[h * 16 + j], u[j] += __shfl_sync(0xffffffffu, bu, h * 16 + j);
-                        }
+                        if (bias) add_columns(g, cv + h * 16), add_columns(u, cv + 32 + h * 16);
                         // h = act(g) u, du = dh act(g), dg = dh u act'(g), in d, g and u
                         with_act(e.act, [&](auto act) {
 #pragma unroll
@@ -789,25 +799,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         stage16(st, lane, h, oh);
                     }
                 }
-                if constexpr (MODE == kGatedBwd) {
-                    __syncwarp();
-                    unstage16(st, lane, out + 2 * p.plane, e.ldo, rows, t.n0 + c0);
-                    __syncwarp();
+                const int row = t.m0 + quad * 32;
+                if constexpr (MODE == kGatedBwd) {  // planes dg, du, h
+                    put(t.n0 + c0, row, 2, rows > 0);
+                    reuse();
                     stage16(st, lane, 0, og[0]);
                     stage16(st, lane, 1, og[1]);
-                    __syncwarp();
-                    unstage16(st, lane, out + p.plane, e.ldo, rows, t.n0 + c0);
+                    put(t.n0 + c0, row, 1, rows > 0);
+                    reuse();
                 }
-                __syncwarp();
                 stage16(st, lane, 0, ou[0]);
                 stage16(st, lane, 1, ou[1]);
-                __syncwarp();
-                unstage16(st, lane, out, e.ldo, rows, t.n0 + c0);
-                __syncwarp();
+                put(t.n0 + c0, row, 0, rows > 0);
             }
             buf ^= 1;
             if (MODE == kGatedBwd || buf == 0) bph ^= 1;
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // outputs written, staging read
     }
     if (!ok && lane == 0) atomicExch(&g_gemm_status, (int)LF_ERR_TIMEOUT);
     tc_fence_before();
@@ -1049,7 +1057,8 @@ struct Mat {
     int64_t inner = 0, rows = 0, ld = 0, planes = 1, plane = 0;
 };
 
-bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_rows) {
+bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_rows,
+            CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     const int es = dtype == LF_F8E4M3 ? 1 : 2;
     const CUtensorMapDataType ty = dtype == LF_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                    : dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -1063,7 +1072,7 @@ bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_ro
     }
     auto call = [&] {
         return fn(map, ty, 3, const_cast<void*>(a.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
     CUresult r = call();
     if (r == CUDA_ERROR_INVALID_CONTEXT) {  // the first call of a host thread (an autograd worker): bind the device's context
@@ -1073,6 +1082,11 @@ bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_ro
     if (r != CUDA_SUCCESS) set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
     return r == CUDA_SUCCESS;
 }
+
+bool encode_out(CUtensorMap* map, const Mat& a, int dtype) { return encode(map, a, dtype, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B); }
+
+// Whether TMA can address rows of ld elements of es bytes at p.
+bool tma_ok(const void* p, int64_t ld, int es) { return aligned(p, 16) && ld * es % 16 == 0; }
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -1141,7 +1155,7 @@ uint32_t idesc_of(int dtype, bool a_mn, bool b_mn, int ctas, int n) {
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kBM * ctas >> 4) << 24);
 }
 
-template <auto Kernel>
+template <auto Kernel, bool FP8>
 int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
     const int row_tiles = g.msegs * g.tiles_m, group = std::min(row_tiles, kGroupRows / (kBM * ctas));
     g.per_split = Divisor(row_tiles * g.tiles_n);
@@ -1149,7 +1163,7 @@ int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
     g.per_seg = Divisor(g.tiles_m);
     g.group_rows = Divisor(group);
     g.last_rows = Divisor(row_tiles % group ? row_tiles % group : group);
-    constexpr int rest = kEpiWarps * (kStageOut + kColumnBytes) + kBarrierBytes;
+    constexpr int rest = kEpiWarps * (kStageOut + column_bytes<FP8>()) + kBarrierBytes;
     g.stages = std::min(kMaxStages, (kSmemLimit - rest) / g.stage_bytes);
     static std::once_flag once[64];  // per kernel and device
     int dev = 0;
@@ -1163,7 +1177,7 @@ int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
 
 template <typename T, int MODE, bool FP8>
 int launch_ctas(GemmArgs& g, int ctas, cudaStream_t st) {
-    return ctas == 2 ? launch_gemm<tc_gemm_kernel<T, MODE, FP8, 2>>(g, 2, st) : launch_gemm<tc_gemm_kernel<T, MODE, FP8, 1>>(g, 1, st);
+    return ctas == 2 ? launch_gemm<tc_gemm_kernel<T, MODE, FP8, 2>, FP8>(g, 2, st) : launch_gemm<tc_gemm_kernel<T, MODE, FP8, 1>, FP8>(g, 1, st);
 }
 
 int too_large(const char* what) {
@@ -1202,8 +1216,8 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
     g.a_mn = q.a_mn, g.b_mn = q.b_mn;
     g.idesc = idesc_of(q.op_dtype, q.a_mn, q.b_mn, s.ctas, s.bn);
     g.e = q.e;
-    g.e.vec16 = !part && q.n % 8 == 0 && q.e.ldo % 8 == 0 && aligned(q.e.out, 16) &&
-                (!q.e.res || (q.e.ldr % 8 == 0 && aligned(q.e.res, 16)));
+    g.e.tma = !part && tma_ok(q.e.out, q.e.ldo, 2) && (!q.e.res || (q.n % 8 == 0 && tma_ok(q.e.res, q.e.ldr, 2)));
+    if (g.e.tma && !encode_out(&g.out, {q.e.out, q.n, q.m, q.e.ldo, q.msegs, q.m * q.e.ldo}, q.dtype)) return LF_ERR_CUDA;
     g.part = part;
     g.ldp = up(q.n, 4);
     if (!encode(&g.a, q.a, q.op_dtype, q.a_mn ? 64 : bk, q.a_mn ? bk : kBM)) return LF_ERR_CUDA;
@@ -1217,8 +1231,6 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
 }
 
 // A dense operand as TMA can read it: itself, or a copy with padded rows.
-bool tma_ok(const void* p, int64_t ld, int es) { return aligned(p, 16) && ld * es % 16 == 0; }
-
 Mat operand(const void* p, int64_t rows, int64_t cols, int64_t ld, int es, Arena& ws, cudaStream_t st) {
     if (rows == 0 || cols == 0 || tma_ok(p, ld, es)) return {p, cols, rows, ld, 1, 0};
     const int64_t ldo = up(cols, 16 / es);
@@ -1474,7 +1486,7 @@ int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* 
     g.idesc = idesc_of(a->dtype, false, false, s.ctas, s.bn);
     g.idesc2 = idesc_of(a->dtype, false, true, s.ctas, bh);
     g.e.out = out, g.e.ldo = ldo, g.e.bias = a->b_in, g.e.act = a->activation;
-    g.plane = plane;
+    if (!encode_out(&g.out, {out, a->f, a->m, ldo, bwd ? 3 : 1, plane}, a->dtype)) return LF_ERR_CUDA;
     if (!encode(&g.a, x, a->dtype, 64, kBM) || !encode(&g.b, gate_up(win, a->f), a->dtype, 64, bh)) return LF_ERR_CUDA;
     if (bwd && (!encode(&g.a2, *dy, a->dtype, 64, kBM) || !encode(&g.b2, *wout, a->dtype, 64, 64))) return LF_ERR_CUDA;
     if (bwd)
