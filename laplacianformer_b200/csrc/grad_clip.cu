@@ -2,7 +2,9 @@
 //   n = sqrt(sum over all tensors of g^2),  c = min(1, max_norm / (n + 1e-6)),  out = c g
 //
 // Two kernels over equal chunks of the tensors (their table travels in the
-// launch parameters, so nothing is copied to the device beforehand).  The
+// launch parameters, so nothing is copied to the device beforehand; up to 96
+// tensors in 2.8 KB, up to 512 in 15 KB, which costs the host 4 us more per
+// launch).  The
 // first writes one fp64 partial sum of squares per chunk; in the second every
 // block adds the partials in the same order, so each has the same
 // coefficient without another launch, and scales its chunks, last chunk
@@ -13,15 +15,16 @@
 namespace lfb {
 namespace {
 
-constexpr int kMaxTensors = 512;  // per launch: the table stays under the 32 KB of launch parameters
+constexpr int kFewTensors = 96, kMaxTensors = 512;  // per launch
 constexpr int kThreads = 256;
 
+template <int N>
 struct Table {
-    const void* in[kMaxTensors];
-    void* out[kMaxTensors];
-    int64_t n[kMaxTensors];
-    int first[kMaxTensors + 1];  // first chunk of each tensor within this launch
-    uint8_t dtype[kMaxTensors];
+    const void* in[N];
+    void* out[N];
+    int64_t n[N];
+    int first[N + 1];  // first chunk of each tensor within this launch
+    uint8_t dtype[N];
     int count, chunk;  // tensors; elements per chunk
     int base, total;   // first chunk of this launch among all; chunks of all launches
 };
@@ -100,7 +103,8 @@ __device__ __forceinline__ void scale_to(const T* p, T* o, int64_t n, float c) {
 
 // Tensor that holds chunk k: the last one whose first chunk is <= k (tensors
 // without elements have no chunk and are passed over).
-__device__ __forceinline__ int tensor_of(const Table& t, int k) {
+template <int N>
+__device__ __forceinline__ int tensor_of(const Table<N>& t, int k) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -123,7 +127,8 @@ __device__ __forceinline__ V block_sum(V v, V* sh) {
     return v;
 }
 
-__global__ void __launch_bounds__(kThreads) grad_sq_kernel(const __grid_constant__ Table t, double* part) {
+template <int N>
+__global__ void __launch_bounds__(kThreads) grad_sq_kernel(const __grid_constant__ Table<N> t, double* part) {
     __shared__ double sh[kThreads / 32];
     grid_release();
     grid_wait();
@@ -141,7 +146,8 @@ __global__ void __launch_bounds__(kThreads) grad_sq_kernel(const __grid_constant
     }
 }
 
-__global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_constant__ Table t, const double* part,
+template <int N>
+__global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_constant__ Table<N> t, const double* part,
                                                               float max_norm, float* norm) {
     __shared__ double sh[kThreads / 32];
     grid_release();
@@ -178,6 +184,41 @@ int64_t chunks_of(const int64_t* sizes, int64_t count, int chunk) {
     int64_t k = 0;
     for (int64_t i = 0; i < count; ++i) k += (sizes[i] + chunk - 1) / chunk;
     return k;
+}
+
+template <int N>
+int run_clip(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes, int64_t count, int chunk,
+             int total, float max_norm, float* norm, double* part, cudaStream_t st) {
+    // All sums before the first scaling: a launch scales what it summed last.
+    for (int pass = 0; pass < 2; ++pass) {
+        int64_t i = 0;
+        int base = 0;
+        do {
+            static thread_local Table<N> t;
+            t.chunk = chunk;
+            t.base = base;
+            t.total = total;
+            t.count = 0;
+            t.first[0] = 0;
+            for (; i < count && t.count < N; ++i) {
+                if (sizes[i] == 0) continue;
+                const int j = t.count++;
+                t.in[j] = grads[i];
+                t.out[j] = outs[i];
+                t.n[j] = sizes[i];
+                t.dtype[j] = (uint8_t)dtypes[i];
+                t.first[j + 1] = t.first[j] + (int)((sizes[i] + chunk - 1) / chunk);
+            }
+            const int chunks = t.first[t.count];
+            base += chunks;
+            const int slots = 8 * num_sms();
+            const unsigned grid = (unsigned)(chunks < 1 ? 1 : chunks < slots ? chunks : slots);
+            if (pass == 0) launch_early(grad_sq_kernel<N>, grid, kThreads, 0, 1, st, t, part);
+            else launch_early(grad_scale_kernel<N>, grid, kThreads, 0, 1, st, t, (const double*)part, max_norm, norm);
+            if (int rc = check_launch("lf_clip_grad_norm")) return rc;
+        } while (i < count);
+    }
+    return LF_OK;
 }
 
 }  // namespace
@@ -222,34 +263,6 @@ extern "C" int lf_clip_grad_norm(const void* const* grads, void* const* outs, co
         set_error("lf_clip_grad_norm: too many elements");
         return LF_ERR_UNSUPPORTED;
     }
-    // All sums before the first scaling: a launch scales what it summed last.
-    for (int pass = 0; pass < 2; ++pass) {
-        int64_t i = 0;
-        int base = 0;
-        do {
-            static thread_local Table t;
-            t.chunk = chunk;
-            t.base = base;
-            t.total = (int)total;
-            t.count = 0;
-            t.first[0] = 0;
-            for (; i < count && t.count < kMaxTensors; ++i) {
-                if (sizes[i] == 0) continue;
-                const int j = t.count++;
-                t.in[j] = grads[i];
-                t.out[j] = outs[i];
-                t.n[j] = sizes[i];
-                t.dtype[j] = (uint8_t)dtypes[i];
-                t.first[j + 1] = t.first[j] + (int)((sizes[i] + chunk - 1) / chunk);
-            }
-            const int chunks = t.first[t.count];
-            base += chunks;
-            const int slots = 8 * num_sms();
-            const unsigned grid = (unsigned)(chunks < 1 ? 1 : chunks < slots ? chunks : slots);
-            if (pass == 0) launch_early(grad_sq_kernel, grid, kThreads, 0, 1, st, t, (double*)workspace);
-            else launch_early(grad_scale_kernel, grid, kThreads, 0, 1, st, t, (const double*)workspace, (float)max_norm, norm);
-            if (int rc = check_launch("lf_clip_grad_norm")) return rc;
-        } while (i < count);
-    }
-    return LF_OK;
+    return count <= kFewTensors ? run_clip<kFewTensors>(grads, outs, sizes, dtypes, count, chunk, (int)total, (float)max_norm, norm, (double*)workspace, st)
+                                : run_clip<kMaxTensors>(grads, outs, sizes, dtypes, count, chunk, (int)total, (float)max_norm, norm, (double*)workspace, st);
 }

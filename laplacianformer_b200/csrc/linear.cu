@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     if (warp == 1) tmem_free<CTAS>(tmem);
 }
 
-// Joins the splits of K in order and applies the epilogue.
+// Joins the splits of K in order (eight loads in flight) and applies the epilogue.
 template <typename T>
 __global__ void __launch_bounds__(256) split_join_kernel(const float* part, int splits, int64_t rows, int n, int64_t ldp,
                                                          const Epilogue e) {
@@ -836,6 +836,7 @@ __global__ void __launch_bounds__(256) split_join_kernel(const float* part, int 
         const int64_t row = i / groups;
         const int col = (int)(i - row * groups) * 4;
         float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
         for (int s = 0; s < splits; ++s) {
             const float4 v = *reinterpret_cast<const float4*>(part + ((int64_t)s * rows + row) * ldp + col);
             z.x += v.x, z.y += v.y, z.z += v.z, z.w += v.w;
