@@ -229,7 +229,8 @@ struct Divisor {
     __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
 };
 
-struct alignas(64) GemmArgs {
+// One product out of up to N that a launch runs.
+struct alignas(64) Problem {
     CUtensorMap a, b, a2, b2, out;  // a2, b2: dy and Wout of the gated backward
     Epilogue e;
     float* part;               // split K: raw sums [split][rows][ldp]
@@ -238,10 +239,42 @@ struct alignas(64) GemmArgs {
     int msegs, tiles_m, tiles_n, splits;
     Divisor per_split, per_group, per_seg, group_rows, last_rows;  // tiles; row tiles of a whole and of the last group
     int iters, split_iters, seg_iters;  // K steps in all, per split, per K segment
-    int bn, stages, stage_bytes;        // columns of a tile's (first) product; ring depth
+    int bn;                    // columns of a tile's (first) product
     uint32_t idesc, idesc2;
     bool a_mn, b_mn;
 };
+
+template <int N>
+struct GemmArgs {
+    Problem p[N];
+    int first[N + 1];          // first work unit of each problem; first[N] units in all
+    // Units go to the CTAs (or pairs) in turn.  The last problem's units may be
+    // shorter than the others' (`longer` of them): the CTAs that got one long
+    // unit fewer take `extra` of them each before the turns go on.
+    int longer, extra;
+    int stages, stage_bytes;
+};
+
+// The k-th unit of CTA (or pair) c of P; first[N] or more: none left.
+template <int N>
+__device__ __forceinline__ int unit_of(const GemmArgs<N>& a, int c, int P, int k) {
+    if constexpr (N == 1) return c + k * P;
+    const int longer = a.longer, have = longer > c ? (longer - c + P - 1) / P : 0;
+    if (k < have) return c + k * P;
+    const int j = k - have, ahead = longer % P, behind = P - ahead;
+    if (c >= ahead) return j < a.extra ? longer + j * behind + c - ahead : longer + a.extra * behind + c + (j - a.extra) * P;
+    return longer + a.extra * behind + c + j * P;
+}
+template <int N>
+__device__ __forceinline__ int problem_of(const GemmArgs<N>& a, int& unit) {
+    int i = 0;
+    if constexpr (N > 1) {
+#pragma unroll
+        for (int j = 1; j < N; ++j) i += unit >= a.first[j] ? 1 : 0;
+        unit -= a.first[i];
+    }
+    return i;
+}
 
 __device__ __forceinline__ uint32_t leader_addr(const void* p) {  // the same shared memory in CTA 0 of the cluster
     uint32_t r;
@@ -365,7 +398,7 @@ __device__ __forceinline__ Step gated_step(int i, int n) {
 // Work units: for each split of K, row tiles in groups of kGroupRows, within a
 // group all row tiles of one column tile before the next column tile.
 template <int CTAS>
-__device__ __forceinline__ Tile tile_of(const GemmArgs& p, int unit, int bn_out, int rank) {
+__device__ __forceinline__ Tile tile_of(const Problem& p, int unit, int bn_out, int rank) {
     Tile t;
     t.split = p.per_split.of(unit);
     int r = unit - t.split * (int)p.per_split.d;
@@ -432,10 +465,10 @@ __device__ __forceinline__ T column_value(const T* p, int col, int n) {
 // [g|u] = x Win^T at 0.  The epilogue takes all of a tile's g and u into
 // registers at once, while the next tile's dh is computed, so that neither
 // product waits for outputs.
-template <typename T, int MODE, bool FP8, int CTAS>
-__global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs p) {
+template <typename T, int MODE, bool FP8, int CTAS, int N>
+__global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs<N> args) {
     extern __shared__ __align__(1024) uint8_t smem[];  // stages, output staging, barriers
-    uint8_t* out_stage = smem + p.stages * p.stage_bytes;
+    uint8_t* out_stage = smem + args.stages * args.stage_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * (kStageOut + column_bytes<FP8>()));
     uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *dempty = tempty + 2, *drain = dempty + 2;
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
@@ -444,13 +477,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     constexpr int BK = FP8 ? 128 : 64;
     constexpr int kABytes = kBM * kRowBytes;
     constexpr int kDh = 256;                                   // tensor memory columns of dh
-    const int bh = p.bn / 2;                                   // hidden columns of a gated tile
-    const int bn_out = MODE == kLinear ? p.bn : bh;
     const int phases = MODE == kGatedBwd ? 2 : 1;
 
     grid_release();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 2), mbar_init(&empty[i], 1);
+        for (int i = 0; i < args.stages; ++i) mbar_init(&full[i], 2), mbar_init(&empty[i], 1);
         for (int i = 0; i < 2; ++i)
             mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps * CTAS), mbar_init(&dempty[i], kEpiWarps * CTAS);
         mbar_init(drain, 1);
@@ -463,8 +494,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     tc_fence_after();
     grid_wait();
     const uint32_t tmem = *tmem_ptr;
-    const int units = p.splits * p.msegs * p.tiles_m * p.tiles_n;
-    const int unit0 = blockIdx.x / CTAS, unit_step = gridDim.x / CTAS;
+    const int cta = blockIdx.x / CTAS, ctas = gridDim.x / CTAS;
+    // One work unit after another, in the same order in every role.
+#define LFB_EACH_UNIT(OK)                                                                                        \
+    for (int turn = 0, unit; OK && (unit = unit_of(args, cta, ctas, turn)) < args.first[N]; ++turn)
+#define LFB_PROBLEM(RANK)                                                                                        \
+    const Problem& p = args.p[problem_of(args, unit)];                                                           \
+    const int bh = p.bn / 2; /* hidden columns of a gated tile */                                                \
+    const int bn_out = MODE == kLinear ? p.bn : bh;                                                              \
+    const Tile t = tile_of<CTAS>(p, unit, bn_out, RANK)
     bool ok = true;
 
     if (warp == 0 || warp == 2) {
@@ -474,17 +512,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
         if (elect_one()) {
             int s = 0, issued = 0;
             uint32_t ph = 0;
-            const int bw = p.bn / CTAS;                        // B rows that this CTA holds
             const uint32_t bars = CTAS == 2 ? leader_addr(full) : smem_u32(full);
-            for (int unit = unit0; ok && unit < units; unit += unit_step) {
-                const Tile t = tile_of<CTAS>(p, unit, bn_out, rank);
+            LFB_EACH_UNIT(ok) {
+                LFB_PROBLEM(rank);
+                const int bw = p.bn / CTAS;                    // B rows that this CTA holds
                 const int steps = (t.it1 - t.it0) * phases;
                 int ks = t.it0 / p.seg_iters, in_seg = t.it0 - ks * p.seg_iters;
                 for (int i = 0; i < steps; ++i) {
                     if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
                     const Step step = MODE == kGatedBwd ? gated_step(i, steps / 2) : Step{false, i};
                     const int k0 = (MODE == kLinear ? in_seg : step.it) * BK;
-                    uint8_t* dst = smem + s * p.stage_bytes + (is_a ? 0 : kABytes);
+                    uint8_t* dst = smem + s * args.stage_bytes + (is_a ? 0 : kABytes);
                     const uint32_t bar = bars + 8 * s;
                     if (rank == 0) mbar_expect(&full[s], (is_a ? kABytes : (step.dh ? bh / CTAS : bw) * kRowBytes) * CTAS);
                     if (is_a) {
@@ -506,25 +544,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                     }
                     ++issued;
                     if (MODE == kLinear && ++in_seg == p.seg_iters) in_seg = 0, ++ks;
-                    if (++s == p.stages) s = 0, ph ^= 1;
+                    if (++s == args.stages) s = 0, ph ^= 1;
                 }
             }
             // A wait ran out: let the copies in flight land before the block
             // ends (the leader's barriers count both CTAs' copies).
             if (!ok && rank == 0)
-                for (int k = max(0, issued - p.stages); k < issued; ++k)
-                    mbar_wait(&full[k % p.stages], (k / p.stages) & 1, 100000000ull);
+                for (int k = max(0, issued - args.stages); k < issued; ++k)
+                    mbar_wait(&full[k % args.stages], (k / args.stages) & 1, 100000000ull);
         }
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t go = elect_one() ? 1u : 0u;
-            const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
-            const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
             int s = 0, buf = 0;
             uint32_t ph = 0, bph = 0, dph = 0;
-            for (int unit = unit0; ok && unit < units; unit += unit_step) {
-                const Tile t = tile_of<CTAS>(p, unit, bn_out, 0);
+            LFB_EACH_UNIT(ok) {
+                LFB_PROBLEM(0);
+                const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16, idesc = p.idesc;
+                const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
                 const int steps = (t.it1 - t.it0) * phases;
                 for (int i = 0; i < steps; ++i) {
                     const Step step = MODE == kGatedBwd ? gated_step(i, steps / 2) : Step{false, i};
@@ -539,7 +577,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                     const uint32_t acc = tmem + (MODE != kGatedBwd ? buf * 256 : dh ? kDh + buf * 128 : 0);
                     if (!(ok = mbar_wait(&full[s], ph))) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * p.stage_bytes), sb = sa + kABytes;
+                    const uint32_t sa = smem_u32(smem + s * args.stage_bytes), sb = sa + kABytes;
                     if (dh) {
                         const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sb, 8192, 1024);
 #pragma unroll
@@ -549,10 +587,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         const uint64_t da = make_desc(sa, a_lbo, 1024), db = make_desc(sb, b_lbo, 1024);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma<CTAS, FP8>(acc, da + k * a_step, db + k * b_step, p.idesc, step.it > 0 || k > 0 ? 1u : 0u, go);
+                            mma<CTAS, FP8>(acc, da + k * a_step, db + k * b_step, idesc, step.it > 0 || k > 0 ? 1u : 0u, go);
                     }
                     if (go) commit<CTAS>(&empty[s]);
-                    if (++s == p.stages) s = 0, ph ^= 1;
+                    if (++s == args.stages) s = 0, ph ^= 1;
                 }
                 if (!ok) break;
                 if (go) commit<CTAS>(&tfull[MODE == kGatedBwd ? 0 : buf]);
@@ -571,10 +609,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
         T* cv = reinterpret_cast<T*>(out_stage + kEpiWarps * kStageOut + ew * column_bytes<FP8>());
         float* cs = reinterpret_cast<float*>(cv + 64);
         // Writes the staged 32x32 outputs by TMA, and waits until they may be overwritten.
-        auto put = [&](int col, int row, int plane, bool some) {
+        auto put = [&](const CUtensorMap* out, int col, int row, int plane, bool some) {
             fence_async_smem();
             __syncwarp();
-            if (lane == 0 && some) tma_store(&p.out, st, col, row, plane);
+            if (lane == 0 && some) tma_store(out, st, col, row, plane);
         };
         auto reuse = [&] {
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -582,9 +620,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
         };
         int buf = 0;
         uint32_t bph = 0;
-        const Epilogue& e = p.e;
-        for (int unit = unit0; unit < units; unit += unit_step) {
-            const Tile t = tile_of<CTAS>(p, unit, bn_out, rank);
+        LFB_EACH_UNIT(true) {
+            LFB_PROBLEM(rank);
+            const Epilogue& e = p.e;
             const uint32_t lanes = (uint32_t)(quad * 32) << 16;
             const int rows = p.m - t.m0 - quad * 32;                           // rows that exist from the warp's first on
             const int64_t row0 = (int64_t)t.seg * p.m + t.m0 + quad * 32;      // in the output
@@ -678,7 +716,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         __syncwarp();
                         stage16(st, lane, 0, o[0]);
                         stage16(st, lane, 1, o[1]);
-                        put(t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
+                        put(&p.out, t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
                     }
                 } else {
                     // Any alignment, and split-K partials: raw sums through
@@ -801,16 +839,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 }
                 const int row = t.m0 + quad * 32;
                 if constexpr (MODE == kGatedBwd) {  // planes dg, du, h
-                    put(t.n0 + c0, row, 2, rows > 0);
+                    put(&p.out, t.n0 + c0, row, 2, rows > 0);
                     reuse();
                     stage16(st, lane, 0, og[0]);
                     stage16(st, lane, 1, og[1]);
-                    put(t.n0 + c0, row, 1, rows > 0);
+                    put(&p.out, t.n0 + c0, row, 1, rows > 0);
                     reuse();
                 }
                 stage16(st, lane, 0, ou[0]);
                 stage16(st, lane, 1, ou[1]);
-                put(t.n0 + c0, row, 0, rows > 0);
+                put(&p.out, t.n0 + c0, row, 0, rows > 0);
             }
             buf ^= 1;
             if (MODE == kGatedBwd || buf == 0) bph ^= 1;
@@ -823,55 +861,85 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     sync_all<CTAS>();  // no CTA of a pair leaves while the other's products read its operands
     tc_fence_after();
     if (warp == 1) tmem_free<CTAS>(tmem);
+#undef LFB_EACH_UNIT
+#undef LFB_PROBLEM
 }
 
-// Joins the splits of K in order (eight loads in flight) and applies the epilogue.
+// Joins the splits of K and applies the epilogue, for up to three products
+// (blockIdx.y).  `walkers` threads share four columns, each adds every
+// walkers-th split, and their sums join in order: a thread for all splits of a
+// small output would wait for one load after another.
+struct JoinJob {
+    const float* part;
+    int64_t rows, ldp;
+    int splits, n, walkers;
+    Epilogue e;
+};
+struct JoinJobs {
+    JoinJob job[3];
+};
 template <typename T>
-__global__ void __launch_bounds__(256) split_join_kernel(const float* part, int splits, int64_t rows, int n, int64_t ldp,
-                                                         const Epilogue e) {
+__global__ void __launch_bounds__(256) split_join_kernel(const __grid_constant__ JoinJobs jobs) {
+    __shared__ float4 sh[256];
     grid_release();
     grid_wait();
-    const int64_t groups = ldp / 4, total = rows * groups;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / groups;
+    const JoinJob& j = jobs.job[blockIdx.y];
+    const Epilogue& e = j.e;
+    const int each = 256 / j.walkers, w = threadIdx.x / each, o = threadIdx.x - w * each;
+    const int64_t groups = j.ldp / 4, total = j.rows * groups;
+    for (int64_t base = (int64_t)blockIdx.x * each; base < total; base += (int64_t)gridDim.x * each) {
+        const int64_t i = base + o, row = i / groups;
         const int col = (int)(i - row * groups) * 4;
         float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int s = 0; s < splits; ++s) {
-            const float4 v = *reinterpret_cast<const float4*>(part + ((int64_t)s * rows + row) * ldp + col);
-            z.x += v.x, z.y += v.y, z.z += v.z, z.w += v.w;
+        if (i < total)
+#pragma unroll 4
+            for (int s = w; s < j.splits; s += j.walkers) {
+                const float4 v = *reinterpret_cast<const float4*>(j.part + ((int64_t)s * j.rows + row) * j.ldp + col);
+                z.x += v.x, z.y += v.y, z.z += v.z, z.w += v.w;
+            }
+        if (j.walkers > 1) {
+            __syncthreads();
+            sh[threadIdx.x] = z;
+            __syncthreads();
+            for (int k = 1; w == 0 && k < j.walkers; ++k) {
+                const float4 v = sh[k * each + o];
+                z.x += v.x, z.y += v.y, z.z += v.z, z.w += v.w;
+            }
         }
+        if (w || i >= total) continue;
         if (e.sa) {
             const float s = e.sa[row];
             float* q = reinterpret_cast<float*>(&z);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] *= s * (col + j < n ? e.sb[col + j] : 0.f);
+            for (int k = 0; k < 4; ++k) q[k] *= s * (col + k < j.n ? e.sb[col + k] : 0.f);
         }
         float4 b = make_float4(0.f, 0.f, 0.f, 0.f), x = b;
-        if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, n, false));
-        if (e.res) x = widen4<T>(load4((const T*)e.res + row * e.ldr, col, n, e.vec_res));
+        if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, j.n, false));
+        if (e.res) x = widen4<T>(load4((const T*)e.res + row * e.ldr, col, j.n, e.vec_res));
         with_act(e.act, [&](auto act) {
-            store4((T*)e.out + row * e.ldo, col, n, e.vec_out, finish4<decltype(act)::value>(z, b, x, e.act_bwd));
+            store4((T*)e.out + row * e.ldo, col, j.n, e.vec_out, finish4<decltype(act)::value>(z, b, x, e.act_bwd));
         });
     }
 }
 
 // Copies a matrix whose rows TMA cannot address (row pitch or base not a
-// multiple of 16 bytes) to rows of ldo elements: a warp per row, 16 bytes of
-// output per lane at a time (its scalar loads share cache lines).
+// multiple of 16 bytes) to rows of ldo elements: 16 bytes of output per lane
+// (whose scalar loads share cache lines).
 template <typename U>
 __global__ void __launch_bounds__(256) pack_rows_kernel(const U* in, int64_t ldi, U* out, int64_t ldo, int64_t rows, int64_t cols) {
     constexpr int V = 16 / sizeof(U);
     grid_release();
     grid_wait();
     const int lane = threadIdx.x & 31;
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8)
-        for (int64_t c = lane * V; c < ldo; c += 32 * V) {
-            U v[V];
+    const int64_t per_row = (ldo + 32 * V - 1) / (32 * V), total = rows * per_row;  // warps' work: a row's next 512 bytes
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += (int64_t)gridDim.x * 8) {
+        const int64_t r = i / per_row, c = ((i - r * per_row) * 32 + lane) * V;
+        if (c >= ldo) continue;
+        U v[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = c + j < cols ? in[r * ldi + c + j] : U(0);
-            *reinterpret_cast<uint4*>(out + r * ldo + c) = *reinterpret_cast<const uint4*>(v);
-        }
+        for (int j = 0; j < V; ++j) v[j] = c + j < cols ? in[r * ldi + c + j] : U(0);
+        *reinterpret_cast<uint4*>(out + r * ldo + c) = *reinterpret_cast<const uint4*>(v);
+    }
 }
 
 // Column sums of up to three matrices in one launch (blockIdx.z).  First step:
@@ -926,8 +994,8 @@ __global__ void __launch_bounds__(256) colsum_kernel(const ColsumJobs p) {
         }
 }
 template <typename T>
-__global__ void __launch_bounds__(512) colsum_join_kernel(const ColsumJobs p) {
-    __shared__ float sh[16][33];
+__global__ void __launch_bounds__(1024) colsum_join_kernel(const ColsumJobs p) {
+    __shared__ float sh[32][33];
     grid_release();
     grid_wait();
     const ColsumJob j = p.job[blockIdx.z];
@@ -936,12 +1004,12 @@ __global__ void __launch_bounds__(512) colsum_join_kernel(const ColsumJobs p) {
     float t = 0.f;
     if (c < j.cols)
 #pragma unroll 4
-        for (int s = w; s < p.slices; s += 16) t += j.part[(int64_t)s * j.cols + c];
+        for (int s = w; s < p.slices; s += 32) t += j.part[(int64_t)s * j.cols + c];
     sh[w][lane] = t;
     __syncthreads();
     if (w == 0 && c < j.cols) {
 #pragma unroll
-        for (int i = 1; i < 16; ++i) t += sh[i][lane];
+        for (int i = 1; i < 32; ++i) t += sh[i][lane];
         ((T*)j.out)[c] = Elem<T>::store(t);
     }
 }
@@ -1146,6 +1214,43 @@ Shape choose(const Product& q) {
     return best;
 }
 
+// The same for several products that share a launch (one CTA count and ring):
+// the widest tile that costs least work for each, and splits where a unit
+// would be longer than a quarter of the whole launch.
+double choose_together(const Product* q, int count, int ctas, Shape* out) {
+    const double lanes = (double)num_sms() / ctas;
+    double work = 0, unit[3] = {}, longest = 0, join = 0;
+    int64_t units[3];
+    auto fill = [&](int i, int bn, int s) {
+        const int64_t iters = (q[i].k + 63) / 64 * q[i].ksegs, per = (iters + s - 1) / s;
+        units[i] = (q[i].m + kBM * ctas - 1) / (kBM * ctas) * q[i].msegs * ((q[i].n + bn - 1) / bn) * ((iters + per - 1) / per);
+        unit[i] = std::max(per * step_cycles(ctas, bn, bn), 500 + bn * 10.0);
+        out[i] = {ctas, bn, s};
+        return units[i] * unit[i];
+    };
+    for (int i = 0; i < count; ++i) {
+        int best = 256;
+        double least = 1e30;
+        for (int bn : {256, 128, 64}) {
+            if (ctas == 2 && bn == 64) continue;
+            const double w = fill(i, bn, 1);
+            if (w < 0.99 * least) least = w, best = bn;
+        }
+        work += fill(i, best, 1);
+    }
+    const double limit = std::max(0.25 * work / lanes, 3000.0);
+    work = 0;
+    for (int i = 0; i < count; ++i) {
+        const int64_t iters = (q[i].k + 63) / 64 * q[i].ksegs;
+        int s = 1;
+        while (unit[i] > limit && s < 64 && iters / (2 * s) >= 4) fill(i, out[i].bn, s *= 2);
+        work += units[i] * unit[i];
+        longest = std::max(longest, unit[i]);
+        if (s > 1) join += (double)s * q[i].m * q[i].msegs * q[i].n * 8 / 3400.0;
+    }
+    return work / lanes + 0.5 * longest + join + (join > 0 ? 4000 : 0);
+}
+
 size_t part_bytes(const Product& q, const Shape& s) {
     return s.splits > 1 ? (size_t)s.splits * q.m * q.msegs * up(q.n, 4) * 4 : 0;
 }
@@ -1156,29 +1261,34 @@ uint32_t idesc_of(int dtype, bool a_mn, bool b_mn, int ctas, int n) {
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kBM * ctas >> 4) << 24);
 }
 
-template <auto Kernel, bool FP8>
-int launch_gemm(GemmArgs& g, int ctas, cudaStream_t st) {
+int64_t units_of(const Problem& p) { return (int64_t)p.splits * p.msegs * p.tiles_m * p.tiles_n; }
+
+void set_divisors(Problem& g, int ctas) {
     const int row_tiles = g.msegs * g.tiles_m, group = std::min(row_tiles, kGroupRows / (kBM * ctas));
     g.per_split = Divisor(row_tiles * g.tiles_n);
     g.per_group = Divisor(group * g.tiles_n);
     g.per_seg = Divisor(g.tiles_m);
     g.group_rows = Divisor(group);
     g.last_rows = Divisor(row_tiles % group ? row_tiles % group : group);
+}
+
+template <auto Kernel, bool FP8, int N>
+int launch_gemm(GemmArgs<N>& g, int ctas, cudaStream_t st) {
     constexpr int rest = kEpiWarps * (kStageOut + column_bytes<FP8>()) + kBarrierBytes;
     g.stages = std::min(kMaxStages, (kSmemLimit - rest) / g.stage_bytes);
     static std::once_flag once[64];  // per kernel and device
     int dev = 0;
     cudaGetDevice(&dev);
     std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
-    const int64_t units = (int64_t)g.splits * g.msegs * g.tiles_m * g.tiles_n;
-    const unsigned grid = (unsigned)(std::min<int64_t>(units, num_sms() / ctas) * ctas);
+    const unsigned grid = (unsigned)(std::min(g.first[N], num_sms() / ctas) * ctas);
     launch_early(Kernel, grid, kGemmThreads, (size_t)g.stages * g.stage_bytes + rest, (unsigned)ctas, st, g);
     return check_launch("tc_gemm_kernel");
 }
 
-template <typename T, int MODE, bool FP8>
-int launch_ctas(GemmArgs& g, int ctas, cudaStream_t st) {
-    return ctas == 2 ? launch_gemm<tc_gemm_kernel<T, MODE, FP8, 2>, FP8>(g, 2, st) : launch_gemm<tc_gemm_kernel<T, MODE, FP8, 1>, FP8>(g, 1, st);
+template <typename T, int MODE, bool FP8, int N>
+int launch_ctas(GemmArgs<N>& g, int ctas, cudaStream_t st) {
+    return ctas == 2 ? launch_gemm<tc_gemm_kernel<T, MODE, FP8, 2, N>, FP8>(g, 2, st)
+                     : launch_gemm<tc_gemm_kernel<T, MODE, FP8, 1, N>, FP8>(g, 1, st);
 }
 
 int too_large(const char* what) {
@@ -1186,22 +1296,19 @@ int too_large(const char* what) {
     return LF_ERR_UNSUPPORTED;
 }
 
-int join_splits(const Product& q, const float* part, int splits, cudaStream_t st) {
-    const int64_t rows = q.m * q.msegs, ldp = up(q.n, 4), groups = rows * (ldp / 4);
-    const unsigned grid = (unsigned)std::min<int64_t>((groups + 255) / 256, (int64_t)num_sms() * 16);
-    auto kernel = q.dtype == LF_F16 ? split_join_kernel<__half> : split_join_kernel<__nv_bfloat16>;
-    launch_early(kernel, grid, 256, 0, 1, st, part, splits, rows, (int)q.n, ldp, q.e);
+int join_splits(const JoinJobs& jobs, int count, int dtype, cudaStream_t st) {
+    int64_t most = 1;
+    for (int i = 0; i < count; ++i) most = std::max(most, (jobs.job[i].rows * (jobs.job[i].ldp / 4) * jobs.job[i].walkers + 255) / 256);
+    const dim3 grid((unsigned)std::min<int64_t>(most, (int64_t)num_sms() * 16), (unsigned)count);
+    launch_early(dtype == LF_F16 ? split_join_kernel<__half> : split_join_kernel<__nv_bfloat16>, grid, 256, 0, 1, st, jobs);
     return check_launch("split_join_kernel");
 }
+JoinJob join_of(const Product& q, const float* part, int splits) {
+    return {part, q.m * q.msegs, up(q.n, 4), splits, (int)q.n, splits >= 32 ? 8 : splits >= 8 ? 4 : 1, q.e};
+}
 
-int run_product(const Product& q, Arena& ws, cudaStream_t st) {
-    if (q.m == 0 || q.n == 0) return LF_OK;
-    if (q.k == 0) return ws.base ? join_splits(q, nullptr, 0, st) : LF_OK;  // an empty sum: the epilogue of zero
-    const Shape s = choose(q);
-    float* part = s.splits > 1 ? (float*)ws.take(part_bytes(q, s)) : nullptr;
-    if (!ws.base) return LF_OK;
+int fill_problem(Problem& g, const Product& q, const Shape& s, float* part) {
     const int bk = q.op_dtype == LF_F8E4M3 ? 128 : 64;
-    GemmArgs g{};
     g.m = (int)q.m, g.n = (int)q.n;
     g.msegs = q.msegs;
     g.tiles_m = (int)((q.m + kBM * s.ctas - 1) / (kBM * s.ctas));
@@ -1210,10 +1317,8 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
     g.iters = g.seg_iters * q.ksegs;
     g.split_iters = (g.iters + s.splits - 1) / s.splits;
     g.splits = (g.iters + g.split_iters - 1) / g.split_iters;
-    if (q.m > INT32_MAX - 256 || q.n > INT32_MAX - 256 || (int64_t)g.splits * g.msegs * g.tiles_m * g.tiles_n > INT32_MAX / 2)
-        return too_large("matrix product");
+    if (q.m > INT32_MAX - 256 || q.n > INT32_MAX - 256 || units_of(g) > INT32_MAX / 4) return too_large("matrix product");
     g.bn = s.bn;
-    g.stage_bytes = (kBM + s.bn / s.ctas) * kRowBytes;
     g.a_mn = q.a_mn, g.b_mn = q.b_mn;
     g.idesc = idesc_of(q.op_dtype, q.a_mn, q.b_mn, s.ctas, s.bn);
     g.e = q.e;
@@ -1223,12 +1328,85 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
     g.ldp = up(q.n, 4);
     if (!encode(&g.a, q.a, q.op_dtype, q.a_mn ? 64 : bk, q.a_mn ? bk : kBM)) return LF_ERR_CUDA;
     if (!encode(&g.b, q.b, q.op_dtype, q.b_mn ? 64 : bk, q.b_mn ? bk : s.bn / s.ctas)) return LF_ERR_CUDA;
+    set_divisors(g, s.ctas);
+    return LF_OK;
+}
+
+int stage_bytes_of(const Shape& s) { return (kBM + s.bn / s.ctas) * kRowBytes; }
+
+int run_product(const Product& q, Arena& ws, cudaStream_t st) {
+    if (q.m == 0 || q.n == 0) return LF_OK;
+    JoinJobs join{};
+    if (q.k == 0) {  // an empty sum: the epilogue of zero
+        join.job[0] = join_of(q, nullptr, 0);
+        return ws.base ? join_splits(join, 1, q.dtype, st) : LF_OK;
+    }
+    const Shape s = choose(q);
+    float* part = s.splits > 1 ? (float*)ws.take(part_bytes(q, s)) : nullptr;
+    if (!ws.base) return LF_OK;
+    GemmArgs<1> g{};
+    if (int rc = fill_problem(g.p[0], q, s, part)) return rc;
+    g.first[1] = (int)units_of(g.p[0]);
+    g.stage_bytes = stage_bytes_of(s);
     int rc;
     if (q.op_dtype == LF_F8E4M3)
         rc = q.dtype == LF_F16 ? launch_ctas<__half, kLinear, true>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, true>(g, s.ctas, st);
     else
         rc = q.dtype == LF_F16 ? launch_ctas<__half, kLinear, false>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, false>(g, s.ctas, st);
-    return rc || !part ? rc : join_splits(q, part, g.splits, st);
+    if (rc || !part) return rc;
+    join.job[0] = join_of(q, part, g.p[0].splits);
+    return join_splits(join, 1, q.dtype, st);
+}
+
+// Up to three products of 16-bit operands that do not depend on one another,
+// in one launch: a gradient's products are often too small to fill the SMs
+// one by one, and large ones fill each other's last wave.
+int run_products(const Product* in, int given, Arena& ws, cudaStream_t st) {
+    Product q[3];
+    int count = 0;
+    for (int i = 0; i < given; ++i) {
+        if (in[i].m == 0 || in[i].n == 0 || in[i].k == 0) {
+            if (int rc = run_product(in[i], ws, st)) return rc;
+        } else q[count++] = in[i];
+    }
+    if (count == 0) return LF_OK;
+    if (count == 1) return run_product(q[0], ws, st);
+    Shape one[3], two[3];
+    const Shape* s = choose_together(q, count, 2, two) <= choose_together(q, count, 1, one) ? two : one;
+    float* part[3] = {};
+    for (int i = 0; i < count; ++i)
+        if (s[i].splits > 1) part[i] = (float*)ws.take(part_bytes(q[i], s[i]));
+    if (!ws.base) return LF_OK;
+    // Long units first.
+    int order[3] = {0, 1, 2};
+    double unit[3];
+    for (int i = 0; i < count; ++i) {
+        const int64_t iters = (q[i].k + 63) / 64 * q[i].ksegs;
+        unit[i] = std::max((double)((iters + s[i].splits - 1) / s[i].splits) * step_cycles(s[i].ctas, s[i].bn, s[i].bn), 500 + s[i].bn * 10.0);
+    }
+    std::sort(order, order + count, [&](int a, int b) { return unit[a] > unit[b]; });
+    GemmArgs<3> g{};
+    JoinJobs join{};
+    int joins = 0;
+    int64_t at = 0;
+    for (int i = 0; i < 3; ++i) {
+        g.first[i] = (int)at;
+        if (i >= count) continue;
+        const int k = order[i];
+        if (int rc = fill_problem(g.p[i], q[k], s[k], part[k])) return rc;
+        if (i == count - 1) g.longer = (int)at;
+        at += units_of(g.p[i]);
+        if (at > INT32_MAX / 2) return too_large("matrix products");
+        g.stage_bytes = std::max(g.stage_bytes, stage_bytes_of(s[k]));
+        if (part[k]) join.job[joins++] = join_of(q[k], part[k], g.p[i].splits);
+    }
+    g.first[3] = (int)at;
+    const int lanes = num_sms() / s[0].ctas, ahead = g.longer % lanes, last = (int)units_of(g.p[count - 1]);
+    if (ahead && last > 0 && g.longer + last >= lanes)
+        g.extra = (int)std::min<double>(unit[order[0]] / unit[order[count - 1]] + 0.5, last / (lanes - ahead));
+    const int rc = q[0].dtype == LF_F16 ? launch_ctas<__half, kLinear, false>(g, s[0].ctas, st)
+                                        : launch_ctas<__nv_bfloat16, kLinear, false>(g, s[0].ctas, st);
+    return rc || !joins ? rc : join_splits(join, joins, q[0].dtype, st);
 }
 
 // A dense operand as TMA can read it: itself, or a copy with padded rows.
@@ -1237,7 +1415,7 @@ Mat operand(const void* p, int64_t rows, int64_t cols, int64_t ld, int es, Arena
     const int64_t ldo = up(cols, 16 / es);
     void* out = ws.take((size_t)rows * ldo * es);
     if (out) {
-        const unsigned grid = (unsigned)std::min<int64_t>((rows + 7) / 8, (int64_t)num_sms() * 8);
+        const unsigned grid = (unsigned)std::min<int64_t>((rows * ((ldo * es + 511) / 512) + 7) / 8, (int64_t)num_sms() * 8);
         if (es == 1) launch_early(pack_rows_kernel<uint8_t>, grid, 256, 0, 1, st, (const uint8_t*)p, ld, (uint8_t*)out, ldo, rows, cols);
         else launch_early(pack_rows_kernel<uint16_t>, grid, 256, 0, 1, st, (const uint16_t*)p, ld, (uint16_t*)out, ldo, rows, cols);
     }
@@ -1289,8 +1467,8 @@ int run_colsum(const Columns* c, int count, int64_t rows, int dtype, Arena& ws, 
     p.tx = 1;
     while (p.tx < 32 && p.tx * v < widest) p.tx *= 2;
     const int64_t wide = (widest + p.tx * v - 1) / (p.tx * v);
-    // About eight blocks per SM, each at least four rows per row walker.
-    const int64_t most = std::max<int64_t>(1, 8 * num_sms() / (wide * jobs)), least = 4 * 256 / p.tx;
+    // About four blocks per SM, each at least eight rows per row walker.
+    const int64_t most = std::max<int64_t>(1, 4 * num_sms() / (wide * jobs)), least = 8 * 256 / p.tx;
     p.rows = rows;
     p.slice = std::max(least, (rows + most - 1) / most);
     p.slices = (int)((rows + p.slice - 1) / p.slice);
@@ -1299,10 +1477,10 @@ int run_colsum(const Columns* c, int count, int64_t rows, int dtype, Arena& ws, 
     const dim3 grid((unsigned)wide, (unsigned)p.slices, (unsigned)jobs), join((unsigned)((widest + 31) / 32), 1, (unsigned)jobs);
     if (dtype == LF_F16) {
         launch_early(vec ? colsum_kernel<__half, 8> : colsum_kernel<__half, 1>, grid, 256, 0, 1, st, p);
-        launch_early(colsum_join_kernel<__half>, join, 512, 0, 1, st, p);
+        launch_early(colsum_join_kernel<__half>, join, 1024, 0, 1, st, p);
     } else {
         launch_early(vec ? colsum_kernel<__nv_bfloat16, 8> : colsum_kernel<__nv_bfloat16, 1>, grid, 256, 0, 1, st, p);
-        launch_early(colsum_join_kernel<__nv_bfloat16>, join, 512, 0, 1, st, p);
+        launch_early(colsum_join_kernel<__nv_bfloat16>, join, 1024, 0, 1, st, p);
     }
     return check_launch("colsum_kernel");
 }
@@ -1417,18 +1595,19 @@ int linear_bwd(const lf_linear_t* a, Arena& ws, cudaStream_t st) {
     } else {
         dz = operand(a->dy, m, n, a->lddy, 2, ws, st);
     }
+    Product q[2];
+    int count = 0;
     if (a->dx) {  // dx = dz W: W is read with its k contiguous
-        Product q = weight_product(dz, w, m, k, n, a->dtype, a->dtype);
-        q.b_mn = true;
-        set_out(q.e, a->dx, k);
-        if (int rc = run_product(q, ws, st)) return rc;
+        Product& p = q[count++] = weight_product(dz, w, m, k, n, a->dtype, a->dtype);
+        p.b_mn = true;
+        set_out(p.e, a->dx, k);
     }
     if (a->dw) {  // dW = dz^T x: both operands transposed
-        Product q = weight_product(dz, x, n, k, m, a->dtype, a->dtype);
-        q.a_mn = q.b_mn = true;
-        set_out(q.e, a->dw, k);
-        if (int rc = run_product(q, ws, st)) return rc;
+        Product& p = q[count++] = weight_product(dz, x, n, k, m, a->dtype, a->dtype);
+        p.a_mn = p.b_mn = true;
+        set_out(p.e, a->dw, k);
     }
+    if (int rc = run_products(q, count, ws, st)) return rc;
     const Columns c{dz.p, dz.ld, n, a->db, need_z};
     return run_colsum(&c, 1, m, a->dtype, ws, st);
 }
@@ -1475,7 +1654,8 @@ int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* 
     const bool bwd = dy != nullptr;
     const Shape s = choose_gated(a->m, a->f, a->c, bwd);
     const int bh = s.bn / 2;
-    GemmArgs g{};
+    GemmArgs<1> args{};
+    Problem& g = args.p[0];
     g.m = (int)a->m, g.n = (int)a->f;
     g.msegs = g.splits = 1;
     g.tiles_m = (int)((a->m + kBM * s.ctas - 1) / (kBM * s.ctas));
@@ -1483,18 +1663,20 @@ int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* 
     if ((int64_t)g.tiles_m * g.tiles_n > INT32_MAX / 2) return too_large("gated feed-forward block");
     g.iters = g.split_iters = g.seg_iters = (int)((a->c + 63) / 64);
     g.bn = s.bn;
-    g.stage_bytes = (kBM + s.bn / s.ctas) * kRowBytes;
+    args.stage_bytes = stage_bytes_of(s);
     g.idesc = idesc_of(a->dtype, false, false, s.ctas, s.bn);
     g.idesc2 = idesc_of(a->dtype, false, true, s.ctas, bh);
     g.e.out = out, g.e.ldo = ldo, g.e.bias = a->b_in, g.e.act = a->activation;
     if (!encode_out(&g.out, {out, a->f, a->m, ldo, bwd ? 3 : 1, plane}, a->dtype)) return LF_ERR_CUDA;
     if (!encode(&g.a, x, a->dtype, 64, kBM) || !encode(&g.b, gate_up(win, a->f), a->dtype, 64, bh)) return LF_ERR_CUDA;
     if (bwd && (!encode(&g.a2, *dy, a->dtype, 64, kBM) || !encode(&g.b2, *wout, a->dtype, 64, 64))) return LF_ERR_CUDA;
+    set_divisors(g, s.ctas);
+    args.first[1] = (int)units_of(g);
     if (bwd)
-        return a->dtype == LF_F16 ? launch_ctas<__half, kGatedBwd, false>(g, s.ctas, st)
-                                  : launch_ctas<__nv_bfloat16, kGatedBwd, false>(g, s.ctas, st);
-    return a->dtype == LF_F16 ? launch_ctas<__half, kGated, false>(g, s.ctas, st)
-                              : launch_ctas<__nv_bfloat16, kGated, false>(g, s.ctas, st);
+        return a->dtype == LF_F16 ? launch_ctas<__half, kGatedBwd, false>(args, s.ctas, st)
+                                  : launch_ctas<__nv_bfloat16, kGatedBwd, false>(args, s.ctas, st);
+    return a->dtype == LF_F16 ? launch_ctas<__half, kGated, false>(args, s.ctas, st)
+                              : launch_ctas<__nv_bfloat16, kGated, false>(args, s.ctas, st);
 }
 
 int ffn_fwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
@@ -1533,26 +1715,26 @@ int ffn_bwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
     if (ws.base && f > 0)
         if (int rc = run_gated(a, x, win, &dy, &wout, dz, ld, plane, st)) return rc;
     const Mat both{dz, f, m, ld, 2, plane}, h{dz + 2 * plane, f, m, ld, 1, 0};
+    Product q[3];
+    int count = 0;
     if (a->dx) {  // dx = [dg|du] Win: two K segments of F
-        Product q = weight_product(both, gate_up(win, f), m, c, f, a->dtype, a->dtype);
-        q.b_mn = true;
-        q.ksegs = 2;
-        set_out(q.e, a->dx, c);
-        if (int rc = run_product(q, ws, st)) return rc;
+        Product& p = q[count++] = weight_product(both, gate_up(win, f), m, c, f, a->dtype, a->dtype);
+        p.b_mn = true;
+        p.ksegs = 2;
+        set_out(p.e, a->dx, c);
     }
     if (a->dw_in) {  // two row segments of F
-        Product q = weight_product(both, x, f, c, m, a->dtype, a->dtype);
-        q.a_mn = q.b_mn = true;
-        q.msegs = 2;
-        set_out(q.e, a->dw_in, c);
-        if (int rc = run_product(q, ws, st)) return rc;
+        Product& p = q[count++] = weight_product(both, x, f, c, m, a->dtype, a->dtype);
+        p.a_mn = p.b_mn = true;
+        p.msegs = 2;
+        set_out(p.e, a->dw_in, c);
     }
     if (a->dw_out) {
-        Product q = weight_product(dy, h, c, f, m, a->dtype, a->dtype);
-        q.a_mn = q.b_mn = true;
-        set_out(q.e, a->dw_out, f);
-        if (int rc = run_product(q, ws, st)) return rc;
+        Product& p = q[count++] = weight_product(dy, h, c, f, m, a->dtype, a->dtype);
+        p.a_mn = p.b_mn = true;
+        set_out(p.e, a->dw_out, f);
     }
+    if (int rc = run_products(q, count, ws, st)) return rc;
     uint16_t* db_in = (uint16_t*)a->db_in;
     const Columns cols[3] = {{dz, ld, f, db_in, true}, {dz + plane, ld, f, db_in ? db_in + f : nullptr, true}, {a->dy, a->lddy, c, a->db_out, false}};
     return run_colsum(cols, 3, m, a->dtype, ws, st);
