@@ -381,20 +381,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 struct Tile {
     int seg, m0, n0, split, it0, it1;
 };
-// Order of the gated backward's 2 n steps: kLead steps of dh, while the
-// epilogue still reads the last tile's g and u, then g|u and dh in turn (dh
-// alone would fetch 96 bytes per cycle and SM), then what is left of g|u.
-constexpr int kLead = 4;
-struct Step {
-    bool dh;
-    int it;
-};
-__device__ __forceinline__ Step gated_step(int i, int n) {
-    const int lead = min(kLead, n), j = i - lead, both = 2 * (n - lead);
-    if (j < 0) return {true, i};
-    if (j < both) return {(j & 1) != 0, (j & 1) ? lead + (j >> 1) : j >> 1};
-    return {false, n - lead + (j - both)};
-}
 // Work units: for each split of K, row tiles in groups of kGroupRows, within a
 // group all row tiles of one column tile before the next column tile.
 template <int CTAS>
@@ -423,11 +409,12 @@ __device__ __forceinline__ uint8_t* stage_at(uint8_t* st, int row, int chunk) {
 }
 // Columns 16 half .. of the calling lane's row, as 16-bit values.
 template <typename T>
+__device__ __forceinline__ uint4 pack8(const float* v) {
+    return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+template <typename T>
 __device__ __forceinline__ void pack16(uint4 (&u)[2], const float (&v)[16]) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-        u[c] = make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
-                          pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+    u[0] = pack8<T>(v), u[1] = pack8<T>(v + 8);
 }
 __device__ __forceinline__ void stage16(uint8_t* st, int lane, int half, const uint4 (&u)[2]) {
 #pragma unroll
@@ -461,29 +448,31 @@ __device__ __forceinline__ T column_value(const T* p, int col, int n) {
 // kLinear: out = epilogue(A B^T), two accumulator buffers.
 // kGated: B's tile is bn/2 gate and bn/2 up rows of Win, the accumulator's
 // halves are g and u of the same hidden columns.
-// kGatedBwd: first dh = dy Wout (accumulators at 256 or 384, in turn), then
-// [g|u] = x Win^T at 0.  The epilogue takes all of a tile's g and u into
-// registers at once, while the next tile's dh is computed, so that neither
-// product waits for outputs.
+// kGatedBwd: a tile is 2 bh hidden columns: [g|u] = x Win^T of one half
+// (accumulators from 0 on), dh = dy Wout of both (from 256 on, so that dy is
+// read once for them), then [g|u] of the other half.  All of the tensor memory
+// is in use, so the products of a half wait until the epilogue has taken the
+// last half's g and u into registers, which it does first; dh is overwritten a
+// whole product later.
 template <typename T, int MODE, bool FP8, int CTAS, int N>
 __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_constant__ GemmArgs<N> args) {
     extern __shared__ __align__(1024) uint8_t smem[];  // stages, output staging, barriers
     uint8_t* out_stage = smem + args.stages * args.stage_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * (kStageOut + column_bytes<FP8>()));
-    uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *dempty = tempty + 2, *drain = dempty + 2;
+    uint64_t *empty = full + kMaxStages, *tfull = empty + kMaxStages, *tempty = tfull + 2, *dempty = tempty + 2, *drain = dempty + 1;
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0;
     constexpr int BK = FP8 ? 128 : 64;
     constexpr int kABytes = kBM * kRowBytes;
     constexpr int kDh = 256;                                   // tensor memory columns of dh
-    const int phases = MODE == kGatedBwd ? 2 : 1;
 
     grid_release();
     if (threadIdx.x == 0) {
         for (int i = 0; i < args.stages; ++i) mbar_init(&full[i], 2), mbar_init(&empty[i], 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps * CTAS), mbar_init(&dempty[i], kEpiWarps * CTAS);
+            mbar_init(&tfull[i], 1), mbar_init(&tempty[i], kEpiWarps * CTAS);
+        mbar_init(dempty, kEpiWarps * CTAS);
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -501,8 +490,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
 #define LFB_PROBLEM(RANK)                                                                                        \
     const Problem& p = args.p[problem_of(args, unit)];                                                           \
     const int bh = p.bn / 2; /* hidden columns of a gated tile */                                                \
-    const int bn_out = MODE == kLinear ? p.bn : bh;                                                              \
-    const Tile t = tile_of<CTAS>(p, unit, bn_out, RANK)
+    const Tile t = tile_of<CTAS>(p, unit, MODE == kGated ? bh : p.bn, RANK);                                     \
+    const int subs = MODE == kGatedBwd && t.n0 + bh < p.n ? 2 : 1 /* halves of a kGatedBwd tile */
     bool ok = true;
 
     if (warp == 0 || warp == 2) {
@@ -516,34 +505,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             LFB_EACH_UNIT(ok) {
                 LFB_PROBLEM(rank);
                 const int bw = p.bn / CTAS;                    // B rows that this CTA holds
-                const int steps = (t.it1 - t.it0) * phases;
-                int ks = t.it0 / p.seg_iters, in_seg = t.it0 - ks * p.seg_iters;
-                for (int i = 0; i < steps; ++i) {
+                const int n = t.it1 - t.it0;
+                int ks = t.it0 / p.seg_iters, in_seg = t.it0 - ks * p.seg_iters;  // gated modes: product and step of K
+                for (int left = MODE == kGatedBwd ? n * (1 + subs) : n; left > 0; --left) {
                     if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
-                    const Step step = MODE == kGatedBwd ? gated_step(i, steps / 2) : Step{false, i};
-                    const int k0 = (MODE == kLinear ? in_seg : step.it) * BK;
+                    const bool dh = MODE == kGatedBwd && ks == 1;
+                    const int k0 = in_seg * BK, n0 = MODE == kGatedBwd && ks == 2 ? t.n0 + bh : t.n0;
                     uint8_t* dst = smem + s * args.stage_bytes + (is_a ? 0 : kABytes);
                     const uint32_t bar = bars + 8 * s;
-                    if (rank == 0) mbar_expect(&full[s], (is_a ? kABytes : (step.dh ? bh / CTAS : bw) * kRowBytes) * CTAS);
+                    if (rank == 0) mbar_expect(&full[s], (is_a ? kABytes : bw * kRowBytes) * CTAS);
                     if (is_a) {
-                        if (step.dh) tma_load<CTAS>(dst, &p.a2, bar, k0, t.m0, 0);
-                        else if (!p.a_mn) tma_load<CTAS>(dst, &p.a, bar, k0, t.m0, ks);
+                        if (dh) tma_load<CTAS>(dst, &p.a2, bar, k0, t.m0, 0);
+                        else if (!p.a_mn) tma_load<CTAS>(dst, &p.a, bar, k0, t.m0, MODE == kLinear ? ks : 0);
                         else
                             for (int j = 0; j < kBM / 64; ++j) tma_load<CTAS>(dst + j * 8192, &p.a, bar, t.m0 + 64 * j, k0, t.seg);
-                    } else if (step.dh) {
-                        for (int j = 0; j < bh / CTAS / 64; ++j)
-                            tma_load<CTAS>(dst + j * 8192, &p.b2, bar, t.n0 + rank * (bh / CTAS) + 64 * j, k0, 0);
+                    } else if (dh) {
+                        for (int j = 0; j < bw / 64; ++j) tma_load<CTAS>(dst + j * 8192, &p.b2, bar, t.n0 + rank * bw + 64 * j, k0, 0);
                     } else if (MODE != kLinear) {
-                        if (CTAS == 2) tma_load<CTAS>(dst, &p.b, bar, k0, t.n0, rank);  // one CTA the gate rows, the other the up rows
+                        if (CTAS == 2) tma_load<CTAS>(dst, &p.b, bar, k0, n0, rank);  // one CTA the gate rows, the other the up rows
                         else
-                            for (int j = 0; j < 2; ++j) tma_load<CTAS>(dst + j * bh * kRowBytes, &p.b, bar, k0, t.n0, j);
+                            for (int j = 0; j < 2; ++j) tma_load<CTAS>(dst + j * bh * kRowBytes, &p.b, bar, k0, n0, j);
                     } else if (!p.b_mn) {
                         tma_load<CTAS>(dst, &p.b, bar, k0, t.n0 + rank * bw, ks);
                     } else {
                         for (int j = 0; j < bw / 64; ++j) tma_load<CTAS>(dst + j * 8192, &p.b, bar, t.n0 + rank * bw + 64 * j, k0, ks);
                     }
                     ++issued;
-                    if (MODE == kLinear && ++in_seg == p.seg_iters) in_seg = 0, ++ks;
+                    if (++in_seg == p.seg_iters) in_seg = 0, ++ks;
                     if (++s == args.stages) s = 0, ph ^= 1;
                 }
             }
@@ -563,40 +551,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 LFB_PROBLEM(0);
                 const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16, idesc = p.idesc;
                 const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
-                const int steps = (t.it1 - t.it0) * phases;
-                for (int i = 0; i < steps; ++i) {
-                    const Step step = MODE == kGatedBwd ? gated_step(i, steps / 2) : Step{false, i};
-                    const bool dh = step.dh;
-                    if (step.it == 0) {
-                        // Each accumulator's last reader: the previous tile for g and u, two tiles ago for the others.
-                        if (dh) ok = mbar_wait(&dempty[buf], dph ^ 1);
-                        else ok = mbar_wait(&tempty[MODE == kGatedBwd ? 0 : buf], bph ^ 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    const uint32_t acc = tmem + (MODE != kGatedBwd ? buf * 256 : dh ? kDh + buf * 128 : 0);
-                    if (!(ok = mbar_wait(&full[s], ph))) break;
+                const int n = t.it1 - t.it0, products = MODE == kGatedBwd ? 1 + subs : 1;
+                for (int product = 0; ok && product < products; ++product) {
+                    const bool dh = MODE == kGatedBwd && product == 1;
+                    // The accumulators' last reader: the half before (g and u), the tile before (dh), two tiles ago (others).
+                    if (dh) ok = mbar_wait(dempty, dph ^ 1);
+                    else ok = mbar_wait(&tempty[buf], bph ^ 1);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * args.stage_bytes), sb = sa + kABytes;
-                    if (dh) {
-                        const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sb, 8192, 1024);
+                    const uint32_t acc = tmem + (dh ? kDh : buf * 256);
+                    for (int i = 0; i < n; ++i) {
+                        if (!(ok = mbar_wait(&full[s], ph))) break;
+                        tc_fence_after();
+                        const uint32_t sa = smem_u32(smem + s * args.stage_bytes), sb = sa + kABytes;
+                        const uint64_t da = make_desc(sa, dh ? 16 : a_lbo, 1024), db = make_desc(sb, dh ? 8192 : b_lbo, 1024);
+                        const uint64_t as = dh ? 2 : a_step, bs = dh ? 128 : b_step;
+                        const uint32_t id = dh ? p.idesc2 : idesc;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma<CTAS, FP8>(acc, da + k * 2, db + k * 128, p.idesc2, step.it > 0 || k > 0 ? 1u : 0u, go);
-                    } else {
-                        const uint64_t da = make_desc(sa, a_lbo, 1024), db = make_desc(sb, b_lbo, 1024);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma<CTAS, FP8>(acc, da + k * a_step, db + k * b_step, idesc, step.it > 0 || k > 0 ? 1u : 0u, go);
+                        for (int k = 0; k < 4; ++k) mma<CTAS, FP8>(acc, da + k * as, db + k * bs, id, i > 0 || k > 0 ? 1u : 0u, go);
+                        if (go) commit<CTAS>(&empty[s]);
+                        if (++s == args.stages) s = 0, ph ^= 1;
                     }
-                    if (go) commit<CTAS>(&empty[s]);
-                    if (++s == args.stages) s = 0, ph ^= 1;
+                    if (!ok || (MODE == kGatedBwd && product == 0)) continue;
+                    if (go) commit<CTAS>(&tfull[buf]);
+                    if (MODE != kGatedBwd) buf ^= 1;
+                    if (buf == 0) bph ^= 1;
                 }
-                if (!ok) break;
-                if (go) commit<CTAS>(&tfull[MODE == kGatedBwd ? 0 : buf]);
-                buf ^= 1;
-                if (buf == 0) dph ^= 1;
-                if (MODE == kGatedBwd || buf == 0) bph ^= 1;
+                dph ^= 1;
             }
             if (!ok) {  // products in flight end before the tensor memory is freed
                 if (go) commit<CTAS>(drain);
@@ -620,14 +601,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
         };
         int buf = 0;
         uint32_t bph = 0;
-        LFB_EACH_UNIT(true) {
+        LFB_EACH_UNIT(ok) {
             LFB_PROBLEM(rank);
             const Epilogue& e = p.e;
             const uint32_t lanes = (uint32_t)(quad * 32) << 16;
             const int rows = p.m - t.m0 - quad * 32;                           // rows that exist from the warp's first on
             const int64_t row0 = (int64_t)t.seg * p.m + t.m0 + quad * 32;      // in the output
-            const int cend = min(bn_out, p.n - t.n0);
-            uint64_t* tf = &tfull[MODE == kGatedBwd ? 0 : buf];
+            for (int sub = 0; sub < subs; ++sub) {
+            const int n0 = t.n0 + sub * bh, cend = min(MODE == kLinear ? p.bn : bh, p.n - n0);
+            uint64_t* tf = &tfull[buf];
             const int last = cg * 32 + (cend - cg * 32 - 1) / kEpiCols * kEpiCols;  // this warp's last 32 columns (if it has any)
             auto release = [&](uint64_t* bar) {
                 tc_fence_before();
@@ -637,8 +619,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             if (cg * 32 >= cend) {                                           // none: wait for the tile all the same
                 if (!(ok = mbar_wait(tf, bph))) break;
                 tc_fence_after();
-                release(&tempty[MODE == kGatedBwd ? 0 : buf]);
-                if (MODE == kGatedBwd) release(&dempty[buf]);
+                release(&tempty[buf]);
+                if (MODE == kGatedBwd && sub == subs - 1) release(dempty);
             } else
             if constexpr (MODE == kLinear) {
                 const uint32_t acc = tmem + buf * 256 + lanes;
@@ -779,26 +761,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 }
             } else {
                 const T* bias = (const T*)e.bias;
-                const uint32_t acc = tmem + (MODE == kGated ? buf * 256 : 0) + lanes;
+                const uint32_t acc = tmem + buf * 256 + lanes;
                 const int c0 = cg * 32;                                        // the warp's only columns
-                const T bg = column_value(bias, t.n0 + c0 + lane, p.n);
-                const T bu = column_value(bias ? bias + p.n : bias, t.n0 + c0 + lane, p.n);
+                const T bg = column_value(bias, n0 + c0 + lane, p.n);
+                const T bu = column_value(bias ? bias + p.n : bias, n0 + c0 + lane, p.n);
                 if (!(ok = mbar_wait(tf, bph))) break;
                 tc_fence_after();
-                reuse();
+                if (MODE == kGated) reuse();
                 if (bias) {
                     cv[lane] = bg, cv[32 + lane] = bu;
                     __syncwarp();
                 }
                 // 16 columns at a time; outputs wait as 16-bit pairs.
                 uint4 og[2][2], ou[2][2];
+                if constexpr (MODE == kGated) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c = c0 + h * 16;
-                    float g[16], u[16];
-                    tmem_ld16(acc + c, g);
-                    tmem_ld16(acc + bh + c, u);
-                    if constexpr (MODE == kGated) {
+                    for (int h = 0; h < 2; ++h) {
+                        float g[16], u[16];
+                        tmem_ld16(acc + c0 + h * 16, g);
+                        tmem_ld16(acc + bh + c0 + h * 16, u);
                         tmem_wait_ld();
                         reg_fence(g);
                         reg_fence(u);
@@ -809,49 +790,69 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                             for (int j = 0; j < 16; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
                         });
                         pack16<T>(ou[h], u);
-                    } else {
-                        float d[16];
-                        tmem_ld16(tmem + kDh + buf * 128 + lanes + c, d);
-                        tmem_wait_ld();
-                        reg_fence(g);
-                        reg_fence(u);
-                        reg_fence(d);
-                        if (h == 1) release(&tempty[0]), release(&dempty[buf]);
-                        if (bias) add_columns(g, cv + h * 16), add_columns(u, cv + 32 + h * 16);
-                        // h = act(g) u, du = dh act(g), dg = dh u act'(g), in d, g and u
-                        with_act(e.act, [&](auto act) {
+                    }
+                } else {
+                    float g[2][16], u[2][16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                float a, slope;
-                                act_both<decltype(act)::value>(g[j], a, slope);
-                                const float dh = d[j];
-                                d[j] = a * u[j];
-                                g[j] = a * dh;
-                                u[j] *= slope * dh;
-                            }
-                        });
+                    for (int h = 0; h < 2; ++h) {
+                        tmem_ld16(acc + c0 + h * 16, g[h]);
+                        tmem_ld16(acc + bh + c0 + h * 16, u[h]);
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        reg_fence(g[h]);
+                        reg_fence(u[h]);
+                    }
+                    release(tempty);
+                    reuse();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (bias) add_columns(g[h], cv + h * 16), add_columns(u[h], cv + 32 + h * 16);
                         uint4 oh[2];
-                        pack16<T>(oh, d);
-                        pack16<T>(og[h], g);
-                        pack16<T>(ou[h], u);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {  // eight columns of dh at a time: registers are full
+                            float d[8];
+                            tmem_ld8(tmem + kDh + sub * bh + lanes + c0 + h * 16 + c * 8, d);
+                            tmem_wait_ld();
+                            reg_fence(d);
+                            if (h == 1 && c == 1 && sub == subs - 1) release(dempty);
+                            // h = act(g) u, du = dh act(g), dg = dh u act'(g), in d, g and u
+                            with_act(e.act, [&](auto act) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    float a, slope;
+                                    float &gj = g[h][c * 8 + j], &uj = u[h][c * 8 + j];
+                                    act_both<decltype(act)::value>(gj, a, slope);
+                                    const float dh = d[j];
+                                    d[j] = a * uj;
+                                    gj = a * dh;
+                                    uj *= slope * dh;
+                                }
+                            });
+                            oh[c] = pack8<T>(d);
+                            og[h][c] = pack8<T>(&g[h][c * 8]);
+                            ou[h][c] = pack8<T>(&u[h][c * 8]);
+                        }
                         stage16(st, lane, h, oh);
                     }
                 }
                 const int row = t.m0 + quad * 32;
                 if constexpr (MODE == kGatedBwd) {  // planes dg, du, h
-                    put(&p.out, t.n0 + c0, row, 2, rows > 0);
+                    put(&p.out, n0 + c0, row, 2, rows > 0);
                     reuse();
                     stage16(st, lane, 0, og[0]);
                     stage16(st, lane, 1, og[1]);
-                    put(&p.out, t.n0 + c0, row, 1, rows > 0);
+                    put(&p.out, n0 + c0, row, 1, rows > 0);
                     reuse();
                 }
                 stage16(st, lane, 0, ou[0]);
                 stage16(st, lane, 1, ou[1]);
-                put(&p.out, t.n0 + c0, row, 0, rows > 0);
+                put(&p.out, n0 + c0, row, 0, rows > 0);
             }
-            buf ^= 1;
-            if (MODE == kGatedBwd || buf == 0) bph ^= 1;
+            if (MODE != kGatedBwd) buf ^= 1;
+            if (buf == 0) bph ^= 1;
+            }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // outputs written, staging read
     }
@@ -1630,20 +1631,20 @@ int check_ffn(const char* what, const lf_gated_ffn_t* a) {
 Mat gate_up(Mat w, int64_t f) { return {w.p, w.inner, f, w.ld, 2, f * w.ld}; }
 
 // Tile of the gated kernels by the same estimate as choose(); bn counts gate
-// and up columns.  The backward's third product is as wide as one of them.
+// and up columns.  A tile of the backward has two halves of bn/2 hidden
+// columns and a third product that is as wide as bn; about 700 cycles of each
+// half's epilogue are not covered by products.
 Shape choose_gated(int64_t m, int64_t f, int64_t c, bool bwd) {
     const int64_t iters = (c + 63) / 64, sms = num_sms();
     Shape best{1, 128, 1};
     double least = 1e30;
     for (int ctas : {2, 1})
         for (int bh : {128, 64, 32}) {
-            if (bh < (ctas == 2 ? 128 : bwd ? 64 : 32)) continue;
-            const int64_t tiles = (m + kBM * ctas - 1) / (kBM * ctas) * ((f + bh - 1) / bh), waves = (tiles * ctas + sms - 1) / sms;
-            const double first = iters * step_cycles(ctas, 2 * bh, 2 * bh), second = bwd ? iters * step_cycles(ctas, bh, bh) : 0;
-            const double epi = 500 + bh * (bwd ? 40.0 : 20.0);
-            // The backward's epilogue overlaps only the next tile's second product.
-            const double t = bwd ? waves * (first + std::max(second, epi)) + std::min(second, epi)
-                                 : waves * std::max(first, epi) + std::min(first, epi);
+            if (bh < (ctas == 2 && !bwd ? 128 : bwd ? 64 : 32)) continue;
+            const int64_t width = bwd ? 2 * bh : bh;
+            const int64_t tiles = (m + kBM * ctas - 1) / (kBM * ctas) * ((f + width - 1) / width), waves = (tiles * ctas + sms - 1) / sms;
+            const double main = iters * step_cycles(ctas, 2 * bh, 2 * bh), epi = 500 + bh * (bwd ? 25.0 : 15.0);
+            const double t = bwd ? waves * std::max(3 * main + 1400, 2 * epi) + epi : waves * std::max(main, epi) + std::min(main, epi);
             if (t < least) least = t, best = {ctas, 2 * bh, 1};
         }
     return best;
@@ -1659,13 +1660,14 @@ int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* 
     g.m = (int)a->m, g.n = (int)a->f;
     g.msegs = g.splits = 1;
     g.tiles_m = (int)((a->m + kBM * s.ctas - 1) / (kBM * s.ctas));
-    g.tiles_n = (int)((a->f + bh - 1) / bh);
+    const int width = bwd ? 2 * bh : bh;  // hidden columns of a tile
+    g.tiles_n = (int)((a->f + width - 1) / width);
     if ((int64_t)g.tiles_m * g.tiles_n > INT32_MAX / 2) return too_large("gated feed-forward block");
     g.iters = g.split_iters = g.seg_iters = (int)((a->c + 63) / 64);
     g.bn = s.bn;
     args.stage_bytes = stage_bytes_of(s);
     g.idesc = idesc_of(a->dtype, false, false, s.ctas, s.bn);
-    g.idesc2 = idesc_of(a->dtype, false, true, s.ctas, bh);
+    g.idesc2 = idesc_of(a->dtype, false, true, s.ctas, s.bn);
     g.e.out = out, g.e.ldo = ldo, g.e.bias = a->b_in, g.e.act = a->activation;
     if (!encode_out(&g.out, {out, a->f, a->m, ldo, bwd ? 3 : 1, plane}, a->dtype)) return LF_ERR_CUDA;
     if (!encode(&g.a, x, a->dtype, 64, kBM) || !encode(&g.b, gate_up(win, a->f), a->dtype, 64, bh)) return LF_ERR_CUDA;
