@@ -46,7 +46,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> GatedFeed
     int64_t activation, bool need_x, bool need_w_in, bool need_w_out, bool need_b_in, bool need_b_out);
 
 // Writes the clipped gradients to `outs` (which may be `grads`) and returns the norm (a float32 scalar).
-at::Tensor ClipGradNorm(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs, double max_norm);
+at::Tensor ClipGradNorm(const std::vector<const at::Tensor*>& grads, const std::vector<const at::Tensor*>& outs, double max_norm);
 
 // The same operators as autograd nodes; without a tensor that requires a
 // gradient they are the _forward functions.  RmsNorm returns (y, s).

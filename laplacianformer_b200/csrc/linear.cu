@@ -208,7 +208,7 @@ constexpr int kEpiWarps = 16;             // four per 32-lane quarter of the ten
 constexpr int kControlWarps = 3;          // copies of A, products, copies of B
 constexpr int kGemmThreads = 32 * (kControlWarps + kEpiWarps);
 constexpr int kStageOut = 2048;           // output staging per epilogue warp: 32 rows of 64 bytes
-// and the values of 32 columns: two 16-bit biases, or one and an fp32 scale
+// and the values of 32 columns: two 16-bit biases, or a scale and a bias in fp32
 template <bool FP8>
 constexpr int column_bytes() { return FP8 ? 256 : 128; }
 constexpr int kEpiCols = kEpiWarps / 4 * 32;  // columns that the epilogue warps read at a time
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
         const int ew = warp - kControlWarps, quad = warp & 3, cg = ew >> 2;  // lanes of the tensor memory, columns of a tile
         uint8_t* st = out_stage + ew * kStageOut;
         T* cv = reinterpret_cast<T*>(out_stage + kEpiWarps * kStageOut + ew * column_bytes<FP8>());
-        float* cs = reinterpret_cast<float*>(cv + 64);
+        float* cs = reinterpret_cast<float*>(cv);  // 8-bit form: 32 scales, then 32 biases
         // Writes the staged 32x32 outputs by TMA, and waits until they may be overwritten.
         auto put = [&](const CUtensorMap* out, int col, int row, int plane, bool some) {
             fence_async_smem();
@@ -648,8 +648,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                     tc_fence_after();
                     for (int c0 = first; c0 < cend; c0 += kEpiCols) {
                         reuse();
-                        if (e.bias) cv[lane] = bias;
-                        if (FP8) cs[lane] = sb;
+                        if (FP8) cs[lane] = sb, cs[32 + lane] = Elem<T>::load(bias);
+                        else if (e.bias) cv[lane] = bias;
                         if (e.res) {  // to the lane that owns the row
 #pragma unroll
                             for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
@@ -664,11 +664,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                             tmem_wait_ld();
                             reg_fence(v);
                             if (h == 1 && c0 == last) release(&tempty[buf]);
-                            if (FP8) {
+                            if (FP8) {  // (v sw) sx + b in pairs
+                                const uint64_t sx = pk2(sa, sa);
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] *= sa * cs[h * 16 + j];
-                            }
-                            if (e.bias) add_columns(v, cv + h * 16);
+                                for (int j = 0; j < 16; j += 2) {
+                                    const uint64_t w = *reinterpret_cast<const uint64_t*>(cs + h * 16 + j);
+                                    const uint64_t b = *reinterpret_cast<const uint64_t*>(cs + 32 + h * 16 + j);
+                                    upk2(fma2(mul2(pk2(v[j], v[j + 1]), w), sx, b), v[j], v[j + 1]);
+                                }
+                            } else if (e.bias) add_columns(v, cv + h * 16);
                             if (e.act != LF_ACT_NONE)
                                 with_act(e.act, [&](auto act) {
 #pragma unroll

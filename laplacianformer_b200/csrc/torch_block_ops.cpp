@@ -1,6 +1,7 @@
 // PyTorch-tensor front end of the block operators: argument checks, output and
 // workspace allocation on the current stream, then one call into the C ABI.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -90,13 +91,18 @@ Rows as_rows(const at::Tensor& t) {
     return {t.contiguous(), cols};
 }
 
+// A contiguous tensor of the caching allocator on like's device (without the
+// dispatcher, which would take longer than a small operator's launch).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& like) { return fresh(sizes, like.scalar_type(), like); }
+
 at::Tensor workspace(size_t bytes, const at::Tensor& like) {
-    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+    return bytes ? fresh({(int64_t)bytes}, at::kByte, like) : at::Tensor();
 }
 
-at::Tensor maybe(bool want, at::IntArrayRef sizes, const at::Tensor& like) {
-    return want ? at::empty(sizes, like.options()) : at::Tensor();
-}
+at::Tensor maybe(bool want, at::IntArrayRef sizes, const at::Tensor& like) { return want ? fresh(sizes, like) : at::Tensor(); }
 void* mut(at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 at::Tensor dense(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
@@ -124,9 +130,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> RmsNorm_forward(const at::Tensor&
     check_norm(x_, weight_, residual_);
     c10::cuda::CUDAGuard guard(x_.device());
     const at::Tensor x = dense(x_), weight = dense(weight_), residual = dense(residual_);
-    at::Tensor y = at::empty_like(x), s, rstd;
-    if (residual.defined()) s = at::empty_like(x);
-    if (keep) rstd = at::empty({rows_of(x)}, x.options().dtype(at::kFloat));
+    at::Tensor y = fresh(x.sizes(), x), s, rstd;
+    if (residual.defined()) s = fresh(x.sizes(), x);
+    if (keep) rstd = fresh({rows_of(x)}, at::kFloat, x);
     raise_on(lf_rms_norm_fwd(ptr(x), ptr(residual), ptr(weight), mut(y), mut(s), (float*)mut(rstd), rows_of(x), x.size(-1),
                              dtype_code(x), eps, stream_of(x)),
              "RmsNorm_forward");
@@ -159,9 +165,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> RmsNorm_quant_forward(const at::T
     check_norm(x_, weight_, residual_);
     c10::cuda::CUDAGuard guard(x_.device());
     const at::Tensor x = dense(x_), weight = dense(weight_), residual = dense(residual_);
-    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), s;
-    at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
-    if (residual.defined()) s = at::empty_like(x);
+    at::Tensor q = fresh(x.sizes(), at::kFloat8_e4m3fn, x), s;
+    at::Tensor scale = fresh(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+    if (residual.defined()) s = fresh(x.sizes(), x);
     raise_on(lf_rms_norm_quant_fwd(ptr(x), ptr(residual), ptr(weight), mut(q), (float*)mut(scale), mut(s), rows_of(x),
                                    x.size(-1), dtype_code(x), eps, stream_of(x)),
              "RmsNorm_quant_forward");
@@ -173,8 +179,8 @@ std::tuple<at::Tensor, at::Tensor> Quantize_rows(const at::Tensor& x_) {
     TORCH_CHECK(x_.dim() >= 1, "x must have at least one dimension");
     c10::cuda::CUDAGuard guard(x_.device());
     const at::Tensor x = dense(x_);
-    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-    at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    at::Tensor q = fresh(x.sizes(), at::kFloat8_e4m3fn, x);
+    at::Tensor scale = fresh(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
     raise_on(lf_quantize_rows(ptr(x), mut(q), (float*)mut(scale), rows_of(x), x.size(-1), dtype_code(x), stream_of(x)),
              "Quantize_rows");
     return {q, scale};
@@ -216,7 +222,7 @@ at::Tensor Linear_forward(const at::Tensor& x, const at::Tensor& weight, const a
                           int64_t activation) {
     LinearCall c = linear_call(x, weight, bias, residual, activation, x);
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor y = at::empty(with_last(x, c.a.n), x.options());
+    at::Tensor y = fresh(with_last(x, c.a.n), x);
     c.a.y = y.data_ptr();
     c.a.dtype = dtype_code(x);
     const size_t need = lf_linear_fwd_workspace_size(&c.a);
@@ -232,7 +238,7 @@ at::Tensor Linear_quant_forward(const at::Tensor& q, const at::Tensor& scale, co
     TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be float16 or bfloat16");
     need_cuda(q, "q");
     c10::cuda::CUDAGuard guard(q.device());
-    at::Tensor like = at::empty({0}, q.options().dtype(dtype));
+    at::Tensor like = fresh({0}, dtype, q);
     LinearCall c = linear_call(q, weight, bias, residual, activation, like);
     for (const auto* s : {&scale, &weight_scale}) {
         need_cuda(*s, "scale");
@@ -240,7 +246,7 @@ at::Tensor Linear_quant_forward(const at::Tensor& q, const at::Tensor& scale, co
     }
     TORCH_CHECK(scale.numel() == c.a.m && weight_scale.numel() == c.a.n, "scales must have one value per row");
     const at::Tensor sx = dense(scale), sw = dense(weight_scale);
-    at::Tensor y = at::empty(with_last(q, c.a.n), like.options());
+    at::Tensor y = fresh(with_last(q, c.a.n), like);
     c.a.y = y.data_ptr();
     c.a.x_scale = (const float*)sx.data_ptr(), c.a.w_scale = (const float*)sw.data_ptr();
     c.a.dtype = dtype_code(like);
@@ -307,7 +313,7 @@ at::Tensor GatedFeedForward_forward(const at::Tensor& x, const at::Tensor& w_in,
                                     int64_t activation) {
     FfnCall k = ffn_call(x, w_in, w_out, b_in, b_out, residual, activation);
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor y = at::empty(x.sizes(), x.options());
+    at::Tensor y = fresh(x.sizes(), x);
     k.a.y = y.data_ptr();
     const size_t need = lf_gated_ffn_fwd_workspace_size(&k.a);
     at::Tensor ws = workspace(need, x);
@@ -333,7 +339,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> GatedFeed
     return {dx, dwi, dwo, dbi, dbo};
 }
 
-at::Tensor ClipGradNorm(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs, double max_norm) {
+at::Tensor ClipGradNorm(const std::vector<const at::Tensor*>& grads, const std::vector<const at::Tensor*>& outs, double max_norm) {
     TORCH_CHECK(!grads.empty(), "clip_grad_norm needs at least one gradient");
     TORCH_CHECK(grads.size() == outs.size(), "one output per gradient expected");
     const size_t n = grads.size();
@@ -341,30 +347,31 @@ at::Tensor ClipGradNorm(const std::vector<at::Tensor>& grads, const std::vector<
     std::vector<void*> out(n);
     std::vector<int64_t> sizes(n);
     std::vector<int> dtypes(n);
+    const at::Device device = grads[0]->device();
     for (size_t i = 0; i < n; ++i) {
-        need_cuda(grads[i], "gradient");
-        TORCH_CHECK(grads[i].device() == grads[0].device(), "all gradients must be on one device");
-        check_operand(outs[i], grads[i], "output");
-        TORCH_CHECK(outs[i].sizes() == grads[i].sizes(), "an output must have its gradient's shape and strides");
-        if (!grads[i].is_contiguous() || !outs[i].is_contiguous()) {
-            TORCH_CHECK(grads[i].is_non_overlapping_and_dense(), "gradients must be dense");
-            TORCH_CHECK(outs[i].strides() == grads[i].strides(), "an output must have its gradient's shape and strides");
+        const at::Tensor &g = *grads[i], &o = *outs[i];
+        need_cuda(g, "gradient");
+        TORCH_CHECK(g.device() == device, "all gradients must be on one device");
+        check_operand(o, g, "output");
+        TORCH_CHECK(o.sizes() == g.sizes(), "an output must have its gradient's shape and strides");
+        if (!g.is_contiguous() || !o.is_contiguous()) {
+            TORCH_CHECK(g.is_non_overlapping_and_dense(), "gradients must be dense");
+            TORCH_CHECK(o.strides() == g.strides(), "an output must have its gradient's shape and strides");
         }
-        in[i] = grads[i].data_ptr();
-        out[i] = outs[i].data_ptr();
-        sizes[i] = grads[i].numel();
-        dtypes[i] = dtype_code(grads[i]);
+        in[i] = g.data_ptr();
+        out[i] = o.data_ptr();
+        sizes[i] = g.numel();
+        dtypes[i] = dtype_code(g);
     }
-    c10::cuda::CUDAGuard guard(grads[0].device());
-    at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+    c10::cuda::CUDAGuard guard(device);
+    at::Tensor norm = fresh({}, at::kFloat, *grads[0]);
     const size_t need = lf_clip_grad_norm_workspace_size(sizes.data(), (int64_t)n);
-    at::Tensor ws = workspace(need, grads[0]);
+    at::Tensor ws = workspace(need, *grads[0]);
     raise_on(lf_clip_grad_norm(in.data(), out.data(), sizes.data(), dtypes.data(), (int64_t)n, max_norm,
-                               (float*)norm.data_ptr(), mut(ws), need, stream_of(grads[0])),
+                               (float*)norm.data_ptr(), mut(ws), need, stream_of(*grads[0])),
              "ClipGradNorm");
     return norm;
 }
-
 
 // ---------------------------------------------------------------------------
 // Autograd nodes.  They live here rather than in Python because a small

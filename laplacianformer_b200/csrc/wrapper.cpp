@@ -147,5 +147,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           [=](const at::Tensor& x, const at::Tensor& wi, const at::Tensor& wo, const T& bi, const T& bo, const T& r,
               int64_t act) { return GatedFeedForward(x, wi, wo, t(bi), t(bo), t(r), act); },
           "GatedFeedForward (x, w_in, w_out, b_in, b_out, residual, activation) -> y, with autograd");
-    m.def("ClipGradNorm", &ClipGradNorm, "ClipGradNorm (grads, outs, max_norm) -> norm");
+    // Lists are read in place: a copied Tensor per gradient would cost more than the kernels on a small model.
+    auto tensors = [](const py::list& list) {
+        std::vector<const at::Tensor*> v(list.size());
+        for (size_t i = 0; i < v.size(); ++i) {
+            PyObject* p = PyList_GET_ITEM(list.ptr(), (Py_ssize_t)i);
+            TORCH_CHECK(THPVariable_Check(p), "tensors expected");
+            v[i] = &THPVariable_Unpack(p);
+        }
+        return v;
+    };
+    m.def("ClipGradNorm",
+          [=](const py::list& grads, const py::list& outs, double max_norm) {
+              return ClipGradNorm(tensors(grads), tensors(outs), max_norm);
+          },
+          "ClipGradNorm (grads, outs, max_norm) -> norm");
 }
