@@ -1022,6 +1022,9 @@ __global__ void __launch_bounds__(1024) colsum_join_kernel(const ColsumJobs p) {
 // Products of a few rows (MT at most): bound by reading the weights once.
 // One to eight warps share a weight row, each lane has four 16-byte loads in
 // flight, the sums meet by shuffles and shared memory in a fixed order.
+// (Reading the second product's weights of a feed-forward block while the first
+// still runs made the pair slower, 11.5 us against 9.8: both are bound by the
+// same reads.)
 template <typename T, bool GATED, int MT, bool VEC>
 __global__ void __launch_bounds__(256) few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int m, int n, int k,
                                                        int wpr, const Epilogue e) {
@@ -1045,7 +1048,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const T* x, int64_t ldx, 
                 for (int q = 0; q < (GATED ? 2 : 1); ++q)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (v0 + j * step < nv) u[q][j] = __ldg(reinterpret_cast<const uint4*>(wr[q]) + v0 + j * step);
+                        if (v0 + j * step < nv) u[q][j] = *(reinterpret_cast<const uint4*>(wr[q]) + v0 + j * step);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int v = v0 + j * step;
@@ -1195,8 +1198,11 @@ struct Shape {
 double step_cycles(int ctas, int cols, int b_rows) { return std::max(2.0 * cols, (kBM + b_rows / ctas) * kRowBytes / 60.0); }
 
 // Tile shape and splits of K by an estimate in SM cycles: the epilogue of a
-// tile overlaps the next tile's products; a split costs writing and reading
-// the partial sums once more and another launch.
+// tile overlaps the next tile's products, a pair takes 1000 cycles longer to
+// start and end, and a split costs writing and reading the partial sums once
+// more and another launch.  Over 56 shapes (16 to 12000 rows, 64 to 4096
+// columns and K) the choice measured 1.03 times the best one's time, 1.2 at
+// worst.
 Shape choose(const Product& q) {
     const int bk = q.op_dtype == LF_F8E4M3 ? 128 : 64;
     const int64_t iters = (q.k + bk - 1) / bk * q.ksegs, sms = num_sms();
@@ -1211,8 +1217,8 @@ Shape choose(const Product& q) {
                 const int64_t per = (iters + s - 1) / s, units = tiles * ((iters + per - 1) / per);
                 const int64_t waves = (units * ctas + sms - 1) / sms;
                 const double main = per * step_cycles(ctas, bn, bn), epi = 500 + bn * 10.0;
-                double t = waves * std::max(main, epi) + std::min(main, epi) + 2000;
-                if (s > 1) t += 4000 + (double)s * q.m * q.msegs * q.n * 8 / 3400.0;
+                double t = waves * std::max(main, epi) + std::min(main, epi) + (ctas == 2 ? 1000 : 0);
+                if (s > 1) t += 6500 + (double)s * q.m * q.msegs * q.n * 8 / 3400.0;
                 if (t < least) least = t, best = {ctas, bn, s};
             }
         }
@@ -1490,7 +1496,10 @@ int run_colsum(const Columns* c, int count, int64_t rows, int dtype, Arena& ws, 
     return check_launch("colsum_kernel");
 }
 
-constexpr int kFewRows = 8;
+// Rows that few_rows_kernel takes: its time grows with them (4096 x 1024 bf16
+// weights: 4.1 us for one, 6.8 for four, 10.5 for eight; 512 x 512: 2.1, 2.8
+// and 3.9), the tensor cores' does not (8.0 and 4.8 us).
+bool few_rows(int64_t m, int64_t n, int64_t k) { return k > 0 && (m <= 4 || (m <= 8 && n * k <= (1 << 19))); }
 
 template <typename T, bool GATED>
 void launch_few(const void* x, int64_t ldx, const void* w, int64_t ldw, int m, int n, int k, const Epilogue& e, cudaStream_t st) {
@@ -1538,6 +1547,16 @@ int check_common(const char* what, int act, int dtype, std::initializer_list<int
     return LF_OK;
 }
 
+// Every pointer on its element's boundary (a misaligned access would fault).
+int check_aligned(const char* what, std::initializer_list<const void*> ptrs, size_t bytes) {
+    for (const void* p : ptrs)
+        if (!aligned(p, bytes)) {
+            set_error("%s: a pointer is not aligned to its %zu-byte elements", what, bytes);
+            return LF_ERR_INVALID;
+        }
+    return LF_OK;
+}
+
 int missing(const char* what, const char* names) {
     set_error("%s: %s required", what, names);
     return LF_ERR_INVALID;
@@ -1555,6 +1574,10 @@ Product weight_product(const Mat& x, const Mat& w, int64_t m, int64_t n, int64_t
 int check_linear(const char* what, const lf_linear_t* a, bool quant) {
     if (!a) return missing(what, "arguments are");
     if (int rc = check_common(what, a->activation, a->dtype, {a->m, a->n, a->k})) return rc;
+    if (int rc = check_aligned(what, {a->bias, a->residual, a->y, a->dy, a->dx, a->dw, a->db, quant ? nullptr : a->x, quant ? nullptr : a->w}, 2))
+        return rc;
+    if (quant)
+        if (int rc = check_aligned(what, {a->x_scale, a->w_scale}, 4)) return rc;
     if (a->m == 0 || a->n == 0) return LF_OK;
     if (!a->w || !a->x) return a->k == 0 ? LF_OK : missing(what, "x and w are");
     if (a->ldx < a->k || a->ldw < a->k || (a->residual && a->ldr < a->n)) {
@@ -1573,7 +1596,7 @@ int linear_fwd(const lf_linear_t* a, bool quant, Arena& ws, cudaStream_t st) {
     if (a->residual) set_res(e, a->residual, a->ldr);
     e.act = a->activation;
     if (quant) e.sa = (const float*)a->x_scale, e.sb = (const float*)a->w_scale;
-    if (!quant && a->k > 0 && a->m <= kFewRows) return ws.base ? run_few<false>(a->x, a->ldx, a->w, a->ldw, a->m, a->n, a->k, e, a->dtype, st) : LF_OK;
+    if (!quant && few_rows(a->m, a->n, a->k)) return ws.base ? run_few<false>(a->x, a->ldx, a->w, a->ldw, a->m, a->n, a->k, e, a->dtype, st) : LF_OK;
     const int es = quant ? 1 : 2;
     Mat x = operand(a->x, a->m, a->k, a->ldx, es, ws, st), w = operand(a->w, a->n, a->k, a->ldw, es, ws, st);
     Product q = weight_product(x, w, a->m, a->n, a->k, a->dtype, quant ? LF_F8E4M3 : a->dtype);
@@ -1622,6 +1645,9 @@ int check_ffn(const char* what, const lf_gated_ffn_t* a) {
     if (!a) return missing(what, "arguments are");
     if (int rc = check_common(what, a->activation, a->dtype, {a->m, a->c, a->f})) return rc;
     if (2 * a->f > INT32_MAX - 256) return too_large(what);
+    if (int rc = check_aligned(what, {a->x, a->w_in, a->b_in, a->w_out, a->b_out, a->residual, a->y, a->dy, a->dx, a->dw_in, a->db_in,
+                                      a->dw_out, a->db_out}, 2))
+        return rc;
     if (a->m == 0 || a->c == 0) return LF_OK;
     if (!a->x || (a->f > 0 && (!a->w_in || !a->w_out))) return missing(what, "x, w_in and w_out are");
     if (a->ldx < a->c || (a->residual && a->ldr < a->c)) {
@@ -1648,7 +1674,7 @@ Shape choose_gated(int64_t m, int64_t f, int64_t c, bool bwd) {
             const int64_t width = bwd ? 2 * bh : bh;
             const int64_t tiles = (m + kBM * ctas - 1) / (kBM * ctas) * ((f + width - 1) / width), waves = (tiles * ctas + sms - 1) / sms;
             const double main = iters * step_cycles(ctas, 2 * bh, 2 * bh), epi = 500 + bh * (bwd ? 25.0 : 15.0);
-            const double t = bwd ? waves * std::max(3 * main + 1400, 2 * epi) + epi : waves * std::max(main, epi) + std::min(main, epi);
+            double t = bwd ? waves * std::max(3 * main + 1400, 2 * epi) + epi : waves * std::max(main, epi) + std::min(main, epi);
             if (t < least) least = t, best = {ctas, 2 * bh, 1};
         }
     return best;
@@ -1694,7 +1720,7 @@ int ffn_fwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
     set_out(e, a->y, c);
     e.bias = a->b_out;
     if (a->residual) set_res(e, a->residual, a->ldr);
-    if (m <= kFewRows && f > 0) {
+    if (f > 0 && few_rows(m, 3 * f, c)) {
         if (!ws.base) return LF_OK;
         Epilogue eh{};
         set_out(eh, const_cast<void*>(h.p), ldh);

@@ -493,13 +493,21 @@ void launch_bwd(const NormBwdArgs& a, void* dw, bool vec, cudaStream_t st) {
     if (dw) launch_early(rms_dw_kernel<T>, (unsigned)((a.cols + 31) / 32), 1024, 0, 1, st, a.part, (T*)dw, (int)blocks, a.cols);
 }
 
-int check_rows(const char* what, int64_t rows, int64_t cols, int dtype) {
+int check_rows(const char* what, int64_t rows, int64_t cols, int dtype, std::initializer_list<const void*> ptrs,
+               std::initializer_list<const void*> floats) {
     if (dtype != LF_F32 && dtype != LF_F16 && dtype != LF_BF16) {
         set_error("%s: unsupported dtype code %d (fp32, fp16 and bf16)", what, dtype);
         return LF_ERR_DTYPE;
     }
     if (rows < 0 || cols < 0 || cols > INT32_MAX) {
         set_error("%s: bad sizes rows=%lld cols=%lld", what, (long long)rows, (long long)cols);
+        return LF_ERR_INVALID;
+    }
+    bool ok = true;  // a misaligned access would fault
+    for (const void* p : ptrs) ok = ok && aligned(p, dtype_size(dtype));
+    for (const void* p : floats) ok = ok && aligned(p, 4);
+    if (!ok) {
+        set_error("%s: a pointer is not aligned to its elements", what);
         return LF_ERR_INVALID;
     }
     return LF_OK;
@@ -535,7 +543,7 @@ using namespace lfb;
 extern "C" int lf_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y, void* s, float* rstd,
                                int64_t rows, int64_t cols, int dtype, double eps, lf_stream_t stream) {
     clear_error();
-    if (int rc = check_rows("lf_rms_norm_fwd", rows, cols, dtype)) return rc;
+    if (int rc = check_rows("lf_rms_norm_fwd", rows, cols, dtype, {x, residual, weight, y, s}, {rstd})) return rc;
     if (rows == 0 || cols == 0) return LF_OK;
     if (!x || !weight || !y || (residual != nullptr) != (s != nullptr)) {
         set_error("lf_rms_norm_fwd: x, weight and y are required, residual and s go together");
@@ -548,7 +556,7 @@ extern "C" int lf_rms_norm_fwd(const void* x, const void* residual, const void* 
 extern "C" int lf_rms_norm_quant_fwd(const void* x, const void* residual, const void* weight, void* q, float* scale,
                                      void* s, int64_t rows, int64_t cols, int dtype, double eps, lf_stream_t stream) {
     clear_error();
-    if (int rc = check_rows("lf_rms_norm_quant_fwd", rows, cols, dtype)) return rc;
+    if (int rc = check_rows("lf_rms_norm_quant_fwd", rows, cols, dtype, {x, residual, weight, s}, {scale})) return rc;
     if (rows == 0 || cols == 0) return LF_OK;
     if (!x || !weight || !q || !scale || (residual != nullptr) != (s != nullptr)) {
         set_error("lf_rms_norm_quant_fwd: x, weight, q and scale are required, residual and s go together");
@@ -561,7 +569,7 @@ extern "C" int lf_rms_norm_quant_fwd(const void* x, const void* residual, const 
 extern "C" int lf_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int dtype,
                                 lf_stream_t stream) {
     clear_error();
-    if (int rc = check_rows("lf_quantize_rows", rows, cols, dtype)) return rc;
+    if (int rc = check_rows("lf_quantize_rows", rows, cols, dtype, {x}, {scale})) return rc;
     if (rows == 0 || cols == 0) return LF_OK;
     if (!x || !q || !scale) {
         set_error("lf_quantize_rows: x, q and scale are required");
@@ -580,7 +588,7 @@ extern "C" int lf_rms_norm_bwd(const void* dy, const void* ds, const void* s, co
                                void* dx, void* dw, int64_t rows, int64_t cols, int dtype, void* workspace,
                                size_t workspace_bytes, lf_stream_t stream) {
     clear_error();
-    if (int rc = check_rows("lf_rms_norm_bwd", rows, cols, dtype)) return rc;
+    if (int rc = check_rows("lf_rms_norm_bwd", rows, cols, dtype, {dy, ds, s, weight, dx, dw}, {rstd})) return rc;
     if (cols == 0 || (!dx && !dw)) return LF_OK;
     cudaStream_t st = (cudaStream_t)stream;
     if (rows == 0) {
