@@ -179,7 +179,7 @@ struct Epilogue {
     int64_t ldo, ldr;
     int act;
     bool act_bwd, vec_out, vec_res;
-    bool tma;                // the output's rows can be written by TMA (set by run_product)
+    bool tma, pairs;         // the output's rows can be written by TMA; their elements in pairs
 };
 
 template <int ACT>
@@ -365,19 +365,6 @@ __device__ __forceinline__ void sync_all() {
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t* r = reinterpret_cast<uint32_t*>(v);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-        "%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-
 struct Tile {
     int seg, m0, n0, split, it0, it1;
 };
@@ -595,6 +582,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             __syncwarp();
             if (lane == 0 && some) tma_store(out, st, col, row, plane);
         };
+        // The same for rows that TMA cannot address: 64-byte row segments by
+        // 4-byte stores (PAIRS: rows and columns even) or 2-byte ones.
+        auto put_rows = [&](T* out, int64_t ld, int rows, int cols, bool pairs) {
+            __syncwarp();
+            if (pairs) {
+                const int c = (lane & 15) * 2, r0 = lane >> 4;
+                T* o = out + r0 * ld + c;
+#pragma unroll 4
+                for (int r = r0; r < 32; r += 2, o += 2 * ld)
+                    if (r < rows && c < cols) *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(stage_at(st, r, c >> 3) + (c & 7) * 2);
+            } else {
+                T* o = out + lane;
+#pragma unroll 4
+                for (int r = 0; r < 32; ++r, o += ld)
+                    if (r < rows && lane < cols) *o = *reinterpret_cast<const T*>(stage_at(st, r, lane >> 3) + (lane & 7) * 2);
+            }
+        };
         auto reuse = [&] {
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
@@ -626,7 +630,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                 const uint32_t acc = tmem + buf * 256 + lanes;
                 const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
                 const int first = cg * 32;
-                if (e.tma) {
+                if (!p.part) {
                     // Finished in the accumulator's layout (a lane owns a
                     // row); the column values and the residual of the next
                     // columns are fetched ahead.
@@ -638,6 +642,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         bias = column_value((const T*)e.bias, col, p.n);
                         if (FP8) sb = col < p.n ? e.sb[col] : 1.f;
                         if (!e.res) return;
+                        if (!e.vec_res) {  // a column per lane, two rows per register
+                            const T* q = (const T*)e.res + row0 * e.ldr + col;
+                            uint32_t* w = reinterpret_cast<uint32_t*>(r);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i, q += 2 * e.ldr) {
+                                const T a = 2 * i < rows && col < p.n ? q[0] : Elem<T>::store(0.f);
+                                const T b = 2 * i + 1 < rows && col < p.n ? q[e.ldr] : Elem<T>::store(0.f);
+                                w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&a) | (uint32_t)*reinterpret_cast<const uint16_t*>(&b) << 16;
+                            }
+                            return;
+                        }
                         const T* q = (const T*)e.res + (row0 + (lane >> 2)) * e.ldr + col8;
 #pragma unroll
                         for (int i = 0; i < 4; ++i, q += 8 * e.ldr)
@@ -650,9 +665,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         reuse();
                         if (FP8) cs[lane] = sb, cs[32 + lane] = Elem<T>::load(bias);
                         else if (e.bias) cv[lane] = bias;
-                        if (e.res) {  // to the lane that owns the row
+                        if (e.res && e.vec_res) {  // to the lane that owns the row
 #pragma unroll
                             for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
+                        } else if (e.res) {
+                            const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                *reinterpret_cast<uint16_t*>(stage_at(st, 2 * i, lane >> 3) + (lane & 7) * 2) = (uint16_t)w[i];
+                                *reinterpret_cast<uint16_t*>(stage_at(st, 2 * i + 1, lane >> 3) + (lane & 7) * 2) = (uint16_t)(w[i] >> 16);
+                            }
                         }
                         fetch(c0 + kEpiCols);
                         __syncwarp();
@@ -702,64 +724,34 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         __syncwarp();
                         stage16(st, lane, 0, o[0]);
                         stage16(st, lane, 1, o[1]);
-                        put(&p.out, t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
+                        if (e.tma) put(&p.out, t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
+                        else put_rows((T*)e.out + row0 * e.ldo + t.n0 + c0, e.ldo, rows, cend - c0, e.pairs);
                     }
                 } else {
-                    // Any alignment, and split-K partials: raw sums through
-                    // shared memory, 16 columns at a time, so that a lane has
-                    // four columns of four rows.
+                    // Split-K partials: raw sums through shared memory, 16
+                    // columns at a time, as row segments.
                     if (!(ok = mbar_wait(tf, bph))) break;
                     tc_fence_after();
+                    reuse();  // the last tile may have been another problem's
                     for (int c0 = first; c0 < cend; c0 += kEpiCols) {
 #pragma unroll 1
                         for (int h = 0; h < 2; ++h) {
-                            const int col = t.n0 + c0 + h * 16 + (lane & 3) * 4;
+                            const int col = t.n0 + c0 + h * 16 + (lane & 3) * 4, row = lane >> 2;
                             float v[16];
                             tmem_ld16(acc + c0 + h * 16, v);
                             tmem_wait_ld();
                             reg_fence(v);
                             if (c0 == last && h == 1) release(&tempty[buf]);
+                            __syncwarp();
 #pragma unroll
                             for (int c = 0; c < 4; ++c)
-                                *reinterpret_cast<float4*>(stage_at(st, lane, c)) =
-                                    make_float4(v[4 * c] * sa, v[4 * c + 1] * sa, v[4 * c + 2] * sa, v[4 * c + 3] * sa);
+                                *reinterpret_cast<float4*>(stage_at(st, lane, c)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
                             __syncwarp();
-                            const int row = lane >> 2;
-                            if (p.part) {
-                                float* q = p.part + ((int64_t)t.split * p.msegs * p.m + row0 + row) * p.ldp + col;
+                            float* q = p.part + ((int64_t)t.split * p.msegs * p.m + row0 + row) * p.ldp + col;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i, q += 8 * p.ldp)
-                                    if (i * 8 + row < rows && col < p.ldp)
-                                        *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(stage_at(st, i * 8 + row, lane & 3));
-                            } else {
-                                uint2 r[4];
-                                float4 b = make_float4(0.f, 0.f, 0.f, 0.f), sb = b;
-                                if (e.res) {
-                                    const T* q = (const T*)e.res + (row0 + row) * e.ldr;
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i, q += 8 * e.ldr)
-                                        r[i] = i * 8 + row < rows ? load4(q, col, p.n, e.vec_res) : make_uint2(0u, 0u);
-                                }
-                                if (e.bias) b = widen4<T>(load4((const T*)e.bias, col, p.n, false));
-                                if (FP8) {
-                                    float* q = reinterpret_cast<float*>(&sb);
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) q[j] = col + j < p.n ? e.sb[col + j] : 0.f;
-                                }
-                                T* out = (T*)e.out + (row0 + row) * e.ldo;
-                                with_act(e.act, [&](auto act) {
-                                    T* q = out;
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i, q += 8 * e.ldo)
-                                        if (i * 8 + row < rows) {
-                                            float4 z = *reinterpret_cast<const float4*>(stage_at(st, i * 8 + row, lane & 3));
-                                            if (FP8) z.x *= sb.x, z.y *= sb.y, z.z *= sb.z, z.w *= sb.w;
-                                            const float4 x = e.res ? widen4<T>(r[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
-                                            store4(q, col, p.n, e.vec_out, finish4<decltype(act)::value>(z, b, x, e.act_bwd));
-                                        }
-                                });
-                            }
-                            __syncwarp();
+                            for (int i = 0; i < 4; ++i, q += 8 * p.ldp)
+                                if (i * 8 + row < rows && col < p.ldp)
+                                    *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(stage_at(st, i * 8 + row, lane & 3));
                         }
                     }
                 }
@@ -1203,7 +1195,7 @@ double step_cycles(int ctas, int cols, int b_rows) { return std::max(2.0 * cols,
 // more and another launch.  Over 56 shapes (16 to 12000 rows, 64 to 4096
 // columns and K) the choice measured 1.03 times the best one's time, 1.2 at
 // worst.
-Shape choose(const Product& q) {
+Shape choose(const Product& q, double* cycles = nullptr) {
     const int bk = q.op_dtype == LF_F8E4M3 ? 128 : 64;
     const int64_t iters = (q.k + bk - 1) / bk * q.ksegs, sms = num_sms();
     Shape best{1, 256, 1};
@@ -1222,44 +1214,56 @@ Shape choose(const Product& q) {
                 if (t < least) least = t, best = {ctas, bn, s};
             }
         }
+    if (cycles) *cycles = least;
     return best;
 }
 
-// The same for several products that share a launch (one CTA count and ring):
-// the widest tile that costs least work for each, and splits where a unit
-// would be longer than a quarter of the whole launch.
+// The same for several products that share a launch (one CTA count): for each
+// the widest tile that costs least work, and splits where a unit would be
+// longer than a share of the whole launch (several shares are tried).
 double choose_together(const Product* q, int count, int ctas, Shape* out) {
     const double lanes = (double)num_sms() / ctas;
-    double work = 0, unit[3] = {}, longest = 0, join = 0;
-    int64_t units[3];
-    auto fill = [&](int i, int bn, int s) {
-        const int64_t iters = (q[i].k + 63) / 64 * q[i].ksegs, per = (iters + s - 1) / s;
-        units[i] = (q[i].m + kBM * ctas - 1) / (kBM * ctas) * q[i].msegs * ((q[i].n + bn - 1) / bn) * ((iters + per - 1) / per);
-        unit[i] = std::max(per * step_cycles(ctas, bn, bn), 500 + bn * 10.0);
-        out[i] = {ctas, bn, s};
-        return units[i] * unit[i];
+    double total = 0, least = 1e30;
+    int bn_of[3];
+    auto unit = [&](int i, int bn, int s) {
+        const int64_t iters = (q[i].k + 63) / 64 * q[i].ksegs;
+        return std::max(((iters + s - 1) / s) * step_cycles(ctas, bn, bn), 500 + bn * 10.0);
+    };
+    auto tiles = [&](int i, int bn) {
+        return (double)((q[i].m + kBM * ctas - 1) / (kBM * ctas) * q[i].msegs * ((q[i].n + bn - 1) / bn));
     };
     for (int i = 0; i < count; ++i) {
-        int best = 256;
-        double least = 1e30;
+        double best = 1e30;
         for (int bn : {256, 128, 64}) {
             if (ctas == 2 && bn == 64) continue;
-            const double w = fill(i, bn, 1);
-            if (w < 0.99 * least) least = w, best = bn;
+            const double w = tiles(i, bn) * unit(i, bn, 1);
+            if (w < 0.99 * best) best = w, bn_of[i] = bn;
         }
-        work += fill(i, best, 1);
+        total += best;
     }
-    const double limit = std::max(0.25 * work / lanes, 3000.0);
-    work = 0;
-    for (int i = 0; i < count; ++i) {
-        const int64_t iters = (q[i].k + 63) / 64 * q[i].ksegs;
-        int s = 1;
-        while (unit[i] > limit && s < 64 && iters / (2 * s) >= 4) fill(i, out[i].bn, s *= 2);
-        work += units[i] * unit[i];
-        longest = std::max(longest, unit[i]);
-        if (s > 1) join += (double)s * q[i].m * q[i].msegs * q[i].n * 8 / 3400.0;
+    for (double share : {0.12, 0.25, 0.5, 1.0, 2.0}) {
+        const double limit = std::max(share * total / lanes, 2000.0);
+        double work = 0, longest = 0, shortest = 1e30, filler = 0, join = 0;
+        Shape s[3];
+        for (int i = 0; i < count; ++i) {
+            const int64_t iters = (q[i].k + 63) / 64 * q[i].ksegs;
+            int n = 1;
+            while (unit(i, bn_of[i], n) > limit && n < 64 && iters / (2 * n) >= 4) n *= 2;
+            const double u = unit(i, bn_of[i], n);
+            work += tiles(i, bn_of[i]) * n * u;
+            longest = std::max(longest, u);
+            if (u < shortest) shortest = u, filler = tiles(i, bn_of[i]) * n * u / lanes;
+            if (n > 1) join += (double)n * q[i].m * q[i].msegs * q[i].n * 8 / 3400.0;
+            s[i] = {ctas, bn_of[i], n};
+        }
+        // Short units even out what the long ones leave, where there are enough of them.
+        const double t = std::max(longest, work / lanes + 0.5 * (filler >= longest ? shortest : longest)) + (join > 0 ? 6500 + join : 0) + (ctas == 2 ? 1000 : 0);
+        if (t < least) {
+            least = t;
+            for (int i = 0; i < count; ++i) out[i] = s[i];
+        }
     }
-    return work / lanes + 0.5 * longest + join + (join > 0 ? 4000 : 0);
+    return least;
 }
 
 size_t part_bytes(const Product& q, const Shape& s) {
@@ -1333,7 +1337,9 @@ int fill_problem(Problem& g, const Product& q, const Shape& s, float* part) {
     g.a_mn = q.a_mn, g.b_mn = q.b_mn;
     g.idesc = idesc_of(q.op_dtype, q.a_mn, q.b_mn, s.ctas, s.bn);
     g.e = q.e;
-    g.e.tma = !part && tma_ok(q.e.out, q.e.ldo, 2) && (!q.e.res || (q.n % 8 == 0 && tma_ok(q.e.res, q.e.ldr, 2)));
+    g.e.tma = !part && tma_ok(q.e.out, q.e.ldo, 2);
+    g.e.pairs = q.n % 2 == 0 && q.e.ldo % 2 == 0 && aligned(q.e.out, 4);
+    g.e.vec_res = q.n % 8 == 0 && tma_ok(q.e.res, q.e.ldr, 2);  // here: whole 16-byte chunks
     if (g.e.tma && !encode_out(&g.out, {q.e.out, q.n, q.m, q.e.ldo, q.msegs, q.m * q.e.ldo}, q.dtype)) return LF_ERR_CUDA;
     g.part = part;
     g.ldp = up(q.n, 4);
@@ -1383,7 +1389,19 @@ int run_products(const Product* in, int given, Arena& ws, cudaStream_t st) {
     if (count == 0) return LF_OK;
     if (count == 1) return run_product(q[0], ws, st);
     Shape one[3], two[3];
-    const Shape* s = choose_together(q, count, 2, two) <= choose_together(q, count, 1, one) ? two : one;
+    const double pairs = choose_together(q, count, 2, two), singles = choose_together(q, count, 1, one);
+    const Shape* s = pairs <= singles ? two : one;
+    double apart = 0;
+    for (int i = 0; i < count; ++i) {
+        double t;
+        choose(q[i], &t);
+        apart += t + 2500;  // a launch after the first
+    }
+    if (apart - 2500 < std::min(pairs, singles)) {
+        for (int i = 0; i < count; ++i)
+            if (int rc = run_product(q[i], ws, st)) return rc;
+        return LF_OK;
+    }
     float* part[3] = {};
     for (int i = 0; i < count; ++i)
         if (s[i].splits > 1) part[i] = (float*)ws.take(part_bytes(q[i], s[i]));
