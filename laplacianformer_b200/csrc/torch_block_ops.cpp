@@ -78,15 +78,15 @@ Rows as_rows(const at::Tensor& t) {
     const int64_t cols = t.size(-1);
     if (t.is_contiguous()) return {t, cols};
     if (t.numel() && (cols == 1 || t.stride(-1) == 1)) {
-        int64_t ld = 0, span = 1;  // rows so far are ld apart, span of them
+        int64_t ld = cols, span = 1;  // rows so far are ld apart, span of them
         bool merges = true;
         for (int64_t i = t.dim() - 2; i >= 0 && merges; --i) {
             if (t.size(i) == 1) continue;
-            if (!ld) ld = t.stride(i);
+            if (span == 1) ld = t.stride(i);
             else merges = t.stride(i) == ld * span;
             span *= t.size(i);
         }
-        if (merges && (ld >= cols || !ld)) return {t, ld ? ld : cols};
+        if (merges && ld >= cols) return {t, ld};  // (expanded rows have a stride of zero)
     }
     return {t.contiguous(), cols};
 }

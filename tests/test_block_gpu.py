@@ -294,6 +294,30 @@ def test_linear_strided_and_unaligned(dtype, m):
 
 
 @pytest.mark.parametrize("dtype", DT16)
+def test_expanded_operands(dtype):
+    """Broadcast inputs and gradients have strides of zero: every operand expanded equals its dense copy."""
+    g = gen("expanded", dtype)
+    m, k, n, f = 40, 64, 48, 72
+    x, w, b, r, dy = rand(g, dtype, 1, k).expand(m, k), rand(g, dtype, n, k, scale=0.1), rand(g, dtype, 1).expand(n), \
+        rand(g, dtype, 1, n).expand(m, n), rand(g, dtype, 1, n).expand(m, n)
+    wi, wo, dz = rand(g, dtype, 2 * f, k, scale=0.1), rand(g, dtype, k, f, scale=0.1), rand(g, dtype, m, 1).expand(m, k)
+    wn, dr = rand(g, dtype, 1).expand(k), rand(g, dtype, 1, k).expand(m, k)
+
+    def run(*t):
+        x, w, b, r, dy, wi, wo, dz, wn, dr = t
+        leaf = x.detach().requires_grad_()
+        y = ops.linear(leaf, w, b, activation="silu", residual=r)
+        h = ops.gated_feed_forward(leaf, wi, wo, residual=dz)
+        q, s = ops.rms_norm(leaf, wn, residual=dr)
+        return (y, h, q, s, *(torch.autograd.grad(o, leaf, d)[0] for o, d in ((y, dy), (h, dz), (q, dr))), *ops.rms_norm_quant(x, wn)[:1])
+
+    expanded = (x, w, b, r, dy, wi, wo, dz, wn, dr)
+    for a, c in zip(run(*expanded), run(*(t.contiguous() for t in expanded))):
+        assert torch.equal(a.float(), c.float())
+    assert torch.equal(ops.linear(x.view(1, m, k).expand(3, m, k), w), ops.linear(x.contiguous(), w).expand(3, m, n))
+
+
+@pytest.mark.parametrize("dtype", DT16)
 @pytest.mark.parametrize("shape", [(1, 64, 64), (1, 1000, 512), (7, 33, 96), (128, 256, 128), (200, 96, 144), (300, 515, 1040),
                                    (65, 40, 131), (1000, 1536, 512)])
 @pytest.mark.parametrize("kind", ["plain", "bias silu residual"])
