@@ -10,11 +10,22 @@
 //
 // One persistent kernel (tc_gemm_kernel) runs every product: operands come
 // through TMA into a ring of 128-byte-swizzled stages, one warp issues the
-// tcgen05 products into accumulators in tensor memory, and eight warps turn
+// tcgen05 products into accumulators in tensor memory, and sixteen warps turn
 // finished accumulators into outputs while the next tile's products run.
 // Either operand may be stored K-major or transposed (MN-major), so no
 // product needs a transposed copy.  The backward passes recompute z, g, u and
-// h from x in 32 bits instead of reading rounded copies of them back.
+// h from x in 32 bits instead of reading rounded copies of them back: a
+// feed-forward block keeps nothing but its input between the passes, and its
+// gradients have one 16-bit rounding less, for 2 of 11 units of arithmetic.
+//
+// Roundings to 16 bits besides the outputs': h, dg, du and dz, as operands of
+// the products that follow (the tensor cores take 16-bit operands; a second
+// part of each would double those products).
+//
+// Measured on a B200 (131072 tokens, 1024 channels, 4096 hidden, bf16): gated
+// forward 1.4-1.6 ms (1.4-1.5 PFLOP/s, tensor pipe 95 % active), gated backward
+// 2.75 ms (1.2), down projection 0.81 ms (1.36), the three gradients' products
+// 3.84 ms (1.43), against cuBLAS's 1.38 PFLOP/s under the same power cap.
 #include <cuda.h>
 
 #include <algorithm>
@@ -204,6 +215,11 @@ enum Mode { kLinear, kGated, kGatedBwd };
 
 constexpr int kBM = 128;                  // rows of a tile per CTA
 constexpr int kRowBytes = 128;            // a stage holds 128 bytes of K: 64 16-bit or 128 8-bit elements
+// Sixteen warps hide the epilogue's latencies (eight: 225 against 197 us for
+// 100352 x 64 x 256, forward and backward) at 96 registers each, which the
+// epilogues keep to by 16 columns at a time: the stages leave hardly any L1,
+// so spilled registers cost an L2 round trip (59 against 38 us for the 8-bit
+// 25088 x 512 -> 1536).
 constexpr int kEpiWarps = 16;             // four per 32-lane quarter of the tensor memory
 constexpr int kControlWarps = 3;          // copies of A, products, copies of B
 constexpr int kGemmThreads = 32 * (kControlWarps + kEpiWarps);
@@ -430,7 +446,9 @@ __device__ __forceinline__ T column_value(const T* p, int col, int n) {
 // A CTA (CTAS = 1) or a pair of CTAs on two SMs (CTAS = 2) walks tiles of
 // 128 CTAS rows.  In a pair every CTA holds its own rows of A, half of B's
 // columns and the accumulators of its own rows; its first CTA issues the
-// products of both.
+// products of both.  A 256-column pair tile fetches 64 bytes per cycle and SM
+// where a single CTA's fetches 96, more than L2 delivers (131072 x 1024 x 4096:
+// 10.1 against 14.7 ms, forward and backward).
 //
 // kLinear: out = epilogue(A B^T), two accumulator buffers.
 // kGated: B's tile is bn/2 gate and bn/2 up rows of Win, the accumulator's
