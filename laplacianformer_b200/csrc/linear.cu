@@ -438,6 +438,25 @@ __device__ __forceinline__ void add_columns(float (&v)[16], const T* p) {
     }
 }
 
+// Writes staged outputs to rows that TMA cannot address: 64-byte row segments by
+// 4-byte stores (pairs: rows and columns even) or 2-byte ones.
+template <typename T>
+__device__ __forceinline__ void put_rows(uint8_t* st, int lane, T* out, int64_t ld, int rows, int cols, bool pairs) {
+    __syncwarp();
+    if (pairs) {
+        const int c = (lane & 15) * 2, r0 = lane >> 4;
+        T* o = out + r0 * ld + c;
+#pragma unroll 4
+        for (int r = r0; r < 32; r += 2, o += 2 * ld)
+            if (r < rows && c < cols) *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(stage_at(st, r, c >> 3) + (c & 7) * 2);
+    } else {
+        T* o = out + lane;
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r, o += ld)
+            if (r < rows && lane < cols) *o = *reinterpret_cast<const T*>(stage_at(st, r, lane >> 3) + (lane & 7) * 2);
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ T column_value(const T* p, int col, int n) {
     return p && col < n ? p[col] : Elem<T>::store(0.f);
@@ -600,23 +619,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             __syncwarp();
             if (lane == 0 && some) tma_store(out, st, col, row, plane);
         };
-        // The same for rows that TMA cannot address: 64-byte row segments by
-        // 4-byte stores (PAIRS: rows and columns even) or 2-byte ones.
-        auto put_rows = [&](T* out, int64_t ld, int rows, int cols, bool pairs) {
-            __syncwarp();
-            if (pairs) {
-                const int c = (lane & 15) * 2, r0 = lane >> 4;
-                T* o = out + r0 * ld + c;
-#pragma unroll 4
-                for (int r = r0; r < 32; r += 2, o += 2 * ld)
-                    if (r < rows && c < cols) *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(stage_at(st, r, c >> 3) + (c & 7) * 2);
-            } else {
-                T* o = out + lane;
-#pragma unroll 4
-                for (int r = 0; r < 32; ++r, o += ld)
-                    if (r < rows && lane < cols) *o = *reinterpret_cast<const T*>(stage_at(st, r, lane >> 3) + (lane & 7) * 2);
-            }
-        };
         auto reuse = [&] {
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
@@ -743,7 +745,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
                         stage16(st, lane, 0, o[0]);
                         stage16(st, lane, 1, o[1]);
                         if (e.tma) put(&p.out, t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
-                        else put_rows((T*)e.out + row0 * e.ldo + t.n0 + c0, e.ldo, rows, cend - c0, e.pairs);
+                        else put_rows<T>(st, lane, (T*)e.out + row0 * e.ldo + t.n0 + c0, e.ldo, rows, cend - c0, e.pairs);
                     }
                 } else {
                     // Split-K partials: raw sums through shared memory, 16
@@ -878,6 +880,281 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
     if (warp == 1) tmem_free<CTAS>(tmem);
 #undef LFB_EACH_UNIT
 #undef LFB_PROBLEM
+}
+
+// ---------------------------------------------------------------------------
+// The feed-forward block's forward for at most 128 channels, in one kernel
+// ---------------------------------------------------------------------------
+// With so few channels the products are short and h is most of the traffic (at
+// 64 channels and 256 hidden columns 102 of 140 MB per 100,000 tokens), so h
+// never leaves the SM: a CTA owns 128 tokens and walks the hidden columns in
+// blocks of 64,
+//   [g|u] = x [Wg|Wu]^T      (two accumulator buffers)
+//   h = act(g) u             to shared memory as the next product's A operand
+//   y += h Wout^T            (accumulators of two tiles in turn)
+// One warp issues both products, the next block's first one ahead of this
+// block's second; two groups of eight warps take the blocks in turn, and a
+// tile's y goes to the group of its last block, after that group's next block.
+constexpr int kHB = 64;                   // hidden columns of a block
+constexpr int kNarrow = 128;              // channels
+
+struct alignas(64) NarrowArgs {
+    CUtensorMap x, win, wout, out;
+    Epilogue e;                // out, output bias, residual, activation of the gate
+    const void* b_in;
+    int m, c, f, tiles, blocks, kc, stages;  // kc: 64-channel blocks
+    uint32_t idesc1, idesc2;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __grid_constant__ NarrowArgs p) {
+    extern __shared__ __align__(1024) uint8_t smem[];  // x (two tiles), h (two blocks), weight stages, staging, barriers
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int x_bytes = p.kc * kBM * kRowBytes, w_bytes = p.kc * 3 * kHB * kRowBytes;
+    constexpr int kHBytes = kBM * kRowBytes;
+    uint8_t* const hs = smem + 2 * x_bytes;
+    uint8_t* const ring = hs + 2 * kHBytes;
+    uint8_t* const out_stage = ring + p.stages * w_bytes;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * (kStageOut + column_bytes<false>()));
+    uint64_t *wfull = bars, *wempty = bars + 6, *xfull = bars + 12, *xempty = bars + 14, *gfull = bars + 16, *gempty = bars + 18,
+             *hfull = bars + 20, *hempty = bars + 22, *yfull = bars + 24, *yempty = bars + 26, *drain = bars + 28;
+    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 29);
+    constexpr int kY = 256;                                    // tensor memory columns of y
+    grid_release();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) mbar_init(&wfull[i], 1), mbar_init(&wempty[i], 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&xfull[i], 1), mbar_init(&xempty[i], 1), mbar_init(&gfull[i], 1), mbar_init(&gempty[i], 8);
+            mbar_init(&hfull[i], 8), mbar_init(&hempty[i], 1), mbar_init(&yfull[i], 1), mbar_init(&yempty[i], 8);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_take<1>(tmem_ptr);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_wait();
+    const uint32_t tmem = *tmem_ptr;
+    const int mine = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // this CTA's tiles
+    const int total = mine * p.blocks;                                                  // and their blocks
+    bool ok = true;
+
+    if (warp == 0) {  // x tiles
+        if (elect_one()) {
+            for (int t = 0; ok && t < mine; ++t) {
+                const int b = t & 1;
+                if (!(ok = mbar_wait(&xempty[b], (t >> 1 & 1) ^ 1))) break;
+                mbar_expect(&xfull[b], x_bytes);
+                for (int k = 0; k < p.kc; ++k)
+                    tma_load<1>(smem + b * x_bytes + k * kBM * kRowBytes, &p.x, smem_u32(&xfull[b]), k * 64,
+                                (int)(blockIdx.x + t * gridDim.x) * kBM, 0);
+            }
+            if (!ok)  // a wait ran out: let the copies in flight land
+                for (int t = max(0, mine - 2); t < mine; ++t) mbar_wait(&xfull[t & 1], t >> 1 & 1, 100000000ull);
+        }
+        __syncwarp();
+    } else if (warp == 2) {  // weights: per block 64 gate and 64 up rows of Win by 64 channels, then Wout's columns
+        if (elect_one()) {
+            int s = 0, j = 0, issued = 0;
+            uint32_t ph = 0;
+            for (int g = 0; g < total; ++g) {
+                if (!(ok = mbar_wait(&wempty[s], ph ^ 1))) break;
+                uint8_t* dst = ring + s * w_bytes;
+                const uint32_t bar = smem_u32(&wfull[s]);
+                mbar_expect(&wfull[s], w_bytes);
+                for (int k = 0; k < p.kc; ++k)
+                    for (int half = 0; half < 2; ++half)
+                        tma_load<1>(dst + (2 * k + half) * kHB * kRowBytes, &p.win, bar, k * 64, j * kHB, half);
+                tma_load<1>(dst + 2 * p.kc * kHB * kRowBytes, &p.wout, bar, j * kHB, 0, 0);
+                ++issued;
+                if (++j == p.blocks) j = 0;
+                if (++s == p.stages) s = 0, ph ^= 1;
+            }
+            if (!ok)
+                for (int k = max(0, issued - p.stages); k < issued; ++k)
+                    mbar_wait(&wfull[k % p.stages], (k / p.stages) & 1, 100000000ull);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t go = elect_one() ? 1u : 0u;
+        int s1 = 0, s2 = 0, j1 = 0, j2 = 0, t1 = 0, t2 = 0;    // stage, block and tile of the first and of the second product
+        uint32_t ph1 = 0;
+        for (int g = 0; ok && g <= total; ++g) {
+            if (g < total) {
+                const int b = g & 1;
+                if (j1 == 0) ok = mbar_wait(&xfull[t1 & 1], t1 >> 1 & 1);
+                ok = ok && mbar_wait(&wfull[s1], ph1) && mbar_wait(&gempty[b], (g >> 1 & 1) ^ 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t sx = smem_u32(smem + (t1 & 1) * x_bytes), sw = smem_u32(ring + s1 * w_bytes);
+                for (int k = 0; k < p.kc; ++k) {
+                    const uint64_t da = make_desc(sx + k * kBM * kRowBytes, 16, 1024), db = make_desc(sw + 2 * k * kHB * kRowBytes, 16, 1024);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mma<1, false>(tmem + b * 128, da + i * 2, db + i * 2, p.idesc1, k > 0 || i > 0 ? 1u : 0u, go);
+                }
+                if (go) commit<1>(&gfull[b]);
+                if (++j1 == p.blocks) {
+                    if (go) commit<1>(&xempty[t1 & 1]);
+                    j1 = 0, ++t1;
+                }
+                if (++s1 == p.stages) s1 = 0, ph1 ^= 1;
+            }
+            if (g > 0) {
+                const int b = (g - 1) & 1;
+                if (j2 == 0) ok = mbar_wait(&yempty[t2 & 1], (t2 >> 1 & 1) ^ 1);
+                ok = ok && mbar_wait(&hfull[b], (g - 1) >> 1 & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t da = make_desc(smem_u32(hs + b * kHBytes), 16, 1024);
+                const uint64_t db = make_desc(smem_u32(ring + s2 * w_bytes) + 2 * p.kc * kHB * kRowBytes, 16, 1024);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kY + (t2 & 1) * 128, da + i * 2, db + i * 2, p.idesc2, j2 > 0 || i > 0 ? 1u : 0u, go);
+                if (go) commit<1>(&hempty[b]);
+                if (go) commit<1>(&wempty[s2]);
+                if (++j2 == p.blocks) {
+                    if (go) commit<1>(&yfull[t2 & 1]);
+                    j2 = 0, ++t2;
+                }
+                if (++s2 == p.stages) s2 = 0;
+            }
+        }
+        if (!ok) {
+            if (go) commit<1>(drain);
+            mbar_wait(drain, 0, 100000000ull);
+        }
+    } else {
+        const int ew = warp - kControlWarps, quad = warp & 3, half = ew >> 2 & 1, group = ew >> 3;
+        uint8_t* st = out_stage + ew * kStageOut;
+        T* cv = reinterpret_cast<T*>(out_stage + kEpiWarps * kStageOut + ew * column_bytes<false>());
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const Epilogue& e = p.e;
+        auto arrive = [&](uint64_t* bar) {
+            __syncwarp();
+            if (lane == 0) arrive_leader<1>(bar);
+        };
+        // y of tile t: accumulators, output bias, residual.
+        auto finish = [&](int t) {
+            const int m0 = (int)(blockIdx.x + t * gridDim.x) * kBM + quad * 32, rows = p.m - m0;
+            if (!(ok = mbar_wait(&yfull[t & 1], t >> 1 & 1))) return;
+            tc_fence_after();
+            const int last = half * 32 < p.c ? half * 32 + (p.c - 1 - half * 32) / 64 * 64 : -1;
+            for (int c0 = half * 32; c0 < p.c; c0 += 64) {
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+                if (e.bias) cv[lane] = column_value((const T*)e.bias, c0 + lane, p.c);
+                if (e.res && e.vec_res) {
+                    const int col8 = c0 + (lane & 3) * 8;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = i * 8 + (lane >> 2);
+                        *reinterpret_cast<uint4*>(stage_at(st, r, lane & 3)) =
+                            r < rows && col8 < p.c ? *reinterpret_cast<const uint4*>((const T*)e.res + (int64_t)(m0 + r) * e.ldr + col8) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+                } else if (e.res) {
+#pragma unroll 8
+                    for (int r = 0; r < 32; ++r)
+                        *reinterpret_cast<T*>(stage_at(st, r, lane >> 3) + (lane & 7) * 2) =
+                            r < rows && c0 + lane < p.c ? ((const T*)e.res)[(int64_t)(m0 + r) * e.ldr + c0 + lane] : Elem<T>::store(0.f);
+                }
+                __syncwarp();
+                uint4 o[2][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v[16];
+                    tmem_ld16(tmem + kY + (t & 1) * 128 + lanes + c0 + h * 16, v);
+                    tmem_wait_ld();
+                    reg_fence(v);
+                    if (e.bias) add_columns(v, cv + h * 16);
+                    if (e.res) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(stage_at(st, lane, 2 * h + c));
+                            const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 x = unpack2<T>(w[k]);
+                                v[8 * c + 2 * k] += x.x, v[8 * c + 2 * k + 1] += x.y;
+                            }
+                        }
+                    }
+                    pack16<T>(o[h], v);
+                }
+                if (c0 == last) {
+                    tc_fence_before();
+                    arrive(&yempty[t & 1]);
+                }
+                __syncwarp();
+                stage16(st, lane, 0, o[0]);
+                stage16(st, lane, 1, o[1]);
+                if (e.tma) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && rows > 0) tma_store(&p.out, st, c0, m0, 0);
+                } else {
+                    put_rows<T>(st, lane, (T*)e.out + (int64_t)m0 * e.ldo + c0, e.ldo, rows, p.c - c0, e.pairs);
+                }
+            }
+            if (last < 0) {
+                tc_fence_before();
+                arrive(&yempty[t & 1]);
+            }
+        };
+        int owed = -1;  // a tile whose y this group still has to write
+        for (int g = group; ok && g < total; g += 2) {
+            const int t = g / p.blocks, j = g - t * p.blocks, n0 = j * kHB + half * 32;
+            const T bg = column_value((const T*)p.b_in, n0 + lane, p.f);
+            const T bu = column_value(p.b_in ? (const T*)p.b_in + p.f : nullptr, n0 + lane, p.f);
+            if (!(ok = mbar_wait(&gfull[group], g >> 1 & 1))) break;
+            tc_fence_after();
+            if (p.b_in) {
+                cv[lane] = bg, cv[32 + lane] = bu;
+                __syncwarp();
+            }
+            uint4 o[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float gt[16], u[16];
+                const uint32_t acc = tmem + group * 128 + lanes + half * 32 + h * 16;
+                tmem_ld16(acc, gt);
+                tmem_ld16(acc + kHB, u);
+                tmem_wait_ld();
+                reg_fence(gt);
+                reg_fence(u);
+                if (h == 1) {
+                    tc_fence_before();
+                    arrive(&gempty[group]);
+                }
+                if (p.b_in) add_columns(gt, cv + h * 16), add_columns(u, cv + 32 + h * 16);
+                with_act(e.act, [&](auto act) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) u[k] *= act_value<decltype(act)::value>(gt[k]);
+                });
+                pack16<T>(o[h], u);
+            }
+            if (!(ok = mbar_wait(&hempty[group], (g >> 1 & 1) ^ 1))) break;
+            const int row = quad * 32 + lane;
+            uint8_t* hr = hs + group * kHBytes + row * kRowBytes;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) *reinterpret_cast<uint4*>(hr + (((half * 4 + h * 2 + c) ^ (row & 7)) << 4)) = o[h][c];
+            fence_async_smem();
+            arrive(&hfull[group]);
+            if (owed >= 0) {
+                finish(owed);
+                owed = -1;
+            }
+            if (j == p.blocks - 1) owed = t;
+        }
+        if (ok && owed >= 0) finish(owed);
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    if (!ok && lane == 0) atomicExch(&g_gemm_status, (int)LF_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_free<1>(tmem);
 }
 
 // Joins the splits of K and applies the epilogue, for up to three products
@@ -1747,11 +2024,52 @@ int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* 
                               : launch_ctas<__nv_bfloat16, kGated, false>(args, s.ctas, st);
 }
 
+template <typename T>
+int launch_narrow(NarrowArgs& g, cudaStream_t st) {
+    const int w_bytes = g.kc * 3 * kHB * kRowBytes, rest = 2 * g.kc * kBM * kRowBytes + 2 * kBM * kRowBytes +
+                                                           kEpiWarps * (kStageOut + column_bytes<false>()) + kBarrierBytes;
+    g.stages = std::min(6, (kSmemLimit - rest) / w_bytes);
+    static std::once_flag once[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(narrow_ffn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
+    launch_early(narrow_ffn_kernel<T>, (unsigned)std::min(g.tiles, num_sms()), kGemmThreads, (size_t)g.stages * w_bytes + rest, 1, st, g);
+    return check_launch("narrow_ffn_kernel");
+}
+
+// Whether the forward runs as one kernel: few channels, and enough tiles of 128
+// tokens for the SMs, since a CTA takes a tile's hidden columns one after another.
+bool narrow(const lf_gated_ffn_t* a) {
+    return a->f > 0 && a->c <= kNarrow && (a->m + kBM - 1) / kBM >= num_sms();
+}
+
+int run_narrow(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat& wout, const Epilogue& e, cudaStream_t st) {
+    NarrowArgs g{};
+    g.e = e;
+    g.e.act = a->activation;
+    g.e.tma = tma_ok(e.out, e.ldo, 2);
+    g.e.pairs = a->c % 2 == 0 && e.ldo % 2 == 0 && aligned(e.out, 4);
+    g.e.vec_res = a->c % 8 == 0 && tma_ok(e.res, e.ldr, 2);
+    g.b_in = a->b_in;
+    g.m = (int)a->m, g.c = (int)a->c, g.f = (int)a->f;
+    g.tiles = (int)((a->m + kBM - 1) / kBM);
+    g.blocks = (int)((a->f + kHB - 1) / kHB);
+    g.kc = (int)((a->c + 63) / 64);
+    if ((int64_t)g.tiles * g.blocks > INT32_MAX / 2) return too_large("gated feed-forward block");
+    g.idesc1 = idesc_of(a->dtype, false, false, 1, 2 * kHB);
+    g.idesc2 = idesc_of(a->dtype, false, false, 1, g.kc * 64);
+    if (!encode(&g.x, x, a->dtype, 64, kBM) || !encode(&g.win, gate_up(win, a->f), a->dtype, 64, kHB) ||
+        !encode(&g.wout, wout, a->dtype, 64, g.kc * 64))
+        return LF_ERR_CUDA;
+    if (g.e.tma && !encode_out(&g.out, {e.out, a->c, a->m, e.ldo, 1, 0}, a->dtype)) return LF_ERR_CUDA;
+    return a->dtype == LF_F16 ? launch_narrow<__half>(g, st) : launch_narrow<__nv_bfloat16>(g, st);
+}
+
 int ffn_fwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
     const int64_t m = a->m, c = a->c, f = a->f;
     if (m == 0 || c == 0) return LF_OK;
     const int64_t ldh = up(f, 8);
-    Mat h{ws.take((size_t)m * ldh * 2), f, m, ldh, 1, 0};
+    Mat h{narrow(a) ? nullptr : ws.take((size_t)m * ldh * 2), f, m, ldh, 1, 0};
     Epilogue e{};
     set_out(e, a->y, c);
     e.bias = a->b_out;
@@ -1766,6 +2084,7 @@ int ffn_fwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
     }
     Mat x = operand(a->x, m, c, a->ldx, 2, ws, st), win = operand(a->w_in, 2 * f, c, c, 2, ws, st);
     Mat wout = operand(a->w_out, c, f, f, 2, ws, st);
+    if (narrow(a)) return ws.base ? run_narrow(a, x, win, wout, e, st) : LF_OK;
     if (ws.base && f > 0)
         if (int rc = run_gated(a, x, win, nullptr, nullptr, const_cast<void*>(h.p), ldh, 0, st)) return rc;
     Product q = weight_product(h, wout, m, c, f, a->dtype, a->dtype);

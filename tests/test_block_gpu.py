@@ -349,7 +349,8 @@ def test_linear_offsets_beyond_31_bits():
 # ------------------------------------------------------------------ gated feed-forward block
 
 FFN_SHAPES = [(1, 8, 8), (1, 64, 171), (3, 33, 65), (8, 512, 1365), (9, 64, 256), (130, 40, 72), (128, 64, 128), (197, 96, 200),
-              (300, 130, 257), (1000, 64, 256), (257, 512, 1365), (20, 1031, 50)]
+              (300, 130, 257), (1000, 64, 256), (257, 512, 1365), (20, 1031, 50),
+              (18945, 64, 200), (19000, 128, 136), (38001, 40, 65), (19500, 100, 64), (56900, 24, 17)]
 
 
 @pytest.mark.parametrize("dtype", DT16)
