@@ -883,7 +883,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------------------
-// The feed-forward block's forward for at most 128 channels, in one kernel
+// The feed-forward block's forward for at most 64 channels, in one kernel
 // ---------------------------------------------------------------------------
 // With so few channels the products are short and h is most of the traffic (at
 // 64 channels and 256 hidden columns 102 of 140 MB per 100,000 tokens), so h
@@ -892,17 +892,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
 //   [g|u] = x [Wg|Wu]^T      (two accumulator buffers)
 //   h = act(g) u             to shared memory as the next product's A operand
 //   y += h Wout^T            (accumulators of two tiles in turn)
-// One warp issues both products, the next block's first one ahead of this
-// block's second; two groups of eight warps take the blocks in turn, and a
-// tile's y goes to the group of its last block, after that group's next block.
+// Each product has a warp that issues it, so that the first ones run ahead of
+// the second ones; two groups of eight epilogue warps take the blocks in turn,
+// and a tile's y goes to the group of its last block, after that group's next
+// block.  Up to five blocks of weights (320 hidden columns) are copied once and
+// stay; more go through a ring.
 constexpr int kHB = 64;                   // hidden columns of a block
-constexpr int kNarrow = 128;              // channels
+constexpr int kNarrow = 64;               // channels
 
 struct alignas(64) NarrowArgs {
     CUtensorMap x, win, wout, out;
     Epilogue e;                // out, output bias, residual, activation of the gate
     const void* b_in;
-    int m, c, f, tiles, blocks, kc, stages;  // kc: 64-channel blocks
+    int m, c, f, tiles, blocks, stages;
     uint32_t idesc1, idesc2;
 };
 
@@ -910,7 +912,7 @@ template <typename T>
 __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __grid_constant__ NarrowArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];  // x (two tiles), h (two blocks), weight stages, staging, barriers
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int x_bytes = p.kc * kBM * kRowBytes, w_bytes = p.kc * 3 * kHB * kRowBytes;
+    constexpr int x_bytes = kBM * kRowBytes, w_bytes = 3 * kHB * kRowBytes;
     constexpr int kHBytes = kBM * kRowBytes;
     uint8_t* const hs = smem + 2 * x_bytes;
     uint8_t* const ring = hs + 2 * kHBytes;
@@ -918,7 +920,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
     uint64_t* const bars = reinterpret_cast<uint64_t*>(out_stage + kEpiWarps * (kStageOut + column_bytes<false>()));
     uint64_t *wfull = bars, *wempty = bars + 6, *xfull = bars + 12, *xempty = bars + 14, *gfull = bars + 16, *gempty = bars + 18,
              *hfull = bars + 20, *hempty = bars + 22, *yfull = bars + 24, *yempty = bars + 26, *drain = bars + 28;
-    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 29);
+    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 30);
     constexpr int kY = 256;                                    // tensor memory columns of y
     grid_release();
     if (threadIdx.x == 0) {
@@ -927,7 +929,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
             mbar_init(&xfull[i], 1), mbar_init(&xempty[i], 1), mbar_init(&gfull[i], 1), mbar_init(&gempty[i], 8);
             mbar_init(&hfull[i], 8), mbar_init(&hempty[i], 1), mbar_init(&yfull[i], 1), mbar_init(&yempty[i], 8);
         }
-        mbar_init(drain, 1);
+        mbar_init(&drain[0], 1), mbar_init(&drain[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_take<1>(tmem_ptr);
@@ -938,90 +940,90 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
     const uint32_t tmem = *tmem_ptr;
     const int mine = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // this CTA's tiles
     const int total = mine * p.blocks;                                                  // and their blocks
+    const bool resident = p.blocks <= p.stages;                                         // all weights stay in shared memory
+    const int ring_len = resident ? p.blocks : p.stages;
     bool ok = true;
 
-    if (warp == 0) {  // x tiles
+    if (warp == 2) {  // copies: x tiles; per block 64 gate and 64 up rows of Win and Wout's columns
         if (elect_one()) {
-            for (int t = 0; ok && t < mine; ++t) {
-                const int b = t & 1;
-                if (!(ok = mbar_wait(&xempty[b], (t >> 1 & 1) ^ 1))) break;
-                mbar_expect(&xfull[b], x_bytes);
-                for (int k = 0; k < p.kc; ++k)
-                    tma_load<1>(smem + b * x_bytes + k * kBM * kRowBytes, &p.x, smem_u32(&xfull[b]), k * 64,
-                                (int)(blockIdx.x + t * gridDim.x) * kBM, 0);
-            }
-            if (!ok)  // a wait ran out: let the copies in flight land
-                for (int t = max(0, mine - 2); t < mine; ++t) mbar_wait(&xfull[t & 1], t >> 1 & 1, 100000000ull);
-        }
-        __syncwarp();
-    } else if (warp == 2) {  // weights: per block 64 gate and 64 up rows of Win by 64 channels, then Wout's columns
-        if (elect_one()) {
-            int s = 0, j = 0, issued = 0;
+            int s = 0, j = 0, t = 0, issued = 0;
             uint32_t ph = 0;
             for (int g = 0; g < total; ++g) {
-                if (!(ok = mbar_wait(&wempty[s], ph ^ 1))) break;
-                uint8_t* dst = ring + s * w_bytes;
-                const uint32_t bar = smem_u32(&wfull[s]);
-                mbar_expect(&wfull[s], w_bytes);
-                for (int k = 0; k < p.kc; ++k)
-                    for (int half = 0; half < 2; ++half)
-                        tma_load<1>(dst + (2 * k + half) * kHB * kRowBytes, &p.win, bar, k * 64, j * kHB, half);
-                tma_load<1>(dst + 2 * p.kc * kHB * kRowBytes, &p.wout, bar, j * kHB, 0, 0);
-                ++issued;
+                if (j == 0) {
+                    const int b = t & 1;
+                    if (!(ok = mbar_wait(&xempty[b], (t >> 1 & 1) ^ 1))) break;
+                    mbar_expect(&xfull[b], x_bytes);
+                    tma_load<1>(smem + b * x_bytes, &p.x, smem_u32(&xfull[b]), 0, (int)(blockIdx.x + t * gridDim.x) * kBM, 0);
+                    ++t;
+                }
+                if (!resident || g < p.blocks) {
+                    if (!(ok = mbar_wait(&wempty[s], ph ^ 1))) break;
+                    uint8_t* dst = ring + s * w_bytes;
+                    const uint32_t bar = smem_u32(&wfull[s]);
+                    mbar_expect(&wfull[s], w_bytes);
+                    tma_load<1>(dst, &p.win, bar, 0, j * kHB, 0);  // both planes: gate, then up rows
+                    tma_load<1>(dst + 2 * kHB * kRowBytes, &p.wout, bar, j * kHB, 0, 0);
+                    ++issued;
+                    if (++s == p.stages) s = 0, ph ^= 1;
+                }
                 if (++j == p.blocks) j = 0;
-                if (++s == p.stages) s = 0, ph ^= 1;
             }
-            if (!ok)
+            if (!ok) {  // a wait ran out: let the copies in flight land
+                for (int k = max(0, t - 2); k < t; ++k) mbar_wait(&xfull[k & 1], k >> 1 & 1, 100000000ull);
                 for (int k = max(0, issued - p.stages); k < issued; ++k)
                     mbar_wait(&wfull[k % p.stages], (k / p.stages) & 1, 100000000ull);
+            }
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == 1) {  // [g|u] = x [Wg|Wu]^T
         const uint32_t go = elect_one() ? 1u : 0u;
-        int s1 = 0, s2 = 0, j1 = 0, j2 = 0, t1 = 0, t2 = 0;    // stage, block and tile of the first and of the second product
-        uint32_t ph1 = 0;
-        for (int g = 0; ok && g <= total; ++g) {
-            if (g < total) {
-                const int b = g & 1;
-                if (j1 == 0) ok = mbar_wait(&xfull[t1 & 1], t1 >> 1 & 1);
-                ok = ok && mbar_wait(&wfull[s1], ph1) && mbar_wait(&gempty[b], (g >> 1 & 1) ^ 1);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t sx = smem_u32(smem + (t1 & 1) * x_bytes), sw = smem_u32(ring + s1 * w_bytes);
-                for (int k = 0; k < p.kc; ++k) {
-                    const uint64_t da = make_desc(sx + k * kBM * kRowBytes, 16, 1024), db = make_desc(sw + 2 * k * kHB * kRowBytes, 16, 1024);
+        int s = 0, j = 0, t = 0;
+        uint32_t ph = 0;
+        for (int g = 0; g < total; ++g) {
+            const int b = g & 1;
+            if (j == 0) ok = mbar_wait(&xfull[t & 1], t >> 1 & 1);
+            ok = ok && mbar_wait(&wfull[s], resident ? 0 : ph) && mbar_wait(&gempty[b], (g >> 1 & 1) ^ 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t da = make_desc(smem_u32(smem + (t & 1) * x_bytes), 16, 1024), db = make_desc(smem_u32(ring + s * w_bytes), 16, 1024);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mma<1, false>(tmem + b * 128, da + i * 2, db + i * 2, p.idesc1, k > 0 || i > 0 ? 1u : 0u, go);
-                }
-                if (go) commit<1>(&gfull[b]);
-                if (++j1 == p.blocks) {
-                    if (go) commit<1>(&xempty[t1 & 1]);
-                    j1 = 0, ++t1;
-                }
-                if (++s1 == p.stages) s1 = 0, ph1 ^= 1;
+            for (int i = 0; i < 4; ++i) mma<1, false>(tmem + b * 128, da + i * 2, db + i * 2, p.idesc1, i > 0 ? 1u : 0u, go);
+            if (go) commit<1>(&gfull[b]);
+            if (++j == p.blocks) {
+                if (go) commit<1>(&xempty[t & 1]);
+                j = 0, ++t;
             }
-            if (g > 0) {
-                const int b = (g - 1) & 1;
-                if (j2 == 0) ok = mbar_wait(&yempty[t2 & 1], (t2 >> 1 & 1) ^ 1);
-                ok = ok && mbar_wait(&hfull[b], (g - 1) >> 1 & 1);
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t da = make_desc(smem_u32(hs + b * kHBytes), 16, 1024);
-                const uint64_t db = make_desc(smem_u32(ring + s2 * w_bytes) + 2 * p.kc * kHB * kRowBytes, 16, 1024);
+            if (++s == ring_len) s = 0, ph ^= 1;
+        }
+        if (!ok) {  // products in flight end before the tensor memory is freed
+            if (go) commit<1>(&drain[0]);
+            mbar_wait(&drain[0], 0, 100000000ull);
+        }
+    } else if (warp == 0) {  // y += h Wout^T
+        const uint32_t go = elect_one() ? 1u : 0u;
+        int s = 0, j = 0, t = 0;
+        uint32_t ph = 0;
+        for (int g = 0; g < total; ++g) {
+            const int b = g & 1;
+            if (j == 0) ok = mbar_wait(&yempty[t & 1], (t >> 1 & 1) ^ 1);
+            ok = ok && mbar_wait(&wfull[s], resident ? 0 : ph) && mbar_wait(&hfull[b], g >> 1 & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t da = make_desc(smem_u32(hs + b * kHBytes), 16, 1024);
+            const uint64_t db = make_desc(smem_u32(ring + s * w_bytes) + 2 * kHB * kRowBytes, 16, 1024);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kY + (t2 & 1) * 128, da + i * 2, db + i * 2, p.idesc2, j2 > 0 || i > 0 ? 1u : 0u, go);
-                if (go) commit<1>(&hempty[b]);
-                if (go) commit<1>(&wempty[s2]);
-                if (++j2 == p.blocks) {
-                    if (go) commit<1>(&yfull[t2 & 1]);
-                    j2 = 0, ++t2;
-                }
-                if (++s2 == p.stages) s2 = 0;
+            for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kY + (t & 1) * 128, da + i * 2, db + i * 2, p.idesc2, j > 0 || i > 0 ? 1u : 0u, go);
+            if (go) commit<1>(&hempty[b]);
+            if (go && !resident) commit<1>(&wempty[s]);  // h was made of the first product, so that one has read its weights too
+            if (++j == p.blocks) {
+                if (go) commit<1>(&yfull[t & 1]);
+                j = 0, ++t;
             }
+            if (++s == ring_len) s = 0, ph ^= 1;
         }
         if (!ok) {
-            if (go) commit<1>(drain);
-            mbar_wait(drain, 0, 100000000ull);
+            if (go) commit<1>(&drain[1]);
+            mbar_wait(&drain[1], 0, 100000000ull);
         }
     } else {
         const int ew = warp - kControlWarps, quad = warp & 3, half = ew >> 2 & 1, group = ew >> 3;
@@ -1033,24 +1035,31 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
             __syncwarp();
             if (lane == 0) arrive_leader<1>(bar);
         };
+        // A warp writes 32 rows and 32 columns of a tile's y.
+        const int c0 = half * 32;
+        auto first_row = [&](int t) { return (int)(blockIdx.x + t * gridDim.x) * kBM + quad * 32; };
+        uint4 r[4];  // its residual, where that comes in 16-byte chunks
+        auto fetch = [&](int t) {
+            if (!e.res || !e.vec_res) return;
+            const int m0 = first_row(t), col8 = c0 + (lane & 3) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = m0 + i * 8 + (lane >> 2);
+                r[i] = row < p.m && col8 < p.c ? *reinterpret_cast<const uint4*>((const T*)e.res + (int64_t)row * e.ldr + col8) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
         // y of tile t: accumulators, output bias, residual.
         auto finish = [&](int t) {
-            const int m0 = (int)(blockIdx.x + t * gridDim.x) * kBM + quad * 32, rows = p.m - m0;
+            const int m0 = first_row(t), rows = p.m - m0;
             if (!(ok = mbar_wait(&yfull[t & 1], t >> 1 & 1))) return;
             tc_fence_after();
-            const int last = half * 32 < p.c ? half * 32 + (p.c - 1 - half * 32) / 64 * 64 : -1;
-            for (int c0 = half * 32; c0 < p.c; c0 += 64) {
+            if (c0 < p.c) {
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
                 if (e.bias) cv[lane] = column_value((const T*)e.bias, c0 + lane, p.c);
                 if (e.res && e.vec_res) {
-                    const int col8 = c0 + (lane & 3) * 8;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = i * 8 + (lane >> 2);
-                        *reinterpret_cast<uint4*>(stage_at(st, r, lane & 3)) =
-                            r < rows && col8 < p.c ? *reinterpret_cast<const uint4*>((const T*)e.res + (int64_t)(m0 + r) * e.ldr + col8) : make_uint4(0u, 0u, 0u, 0u);
-                    }
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
                 } else if (e.res) {
 #pragma unroll 8
                     for (int r = 0; r < 32; ++r)
@@ -1080,11 +1089,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
                     }
                     pack16<T>(o[h], v);
                 }
-                if (c0 == last) {
-                    tc_fence_before();
-                    arrive(&yempty[t & 1]);
-                }
-                __syncwarp();
+                tc_fence_before();
+                arrive(&yempty[t & 1]);
                 stage16(st, lane, 0, o[0]);
                 stage16(st, lane, 1, o[1]);
                 if (e.tma) {
@@ -1094,15 +1100,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
                 } else {
                     put_rows<T>(st, lane, (T*)e.out + (int64_t)m0 * e.ldo + c0, e.ldo, rows, p.c - c0, e.pairs);
                 }
-            }
-            if (last < 0) {
-                tc_fence_before();
-                arrive(&yempty[t & 1]);
-            }
+            } else arrive(&yempty[t & 1]);
         };
         int owed = -1;  // a tile whose y this group still has to write
+        int t = group / p.blocks, j = group - t * p.blocks;     // this block's tile and place in it
         for (int g = group; ok && g < total; g += 2) {
-            const int t = g / p.blocks, j = g - t * p.blocks, n0 = j * kHB + half * 32;
+            const int n0 = j * kHB + half * 32;
             const T bg = column_value((const T*)p.b_in, n0 + lane, p.f);
             const T bu = column_value(p.b_in ? (const T*)p.b_in + p.f : nullptr, n0 + lane, p.f);
             if (!(ok = mbar_wait(&gfull[group], g >> 1 & 1))) break;
@@ -1145,7 +1148,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
                 finish(owed);
                 owed = -1;
             }
-            if (j == p.blocks - 1) owed = t;
+            if (j == p.blocks - 1) fetch(owed = t);
+            for (j += 2; j >= p.blocks; j -= p.blocks) ++t;
         }
         if (ok && owed >= 0) finish(owed);
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -1422,13 +1426,13 @@ struct Mat {
 };
 
 bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_rows,
-            CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+            CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B, int box_planes = 1) {
     const int es = dtype == LF_F8E4M3 ? 1 : 2;
     const CUtensorMapDataType ty = dtype == LF_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                    : dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const cuuint64_t dims[3] = {(cuuint64_t)a.inner, (cuuint64_t)a.rows, (cuuint64_t)a.planes};
     const cuuint64_t strides[2] = {(cuuint64_t)(a.ld * es), (cuuint64_t)((a.planes > 1 ? a.plane : a.rows * a.ld) * es)};
-    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_planes}, step[3] = {1, 1, 1};
     EncodeFn fn = encode_fn();
     if (!fn) {
         set_error("cuTensorMapEncodeTiled is not available");
@@ -2026,8 +2030,7 @@ int run_gated(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat* 
 
 template <typename T>
 int launch_narrow(NarrowArgs& g, cudaStream_t st) {
-    const int w_bytes = g.kc * 3 * kHB * kRowBytes, rest = 2 * g.kc * kBM * kRowBytes + 2 * kBM * kRowBytes +
-                                                           kEpiWarps * (kStageOut + column_bytes<false>()) + kBarrierBytes;
+    constexpr int w_bytes = 3 * kHB * kRowBytes, rest = 4 * kBM * kRowBytes + kEpiWarps * (kStageOut + column_bytes<false>()) + kBarrierBytes;
     g.stages = std::min(6, (kSmemLimit - rest) / w_bytes);
     static std::once_flag once[64];
     int dev = 0;
@@ -2037,10 +2040,14 @@ int launch_narrow(NarrowArgs& g, cudaStream_t st) {
     return check_launch("narrow_ffn_kernel");
 }
 
-// Whether the forward runs as one kernel: few channels, and enough tiles of 128
-// tokens for the SMs, since a CTA takes a tile's hidden columns one after another.
+// Whether the forward runs as one kernel: few channels, and either few hidden
+// columns or enough tiles of 128 tokens, since a CTA takes a tile's hidden
+// columns one after another (64 channels, bf16, us, one kernel and two:
+// 100352 tokens, 256 hidden 31 and 41; 500 tokens 8.0 and 9.3; 100352 tokens,
+// 1024 hidden 85 and 126; 9472 tokens 18 and 19; 2000 tokens 18 and 13).
 bool narrow(const lf_gated_ffn_t* a) {
-    return a->f > 0 && a->c <= kNarrow && (a->m + kBM - 1) / kBM >= num_sms();
+    return a->f > 0 && a->c <= kNarrow && !few_rows(a->m, 3 * a->f, a->c) &&
+           (a->f <= 5 * kHB || 2 * ((a->m + kBM - 1) / kBM) >= num_sms());
 }
 
 int run_narrow(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat& wout, const Epilogue& e, cudaStream_t st) {
@@ -2054,12 +2061,11 @@ int run_narrow(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat&
     g.m = (int)a->m, g.c = (int)a->c, g.f = (int)a->f;
     g.tiles = (int)((a->m + kBM - 1) / kBM);
     g.blocks = (int)((a->f + kHB - 1) / kHB);
-    g.kc = (int)((a->c + 63) / 64);
     if ((int64_t)g.tiles * g.blocks > INT32_MAX / 2) return too_large("gated feed-forward block");
     g.idesc1 = idesc_of(a->dtype, false, false, 1, 2 * kHB);
-    g.idesc2 = idesc_of(a->dtype, false, false, 1, g.kc * 64);
-    if (!encode(&g.x, x, a->dtype, 64, kBM) || !encode(&g.win, gate_up(win, a->f), a->dtype, 64, kHB) ||
-        !encode(&g.wout, wout, a->dtype, 64, g.kc * 64))
+    g.idesc2 = idesc_of(a->dtype, false, false, 1, kNarrow);
+    if (!encode(&g.x, x, a->dtype, 64, kBM) || !encode(&g.win, gate_up(win, a->f), a->dtype, 64, kHB, CU_TENSOR_MAP_SWIZZLE_128B, 2) ||
+        !encode(&g.wout, wout, a->dtype, 64, kNarrow))
         return LF_ERR_CUDA;
     if (g.e.tma && !encode_out(&g.out, {e.out, a->c, a->m, e.ldo, 1, 0}, a->dtype)) return LF_ERR_CUDA;
     return a->dtype == LF_F16 ? launch_narrow<__half>(g, st) : launch_narrow<__nv_bfloat16>(g, st);
