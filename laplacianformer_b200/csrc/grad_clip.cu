@@ -2,13 +2,12 @@
 //   n = sqrt(sum over all tensors of g^2),  c = min(1, max_norm / (n + 1e-6)),  out = c g
 //
 // Two kernels over equal chunks of the tensors (their table travels in the
-// launch parameters, so nothing is copied to the device beforehand; up to 96
-// tensors in 2.8 KB, up to 512 in 15 KB, which costs the host 4 us more per
-// launch).  The
-// first writes one fp64 partial sum of squares per chunk; in the second every
-// block adds the partials in the same order, so each has the same
-// coefficient without another launch, and scales its chunks, last chunk
-// first: what the first kernel read last is still in L2.  No atomics: the
+// launch parameters, so nothing is copied to the device beforehand; it is sized
+// by the tensors, 29 bytes each: 15 KB for 512 cost the host 4 us more per launch
+// than 2.8 KB for 96).  The first writes one fp64 partial sum of squares per
+// chunk; in the second every block adds the partials in the same order, so each
+// has the same coefficient without another launch, and scales its chunks, last
+// chunk first: what the first kernel read last is still in L2.  No atomics: the
 // norm does not depend on timing.  A chunk's squares are added in fp32 by 256
 // threads (at most 256 each), the rest in fp64.
 //
@@ -19,7 +18,7 @@
 namespace lfb {
 namespace {
 
-constexpr int kFewTensors = 96, kMaxTensors = 512;  // per launch
+constexpr int kFewTensors = 96, kSomeTensors = 256, kMaxTensors = 512;  // per launch
 constexpr int kThreads = 256;
 
 template <int N>
@@ -267,6 +266,6 @@ extern "C" int lf_clip_grad_norm(const void* const* grads, void* const* outs, co
         set_error("lf_clip_grad_norm: too many elements");
         return LF_ERR_UNSUPPORTED;
     }
-    return count <= kFewTensors ? run_clip<kFewTensors>(grads, outs, sizes, dtypes, count, chunk, (int)total, (float)max_norm, norm, (double*)workspace, st)
-                                : run_clip<kMaxTensors>(grads, outs, sizes, dtypes, count, chunk, (int)total, (float)max_norm, norm, (double*)workspace, st);
+    auto run = count <= kFewTensors ? run_clip<kFewTensors> : count <= kSomeTensors ? run_clip<kSomeTensors> : run_clip<kMaxTensors>;
+    return run(grads, outs, sizes, dtypes, count, chunk, (int)total, (float)max_norm, norm, (double*)workspace, st);
 }

@@ -8,7 +8,8 @@
 //               dh = dy Wout,  dg = dh u act'(g),  du = dh act(g)
 //               dx = [dg|du] Win,  dWin = [dg|du]^T x,  dWout = dy^T h
 //
-// One persistent kernel (tc_gemm_kernel) runs every product: operands come
+// One persistent kernel (tc_gemm_kernel) runs every product (narrow_ffn_kernel
+// the whole forward of a block of at most 64 channels): operands come
 // through TMA into a ring of 128-byte-swizzled stages, one warp issues the
 // tcgen05 products into accumulators in tensor memory, and sixteen warps turn
 // finished accumulators into outputs while the next tile's products run.

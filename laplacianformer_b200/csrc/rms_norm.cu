@@ -399,7 +399,9 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, T* dw, 
 // registers per thread cost more occupancy than the wider row groups' block
 // reductions (bf16 width 1024: forward (2,64) 167 us, (1,128) 209, (4,32) 277;
 // backward (1,128) 181, (2,64) 183, (4,32) 391; width 512 forward (2,32) 96,
-// (1,64) 103).  Other rows use scalar (still coalesced) accesses, four or
+// (1,64) 103).  Widths between powers of two get row groups of three warps or
+// six, so that few threads idle (width 1536, 65536 rows: forward (2,96) 128,
+// (2,128) 144; backward (1,192) 141, (1,256) 162).  Other rows use scalar (still coalesced) accesses, four or
 // eight per thread.
 #define LFB_NORM_FWD(T, V, cols, vec, CALL)             \
     if (vec) {                                          \
@@ -408,7 +410,9 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, T* dw, 
         else if (cols <= 32 * V) { CALL(T, V, 1, 32); } \
         else if (cols <= 64 * V) { CALL(T, V, 2, 32); } \
         else if (cols <= 128 * V) { CALL(T, V, 2, 64); } \
+        else if (cols <= 192 * V) { CALL(T, V, 2, 96); } \
         else if (cols <= 256 * V) { CALL(T, V, 2, 128); } \
+        else if (cols <= 384 * V) { CALL(T, V, 2, 192); } \
         else if (cols <= 512 * V) { CALL(T, V, 2, 256); } \
         else if (cols <= 1024 * V) { CALL(T, V, 2, 512); } \
         else if (cols <= 2048 * V) { CALL(T, V, 4, 512); } \
@@ -420,7 +424,9 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, T* dw, 
         else if (cols <= 16 * V) { CALL(T, V, 1, 16); } \
         else if (cols <= 32 * V) { CALL(T, V, 1, 32); } \
         else if (cols <= 64 * V) { CALL(T, V, 1, 64); } \
+        else if (cols <= 96 * V) { CALL(T, V, 1, 96); } \
         else if (cols <= 128 * V) { CALL(T, V, 1, 128); } \
+        else if (cols <= 192 * V) { CALL(T, V, 1, 192); } \
         else if (cols <= 256 * V) { CALL(T, V, 1, 256); } \
         else if (cols <= 512 * V) { CALL(T, V, 1, 512); } \
         else if (cols <= 1024 * V) { CALL(T, V, 2, 512); } \
