@@ -449,7 +449,8 @@ __device__ __forceinline__ void put_rows(uint8_t* st, int lane, T* out, int64_t 
         T* o = out + r0 * ld + c;
 #pragma unroll 4
         for (int r = r0; r < 32; r += 2, o += 2 * ld)
-            if (r < rows && c < cols) *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(stage_at(st, r, c >> 3) + (c & 7) * 2);
+            if (r < rows && c < cols)
+                *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(stage_at(st, r, c >> 3) + (c & 7) * 2);
     } else {
         T* o = out + lane;
 #pragma unroll 4
@@ -633,242 +634,242 @@ __global__ void __launch_bounds__(kGemmThreads, 1) tc_gemm_kernel(const __grid_c
             const int rows = p.m - t.m0 - quad * 32;                           // rows that exist from the warp's first on
             const int64_t row0 = (int64_t)t.seg * p.m + t.m0 + quad * 32;      // in the output
             for (int sub = 0; sub < subs; ++sub) {
-            const int n0 = t.n0 + sub * bh, cend = min(MODE == kLinear ? p.bn : bh, p.n - n0);
-            uint64_t* tf = &tfull[buf];
-            const int last = cg * 32 + (cend - cg * 32 - 1) / kEpiCols * kEpiCols;  // this warp's last 32 columns (if it has any)
-            auto release = [&](uint64_t* bar) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) arrive_leader<CTAS>(bar);
-            };
-            if (cg * 32 >= cend) {                                           // none: wait for the tile all the same
-                if (!(ok = mbar_wait(tf, bph))) break;
-                tc_fence_after();
-                release(&tempty[buf]);
-                if (MODE == kGatedBwd && sub == subs - 1) release(dempty);
-            } else
-            if constexpr (MODE == kLinear) {
-                const uint32_t acc = tmem + buf * 256 + lanes;
-                const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
-                const int first = cg * 32;
-                if (!p.part) {
-                    // Finished in the accumulator's layout (a lane owns a
-                    // row); the column values and the residual of the next
-                    // columns are fetched ahead.
-                    T bias;
-                    float sb = 1.f;
-                    uint4 r[4];
-                    auto fetch = [&](int c0) {
-                        const int col = t.n0 + c0 + lane, col8 = t.n0 + c0 + (lane & 3) * 8;
-                        bias = column_value((const T*)e.bias, col, p.n);
-                        if (FP8) sb = col < p.n ? e.sb[col] : 1.f;
-                        if (!e.res) return;
-                        if (!e.vec_res) {  // a column per lane, two rows per register
-                            const T* q = (const T*)e.res + row0 * e.ldr + col;
-                            uint32_t* w = reinterpret_cast<uint32_t*>(r);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i, q += 2 * e.ldr) {
-                                const T a = 2 * i < rows && col < p.n ? q[0] : Elem<T>::store(0.f);
-                                const T b = 2 * i + 1 < rows && col < p.n ? q[e.ldr] : Elem<T>::store(0.f);
-                                w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&a) | (uint32_t)*reinterpret_cast<const uint16_t*>(&b) << 16;
-                            }
-                            return;
-                        }
-                        const T* q = (const T*)e.res + (row0 + (lane >> 2)) * e.ldr + col8;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i, q += 8 * e.ldr)
-                            r[i] = i * 8 + (lane >> 2) < rows && col8 < p.n ? *reinterpret_cast<const uint4*>(q) : make_uint4(0u, 0u, 0u, 0u);
-                    };
-                    fetch(first);
-                    if (!(ok = mbar_wait(tf, bph))) break;
-                    tc_fence_after();
-                    for (int c0 = first; c0 < cend; c0 += kEpiCols) {
-                        reuse();
-                        if (FP8) cs[lane] = sb, cs[32 + lane] = Elem<T>::load(bias);
-                        else if (e.bias) cv[lane] = bias;
-                        if (e.res && e.vec_res) {  // to the lane that owns the row
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
-                        } else if (e.res) {
-                            const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                *reinterpret_cast<uint16_t*>(stage_at(st, 2 * i, lane >> 3) + (lane & 7) * 2) = (uint16_t)w[i];
-                                *reinterpret_cast<uint16_t*>(stage_at(st, 2 * i + 1, lane >> 3) + (lane & 7) * 2) = (uint16_t)(w[i] >> 16);
-                            }
-                        }
-                        fetch(c0 + kEpiCols);
-                        __syncwarp();
-                        uint4 o[2][2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float v[16];
-                            tmem_ld16(acc + c0 + h * 16, v);
-                            tmem_wait_ld();
-                            reg_fence(v);
-                            if (h == 1 && c0 == last) release(&tempty[buf]);
-                            if (FP8) {  // (v sw) sx + b in pairs
-                                const uint64_t sx = pk2(sa, sa);
-#pragma unroll
-                                for (int j = 0; j < 16; j += 2) {
-                                    const uint64_t w = *reinterpret_cast<const uint64_t*>(cs + h * 16 + j);
-                                    const uint64_t b = *reinterpret_cast<const uint64_t*>(cs + 32 + h * 16 + j);
-                                    upk2(fma2(mul2(pk2(v[j], v[j + 1]), w), sx, b), v[j], v[j + 1]);
-                                }
-                            } else if (e.bias) add_columns(v, cv + h * 16);
-                            if (e.act != LF_ACT_NONE)
-                                with_act(e.act, [&](auto act) {
-#pragma unroll
-                                    for (int j = 0; j < 16; ++j) {
-                                        float a, slope;
-                                        if (e.act_bwd) act_both<decltype(act)::value>(v[j], a, slope);
-                                        else slope = act_value<decltype(act)::value>(v[j]);
-                                        v[j] = slope;
-                                    }
-                                });
-                            if (e.res) {  // added to the activation, or dy times its derivative
-#pragma unroll
-                                for (int c = 0; c < 2; ++c) {
-                                    const uint4 u = *reinterpret_cast<const uint4*>(stage_at(st, lane, 2 * h + c));
-                                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) {
-                                        const float2 x = unpack2<T>(w[k]);
-                                        float &y0 = v[8 * c + 2 * k], &y1 = v[8 * c + 2 * k + 1];
-                                        y0 = e.act_bwd ? y0 * x.x : y0 + x.x;
-                                        y1 = e.act_bwd ? y1 * x.y : y1 + x.y;
-                                    }
-                                }
-                            }
-                            pack16<T>(o[h], v);
-                        }
-                        __syncwarp();
-                        stage16(st, lane, 0, o[0]);
-                        stage16(st, lane, 1, o[1]);
-                        if (e.tma) put(&p.out, t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
-                        else put_rows<T>(st, lane, (T*)e.out + row0 * e.ldo + t.n0 + c0, e.ldo, rows, cend - c0, e.pairs);
-                    }
-                } else {
-                    // Split-K partials: raw sums through shared memory, 16
-                    // columns at a time, as row segments.
-                    if (!(ok = mbar_wait(tf, bph))) break;
-                    tc_fence_after();
-                    reuse();  // the last tile may have been another problem's
-                    for (int c0 = first; c0 < cend; c0 += kEpiCols) {
-#pragma unroll 1
-                        for (int h = 0; h < 2; ++h) {
-                            const int col = t.n0 + c0 + h * 16 + (lane & 3) * 4, row = lane >> 2;
-                            float v[16];
-                            tmem_ld16(acc + c0 + h * 16, v);
-                            tmem_wait_ld();
-                            reg_fence(v);
-                            if (c0 == last && h == 1) release(&tempty[buf]);
-                            __syncwarp();
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                *reinterpret_cast<float4*>(stage_at(st, lane, c)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                            __syncwarp();
-                            float* q = p.part + ((int64_t)t.split * p.msegs * p.m + row0 + row) * p.ldp + col;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i, q += 8 * p.ldp)
-                                if (i * 8 + row < rows && col < p.ldp)
-                                    *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(stage_at(st, i * 8 + row, lane & 3));
-                        }
-                    }
-                }
-            } else {
-                const T* bias = (const T*)e.bias;
-                const uint32_t acc = tmem + buf * 256 + lanes;
-                const int c0 = cg * 32;                                        // the warp's only columns
-                const T bg = column_value(bias, n0 + c0 + lane, p.n);
-                const T bu = column_value(bias ? bias + p.n : bias, n0 + c0 + lane, p.n);
-                if (!(ok = mbar_wait(tf, bph))) break;
-                tc_fence_after();
-                if (MODE == kGated) reuse();
-                if (bias) {
-                    cv[lane] = bg, cv[32 + lane] = bu;
+                const int n0 = t.n0 + sub * bh, cend = min(MODE == kLinear ? p.bn : bh, p.n - n0);
+                uint64_t* tf = &tfull[buf];
+                const int last = cg * 32 + (cend - cg * 32 - 1) / kEpiCols * kEpiCols;  // this warp's last 32 columns (if it has any)
+                auto release = [&](uint64_t* bar) {
+                    tc_fence_before();
                     __syncwarp();
-                }
-                // 16 columns at a time; outputs wait as 16-bit pairs.
-                uint4 og[2][2], ou[2][2];
-                if constexpr (MODE == kGated) {
+                    if (lane == 0) arrive_leader<CTAS>(bar);
+                };
+                if (cg * 32 >= cend) {                                           // none: wait for the tile all the same
+                    if (!(ok = mbar_wait(tf, bph))) break;
+                    tc_fence_after();
+                    release(&tempty[buf]);
+                    if (MODE == kGatedBwd && sub == subs - 1) release(dempty);
+                } else
+                if constexpr (MODE == kLinear) {
+                    const uint32_t acc = tmem + buf * 256 + lanes;
+                    const float sa = FP8 && lane < rows && !p.part ? e.sa[row0 + lane] : 1.f;
+                    const int first = cg * 32;
+                    if (!p.part) {
+                        // Finished in the accumulator's layout (a lane owns a
+                        // row); the column values and the residual of the next
+                        // columns are fetched ahead.
+                        T bias;
+                        float sb = 1.f;
+                        uint4 r[4];
+                        auto fetch = [&](int c0) {
+                            const int col = t.n0 + c0 + lane, col8 = t.n0 + c0 + (lane & 3) * 8;
+                            bias = column_value((const T*)e.bias, col, p.n);
+                            if (FP8) sb = col < p.n ? e.sb[col] : 1.f;
+                            if (!e.res) return;
+                            if (!e.vec_res) {  // a column per lane, two rows per register
+                                const T* q = (const T*)e.res + row0 * e.ldr + col;
+                                uint32_t* w = reinterpret_cast<uint32_t*>(r);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float g[16], u[16];
-                        tmem_ld16(acc + c0 + h * 16, g);
-                        tmem_ld16(acc + bh + c0 + h * 16, u);
-                        tmem_wait_ld();
-                        reg_fence(g);
-                        reg_fence(u);
-                        if (h == 1) release(&tempty[buf]);
-                        if (bias) add_columns(g, cv + h * 16), add_columns(u, cv + 32 + h * 16);
-                        with_act(e.act, [&](auto act) {
+                                for (int i = 0; i < 16; ++i, q += 2 * e.ldr) {
+                                    const T a = 2 * i < rows && col < p.n ? q[0] : Elem<T>::store(0.f);
+                                    const T b = 2 * i + 1 < rows && col < p.n ? q[e.ldr] : Elem<T>::store(0.f);
+                                    w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&a) | (uint32_t)*reinterpret_cast<const uint16_t*>(&b) << 16;
+                                }
+                                return;
+                            }
+                            const T* q = (const T*)e.res + (row0 + (lane >> 2)) * e.ldr + col8;
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
-                        });
-                        pack16<T>(ou[h], u);
+                            for (int i = 0; i < 4; ++i, q += 8 * e.ldr)
+                                r[i] = i * 8 + (lane >> 2) < rows && col8 < p.n ? *reinterpret_cast<const uint4*>(q) : make_uint4(0u, 0u, 0u, 0u);
+                        };
+                        fetch(first);
+                        if (!(ok = mbar_wait(tf, bph))) break;
+                        tc_fence_after();
+                        for (int c0 = first; c0 < cend; c0 += kEpiCols) {
+                            reuse();
+                            if (FP8) cs[lane] = sb, cs[32 + lane] = Elem<T>::load(bias);
+                            else if (e.bias) cv[lane] = bias;
+                            if (e.res && e.vec_res) {  // to the lane that owns the row
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage_at(st, i * 8 + (lane >> 2), lane & 3)) = r[i];
+                            } else if (e.res) {
+                                const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    *reinterpret_cast<uint16_t*>(stage_at(st, 2 * i, lane >> 3) + (lane & 7) * 2) = (uint16_t)w[i];
+                                    *reinterpret_cast<uint16_t*>(stage_at(st, 2 * i + 1, lane >> 3) + (lane & 7) * 2) = (uint16_t)(w[i] >> 16);
+                                }
+                            }
+                            fetch(c0 + kEpiCols);
+                            __syncwarp();
+                            uint4 o[2][2];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                float v[16];
+                                tmem_ld16(acc + c0 + h * 16, v);
+                                tmem_wait_ld();
+                                reg_fence(v);
+                                if (h == 1 && c0 == last) release(&tempty[buf]);
+                                if (FP8) {  // (v sw) sx + b in pairs
+                                    const uint64_t sx = pk2(sa, sa);
+#pragma unroll
+                                    for (int j = 0; j < 16; j += 2) {
+                                        const uint64_t w = *reinterpret_cast<const uint64_t*>(cs + h * 16 + j);
+                                        const uint64_t b = *reinterpret_cast<const uint64_t*>(cs + 32 + h * 16 + j);
+                                        upk2(fma2(mul2(pk2(v[j], v[j + 1]), w), sx, b), v[j], v[j + 1]);
+                                    }
+                                } else if (e.bias) add_columns(v, cv + h * 16);
+                                if (e.act != LF_ACT_NONE)
+                                    with_act(e.act, [&](auto act) {
+#pragma unroll
+                                        for (int j = 0; j < 16; ++j) {
+                                            float a, slope;
+                                            if (e.act_bwd) act_both<decltype(act)::value>(v[j], a, slope);
+                                            else slope = act_value<decltype(act)::value>(v[j]);
+                                            v[j] = slope;
+                                        }
+                                    });
+                                if (e.res) {  // added to the activation, or dy times its derivative
+#pragma unroll
+                                    for (int c = 0; c < 2; ++c) {
+                                        const uint4 u = *reinterpret_cast<const uint4*>(stage_at(st, lane, 2 * h + c));
+                                        const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+                                        for (int k = 0; k < 4; ++k) {
+                                            const float2 x = unpack2<T>(w[k]);
+                                            float &y0 = v[8 * c + 2 * k], &y1 = v[8 * c + 2 * k + 1];
+                                            y0 = e.act_bwd ? y0 * x.x : y0 + x.x;
+                                            y1 = e.act_bwd ? y1 * x.y : y1 + x.y;
+                                        }
+                                    }
+                                }
+                                pack16<T>(o[h], v);
+                            }
+                            __syncwarp();
+                            stage16(st, lane, 0, o[0]);
+                            stage16(st, lane, 1, o[1]);
+                            if (e.tma) put(&p.out, t.n0 + c0, t.m0 + quad * 32, t.seg, rows > 0);
+                            else put_rows<T>(st, lane, (T*)e.out + row0 * e.ldo + t.n0 + c0, e.ldo, rows, cend - c0, e.pairs);
+                        }
+                    } else {
+                        // Split-K partials: raw sums through shared memory, 16
+                        // columns at a time, as row segments.
+                        if (!(ok = mbar_wait(tf, bph))) break;
+                        tc_fence_after();
+                        reuse();  // the last tile may have been another problem's
+                        for (int c0 = first; c0 < cend; c0 += kEpiCols) {
+#pragma unroll 1
+                            for (int h = 0; h < 2; ++h) {
+                                const int col = t.n0 + c0 + h * 16 + (lane & 3) * 4, row = lane >> 2;
+                                float v[16];
+                                tmem_ld16(acc + c0 + h * 16, v);
+                                tmem_wait_ld();
+                                reg_fence(v);
+                                if (c0 == last && h == 1) release(&tempty[buf]);
+                                __syncwarp();
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    *reinterpret_cast<float4*>(stage_at(st, lane, c)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                                __syncwarp();
+                                float* q = p.part + ((int64_t)t.split * p.msegs * p.m + row0 + row) * p.ldp + col;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i, q += 8 * p.ldp)
+                                    if (i * 8 + row < rows && col < p.ldp)
+                                        *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(stage_at(st, i * 8 + row, lane & 3));
+                            }
+                        }
                     }
                 } else {
-                    float g[2][16], u[2][16];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        tmem_ld16(acc + c0 + h * 16, g[h]);
-                        tmem_ld16(acc + bh + c0 + h * 16, u[h]);
+                    const T* bias = (const T*)e.bias;
+                    const uint32_t acc = tmem + buf * 256 + lanes;
+                    const int c0 = cg * 32;                                        // the warp's only columns
+                    const T bg = column_value(bias, n0 + c0 + lane, p.n);
+                    const T bu = column_value(bias ? bias + p.n : bias, n0 + c0 + lane, p.n);
+                    if (!(ok = mbar_wait(tf, bph))) break;
+                    tc_fence_after();
+                    if (MODE == kGated) reuse();
+                    if (bias) {
+                        cv[lane] = bg, cv[32 + lane] = bu;
+                        __syncwarp();
                     }
-                    tmem_wait_ld();
+                    // 16 columns at a time; outputs wait as 16-bit pairs.
+                    uint4 og[2][2], ou[2][2];
+                    if constexpr (MODE == kGated) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        reg_fence(g[h]);
-                        reg_fence(u[h]);
-                    }
-                    release(tempty);
-                    reuse();
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (bias) add_columns(g[h], cv + h * 16), add_columns(u[h], cv + 32 + h * 16);
-                        uint4 oh[2];
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {  // eight columns of dh at a time: registers are full
-                            float d[8];
-                            tmem_ld8(tmem + kDh + sub * bh + lanes + c0 + h * 16 + c * 8, d);
+                        for (int h = 0; h < 2; ++h) {
+                            float g[16], u[16];
+                            tmem_ld16(acc + c0 + h * 16, g);
+                            tmem_ld16(acc + bh + c0 + h * 16, u);
                             tmem_wait_ld();
-                            reg_fence(d);
-                            if (h == 1 && c == 1 && sub == subs - 1) release(dempty);
-                            // h = act(g) u, du = dh act(g), dg = dh u act'(g), in d, g and u
+                            reg_fence(g);
+                            reg_fence(u);
+                            if (h == 1) release(&tempty[buf]);
+                            if (bias) add_columns(g, cv + h * 16), add_columns(u, cv + 32 + h * 16);
                             with_act(e.act, [&](auto act) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    float a, slope;
-                                    float &gj = g[h][c * 8 + j], &uj = u[h][c * 8 + j];
-                                    act_both<decltype(act)::value>(gj, a, slope);
-                                    const float dh = d[j];
-                                    d[j] = a * uj;
-                                    gj = a * dh;
-                                    uj *= slope * dh;
-                                }
+                                for (int j = 0; j < 16; ++j) u[j] *= act_value<decltype(act)::value>(g[j]);
                             });
-                            oh[c] = pack8<T>(d);
-                            og[h][c] = pack8<T>(&g[h][c * 8]);
-                            ou[h][c] = pack8<T>(&u[h][c * 8]);
+                            pack16<T>(ou[h], u);
                         }
-                        stage16(st, lane, h, oh);
+                    } else {
+                        float g[2][16], u[2][16];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            tmem_ld16(acc + c0 + h * 16, g[h]);
+                            tmem_ld16(acc + bh + c0 + h * 16, u[h]);
+                        }
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            reg_fence(g[h]);
+                            reg_fence(u[h]);
+                        }
+                        release(tempty);
+                        reuse();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (bias) add_columns(g[h], cv + h * 16), add_columns(u[h], cv + 32 + h * 16);
+                            uint4 oh[2];
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {  // eight columns of dh at a time: registers are full
+                                float d[8];
+                                tmem_ld8(tmem + kDh + sub * bh + lanes + c0 + h * 16 + c * 8, d);
+                                tmem_wait_ld();
+                                reg_fence(d);
+                                if (h == 1 && c == 1 && sub == subs - 1) release(dempty);
+                                // h = act(g) u, du = dh act(g), dg = dh u act'(g), in d, g and u
+                                with_act(e.act, [&](auto act) {
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) {
+                                        float a, slope;
+                                        float &gj = g[h][c * 8 + j], &uj = u[h][c * 8 + j];
+                                        act_both<decltype(act)::value>(gj, a, slope);
+                                        const float dh = d[j];
+                                        d[j] = a * uj;
+                                        gj = a * dh;
+                                        uj *= slope * dh;
+                                    }
+                                });
+                                oh[c] = pack8<T>(d);
+                                og[h][c] = pack8<T>(&g[h][c * 8]);
+                                ou[h][c] = pack8<T>(&u[h][c * 8]);
+                            }
+                            stage16(st, lane, h, oh);
+                        }
                     }
+                    const int row = t.m0 + quad * 32;
+                    if constexpr (MODE == kGatedBwd) {  // planes dg, du, h
+                        put(&p.out, n0 + c0, row, 2, rows > 0);
+                        reuse();
+                        stage16(st, lane, 0, og[0]);
+                        stage16(st, lane, 1, og[1]);
+                        put(&p.out, n0 + c0, row, 1, rows > 0);
+                        reuse();
+                    }
+                    stage16(st, lane, 0, ou[0]);
+                    stage16(st, lane, 1, ou[1]);
+                    put(&p.out, n0 + c0, row, 0, rows > 0);
                 }
-                const int row = t.m0 + quad * 32;
-                if constexpr (MODE == kGatedBwd) {  // planes dg, du, h
-                    put(&p.out, n0 + c0, row, 2, rows > 0);
-                    reuse();
-                    stage16(st, lane, 0, og[0]);
-                    stage16(st, lane, 1, og[1]);
-                    put(&p.out, n0 + c0, row, 1, rows > 0);
-                    reuse();
-                }
-                stage16(st, lane, 0, ou[0]);
-                stage16(st, lane, 1, ou[1]);
-                put(&p.out, n0 + c0, row, 0, rows > 0);
-            }
-            if (MODE != kGatedBwd) buf ^= 1;
-            if (buf == 0) bph ^= 1;
+                if (MODE != kGatedBwd) buf ^= 1;
+                if (buf == 0) bph ^= 1;
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // outputs written, staging read
@@ -986,7 +987,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
             ok = ok && mbar_wait(&wfull[s], resident ? 0 : ph) && mbar_wait(&gempty[b], (g >> 1 & 1) ^ 1);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t da = make_desc(smem_u32(smem + (t & 1) * x_bytes), 16, 1024), db = make_desc(smem_u32(ring + s * w_bytes), 16, 1024);
+            const uint64_t da = make_desc(smem_u32(smem + (t & 1) * x_bytes), 16, 1024);
+            const uint64_t db = make_desc(smem_u32(ring + s * w_bytes), 16, 1024);
 #pragma unroll
             for (int i = 0; i < 4; ++i) mma<1, false>(tmem + b * 128, da + i * 2, db + i * 2, p.idesc1, i > 0 ? 1u : 0u, go);
             if (go) commit<1>(&gfull[b]);
@@ -1013,7 +1015,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
             const uint64_t da = make_desc(smem_u32(hs + b * kHBytes), 16, 1024);
             const uint64_t db = make_desc(smem_u32(ring + s * w_bytes) + 2 * kHB * kRowBytes, 16, 1024);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kY + (t & 1) * 128, da + i * 2, db + i * 2, p.idesc2, j > 0 || i > 0 ? 1u : 0u, go);
+            for (int i = 0; i < 4; ++i)
+                mma<1, false>(tmem + kY + (t & 1) * 128, da + i * 2, db + i * 2, p.idesc2, j > 0 || i > 0 ? 1u : 0u, go);
             if (go) commit<1>(&hempty[b]);
             if (go && !resident) commit<1>(&wempty[s]);  // h was made of the first product, so that one has read its weights too
             if (++j == p.blocks) {
@@ -1046,7 +1049,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = m0 + i * 8 + (lane >> 2);
-                r[i] = row < p.m && col8 < p.c ? *reinterpret_cast<const uint4*>((const T*)e.res + (int64_t)row * e.ldr + col8) : make_uint4(0u, 0u, 0u, 0u);
+                r[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (row < p.m && col8 < p.c) r[i] = *reinterpret_cast<const uint4*>((const T*)e.res + (int64_t)row * e.ldr + col8);
             }
         };
         // y of tile t: accumulators, output bias, residual.
@@ -1557,7 +1561,8 @@ double choose_together(const Product* q, int count, int ctas, Shape* out) {
             s[i] = {ctas, bn_of[i], n};
         }
         // Short units even out what the long ones leave, where there are enough of them.
-        const double t = std::max(longest, work / lanes + 0.5 * (filler >= longest ? shortest : longest)) + (join > 0 ? 6500 + join : 0) + (ctas == 2 ? 1000 : 0);
+        const double uneven = 0.5 * (filler >= longest ? shortest : longest);
+        const double t = std::max(longest, work / lanes + uneven) + (join > 0 ? 6500 + join : 0) + (ctas == 2 ? 1000 : 0);
         if (t < least) {
             least = t;
             for (int i = 0; i < count; ++i) out[i] = s[i];
@@ -1665,11 +1670,12 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
     if (int rc = fill_problem(g.p[0], q, s, part)) return rc;
     g.first[1] = (int)units_of(g.p[0]);
     g.stage_bytes = stage_bytes_of(s);
+    const bool half = q.dtype == LF_F16;
     int rc;
     if (q.op_dtype == LF_F8E4M3)
-        rc = q.dtype == LF_F16 ? launch_ctas<__half, kLinear, true>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, true>(g, s.ctas, st);
+        rc = half ? launch_ctas<__half, kLinear, true>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, true>(g, s.ctas, st);
     else
-        rc = q.dtype == LF_F16 ? launch_ctas<__half, kLinear, false>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, false>(g, s.ctas, st);
+        rc = half ? launch_ctas<__half, kLinear, false>(g, s.ctas, st) : launch_ctas<__nv_bfloat16, kLinear, false>(g, s.ctas, st);
     if (rc || !part) return rc;
     join.job[0] = join_of(q, part, g.p[0].splits);
     return join_splits(join, 1, q.dtype, st);
