@@ -1166,6 +1166,340 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
     if (warp == 1) tmem_free<1>(tmem);
 }
 
+// ---------------------------------------------------------------------------
+// The feed-forward block's backward for at most 64 channels and 256 hidden
+// columns, in one kernel
+// ---------------------------------------------------------------------------
+// Here too the hidden tensors (h, dg, du: 154 MB written and 256 read again for
+// 100,000 tokens of 64 channels and 256 hidden columns, where x, dy and dx have
+// 38) stay in the SM.  A CTA owns 128 hidden columns, whose weights stay in
+// shared memory, and every slots-th tile of 128 tokens; it takes them in two
+// blocks of 64 columns:
+//   [g|u] = x [Wg|Wu]^T,  dh = dy Wout
+//   dg = dh u act'(g),  du = dh act(g),  h = act(g) u     to shared memory
+//   dx += dg Wg + du Wu
+// and once a tile
+//   dWg += dg^T x,  dWu += du^T x,  dWout^T += h^T dy,  db += [dg|du]^T 1
+// whose sums stay in tensor memory until the last tile; the partial sums of the
+// slots are joined by another launch.  The tiles in shared memory serve as K-major
+// operands for dx and as transposed ones for the weights.  More than 128 hidden
+// columns take a cluster of two CTAs, one for each half, on the same tokens: each
+// sends the other half of the rows of its dx through distributed shared memory
+// and writes the sum for its own.
+constexpr int kBwdHidden = 128;           // hidden columns of a CTA
+
+struct alignas(64) NarrowBwdArgs {
+    CUtensorMap x, dy, win, wout;
+    const void* b_in;
+    void* dx;
+    float *part_in, *part_out, *part_b;   // [slots][2f][ld_in], [slots][c][ld_out], [slots][ld_b]; null: not asked for
+    int ld_in, ld_out, ld_b;
+    int m, c, f, tiles, blocks, act;
+    bool vec_dx;
+    uint32_t id_gu, id_n, id_w, id_b;
+};
+
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {  // the same shared memory in another CTA of the cluster
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void peer_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool peer_wait(uint64_t* bar, uint32_t parity) {
+    const bool done = mbar_wait(bar, parity);
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    return done;
+}
+
+template <typename T, int CTAS>
+__global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_bwd_kernel(const __grid_constant__ NarrowBwdArgs p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    constexpr int tile_bytes = kBM * kRowBytes, w_bytes = 3 * kHB * kRowBytes;
+    uint8_t* const weights = smem + 4 * tile_bytes;            // after two of x | dy
+    uint8_t* const dg_s = weights + 2 * w_bytes;               // dg, du, h: two blocks each
+    uint8_t *const du_s = dg_s + 2 * tile_bytes, *const h_s = du_s + 2 * tile_bytes;
+    uint8_t* const inbox = h_s + 2 * tile_bytes;               // dx rows from the other CTA
+    uint8_t* const ones = inbox + 16384;                       // B operand of the bias gradients
+    T* const bias = reinterpret_cast<T*>(ones + 2048);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(bias + 2 * kBwdHidden);
+    uint64_t *wfull = bars, *xfull = bars + 1, *xempty = bars + 3, *gfull = bars + 5, *gempty = bars + 6, *hfull = bars + 7,
+             *hempty = bars + 9, *dxfull = bars + 10, *dxempty = bars + 11, *infull = bars + 12, *inempty = bars + 13,
+             *done = bars + 14, *drain = bars + 15;
+    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 17);
+    constexpr int kDh = 128, kDx = 192, kDw = 256, kDb = 448;  // tensor memory columns; g and u from 0 on
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, slot = (int)blockIdx.x / CTAS, slots = (int)gridDim.x / CTAS;
+    grid_release();
+    if (threadIdx.x == 0) {
+        mbar_init(wfull, 1), mbar_init(gfull, 1), mbar_init(gempty, kEpiWarps), mbar_init(hempty, 1);
+        mbar_init(dxfull, 1), mbar_init(dxempty, kEpiWarps), mbar_init(infull, 8), mbar_init(inempty, 8), mbar_init(done, 1);
+        for (int i = 0; i < 2; ++i)
+            mbar_init(&xfull[i], 1), mbar_init(&xempty[i], 1), mbar_init(&hfull[i], kEpiWarps), mbar_init(&drain[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    for (int i = threadIdx.x; i < 512; i += kGemmThreads) {
+        const uint32_t one = pack2<T>(1.f, 1.f);
+        reinterpret_cast<uint32_t*>(ones)[i] = one;
+    }
+    fence_async_smem();
+    grid_wait();
+    if (threadIdx.x < 2 * kBwdHidden) {
+        const int up = threadIdx.x >= kBwdHidden, col = rank * kBwdHidden + (threadIdx.x & (kBwdHidden - 1));
+        bias[threadIdx.x] = column_value(p.b_in ? (const T*)p.b_in + (up ? p.f : 0) : nullptr, col, p.f);
+    }
+    if (warp == 1) tmem_take<1>(tmem_ptr);
+    tc_fence_before();
+    __syncthreads();
+    sync_all<CTAS>();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    const int mine = (p.tiles - slot + slots - 1) / slots;
+    const int n_first = rank * kBwdHidden;
+    bool ok = true;
+
+    if (warp == 2) {  // copies: the weights once, then x and dy of a tile
+        if (elect_one()) {
+            mbar_expect(wfull, p.blocks * w_bytes);
+            for (int j = 0; j < p.blocks; ++j) {
+                uint8_t* dst = weights + j * w_bytes;
+                tma_load<1>(dst, &p.win, smem_u32(wfull), 0, n_first + j * kHB, 0);  // both planes: gate, then up rows
+                tma_load<1>(dst + 2 * kHB * kRowBytes, &p.wout, smem_u32(wfull), n_first + j * kHB, 0, 0);
+            }
+            int t = 0;
+            for (; t < mine; ++t) {
+                const int b = t & 1;
+                if (!(ok = mbar_wait(&xempty[b], (t >> 1 & 1) ^ 1))) break;
+                mbar_expect(&xfull[b], 2 * tile_bytes);
+                uint8_t* dst = smem + b * 2 * tile_bytes;
+                tma_load<1>(dst, &p.x, smem_u32(&xfull[b]), 0, (slot + t * slots) * kBM, 0);
+                tma_load<1>(dst + tile_bytes, &p.dy, smem_u32(&xfull[b]), 0, (slot + t * slots) * kBM, 0);
+            }
+            if (!ok) {  // a wait ran out: let the copies in flight land
+                mbar_wait(wfull, 0, 100000000ull);
+                for (int k = max(0, t - 2); k < t; ++k) mbar_wait(&xfull[k & 1], k >> 1 & 1, 100000000ull);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {  // [g|u] = x [Wg|Wu]^T, dh = dy Wout
+        const uint32_t go = elect_one() ? 1u : 0u;
+        ok = mbar_wait(wfull, 0);
+        for (int t = 0, g = 0; ok && t < mine; ++t) {
+            if (!(ok = mbar_wait(&xfull[t & 1], t >> 1 & 1))) break;
+            const uint64_t dx = make_desc(smem_u32(smem + (t & 1) * 2 * tile_bytes), 16, 1024);
+            const uint64_t ddy = make_desc(smem_u32(smem + (t & 1) * 2 * tile_bytes) + tile_bytes, 16, 1024);
+            for (int j = 0; j < p.blocks; ++j, ++g) {
+                if (!(ok = mbar_wait(gempty, (g & 1) ^ 1))) break;
+                tc_fence_after();
+                const uint32_t w = smem_u32(weights + j * w_bytes);
+                const uint64_t dw = make_desc(w, 16, 1024), dwo = make_desc(w + 2 * kHB * kRowBytes, 8192, 1024);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma<1, false>(tmem, dx + i * 2, dw + i * 2, p.id_gu, i > 0 ? 1u : 0u, go);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kDh, ddy + i * 2, dwo + i * 128, p.id_n, i > 0 ? 1u : 0u, go);
+                if (go) commit<1>(gfull);
+            }
+        }
+        if (!ok) {  // products in flight end before the tensor memory is freed
+            if (go) commit<1>(&drain[0]);
+            mbar_wait(&drain[0], 0, 100000000ull);
+        }
+    } else if (warp == 0) {  // dx of a tile and the weights' sums
+        const uint32_t go = elect_one() ? 1u : 0u;
+        ok = mbar_wait(wfull, 0);
+        for (int t = 0; ok && t < mine; ++t) {
+            ok = mbar_wait(&xfull[t & 1], t >> 1 & 1) && (!p.dx || mbar_wait(dxempty, (t & 1) ^ 1));
+            for (int j = 0; ok && j < p.blocks; ++j) {
+                if (!(ok = mbar_wait(&hfull[j], t & 1))) break;
+                tc_fence_after();
+                if (!p.dx) continue;
+                const uint64_t dwg = make_desc(smem_u32(weights + j * w_bytes), 8192, 1024);
+                const uint64_t dwu = make_desc(smem_u32(weights + j * w_bytes) + kHB * kRowBytes, 8192, 1024);
+                const uint64_t dg = make_desc(smem_u32(dg_s + j * tile_bytes), 16, 1024), du = make_desc(smem_u32(du_s + j * tile_bytes), 16, 1024);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kDx, dg + i * 2, dwg + i * 128, p.id_n, j > 0 || i > 0 ? 1u : 0u, go);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kDx, du + i * 2, dwu + i * 128, p.id_n, 1u, go);
+            }
+            if (!ok) break;
+            if (go && p.dx) commit<1>(dxfull);
+            // the tiles again, transposed: 128 hidden columns by 128 tokens
+            const uint64_t dg = make_desc(smem_u32(dg_s), tile_bytes, 1024), du = make_desc(smem_u32(du_s), tile_bytes, 1024);
+            const uint64_t h = make_desc(smem_u32(h_s), tile_bytes, 1024), one = make_desc(smem_u32(ones), 16, 1024);
+            const uint64_t x = make_desc(smem_u32(smem + (t & 1) * 2 * tile_bytes), 8192, 1024);
+            const uint64_t dy = make_desc(smem_u32(smem + (t & 1) * 2 * tile_bytes) + tile_bytes, 8192, 1024);
+#pragma unroll 1
+            for (int i = 0; i < kBM / 16; ++i) {
+                const uint32_t more = t > 0 || i > 0 ? 1u : 0u;
+                if (p.part_in) {
+                    mma<1, false>(tmem + kDw, dg + i * 128, x + i * 128, p.id_w, more, go);
+                    mma<1, false>(tmem + kDw + 64, du + i * 128, x + i * 128, p.id_w, more, go);
+                }
+                if (p.part_out) mma<1, false>(tmem + kDw + 128, h + i * 128, dy + i * 128, p.id_w, more, go);
+                if (p.part_b) {
+                    mma<1, false>(tmem + kDb, dg + i * 128, one, p.id_b, more, go);
+                    mma<1, false>(tmem + kDb + 16, du + i * 128, one, p.id_b, more, go);
+                }
+            }
+            if (go) commit<1>(hempty), commit<1>(&xempty[t & 1]);
+        }
+        if (ok && go) commit<1>(done);
+        if (!ok) {
+            if (go) commit<1>(&drain[1]);
+            mbar_wait(&drain[1], 0, 100000000ull);
+        }
+    } else {
+        const int ew = warp - kControlWarps, quad = warp & 3, c0 = (ew >> 2) * 16;  // 32 rows and 16 columns of everything
+        const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + c0;
+        const int row = quad * 32 + lane;
+        auto arrive = [&](uint64_t* bar) {
+            __syncwarp();
+            if (lane == 0) arrive_leader<1>(bar);
+        };
+        const bool owner = CTAS == 1 || quad >> 1 == rank;       // whether this CTA writes the warp's rows of dx
+        uint8_t* const box = inbox + ((quad & 1) * 4 + (ew >> 2)) * 2048 + lane * 16;
+        auto finish = [&](int t) {
+            if (!(ok = mbar_wait(dxfull, t & 1))) return;
+            tc_fence_after();
+            float v[16];
+            tmem_ld16(acc + kDx, v);
+            tmem_wait_ld();
+            reg_fence(v);
+            tc_fence_before();
+            arrive(dxempty);
+            if constexpr (CTAS == 2) {
+                if (!owner) {
+                    if (!(ok = peer_wait(inempty, (t & 1) ^ 1))) return;
+                    const uint32_t dst = peer_addr(box, rank ^ 1);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * 512), "f"(v[4 * k]), "f"(v[4 * k + 1]),
+                                     "f"(v[4 * k + 2]), "f"(v[4 * k + 3])
+                                     : "memory");
+                    __syncwarp();
+                    if (lane == 0) peer_arrive(peer_addr(infull, rank ^ 1));
+                    return;
+                }
+                if (!(ok = peer_wait(infull, t & 1))) return;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 u = *reinterpret_cast<const float4*>(box + k * 512);
+                    v[4 * k] += u.x, v[4 * k + 1] += u.y, v[4 * k + 2] += u.z, v[4 * k + 3] += u.w;
+                }
+                __syncwarp();
+                if (lane == 0) peer_arrive(peer_addr(inempty, rank ^ 1));
+            }
+            const int r = (slot + t * slots) * kBM + row;
+            uint4 u[2];
+            pack16<T>(u, v);
+            if (r < p.m) {
+                T* o = (T*)p.dx + (int64_t)r * p.c + c0;
+                if (p.vec_dx) {
+                    if (c0 < p.c) reinterpret_cast<uint4*>(o)[0] = u[0];
+                    if (c0 + 8 < p.c) reinterpret_cast<uint4*>(o)[1] = u[1];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (c0 + k < p.c) o[k] = Elem<T>::store(v[k]);
+                }
+            }
+            __syncwarp();
+        };
+        int owed = -1;  // a tile whose dx is still to be written
+        for (int t = 0, g = 0; ok && t < mine; ++t) {
+            for (int j = 0; j < p.blocks; ++j, ++g) {
+                if (!(ok = mbar_wait(gfull, g & 1))) break;
+                tc_fence_after();
+                float gt[16], u[16], d[16];
+                tmem_ld16(acc, gt);
+                tmem_ld16(acc + kHB, u);
+                tmem_ld16(acc + kDh, d);
+                tmem_wait_ld();
+                reg_fence(gt);
+                reg_fence(u);
+                reg_fence(d);
+                tc_fence_before();
+                arrive(gempty);
+                if (p.b_in) add_columns(gt, bias + j * kHB + c0), add_columns(u, bias + kBwdHidden + j * kHB + c0);
+                with_act(p.act, [&](auto act) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float a, slope;
+                        act_both<decltype(act)::value>(gt[k], a, slope);
+                        gt[k] = d[k] * u[k] * slope;
+                        u[k] *= a;
+                        d[k] *= a;
+                    }
+                });
+                const int left = p.f - (n_first + j * kHB + c0);
+                if (left < 16) {  // columns past the last: zeros even where x or dy is infinite
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (k >= left) gt[k] = u[k] = d[k] = 0.f;
+                }
+                uint4 o[3][2];
+                pack16<T>(o[0], gt);
+                pack16<T>(o[1], d);
+                pack16<T>(o[2], u);
+                if (!(ok = mbar_wait(hempty, (t & 1) ^ 1))) break;
+                uint8_t* const at = dg_s + j * tile_bytes + row * kRowBytes;
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        *reinterpret_cast<uint4*>(at + k * 2 * tile_bytes + (((c0 / 8 + c) ^ (row & 7)) << 4)) = o[k][c];
+                fence_async_smem();
+                arrive(&hfull[j]);
+                if (owed >= 0) {
+                    finish(owed);
+                    owed = -1;
+                }
+                if (!ok) break;
+            }
+            if (p.dx) owed = t;
+        }
+        if (ok && owed >= 0) finish(owed);
+        if (ok && (ok = mbar_wait(done, 0))) {  // the slot's partial sums
+            tc_fence_after();
+            const int n = n_first + row;
+            float v[16];
+            if (p.part_in) {
+                for (int plane = 0; plane < 2; ++plane) {
+                    tmem_ld16(acc + kDw + plane * 64, v);
+                    tmem_wait_ld();
+                    reg_fence(v);
+                    float* o = p.part_in + ((int64_t)slot * 2 * p.f + plane * p.f + n) * p.ld_in + c0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (n < p.f && c0 + 4 * k < p.ld_in)
+                            reinterpret_cast<float4*>(o)[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                }
+            }
+            if (p.part_out) {
+                tmem_ld16(acc + kDw + 128, v);
+                tmem_wait_ld();
+                reg_fence(v);
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (n < p.f && c0 + k < p.c) p.part_out[((int64_t)slot * p.c + c0 + k) * p.ld_out + n] = v[k];
+            }
+            if (p.part_b && c0 < 32) {  // 16 equal columns each for gate and up
+                tmem_ld16(acc + kDb, v);
+                tmem_wait_ld();
+                reg_fence(v);
+                if (n < p.f) p.part_b[(int64_t)slot * p.ld_b + (c0 ? p.f : 0) + n] = v[0];
+            }
+        }
+    }
+    if (!ok && lane == 0) atomicExch(&g_gemm_status, (int)LF_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    sync_all<CTAS>();  // the other CTA may still write to this one's shared memory
+    tc_fence_after();
+    if (warp == 1) tmem_free<1>(tmem);
+}
+
 // Joins the splits of K and applies the epilogue, for up to three products
 // (blockIdx.y).  `walkers` threads share four columns, each adds every
 // walkers-th split, and their sums join in order: a thread for all splits of a
@@ -2078,6 +2412,62 @@ int run_narrow(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat&
     return a->dtype == LF_F16 ? launch_narrow<__half>(g, st) : launch_narrow<__nv_bfloat16>(g, st);
 }
 
+template <typename T, int CTAS>
+int launch_narrow_bwd(const NarrowBwdArgs& g, int slots, cudaStream_t st) {
+    constexpr int bytes = 10 * kBM * kRowBytes + 6 * kHB * kRowBytes + 16384 + 2048 + 2 * kBwdHidden * (int)sizeof(T) + kBarrierBytes;
+    static_assert(bytes <= kSmemLimit, "shared memory");
+    static std::once_flag once[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(narrow_ffn_bwd_kernel<T, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
+    launch_early(narrow_ffn_bwd_kernel<T, CTAS>, (unsigned)(slots * CTAS), kGemmThreads, (size_t)bytes, CTAS, st, g);
+    return check_launch("narrow_ffn_bwd_kernel");
+}
+
+// Whether the backward runs as one kernel and a join.
+bool narrow_bwd(const lf_gated_ffn_t* a) { return a->f > 0 && a->c <= kNarrow && a->f <= 2 * kBwdHidden; }
+
+int run_narrow_bwd(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat& wout, const Mat& dy, Arena& ws, cudaStream_t st) {
+    const int64_t m = a->m, c = a->c, f = a->f;
+    if (m > INT32_MAX - 256) return too_large("gated feed-forward block");
+    NarrowBwdArgs g{};
+    const int ctas = f > kBwdHidden ? 2 : 1;
+    g.tiles = (int)((m + kBM - 1) / kBM);
+    const int slots = std::min(g.tiles, num_sms() / ctas);
+    g.ld_in = (int)up(c, 4), g.ld_out = (int)up(f, 4), g.ld_b = (int)up(2 * f, 4);
+    if (a->dw_in) g.part_in = (float*)ws.take((size_t)slots * 2 * f * g.ld_in * 4);
+    if (a->dw_out) g.part_out = (float*)ws.take((size_t)slots * c * g.ld_out * 4);
+    if (a->db_in) g.part_b = (float*)ws.take((size_t)slots * g.ld_b * 4);
+    if (!ws.base) return LF_OK;
+    g.b_in = a->b_in, g.dx = a->dx, g.act = a->activation;
+    g.m = (int)m, g.c = (int)c, g.f = (int)f;
+    g.blocks = f > kHB ? 2 : 1;
+    g.vec_dx = c % 8 == 0 && aligned(a->dx, 16);
+    g.id_gu = idesc_of(a->dtype, false, false, 1, 2 * kHB);
+    g.id_n = idesc_of(a->dtype, false, true, 1, 64);
+    g.id_w = idesc_of(a->dtype, true, true, 1, 64);
+    g.id_b = idesc_of(a->dtype, true, false, 1, 16);
+    if (!encode(&g.x, x, a->dtype, 64, kBM) || !encode(&g.dy, dy, a->dtype, 64, kBM) ||
+        !encode(&g.win, gate_up(win, f), a->dtype, 64, kHB, CU_TENSOR_MAP_SWIZZLE_128B, 2) || !encode(&g.wout, wout, a->dtype, 64, kNarrow))
+        return LF_ERR_CUDA;
+    const bool half = a->dtype == LF_F16;
+    int rc;
+    if (ctas == 2) rc = half ? launch_narrow_bwd<__half, 2>(g, slots, st) : launch_narrow_bwd<__nv_bfloat16, 2>(g, slots, st);
+    else rc = half ? launch_narrow_bwd<__half, 1>(g, slots, st) : launch_narrow_bwd<__nv_bfloat16, 1>(g, slots, st);
+    if (rc) return rc;
+    JoinJobs jobs{};
+    int count = 0;
+    auto join = [&](const float* part, int64_t rows, int64_t ld, int64_t cols, void* out) {
+        if (!part) return;
+        JoinJob& j = jobs.job[count++] = {part, rows, ld, slots, (int)cols, slots >= 32 ? 8 : slots >= 8 ? 4 : 1, {}};
+        set_out(j.e, out, cols);
+    };
+    join(g.part_in, 2 * f, g.ld_in, c, a->dw_in);
+    join(g.part_out, c, g.ld_out, f, a->dw_out);
+    join(g.part_b, 1, g.ld_b, 2 * f, a->db_in);
+    return count ? join_splits(jobs, count, a->dtype, st) : LF_OK;
+}
+
 int ffn_fwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
     const int64_t m = a->m, c = a->c, f = a->f;
     if (m == 0 || c == 0) return LF_OK;
@@ -2109,9 +2499,14 @@ int ffn_bwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
     const int64_t m = a->m, c = a->c, f = a->f;
     if (m == 0 || c == 0) return LF_OK;
     const int64_t ld = up(f, 8), plane = m * ld;
-    uint16_t* dz = (uint16_t*)ws.take((size_t)3 * plane * 2);  // dg, du, h
     Mat x = operand(a->x, m, c, a->ldx, 2, ws, st), win = operand(a->w_in, 2 * f, c, c, 2, ws, st);
     Mat wout = operand(a->w_out, c, f, f, 2, ws, st), dy = operand(a->dy, m, c, a->lddy, 2, ws, st);
+    if (narrow_bwd(a)) {
+        if (int rc = run_narrow_bwd(a, x, win, wout, dy, ws, st)) return rc;
+        const Columns sums{a->dy, a->lddy, c, a->db_out, false};
+        return run_colsum(&sums, 1, m, a->dtype, ws, st);
+    }
+    uint16_t* dz = (uint16_t*)ws.take((size_t)3 * plane * 2);  // dg, du, h
     if (ws.base && f > 0)
         if (int rc = run_gated(a, x, win, &dy, &wout, dz, ld, plane, st)) return rc;
     const Mat both{dz, f, m, ld, 2, plane}, h{dz + 2 * plane, f, m, ld, 1, 0};

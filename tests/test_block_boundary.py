@@ -64,7 +64,9 @@ def test_gated_ffn_sizes():
     wide = {"c": 128, "ldx": 128, "ldr": 128}
     assert L.lf_gated_ffn_fwd_workspace_size(ffn(**wide)) >= 100 * 96 * 2  # h of 100 x 96
     assert L.lf_gated_ffn_fwd_workspace_size(ffn()) == 0  # up to 64 channels h stays in shared memory
-    assert L.lf_gated_ffn_bwd_workspace_size(ffn(dy=P, lddy=64, dx=P)) >= 3 * 100 * 96 * 2
+    assert L.lf_gated_ffn_bwd_workspace_size(ffn(dy=P, lddy=128, dx=P, **wide)) >= 3 * 100 * 96 * 2  # dg, du and h
+    assert L.lf_gated_ffn_bwd_workspace_size(ffn(dy=P, lddy=64, dx=P)) == 0  # these too stay there
+    assert L.lf_gated_ffn_bwd_workspace_size(ffn(dy=P, lddy=64, dw_out=P)) >= 64 * 96 * 4  # its partial sums
     assert L.lf_gated_ffn_fwd(ffn(**wide), None, 0, None) == capi.LF_ERR_INVALID and b"workspace" in L.lf_last_error()
     assert L.lf_gated_ffn_bwd(ffn(dx=P), P, 1 << 30, None) == capi.LF_ERR_INVALID  # no dy
     assert L.lf_gated_ffn_fwd(ffn(m=0), None, 0, None) == capi.LF_OK
