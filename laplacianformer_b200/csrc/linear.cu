@@ -1187,6 +1187,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
 // sends the other half of the rows of its dx through distributed shared memory
 // and writes the sum for its own.
 constexpr int kBwdHidden = 128;           // hidden columns of a CTA
+constexpr int kBwdThreads = kGemmThreads + 128;  // and four warps that write dx
 
 struct alignas(64) NarrowBwdArgs {
     CUtensorMap x, dy, win, wout;
@@ -1214,7 +1215,7 @@ __device__ __forceinline__ bool peer_wait(uint64_t* bar, uint32_t parity) {
 }
 
 template <typename T, int CTAS>
-__global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_bwd_kernel(const __grid_constant__ NarrowBwdArgs p) {
+__global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __grid_constant__ NarrowBwdArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int tile_bytes = kBM * kRowBytes, w_bytes = 3 * kHB * kRowBytes;
     uint8_t* const weights = smem + 4 * tile_bytes;            // after two of x | dy
@@ -1234,12 +1235,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_bwd_kernel(const _
     grid_release();
     if (threadIdx.x == 0) {
         mbar_init(wfull, 1), mbar_init(gfull, 1), mbar_init(gempty, kEpiWarps), mbar_init(hempty, 1);
-        mbar_init(dxfull, 1), mbar_init(dxempty, kEpiWarps), mbar_init(infull, 8), mbar_init(inempty, 8), mbar_init(done, 1);
+        mbar_init(dxfull, 1), mbar_init(dxempty, 4), mbar_init(infull, 2), mbar_init(inempty, 2), mbar_init(done, 1);
         for (int i = 0; i < 2; ++i)
             mbar_init(&xfull[i], 1), mbar_init(&xempty[i], 1), mbar_init(&hfull[i], kEpiWarps), mbar_init(&drain[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    for (int i = threadIdx.x; i < 512; i += kGemmThreads) {
+    for (int i = threadIdx.x; i < 512; i += kBwdThreads) {
         const uint32_t one = pack2<T>(1.f, 1.f);
         reinterpret_cast<uint32_t*>(ones)[i] = one;
     }
@@ -1349,6 +1350,64 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_bwd_kernel(const _
             if (go) commit<1>(&drain[1]);
             mbar_wait(&drain[1], 0, 100000000ull);
         }
+    } else if (warp >= kControlWarps + kEpiWarps) {  // dx: a warp has 32 of a tile's rows
+        const int quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + kDx;
+        const bool owner = CTAS == 1 || quad >> 1 == rank;  // whether this CTA writes them
+        uint8_t* const box = inbox + (quad & 1) * 8192 + lane * 16;
+        for (int t = 0; p.dx && t < mine; ++t) {
+            ok = mbar_wait(dxfull, t & 1);
+            if (CTAS == 2) ok = ok && (owner ? peer_wait(infull, t & 1) : peer_wait(inempty, (t & 1) ^ 1));
+            if (!ok) break;
+            tc_fence_after();
+            const int r = (slot + t * slots) * kBM + row;
+#pragma unroll
+            for (int c0 = 0; c0 < 64; c0 += 16) {
+                float v[16];
+                tmem_ld16(acc + c0, v);
+                tmem_wait_ld();
+                reg_fence(v);
+                if (c0 == 48) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_leader<1>(dxempty);
+                }
+                if (CTAS == 2 && !owner) {
+                    const uint32_t dst = peer_addr(box + c0 * 128, rank ^ 1);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * 512), "f"(v[4 * k]), "f"(v[4 * k + 1]),
+                                     "f"(v[4 * k + 2]), "f"(v[4 * k + 3])
+                                     : "memory");
+                    continue;
+                }
+                if (CTAS == 2) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float4 u = *reinterpret_cast<const float4*>(box + c0 * 128 + k * 512);
+                        v[4 * k] += u.x, v[4 * k + 1] += u.y, v[4 * k + 2] += u.z, v[4 * k + 3] += u.w;
+                    }
+                }
+                if (r < p.m) {
+                    uint4 u[2];
+                    pack16<T>(u, v);
+                    T* o = (T*)p.dx + (int64_t)r * p.c + c0;
+                    if (p.vec_dx) {
+                        if (c0 < p.c) reinterpret_cast<uint4*>(o)[0] = u[0];
+                        if (c0 + 8 < p.c) reinterpret_cast<uint4*>(o)[1] = u[1];
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (c0 + k < p.c) o[k] = Elem<T>::store(v[k]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (CTAS == 2) {
+                __syncwarp();
+                if (lane == 0) peer_arrive(peer_addr(owner ? inempty : infull, rank ^ 1));
+            }
+        }
     } else {
         const int ew = warp - kControlWarps, quad = warp & 3, c0 = (ew >> 2) * 16;  // 32 rows and 16 columns of everything
         const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + c0;
@@ -1357,56 +1416,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_bwd_kernel(const _
             __syncwarp();
             if (lane == 0) arrive_leader<1>(bar);
         };
-        const bool owner = CTAS == 1 || quad >> 1 == rank;       // whether this CTA writes the warp's rows of dx
-        uint8_t* const box = inbox + ((quad & 1) * 4 + (ew >> 2)) * 2048 + lane * 16;
-        auto finish = [&](int t) {
-            if (!(ok = mbar_wait(dxfull, t & 1))) return;
-            tc_fence_after();
-            float v[16];
-            tmem_ld16(acc + kDx, v);
-            tmem_wait_ld();
-            reg_fence(v);
-            tc_fence_before();
-            arrive(dxempty);
-            if constexpr (CTAS == 2) {
-                if (!owner) {
-                    if (!(ok = peer_wait(inempty, (t & 1) ^ 1))) return;
-                    const uint32_t dst = peer_addr(box, rank ^ 1);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * 512), "f"(v[4 * k]), "f"(v[4 * k + 1]),
-                                     "f"(v[4 * k + 2]), "f"(v[4 * k + 3])
-                                     : "memory");
-                    __syncwarp();
-                    if (lane == 0) peer_arrive(peer_addr(infull, rank ^ 1));
-                    return;
-                }
-                if (!(ok = peer_wait(infull, t & 1))) return;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float4 u = *reinterpret_cast<const float4*>(box + k * 512);
-                    v[4 * k] += u.x, v[4 * k + 1] += u.y, v[4 * k + 2] += u.z, v[4 * k + 3] += u.w;
-                }
-                __syncwarp();
-                if (lane == 0) peer_arrive(peer_addr(inempty, rank ^ 1));
-            }
-            const int r = (slot + t * slots) * kBM + row;
-            uint4 u[2];
-            pack16<T>(u, v);
-            if (r < p.m) {
-                T* o = (T*)p.dx + (int64_t)r * p.c + c0;
-                if (p.vec_dx) {
-                    if (c0 < p.c) reinterpret_cast<uint4*>(o)[0] = u[0];
-                    if (c0 + 8 < p.c) reinterpret_cast<uint4*>(o)[1] = u[1];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        if (c0 + k < p.c) o[k] = Elem<T>::store(v[k]);
-                }
-            }
-            __syncwarp();
-        };
-        int owed = -1;  // a tile whose dx is still to be written
         for (int t = 0, g = 0; ok && t < mine; ++t) {
             for (int j = 0; j < p.blocks; ++j, ++g) {
                 if (!(ok = mbar_wait(gfull, g & 1))) break;
@@ -1451,15 +1460,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_bwd_kernel(const _
                         *reinterpret_cast<uint4*>(at + k * 2 * tile_bytes + (((c0 / 8 + c) ^ (row & 7)) << 4)) = o[k][c];
                 fence_async_smem();
                 arrive(&hfull[j]);
-                if (owed >= 0) {
-                    finish(owed);
-                    owed = -1;
-                }
-                if (!ok) break;
             }
-            if (p.dx) owed = t;
         }
-        if (ok && owed >= 0) finish(owed);
         if (ok && (ok = mbar_wait(done, 0))) {  // the slot's partial sums
             tc_fence_after();
             const int n = n_first + row;
@@ -2420,7 +2422,7 @@ int launch_narrow_bwd(const NarrowBwdArgs& g, int slots, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(narrow_ffn_bwd_kernel<T, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
-    launch_early(narrow_ffn_bwd_kernel<T, CTAS>, (unsigned)(slots * CTAS), kGemmThreads, (size_t)bytes, CTAS, st, g);
+    launch_early(narrow_ffn_bwd_kernel<T, CTAS>, (unsigned)(slots * CTAS), kBwdThreads, (size_t)bytes, CTAS, st, g);
     return check_launch("narrow_ffn_bwd_kernel");
 }
 
