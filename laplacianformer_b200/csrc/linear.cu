@@ -1138,6 +1138,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
 #pragma unroll
                     for (int k = 0; k < 16; ++k) u[k] *= act_value<decltype(act)::value>(gt[k]);
                 });
+                const int left = p.f - (n0 + h * 16);
+                if (left < 16) {  // columns past the last: zeros even where x is infinite
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (k >= left) u[k] = 0.f;
+                }
                 pack16<T>(o[h], u);
             }
             if (!(ok = mbar_wait(&hempty[group], (g >> 1 & 1) ^ 1))) break;
@@ -1185,7 +1191,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
 // operands for dx and as transposed ones for the weights.  More than 128 hidden
 // columns take a cluster of two CTAs, one for each half, on the same tokens: each
 // sends the other half of the rows of its dx through distributed shared memory
-// and writes the sum for its own.
+// and writes the sum for its own; four warps do that, so that the epilogue warps
+// need not wait for the other CTA (100352 x 64 x 256: 52 against 73 us).
+//
+// At that size the kernel reads x and dy once from memory (26 MB) and is bound
+// by the latency of a block's round from products to shared memory (3400
+// cycles, of which the matrix pipe is busy for a third and the issue slots for
+// another): with g, u and dh beside the sums, the tensor memory has no room for a second
+// block's.  Blocks of 32 columns in two groups of warps measured 56 us.
 constexpr int kBwdHidden = 128;           // hidden columns of a CTA
 constexpr int kBwdThreads = kGemmThreads + 128;  // and four warps that write dx
 
@@ -2426,7 +2439,12 @@ int launch_narrow_bwd(const NarrowBwdArgs& g, int slots, cudaStream_t st) {
     return check_launch("narrow_ffn_bwd_kernel");
 }
 
-// Whether the backward runs as one kernel and a join.
+// Whether the backward runs as one kernel and a join: wherever the weights and
+// the sums of their gradients fit two SMs, since then it is as fast at the
+// smallest sizes and faster above (GPU time in us with bf16, 64 channels,
+// against the gated backward, three products and a join: 128 tokens, 64 hidden
+// 14.5 and 14.5; 500, 256: 25 and 29; 9472, 256: 22 and 31; 100352, 64: 33 and
+// 63; 100352, 256: 64 and 126; 401408, 176: 201 and 377).
 bool narrow_bwd(const lf_gated_ffn_t* a) { return a->f > 0 && a->c <= kNarrow && a->f <= 2 * kBwdHidden; }
 
 int run_narrow_bwd(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const Mat& wout, const Mat& dy, Arena& ws, cudaStream_t st) {

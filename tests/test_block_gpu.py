@@ -496,6 +496,24 @@ def test_nan_and_infinity_stay_in_their_rows():
         assert torch.equal(got[keep], ref[keep]) and got[17].isnan().all() and not got[250].isfinite().all()
 
 
+@pytest.mark.parametrize("shape", [(3, 8, 40), (200, 8, 40), (200, 64, 200), (200, 100, 40)])
+def test_infinite_row_of_the_feed_forward_block(shape):
+    # all positive: an infinite row is infinite and not NaN, whatever a tile holds past the last hidden column
+    m, c, f = shape
+    g = gen("infinite row", shape)
+    x, dy = rand(g, torch.bfloat16, m, c).abs(), rand(g, torch.bfloat16, m, c).abs()
+    wi, wo = rand(g, torch.bfloat16, 2 * f, c).abs() + 0.1, rand(g, torch.bfloat16, c, f).abs() + 0.1
+    run = lambda x: ops.gated_feed_forward(x, wi, wo, activation="relu")  # noqa: E731
+    keep = torch.arange(m, device="cuda") != 1
+    bad = torch.where(keep[:, None], x, float("inf"))
+    clean, got = run(x), run(bad)
+    assert clean.isfinite().all() and torch.equal(got[keep], clean[keep]) and (got[1] == float("inf")).all()
+    leaves = [t.requires_grad_() for t in (x, wi, wo)]
+    wi_run = lambda d: torch.autograd.grad(ops.gated_feed_forward(*leaves, activation="relu"), leaves, d)  # noqa: E731
+    ref, grads = wi_run(dy), wi_run(torch.where(keep[:, None], dy, float("inf")))
+    assert torch.equal(grads[0][keep], ref[0][keep]) and all((t == float("inf")).all() for t in (grads[0][1], *grads[1:]))
+
+
 def test_other_stream_and_determinism():
     g = gen("stream")
     x, wi, wo = rand(g, torch.float16, 3000, 96), rand(g, torch.float16, 512, 96, scale=0.1), rand(g, torch.float16, 96, 256, scale=0.1)
