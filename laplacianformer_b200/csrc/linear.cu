@@ -1185,7 +1185,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
 //   dg = dh u act'(g),  du = dh act(g),  h = act(g) u     to shared memory
 //   dx += dg Wg + du Wu
 // and once a tile
-//   dWg += dg^T x,  dWu += du^T x,  dWout^T += h^T dy,  db += [dg|du]^T 1
+//   dWg += dg^T x,  dWu += du^T x,  dWout^T += h^T dy,
+//   db_in += [dg|du]^T 1,  db_out += dy^T 1
 // whose sums stay in tensor memory until the last tile; the partial sums of the
 // slots are joined by another launch.  The tiles in shared memory serve as K-major
 // operands for dx and as transposed ones for the weights.  More than 128 hidden
@@ -1206,8 +1207,9 @@ struct alignas(64) NarrowBwdArgs {
     CUtensorMap x, dy, win, wout;
     const void* b_in;
     void* dx;
-    float *part_in, *part_out, *part_b;   // [slots][2f][ld_in], [slots][c][ld_out], [slots][ld_b]; null: not asked for
-    int ld_in, ld_out, ld_b;
+    float *part_in, *part_out;            // [slots][2f][ld_in], [slots][c][ld_out]; null: not asked for
+    float *part_bi, *part_bo;             // [slots][ld_bi], [slots][ld_bo]: the biases'
+    int ld_in, ld_out, ld_bi, ld_bo;
     int m, c, f, tiles, blocks, act;
     bool vec_dx;
     uint32_t id_gu, id_n, id_w, id_b;
@@ -1343,6 +1345,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
             const uint64_t h = make_desc(smem_u32(h_s), tile_bytes, 1024), one = make_desc(smem_u32(ones), 16, 1024);
             const uint64_t x = make_desc(smem_u32(smem + (t & 1) * 2 * tile_bytes), 8192, 1024);
             const uint64_t dy = make_desc(smem_u32(smem + (t & 1) * 2 * tile_bytes) + tile_bytes, 8192, 1024);
+            const uint64_t x_dy = make_desc(smem_u32(smem + (t & 1) * 2 * tile_bytes), tile_bytes, 1024);  // rows 64 on are dy's
 #pragma unroll 1
             for (int i = 0; i < kBM / 16; ++i) {
                 const uint32_t more = t > 0 || i > 0 ? 1u : 0u;
@@ -1351,7 +1354,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
                     mma<1, false>(tmem + kDw + 64, du + i * 128, x + i * 128, p.id_w, more, go);
                 }
                 if (p.part_out) mma<1, false>(tmem + kDw + 128, h + i * 128, dy + i * 128, p.id_w, more, go);
-                if (p.part_b) {
+                if (p.part_bo && rank == 0) mma<1, false>(tmem + kDb + 32, x_dy + i * 128, one, p.id_b, more, go);
+                if (p.part_bi) {
                     mma<1, false>(tmem + kDb, dg + i * 128, one, p.id_b, more, go);
                     mma<1, false>(tmem + kDb + 16, du + i * 128, one, p.id_b, more, go);
                 }
@@ -1499,11 +1503,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
                 for (int k = 0; k < 16; ++k)
                     if (n < p.f && c0 + k < p.c) p.part_out[((int64_t)slot * p.c + c0 + k) * p.ld_out + n] = v[k];
             }
-            if (p.part_b && c0 < 32) {  // 16 equal columns each for gate and up
+            if (p.part_bo && rank == 0 && c0 == 0) {
+                tmem_ld16(acc + kDb + 32, v);
+                tmem_wait_ld();
+                reg_fence(v);
+                if (row >= 64 && row - 64 < p.c) p.part_bo[(int64_t)slot * p.ld_bo + row - 64] = v[0];
+                __syncwarp();
+            }
+            if (p.part_bi && c0 < 32) {  // 16 equal columns each for gate and up
                 tmem_ld16(acc + kDb, v);
                 tmem_wait_ld();
                 reg_fence(v);
-                if (n < p.f) p.part_b[(int64_t)slot * p.ld_b + (c0 ? p.f : 0) + n] = v[0];
+                if (n < p.f) p.part_bi[(int64_t)slot * p.ld_bi + (c0 ? p.f : 0) + n] = v[0];
             }
         }
     }
@@ -1515,7 +1526,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
     if (warp == 1) tmem_free<1>(tmem);
 }
 
-// Joins the splits of K and applies the epilogue, for up to three products
+// Joins the splits of K and applies the epilogue, for up to four products
 // (blockIdx.y).  `walkers` threads share four columns, each adds every
 // walkers-th split, and their sums join in order: a thread for all splits of a
 // small output would wait for one load after another.
@@ -1526,7 +1537,7 @@ struct JoinJob {
     Epilogue e;
 };
 struct JoinJobs {
-    JoinJob job[3];
+    JoinJob job[4];
 };
 template <typename T>
 __global__ void __launch_bounds__(256) split_join_kernel(const __grid_constant__ JoinJobs jobs) {
@@ -2454,10 +2465,11 @@ int run_narrow_bwd(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const 
     const int ctas = f > kBwdHidden ? 2 : 1;
     g.tiles = (int)((m + kBM - 1) / kBM);
     const int slots = std::min(g.tiles, num_sms() / ctas);
-    g.ld_in = (int)up(c, 4), g.ld_out = (int)up(f, 4), g.ld_b = (int)up(2 * f, 4);
+    g.ld_in = (int)up(c, 4), g.ld_out = (int)up(f, 4), g.ld_bi = (int)up(2 * f, 4), g.ld_bo = (int)up(c, 4);
     if (a->dw_in) g.part_in = (float*)ws.take((size_t)slots * 2 * f * g.ld_in * 4);
     if (a->dw_out) g.part_out = (float*)ws.take((size_t)slots * c * g.ld_out * 4);
-    if (a->db_in) g.part_b = (float*)ws.take((size_t)slots * g.ld_b * 4);
+    if (a->db_in) g.part_bi = (float*)ws.take((size_t)slots * g.ld_bi * 4);
+    if (a->db_out) g.part_bo = (float*)ws.take((size_t)slots * g.ld_bo * 4);
     if (!ws.base) return LF_OK;
     g.b_in = a->b_in, g.dx = a->dx, g.act = a->activation;
     g.m = (int)m, g.c = (int)c, g.f = (int)f;
@@ -2484,7 +2496,8 @@ int run_narrow_bwd(const lf_gated_ffn_t* a, const Mat& x, const Mat& win, const 
     };
     join(g.part_in, 2 * f, g.ld_in, c, a->dw_in);
     join(g.part_out, c, g.ld_out, f, a->dw_out);
-    join(g.part_b, 1, g.ld_b, 2 * f, a->db_in);
+    join(g.part_bi, 1, g.ld_bi, 2 * f, a->db_in);
+    join(g.part_bo, 1, g.ld_bo, c, a->db_out);
     return count ? join_splits(jobs, count, a->dtype, st) : LF_OK;
 }
 
@@ -2521,11 +2534,7 @@ int ffn_bwd(const lf_gated_ffn_t* a, Arena& ws, cudaStream_t st) {
     const int64_t ld = up(f, 8), plane = m * ld;
     Mat x = operand(a->x, m, c, a->ldx, 2, ws, st), win = operand(a->w_in, 2 * f, c, c, 2, ws, st);
     Mat wout = operand(a->w_out, c, f, f, 2, ws, st), dy = operand(a->dy, m, c, a->lddy, 2, ws, st);
-    if (narrow_bwd(a)) {
-        if (int rc = run_narrow_bwd(a, x, win, wout, dy, ws, st)) return rc;
-        const Columns sums{a->dy, a->lddy, c, a->db_out, false};
-        return run_colsum(&sums, 1, m, a->dtype, ws, st);
-    }
+    if (narrow_bwd(a)) return run_narrow_bwd(a, x, win, wout, dy, ws, st);
     uint16_t* dz = (uint16_t*)ws.take((size_t)3 * plane * 2);  // dg, du, h
     if (ws.base && f > 0)
         if (int rc = run_gated(a, x, win, &dy, &wout, dz, ld, plane, st)) return rc;
