@@ -9,7 +9,8 @@
 //               dx = [dg|du] Win,  dWin = [dg|du]^T x,  dWout = dy^T h
 //
 // One persistent kernel (tc_gemm_kernel) runs every product (narrow_ffn_kernel
-// the whole forward of a block of at most 64 channels): operands come
+// the whole forward of a block of at most 64 channels, narrow_ffn_bwd_kernel its
+// backward with at most 256 hidden columns): operands come
 // through TMA into a ring of 128-byte-swizzled stages, one warp issues the
 // tcgen05 products into accumulators in tensor memory, and sixteen warps turn
 // finished accumulators into outputs while the next tile's products run.
@@ -1197,9 +1198,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) narrow_ffn_kernel(const __gri
 //
 // At that size the kernel reads x and dy once from memory (26 MB) and is bound
 // by the latency of a block's round from products to shared memory (3400
-// cycles, of which the matrix pipe is busy for a third and the issue slots for
-// another): with g, u and dh beside the sums, the tensor memory has no room for a second
-// block's.  Blocks of 32 columns in two groups of warps measured 56 us.
+// cycles, of which the matrix pipe is busy for a quarter and the issue slots for
+// a third): beside the sums, the tensor memory has no room for a second block's g, u
+// and dh.  Blocks of 32 columns in two groups of warps measured 56 us.
 constexpr int kBwdHidden = 128;           // hidden columns of a CTA
 constexpr int kBwdThreads = kGemmThreads + 128;  // and four warps that write dx
 
@@ -1255,10 +1256,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
             mbar_init(&xfull[i], 1), mbar_init(&xempty[i], 1), mbar_init(&hfull[i], kEpiWarps), mbar_init(&drain[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    for (int i = threadIdx.x; i < 512; i += kBwdThreads) {
-        const uint32_t one = pack2<T>(1.f, 1.f);
-        reinterpret_cast<uint32_t*>(ones)[i] = one;
-    }
+    for (int i = threadIdx.x; i < 512; i += kBwdThreads) reinterpret_cast<uint32_t*>(ones)[i] = pack2<T>(1.f, 1.f);
     fence_async_smem();
     grid_wait();
     if (threadIdx.x < 2 * kBwdHidden) {
@@ -1332,7 +1330,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
                 if (!p.dx) continue;
                 const uint64_t dwg = make_desc(smem_u32(weights + j * w_bytes), 8192, 1024);
                 const uint64_t dwu = make_desc(smem_u32(weights + j * w_bytes) + kHB * kRowBytes, 8192, 1024);
-                const uint64_t dg = make_desc(smem_u32(dg_s + j * tile_bytes), 16, 1024), du = make_desc(smem_u32(du_s + j * tile_bytes), 16, 1024);
+                const uint64_t dg = make_desc(smem_u32(dg_s + j * tile_bytes), 16, 1024);
+                const uint64_t du = make_desc(smem_u32(du_s + j * tile_bytes), 16, 1024);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mma<1, false>(tmem + kDx, dg + i * 2, dwg + i * 128, p.id_n, j > 0 || i > 0 ? 1u : 0u, go);
 #pragma unroll
@@ -1354,7 +1353,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
                     mma<1, false>(tmem + kDw + 64, du + i * 128, x + i * 128, p.id_w, more, go);
                 }
                 if (p.part_out) mma<1, false>(tmem + kDw + 128, h + i * 128, dy + i * 128, p.id_w, more, go);
-                if (p.part_bo && rank == 0) mma<1, false>(tmem + kDb + 32, x_dy + i * 128, one, p.id_b, more, go);
+                if (p.part_bo && rank == 0)
+                    mma<1, false>(tmem + kDb + 32, x_dy + i * 128, one, p.id_b, more, go);
                 if (p.part_bi) {
                     mma<1, false>(tmem + kDb, dg + i * 128, one, p.id_b, more, go);
                     mma<1, false>(tmem + kDb + 16, du + i * 128, one, p.id_b, more, go);
@@ -1393,8 +1393,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) narrow_ffn_bwd_kernel(const __
                     const uint32_t dst = peer_addr(box + c0 * 128, rank ^ 1);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * 512), "f"(v[4 * k]), "f"(v[4 * k + 1]),
-                                     "f"(v[4 * k + 2]), "f"(v[4 * k + 3])
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * 512), "f"(v[4 * k]),
+                                     "f"(v[4 * k + 1]), "f"(v[4 * k + 2]), "f"(v[4 * k + 3])
                                      : "memory");
                     continue;
                 }
@@ -2445,8 +2445,9 @@ int launch_narrow_bwd(const NarrowBwdArgs& g, int slots, cudaStream_t st) {
     static std::once_flag once[64];
     int dev = 0;
     cudaGetDevice(&dev);
-    std::call_once(once[dev & 63], [] { cudaFuncSetAttribute(narrow_ffn_bwd_kernel<T, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
-    launch_early(narrow_ffn_bwd_kernel<T, CTAS>, (unsigned)(slots * CTAS), kBwdThreads, (size_t)bytes, CTAS, st, g);
+    const auto kernel = narrow_ffn_bwd_kernel<T, CTAS>;
+    std::call_once(once[dev & 63], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit); });
+    launch_early(kernel, (unsigned)(slots * CTAS), kBwdThreads, (size_t)bytes, CTAS, st, g);
     return check_launch("narrow_ffn_bwd_kernel");
 }
 
