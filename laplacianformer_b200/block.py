@@ -7,7 +7,8 @@
     out    = gated_feed_forward(m, W_in, W_out, residual=s)
 
 fp16 or bf16.  For serving, :meth:`LaplacianBlock.quantize_` lays the query-key-value weights out in 8 bits; the
-norm then writes 8-bit activations for them (no gradient).
+norm then writes 8-bit activations for them (no gradient).  The 16-bit weights stay the parameter: the 8-bit ones are
+made anew after they have changed, and are not part of the module's state.
 """
 from __future__ import annotations
 
@@ -38,17 +39,51 @@ class LaplacianBlock(torch.nn.Module):
         self.w_qkv, self.b_qkv = weight(3 * dim, dim), torch.nn.Parameter(torch.zeros(3 * dim, **kw))
         self.w_proj, self.b_proj = weight(dim, dim), torch.nn.Parameter(torch.zeros(dim, **kw))
         self.w_in, self.w_out = weight(2 * hidden, dim), weight(dim, hidden)
-        self.q8 = None
+        self.quantized = False
+        self.q8 = self._q8_of = None
 
     def quantize_(self) -> "LaplacianBlock":
-        """Keeps the query-key-value weights in 8 bits too; forward passes without gradients use them from now on."""
-        self.q8 = ops.quantize_rows(self.w_qkv.detach())
+        """Keeps the query-key-value weights in 8 bits too; forward passes without gradients use them from now on.
+
+        They are laid out again when w_qkv has been written, replaced or moved since, when the module changes between
+        train() and eval(), and within every captured graph.  The only write that this cannot see is one through
+        w_qkv.data in between, which leaves no trace: call quantize_() after it."""
+        self.quantized = True
+        self._lay_out()
         return self
 
+    def _lay_out(self):
+        """w_qkv in 8 bits, with what shows that it has changed since: the parameter itself, its storage (held, so that
+        its address is not given to another) and its version."""
+        w = self.w_qkv.detach()
+        pair = ops.quantize_rows(w)
+        if w.is_cuda and torch.cuda.is_current_stream_capturing():
+            return pair  # belongs to the graph, whose replays shall follow the weights
+        self.q8, self._q8_of = pair, (self.w_qkv, w, None if w.is_inference() else w._version)
+        return pair
+
+    def _weights8(self):
+        if self._q8_of is not None and not (self.w_qkv.is_cuda and torch.cuda.is_current_stream_capturing()):
+            of, w, version = self._q8_of
+            if of is self.w_qkv and w.data_ptr() == of.data_ptr() and version is not None and of._version == version:
+                return self.q8
+        return self._lay_out()
+
+    def _drop8(self):
+        self.q8 = self._q8_of = None
+
+    def train(self, mode: bool = True) -> "LaplacianBlock":
+        self._drop8()
+        return super().train(mode)
+
+    def _apply(self, *args, **kwargs):  # to(), cuda(), half() and the like
+        self._drop8()
+        return super()._apply(*args, **kwargs)
+
     def _qkv(self, x: torch.Tensor) -> torch.Tensor:
-        if self.q8 is not None and not torch.is_grad_enabled():
+        if self.quantized and not torch.is_grad_enabled():
             q, scale = ops.rms_norm_quant(x, self.norm1)
-            return ops.linear_quant(q, scale, *self.q8, self.b_qkv, dtype=x.dtype)
+            return ops.linear_quant(q, scale, *self._weights8(), self.b_qkv, dtype=x.dtype)
         return ops.linear(ops.rms_norm(x, self.norm1), self.w_qkv, self.b_qkv)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
