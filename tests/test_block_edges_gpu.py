@@ -1,0 +1,50 @@
+"""Edges of the block operators on a GPU: the activations' tails, rows and sums that are empty, tiny or huge, strided
+operands, gradients of some inputs only, graphs, refusals, and the extension's and the C ABI's own entry points."""
+import ctypes
+import math
+
+import pytest
+import torch
+import test_block_gpu as base
+from test_block_gpu import DT16, E, TINY, U, act64, gen, rand, slope64, slope_err, within
+
+from laplacianformer_b200 import capi, ops
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ activations
+
+
+def act_parts(z, name):
+    """The gate p with act(z) = z p, the two terms of act'(z) = p + z p', and the relative error that p may have in 32
+    bits: 8 E for the exponential, the reciprocal and the additions (16 E with a polynomial of seven terms), and what the
+    rounding of the exponential's argument adds (1.5 units in 2^-24 of it for the sigmoid, 2.5 for z^2 / 2, 6 for the
+    cubic).  z p' is formed of rounded 1 - p, so its error counts from its size without that factor."""
+    if name == "silu":
+        p, q = torch.sigmoid(z), torch.sigmoid(-z)
+        return p, z * p * q, (z * p).abs(), (8 + z.abs()) * E
+    if name == "gelu_tanh":
+        k = 2 * math.sqrt(2 / math.pi)
+        a, da = k * (z + 0.044715 * z**3), k * (1 + 3 * 0.044715 * z * z)
+        p, q = torch.sigmoid(a), torch.sigmoid(-a)
+        return p, z * p * q * da, (z * p).abs() * da, (8 + 3 * a.abs()) * E
+    t = z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    return 0.5 * torch.erfc(-z / math.sqrt(2)), t, t.abs(), (16 + z * z) * E
+
+
+@pytest.mark.parametrize("dtype", DT16)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_activation_tails(dtype, act):
+    """Values and slopes keep their leading digits where they are small: z itself through an identity weight."""
+    n = 64
+    z = torch.linspace(-8 if act == "gelu_tanh" else -12, 12, 700 * n, dtype=torch.float64).to(dtype).cuda().reshape(-1, n)
+    x, eye = z.clone().requires_grad_(), torch.eye(n, dtype=dtype, device="cuda")
+    y = ops.linear(x, eye, activation=act)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))  # the slope, rounded once as the product's operand
+    z = z.double()
+    p, zdp, steep, rel = act_parts(z, act)
+    u, tiny = U[dtype], TINY[dtype]
+    within(y.detach(), z * p, u * (z * p).abs() + 1.01 * rel * (z * p).abs() + tiny, "value")
+    s = p + zdp
+    within(dx, s, u * s.abs() + 1.01 * (2 * rel + 4 * E) * (p + steep) + tiny, "slope")
