@@ -71,21 +71,21 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 __device__ __forceinline__ float sigmoid(float z) { return rcp_fast(1.f + exp2_fast(-1.44269504f * z)); }
 
-// Phi(z) and phi(z) of the normal distribution.  Phi(-x) = t P(t) e^(-x^2/2) / 2
+// Phi(z) and phi(z) of the normal distribution.  Phi(-x) = t P(t) e^(-x^2/2)
 // with t = 1/(1 + 0.37295830 x/sqrt(2)), a form in which the relative error stays
 // small however far out x is (an approximation of erf to an absolute error
 // loses the tail's digits: at z = -4 gelu(z) is 1.3e-4).  P is this file's own
-// minimax fit of e^(y^2) erfc(y) / t over 0 <= y <= 9.4, relative error 5.2e-7; the
+// minimax fit of e^(y^2) erfc(y) / (2 t) over 0 <= y <= 9.4, relative error 5.2e-7; the
 // exponential is the density's, and its rounded argument costs z^2 2^-23 more.
 __device__ __forceinline__ float normal_cdf(float z, float& density) {
     const float t = rcp_fast(__fmaf_rn(0.26372134f, fabsf(z), 1.f));
     const float e = exp2_fast(-0.72134752f * z * z);
-    float q = __fmaf_rn(t, -0.13936391f, 0.41136116f);
-    q = __fmaf_rn(t, q, -0.15810639f);
-    q = __fmaf_rn(t, q, 0.30086389f);
-    q = __fmaf_rn(t, q, 0.15948902f);
-    q = __fmaf_rn(t, q, 0.2156473f);
-    q = __fmaf_rn(t, q, 0.21010844f) * (t * e) * 0.5f;  // Phi(-|z|)
+    float q = __fmaf_rn(t, -0.069681955f, 0.20568058f);
+    q = __fmaf_rn(t, q, -0.079053195f);
+    q = __fmaf_rn(t, q, 0.150431945f);
+    q = __fmaf_rn(t, q, 0.07974451f);
+    q = __fmaf_rn(t, q, 0.10782365f);
+    q = __fmaf_rn(t, q, 0.10505422f) * (t * e);  // Phi(-|z|)
     density = e * 0.39894228f;
     return z >= 0.f ? 1.f - q : q;
 }
