@@ -34,7 +34,7 @@ def act_parts(z, name):
 
 
 @pytest.mark.parametrize("dtype", DT16)
-@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_activation_tails(dtype, act):
     """Values and slopes keep their leading digits where they are small: z itself through an identity weight."""
     n = 64
