@@ -571,8 +571,9 @@ extern "C" int lf_rms_norm_quant_fwd(const void* x, const void* residual, const 
                                      void* s, int64_t rows, int64_t cols, int dtype, double eps, lf_stream_t stream) {
     clear_error();
     if (int rc = check_rows("lf_rms_norm_quant_fwd", rows, cols, dtype, {x, residual, weight, s}, {scale})) return rc;
-    if (rows == 0 || cols == 0) return LF_OK;
-    if (!x || !weight || !q || !scale || (residual != nullptr) != (s != nullptr)) {
+    if (rows == 0) return LF_OK;
+    // Rows without values have a scale as well: the kernel reads and writes nothing else of them.
+    if (!scale || (cols > 0 && (!x || !weight || !q || (residual != nullptr) != (s != nullptr)))) {
         set_error("lf_rms_norm_quant_fwd: x, weight, q and scale are required, residual and s go together");
         return LF_ERR_INVALID;
     }
@@ -584,8 +585,8 @@ extern "C" int lf_quantize_rows(const void* x, void* q, float* scale, int64_t ro
                                 lf_stream_t stream) {
     clear_error();
     if (int rc = check_rows("lf_quantize_rows", rows, cols, dtype, {x}, {scale})) return rc;
-    if (rows == 0 || cols == 0) return LF_OK;
-    if (!x || !q || !scale) {
+    if (rows == 0) return LF_OK;
+    if (!scale || (cols > 0 && (!x || !q))) {
         set_error("lf_quantize_rows: x, q and scale are required");
         return LF_ERR_INVALID;
     }

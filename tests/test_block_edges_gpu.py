@@ -48,3 +48,38 @@ def test_activation_tails(dtype, act):
     within(y.detach(), z * p, u * (z * p).abs() + 1.01 * rel * (z * p).abs() + tiny, "value")
     s = p + zdp
     within(dx, s, u * s.abs() + 1.01 * (2 * rel + 4 * E) * (p + steep) + tiny, "slope")
+
+
+# ------------------------------------------------------------------ rows without values, tiny rows
+
+
+def poison(n):
+    """Leaves NaN where the caching allocator takes the next small tensors from."""
+    torch.cuda.synchronize()
+    keep = [torch.full((n,), float("nan"), device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    del keep
+
+
+@pytest.mark.parametrize("dtype", list(U))
+def test_scales_of_empty_rows(dtype):
+    """A row without values is a row of zeros: its scale is 1."""
+    z = lambda *s: torch.zeros(*s, device="cuda", dtype=dtype)  # noqa: E731
+    for call in (lambda: ops.quantize_rows(z(5, 0)), lambda: ops.rms_norm_quant(z(5, 0), z(0)),
+                 lambda: ops.rms_norm_quant(z(5, 0), z(0), residual=z(5, 0))):
+        poison(5)
+        q, scale = call()[:2]
+        assert q.shape == (5, 0) and torch.equal(scale, torch.ones(5, device="cuda"))
+    assert ops.quantize_rows(z(0, 8))[1].shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", DT16)
+@pytest.mark.parametrize("m", [1, 5, 200])
+def test_linear_quant_of_empty_sums(dtype, m):
+    b, r = rand(gen("k0 quant"), dtype, 24), rand(gen("r0 quant", m), dtype, m, 24)
+    poison(m)
+    q, sx = ops.quantize_rows(torch.zeros(m, 0, device="cuda"))
+    poison(24)
+    wq, sw = ops.quantize_rows(torch.zeros(24, 0, device="cuda"))
+    y = ops.linear_quant(q, sx, wq, sw, b, residual=r, dtype=dtype)
+    within(y, b.double() + r.double(), (U[dtype] + E) * (b.double().abs() + r.double().abs()), "k = 0")
