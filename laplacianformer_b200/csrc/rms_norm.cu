@@ -65,6 +65,13 @@ __device__ __forceinline__ float group_reduce(float v, float* red) {
     return v;
 }
 
+// The scale of a row whose largest size is m.  The quotient is what may not be
+// zero: it underflows for m below 3e-43 (fp32 rows), where zeros would become NaN.
+__device__ __forceinline__ float row_scale(float m) {
+    const float scale = m / kE4m3Max;
+    return scale == 0.f ? 1.f : scale;
+}
+
 __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
@@ -179,7 +186,7 @@ __global__ void __launch_bounds__(block_of<G>(), fwd_blocks<NV, G>()) rms_fwd_ke
 #pragma unroll
             for (int i = 0; i < NV * VEC; ++i) m = max_nan(m, fabsf(v[i]));
             m = group_reduce<G, true>(m, red);
-            const float scale = m == 0.f ? 1.f : m / kE4m3Max;
+            const float scale = row_scale(m);
             if (live && g == 0) p.scale[base + sub] = scale;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -216,7 +223,7 @@ __global__ void __launch_bounds__(512) rms_fwd_long_kernel(const NormArgs p) {
             if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
         }
         for (int pass = QUANT ? 0 : 1; pass < 2; ++pass) {
-            const float scale = QUANT && pass ? (m == 0.f ? 1.f : m / kE4m3Max) : 1.f;
+            const float scale = QUANT && pass ? row_scale(m) : 1.f;
             if (QUANT && pass && threadIdx.x == 0) p.scale[row] = scale;
             for (int64_t c = threadIdx.x; c < p.cols; c += 512) {
                 float t = Elem<T>::load(x[c]);

@@ -83,3 +83,16 @@ def test_linear_quant_of_empty_sums(dtype, m):
     wq, sw = ops.quantize_rows(torch.zeros(24, 0, device="cuda"))
     y = ops.linear_quant(q, sx, wq, sw, b, residual=r, dtype=dtype)
     within(y, b.double() + r.double(), (U[dtype] + E) * (b.double().abs() + r.double().abs()), "k = 0")
+
+
+@pytest.mark.parametrize("cols", [5, 64, 771, 20000])
+def test_scale_of_tiny_rows(cols):
+    """fp32 rows whose largest value divided by 448 is zero: scale 1 and zeros, as a row of zeros has."""
+    x = torch.zeros(4, cols, device="cuda")
+    x[0, 1], x[1, :], x[2, 3], x[3, 0] = 1.4e-45, 2.0e-43, -1e-42, 1.0
+    q, scale = ops.quantize_rows(x)
+    assert torch.equal(scale[:2], torch.ones(2, device="cuda")) and (q[:2].float() == 0).all()
+    assert (scale > 0).all() and q.float().isfinite().all()
+    w = torch.full((cols,), 1e-44, device="cuda")
+    q, scale = ops.rms_norm_quant(torch.ones(2, cols, device="cuda"), w)
+    assert torch.equal(scale, torch.ones(2, device="cuda")) and (q.float() == 0).all()
