@@ -2269,7 +2269,7 @@ int check_linear(const char* what, const lf_linear_t* a, bool quant) {
     if (quant)
         if (int rc = check_aligned(what, {a->x_scale, a->w_scale}, 4)) return rc;
     if (a->m == 0 || a->n == 0) return LF_OK;
-    if (!a->w || !a->x) return a->k == 0 ? LF_OK : missing(what, "x and w are");
+    if (a->k > 0 && (!a->w || !a->x)) return missing(what, "x and w are");
     if (a->ldx < a->k || a->ldw < a->k || (a->residual && a->ldr < a->n)) {
         set_error("%s: a row stride is shorter than its row", what);
         return LF_ERR_INVALID;
