@@ -13,6 +13,10 @@
 //
 // Bound by memory: 302 M bf16 gradients (0.6 GB) 105 us for the sums (5.8
 // TB/s) and 200 us for the scaling (6.0 TB/s), of 6.5 measured for a copy.
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "lf_common.cuh"
 
 namespace lfb {
@@ -189,6 +193,40 @@ int64_t chunks_of(const int64_t* sizes, int64_t count, int chunk) {
     return k;
 }
 
+// Whether a tensor that is written shares memory with another one (an output
+// with any other output, or with any gradient but its own in place): its
+// elements would be read before or after the write by chance.  Gradients that
+// are only read may overlap.  Of a call of 11 us for 80 tensors this takes 0.3 us
+// in order of address (views of one buffer) and 0.8 in any order; 5 of 55 for 700.
+bool overlapping(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes, int64_t count) {
+    struct Span {
+        uintptr_t at, end;
+    };
+    std::vector<Span> written, read;
+    written.reserve(count);
+    for (int64_t i = 0; i < count; ++i) {
+        const size_t bytes = (size_t)sizes[i] * dtype_size(dtypes[i]);
+        if (bytes == 0) continue;
+        const uintptr_t g = (uintptr_t)grads[i], o = (uintptr_t)outs[i];
+        written.push_back({o, o + bytes});
+        if (g != o) read.push_back({g, g + bytes});
+    }
+    const auto before = [](const Span& a, const Span& b) { return a.at < b.at; };
+    for (auto* v : {&written, &read})
+        if (!std::is_sorted(v->begin(), v->end(), before)) std::sort(v->begin(), v->end(), before);
+    uintptr_t written_to = 0, read_to = 0;  // ends of the tensors that start before
+    auto r = read.begin();
+    for (const Span& w : written) {
+        for (; r != read.end() && r->at < w.at; ++r) {
+            if (r->at < written_to) return true;
+            read_to = std::max(read_to, r->end);
+        }
+        if (w.at < written_to || w.at < read_to) return true;
+        written_to = w.end;
+    }
+    return r != read.end() && r->at < written_to;
+}
+
 template <int N>
 int run_clip(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes, int64_t count, int chunk,
              int total, float max_norm, float* norm, double* part, cudaStream_t st) {
@@ -255,6 +293,15 @@ extern "C" int lf_clip_grad_norm(const void* const* grads, void* const* outs, co
             set_error("lf_clip_grad_norm: bad size or pointer of tensor %lld", (long long)i);
             return LF_ERR_INVALID;
         }
+    }
+    try {
+        if (overlapping(grads, outs, sizes, dtypes, count)) {
+            set_error("lf_clip_grad_norm: tensors overlap (an output may share memory with its own gradient alone)");
+            return LF_ERR_INVALID;
+        }
+    } catch (const std::bad_alloc&) {
+        set_error("lf_clip_grad_norm: out of host memory for %lld tensors", (long long)count);
+        return LF_ERR_UNSUPPORTED;
     }
     if (!workspace || !aligned(workspace, 8) || workspace_bytes < lf_clip_grad_norm_workspace_size(sizes, count)) {
         set_error("lf_clip_grad_norm: needs %zu bytes of workspace", lf_clip_grad_norm_workspace_size(sizes, count));

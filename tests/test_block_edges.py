@@ -1,5 +1,7 @@
 """CPU-side checks of the block operators' edges: refusals that depend on empty sizes or on overlapping memory, workspace
 bounds and the assignment of work units in shared launches."""
+import ctypes
+
 import pytest
 
 from laplacianformer_b200 import capi
@@ -23,3 +25,38 @@ def test_linear_refusals_of_empty_sums(change, x):
 def test_linear_quant_needs_scales_of_empty_sums(x, scales):
     a = capi.Linear(x=x, w=x, y=P, m=100, n=32, k=0, dtype=capi.LF_BF16, **scales)
     assert L.lf_linear_quant_fwd(a, None, 0, None) == capi.LF_ERR_INVALID and b"scale" in L.lf_last_error()
+
+
+def clip(grads, outs, sizes, dtypes):
+    """lf_clip_grad_norm on (pretended) addresses; without a GPU what is not refused ends in LF_ERR_CUDA."""
+    n = len(grads)
+    t = lambda ty, v: (ty * n)(*v)  # noqa: E731
+    return L.lf_clip_grad_norm(t(ctypes.c_void_p, grads), t(ctypes.c_void_p, outs), t(ctypes.c_int64, sizes), t(ctypes.c_int, dtypes), n, 1.0, P,
+                               2 * P, 1 << 20, None)
+
+
+# Tensors of 64 fp32 elements (256 bytes) at these offsets, as (grads, outs).
+@pytest.mark.parametrize("grads, outs", [
+    ((0, 0), (0, 0)),                        # one gradient twice, in place
+    ((0, 0), (1024, 1024)),                  # one output twice
+    ((0, 512), (0, 128)),                    # an output beside its own in-place neighbour's end
+    ((0, 252), (0, 252)),                    # views that share an element, in place
+    ((0, 512), (1024, 1276)),                # outputs that share an element
+    ((0, 512), (4, 1024)),                   # an output that starts inside its gradient
+    ((512, 0), (508, 1024)),                 # or ends inside it
+    ((0, 512), (512, 1024)),                 # an output on another's gradient
+    ((0, 512, 1024), (512, 0, 1024)),        # outputs exchanged
+    ((0, 0, 512), (0, 1024, 512)),           # read again by the second gradient while the first is written
+    ((4096, 0, 2048), (4096, 2052, 2048)),   # not in order of address
+])
+def test_clip_refuses_overlapping_tensors(grads, outs):
+    base = 1 << 30
+    n = len(grads)
+    code = clip([base + v for v in grads], [base + v for v in outs], [64] * n, [capi.LF_F32] * n)
+    assert code == capi.LF_ERR_INVALID and b"overlap" in L.lf_last_error()
+
+
+def test_clip_refuses_a_view_beside_its_base():
+    base = 1 << 30
+    assert clip([base, base + 100], [base, base + 100], [1000, 10], [capi.LF_F16, capi.LF_BF16]) == capi.LF_ERR_INVALID
+    assert clip([base + 100, base], [base + 100, base], [10, 1000], [capi.LF_F16, capi.LF_BF16]) == capi.LF_ERR_INVALID

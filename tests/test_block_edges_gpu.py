@@ -96,3 +96,22 @@ def test_scale_of_tiny_rows(cols):
     w = torch.full((cols,), 1e-44, device="cuda")
     q, scale = ops.rms_norm_quant(torch.ones(2, cols, device="cuda"), w)
     assert torch.equal(scale, torch.ones(2, device="cuda")) and (q.float() == 0).all()
+
+
+# ------------------------------------------------------------------ clipping
+
+
+def test_clip_grad_norm_of_shared_memory():
+    """Gradients that are only read may be the same one or overlap; written ones may not."""
+    g = rand(gen("shared"), torch.float32, 1000)
+    for grads in ([g, g], [g, g[100:300]]):
+        n64 = math.sqrt(sum(float(t.double().square().sum()) for t in grads))
+        norm, out = ops.clip_grad_norm(grads, 0.5)
+        assert abs(float(norm) - n64) <= 300 * E * n64
+        for a, b in zip(grads, out):
+            ref = a.double() * (0.5 / (n64 + 1e-6))
+            within(b, ref, (U[torch.float32] + 310 * E) * ref.abs() + TINY[torch.float32], "shared")
+        before = g.clone()
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.clip_grad_norm(grads, 0.5, out=grads)
+        assert torch.equal(g, before)
