@@ -370,6 +370,10 @@ at::Tensor ClipGradNorm(const std::vector<const at::Tensor*>& grads, const std::
     raise_on(lf_clip_grad_norm(in.data(), out.data(), sizes.data(), dtypes.data(), (int64_t)n, max_norm,
                                (float*)norm.data_ptr(), mut(ws), need, stream_of(*grads[0])),
              "ClipGradNorm");
+    // The outputs were written behind autograd's back: tell it, so that a
+    // backward pass that saved one of them is refused.
+    for (const at::Tensor* o : outs)
+        if (!o->is_inference()) o->unsafeGetTensorImpl()->bump_version();
     return norm;
 }
 

@@ -115,3 +115,20 @@ def test_clip_grad_norm_of_shared_memory():
         with pytest.raises(RuntimeError, match="overlap"):
             ops.clip_grad_norm(grads, 0.5, out=grads)
         assert torch.equal(g, before)
+
+
+def test_clip_grad_norm_counts_as_a_write():
+    """Written tensors get a new version, so that autograd refuses to use what it saved before."""
+    a, b = (torch.ones(40, device="cuda") for _ in range(2))
+    x = torch.ones(40, device="cuda", requires_grad=True)
+    y = (x * a).sum()
+    va, vb = a._version, b._version
+    ops.clip_grad_norm([a], 0.5, out=[b])
+    assert a._version == va and b._version > vb
+    ops.clip_grad_norm([a], 0.5, out=[a])
+    assert a._version > va
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        c = torch.full((4,), 2.0, device="cuda")
+        assert abs(float(ops.clip_grad_norm([c], 1.0, out=[c])[0]) - 4) < 1e-5 and abs(float(c[0]) - 0.5) < 1e-5
