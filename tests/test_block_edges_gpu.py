@@ -101,6 +101,21 @@ def test_scale_of_tiny_rows(cols):
 # ------------------------------------------------------------------ clipping
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("where", [0, 3, 70000, 200000])
+def test_clip_grad_norm_of_huge_values(dtype, where):
+    """Squares that pass the largest fp32 number: the norm is finite, so gradients are scaled and not erased."""
+    g = gen("huge", dtype, where)
+    flat = rand(g, dtype, 200001, scale=1e20)
+    flat[where] = 1e25
+    grads = list(flat.split([1001, 100000, 99000]))
+    n64 = float(flat.double().norm())
+    norm, out = ops.clip_grad_norm(grads, 2.0)
+    assert abs(float(norm) - n64) <= 300 * E * n64
+    ref = flat.double() * (2.0 / (n64 + 1e-6))
+    within(torch.cat(out), ref, (U[dtype] + 310 * E) * ref.abs() + TINY[dtype], "clipped")
+
+
 def test_clip_grad_norm_of_shared_memory():
     """Gradients that are only read may be the same one or overlap; written ones may not."""
     g = rand(gen("shared"), torch.float32, 1000)
