@@ -466,17 +466,22 @@ struct GatedFeedForwardNode : torch::autograd::Function<GatedFeedForwardNode> {
     }
 };
 
-bool tracked(std::initializer_list<const at::Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const at::Tensor* t : ts)
-        if (t->defined() && t->requires_grad()) return true;
-    return false;
+// Whether a backward pass can be asked for.  There is no forward-mode
+// derivative: a tangent that the plain call would drop is refused.
+bool tracked(const char* op, std::initializer_list<const at::Tensor*> ts) {
+    bool any = false;
+    for (const at::Tensor* t : ts) {
+        if (!t->defined()) continue;
+        TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), std::string(op) + " has no forward-mode derivative");
+        any = any || t->requires_grad();
+    }
+    return any && at::GradMode::is_enabled();
 }
 
 }  // namespace
 
 std::tuple<at::Tensor, at::Tensor> RmsNorm(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& residual, double eps) {
-    if (tracked({&x, &weight, &residual})) {
+    if (tracked("rms_norm", {&x, &weight, &residual})) {
         variable_list out = RmsNormNode::apply(x, weight, as_opt(residual), eps);
         return {out[0], out.size() > 1 ? out[1] : at::Tensor()};
     }
@@ -485,13 +490,13 @@ std::tuple<at::Tensor, at::Tensor> RmsNorm(const at::Tensor& x, const at::Tensor
 }
 
 at::Tensor Linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, const at::Tensor& residual, int64_t act) {
-    if (tracked({&x, &weight, &bias, &residual})) return LinearNode::apply(x, weight, as_opt(bias), as_opt(residual), act);
+    if (tracked("linear", {&x, &weight, &bias, &residual})) return LinearNode::apply(x, weight, as_opt(bias), as_opt(residual), act);
     return Linear_forward(x, weight, bias, residual, act);
 }
 
 at::Tensor GatedFeedForward(const at::Tensor& x, const at::Tensor& w_in, const at::Tensor& w_out, const at::Tensor& b_in,
                             const at::Tensor& b_out, const at::Tensor& residual, int64_t act) {
-    if (tracked({&x, &w_in, &w_out, &b_in, &b_out, &residual}))
+    if (tracked("gated_feed_forward", {&x, &w_in, &w_out, &b_in, &b_out, &residual}))
         return GatedFeedForwardNode::apply(x, w_in, w_out, as_opt(b_in), as_opt(b_out), as_opt(residual), act);
     return GatedFeedForward_forward(x, w_in, w_out, b_in, b_out, residual, act);
 }

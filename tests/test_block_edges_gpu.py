@@ -147,3 +147,34 @@ def test_clip_grad_norm_counts_as_a_write():
     with torch.inference_mode():
         c = torch.full((4,), 2.0, device="cuda")
         assert abs(float(ops.clip_grad_norm([c], 1.0, out=[c])[0]) - 4) < 1e-5 and abs(float(c[0]) - 0.5) < 1e-5
+
+
+# ------------------------------------------------------------------ other kinds of differentiation
+
+
+def forms(dtype=torch.bfloat16):
+    """Each differentiable operator as a function of x."""
+    g = gen("forms", dtype)
+    w, wi, wo = rand(g, dtype, 24, 32, scale=0.2), rand(g, dtype, 80, 32, scale=0.2), rand(g, dtype, 32, 40, scale=0.2)
+    wn, r = rand(g, dtype, 32), rand(g, dtype, 12, 32)
+    return {"rms_norm": lambda x: ops.rms_norm(x, wn), "rms_norm residual": lambda x: ops.rms_norm(r, wn, residual=x)[0],
+            "rms_norm weight": lambda x: ops.rms_norm(r, x[0]), "linear": lambda x: ops.linear(x, w),
+            "linear weight": lambda x: ops.linear(r, x, activation="gelu"), "linear residual": lambda x: ops.linear(r, wi[:32], residual=x),
+            "gated_feed_forward": lambda x: ops.gated_feed_forward(x, wi, wo),
+            "gated_feed_forward residual": lambda x: ops.gated_feed_forward(r, wi, wo, residual=x)}
+
+
+@pytest.mark.parametrize("form", ["rms_norm", "rms_norm residual", "rms_norm weight", "linear", "linear weight", "linear residual",
+                                  "gated_feed_forward", "gated_feed_forward residual"])
+def test_forward_mode_is_refused(form):
+    """There is no forward-mode derivative, and a tangent is not dropped in silence."""
+    from torch.autograd import forward_ad
+
+    f = forms()[form]
+    x, t = (rand(gen("dual", k), torch.bfloat16, 12, 32) for k in "xt")
+    for tracked in (False, True):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x.clone().requires_grad_(tracked), t)
+            with pytest.raises(RuntimeError, match="forward"):
+                f(dual)
+        f(x)
