@@ -473,10 +473,16 @@ unsigned row_blocks(int64_t rows, int per_block, int slots) {
     return (unsigned)(want < slots ? want : slots);
 }
 
-// Rows of partial sums in the backward's workspace: never fewer than its
-// blocks, of which there are at most 2048 threads' worth per SM.
+// Blocks per SM of the backward, at most 2048 threads' worth: by the smallest
+// block that any type and alignment takes for a row of this width (the tables
+// above; up to 256 columns eight, which is as many as a warp per row gives).
+int64_t bwd_blocks_per_sm(int64_t cols) {
+    return cols <= 256 ? 8 : 2048 / (cols <= 512 ? 64 : cols <= 768 ? 96 : cols <= 1024 ? 128 : cols <= 1536 ? 192 : cols <= 2048 ? 256 : 512);
+}
+
+// Rows of partial sums in the backward's workspace: never fewer than its blocks.
 int64_t bwd_part_rows(int64_t rows, int64_t cols) {
-    const int64_t most = (int64_t)num_sms() * (cols <= 256 ? 8 : 32);
+    const int64_t most = (int64_t)num_sms() * bwd_blocks_per_sm(cols);
     return rows < most ? rows : most;
 }
 

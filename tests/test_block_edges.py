@@ -60,3 +60,13 @@ def test_clip_refuses_a_view_beside_its_base():
     base = 1 << 30
     assert clip([base, base + 100], [base, base + 100], [1000, 10], [capi.LF_F16, capi.LF_BF16]) == capi.LF_ERR_INVALID
     assert clip([base + 100, base], [base + 100, base], [10, 1000], [capi.LF_F16, capi.LF_BF16]) == capi.LF_ERR_INVALID
+
+
+# Rows of partial sums that the norm's backward can write: one per resident block, of at most 2048 threads an SM.  Widths
+# from the narrowest row groups to rows that are read twice.
+@pytest.mark.parametrize("cols, per_sm", [(64, 8), (256, 8), (512, 32), (768, 21), (1024, 16), (1536, 10), (2048, 8), (2049, 4), (8192, 4), (20000, 4)])
+def test_norm_workspace_has_a_row_per_resident_block(cols, per_sm):
+    sms = L.lf_rms_norm_bwd_workspace_size(1 << 20, 64) // (8 * 64 * 4)
+    assert 100 <= sms <= 200
+    assert L.lf_rms_norm_bwd_workspace_size(1 << 20, cols) == per_sm * sms * cols * 4
+    assert L.lf_rms_norm_bwd_workspace_size(3, cols) == 3 * cols * 4
