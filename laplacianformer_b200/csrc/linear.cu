@@ -35,6 +35,7 @@
 #include <type_traits>
 
 #include "tc_ptx.cuh"
+#include "unit_plan.h"
 
 namespace lfb {
 
@@ -272,10 +273,7 @@ template <int N>
 struct GemmArgs {
     Problem p[N];
     int first[N + 1];          // first work unit of each problem; first[N] units in all
-    // Units go to the CTAs (or pairs) in turn.  The last problem's units may be
-    // shorter than the others' (`longer` of them): the CTAs that got one long
-    // unit fewer take `extra` of them each before the turns go on.
-    int longer, extra;
+    int longer, extra;         // units of the problems before the last; see unit_plan.h
     int stages, stage_bytes;
 };
 
@@ -283,11 +281,7 @@ struct GemmArgs {
 template <int N>
 __device__ __forceinline__ int unit_of(const GemmArgs<N>& a, int c, int P, int k) {
     if constexpr (N == 1) return c + k * P;
-    const int longer = a.longer, have = longer > c ? (longer - c + P - 1) / P : 0;
-    if (k < have) return c + k * P;
-    const int j = k - have, ahead = longer % P, behind = P - ahead;
-    if (c >= ahead) return j < a.extra ? longer + j * behind + c - ahead : longer + a.extra * behind + c + (j - a.extra) * P;
-    return longer + a.extra * behind + c + j * P;
+    else return unit_at(a.longer, a.extra, c, P, k);
 }
 template <int N>
 __device__ __forceinline__ int problem_of(const GemmArgs<N>& a, int& unit) {
@@ -2102,9 +2096,9 @@ int run_products(const Product* in, int given, Arena& ws, cudaStream_t st) {
         if (part[k]) join.job[joins++] = join_of(q[k], part[k], g.p[i].splits);
     }
     g.first[3] = (int)at;
-    const int lanes = num_sms() / s[0].ctas, ahead = g.longer % lanes, last = (int)units_of(g.p[count - 1]);
-    if (ahead && last > 0 && g.longer + last >= lanes)
-        g.extra = (int)std::min<double>(unit[order[0]] / unit[order[count - 1]] + 0.5, last / (lanes - ahead));
+    // The long units' last turn is the problem's before the last.
+    g.extra = extra_units(g.longer, (int)at - g.longer, std::min((int)at, num_sms() / s[0].ctas),
+                          unit[order[count - 2]] / unit[order[count - 1]]);
     const int rc = q[0].dtype == LF_F16 ? launch_ctas<__half, kLinear, false>(g, s[0].ctas, st)
                                         : launch_ctas<__nv_bfloat16, kLinear, false>(g, s[0].ctas, st);
     return rc || !joins ? rc : join_splits(join, joins, q[0].dtype, st);

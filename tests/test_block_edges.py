@@ -1,6 +1,8 @@
 """CPU-side checks of the block operators' edges: refusals that depend on empty sizes or on overlapping memory, workspace
 bounds and the assignment of work units in shared launches."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 
@@ -70,3 +72,46 @@ def test_norm_workspace_has_a_row_per_resident_block(cols, per_sm):
     assert 100 <= sms <= 200
     assert L.lf_rms_norm_bwd_workspace_size(1 << 20, cols) == per_sm * sms * cols * 4
     assert L.lf_rms_norm_bwd_workspace_size(3, cols) == 3 * cols * 4
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    """The kernels' own assignment of work units, compiled for the host."""
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text('#include "unit_plan.h"\n'
+                                'extern "C" int unit_at(int l, int e, int c, int p, int k) { return lfb::unit_at(l, e, c, p, k); }\n'
+                                'extern "C" int extra_units(int l, int n, int p, double r) { return lfb::extra_units(l, n, p, r); }\n')
+    csrc = os.path.join(os.path.dirname(capi.__file__), "csrc")
+    subprocess.check_call(["g++", "-O1", "-shared", "-fPIC", "-I", csrc, str(d / "plan.cpp"), "-o", str(d / "plan.so")])
+    lib = ctypes.CDLL(str(d / "plan.so"))
+    lib.extra_units.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_double]
+    return lib
+
+
+def assigned(plan, longer, last, lanes, ratio):
+    """Units of each CTA of a launch of `longer` units and `last` shorter ones on at most `lanes` CTAs."""
+    total = longer + last
+    P = min(lanes, total)
+    extra, out = plan.extra_units(longer, last, P, ratio), []
+    for c in range(P):
+        mine, k = [], 0
+        while (u := plan.unit_at(longer, extra, c, P, k)) < total:
+            mine.append(u)
+            k += 1
+        out.append(mine)
+    return out
+
+
+@pytest.mark.parametrize("longer, last, lanes", [(1, 1, 148), (28, 36, 74), (32, 32, 74), (16, 48, 148), (64, 128, 148), (147, 1, 148), (148, 5, 148),
+                                                 (149, 3, 148), (200, 400, 148), (74, 74, 74), (75, 75, 74), (1, 500, 74), (500, 1, 74), (0, 9, 74),
+                                                 (30, 43, 74), (30, 45, 74), (1000, 1000, 148), (7, 0, 74)])
+@pytest.mark.parametrize("ratio", [1.0, 1.4, 2.0, 3.7, 9.0])
+def test_shared_launches_use_every_lane(plan, longer, last, lanes, ratio):
+    """Each unit once, in rising order on a CTA, none idle while another has two, and loads within a long unit."""
+    cta = assigned(plan, longer, last, lanes, ratio)
+    assert sorted(u for mine in cta for u in mine) == list(range(longer + last))
+    assert all(mine == sorted(mine) and mine for mine in cta)
+    load = [sum(ratio if u < longer else 1 for u in mine) for mine in cta]
+    assert max(load) - min(load) <= max(ratio, 1) + 1
+    if longer + last <= lanes:
+        assert all(len(mine) == 1 for mine in cta)
