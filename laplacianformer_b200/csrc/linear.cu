@@ -123,7 +123,8 @@ __device__ __forceinline__ void act_both(float z, float& a, float& slope) {
     } else if constexpr (ACT == LF_ACT_GELU_TANH) {
         const float p = tanh_gate(z);
         a = z * p;
-        slope = __fmaf_rn(a * (1.f - p), __fmaf_rn(0.21406445f * z, z, 1.59576912f), p);  // d/dz of the gate's argument: k (1 + 3 c z^2)
+        const float d = fminf(__fmaf_rn(0.21406445f * z, z, 1.59576912f), 1e30f);  // of the gate's argument: k (1 + 3 c z^2),
+        slope = __fmaf_rn(a * (1.f - p), d, p);                                   // finite where p is 0 or 1
     } else {
         a = z;
         slope = 1.f;

@@ -50,6 +50,19 @@ def test_activation_tails(dtype, act):
     within(dx, s, u * s.abs() + 1.01 * (2 * rel + 4 * E) * (p + steep) + tiny, "slope")
 
 
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
+def test_activations_of_huge_values(act):
+    """Finite values whose squares or cubes pass fp32's range: z or 0, with a slope of 1 or 0."""
+    n = 64
+    z = torch.tensor([s * v for v in (60000.0, 1e10, 1.2e13, 1e19, 2e19, 1e30, 3e38) for s in (1, -1)]).bfloat16().cuda()
+    x = torch.zeros(z.numel(), n, dtype=torch.bfloat16, device="cuda")
+    x[:, 5] = z
+    x.requires_grad_()
+    y = ops.linear(x, torch.eye(n, dtype=torch.bfloat16, device="cuda"), activation=act)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(y[:, 5], torch.relu(z)) and torch.equal(dx[:, 5].float(), (z > 0).float())
+
+
 # ------------------------------------------------------------------ rows without values, tiny rows
 
 
