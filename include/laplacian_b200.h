@@ -49,7 +49,7 @@ enum lf_dtype {
 enum lf_activation {
     LF_ACT_NONE = 0,
     LF_ACT_RELU = 1,
-    LF_ACT_GELU = 2,      /* z Phi(z), by erf */
+    LF_ACT_GELU = 2,      /* z Phi(z), Phi the normal distribution (to a relative (16 + z^2) 2^-23, tail included) */
     LF_ACT_GELU_TANH = 3, /* its tanh approximation */
     LF_ACT_SILU = 4       /* z / (1 + exp(-z)) */
 };
@@ -380,8 +380,9 @@ LF_API int lf_rms_norm_bwd(const void* dy, const void* ds, const void* s, const 
                            void* dx, void* dw, int64_t rows, int64_t cols, int dtype, void* workspace,
                            size_t workspace_bytes, lf_stream_t stream);
 
-/* lf_rms_norm_fwd with its output in 8 bits: per row scale = max|y| / 448 (1 for
-   a row of zeros) and q = e4m3(y / scale), from the unrounded y. */
+/* lf_rms_norm_fwd with its output in 8 bits: per row scale = max|y| / 448 (1
+   where that is zero: rows of zeros, of no column, or below 3e-43) and
+   q = e4m3(y / scale), from the unrounded y. */
 LF_API int lf_rms_norm_quant_fwd(const void* x, const void* residual, const void* weight, void* q, float* scale, void* s,
                                  int64_t rows, int64_t cols, int dtype, double eps, lf_stream_t stream);
 
@@ -413,7 +414,8 @@ LF_API int lf_linear_quant_fwd(const lf_linear_t* args, void* workspace, size_t 
 
 /* Gradients of lf_linear_fwd: with z = x w^T + bias recomputed where there is
    an activation, dz = dy act'(z) (rounded to dtype as an operand of the
-   products that follow), dx = dz w, dw = dz^T x, db = sum of dz's rows.  The
+   products that follow, infinite beyond 65504 in fp16), dx = dz w, dw = dz^T x,
+   db = sum of dz's rows.  The
    residual's gradient is dy.  The workspace sizes of this and the other
    struct entry points depend on the sizes, the strides, the alignment of the
    pointers and which gradients are asked for: ask with the struct that will
@@ -424,7 +426,9 @@ LF_API int lf_linear_bwd(const lf_linear_t* args, void* workspace, size_t worksp
 /* Gated feed-forward block on m tokens of c channels, hidden width f:
    [g|u] = x w_in^T + b_in with w_in [2f, c] (gate rows, then up rows),
    h = act(g) u (rounded to dtype as an operand), y = h w_out^T + b_out + residual
-   with w_out [c, f].  Weights, y and the gradients are dense. */
+   with w_out [c, f].  Weights, y and the gradients are dense.  In fp16 h, and dg
+   and du in the backward, become infinite beyond 65504 although sums of them
+   might not be; bf16 has fp32's range. */
 typedef struct lf_gated_ffn {
     const void *x, *w_in, *b_in, *w_out, *b_out, *residual;
     void* y;
@@ -446,9 +450,12 @@ LF_API int lf_gated_ffn_bwd(const lf_gated_ffn_t* args, void* workspace, size_t 
 /* norm = sqrt of the sum of squares over all `count` tensors, and
    outs[i] = min(1, max_norm / (norm + 1e-6)) * grads[i].  Tensor i has sizes[i]
    elements of type dtypes[i] (F32, F16 or BF16, mixed freely); outs[i] may be
-   grads[i].  A norm that is not finite gives what the formula gives (NaN
-   gradients).  The tables are host arrays, read before the call returns;
-   norm is one device float. */
+   grads[i].  Otherwise an output shares memory with no output and no gradient:
+   such calls are refused.  Gradients that no output touches may overlap.  The
+   norm is finite wherever it fits fp32.  A NaN norm gives NaN everywhere; an
+   infinite one zeros, and NaN at infinite elements, as the formula does.  The
+   tables are host arrays, read before the call returns; norm is one device
+   float. */
 LF_API size_t lf_clip_grad_norm_workspace_size(const int64_t* sizes, int64_t count);
 LF_API int lf_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes,
                              int64_t count, double max_norm, float* norm, void* workspace, size_t workspace_bytes,

@@ -22,12 +22,14 @@
 //
 // Roundings to 16 bits besides the outputs': h, dg, du and dz, as operands of
 // the products that follow (the tensor cores take 16-bit operands; a second
-// part of each would double those products).
+// part of each would double those products).  The bias gradients of the
+// activation and of the gate are sums of these rounded values, and in fp16 all
+// four become infinite beyond 65504.
 //
 // Measured on a B200 (131072 tokens, 1024 channels, 4096 hidden, bf16): gated
-// forward 1.4-1.6 ms (1.4-1.5 PFLOP/s, tensor pipe 95 % active), gated backward
-// 2.75 ms (1.2), down projection 0.81 ms (1.36), the three gradients' products
-// 3.84 ms (1.43), against cuBLAS's 1.38 PFLOP/s under the same power cap.
+// forward 1.4-1.7 ms (1.3-1.5 PFLOP/s, tensor pipe 95 % active), gated backward
+// 2.75-2.86 ms (1.2), down projection 0.81-0.85 ms (1.3), the three gradients'
+// products 3.84-4.03 ms (1.4), against cuBLAS's 1.38 PFLOP/s under the same power cap.
 #include <cuda.h>
 
 #include <algorithm>
@@ -2044,7 +2046,10 @@ int run_product(const Product& q, Arena& ws, cudaStream_t st) {
 
 // Up to three products of 16-bit operands that do not depend on one another,
 // in one launch: a gradient's products are often too small to fill the SMs
-// one by one, and large ones fill each other's last wave.
+// one by one, and large ones fill each other's last wave.  Where the estimates
+// say so they run apart: over 44 drawn backward passes (16 to 40000 rows) the
+// rule measured 1.002 times the better way's time, 1.10 at worst (always shared
+// 1.008, always apart 1.15).
 int run_products(const Product* in, int given, Arena& ws, cudaStream_t st) {
     Product q[3];
     int count = 0;
@@ -2412,7 +2417,10 @@ int launch_narrow(NarrowArgs& g, cudaStream_t st) {
 // columns or enough tiles of 128 tokens, since a CTA takes a tile's hidden
 // columns one after another (64 channels, bf16, us, one kernel and two:
 // 100352 tokens, 256 hidden 31 and 41; 500 tokens 8.0 and 9.3; 100352 tokens,
-// 1024 hidden 85 and 126; 9472 tokens 18 and 19; 2000 tokens 18 and 13).
+// 1024 hidden 85 and 126; 9472 tokens 18 and 19; 2000 tokens 18 and 13).  From
+// 65 to 128 channels one kernel, with its weights through a ring, was slower than
+// two (100352 tokens: 96 channels, 384 hidden 71 and 62; 128, 512 90 and 80; at
+// most 4 % faster, 72, 256: 56 and 57).
 bool narrow(const lf_gated_ffn_t* a) {
     return a->f > 0 && a->c <= kNarrow && !few_rows(a->m, 3 * a->f, a->c) &&
            (a->f <= 5 * kHB || 2 * ((a->m + kBM - 1) / kBM) >= num_sms());

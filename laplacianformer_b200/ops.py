@@ -189,7 +189,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension, s = x + residual.
 
     Returns y, or (y, s) when a residual is given (s continues the residual
-    stream).  fp32, fp16 and bf16; statistics in fp32."""
+    stream).  fp32, fp16 and bf16; statistics in fp32.  Strided rows are copied first."""
     y, s = ext().RmsNorm(x, weight, residual, eps)
     return y if residual is None else (y, s)
 
@@ -208,11 +208,15 @@ def quantize_rows(x: torch.Tensor):
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
            residual: torch.Tensor | None = None) -> torch.Tensor:
-    """activation(x @ weight.T + bias) + residual in one kernel, for fp16 and bf16.
+    """activation(x @ weight.T + bias) + residual, finished in the product's kernel, for fp16 and bf16.
 
     x [..., K] (rows may be strided), weight [N, K] as torch.nn.Linear keeps it,
-    bias [N], residual [..., N].  activation: none, relu, gelu, gelu_tanh or
-    silu; the backward recomputes the pre-activation instead of keeping it."""
+    bias [N], residual [..., N], all of one dtype (autocast is not followed).
+    activation: none, relu, gelu, gelu_tanh or silu; the backward recomputes the
+    pre-activation instead of keeping it.  Operands whose rows do not start on
+    16-byte boundaries are packed in a launch before, and a product with few
+    output tiles is split along K and joined in a launch after.  First order,
+    reverse mode only."""
     return ext().Linear(x, weight, bias, residual, _act(activation))
 
 
@@ -232,9 +236,12 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
                        residual: torch.Tensor | None = None) -> torch.Tensor:
     """(activation(g) * u) @ w_out.T + b_out + residual with [g | u] = x @ w_in.T + b_in, for fp16 and bf16.
 
-    x [..., C], w_in [2F, C] (gate rows, then up rows), w_out [C, F].  Both
-    projections, the activation and the product run in one kernel; between the
-    passes only x is kept, the backward recomputes the projections."""
+    x [..., C], w_in [2F, C] (gate rows, then up rows), w_out [C, F], all of one
+    dtype.  Gate and up projection, the activation and their product run in one
+    kernel and the down projection in another; with up to 64 channels all of it
+    is one kernel (except for few tokens of many hidden columns).  Between the
+    passes only x is kept, the backward recomputes the projections.  In fp16 the
+    hidden values and their gradients become infinite beyond 65504."""
     return ext().GatedFeedForward(x, w_in, w_out, b_in, b_out, residual, _act(activation))
 
 
@@ -243,7 +250,8 @@ def clip_grad_norm(grads, max_norm: float, out=None):
 
     Returns (norm, out): norm a float32 device scalar (nothing is read back to
     the host), out the clipped tensors.  `out` may be given, `grads` itself
-    included (in place).  fp32, fp16 and bf16 tensors may be mixed."""
+    included (in place); written tensors may not overlap others.  fp32, fp16 and
+    bf16 tensors may be mixed.  A NaN norm gives NaN, an infinite one zeros."""
     grads = list(grads)
     out = [torch.empty_like(g) for g in grads] if out is None else list(out)
     return ext().ClipGradNorm(grads, out, float(max_norm)), out
