@@ -40,7 +40,12 @@ class LaplacianBlock(torch.nn.Module):
         self.w_proj, self.b_proj = weight(dim, dim), torch.nn.Parameter(torch.zeros(dim, **kw))
         self.w_in, self.w_out = weight(2 * hidden, dim), weight(dim, hidden)
         self.quantized = False
-        self.q8 = self._q8_of = None
+        self._q8 = None
+
+    @property
+    def q8(self):
+        """The 8-bit query-key-value weights and their scales, where they are laid out."""
+        return None if self._q8 is None else self._q8[0]
 
     def quantize_(self) -> "LaplacianBlock":
         """Keeps the query-key-value weights in 8 bits too; forward passes without gradients use them from now on.
@@ -53,31 +58,39 @@ class LaplacianBlock(torch.nn.Module):
         return self
 
     def _lay_out(self):
-        """w_qkv in 8 bits, with what shows that it has changed since: the parameter itself, its storage (held, so that
-        its address is not given to another) and its version."""
+        """w_qkv in 8 bits, kept with what shows that it has changed since (the parameter itself, its storage, which is
+        held so that its address is not given to another, and its version) and with the stream that made it."""
         w = self.w_qkv.detach()
         pair = ops.quantize_rows(w)
-        if w.is_cuda and torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_current_stream_capturing():
             return pair  # belongs to the graph, whose replays shall follow the weights
-        self.q8, self._q8_of = pair, (self.w_qkv, w, None if w.is_inference() else w._version)
+        stream = torch.cuda.current_stream(w.device)
+        self._q8 = pair, self.w_qkv, w, None if w.is_inference() else w._version, stream, stream.record_event()
         return pair
 
     def _weights8(self):
-        if self._q8_of is not None and not (self.w_qkv.is_cuda and torch.cuda.is_current_stream_capturing()):
-            of, w, version = self._q8_of
-            if of is self.w_qkv and w.data_ptr() == of.data_ptr() and version is not None and of._version == version:
-                return self.q8
-        return self._lay_out()
+        kept = self._q8  # read once: another thread may lay out at the same time
+        if kept is None or torch.cuda.is_current_stream_capturing():
+            return self._lay_out()
+        pair, of, w, version, stream, made = kept
+        if of is not self.w_qkv or w.data_ptr() != of.data_ptr() or version is None or of._version != version:
+            return self._lay_out()
+        here = torch.cuda.current_stream(w.device)
+        if here != stream:
+            here.wait_event(made)
+            for t in pair:
+                t.record_stream(here)
+        return pair
 
-    def _drop8(self):
-        self.q8 = self._q8_of = None
+    def __getstate__(self):  # copies and pickles lay out their own
+        return {**self.__dict__, "_q8": None}
 
     def train(self, mode: bool = True) -> "LaplacianBlock":
-        self._drop8()
+        self._q8 = None
         return super().train(mode)
 
     def _apply(self, *args, **kwargs):  # to(), cuda(), half() and the like
-        self._drop8()
+        self._q8 = None
         return super()._apply(*args, **kwargs)
 
     def _qkv(self, x: torch.Tensor) -> torch.Tensor:

@@ -1,5 +1,6 @@
 """The 8-bit form of LaplacianBlock beside weights that change after it was laid out."""
 import copy
+import io
 
 import pytest
 import torch
@@ -84,3 +85,41 @@ def test_block_quantized_copies_and_modes():
         torch.cuda.synchronize()
         assert torch.equal(y, eight_bit(b, x)) and torch.equal(b(x), y)
     assert set(b.state_dict()) == set(LaplacianBlock(64, heads=2, grid=8).state_dict())
+
+
+def test_block_quantized_on_another_stream():
+    """A forward on one stream lays the weights out late; one on another stream waits for that, and keeps them alive."""
+    torch.manual_seed(4)
+    b = LaplacianBlock(64, heads=2, grid=8, device="cuda").quantize_()
+    x = torch.randn(2, 64, 64, device="cuda").bfloat16()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        for _ in range(3):
+            b.w_qkv.mul_(1.25)
+            want = eight_bit(b, x)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(one):
+                torch.cuda._sleep(50_000_000)
+                first = b(x)
+            with torch.cuda.stream(two):
+                second = b(x)
+                b.eval()  # drops what stream two still reads
+                third = b(x)
+            torch.cuda.synchronize()
+            for y in (first, second, third):
+                assert torch.equal(y, want)
+
+
+def test_block_quantized_copies_by_pickle():
+    torch.manual_seed(5)
+    b = LaplacianBlock(64, heads=2, grid=8, device="cuda").quantize_()
+    x = torch.randn(2, 64, 64, device="cuda").bfloat16()
+    with torch.no_grad():
+        want = b(x)
+        f = io.BytesIO()
+        torch.save(b, f)
+        f.seek(0)
+        c = torch.load(f, weights_only=False)
+        assert c.quantized and torch.equal(c(x), want)
+        c.w_qkv.neg_()
+        assert torch.equal(c(x), eight_bit(c, x))
