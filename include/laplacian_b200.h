@@ -461,6 +461,121 @@ LF_API int lf_clip_grad_norm(const void* const* grads, void* const* outs, const 
                              int64_t count, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
                              lf_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+   Causal operators: attention and positions of a block that reads its tokens
+   in order, and the norms around a sublayer.  The reference has none of them.
+   ------------------------------------------------------------------------- */
+
+/* Causal linear attention with a decay l = exp(log_decay[h]) per head:
+     S_t = l S_(t-1) + k_t v_t^T,   o_t = scale q_t S_t,   S_(-1) = state (NULL: 0)
+   q, k, v, d_o: heads of key_size or value_size (up to 128) contiguous elements
+   of F16 or BF16, with strides in elements of sequences, heads and tokens.
+   o, dq, dk, dv are dense [b, t, h, size], states dense fp32 [b, h, key_size,
+   value_size].  log_decay: h floats, meant to be at most 0 (-inf: a token sees
+   itself alone).  lengths: NULL, or tokens of each sequence (taken as 0 to t):
+   later tokens are not read into any result, and their rows of the outputs are 0.
+   state_out (may be NULL): the state after the last token.
+   The backward takes d_o and (NULL: 0) d_state_out and writes the gradients that
+   are not NULL; d_state needs dv.  Scores (scale q k^T, and scale d_o v^T in the
+   backward) are operands of a second product in dtype: in fp16 they become
+   infinite beyond 65504.  A value that is not finite reaches all outputs of its
+   128-token chunk.  Workspaces are 256-byte aligned; their sizes depend on the
+   sizes, strides and pointers: ask with the struct that will run. */
+typedef struct lf_decay_attention {
+    const void *q, *k, *v;
+    const float *log_decay, *state;
+    const int64_t* lengths;
+    void* o;
+    float* state_out;
+    const void* d_o;
+    const float* d_state_out;
+    void *dq, *dk, *dv;
+    float* d_state;
+    int64_t q_strides[3], k_strides[3], v_strides[3], do_strides[3];
+    int64_t b, h, t, key_size, value_size;
+    double scale;
+    int32_t dtype;
+} lf_decay_attention_t;
+
+LF_API size_t lf_decay_attention_fwd_workspace_size(const lf_decay_attention_t* args);
+LF_API int lf_decay_attention_fwd(const lf_decay_attention_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+LF_API size_t lf_decay_attention_bwd_workspace_size(const lf_decay_attention_t* args);
+LF_API int lf_decay_attention_bwd(const lf_decay_attention_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
+/* The same for one token of each sequence: state (dense fp32 [b, h, key_size,
+   value_size]) is updated in place, o is dense [b, h, value_size].  F32, F16 or
+   BF16; strides in elements of sequences and heads. */
+typedef struct lf_decay_step {
+    const void *q, *k, *v;
+    const float* log_decay;
+    float* state;
+    void* o;
+    int64_t q_strides[2], k_strides[2], v_strides[2];
+    int64_t b, h, key_size, value_size;
+    double scale;
+    int32_t dtype;
+} lf_decay_step_t;
+
+LF_API int lf_decay_attention_step(const lf_decay_step_t* args, lf_stream_t stream);
+
+/* Rotary positions of up to two tensors of heads (queries and keys) in one
+   launch: pair i of a head turns by position * frequencies[i] (radians, at most
+   128 pairs; a host array, read before the call returns) and is scaled by
+   magnitude.  Pairs are channels (i, i + pairs), or (2i, 2i + 1) if interleaved; channels
+   from 2 pairs on are copied.  inverse: the opposite angle (the backward pass).
+   x[i]: heads[i] heads of `size` contiguous elements, strides in elements of
+   sequences, heads and tokens; y[i] dense [b, t, heads, size], which may be x[i]
+   where that is dense.  positions: int64, position_stride apart between
+   sequences (0: shared), or NULL: offset + token.  The angle is formed in 64
+   bits.  F32, F16 or BF16. */
+typedef struct lf_rotary {
+    const void* x[2];
+    void* y[2];
+    int64_t strides[2][3];
+    int64_t heads[2];
+    const int64_t* positions;
+    int64_t position_stride, offset;
+    const double* frequencies;
+    int64_t b, t, size, pairs;
+    double magnitude;
+    int32_t interleaved, inverse, dtype;
+} lf_rotary_t;
+
+LF_API int lf_rotary(const lf_rotary_t* args, lf_stream_t stream);
+
+/* Activations of a gate. */
+enum lf_gate {
+    LF_GATE_NONE = 0,
+    LF_GATE_SIGMOID = 1,
+    LF_GATE_SILU = 2,
+    LF_GATE_TANH = 3
+};
+
+/* The norms after a sublayer and before the next one, with the gate, the
+   residual scale and the residual's addition between them:
+     s = residual + scale act(gate) (x / sqrt(mean(x^2) + eps) weight),
+     y = s / sqrt(mean(s^2) + eps) next_weight.
+   Dense rows of `cols` elements, F32, F16 or BF16; y is computed from the
+   unrounded s.  gate: NULL (1), or rows / rows_per_gate rows of which each
+   serves rows_per_gate rows in turn.  next_weight and y: both NULL leave the
+   second norm out.  rstd: NULL, or 2 * rows floats kept for the backward.
+   The backward takes dy and ds (one of them may be NULL) and writes the gradients that are not
+   NULL.  Rows of a workspace: ask with the struct that will run; 16-byte aligned. */
+typedef struct lf_sandwich_norm {
+    const void *x, *weight, *residual, *gate, *next_weight;
+    void *s, *y;
+    float* rstd;
+    const void *dy, *ds;
+    void *dx, *d_weight, *d_residual, *d_gate, *d_next_weight;
+    int64_t rows, cols, rows_per_gate;
+    double scale, eps;
+    int32_t activation, dtype;
+} lf_sandwich_norm_t;
+
+LF_API int lf_sandwich_norm_fwd(const lf_sandwich_norm_t* args, lf_stream_t stream);
+LF_API size_t lf_sandwich_norm_bwd_workspace_size(const lf_sandwich_norm_t* args);
+LF_API int lf_sandwich_norm_bwd(const lf_sandwich_norm_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -46,7 +46,41 @@ class GatedFfn(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("activation", "dtype")])
 
 
+class DecayAttention(ctypes.Structure):
+    """lf_decay_attention_t: causal linear attention with a decay per head, and its gradients."""
+
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "log_decay", "state", "lengths", "o", "state_out", "d_o", "d_state_out", "dq", "dk",
+                                   "dv", "d_state")]
+                + [(n, _I64 * 3) for n in ("q_strides", "k_strides", "v_strides", "do_strides")]
+                + [(n, _I64) for n in ("b", "h", "t", "key_size", "value_size")] + [("scale", _D), ("dtype", ctypes.c_int32)])
+
+
+class DecayStep(ctypes.Structure):
+    """lf_decay_step_t: one token of it."""
+
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "log_decay", "state", "o")] + [(n, _I64 * 2) for n in ("q_strides", "k_strides", "v_strides")]
+                + [(n, _I64) for n in ("b", "h", "key_size", "value_size")] + [("scale", _D), ("dtype", ctypes.c_int32)])
+
+
+class Rotary(ctypes.Structure):
+    """lf_rotary_t: rotary positions of queries and keys."""
+
+    _fields_ = ([("x", _P * 2), ("y", _P * 2), ("strides", (_I64 * 3) * 2), ("heads", _I64 * 2), ("positions", _P), ("position_stride", _I64),
+                 ("offset", _I64), ("frequencies", ctypes.POINTER(_D))] + [(n, _I64) for n in ("b", "t", "size", "pairs")]
+                + [("magnitude", _D)] + [(n, ctypes.c_int32) for n in ("interleaved", "inverse", "dtype")])
+
+
+class SandwichNorm(ctypes.Structure):
+    """lf_sandwich_norm_t: the norms around a sublayer, its gate and residual scale, and their gradients."""
+
+    _fields_ = ([(n, _P) for n in ("x", "weight", "residual", "gate", "next_weight", "s", "y", "rstd", "dy", "ds", "dx", "d_weight",
+                                   "d_residual", "d_gate", "d_next_weight")]
+                + [(n, _I64) for n in ("rows", "cols", "rows_per_gate")] + [("scale", _D), ("eps", _D)]
+                + [(n, ctypes.c_int32) for n in ("activation", "dtype")])
+
+
 _LIN, _FFN, _SZ = ctypes.POINTER(Linear), ctypes.POINTER(GatedFfn), ctypes.c_size_t
+_DEC, _STEP, _ROT, _SAN = (ctypes.POINTER(t) for t in (DecayAttention, DecayStep, Rotary, SandwichNorm))
 
 # name -> (restype, argtypes); the exported symbol set of include/laplacian_b200.h
 SIGNATURES = {
@@ -100,6 +134,15 @@ SIGNATURES = {
     "lf_gated_ffn_bwd": (_I, [_FFN, _P, _SZ, _P]),
     "lf_clip_grad_norm_workspace_size": (_SZ, [_P, _I64]),
     "lf_clip_grad_norm": (_I, [_P, _P, _P, _P, _I64, _D, _P, _P, _SZ, _P]),
+    "lf_decay_attention_fwd_workspace_size": (_SZ, [_DEC]),
+    "lf_decay_attention_fwd": (_I, [_DEC, _P, _SZ, _P]),
+    "lf_decay_attention_bwd_workspace_size": (_SZ, [_DEC]),
+    "lf_decay_attention_bwd": (_I, [_DEC, _P, _SZ, _P]),
+    "lf_decay_attention_step": (_I, [_STEP, _P]),
+    "lf_rotary": (_I, [_ROT, _P]),
+    "lf_sandwich_norm_fwd": (_I, [_SAN, _P]),
+    "lf_sandwich_norm_bwd_workspace_size": (_SZ, [_SAN]),
+    "lf_sandwich_norm_bwd": (_I, [_SAN, _P, _SZ, _P]),
 }
 
 LF_MAX_PEERS = 8

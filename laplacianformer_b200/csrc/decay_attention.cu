@@ -1,0 +1,914 @@
+// Causal linear attention with a decay per head, its backward pass, and its
+// form for single tokens.
+//
+//   S_t = l S_(t-1) + k_t v_t^T,   o_t = sigma q_t S_t,   l = exp(log_decay[h])
+//
+// Prompts and training go by chunks of 128 tokens.  Within a chunk, with G the
+// state decayed to the chunk's first token (l S before it):
+//   o_i = sigma [ sum_(j<=i) l^(i-j) (q_i . k_j) v_j + l^i q_i G ]
+//   G'  = l^n G + sum_j l^(n-j) k_j v_j^T            (n tokens, j from 0)
+// The gradients are the same recurrence with other operands, so one kernel
+// makes all four (out = mix(a, b, c)):
+//   o  = mix(q, k, v)    dq = mix(do, v, k)          forwards in time
+//   dk = mix(v, do, q)   dv = mix(k, q, do)          backwards
+// and the gradient of the first state is the last dv state.
+//
+// Every power of l is taken of a difference of positions and is at most 1 for
+// a decay: nothing is divided by a small power.  Sums and states are fp32.
+// Rounded to 16 bits as operands of products, besides the inputs: the weighted
+// scores (once), the state that q meets (once; fp16: scaled by a power of two
+// into its range), and l^(n-j) b_j, which goes in as two 16-bit parts so that
+// the state keeps about 17 bits (bf16) or 22 (fp16) of each term.
+#include <algorithm>
+
+#include "tc_ptx.cuh"
+#include "tma_map.h"
+
+namespace lfb {
+
+// Set by a kernel whose bounded wait expired (merged into lf_device_status).
+__device__ int g_decay_status = 0;
+
+int decay_status(bool clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_decay_status, sizeof(int)) != cudaSuccess) return LF_ERR_CUDA;
+    if (clear) {
+        int z = 0;
+        if (cudaMemcpyToSymbol(g_decay_status, &z, sizeof(int)) != cudaSuccess) return LF_ERR_CUDA;
+    }
+    return v;
+}
+
+namespace {
+
+constexpr int kChunk = 128;           // tokens per chunk: rows of a product's tile
+constexpr int kRing = 5;              // operand tiles in flight: the chunk's three and the next one's first two
+constexpr int kEpi = 256;             // threads that turn accumulators into operands and outputs
+constexpr int kThreads = kEpi + 64;   // and a warp for copies, a warp for products
+constexpr int kBlock = kChunk * 128;  // bytes of 128 rows of 64 columns
+
+struct alignas(64) MixArgs {
+    CUtensorMap a, b, c, out;
+    const float* log_decay;
+    const float* g0;         // state before the first token (to be decayed by l), or with `rev` the gradient of the last state
+    float* gout;             // state after the last token, or with `rev` the gradient of the first state
+    float* ends;             // [bh][nseg][64W][64W]: what each segment adds to the state
+    const int64_t* lengths;  // tokens per sequence, or null
+    void* o;                 // rows of dc elements, where TMA cannot write them
+    int64_t o_sb, o_sh, o_st;
+    int heads, t, da, dc, chunks, nseg, per_seg, items;
+    int g0_row, g0_col;      // strides within a state matrix (transposed for dq and dk)
+    float scale, g0_scale, gout_scale;
+    int ksteps, nb;          // 16-column steps of da; dc rounded up to 16
+    uint32_t id_qk, id_qg, id_pv, id_kv;
+    int tma_out;
+};
+
+template <int W>
+constexpr int mix_smem() {
+    // ring, low parts (then the output's staging), state operand, tables, barriers
+    return 1024 + (kRing + 1) * W * kBlock + 64 * W * 128 * W + 1024 + 256;
+}
+
+__device__ __forceinline__ void load4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int h, int t, int b) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(h), "r"(t), "r"(b)
+                 : "memory");
+}
+__device__ __forceinline__ void store4d(const CUtensorMap* map, const void* src, int x, int h, int t, int b) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+                 "r"(smem_u32(src)), "r"(x), "r"(h), "r"(t), "r"(b)
+                 : "memory");
+}
+__device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Barrier of the epilogue's threads; whether `ok` holds for all of them, so that they leave together.
+__device__ __forceinline__ bool epi_sync(bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+        : "=r"(r)
+        : "r"((uint32_t)ok), "n"(kEpi)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void sts16(uint8_t* p, uint4 v) { *reinterpret_cast<uint4*>(p) = v; }
+
+// l^n; 1 for n = 0 whatever l is.
+__device__ __forceinline__ float power(float g, int64_t n) { return n == 0 ? 1.f : expf((float)n * g); }
+
+struct Item {
+    int bh, b, h, seg, first, n, active;
+    int64_t len;
+};
+template <bool REV, bool ENDS>
+__device__ __forceinline__ Item item_of(const MixArgs& p, int i) {
+    Item t;
+    const int segs = ENDS ? p.nseg - 1 : p.nseg;  // nobody follows the last segment
+    t.bh = i / segs;
+    t.seg = i - t.bh * segs + (ENDS && REV ? 1 : 0);
+    t.b = t.bh / p.heads;
+    t.h = t.bh - t.b * p.heads;
+    t.len = p.t;
+    if (p.lengths) {
+        const int64_t n = p.lengths[t.b];
+        t.len = n < 0 ? 0 : n < p.t ? n : p.t;
+    }
+    t.active = (int)((t.len + kChunk - 1) / kChunk);
+    t.first = t.seg * p.per_seg;
+    const int last = min(min(t.first + p.per_seg, p.chunks), t.active);
+    t.n = max(0, last - t.first);
+    return t;
+}
+
+// Power of two that takes mx into [2^14, 2^15); 1 for 0 and for what is not finite.
+__device__ __forceinline__ float range_scale(uint32_t bits) {
+    const int e = (int)(bits >> 23);
+    if (bits == 0 || e == 0xff) return 1.f;
+    return __uint_as_float((uint32_t)max(1, min(127 + 141 - e, 254)) << 23);
+}
+
+// W: 64-column blocks per operand row (head sizes up to 64 W).  REV: backwards
+// in time.  ENDS: only what a segment adds to the state.
+template <typename T, int W, bool REV, bool ENDS>
+__global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(const __grid_constant__ MixArgs p) {
+    constexpr int kTile = W * kBlock, kState = 64 * W;                        // state rows
+    constexpr int kO = 128, kKv = 128 + 64 * W, kCols = W == 1 ? 256 : 512;   // tensor memory columns; scores from 0 on
+    constexpr bool F16 = std::is_same<T, __half>::value;
+    extern __shared__ uint8_t raw[];
+    uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const low = ring + kRing * kTile;
+    uint8_t* const gop = low + kTile;                                         // [state row][dc], 64 columns a block
+    float* const pw = reinterpret_cast<float*>(gop + kState * 128 * W);       // l^n, n = 0..128
+    float* const back = pw + 132;                                             // l^(31-n)
+    uint32_t* const gmax = reinterpret_cast<uint32_t*>(back + 32);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 256);
+    uint64_t *full = bars, *empty = bars + kRing, *s_full = bars + 2 * kRing, *k_ready = s_full + 1, *p_ready = s_full + 2,
+             *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7;
+    uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 8);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    grid_release();
+    if (tid == 0) {
+        for (int i = 0; i < kRing; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        mbar_init(s_full, 1), mbar_init(kv_full, 1), mbar_init(o_full, 1), mbar_init(qg_full, 1), mbar_init(drain, 1);
+        mbar_init(k_ready, kEpi), mbar_init(p_ready, kEpi), mbar_init(g_ready, kEpi);
+        gmax[0] = gmax[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) tmem_alloc(tmem_ptr, kCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_wait();
+    const uint32_t tmem = *tmem_ptr;
+    constexpr int kTiles = ENDS ? 2 : 3;
+    bool ok = true;
+
+    if (warp == 8) {  // copies
+        if (elect_one()) {
+            int n = 0;
+            for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
+                const Item t = item_of<REV, ENDS>(p, i);
+                for (int k = 0; ok && k < t.n; ++k) {
+                    const int t0 = (REV ? t.first + t.n - 1 - k : t.first + k) * kChunk;
+                    for (int j = 3 - kTiles; j < 3; ++j) {
+                        const int s = n % kRing;
+                        if (!(ok = mbar_wait(&empty[s], (n / kRing & 1) ^ 1))) break;
+                        expect(&full[s], kTile);
+                        const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
+                        for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
+                        ++n;
+                    }
+                }
+            }
+            if (!ok)  // a wait ran out: let the copies in flight land
+                for (int k = max(0, n - kRing); k < n; ++k) mbar_wait(&full[k % kRing], k / kRing & 1, 100000000ull);
+        }
+        __syncwarp();
+    } else if (warp == 9) {  // products
+        const uint32_t go = elect_one() ? 1u : 0u;
+        int n = 0, cc = 0;
+        for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
+            const Item t = item_of<REV, ENDS>(p, i);
+            for (int k = 0; k < t.n; ++k, ++cc, n += kTiles) {
+                const int na = n, nk = n + kTiles - 2, nv = nk + 1;
+                const uint32_t sk = smem_u32(ring + nk % kRing * kTile), sv = smem_u32(ring + nv % kRing * kTile);
+                if (!(ok = mbar_wait(&full[nk % kRing], nk / kRing & 1))) break;
+                bool has_g = false;
+                if constexpr (!ENDS) {
+                    const int first = REV ? (t.active - 1) / p.per_seg : 0;  // the segment that the sequence starts with
+                    has_g = k > 0 || p.g0 || t.seg != first;
+                    const uint32_t sa = smem_u32(ring + na % kRing * kTile);
+                    if (!(ok = mbar_wait(&full[na % kRing], na / kRing & 1))) break;
+                    if (cc > 0 && !(ok = mbar_wait(o_full, (cc - 1) & 1))) break;  // the scores' columns hold its operand
+                    tc_fence_after();
+                    const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sk, 16, 1024);
+                    for (int s = 0; s < p.ksteps; ++s) {
+                        const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
+                        mma_f16(tmem, da + at, db + at, p.id_qk, s > 0 ? 1u : 0u, go);
+                    }
+                    if (go) mma_commit(s_full);
+                    if (!(ok = mbar_wait(g_ready, cc & 1))) break;
+                    tc_fence_after();
+                    if (has_g) {
+                        const uint64_t dg = make_desc(smem_u32(gop), kState * 128, 1024);
+                        for (int s = 0; s < p.ksteps; ++s) {
+                            const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
+                            mma_f16(tmem + kO, da + at, dg + (uint64_t)(s * 128), p.id_qg, s > 0 ? 1u : 0u, go);
+                        }
+                        if (go) mma_commit(qg_full);
+                    }
+                    if (go) mma_commit(&empty[na % kRing]);
+                }
+                if (!(ok = mbar_wait(k_ready, cc & 1) && mbar_wait(&full[nv % kRing], nv / kRing & 1))) break;
+                tc_fence_after();
+                {
+                    const uint64_t dh = make_desc(sk, kBlock, 1024), dl = make_desc(smem_u32(low), kBlock, 1024);
+                    const uint64_t dv = make_desc(sv, kBlock, 1024);
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, s > 0 ? 1u : 0u, go);
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, 1u, go);
+                    if (go) mma_commit(kv_full), mma_commit(&empty[nk % kRing]);
+                    if constexpr (!ENDS) {
+                        if (!(ok = mbar_wait(p_ready, cc & 1))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int s = 0; s < 8; ++s)  // scores of columns 64 on lie 64 columns further
+                            mma_f16_ts(tmem + kO, tmem + (s >> 2) * 64 + (s & 3) * 8, dv + (uint64_t)(s * 128), p.id_pv, has_g || s > 0 ? 1u : 0u, go);
+                        if (go) mma_commit(o_full);
+                    }
+                    if (go) mma_commit(&empty[nv % kRing]);
+                }
+            }
+        }
+        if (!ok) {  // products in flight end before the tensor memory is freed
+            if (go) mma_commit(drain);
+            mbar_wait(drain, 0, 100000000ull);
+        }
+        __syncwarp();
+    } else {
+        const int quad = warp & 3, half = warp >> 2;
+        const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16);
+        const int row = quad * 32 + lane;                         // of a chunk
+        // The state: the accumulators of 64 rows are 16 in each quarter of the lanes.
+        const int srow = W == 1 ? quad * 16 + lane : row;
+        const bool live = W == 2 || lane < 16;
+        const int col0 = half * 32 * W;                           // this thread's columns of the state and of the output
+        float G[32 * W];
+        int n = 0, cc = 0, qg = 0, puts = 0;
+        for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
+            const Item t = item_of<REV, ENDS>(p, i);
+            const float g = p.log_decay[t.h];
+            epi_sync(true);  // the tables' last readers are done
+            if (tid <= kChunk) pw[tid] = power(g, tid);
+            if (tid < 32) back[tid] = power(g, 31 - tid);
+            const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
+            bool has_g = !ENDS && (p.g0 || (t.n > 0 && t.seg != first_seg));
+            // ---- the state before this segment
+#pragma unroll
+            for (int j = 0; j < 32 * W; ++j) G[j] = 0.f;
+            if (!ENDS && has_g && live) {
+                if (p.g0 && srow < p.da) {
+                    // tokens that come before, and one step more into the chunk's terms
+                    const int64_t before = REV ? t.len - min(t.len, (int64_t)(t.first + t.n) * kChunk) : (int64_t)t.first * kChunk;
+                    const float w = (t.n > 0 ? power(g, before) * (REV ? 1.f : power(g, 1)) : 1.f) * p.g0_scale;
+                    const float* src = p.g0 + (int64_t)t.bh * p.da * p.dc + (int64_t)srow * p.g0_row;
+#pragma unroll
+                    for (int j = 0; j < 32 * W; ++j)
+                        if (col0 + j < p.dc) G[j] = w * src[(int64_t)(col0 + j) * p.g0_col];
+                }
+                if (t.n > 0)
+                    for (int u = REV ? t.seg + 1 : 0; REV ? u <= first_seg : u < t.seg; ++u) {
+                        const float w = power(g, (int64_t)((REV ? u - t.seg : t.seg - u) - 1) * p.per_seg * kChunk);
+                        const float4* e = reinterpret_cast<const float4*>(p.ends + (((int64_t)t.bh * p.nseg + u) * kState + srow) * kState + col0);
+#pragma unroll
+                        for (int j = 0; j < 8 * W; ++j) {
+                            const float4 v = e[j];
+                            G[4 * j] = __fmaf_rn(w, v.x, G[4 * j]), G[4 * j + 1] = __fmaf_rn(w, v.y, G[4 * j + 1]);
+                            G[4 * j + 2] = __fmaf_rn(w, v.z, G[4 * j + 2]), G[4 * j + 3] = __fmaf_rn(w, v.w, G[4 * j + 3]);
+                        }
+                    }
+            }
+            float unscale = 1.f;
+            // G as an operand: rows of dc columns, in fp16 times a power of two that keeps the largest in range.
+            auto put_state = [&] {
+                float s = 1.f;
+                if constexpr (F16) {
+                    float m = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32 * W; ++j) m = fmaxf(m, fabsf(G[j]));
+                    const uint32_t wm = __reduce_max_sync(0xffffffffu, live ? __float_as_uint(m) : 0u);
+                    const int slot = puts++ & 1;
+                    if (lane == 0) atomicMax(&gmax[slot], wm);
+                    epi_sync(true);
+                    s = range_scale(gmax[slot]);
+                    if (tid == 0) gmax[slot ^ 1] = 0;
+                    unscale = 1.f / s;
+                }
+                if (live) {
+                    uint8_t* const dst = gop + (W == 2 ? half * kState * 128 : 0) + srow * 128;
+#pragma unroll
+                    for (int j = 0; j < 4 * W; ++j) {
+                        const float* v = &G[8 * j];
+                        const int ch = (W == 1 ? half * 4 : 0) + j;
+                        sts16(dst + ((ch ^ (srow & 7)) << 4), make_uint4(pack2<T>(v[0] * s, v[1] * s), pack2<T>(v[2] * s, v[3] * s),
+                                                                        pack2<T>(v[4] * s, v[5] * s), pack2<T>(v[6] * s, v[7] * s)));
+                    }
+                }
+                fence_async_smem();
+            };
+            if constexpr (!ENDS) {
+                if (t.n > 0) {
+                    if (has_g) put_state();
+                    arrive(g_ready);
+                }
+            }
+            epi_sync(true);  // the tables are written
+            // ---- chunks
+            for (int k = 0; k < t.n; ++k, ++cc, n += kTiles) {
+                const int chunk = REV ? t.first + t.n - 1 - k : t.first + k;
+                const int L = (int)min((int64_t)kChunk, t.len - (int64_t)chunk * kChunk);
+                const int nk = n + kTiles - 2, nv = nk + 1;
+                uint8_t* const tk = ring + nk % kRing * kTile;
+                // The last state is that after the last token, not decayed further.
+                const int e = !REV && !ENDS && p.gout && chunk == t.active - 1 ? 1 : 0;
+                ok = mbar_wait(&full[nk % kRing], nk / kRing & 1) && ok;
+                if constexpr (!ENDS) {
+                    ok = mbar_wait(s_full, cc & 1) && ok;  // the scores are done: b may be overwritten
+                    if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    if (!(ok = epi_sync(ok))) break;  // and the last output has left the staging
+                }
+                tc_fence_after();
+                {  // b_j times its power of l, in two parts
+                    const int r = tid >> 1, part = tid & 1;
+                    const float w = r >= L ? 0.f : REV ? pw[r + 1] : pw[L - e - r];
+                    uint8_t *hi = tk, *lo = low;
+                    if (W == 2) hi += part * kBlock, lo += part * kBlock;
+                    hi += r * 128, lo += r * 128;
+#pragma unroll
+                    for (int j = 0; j < 4 * W; ++j) {
+                        const int ch = W == 1 ? part * 4 + j : j ^ (part << 2), at = (ch ^ (r & 7)) << 4;
+                        uint4 v = *reinterpret_cast<const uint4*>(hi + at), l;
+                        uint32_t *x = reinterpret_cast<uint32_t*>(&v), *y = reinterpret_cast<uint32_t*>(&l);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            float2 f = unpack2<T>(x[q]);
+                            f.x *= w, f.y *= w;
+                            x[q] = pack2<T>(f.x, f.y);
+                            const float2 h = unpack2<T>(x[q]);
+                            y[q] = pack2<T>(f.x - h.x, f.y - h.y);
+                        }
+                        if (r >= L) v = l = make_uint4(0u, 0u, 0u, 0u);
+                        sts16(hi + at, v);
+                        sts16(lo + at, l);
+                    }
+                }
+                if (L < kChunk) {  // rows past the sequence: zeros, whatever they hold
+                    ok = mbar_wait(&full[nv % kRing], nv / kRing & 1) && ok;
+                    uint8_t* const tv = ring + nv % kRing * kTile;
+                    for (int j = tid; j < (kChunk - L) * 8 * W; j += kEpi) {
+                        const int r = L + j / (8 * W), u = j % (8 * W);
+                        sts16(tv + (u >> 3) * kBlock + r * 128 + ((u & 7) << 4), make_uint4(0u, 0u, 0u, 0u));
+                    }
+                }
+                fence_async_smem();
+                arrive(k_ready);
+                if constexpr (!ENDS) {
+                    // ---- weighted scores: row `row`, columns 64 half on, in blocks of 32
+#pragma unroll
+                    for (int bl = 0; bl < 2; ++bl) {
+                        const int blk = half * 2 + bl;
+                        uint32_t u[16];
+                        if (REV ? blk < quad : blk > quad) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) u[j] = 0u;
+                        } else {
+                            float v[32];
+                            tmem_ld32(tq + blk * 32, v);
+                            tmem_wait_ld();
+                            reg_fence(v);
+                            if (blk == quad) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    const int d = REV ? j - lane : lane - j;
+                                    v[j] = d >= 0 ? v[j] * (pw[max(d, 0)] * p.scale) : 0.f;
+                                }
+                            } else {
+                                const float rf = pw[REV ? blk * 32 - row : row - blk * 32 - 31] * p.scale;
+                                const uint64_t rf2 = pk2(rf, rf);
+                                const float4* cf = reinterpret_cast<const float4*>(REV ? pw : back);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const float4 f = cf[j];
+                                    upk2(mul2(mul2(pk2(v[4 * j], v[4 * j + 1]), rf2), pk2(f.x, f.y)), v[4 * j], v[4 * j + 1]);
+                                    upk2(mul2(mul2(pk2(v[4 * j + 2], v[4 * j + 3]), rf2), pk2(f.z, f.w)), v[4 * j + 2], v[4 * j + 3]);
+                                }
+                            }
+                            if (REV && L < kChunk) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = blk * 32 + j < L ? v[j] : 0.f;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) u[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+                        }
+                        tmem_st16(tq + half * 64 + bl * 16, u);
+                    }
+                    if (has_g) {  // what the state gives, times the row's power
+                        ok = mbar_wait(qg_full, qg++ & 1) && ok;
+                        tc_fence_after();
+                        const int d = REV ? L - 1 - row : row;
+                        const float w = (d >= 0 ? pw[d] : 0.f) * p.scale * unscale;
+#pragma unroll
+                        for (int c = 0; c < 2 * W; ++c) {
+                            if (col0 + 16 * c < p.nb) {
+                                float v[16];
+                                tmem_ld16(tq + kO + col0 + 16 * c, v);
+                                tmem_wait_ld();
+                                reg_fence(v);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) v[j] *= w;
+                                tmem_st16(tq + kO + col0 + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v));
+                            }
+                        }
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    arrive(p_ready);
+                }
+                // ---- the state after this chunk
+                ok = mbar_wait(kv_full, cc & 1) && ok;
+                tc_fence_after();
+                {
+                    const float w = pw[L - e];
+#pragma unroll
+                    for (int c = 0; c < 2 * W; ++c) {
+                        if (col0 + 16 * c < p.nb) {
+                            float v[16];
+                            tmem_ld16(tq + kKv + col0 + 16 * c, v);
+                            tmem_wait_ld();
+                            reg_fence(v);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) G[16 * c + j] = __fmaf_rn(G[16 * c + j], w, v[j]);
+                        }
+                    }
+                }
+                has_g = true;
+                if constexpr (ENDS) {
+                    tc_fence_before();
+                    if (!(ok = epi_sync(ok))) break;  // low may be written again, and the accumulator
+                    continue;
+                }
+                if (k + 1 < t.n) put_state();
+                // ---- the output
+                ok = mbar_wait(o_full, cc & 1) && ok;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 2 * W; ++c) {
+                    if (col0 + 16 * c < p.nb) {
+                        float v[16];
+                        tmem_ld16(tq + kO + col0 + 16 * c, v);
+                        tmem_wait_ld();
+                        reg_fence(v);
+                        uint4 o[2];
+                        uint32_t* u = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) u[j] = row < L ? pack2<T>(v[2 * j], v[2 * j + 1]) : 0u;
+                        const int ch = (W == 1 ? half * 4 : 0) + 2 * c;
+                        uint8_t* const dst = low + (W == 2 ? half * kBlock : 0) + row * 128;
+                        sts16(dst + ((ch ^ (row & 7)) << 4), o[0]);
+                        sts16(dst + (((ch + 1) ^ (row & 7)) << 4), o[1]);
+                    }
+                }
+                tc_fence_before();
+                if (k + 1 < t.n) arrive(g_ready);  // the state operand is written and the output's columns are read
+                fence_async_smem();
+                if (!(ok = epi_sync(ok))) break;
+                if (p.tma_out) {
+                    if (tid == 0) {
+                        for (int w = 0; w < W; ++w)
+                            if (w * 64 < p.dc) store4d(&p.out, low + w * kBlock, w * 64, t.h, chunk * kChunk, t.b);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                } else {
+                    T* const o = (T*)p.o + t.b * p.o_sb + t.h * p.o_sh + (int64_t)chunk * kChunk * p.o_st;
+                    const int rows = min(kChunk, p.t - chunk * kChunk);
+                    for (int r = warp; r < rows; r += kEpi / 32)
+                        for (int c = lane; c < p.dc; c += 32)
+                            o[r * p.o_st + c] = *reinterpret_cast<const T*>(low + (c >> 6) * kBlock + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2);
+                }
+            }
+            if (!ok) break;
+            if constexpr (ENDS) {
+                if (t.n > 0 && live) {
+                    float4* e = reinterpret_cast<float4*>(p.ends + (((int64_t)t.bh * p.nseg + t.seg) * kState + srow) * kState + col0);
+#pragma unroll
+                    for (int j = 0; j < 8 * W; ++j) e[j] = make_float4(G[4 * j], G[4 * j + 1], G[4 * j + 2], G[4 * j + 3]);
+                }
+            } else {
+                // ---- rows past the sequence in this segment's whole chunks
+                const int end = min(t.first + p.per_seg, p.chunks);
+                const int64_t z0 = (int64_t)max(t.first + t.n, t.first) * kChunk, z1 = min((int64_t)end * kChunk, (int64_t)p.t);
+                T* const o = (T*)p.o + t.b * p.o_sb + t.h * p.o_sh;
+                for (int64_t r = z0 + warp; r < z1; r += kEpi / 32)
+                    for (int c = lane; c < p.dc; c += 32) o[r * p.o_st + c] = Elem<T>::store(0.f);
+                // ---- the state at the end, from the segment that got there (without tokens: as it was)
+                const bool mine = t.active == 0 ? t.seg == 0 : REV ? t.seg == 0 : t.n > 0 && t.first + t.n == t.active;
+                if (p.gout && mine && live && srow < p.da) {
+                    float* const dst = p.gout + (int64_t)t.bh * p.da * p.dc + (int64_t)srow * p.dc;
+#pragma unroll
+                    for (int j = 0; j < 32 * W; ++j)
+                        if (col0 + j < p.dc) dst[col0 + j] = G[j] * p.gout_scale;
+                }
+            }
+        }
+        if (!ENDS && tid == 0 && p.tma_out) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    if (!ok) atomicExch(&g_decay_status, (int)LF_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, kCols);
+}
+
+// Copies heads that TMA cannot address to [b][t][h][dp], dp a multiple of 8: 16 bytes of output per thread.
+struct PackArgs {
+    const uint16_t* in;
+    uint16_t* out;
+    int64_t sb, sh, st, rows;
+    int heads, t, d, dp;
+};
+__global__ void __launch_bounds__(256) pack_heads_kernel(const PackArgs p) {
+    grid_release();
+    grid_wait();
+    const int per = p.dp / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.rows * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per, bt = r / p.heads, b = bt / p.t;
+        const int c = (int)(i - r * per) * 8;
+        const uint16_t* src = p.in + b * p.sb + (r - bt * p.heads) * p.sh + (bt - b * p.t) * p.st;
+        uint16_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < p.d ? src[c + j] : (uint16_t)0;
+        *reinterpret_cast<uint4*>(p.out + i * 8) = *reinterpret_cast<const uint4*>(v);
+    }
+}
+
+// One token: S = l S + k v^T in place, o = sigma q S.  A block per head: the
+// threads cover rows of dv columns (VEC each), so the state is read and written
+// once, coalesced, and each thread sums q S over the rows it holds; the row
+// groups' sums join in order.
+struct StepArgs {
+    const void *q, *k, *v;
+    const float* log_decay;
+    float* state;
+    void* o;
+    int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
+    int heads, dk, dv, tx;
+    float scale;
+};
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) decay_step_kernel(const StepArgs p) {
+    __shared__ float sum[256 * VEC], qk[2][128];
+    grid_release();
+    grid_wait();
+    const int64_t bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads;
+    const int c = (threadIdx.x % p.tx) * VEC, rg = threadIdx.x / p.tx, groups = 256 / p.tx;
+    const T *q = (const T*)p.q + b * p.q_sb + h * p.q_sh, *k = (const T*)p.k + b * p.k_sb + h * p.k_sh;
+    const T* v = (const T*)p.v + b * p.v_sb + h * p.v_sh;
+    float* S = p.state + bh * p.dk * p.dv + c;
+    const bool in = c < p.dv;
+    float x[4][VEC], vv[VEC], acc[VEC];
+    // The first rows are on their way while the small operands come.
+    auto fetch = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + i * groups;
+            if (in && r < p.dk) {
+                if constexpr (VEC == 4) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(S + r * p.dv);
+                else x[i][0] = S[r * p.dv];
+            }
+        }
+    };
+    fetch(rg);
+    const float l = expf(p.log_decay[h]);
+    if (threadIdx.x < p.dk) qk[0][threadIdx.x] = Elem<T>::load(q[threadIdx.x]) * p.scale;
+    else if (threadIdx.x >= 128 && threadIdx.x - 128 < p.dk) qk[1][threadIdx.x - 128] = Elem<T>::load(k[threadIdx.x - 128]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) vv[j] = in ? Elem<T>::load(v[c + j]) : 0.f, acc[j] = 0.f;
+    __syncthreads();
+    for (int r0 = rg; r0 < p.dk; r0 += 4 * groups) {
+        if (r0 != rg) fetch(r0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + i * groups;
+            if (in && r < p.dk) {
+                const float kr = qk[1][r], qr = qk[0][r];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    x[i][j] = __fmaf_rn(x[i][j], l, kr * vv[j]);
+                    acc[j] = __fmaf_rn(qr, x[i][j], acc[j]);
+                }
+                if constexpr (VEC == 4) *reinterpret_cast<float4*>(S + r * p.dv) = *reinterpret_cast<const float4*>(x[i]);
+                else S[r * p.dv] = x[i][0];
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[threadIdx.x * VEC + j] = acc[j];
+    __syncthreads();
+    if (threadIdx.x < p.dv) {
+        float t = 0.f;
+        for (int i = 0; i < groups; ++i) t += sum[i * p.tx * VEC + threadIdx.x];
+        ((T*)p.o)[bh * p.dv + threadIdx.x] = Elem<T>::store(t);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+// Heads of d elements: strides of sequences, heads and tokens in elements.
+struct Heads {
+    const void* p;
+    int64_t sb, sh, st, d;
+};
+struct Sizes {
+    int64_t b, h, t;
+};
+
+bool tma_heads(const Heads& x, const Sizes& z) {
+    const int64_t n[3] = {z.b, z.h, z.t}, s[3] = {x.sb, x.sh, x.st};
+    if (!aligned(x.p, 16)) return false;
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 != 0 || s[i] >= (int64_t)1 << 38)) return false;
+    return true;
+}
+int64_t padded(int64_t d) { return (d + 7) / 8 * 8; }
+size_t packed_bytes(const Heads& x, const Sizes& z) {
+    return tma_heads(x, z) ? 0 : (size_t)(z.b * z.h * z.t * padded(x.d) * 2 + 255) / 256 * 256;
+}
+
+// x itself, or a copy at `at` (moved on) that TMA can read.
+Heads addressable(const Heads& x, const Sizes& z, uint8_t*& at, cudaStream_t st) {
+    if (tma_heads(x, z)) return x;
+    const int64_t dp = padded(x.d), rows = z.b * z.h * z.t;
+    PackArgs a{(const uint16_t*)x.p, (uint16_t*)at, x.sb, x.sh, x.st, rows, (int)z.h, (int)z.t, (int)x.d, (int)dp};
+    const int64_t blocks = std::min<int64_t>((rows * (dp / 8) + 255) / 256, (int64_t)num_sms() * 8);
+    launch_early(pack_heads_kernel, (unsigned)blocks, 256, 0, 1, st, a);
+    Heads y{at, z.t * z.h * dp, dp, z.h * dp, x.d};
+    at += packed_bytes(x, z);
+    return y;
+}
+
+bool encode_heads(CUtensorMap* map, const Heads& x, const Sizes& z, int dtype) {
+    const cuuint64_t dims[4] = {(cuuint64_t)x.d, (cuuint64_t)z.h, (cuuint64_t)z.t, (cuuint64_t)z.b};
+    const cuuint64_t strides[3] = {(cuuint64_t)(z.h > 1 ? x.sh * 2 : 16), (cuuint64_t)(z.t > 1 ? x.st * 2 : 16),
+                                   (cuuint64_t)(z.b > 1 ? x.sb * 2 : 16)};
+    const cuuint32_t box[4] = {64, 1, kChunk, 1};
+    return encode_tiled(map, dtype == LF_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.p, dims,
+                        strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int blocks_of(int64_t da, int64_t dc) { return da <= 64 && dc <= 64 ? 1 : 2; }
+
+// Segments per sequence.
+int segments(const Sizes& z, int w) {
+    const int64_t chunks = (z.t + kChunk - 1) / kChunk, bh = z.b * z.h, slots = (int64_t)num_sms() * (w == 1 ? 2 : 1);
+    double least = 1e30;
+    int best = 1;
+    for (int64_t n = 1; n <= std::min<int64_t>(chunks, 64); ++n) {
+        const int64_t per = (chunks + n - 1) / n, segs = (chunks + per - 1) / per;
+        if (segs != n) continue;
+        const auto pass = [&](int64_t items, double chunk) { return (double)((items + slots - 1) / slots) * (per * chunk + 1.0); };
+        const double t = pass(bh * n, 1.0) + (n > 1 ? pass(bh * (n - 1), 0.5) + 2.0 : 0.0);
+        if (t < least) least = t, best = (int)n;
+    }
+    return best;
+}
+
+size_t ends_bytes(const Sizes& z, int w) {
+    const int n = segments(z, w);
+    return n > 1 ? (size_t)z.b * z.h * n * (64 * w) * (64 * w) * 4 : 0;
+}
+
+uint32_t idesc(int dtype, bool a_mn, bool b_mn, int m, int n) {
+    const uint32_t f = dtype == LF_BF16 ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
+}
+
+template <auto Kernel>
+void allow_smem(int bytes) {
+    static std::once_flag once[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::call_once(once[dev & 63], [&] { cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+}
+
+template <typename T, int W, bool REV, bool ENDS>
+void launch_mix(const MixArgs& a, cudaStream_t st) {
+    constexpr auto kernel = decay_mix_kernel<T, W, REV, ENDS>;
+    allow_smem<kernel>(mix_smem<W>());
+    const int grid = std::min(a.items, num_sms() * (W == 1 ? 2 : 1));
+    launch_early(kernel, (unsigned)grid, kThreads, mix_smem<W>(), 1, st, a);
+}
+
+struct Mix {
+    Heads a, b, c, out;
+    const float *g0 = nullptr;
+    float* gout = nullptr;
+    bool transposed = false;  // the state matrices are [dc][da]
+    bool rev = false;
+};
+
+int run_mix(const Mix& m, const Sizes& z, const float* log_decay, const int64_t* lengths, double scale, int dtype, float* ends,
+            cudaStream_t st) {
+    const int w = blocks_of(m.a.d, m.c.d);
+    MixArgs p{};
+    p.log_decay = log_decay, p.lengths = lengths, p.g0 = m.g0, p.gout = m.gout, p.ends = ends;
+    p.o = const_cast<void*>(m.out.p), p.o_sb = m.out.sb, p.o_sh = m.out.sh, p.o_st = m.out.st;
+    p.heads = (int)z.h, p.t = (int)z.t, p.da = (int)m.a.d, p.dc = (int)m.c.d;
+    p.chunks = (int)((z.t + kChunk - 1) / kChunk);
+    p.nseg = segments(z, w);
+    p.per_seg = (p.chunks + p.nseg - 1) / p.nseg;
+    p.g0_row = m.transposed ? 1 : p.dc, p.g0_col = m.transposed ? p.da : 1;
+    p.scale = (float)scale, p.g0_scale = m.rev ? (float)(1.0 / scale) : 1.f, p.gout_scale = m.rev ? (float)scale : 1.f;
+    p.ksteps = (p.da + 15) / 16, p.nb = (p.dc + 15) / 16 * 16;
+    p.id_qk = idesc(dtype, false, false, 128, 128), p.id_qg = idesc(dtype, false, true, 128, p.nb);
+    p.id_pv = p.id_qg, p.id_kv = idesc(dtype, true, true, 64 * w, p.nb);
+    p.tma_out = tma_heads(m.out, z) ? 1 : 0;
+    if (!encode_heads(&p.a, m.a, z, dtype) || !encode_heads(&p.b, m.b, z, dtype) || !encode_heads(&p.c, m.c, z, dtype)) return LF_ERR_CUDA;
+    if (p.tma_out && !encode_heads(&p.out, m.out, z, dtype)) return LF_ERR_CUDA;
+    const int64_t bh = z.b * z.h;
+#define LFB_MIX(T, W, REV)                                                                             {                                                                                                      if (p.nseg > 1) p.items = (int)(bh * (p.nseg - 1)), launch_mix<T, W, REV, true>(p, st);            p.items = (int)(bh * p.nseg), launch_mix<T, W, REV, false>(p, st);                             }
+    if (dtype == LF_F16) {
+        if (w == 1) { if (m.rev) LFB_MIX(__half, 1, true) else LFB_MIX(__half, 1, false) }
+        else { if (m.rev) LFB_MIX(__half, 2, true) else LFB_MIX(__half, 2, false) }
+    } else {
+        if (w == 1) { if (m.rev) LFB_MIX(__nv_bfloat16, 1, true) else LFB_MIX(__nv_bfloat16, 1, false) }
+        else { if (m.rev) LFB_MIX(__nv_bfloat16, 2, true) else LFB_MIX(__nv_bfloat16, 2, false) }
+    }
+#undef LFB_MIX
+    return check_launch("decay_attention");
+}
+
+int refuse(const char* what, const char* why) {
+    set_error("%s: %s", what, why);
+    return LF_ERR_INVALID;
+}
+
+int check_sizes(const char* what, int64_t b, int64_t h, int64_t t, int64_t dk, int64_t dv) {
+    if (b < 0 || h < 0 || t < 0 || dk < 1 || dv < 1) return refuse(what, "bad sizes");
+    if (dk > 128 || dv > 128) {
+        set_error("%s: head sizes up to 128 are supported, got %lld and %lld", what, (long long)dk, (long long)dv);
+        return LF_ERR_UNSUPPORTED;
+    }
+    // Work units and token numbers are 32-bit.
+    if (t > INT32_MAX - kChunk || (b > 0 && h > INT32_MAX / 64 / b)) {
+        set_error("%s: b*h up to 2^25 and t up to 2^31 - 129 are supported", what);
+        return LF_ERR_UNSUPPORTED;
+    }
+    return LF_OK;
+}
+
+int check_attention(const char* what, const lf_decay_attention_t* a, bool bwd) {
+    if (!a) return refuse(what, "no arguments");
+    if (a->dtype != LF_F16 && a->dtype != LF_BF16) {
+        set_error("%s: unsupported dtype code %d (fp16 and bf16)", what, a->dtype);
+        return LF_ERR_DTYPE;
+    }
+    if (int rc = check_sizes(what, a->b, a->h, a->t, a->key_size, a->value_size)) return rc;
+    if (!(a->scale > 0) || !(a->scale < 1e30) || a->scale < 1e-30) return refuse(what, "scale must be between 1e-30 and 1e30");
+    for (const void* p : {(const void*)a->q, (const void*)a->k, (const void*)a->v, (const void*)a->o, a->d_o, (const void*)a->dq,
+                          (const void*)a->dk, (const void*)a->dv})
+        if (!aligned(p, 2)) return refuse(what, "a pointer is not aligned to its elements");
+    for (const void* p : {(const void*)a->log_decay, (const void*)a->state, (const void*)a->state_out, (const void*)a->d_state_out,
+                          (const void*)a->d_state})
+        if (!aligned(p, 4)) return refuse(what, "a pointer is not aligned to its elements");
+    if (!aligned(a->lengths, 8)) return refuse(what, "a pointer is not aligned to its elements");
+    if (a->b == 0 || a->h == 0) return LF_OK;
+    if (!a->log_decay) return refuse(what, "log_decay is required");
+    if (a->t > 0 && (!a->q || !a->k || !a->v || (!bwd && !a->o) || (bwd && !a->d_o))) return refuse(what, "q, k, v and the output or its gradient are required");
+    if (bwd && a->t > 0 && a->d_state && !a->dv) return refuse(what, "the state's gradient comes with dv");
+    return LF_OK;
+}
+
+Heads heads_of(const void* p, const int64_t* s, int64_t d) { return {p, s[0], s[1], s[2], d}; }
+Heads dense_heads(void* p, const Sizes& z, int64_t d) { return {p, z.t * z.h * d, d, z.h * d, d}; }
+
+// T = 0: the state passes through.
+int pass_state(const char* what, const float* from, float* to, size_t bytes, cudaStream_t st) {
+    if (to && (from ? cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(to, 0, bytes, st)) != cudaSuccess)
+        return check_launch(what);
+    return LF_OK;
+}
+
+}  // namespace
+}  // namespace lfb
+
+using namespace lfb;
+
+extern "C" size_t lf_decay_attention_fwd_workspace_size(const lf_decay_attention_t* a) {
+    if (!a || check_attention("lf_decay_attention_fwd", a, false) || a->b == 0 || a->h == 0 || a->t == 0) return 0;
+    const Sizes z{a->b, a->h, a->t};
+    return packed_bytes(heads_of(a->q, a->q_strides, a->key_size), z) + packed_bytes(heads_of(a->k, a->k_strides, a->key_size), z) +
+           packed_bytes(heads_of(a->v, a->v_strides, a->value_size), z) + ends_bytes(z, blocks_of(a->key_size, a->value_size));
+}
+
+extern "C" int lf_decay_attention_fwd(const lf_decay_attention_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
+    clear_error();
+    const char* what = "lf_decay_attention_fwd";
+    if (int rc = check_attention(what, a, false)) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a->b == 0 || a->h == 0) return LF_OK;
+    if (a->t == 0) return pass_state(what, a->state, a->state_out, (size_t)(a->b * a->h * a->key_size * a->value_size) * 4, st);
+    const size_t need = lf_decay_attention_fwd_workspace_size(a);
+    if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) {
+        set_error("%s: needs %zu bytes of 256-byte aligned workspace, got %zu", what, need, workspace ? workspace_bytes : (size_t)0);
+        return LF_ERR_INVALID;
+    }
+    const Sizes z{a->b, a->h, a->t};
+    uint8_t* at = (uint8_t*)workspace;
+    Mix m;
+    m.a = addressable(heads_of(a->q, a->q_strides, a->key_size), z, at, st);
+    m.b = addressable(heads_of(a->k, a->k_strides, a->key_size), z, at, st);
+    m.c = addressable(heads_of(a->v, a->v_strides, a->value_size), z, at, st);
+    m.out = dense_heads(a->o, z, a->value_size);
+    m.g0 = a->state, m.gout = a->state_out;
+    return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, (float*)at, st);
+}
+
+extern "C" size_t lf_decay_attention_bwd_workspace_size(const lf_decay_attention_t* a) {
+    if (!a || check_attention("lf_decay_attention_bwd", a, true) || a->b == 0 || a->h == 0 || a->t == 0) return 0;
+    const Sizes z{a->b, a->h, a->t};
+    return packed_bytes(heads_of(a->q, a->q_strides, a->key_size), z) + packed_bytes(heads_of(a->k, a->k_strides, a->key_size), z) +
+           packed_bytes(heads_of(a->v, a->v_strides, a->value_size), z) + packed_bytes(heads_of(a->d_o, a->do_strides, a->value_size), z) +
+           ends_bytes(z, blocks_of(a->key_size, a->value_size));
+}
+
+extern "C" int lf_decay_attention_bwd(const lf_decay_attention_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
+    clear_error();
+    const char* what = "lf_decay_attention_bwd";
+    if (int rc = check_attention(what, a, true)) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a->b == 0 || a->h == 0) return LF_OK;
+    if (a->t == 0) return pass_state(what, a->d_state_out, a->d_state, (size_t)(a->b * a->h * a->key_size * a->value_size) * 4, st);
+    const size_t need = lf_decay_attention_bwd_workspace_size(a);
+    if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) {
+        set_error("%s: needs %zu bytes of 256-byte aligned workspace, got %zu", what, need, workspace ? workspace_bytes : (size_t)0);
+        return LF_ERR_INVALID;
+    }
+    const Sizes z{a->b, a->h, a->t};
+    uint8_t* at = (uint8_t*)workspace;
+    const Heads q = addressable(heads_of(a->q, a->q_strides, a->key_size), z, at, st);
+    const Heads k = addressable(heads_of(a->k, a->k_strides, a->key_size), z, at, st);
+    const Heads v = addressable(heads_of(a->v, a->v_strides, a->value_size), z, at, st);
+    const Heads g = addressable(heads_of(a->d_o, a->do_strides, a->value_size), z, at, st);
+    auto mix = [&](const Heads& x, const Heads& y, const Heads& w, void* out, const float* g0, float* gout, bool transposed, bool rev) {
+        Mix m;
+        m.a = x, m.b = y, m.c = w, m.out = dense_heads(out, z, w.d), m.g0 = g0, m.gout = gout, m.transposed = transposed, m.rev = rev;
+        return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, (float*)at, st);
+    };
+    if (a->dq)
+        if (int rc = mix(g, v, k, a->dq, a->state, nullptr, true, false)) return rc;
+    if (a->dk)
+        if (int rc = mix(v, g, q, a->dk, a->d_state_out, nullptr, true, true)) return rc;
+    if (a->dv)
+        if (int rc = mix(k, q, g, a->dv, a->d_state_out, a->d_state, false, true)) return rc;
+    return LF_OK;
+}
+
+extern "C" int lf_decay_attention_step(const lf_decay_step_t* a, lf_stream_t stream) {
+    clear_error();
+    const char* what = "lf_decay_attention_step";
+    if (!a) return refuse(what, "no arguments");
+    if (a->dtype != LF_F32 && a->dtype != LF_F16 && a->dtype != LF_BF16) {
+        set_error("%s: unsupported dtype code %d (fp32, fp16 and bf16)", what, a->dtype);
+        return LF_ERR_DTYPE;
+    }
+    if (int rc = check_sizes(what, a->b, a->h, 1, a->key_size, a->value_size)) return rc;
+    if (!(a->scale > 0) || !(a->scale < 1e30) || a->scale < 1e-30) return refuse(what, "scale must be between 1e-30 and 1e30");
+    if (a->b == 0 || a->h == 0) return LF_OK;
+    if (!a->q || !a->k || !a->v || !a->o || !a->state || !a->log_decay) return refuse(what, "every operand is required");
+    for (const void* p : {a->q, a->k, a->v, (const void*)a->o})
+        if (!aligned(p, dtype_size(a->dtype))) return refuse(what, "a pointer is not aligned to its elements");
+    for (const void* p : {(const void*)a->state, (const void*)a->log_decay})
+        if (!aligned(p, 4)) return refuse(what, "a pointer is not aligned to its elements");
+    const bool vec = a->value_size % 4 == 0 && aligned(a->state, 16);
+    StepArgs p{a->q, a->k, a->v, a->log_decay, a->state, a->o, a->q_strides[0], a->q_strides[1], a->k_strides[0], a->k_strides[1],
+               a->v_strides[0], a->v_strides[1], (int)a->h, (int)a->key_size, (int)a->value_size, 1, (float)a->scale};
+    while (p.tx * (vec ? 4 : 1) < p.dv) p.tx *= 2;
+    const unsigned grid = (unsigned)(a->b * a->h);
+    cudaStream_t st = (cudaStream_t)stream;
+#define LFB_STEP(T) (vec ? launch_early(decay_step_kernel<T, 4>, grid, 256, 0, 1, st, p) : launch_early(decay_step_kernel<T, 1>, grid, 256, 0, 1, st, p))
+    if (a->dtype == LF_F32) LFB_STEP(float);
+    else if (a->dtype == LF_F16) LFB_STEP(__half);
+    else LFB_STEP(__nv_bfloat16);
+#undef LFB_STEP
+    return check_launch(what);
+}

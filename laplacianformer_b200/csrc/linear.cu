@@ -30,13 +30,12 @@
 // forward 1.4-1.7 ms (1.3-1.5 PFLOP/s, tensor pipe 95 % active), gated backward
 // 2.75-2.86 ms (1.2), down projection 0.81-0.85 ms (1.3), the three gradients'
 // products 3.84-4.03 ms (1.4), against cuBLAS's 1.38 PFLOP/s under the same power cap.
-#include <cuda.h>
-
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
 
 #include "tc_ptx.cuh"
+#include "tma_map.h"
 #include "unit_plan.h"
 
 namespace lfb {
@@ -144,26 +143,6 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
     }
 }
 
-// ---------------------------------------------------------------------------
-// 16-bit pairs
-// ---------------------------------------------------------------------------
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u);
-template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&u));
-}
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
-}
-
 // Four consecutive elements of a row of n at p (column c); beyond the row: 0.
 template <typename T>
 __device__ __forceinline__ uint2 load4(const T* p, int c, int n, bool vec) {
@@ -245,17 +224,6 @@ constexpr int kTmemAll = 512;
 constexpr int kBarrierBytes = 256;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kGroupRows = 2048;          // rows that are walked together, so that their operands stay in L2
-
-// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery 1994).
-struct Divisor {
-    uint32_t d, mul, shift;
-    Divisor() = default;
-    explicit Divisor(uint32_t v) : d(v), shift(0) {
-        while ((1u << shift) < d) ++shift;
-        mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
-};
 
 // One product out of up to N that a launch runs.
 struct alignas(64) Problem {
@@ -1769,23 +1737,6 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const T* x, int64_t ldx, 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-    static std::once_flag once;
-    static EncodeFn fn = nullptr;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (EncodeFn)p;
-    });
-    return fn;
-}
-
 // A matrix in device memory as TMA sees it: `rows` rows of `inner` contiguous
 // elements, ld elements apart, in `planes` planes `plane` elements apart.
 struct Mat {
@@ -1800,23 +1751,8 @@ bool encode(CUtensorMap* map, const Mat& a, int dtype, int box_inner, int box_ro
                                    : dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const cuuint64_t dims[3] = {(cuuint64_t)a.inner, (cuuint64_t)a.rows, (cuuint64_t)a.planes};
     const cuuint64_t strides[2] = {(cuuint64_t)(a.ld * es), (cuuint64_t)((a.planes > 1 ? a.plane : a.rows * a.ld) * es)};
-    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_planes}, step[3] = {1, 1, 1};
-    EncodeFn fn = encode_fn();
-    if (!fn) {
-        set_error("cuTensorMapEncodeTiled is not available");
-        return false;
-    }
-    auto call = [&] {
-        return fn(map, ty, 3, const_cast<void*>(a.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    };
-    CUresult r = call();
-    if (r == CUDA_ERROR_INVALID_CONTEXT) {  // the first call of a host thread (an autograd worker): bind the device's context
-        int dev = 0;
-        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = call();
-    }
-    if (r != CUDA_SUCCESS) set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return r == CUDA_SUCCESS;
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_planes};
+    return encode_tiled(map, ty, 3, a.p, dims, strides, box, swizzle);
 }
 
 bool encode_out(CUtensorMap* map, const Mat& a, int dtype) { return encode(map, a, dtype, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B); }

@@ -45,6 +45,7 @@ __device__ int g_ns_status = 0;
 
 int peer_status(bool clear);  // peer.cu
 int gemm_status(bool clear);  // linear.cu
+int decay_status(bool clear);  // decay_attention.cu
 
 namespace {
 
@@ -1904,6 +1905,7 @@ extern "C" int lf_device_status(int clear) {
     }
     const int pv = peer_status(clear != 0);  // the peer barrier's word
     const int mv = gemm_status(clear != 0);  // the matrix product's
-    return v ? v : pv ? pv : mv;
+    const int dv = decay_status(clear != 0); // the decayed attention's
+    return v ? v : pv ? pv : mv ? mv : dv;
 }
 

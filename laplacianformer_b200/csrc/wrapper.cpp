@@ -5,6 +5,7 @@
 #include <string>
 
 #include "BlockOperators.h"
+#include "CausalOperators.h"
 #include "LaplaceSubtraction.h"
 #include "NewtonInverse.h"
 #include "laplacian_b200.h"
@@ -147,6 +148,61 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           [=](const at::Tensor& x, const at::Tensor& wi, const at::Tensor& wo, const T& bi, const T& bo, const T& r,
               int64_t act) { return GatedFeedForward(x, wi, wo, t(bi), t(bo), t(r), act); },
           "GatedFeedForward (x, w_in, w_out, b_in, b_out, residual, activation) -> y, with autograd");
+    // Causal operators (no counterpart in the reference module).
+    m.def("DecayAttention_forward",
+          [=](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, const T& s, const T& n, double scale, bool want) {
+              auto [y, e] = DecayAttention_forward(q, k, v, g, t(s), t(n), scale, want);
+              return std::make_tuple(y, o(e));
+          },
+          "DecayAttention_forward (q, k, v, log_decay, state, lengths, scale, want_state) -> (o, state)");
+    m.def("DecayAttention_backward",
+          [=](const at::Tensor& d, const T& ds, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, const T& s,
+              const T& n, double scale, bool nq, bool nk, bool nv, bool ns) {
+              auto [a, b, c, e] = DecayAttention_backward(d, t(ds), q, k, v, g, t(s), t(n), scale, nq, nk, nv, ns);
+              return std::make_tuple(o(a), o(b), o(c), o(e));
+          },
+          "DecayAttention_backward (d_o, d_state, q, k, v, log_decay, state, lengths, scale, need_q, need_k, need_v, need_state) -> "
+          "(dq, dk, dv, d_state)");
+    m.def("DecayAttention_step", &DecayAttention_step,
+          "DecayAttention_step (q, k, v, log_decay, state, scale) -> o; state is updated in place");
+    m.def("DecayAttention",
+          [=](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, const T& s, const T& n, double scale, bool want) {
+              auto [y, e] = DecayAttention(q, k, v, g, t(s), t(n), scale, want);
+              return std::make_tuple(y, o(e));
+          },
+          "DecayAttention (q, k, v, log_decay, state, lengths, scale, want_state) -> (o, state), with autograd");
+    m.def("Rotary_forward",
+          [=](const at::Tensor& q, const T& k, const at::Tensor& f, const T& pos, int64_t offset, bool interleaved, double magnitude, bool inverse) {
+              auto [a, b] = Rotary_forward(q, t(k), f, t(pos), offset, interleaved, magnitude, inverse);
+              return std::make_tuple(a, o(b));
+          },
+          "Rotary_forward (q, k, frequencies, positions, offset, interleaved, magnitude, inverse) -> (q, k)");
+    m.def("Rotary",
+          [=](const at::Tensor& q, const T& k, const at::Tensor& f, const T& pos, int64_t offset, bool interleaved, double magnitude) {
+              auto [a, b] = Rotary(q, t(k), f, t(pos), offset, interleaved, magnitude);
+              return std::make_tuple(a, o(b));
+          },
+          "Rotary (q, k, frequencies, positions, offset, interleaved, magnitude) -> (q, k), with autograd");
+    m.def("SandwichNorm_forward",
+          [=](const at::Tensor& x, const at::Tensor& w, const at::Tensor& r, const T& g, const T& n, int64_t act, double scale, double eps, bool keep) {
+              auto [s, y, rstd] = SandwichNorm_forward(x, w, r, t(g), t(n), act, scale, eps, keep);
+              return std::make_tuple(s, o(y), o(rstd));
+          },
+          "SandwichNorm_forward (x, weight, residual, gate, next_weight, gate_activation, scale, eps, keep) -> (s, y, rstd)");
+    m.def("SandwichNorm_backward",
+          [=](const T& ds, const T& dy, const at::Tensor& x, const at::Tensor& s, const at::Tensor& rstd, const at::Tensor& w, const T& g, const T& n,
+              int64_t act, double scale, double eps, bool nx, bool nw, bool nr, bool ng, bool nn) {
+              auto [a, b, c, d, e] = SandwichNorm_backward(t(ds), t(dy), x, s, rstd, w, t(g), t(n), act, scale, eps, nx, nw, nr, ng, nn);
+              return std::make_tuple(o(a), o(b), o(c), o(d), o(e));
+          },
+          "SandwichNorm_backward (ds, dy, x, s, rstd, weight, gate, next_weight, gate_activation, scale, eps, need_x, need_w, need_r, need_g, "
+          "need_n) -> (dx, dw, dr, dg, dn)");
+    m.def("SandwichNorm",
+          [=](const at::Tensor& x, const at::Tensor& w, const at::Tensor& r, const T& g, const T& n, int64_t act, double scale, double eps) {
+              auto [s, y] = SandwichNorm(x, w, r, t(g), t(n), act, scale, eps);
+              return std::make_tuple(s, o(y));
+          },
+          "SandwichNorm (x, weight, residual, gate, next_weight, gate_activation, scale, eps) -> (s, y), with autograd");
     // Lists are read in place: a copied Tensor per gradient would cost more than the kernels on a small model.
     auto tensors = [](const py::list& list) {
         std::vector<const at::Tensor*> v(list.size());

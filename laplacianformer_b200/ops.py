@@ -16,10 +16,16 @@ nodes of the extension),
 :func:`rms_norm_quant`, :func:`quantize_rows` and :func:`linear_quant` for
 serving with 8-bit operands, and :func:`clip_grad_norm`.
 
+What a block that reads its tokens in order needs (none of it in the reference):
+:func:`decay_attention`, its form for single tokens :func:`decay_attention_step`,
+:func:`rotary`, and :func:`sandwich_norm`, the norms around a sublayer.
+
 Every call goes to the ``Laplace_subtraction_cuda`` extension; there is no CPU
 fallback and a missing extension raises ImportError.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -255,3 +261,93 @@ def clip_grad_norm(grads, max_norm: float, out=None):
     grads = list(grads)
     out = [torch.empty_like(g) for g in grads] if out is None else list(out)
     return ext().ClipGradNorm(grads, out, float(max_norm)), out
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor | None = None,
+                    lengths: torch.Tensor | None = None, scale: float | None = None, return_state: bool = False):
+    """Causal linear attention with a decay per head: S_t = exp(log_decay) S_(t-1) + k_t v_t^T, o_t = scale q_t S_t.
+
+    q, k [B, H, N, Dk] and v [B, H, N, Dv], fp16 or bf16, sizes up to 128, with any strides (views of a joint projection
+    are read in place); log_decay float32 [H], meant to be at most 0 (no gradient).  state: float32 [B, H, Dk, Dv] before
+    the first token (zeros if None).  lengths: int64 [B] on the GPU, for sequences padded at their end: tokens past the
+    length enter no result, and their outputs and gradients are 0.  scale defaults to Dk^-0.5.
+
+    Returns o [B, H, N, Dv] (in memory [B, N, H, Dv], so that o.transpose(1, 2).reshape(B, N, H * Dv) copies nothing), or
+    (o, state after the last token) with return_state, for the next piece of a prompt or :func:`decay_attention_step`.
+    Work is linear in N, by chunks of 128 tokens on the tensor cores; a value that is not finite reaches its whole chunk.
+    In fp16 the scores become infinite beyond 65504.  First order, reverse mode only."""
+    o, s = ext().DecayAttention(q, k, v, log_decay, state, lengths, q.shape[-1] ** -0.5 if scale is None else scale, return_state)
+    return (o, s) if return_state else o
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
+                         scale: float | None = None) -> torch.Tensor:
+    """:func:`decay_attention` of one token per sequence: q, k [B, H, Dk], v [B, H, Dv] (fp32, fp16 or bf16); the state,
+    contiguous float32 [B, H, Dk, Dv], is updated in place.  Returns o [B, H, Dv].  No gradient."""
+    return ext().DecayAttention_step(q, k, v, log_decay, state, q.shape[-1] ** -0.5 if scale is None else scale)
+
+
+ROTARY_SCALINGS = ("none", "linear", "base", "by_parts")
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_length: float | None = None,
+                       low: float = 1.0, high: float = 32.0) -> torch.Tensor:
+    """Radians per position of the dim / 2 pairs of :func:`rotary`, base^(-2i / dim), float64 on the host.
+
+    For contexts `factor` times longer than the trained ones: "linear" divides all frequencies by factor (positions are
+    interpolated), "base" raises the base by factor^(dim / (dim - 2)) (the last pair is interpolated, the first kept), and
+    "by_parts" keeps pairs that turn over `high` times within original_length, interpolates those below `low` turns, and
+    blends in between."""
+    if dim < 0 or dim % 2:
+        raise ValueError("dim must be even")
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"unknown scaling {scaling!r}: one of {', '.join(ROTARY_SCALINGS)}")
+    if not factor > 0 or not base > 0:
+        raise ValueError("base and factor must be positive")
+    if scaling == "base" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    f = torch.pow(torch.tensor(base, dtype=torch.float64), torch.arange(0, dim, 2, dtype=torch.float64) / -max(dim, 1))
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "by_parts":
+        if original_length is None or not high > low:
+            raise ValueError("by_parts needs original_length, and high above low")
+        keep = ((original_length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f * (keep + (1 - keep) / factor)
+    return f
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, frequencies: torch.Tensor, positions: torch.Tensor | None = None, offset: int = 0,
+           interleaved: bool = False, magnitude: float = 1.0):
+    """Rotary positions: pair i of each head turns by position * frequencies[i] and is scaled by magnitude.
+
+    q [B, H, N, D] and k [B, Hk, N, D] (or None), fp32, fp16 or bf16, with any strides; frequencies from
+    :func:`rotary_frequencies` (at most 128 pairs; channels past the pairs are copied).  Pairs are channels (i, i + pairs),
+    or (2i, 2i + 1) if interleaved.  positions: int64 [N] or [B, N] on the GPU, or None: offset, offset + 1 and so on.
+    Angles are formed in 64 bits, so far positions lose nothing.
+
+    Returns (q, k) turned, or q alone without k, in memory [B, N, H, D].  First order, reverse mode only."""
+    y, z = ext().Rotary(q, k, frequencies, positions, offset, interleaved, magnitude)
+    return y if k is None else (y, z)
+
+
+GATE_ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
+
+
+def sandwich_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor, gate: torch.Tensor | None = None,
+                  next_weight: torch.Tensor | None = None, gate_activation: str = "none", scale: float = 1.0, eps: float = 1e-6):
+    """What lies between two sublayers: the norm after one, its gate, the residual scale, the addition, the next one's norm.
+
+        s = residual + scale * gate_activation(gate) * rms_norm(x, weight)
+        y = rms_norm(s, next_weight)
+
+    Returns (y, s), or s alone without next_weight.  fp32, fp16 and bf16, all of one dtype; statistics in fp32, y from the
+    unrounded s.  gate: x's shape (per token), [..., 1, C] (shared by the tokens of a sequence) or [C]; in general ones in
+    the place of x's last dimensions before the channels.  Strided operands are copied first.  First order, reverse mode
+    only."""
+    try:
+        act = GATE_ACTIVATIONS[gate_activation]
+    except KeyError:
+        raise ValueError(f"unknown gate activation {gate_activation!r}: one of {', '.join(GATE_ACTIVATIONS)}") from None
+    s, y = ext().SandwichNorm(x, weight, residual, gate, next_weight, act, scale, eps)
+    return s if next_weight is None else (y, s)

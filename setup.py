@@ -28,6 +28,7 @@ setup(
                 os.path.join("laplacianformer_b200", "csrc", "wrapper.cpp"),
                 os.path.join("laplacianformer_b200", "csrc", "torch_ops.cpp"),
                 os.path.join("laplacianformer_b200", "csrc", "torch_block_ops.cpp"),
+                os.path.join("laplacianformer_b200", "csrc", "torch_causal_ops.cpp"),
             ],
             include_dirs=[os.path.join(HERE, "include")],
             define_macros=[("WITH_CUDA", None)],
