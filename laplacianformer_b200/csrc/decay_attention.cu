@@ -20,6 +20,7 @@
 // into its range), and l^(n-j) b_j, which goes in as two 16-bit parts so that
 // the state keeps about 17 bits (bf16) or 22 (fp16) of each term.
 #include <algorithm>
+#include <type_traits>
 
 #include "tc_ptx.cuh"
 #include "tma_map.h"
@@ -46,17 +47,19 @@ constexpr int kRing = 5;              // operand tiles in flight: the chunk's th
 constexpr int kEpi = 256;             // threads that turn accumulators into operands and outputs
 constexpr int kThreads = kEpi + 64;   // and a warp for copies, a warp for products
 constexpr int kBlock = kChunk * 128;  // bytes of 128 rows of 64 columns
+constexpr uint32_t kNegateA = 1u << 13;  // of an instruction descriptor: the product with -A
 
 struct alignas(64) MixArgs {
     CUtensorMap a, b, c, out;
     const float* log_decay;
     const float* g0;         // state before the first token (to be decayed by l), or with `rev` the gradient of the last state
     float* gout;             // state after the last token, or with `rev` the gradient of the first state
-    float* ends;             // [bh][nseg][64W][64W]: what each segment adds to the state
+    float* ends;             // [bh][nseg][units][64W][64W]: what each unit of a segment adds to the state
     const int64_t* lengths;  // tokens per sequence, or null
     void* o;                 // rows of dc elements, where TMA cannot write them
     int64_t o_sb, o_sh, o_st;
     int heads, t, da, dc, chunks, nseg, per_seg, items;
+    int unit, units;         // chunks per unit, units per segment
     int g0_row, g0_col;      // strides within a state matrix (transposed for dq and dk)
     float scale, g0_scale, gout_scale;
     int ksteps, nb;          // 16-column steps of da; dc rounded up to 16
@@ -66,8 +69,15 @@ struct alignas(64) MixArgs {
 
 template <int W>
 constexpr int mix_smem() {
-    // ring, low parts (then the output's staging), state operand, tables, barriers
-    return 1024 + (kRing + 1) * W * kBlock + 64 * W * 128 * W + 1024 + 256;
+    // ring, low parts (then the output's staging), state operand, tables and barriers
+    return 1024 + (kRing + 1) * W * kBlock + 64 * W * 128 * W + 2048;
+}
+
+template <int W>
+constexpr int kEndsRing = 4;  // tiles in flight of the sums before a segment
+template <int W>
+constexpr int ends_smem() {
+    return 1024 + (kEndsRing<W> + 2) * W * kBlock + 256;
 }
 
 __device__ __forceinline__ void load4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int h, int t, int b) {
@@ -84,6 +94,32 @@ __device__ __forceinline__ void store4d(const CUtensorMap* map, const void* src,
 __device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+// mbar_wait() for waits that are mostly short: the clock is read only after a run of tries, so that waiting warps take few
+// issue slots from the working ones (they took more than half: 4096 tokens of 128 heads 78 us with mbar_wait, XX with this).
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
+    const uint32_t addr = smem_u32(bar);
+    uint64_t t0 = 0;
+    for (uint32_t spin = 0;; ++spin) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t.reg .b32 n;\n\t"
+            "mov.b32 n, 0;\n"
+            "TRY%=:\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "@p bra DONE%=;\n\t"
+            "add.u32 n, n, 1;\n\t"
+            "setp.lt.u32 q, n, 64;\n\t"
+            "@q bra TRY%=;\n"
+            "DONE%=:\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity), "r"(20000u)
+            : "memory");
+        if (done) return true;
+        if (spin == 0) t0 = global_ns();
+        else if (global_ns() - t0 > 2000000000ull) return false;
+    }
+}
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -98,6 +134,25 @@ __device__ __forceinline__ bool epi_sync(bool ok) {
         : "memory");
     return r != 0;
 }
+// Pairs of 16-bit values, each product and sum rounded once.
+template <typename T> __device__ __forceinline__ uint32_t mul16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint32_t fma16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// The lowest n bits (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t keep_low(int n) {
+    uint32_t r;
+    asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(0xffffffffu), "r"(max(n, 0)));  // (shifts past the width give 0)
+    return ~r;
+}
 __device__ __forceinline__ void sts16(uint8_t* p, uint4 v) { *reinterpret_cast<uint4*>(p) = v; }
 
 // l^n; 1 for n = 0 whatever l is.
@@ -107,19 +162,18 @@ struct Item {
     int bh, b, h, seg, first, n, active;
     int64_t len;
 };
-template <bool REV, bool ENDS>
+__device__ __forceinline__ int64_t tokens_in(const MixArgs& p, int b) {
+    if (!p.lengths) return p.t;
+    const int64_t n = p.lengths[b];
+    return n < 0 ? 0 : n < p.t ? n : p.t;
+}
 __device__ __forceinline__ Item item_of(const MixArgs& p, int i) {
     Item t;
-    const int segs = ENDS ? p.nseg - 1 : p.nseg;  // nobody follows the last segment
-    t.bh = i / segs;
-    t.seg = i - t.bh * segs + (ENDS && REV ? 1 : 0);
+    t.bh = i / p.nseg;
+    t.seg = i - t.bh * p.nseg;
     t.b = t.bh / p.heads;
     t.h = t.bh - t.b * p.heads;
-    t.len = p.t;
-    if (p.lengths) {
-        const int64_t n = p.lengths[t.b];
-        t.len = n < 0 ? 0 : n < p.t ? n : p.t;
-    }
+    t.len = tokens_in(p, t.b);
     t.active = (int)((t.len + kChunk - 1) / kChunk);
     t.first = t.seg * p.per_seg;
     const int last = min(min(t.first + p.per_seg, p.chunks), t.active);
@@ -134,9 +188,208 @@ __device__ __forceinline__ float range_scale(uint32_t bits) {
     return __uint_as_float((uint32_t)max(1, min(127 + 141 - e, 254)) << 23);
 }
 
+// Scales rows of a tile of b, 8 at a time (eight lanes to a row, so that no bank is met twice): b w in two parts, the
+// first in place, the second negated in `low`; w0 and w1 are a row's weight in two parts, for the rows 4 apart.
+//   high = b w0 rounded;  b w0 - high is exact (it has no more bits than b), and b w1 joins it with one rounding
+template <typename T, int W>
+__device__ __forceinline__ void scale_rows(uint8_t* tile, uint8_t* low, int row0, int lane, const uint32_t (&wh)[2], const uint32_t (&wl)[2]) {
+    const int r = row0 + (lane >> 3), ch = lane & 7;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        uint4 x[2];
+        int at[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            at[i] = w * kBlock + (r + 4 * i) * 128 + ((ch ^ ((r + 4 * i) & 7)) << 4);
+            x[i] = *reinterpret_cast<const uint4*>(tile + at[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                h[q] = mul16x2<T>(v[q], wh[i]);
+                l[q] = fma16x2<T>(v[q], wl[i] ^ 0x80008000u, fma16x2<T>(v[q], wh[i] ^ 0x80008000u, h[q]));
+            }
+            sts16(tile + at[i], make_uint4(h[0], h[1], h[2], h[3]));
+            sts16(low + at[i], make_uint4(l[0], l[1], l[2], l[3]));
+        }
+    }
+}
+// A weight in two 16-bit parts, side by side; and each twice for packed arithmetic.
+template <typename T>
+__device__ __forceinline__ uint32_t split_weight(float w) {
+    const T hi = Elem<T>::store(w);
+    return pack2<T>(w, w - Elem<T>::load(hi));
+}
+__device__ __forceinline__ void spread(uint32_t w, uint32_t& wh, uint32_t& wl) {
+    wh = __byte_perm(w, w, 0x1010);
+    wl = __byte_perm(w, w, 0x3232);
+}
+// Rows past the sequence's end: zeros, whatever they hold.
+template <int W>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int thread, int threads) {
+    for (int j = thread; j < (kChunk - from) * 8 * W; j += threads) {
+        const int r = from + j / (8 * W), u = j % (8 * W);
+        sts16(tile + (u >> 3) * kBlock + r * 128 + ((u & 7) << 4), make_uint4(0u, 0u, 0u, 0u));
+    }
+}
+
+// What units of chunks add to the state, for the segments that go on after them: sum_j l^(n-j) b_j c_j^T with all weights
+// taken to the unit's end, so that the products of its chunks follow one another on one accumulator (weights that
+// underflow are of tokens that do not matter any more).  Two warps copy and multiply, eight scale b.
+template <typename T, int W, bool REV>
+__global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_constant__ MixArgs p) {
+    constexpr int kTile = W * kBlock, kState = 64 * W, kTiles = kEndsRing<W>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const lows = ring + kTiles * kTile;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(lows + 2 * kTile);
+    uint64_t *full = bars, *empty = bars + kTiles, *ready = empty + kTiles, *used = ready + 2, *done = used + 2, *read = done + 1, *drain = done + 2;
+    uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    grid_release();
+    if (tid == 0) {
+        for (int i = 0; i < kTiles; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&ready[i], kEpi), mbar_init(&used[i], 1);
+        mbar_init(done, 1), mbar_init(read, kEpi / 2), mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) tmem_alloc(tmem_ptr, 128);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_wait();
+    const uint32_t tmem = *tmem_ptr;
+    bool ok = true;
+    // Unit i of the segments that others follow.
+    struct Unit {
+        int b, h, first, n;  // chunks
+        int64_t len, slot;
+    };
+    auto unit_of = [&](int i) {
+        const int per = (p.nseg - 1) * p.units, bh = i / per, r = i - bh * per, seg = r / p.units + (REV ? 1 : 0), u = r % p.units;
+        Unit x;
+        x.b = bh / p.heads, x.h = bh - x.b * p.heads;
+        x.len = tokens_in(p, x.b);
+        x.slot = ((int64_t)bh * p.nseg + seg) * p.units + u;
+        x.first = seg * p.per_seg + u * p.unit;
+        const int end = min(min(x.first + p.unit, (seg + 1) * p.per_seg), p.chunks), active = (int)((x.len + kChunk - 1) / kChunk);
+        // Forwards only whole units are asked for.
+        x.n = REV ? max(0, min(end, active) - x.first) : end > x.first && (int64_t)end * kChunk <= x.len ? end - x.first : 0;
+        return x;
+    };
+    const int count = p.items;
+    if (warp == 8) {
+        if (elect_one()) {
+            int n = 0;
+            for (int i = blockIdx.x; ok && i < count; i += gridDim.x) {
+                const Unit x = unit_of(i);
+                for (int k = 0; ok && k < x.n; ++k)
+                    for (int j = 0; j < 2; ++j, ++n) {
+                        const int s = n % kTiles;
+                        if (!(ok = wait_for(&empty[s], (n / kTiles & 1) ^ 1))) break;
+                        expect(&full[s], kTile);
+                        for (int w = 0; w < W; ++w)
+                            load4d(ring + s * kTile + w * kBlock, j ? &p.c : &p.b, &full[s], w * 64, x.h, (x.first + k) * kChunk, x.b);
+                    }
+            }
+            if (!ok)
+                for (int k = max(0, n - kTiles); k < n; ++k) mbar_wait(&full[k % kTiles], k / kTiles & 1, 100000000ull);
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        const uint32_t go = elect_one() ? 1u : 0u;
+        int m = 0, items = 0;
+        for (int i = blockIdx.x; ok && i < count; i += gridDim.x) {
+            const Unit x = unit_of(i);
+            if (x.n == 0) continue;
+            if (items > 0 && !(ok = wait_for(read, (items - 1) & 1))) break;  // the last sum has been read
+            for (int k = 0; k < x.n; ++k, ++m) {
+                const int nb = 2 * m % kTiles, nc = (2 * m + 1) % kTiles;
+                if (!(ok = wait_for(&full[nc], (2 * m + 1) / kTiles & 1) && wait_for(&ready[m & 1], m >> 1 & 1))) break;
+                tc_fence_after();
+                const uint64_t dh = make_desc(smem_u32(ring + nb * kTile), kBlock, 1024), dl = make_desc(smem_u32(lows + (m & 1) * kTile), kBlock, 1024);
+                const uint64_t dv = make_desc(smem_u32(ring + nc * kTile), kBlock, 1024);
+#pragma unroll
+                for (int s = 0; s < 8; ++s) mma_f16(tmem, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, k > 0 || s > 0 ? 1u : 0u, go);
+#pragma unroll
+                for (int s = 0; s < 8; ++s) mma_f16(tmem, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, 1u, go);
+                if (go) mma_commit(&empty[nb]), mma_commit(&empty[nc]), mma_commit(&used[m & 1]);
+            }
+            if (!ok) break;
+            if (go) mma_commit(done);
+            ++items;
+        }
+        if (!ok) {
+            if (go) mma_commit(drain);
+            mbar_wait(drain, 0, 100000000ull);
+        }
+        __syncwarp();
+    } else {
+        const int quad = warp & 3;
+        const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16);
+        int m = 0, items = 0;
+        for (int i = blockIdx.x; i < count; i += gridDim.x) {
+            const Unit x = unit_of(i);
+            if (x.n == 0) continue;
+            const float g = p.log_decay[x.h];
+            for (int k = 0; k < x.n; ++k, ++m) {
+                const int nb = 2 * m % kTiles, nc = (2 * m + 1) % kTiles;
+                const int L = (int)min((int64_t)kChunk, x.len - (int64_t)(x.first + k) * kChunk);
+                uint32_t wh[2][2], wl[2][2];  // of the 16 rows of this warp
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = warp * 16 + (i >> 1) * 8 + (i & 1) * 4 + (lane >> 3);
+                    const int64_t n = REV ? (int64_t)k * kChunk + r + 1 : (int64_t)(x.n - k) * kChunk - r;
+                    spread(split_weight<T>(power(g, n)), wh[i >> 1][i & 1], wl[i >> 1][i & 1]);
+                }
+                uint8_t* const low = lows + (m & 1) * kTile;
+                ok = ok && wait_for(&full[nb], 2 * m / kTiles & 1);
+                ok = ok && wait_for(&used[m & 1], (m >> 1 & 1) ^ 1);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) scale_rows<T, W>(ring + nb * kTile, low, warp * 16 + u * 8, lane, wh[u], wl[u]);
+                if (L < kChunk) {
+                    ok = ok && wait_for(&full[nc], (2 * m + 1) / kTiles & 1);
+                    epi_sync(true);  // (the rows that others scaled)
+                    clear_rows<W>(ring + nb * kTile, L, tid, kEpi), clear_rows<W>(low, L, tid, kEpi), clear_rows<W>(ring + nc * kTile, L, tid, kEpi);
+                }
+                fence_async_smem();
+                arrive(&ready[m & 1]);
+            }
+            if (warp < 4) {
+                ok = ok && wait_for(done, items & 1);
+                tc_fence_after();
+                // The accumulators of 64 rows are 16 in each quarter of the lanes.
+                float* const dst = p.ends + (x.slot * kState + (W == 1 ? quad * 16 + lane : quad * 32 + lane)) * kState;
+#pragma unroll
+                for (int c = 0; c < kState; c += 16) {
+                    float v[16];
+                    tmem_ld16(tq + c, v);
+                    tmem_wait_ld();
+                    reg_fence(v);
+                    if (W == 2 || lane < 16)
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            *reinterpret_cast<float4*>(dst + c + j) = c < p.nb ? make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                tc_fence_before();
+                arrive(read);
+            }
+            ++items;
+        }
+    }
+    if (!ok) atomicExch(&g_decay_status, (int)LF_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, 128);
+}
+
 // W: 64-column blocks per operand row (head sizes up to 64 W).  REV: backwards
-// in time.  ENDS: only what a segment adds to the state.
-template <typename T, int W, bool REV, bool ENDS>
+// in time.
+template <typename T, int W, bool REV>
 __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W;                        // state rows
     constexpr int kO = 128, kKv = 128 + 64 * W, kCols = W == 1 ? 256 : 512;   // tensor memory columns; scores from 0 on
@@ -146,9 +399,9 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     uint8_t* const low = ring + kRing * kTile;
     uint8_t* const gop = low + kTile;                                         // [state row][dc], 64 columns a block
     float* const pw = reinterpret_cast<float*>(gop + kState * 128 * W);       // l^n, n = 0..128
-    float* const back = pw + 132;                                             // l^(31-n)
-    uint32_t* const gmax = reinterpret_cast<uint32_t*>(back + 32);
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 256);
+    float* const factors = pw + 132;                                          // of the scores, see there: two copies, 176 apart
+    uint32_t* const gmax = reinterpret_cast<uint32_t*>(factors + 340);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 474);
     uint64_t *full = bars, *empty = bars + kRing, *s_full = bars + 2 * kRing, *k_ready = s_full + 1, *p_ready = s_full + 2,
              *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7;
     uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 8);
@@ -167,19 +420,19 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     tc_fence_after();
     grid_wait();
     const uint32_t tmem = *tmem_ptr;
-    constexpr int kTiles = ENDS ? 2 : 3;
+    constexpr int kTiles = 3;
     bool ok = true;
 
     if (warp == 8) {  // copies
         if (elect_one()) {
             int n = 0;
             for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
-                const Item t = item_of<REV, ENDS>(p, i);
+                const Item t = item_of(p, i);
                 for (int k = 0; ok && k < t.n; ++k) {
                     const int t0 = (REV ? t.first + t.n - 1 - k : t.first + k) * kChunk;
                     for (int j = 3 - kTiles; j < 3; ++j) {
                         const int s = n % kRing;
-                        if (!(ok = mbar_wait(&empty[s], (n / kRing & 1) ^ 1))) break;
+                        if (!(ok = wait_for(&empty[s], (n / kRing & 1) ^ 1))) break;
                         expect(&full[s], kTile);
                         const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
                         for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
@@ -195,49 +448,51 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
         const uint32_t go = elect_one() ? 1u : 0u;
         int n = 0, cc = 0;
         for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
-            const Item t = item_of<REV, ENDS>(p, i);
+            const Item t = item_of(p, i);
             for (int k = 0; k < t.n; ++k, ++cc, n += kTiles) {
                 const int na = n, nk = n + kTiles - 2, nv = nk + 1;
                 const uint32_t sk = smem_u32(ring + nk % kRing * kTile), sv = smem_u32(ring + nv % kRing * kTile);
-                if (!(ok = mbar_wait(&full[nk % kRing], nk / kRing & 1))) break;
-                bool has_g = false;
-                if constexpr (!ENDS) {
+                if (!(ok = wait_for(&full[nk % kRing], nk / kRing & 1))) break;
+                bool has_g = k > 0;  // there is a state before this chunk
+                {
                     const int first = REV ? (t.active - 1) / p.per_seg : 0;  // the segment that the sequence starts with
                     has_g = k > 0 || p.g0 || t.seg != first;
                     const uint32_t sa = smem_u32(ring + na % kRing * kTile);
-                    if (!(ok = mbar_wait(&full[na % kRing], na / kRing & 1))) break;
-                    if (cc > 0 && !(ok = mbar_wait(o_full, (cc - 1) & 1))) break;  // the scores' columns hold its operand
+                    if (!(ok = wait_for(&full[na % kRing], na / kRing & 1))) break;
+                    if (cc > 0 && !(ok = wait_for(o_full, (cc - 1) & 1))) break;  // the scores' columns hold its operand
                     tc_fence_after();
                     const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sk, 16, 1024);
-                    for (int s = 0; s < p.ksteps; ++s) {
+#pragma unroll
+                    for (int s = 0; s < 4 * W; ++s) {  // (unrolled: an address that the loop computes costs more than the product)
                         const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
-                        mma_f16(tmem, da + at, db + at, p.id_qk, s > 0 ? 1u : 0u, go);
+                        if (s < p.ksteps) mma_f16(tmem, da + at, db + at, p.id_qk, s > 0 ? 1u : 0u, go);
                     }
                     if (go) mma_commit(s_full);
-                    if (!(ok = mbar_wait(g_ready, cc & 1))) break;
+                    if (!(ok = wait_for(g_ready, cc & 1))) break;
                     tc_fence_after();
                     if (has_g) {
                         const uint64_t dg = make_desc(smem_u32(gop), kState * 128, 1024);
-                        for (int s = 0; s < p.ksteps; ++s) {
+#pragma unroll
+                        for (int s = 0; s < 4 * W; ++s) {
                             const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
-                            mma_f16(tmem + kO, da + at, dg + (uint64_t)(s * 128), p.id_qg, s > 0 ? 1u : 0u, go);
+                            if (s < p.ksteps) mma_f16(tmem + kO, da + at, dg + (uint64_t)(s * 128), p.id_qg, s > 0 ? 1u : 0u, go);
                         }
                         if (go) mma_commit(qg_full);
                     }
                     if (go) mma_commit(&empty[na % kRing]);
                 }
-                if (!(ok = mbar_wait(k_ready, cc & 1) && mbar_wait(&full[nv % kRing], nv / kRing & 1))) break;
+                if (!(ok = wait_for(k_ready, cc & 1) && wait_for(&full[nv % kRing], nv / kRing & 1))) break;
                 tc_fence_after();
                 {
                     const uint64_t dh = make_desc(sk, kBlock, 1024), dl = make_desc(smem_u32(low), kBlock, 1024);
                     const uint64_t dv = make_desc(sv, kBlock, 1024);
 #pragma unroll
-                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, s > 0 ? 1u : 0u, go);
+                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, has_g || s > 0 ? 1u : 0u, go);
 #pragma unroll
-                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, 1u, go);
+                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, 1u, go);
                     if (go) mma_commit(kv_full), mma_commit(&empty[nk % kRing]);
-                    if constexpr (!ENDS) {
-                        if (!(ok = mbar_wait(p_ready, cc & 1))) break;
+                    {
+                        if (!(ok = wait_for(p_ready, cc & 1))) break;
                         tc_fence_after();
 #pragma unroll
                         for (int s = 0; s < 8; ++s)  // scores of columns 64 on lie 64 columns further
@@ -261,20 +516,76 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
         const int srow = W == 1 ? quad * 16 + lane : row;
         const bool live = W == 2 || lane < 16;
         const int col0 = half * 32 * W;                           // this thread's columns of the state and of the output
-        float G[32 * W];
+        const int kr = tid >> 1, kpart = tid & 1;                 // the row of b, and half of it, that this thread scales
+        // Factors scale l^(i-j) of this thread's row i, from column 0 on: pairs of them are 8-byte loads from the copy
+        // that has them on that boundary (half a warp's loads meet no bank twice).  Past the diagonal they are 0.
+        const int f0 = REV ? 32 - row : 127 - row;
+        const float* const frow = factors + (f0 & 1 ? 177 : 0) + f0;
         int n = 0, cc = 0, qg = 0, puts = 0;
         for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
-            const Item t = item_of<REV, ENDS>(p, i);
+            const Item t = item_of(p, i);
             const float g = p.log_decay[t.h];
+            const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
+            bool has_g = (p.g0 || (t.n > 0 && t.seg != first_seg));
+            float G[32 * W], unscale = 1.f;
+            // Chunk k of the item, its tokens, and 1 where the state shall not be decayed past its last token.
+            auto chunk_of = [&](int k) { return REV ? t.first + t.n - 1 - k : t.first + k; };
+            auto tokens_of = [&](int k) { return (int)min((int64_t)kChunk, t.len - (int64_t)chunk_of(k) * kChunk); };
+            auto last_of = [&](int k) { return !REV && p.gout && chunk_of(k) == t.active - 1 ? 1 : 0; };
+            // G before chunk k: as an operand (rows of dc columns, in fp16 times a power of two that keeps the largest in
+            // range), and decayed over the chunk to where the products add to it.
+            auto put_state = [&](int k) {
+                {
+                    float s = 1.f;
+                    if constexpr (F16) {
+                        float m = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32 * W; ++j) m = fmaxf(m, fabsf(G[j]));
+                        const uint32_t wm = __reduce_max_sync(0xffffffffu, live ? __float_as_uint(m) : 0u);
+                        const int slot = puts++ & 1;
+                        if (lane == 0) atomicMax(&gmax[slot], wm);
+                        epi_sync(true);
+                        s = range_scale(gmax[slot]);
+                        if (tid == 0) gmax[slot ^ 1] = 0;
+                        unscale = 1.f / s;
+                    }
+                    if (live) {
+                        uint8_t* const dst = gop + (W == 2 ? half * kState * 128 : 0) + srow * 128;
+#pragma unroll
+                        for (int j = 0; j < 4 * W; ++j) {
+                            const float* v = &G[8 * j];
+                            const int ch = (W == 1 ? half * 4 : 0) + j;
+                            const uint4 o = F16 ? make_uint4(pack2<T>(v[0] * s, v[1] * s), pack2<T>(v[2] * s, v[3] * s), pack2<T>(v[4] * s, v[5] * s),
+                                                             pack2<T>(v[6] * s, v[7] * s))
+                                                : make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+                            sts16(dst + ((ch ^ (srow & 7)) << 4), o);
+                        }
+                    }
+                    fence_async_smem();
+                }
+                const float w = pw[tokens_of(k) - last_of(k)];
+                const uint64_t w2 = pk2(w, w);
+#pragma unroll
+                for (int c = 0; c < 2 * W; ++c)
+                    if (col0 + 16 * c < p.nb) {
+                        float v[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) upk2(mul2(pk2(G[16 * c + j], G[16 * c + j + 1]), w2), v[j], v[j + 1]);
+                        tmem_st16(tq + kKv + col0 + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v));
+                    }
+                tmem_wait_st();
+                tc_fence_before();
+            };
             epi_sync(true);  // the tables' last readers are done
             if (tid <= kChunk) pw[tid] = power(g, tid);
-            if (tid < 32) back[tid] = power(g, 31 - tid);
-            const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
-            bool has_g = !ENDS && (p.g0 || (t.n > 0 && t.seg != first_seg));
+            if (tid < 160) {
+                const int d = REV ? tid - 32 : 127 - tid;
+                factors[tid] = factors[176 + tid + 1] = d < 0 ? 0.f : power(g, d) * p.scale;
+            }
             // ---- the state before this segment
 #pragma unroll
             for (int j = 0; j < 32 * W; ++j) G[j] = 0.f;
-            if (!ENDS && has_g && live) {
+            if (has_g && live) {
                 if (p.g0 && srow < p.da) {
                     // tokens that come before, and one step more into the chunk's terms
                     const int64_t before = REV ? t.len - min(t.len, (int64_t)(t.first + t.n) * kChunk) : (int64_t)t.first * kChunk;
@@ -286,103 +597,91 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 }
                 if (t.n > 0)
                     for (int u = REV ? t.seg + 1 : 0; REV ? u <= first_seg : u < t.seg; ++u) {
-                        const float w = power(g, (int64_t)((REV ? u - t.seg : t.seg - u) - 1) * p.per_seg * kChunk);
-                        const float4* e = reinterpret_cast<const float4*>(p.ends + (((int64_t)t.bh * p.nseg + u) * kState + srow) * kState + col0);
+                        // its units, of p.unit chunks each (forwards to the segment's end, backwards to the last token)
+                        const int from = u * p.per_seg, to = min(from + p.per_seg, REV ? t.active : p.chunks), here = REV ? t.first + t.n : t.first;
+                        for (int v = 0; from + v * p.unit < to; ++v) {
+                            const float w = power(g, (int64_t)(REV ? from + v * p.unit - here : here - min(from + (v + 1) * p.unit, to)) * kChunk);
+                            const float4* e = reinterpret_cast<const float4*>(p.ends + ((((int64_t)t.bh * p.nseg + u) * p.units + v) * kState + srow) * kState + col0);
 #pragma unroll
-                        for (int j = 0; j < 8 * W; ++j) {
-                            const float4 v = e[j];
-                            G[4 * j] = __fmaf_rn(w, v.x, G[4 * j]), G[4 * j + 1] = __fmaf_rn(w, v.y, G[4 * j + 1]);
-                            G[4 * j + 2] = __fmaf_rn(w, v.z, G[4 * j + 2]), G[4 * j + 3] = __fmaf_rn(w, v.w, G[4 * j + 3]);
+                            for (int j = 0; j < 8 * W; ++j) {
+                                const float4 x = e[j];
+                                G[4 * j] = __fmaf_rn(w, x.x, G[4 * j]), G[4 * j + 1] = __fmaf_rn(w, x.y, G[4 * j + 1]);
+                                G[4 * j + 2] = __fmaf_rn(w, x.z, G[4 * j + 2]), G[4 * j + 3] = __fmaf_rn(w, x.w, G[4 * j + 3]);
+                            }
                         }
                     }
             }
-            float unscale = 1.f;
-            // G as an operand: rows of dc columns, in fp16 times a power of two that keeps the largest in range.
-            auto put_state = [&] {
-                float s = 1.f;
-                if constexpr (F16) {
-                    float m = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 32 * W; ++j) m = fmaxf(m, fabsf(G[j]));
-                    const uint32_t wm = __reduce_max_sync(0xffffffffu, live ? __float_as_uint(m) : 0u);
-                    const int slot = puts++ & 1;
-                    if (lane == 0) atomicMax(&gmax[slot], wm);
-                    epi_sync(true);
-                    s = range_scale(gmax[slot]);
-                    if (tid == 0) gmax[slot ^ 1] = 0;
-                    unscale = 1.f / s;
-                }
-                if (live) {
-                    uint8_t* const dst = gop + (W == 2 ? half * kState * 128 : 0) + srow * 128;
-#pragma unroll
-                    for (int j = 0; j < 4 * W; ++j) {
-                        const float* v = &G[8 * j];
-                        const int ch = (W == 1 ? half * 4 : 0) + j;
-                        sts16(dst + ((ch ^ (srow & 7)) << 4), make_uint4(pack2<T>(v[0] * s, v[1] * s), pack2<T>(v[2] * s, v[3] * s),
-                                                                        pack2<T>(v[4] * s, v[5] * s), pack2<T>(v[6] * s, v[7] * s)));
-                    }
-                }
-                fence_async_smem();
-            };
-            if constexpr (!ENDS) {
+            epi_sync(true);  // the tables are written
+            {
                 if (t.n > 0) {
-                    if (has_g) put_state();
+                    if (has_g) put_state(0);
                     arrive(g_ready);
                 }
             }
-            epi_sync(true);  // the tables are written
             // ---- chunks
             for (int k = 0; k < t.n; ++k, ++cc, n += kTiles) {
-                const int chunk = REV ? t.first + t.n - 1 - k : t.first + k;
-                const int L = (int)min((int64_t)kChunk, t.len - (int64_t)chunk * kChunk);
+                const int chunk = chunk_of(k), L = tokens_of(k), e = last_of(k);
                 const int nk = n + kTiles - 2, nv = nk + 1;
-                uint8_t* const tk = ring + nk % kRing * kTile;
-                // The last state is that after the last token, not decayed further.
-                const int e = !REV && !ENDS && p.gout && chunk == t.active - 1 ? 1 : 0;
-                ok = mbar_wait(&full[nk % kRing], nk / kRing & 1) && ok;
-                if constexpr (!ENDS) {
-                    ok = mbar_wait(s_full, cc & 1) && ok;  // the scores are done: b may be overwritten
+                // ---- b_j times its power of l, in two parts
+                uint8_t *hi = ring + nk % kRing * kTile + kr * 128, *lo = low + kr * 128;
+                if (W == 2) hi += kpart * kBlock, lo += kpart * kBlock;
+                uint4 x[4];
+                int at[4];
+                const float w = kr >= L ? 0.f : REV ? pw[kr + 1] : pw[L - e - kr];
+                const T w0 = Elem<T>::store(w);
+                const uint32_t wh = pack2<T>(w, w), nh = wh ^ 0x80008000u, nl = pack2<T>(Elem<T>::load(w0) - w, Elem<T>::load(w0) - w);
+                auto fetch = [&](int j0) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        at[j] = ((W == 1 ? kpart * 4 + j : (j0 + j) ^ (kpart << 2)) ^ (kr & 7)) << 4;
+                        x[j] = *reinterpret_cast<const uint4*>(hi + at[j]);
+                    }
+                };
+                ok = wait_for(&full[nk % kRing], nk / kRing & 1) && ok;
+                fetch(0);
+                {
+                    ok = wait_for(s_full, cc & 1) && ok;  // the scores are done: b may be overwritten
                     if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    if (!(ok = epi_sync(ok))) break;  // and the last output has left the staging
+                    if (!(ok = epi_sync(ok))) break;      // and the last output has left the staging
                 }
                 tc_fence_after();
-                {  // b_j times its power of l, in two parts
-                    const int r = tid >> 1, part = tid & 1;
-                    const float w = r >= L ? 0.f : REV ? pw[r + 1] : pw[L - e - r];
-                    uint8_t *hi = tk, *lo = low;
-                    if (W == 2) hi += part * kBlock, lo += part * kBlock;
-                    hi += r * 128, lo += r * 128;
 #pragma unroll
-                    for (int j = 0; j < 4 * W; ++j) {
-                        const int ch = W == 1 ? part * 4 + j : j ^ (part << 2), at = (ch ^ (r & 7)) << 4;
-                        uint4 v = *reinterpret_cast<const uint4*>(hi + at), l;
-                        uint32_t *x = reinterpret_cast<uint32_t*>(&v), *y = reinterpret_cast<uint32_t*>(&l);
+                for (int j0 = 0; j0 < 4 * W; j0 += 4) {
+                    if (j0 > 0) fetch(j0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+                        uint32_t h[4], l[4];
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            float2 f = unpack2<T>(x[q]);
-                            f.x *= w, f.y *= w;
-                            x[q] = pack2<T>(f.x, f.y);
-                            const float2 h = unpack2<T>(x[q]);
-                            y[q] = pack2<T>(f.x - h.x, f.y - h.y);
+                            // high = b wh rounded; b wh - high is exact (it has no more bits than b); b wl joins with one rounding.
+                            // The second part is negated.
+                            h[q] = mul16x2<T>(v[q], wh);
+                            l[q] = fma16x2<T>(v[q], nl, fma16x2<T>(v[q], nh, h[q]));
                         }
-                        if (r >= L) v = l = make_uint4(0u, 0u, 0u, 0u);
-                        sts16(hi + at, v);
-                        sts16(lo + at, l);
+                        sts16(hi + at[j], make_uint4(h[0], h[1], h[2], h[3]));
+                        sts16(lo + at[j], make_uint4(l[0], l[1], l[2], l[3]));
                     }
                 }
                 if (L < kChunk) {  // rows past the sequence: zeros, whatever they hold
-                    ok = mbar_wait(&full[nv % kRing], nv / kRing & 1) && ok;
+                    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+                    if (kr >= L)
+                        for (int j = 0; j < 4 * W; ++j) {
+                            const int here = ((W == 1 ? kpart * 4 + j : j) ^ (kr & 7)) << 4;  // (what this thread has written)
+                            sts16(hi + here, none), sts16(lo + here, none);
+                        }
+                    ok = wait_for(&full[nv % kRing], nv / kRing & 1) && ok;
                     uint8_t* const tv = ring + nv % kRing * kTile;
                     for (int j = tid; j < (kChunk - L) * 8 * W; j += kEpi) {
                         const int r = L + j / (8 * W), u = j % (8 * W);
-                        sts16(tv + (u >> 3) * kBlock + r * 128 + ((u & 7) << 4), make_uint4(0u, 0u, 0u, 0u));
+                        sts16(tv + (u >> 3) * kBlock + r * 128 + ((u & 7) << 4), none);
                     }
                 }
                 fence_async_smem();
                 arrive(k_ready);
-                if constexpr (!ENDS) {
+                {
                     // ---- weighted scores: row `row`, columns 64 half on, in blocks of 32
-#pragma unroll
+#pragma unroll 1
                     for (int bl = 0; bl < 2; ++bl) {
                         const int blk = half * 2 + bl;
                         uint32_t u[16];
@@ -392,49 +691,39 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                         } else {
                             float v[32];
                             tmem_ld32(tq + blk * 32, v);
+                            const float2* f = reinterpret_cast<const float2*>(frow + blk * 32);
                             tmem_wait_ld();
                             reg_fence(v);
-                            if (blk == quad) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) {
-                                    const int d = REV ? j - lane : lane - j;
-                                    v[j] = d >= 0 ? v[j] * (pw[max(d, 0)] * p.scale) : 0.f;
-                                }
-                            } else {
-                                const float rf = pw[REV ? blk * 32 - row : row - blk * 32 - 31] * p.scale;
-                                const uint64_t rf2 = pk2(rf, rf);
-                                const float4* cf = reinterpret_cast<const float4*>(REV ? pw : back);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const float4 f = cf[j];
-                                    upk2(mul2(mul2(pk2(v[4 * j], v[4 * j + 1]), rf2), pk2(f.x, f.y)), v[4 * j], v[4 * j + 1]);
-                                    upk2(mul2(mul2(pk2(v[4 * j + 2], v[4 * j + 3]), rf2), pk2(f.z, f.w)), v[4 * j + 2], v[4 * j + 3]);
-                                }
+                            for (int j = 0; j < 16; ++j) {
+                                const float2 c = f[j];
+                                float a, b;
+                                upk2(mul2(pk2(v[2 * j], v[2 * j + 1]), pk2(c.x, c.y)), a, b);
+                                u[j] = pack2<T>(a, b);
                             }
-                            if (REV && L < kChunk) {
+                            if (L < kChunk) {  // (a product with what lies past the sequence may not be finite)
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] = blk * 32 + j < L ? v[j] : 0.f;
+                                for (int j = 0; j < 16; ++j) u[j] &= keep_low(16 * (L - blk * 32) - 32 * j);
                             }
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) u[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
                         }
                         tmem_st16(tq + half * 64 + bl * 16, u);
                     }
                     if (has_g) {  // what the state gives, times the row's power
-                        ok = mbar_wait(qg_full, qg++ & 1) && ok;
+                        ok = wait_for(qg_full, qg++ & 1) && ok;
                         tc_fence_after();
                         const int d = REV ? L - 1 - row : row;
                         const float w = (d >= 0 ? pw[d] : 0.f) * p.scale * unscale;
+                        const uint64_t w2 = pk2(w, w);
 #pragma unroll
-                        for (int c = 0; c < 2 * W; ++c) {
-                            if (col0 + 16 * c < p.nb) {
-                                float v[16];
-                                tmem_ld16(tq + kO + col0 + 16 * c, v);
+                        for (int c = 0; c < W; ++c) {
+                            if (col0 + 32 * c < p.nb) {
+                                float v[32];
+                                tmem_ld32(tq + kO + col0 + 32 * c, v);
                                 tmem_wait_ld();
                                 reg_fence(v);
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] *= w;
-                                tmem_st16(tq + kO + col0 + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v));
+                                for (int j = 0; j < 16; ++j) upk2(mul2(pk2(v[2 * j], v[2 * j + 1]), w2), v[2 * j], v[2 * j + 1]);
+                                tmem_st32(tq + kO + col0 + 32 * c, v);
                             }
                         }
                     }
@@ -443,47 +732,43 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     arrive(p_ready);
                 }
                 // ---- the state after this chunk
-                ok = mbar_wait(kv_full, cc & 1) && ok;
+                ok = wait_for(kv_full, cc & 1) && ok;
                 tc_fence_after();
-                {
-                    const float w = pw[L - e];
 #pragma unroll
-                    for (int c = 0; c < 2 * W; ++c) {
-                        if (col0 + 16 * c < p.nb) {
-                            float v[16];
-                            tmem_ld16(tq + kKv + col0 + 16 * c, v);
-                            tmem_wait_ld();
-                            reg_fence(v);
+                for (int c = 0; c < W; ++c)
+                    if (col0 + 32 * c < p.nb) tmem_ld32(tq + kKv + col0 + 32 * c, reinterpret_cast<float(&)[32]>(G[32 * c]));
+                tmem_wait_ld();
+                reg_fence(G);
+                if (p.nb & 16) {  // the last columns of 32 are nobody's
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) G[16 * c + j] = __fmaf_rn(G[16 * c + j], w, v[j]);
-                        }
-                    }
+                    for (int j = 16; j < 32 * W; j += 32)
+#pragma unroll
+                        for (int m = 0; m < 16; ++m)
+                            if (col0 + j >= p.nb) G[j + m] = 0.f;
                 }
                 has_g = true;
-                if constexpr (ENDS) {
-                    tc_fence_before();
-                    if (!(ok = epi_sync(ok))) break;  // low may be written again, and the accumulator
-                    continue;
-                }
-                if (k + 1 < t.n) put_state();
+                if (k + 1 < t.n) put_state(k + 1);
+                
                 // ---- the output
-                ok = mbar_wait(o_full, cc & 1) && ok;
+                ok = wait_for(o_full, cc & 1) && ok;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 2 * W; ++c) {
-                    if (col0 + 16 * c < p.nb) {
-                        float v[16];
-                        tmem_ld16(tq + kO + col0 + 16 * c, v);
+                for (int c = 0; c < W; ++c) {
+                    if (col0 + 32 * c < p.nb) {
+                        float v[32];
+                        tmem_ld32(tq + kO + col0 + 32 * c, v);
                         tmem_wait_ld();
                         reg_fence(v);
-                        uint4 o[2];
-                        uint32_t* u = reinterpret_cast<uint32_t*>(o);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) u[j] = row < L ? pack2<T>(v[2 * j], v[2 * j + 1]) : 0u;
-                        const int ch = (W == 1 ? half * 4 : 0) + 2 * c;
                         uint8_t* const dst = low + (W == 2 ? half * kBlock : 0) + row * 128;
-                        sts16(dst + ((ch ^ (row & 7)) << 4), o[0]);
-                        sts16(dst + (((ch + 1) ^ (row & 7)) << 4), o[1]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float* x = &v[8 * j];
+                            sts16(dst + ((((W == 1 ? half * 4 : 0) + 4 * c + j) ^ (row & 7)) << 4),
+                                  make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])));
+                        }
+                        if (L < kChunk && row >= L)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) sts16(dst + ((((W == 1 ? half * 4 : 0) + 4 * c + j) ^ (row & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
                     }
                 }
                 tc_fence_before();
@@ -505,13 +790,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 }
             }
             if (!ok) break;
-            if constexpr (ENDS) {
-                if (t.n > 0 && live) {
-                    float4* e = reinterpret_cast<float4*>(p.ends + (((int64_t)t.bh * p.nseg + t.seg) * kState + srow) * kState + col0);
-#pragma unroll
-                    for (int j = 0; j < 8 * W; ++j) e[j] = make_float4(G[4 * j], G[4 * j + 1], G[4 * j + 2], G[4 * j + 3]);
-                }
-            } else {
+            {
                 // ---- rows past the sequence in this segment's whole chunks
                 const int end = min(t.first + p.per_seg, p.chunks);
                 const int64_t z0 = (int64_t)max(t.first + t.n, t.first) * kChunk, z1 = min((int64_t)end * kChunk, (int64_t)p.t);
@@ -528,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 }
             }
         }
-        if (!ENDS && tid == 0 && p.tma_out) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (tid == 0 && p.tma_out) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     if (!ok) atomicExch(&g_decay_status, (int)LF_ERR_TIMEOUT);
     tc_fence_before();
@@ -671,29 +950,40 @@ bool encode_heads(CUtensorMap* map, const Heads& x, const Sizes& z, int dtype) {
                                    (cuuint64_t)(z.b > 1 ? x.sb * 2 : 16)};
     const cuuint32_t box[4] = {64, 1, kChunk, 1};
     return encode_tiled(map, dtype == LF_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.p, dims,
-                        strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+                        strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                        x.d > 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B);  // (a row, not its neighbours')
 }
 
 int blocks_of(int64_t da, int64_t dc) { return da <= 64 && dc <= 64 ? 1 : 2; }
 
-// Segments per sequence.
-int segments(const Sizes& z, int w) {
+// Segments per sequence, and units of the sums that segments need of those before them.
+struct Deal {
+    int nseg, per_seg, unit, units;
+};
+Deal deal(const Sizes& z, int w) {
     const int64_t chunks = (z.t + kChunk - 1) / kChunk, bh = z.b * z.h, slots = (int64_t)num_sms() * (w == 1 ? 2 : 1);
     double least = 1e30;
-    int best = 1;
+    int64_t best = 1;
     for (int64_t n = 1; n <= std::min<int64_t>(chunks, 64); ++n) {
-        const int64_t per = (chunks + n - 1) / n, segs = (chunks + per - 1) / per;
-        if (segs != n) continue;
-        const auto pass = [&](int64_t items, double chunk) { return (double)((items + slots - 1) / slots) * (per * chunk + 1.0); };
-        const double t = pass(bh * n, 1.0) + (n > 1 ? pass(bh * (n - 1), 0.5) + 2.0 : 0.0);
-        if (t < least) least = t, best = (int)n;
+        const int64_t per = (chunks + n - 1) / n;
+        if ((chunks + per - 1) / per != n) continue;
+        // In times of a chunk: rounds of blocks, and a launch that reads b and c of all segments but one.
+        const double t = (double)((bh * n + slots - 1) / slots) * (per + 1.0) + (n > 1 ? 0.5 * (double)(bh * (n - 1) * per) / slots + 3.0 : 0.0);
+        if (t < least) least = t, best = n;
     }
-    return best;
+    Deal d{};
+    d.nseg = (int)best, d.per_seg = (int)((chunks + best - 1) / best), d.unit = d.per_seg, d.units = 1;
+    if (best > 1) {  // units so short that every slot has work, and not shorter than 4 chunks
+        const int64_t want = std::max<int64_t>(1, 2 * slots / (bh * (best - 1)));
+        d.unit = (int)std::max<int64_t>(std::min<int64_t>(4, d.per_seg), (d.per_seg + want - 1) / want);
+        d.units = (d.per_seg + d.unit - 1) / d.unit;
+    }
+    return d;
 }
 
 size_t ends_bytes(const Sizes& z, int w) {
-    const int n = segments(z, w);
-    return n > 1 ? (size_t)z.b * z.h * n * (64 * w) * (64 * w) * 4 : 0;
+    const Deal d = deal(z, w);
+    return d.nseg > 1 ? (size_t)z.b * z.h * d.nseg * d.units * (64 * w) * (64 * w) * 4 : 0;
 }
 
 uint32_t idesc(int dtype, bool a_mn, bool b_mn, int m, int n) {
@@ -710,12 +1000,19 @@ void allow_smem(int bytes) {
     std::call_once(once[dev & 63], [&] { cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
 }
 
-template <typename T, int W, bool REV, bool ENDS>
-void launch_mix(const MixArgs& a, cudaStream_t st) {
-    constexpr auto kernel = decay_mix_kernel<T, W, REV, ENDS>;
+template <typename T, int W, bool REV>
+void launch_mix(MixArgs a, int64_t bh, cudaStream_t st) {
+    const int slots = num_sms() * (W == 1 ? 2 : 1);
+    if (a.nseg > 1) {
+        constexpr auto sums = decay_ends_kernel<T, W, REV>;
+        allow_smem<sums>(ends_smem<W>());
+        a.items = (int)(bh * (a.nseg - 1) * a.units);
+        launch_early(sums, (unsigned)std::min(a.items, slots), kThreads, ends_smem<W>(), 1, st, a);
+    }
+    constexpr auto kernel = decay_mix_kernel<T, W, REV>;
     allow_smem<kernel>(mix_smem<W>());
-    const int grid = std::min(a.items, num_sms() * (W == 1 ? 2 : 1));
-    launch_early(kernel, (unsigned)grid, kThreads, mix_smem<W>(), 1, st, a);
+    a.items = (int)(bh * a.nseg);
+    launch_early(kernel, (unsigned)std::min(a.items, slots), kThreads, mix_smem<W>(), 1, st, a);
 }
 
 struct Mix {
@@ -734,8 +1031,8 @@ int run_mix(const Mix& m, const Sizes& z, const float* log_decay, const int64_t*
     p.o = const_cast<void*>(m.out.p), p.o_sb = m.out.sb, p.o_sh = m.out.sh, p.o_st = m.out.st;
     p.heads = (int)z.h, p.t = (int)z.t, p.da = (int)m.a.d, p.dc = (int)m.c.d;
     p.chunks = (int)((z.t + kChunk - 1) / kChunk);
-    p.nseg = segments(z, w);
-    p.per_seg = (p.chunks + p.nseg - 1) / p.nseg;
+    const Deal d = deal(z, w);
+    p.nseg = d.nseg, p.per_seg = d.per_seg, p.unit = d.unit, p.units = d.units;
     p.g0_row = m.transposed ? 1 : p.dc, p.g0_col = m.transposed ? p.da : 1;
     p.scale = (float)scale, p.g0_scale = m.rev ? (float)(1.0 / scale) : 1.f, p.gout_scale = m.rev ? (float)scale : 1.f;
     p.ksteps = (p.da + 15) / 16, p.nb = (p.dc + 15) / 16 * 16;
@@ -745,13 +1042,13 @@ int run_mix(const Mix& m, const Sizes& z, const float* log_decay, const int64_t*
     if (!encode_heads(&p.a, m.a, z, dtype) || !encode_heads(&p.b, m.b, z, dtype) || !encode_heads(&p.c, m.c, z, dtype)) return LF_ERR_CUDA;
     if (p.tma_out && !encode_heads(&p.out, m.out, z, dtype)) return LF_ERR_CUDA;
     const int64_t bh = z.b * z.h;
-#define LFB_MIX(T, W, REV)                                                                             {                                                                                                      if (p.nseg > 1) p.items = (int)(bh * (p.nseg - 1)), launch_mix<T, W, REV, true>(p, st);            p.items = (int)(bh * p.nseg), launch_mix<T, W, REV, false>(p, st);                             }
+#define LFB_MIX(T, W) (m.rev ? launch_mix<T, W, true>(p, bh, st) : launch_mix<T, W, false>(p, bh, st))
     if (dtype == LF_F16) {
-        if (w == 1) { if (m.rev) LFB_MIX(__half, 1, true) else LFB_MIX(__half, 1, false) }
-        else { if (m.rev) LFB_MIX(__half, 2, true) else LFB_MIX(__half, 2, false) }
+        if (w == 1) LFB_MIX(__half, 1);
+        else LFB_MIX(__half, 2);
     } else {
-        if (w == 1) { if (m.rev) LFB_MIX(__nv_bfloat16, 1, true) else LFB_MIX(__nv_bfloat16, 1, false) }
-        else { if (m.rev) LFB_MIX(__nv_bfloat16, 2, true) else LFB_MIX(__nv_bfloat16, 2, false) }
+        if (w == 1) LFB_MIX(__nv_bfloat16, 1);
+        else LFB_MIX(__nv_bfloat16, 2);
     }
 #undef LFB_MIX
     return check_launch("decay_attention");

@@ -28,7 +28,8 @@ inline EncodeFn encode_fn() {
 
 // Whether the map of `rank` dimensions (innermost first, strides in bytes from the second on) could be made.
 inline bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* p, const cuuint64_t* dims,
-                         const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+                         const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle,
+                         CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
     const cuuint32_t step[5] = {1, 1, 1, 1, 1};
     EncodeFn fn = encode_fn();
     if (!fn) {
@@ -37,7 +38,7 @@ inline bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, c
     }
     auto call = [&] {
         return fn(map, type, (cuuint32_t)rank, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
     CUresult r = call();
     if (r == CUDA_ERROR_INVALID_CONTEXT) {  // the first call of a host thread (an autograd worker): bind the device's context
