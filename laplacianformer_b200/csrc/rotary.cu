@@ -10,6 +10,7 @@
 // product at position 10^6 is off by up to 0.06 radians), then the sine and
 // cosine of the fraction in 32 bits.
 #include <algorithm>
+#include <mutex>
 
 #include "lf_common.cuh"
 
@@ -17,8 +18,8 @@ namespace lfb {
 namespace {
 
 constexpr int kPairs = 128;      // pairs that a head may have
-constexpr int kAngles = 2048;    // sines and cosines that a block holds
-constexpr int kUnits = 4;        // units of a thread in flight
+constexpr int kAngles = 512;     // sines and cosines of a tile
+constexpr int kUnits = 4;        // units of a thread in a tile
 
 struct RotaryArgs {
     const void* x[2];
@@ -27,7 +28,7 @@ struct RotaryArgs {
     const int64_t* positions;
     int64_t position_stride, offset, tokens;   // tokens of all sequences
     double turns[kPairs];                      // frequency / 2 pi
-    Divisor per_token, per_head, per_pair;     // units of a token, of a head; pairs
+    Divisor per_token, per_head, per_pair, per_t;  // units of a token, of a head; pairs; tokens of a sequence
     int heads[2], t, size, pairs, rotated, per_block;
     float magnitude, sign;
 };
@@ -36,89 +37,152 @@ template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Vec {
     T v[VEC];
 };
+template <typename T, int VEC>
+constexpr int rotary_stages() {
+    return sizeof(T) * VEC == 16 ? 3 : 0;
+}
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
 
-// A unit is VEC pairs (HALVES), VEC/2 pairs (neighbours; one pair when VEC is 1), or VEC copied elements.
+// A unit is VEC pairs (HALVES), VEC/2 pairs (neighbours; one pair when VEC is 1), or VEC copied elements.  A block walks
+// over tiles of `per_block` tokens, up to kUnits units to a thread.  With vectors of 16 bytes the units of the next tiles
+// are on their way to places of each thread's own in shared memory while one is turned.
 template <typename T, int VEC, bool HALVES>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryArgs p) {
     constexpr int PAIRS = HALVES ? VEC : VEC == 1 ? 1 : VEC / 2;   // of a unit
     constexpr bool TWO = HALVES || VEC == 1;                       // a unit's pairs lie in two places
-    __shared__ float2 cs[kAngles];
+    constexpr int S = rotary_stages<T, VEC>();
+    using V = Vec<T, VEC>;
+    extern __shared__ __align__(16) uint8_t staged[];              // [stage][unit][place][thread]
+    __shared__ __align__(16) float2 table[2][kAngles];             // cosine and sine of a tile's tokens, by turns
     grid_release();
     grid_wait();
-    const int64_t tok0 = (int64_t)blockIdx.x * p.per_block;
-    const int toks = (int)min((int64_t)p.per_block, p.tokens - tok0), units = toks * (int)p.per_token.d;
-    const int turning = p.rotated;                                 // units of a head that turn; the others are copied
-    Vec<T, VEC> a[kUnits], b[kUnits];
-    int off[kUnits], pair[kUnits];
-    T* dst[kUnits];
-    // Where the unit's elements are: its (first) place, how much further the second is (0: none), and its first angle (-1: copied).
-    auto fetch = [&](int i0) {
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            const int u = i0 + i * 256;
-            off[i] = -1;
-            if (u >= units) continue;
-            const int tok = p.per_token.of(u), r = u - tok * (int)p.per_token.d;
-            int h = p.per_head.of(r);
-            const int e = r - h * (int)p.per_head.d;
-            const int which = h >= p.heads[0] ? 1 : 0;
-            if (which) h -= p.heads[0];
-            const int64_t n = tok0 + tok, s = n / p.t, t = n - s * p.t;
-            int c;
-            if (e < turning) {
-                pair[i] = tok * p.pairs + e * PAIRS;
-                c = HALVES ? e * VEC : e * PAIRS * 2;
-                off[i] = HALVES ? p.pairs : VEC == 1 ? 1 : 0;
-            } else {
-                pair[i] = -1;
-                c = 2 * p.pairs + (e - turning) * VEC;
-                off[i] = 0;
-            }
-            const T* src = (const T*)p.x[which] + s * p.sb[which] + h * p.sh[which] + t * p.st[which] + c;
-            dst[i] = (T*)p.y[which] + (n * p.heads[which] + h) * p.size + c;
-            a[i] = *reinterpret_cast<const Vec<T, VEC>*>(src);
-            if (TWO && off[i]) b[i] = *reinterpret_cast<const Vec<T, VEC>*>(src + off[i]);
-        }
+    const int tiles = (int)((p.tokens + p.per_block - 1) / p.per_block);
+    // Unit u of the tile that starts at token tok0: its elements, how much further the second place is (0: none), its
+    // first angle (-1: copied).
+    struct Unit {
+        const T* src;
+        T* dst;
+        int off, pair;
     };
-    fetch(threadIdx.x);  // on their way while the angles are computed
-    for (int i = threadIdx.x; i < toks * p.pairs; i += 256) {
-        const int tok = p.per_pair.of(i), k = i - tok * p.pairs;
-        const int64_t n = tok0 + tok, s = n / p.t, t = n - s * p.t;
-        const int64_t pos = p.positions ? p.positions[s * p.position_stride + t] : p.offset + t;
-        double turn = (double)pos * p.turns[k];
-        turn -= rint(turn);
-        float sn, c;
-        sincospif(2.f * (float)turn, &sn, &c);
-        cs[i] = make_float2(c * p.magnitude, sn * p.magnitude * p.sign);
+    auto unit_of = [&](int tok0, int u) {
+        Unit x;
+        const int tok = p.per_token.of(u), r = u - tok * (int)p.per_token.d;
+        int h = p.per_head.of(r);
+        const int e = r - h * (int)p.per_head.d;
+        const int which = h >= p.heads[0] ? 1 : 0;
+        if (which) h -= p.heads[0];
+        const int n = tok0 + tok, s = p.per_t.of(n), t = n - s * p.t;
+        int c;
+        if (e < p.rotated) {
+            x.pair = tok * p.pairs + e * PAIRS;
+            c = HALVES ? e * VEC : e * PAIRS * 2;
+            x.off = HALVES ? p.pairs : VEC == 1 ? 1 : 0;
+        } else {
+            x.pair = -1;
+            c = 2 * p.pairs + (e - p.rotated) * VEC;
+            x.off = 0;
+        }
+        x.src = (const T*)p.x[which] + s * p.sb[which] + h * p.sh[which] + t * p.st[which] + c;
+        x.dst = (T*)p.y[which] + ((int64_t)n * p.heads[which] + h) * p.size + c;
+        return x;
+    };
+    auto units_in = [&](int tok0) { return min(p.per_block, (int)(p.tokens - tok0)) * (int)p.per_token.d; };
+    auto place = [&](int stage, int i, int j) { return staged + (((stage * kUnits + i) * 2 + j) * 256 + threadIdx.x) * 16; };
+    auto fetch = [&](int64_t tile, int stage) {
+        if (tile < tiles) {
+            const int tok0 = (int)tile * p.per_block, units = units_in(tok0);
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int u = threadIdx.x + i * 256;
+                if (u >= units) break;
+                const Unit x = unit_of(tok0, u);
+                copy16(place(stage, i, 0), x.src);
+                if (TWO && x.off) copy16(place(stage, i, 1), x.src + x.off);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (S > 0) {
+#pragma unroll
+        for (int k = 0; k + 1 < S; ++k) fetch((int64_t)blockIdx.x + (int64_t)k * gridDim.x, k);
     }
-    __syncthreads();
-    for (int i0 = threadIdx.x; i0 < units; i0 += kUnits * 256) {
-        if (i0 != threadIdx.x) fetch(i0);
+    int stage = 0, turn = 0;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+        const int tok0 = (int)tile * p.per_block, units = units_in(tok0), toks = min(p.per_block, (int)(p.tokens - tok0));
+        float2* const cs = table[turn];
+        for (int i = threadIdx.x; i < toks * p.pairs; i += 256) {
+            const int tok = p.per_pair.of(i), k = i - tok * p.pairs;
+            const int n = tok0 + tok, s = p.per_t.of(n), t = n - s * p.t;
+            const int64_t pos = p.positions ? p.positions[(int64_t)s * p.position_stride + t] : p.offset + t;
+            double turns = (double)pos * p.turns[k];
+            turns -= rint(turns);
+            float sn, c;
+            sincospif(2.f * (float)turns, &sn, &c);
+            cs[i] = make_float2(c * p.magnitude, sn * p.magnitude * p.sign);
+        }
+        if constexpr (S > 0) {
+            fetch(tile + (int64_t)(S - 1) * gridDim.x, stage == 0 ? S - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(S > 0 ? S - 1 : 0) : "memory");
+        }
+        __syncthreads();  // the angles are there; whoever still reads the last tile's has the other table
+        for (int i0 = 0; i0 * 256 < units; i0 += kUnits) {
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            if (off[i] < 0) continue;
-            if (pair[i] >= 0) {
-                const float2* f = cs + pair[i];
-                if constexpr (TWO) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const float x = Elem<T>::load(a[i].v[j]), y = Elem<T>::load(b[i].v[j]);
-                        a[i].v[j] = Elem<T>::store(x * f[j].x - y * f[j].y);
-                        b[i].v[j] = Elem<T>::store(x * f[j].y + y * f[j].x);
-                    }
+            for (int i = 0; i < kUnits; ++i) {
+                const int u = threadIdx.x + (i0 + i) * 256;
+                if (u >= units) break;
+                const Unit x = unit_of(tok0, u);
+                V a, b;
+                if constexpr (S > 0) {
+                    a = *reinterpret_cast<const V*>(place(stage, i, 0));
+                    if (TWO && x.off) b = *reinterpret_cast<const V*>(place(stage, i, 1));
                 } else {
+                    a = *reinterpret_cast<const V*>(x.src);
+                    if (TWO && x.off) b = *reinterpret_cast<const V*>(x.src + x.off);
+                }
+                if (x.pair >= 0) {
+                    const float2* f = cs + x.pair;
+                    if constexpr (TWO) {
 #pragma unroll
-                    for (int j = 0; j < VEC / 2; ++j) {
-                        const float x = Elem<T>::load(a[i].v[2 * j]), y = Elem<T>::load(a[i].v[2 * j + 1]);
-                        a[i].v[2 * j] = Elem<T>::store(x * f[j].x - y * f[j].y);
-                        a[i].v[2 * j + 1] = Elem<T>::store(x * f[j].y + y * f[j].x);
+                        for (int j = 0; j < VEC; ++j) {
+                            const float p0 = Elem<T>::load(a.v[j]), p1 = Elem<T>::load(b.v[j]);
+                            a.v[j] = Elem<T>::store(p0 * f[j].x - p1 * f[j].y);
+                            b.v[j] = Elem<T>::store(p0 * f[j].y + p1 * f[j].x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VEC / 2; ++j) {
+                            const float p0 = Elem<T>::load(a.v[2 * j]), p1 = Elem<T>::load(a.v[2 * j + 1]);
+                            a.v[2 * j] = Elem<T>::store(p0 * f[j].x - p1 * f[j].y);
+                            a.v[2 * j + 1] = Elem<T>::store(p0 * f[j].y + p1 * f[j].x);
+                        }
                     }
                 }
+                *reinterpret_cast<V*>(x.dst) = a;
+                if (TWO && x.off) *reinterpret_cast<V*>(x.dst + x.off) = b;
             }
-            *reinterpret_cast<Vec<T, VEC>*>(dst[i]) = a[i];
-            if (TWO && off[i]) *reinterpret_cast<Vec<T, VEC>*>(dst[i] + off[i]) = b[i];
         }
+        if constexpr (S > 0) stage = stage + 1 == S ? 0 : stage + 1;
     }
+}
+
+template <typename T, int VEC, bool HALVES>
+void launch_tiles(const RotaryArgs& p, int64_t tiles, cudaStream_t st) {
+    constexpr auto kernel = rotary_kernel<T, VEC, HALVES>;
+    constexpr int smem = rotary_stages<T, VEC>() * kUnits * 2 * 256 * 16;
+    static std::once_flag once[64];
+    static int per_sm[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    dev &= 63;
+    std::call_once(once[dev], [&] {
+        int v = 0;
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, kernel, 256, smem) != cudaSuccess || v < 1) v = 1;
+        per_sm[dev] = v;
+    });
+    launch_early(kernel, (unsigned)std::min<int64_t>(tiles, (int64_t)per_sm[dev] * num_sms()), 256, smem, 1, st, p);
 }
 
 template <typename T, bool HALVES>
@@ -127,12 +191,15 @@ void launch_rotary(RotaryArgs& p, bool vec, cudaStream_t st) {
     const int v = vec ? V : 1, pairs = HALVES ? v : vec ? v / 2 : 1;
     p.rotated = p.pairs / pairs;
     const int per_head = p.rotated + (p.size - 2 * p.pairs) / v;
-    p.per_head = Divisor(per_head), p.per_token = Divisor(per_head * (p.heads[0] + p.heads[1])), p.per_pair = Divisor(std::max(1, p.pairs));
-    // A block's threads get kUnits units each where the angles allow it.
-    p.per_block = std::max(1, std::min(kAngles / std::max(1, p.pairs), 256 * kUnits / (int)p.per_token.d));
-    const unsigned grid = (unsigned)((p.tokens + p.per_block - 1) / p.per_block);
-    if (vec) launch_early(rotary_kernel<T, V, HALVES>, grid, 256, 0, 1, st, p);
-    else launch_early(rotary_kernel<T, 1, HALVES>, grid, 256, 0, 1, st, p);
+    p.per_head = Divisor(per_head), p.per_token = Divisor(per_head * (p.heads[0] + p.heads[1])), p.per_pair = Divisor(std::max(1, p.pairs)), p.per_t = Divisor(p.t);
+    // With vectors a tile is what the stages hold; otherwise as many tokens as there is room for angles of, up to 16 units a thread.
+    const int most = (vec ? 1 : 4) * kUnits * 256;
+    p.per_block = std::max(1, std::min(kAngles / std::max(1, p.pairs), most / (int)p.per_token.d));
+    const int64_t tiles = (p.tokens + p.per_block - 1) / p.per_block;
+    if (vec && (int)p.per_token.d <= kUnits * 256) launch_tiles<T, V, HALVES>(p, tiles, st);
+    else if (vec) {  // a token of more units than a tile has places for: by single elements
+        launch_rotary<T, HALVES>(p, false, st);
+    } else launch_tiles<T, 1, HALVES>(p, tiles, st);
 }
 
 }  // namespace

@@ -33,12 +33,44 @@ struct SandwichArgs {
     float *part_w, *part_wn; // [gridDim.x][cols]
     float* part_g;           // [groups][parts][cols] where several blocks share a gate row, else null
     int64_t rows, cols, shared;   // rows per gate row
+    Divisor per_gate;
     int64_t groups, parts, per_part;  // the backward's units: `parts` runs of at most per_part rows in each group of rows
     float alpha, eps;
     int act;
 };
 
-__device__ __forceinline__ float sigmoid_of(float z) { return 1.f / (1.f + __expf(-z)); }
+// (The hardware's exponential and reciprocal, about 2 units in the last place each.)
+__device__ __forceinline__ float sigmoid_of(float z) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-z)));
+    return r;
+}
+
+// Rows on their way.  A row's two reductions follow one another, so a group
+// that waited for its row to arrive first would leave the memory idle.  Each
+// thread copies its packs of the next rows (K operands) to places of its own in
+// shared memory, asynchronously: that takes no registers and no barriers (bf16,
+// 131072x1024, a gate per token: forward 414 -> 212 us, backward 739 -> 380).
+// Rows without 16-byte packs (fp32 6304x771: 29 us so, 26 without) and rows of
+// very wide groups, which do not fit, are loaded when their turn comes.
+template <typename T, int VEC, int NV, int K, int BLOCK>
+struct RowStream {
+    static constexpr int kPack = (int)sizeof(Pack<T, VEC>), kStage = K * NV * BLOCK * kPack;
+    static constexpr int kFit = (96 << 10) / kStage, kStages = kPack < 16 || kFit < 2 ? 0 : kFit < 4 ? kFit : 4;
+    static constexpr int kBytes = kStages * kStage;
+
+    uint8_t* base;  // of this thread
+    __device__ __forceinline__ explicit RowStream(uint8_t* smem) : base(smem + threadIdx.x * kPack) {}
+    __device__ __forceinline__ uint8_t* at(int stage, int k, int i) const { return base + ((stage * K + k) * NV + i) * (BLOCK * kPack); }
+    __device__ __forceinline__ void copy(int stage, int k, int i, const T* src) const {
+        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(at(stage, k, i)));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    }
+    __device__ __forceinline__ Pack<T, VEC> get(int stage, int k, int i) const { return *reinterpret_cast<const Pack<T, VEC>*>(at(stage, k, i)); }
+};
+__device__ __forceinline__ void copies_committed() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // act(g), and with SLOPE its derivative in d.
 template <bool SLOPE, int N>
@@ -73,9 +105,13 @@ __device__ __forceinline__ void gate_values(float (&v)[N], float (&d)[N], int ac
 template <typename T, int VEC, int NV, int G>
 __global__ void __launch_bounds__(block_of<G>()) sandwich_fwd_kernel(const SandwichArgs p) {
     constexpr int RPB = block_of<G>() / G;
+    using Stream = RowStream<T, VEC, NV, 3, block_of<G>()>;
+    constexpr int S = Stream::kStages;
+    extern __shared__ __align__(16) uint8_t staged[];
     __shared__ float red[32];
     grid_release();
     grid_wait();
+    const Stream stream(staged);
     const int g = threadIdx.x % G, sub = threadIdx.x / G, cols = (int)p.cols;
     Pack<T, VEC> w[NV], wn[NV];
 #pragma unroll
@@ -86,19 +122,50 @@ __global__ void __launch_bounds__(block_of<G>()) sandwich_fwd_kernel(const Sandw
         }
     const float inv_cols = 1.f / (float)cols;
     // The row index is clamped, not skipped, so that every lane takes part in the shuffles.
-    for (int64_t base = (int64_t)blockIdx.x * RPB; base < p.rows; base += (int64_t)gridDim.x * RPB) {
+    const int64_t step = (int64_t)gridDim.x * RPB, first = (int64_t)blockIdx.x * RPB;
+    auto row_of = [&](int64_t base) { return min(base + sub, p.rows - 1); };
+    auto gate_of = [&](int64_t row) { return p.shared == 1 ? row * p.cols : (int64_t)p.per_gate.of((int)row) * p.cols; };
+    auto fetch = [&](int64_t base, int stage) {
+        if (base < p.rows) {
+            const int64_t row = row_of(base), off = row * p.cols, goff = p.gate ? gate_of(row) : 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * G + g) * VEC;
+                if (c < cols) {
+                    stream.copy(stage, 0, i, (const T*)p.x + off + c);
+                    stream.copy(stage, 1, i, (const T*)p.r + off + c);
+                    if (p.gate) stream.copy(stage, 2, i, (const T*)p.gate + goff + c);
+                }
+            }
+        }
+        copies_committed();
+    };
+    if constexpr (S > 0) {
+#pragma unroll
+        for (int k = 0; k + 1 < S; ++k) fetch(first + k * step, k);
+    }
+    int stage = 0;
+    for (int64_t base = first; base < p.rows; base += step) {
         const bool live = base + sub < p.rows;
-        const int64_t row = live ? base + sub : p.rows - 1, off = row * p.cols;
-        const int64_t goff = p.shared == 1 ? off : row / p.shared * p.cols;
+        const int64_t row = row_of(base), off = row * p.cols;
         Pack<T, VEC> x[NV], r[NV], ga[NV];
         float ss = 0.f, t[NV * VEC];
+        if constexpr (S > 0) {
+            copies_but<(S > 1 ? S - 2 : 0)>();
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + g) * VEC;
-            if (c < cols) {
-                x[i] = load_pack<T, VEC>((const T*)p.x + off + c);
-                r[i] = load_pack<T, VEC>((const T*)p.r + off + c);
-                if (p.gate) ga[i] = load_pack<T, VEC>((const T*)p.gate + goff + c);
+            for (int i = 0; i < NV; ++i) x[i] = stream.get(stage, 0, i), r[i] = stream.get(stage, 1, i), ga[i] = stream.get(stage, 2, i);
+            fetch(base + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+            stage = stage + 1 == S ? 0 : stage + 1;
+        } else {
+            const int64_t goff = p.gate ? gate_of(row) : 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * G + g) * VEC;
+                if (c < cols) {
+                    x[i] = load_pack<T, VEC>((const T*)p.x + off + c);
+                    r[i] = load_pack<T, VEC>((const T*)p.r + off + c);
+                    if (p.gate) ga[i] = load_pack<T, VEC>((const T*)p.gate + goff + c);
+                }
             }
         }
 #pragma unroll
@@ -236,10 +303,14 @@ __device__ __forceinline__ void put_sums(float (&v)[NV * VEC], D* dst, int cols,
 template <typename T, int VEC, int NV, int G>
 __global__ void __launch_bounds__(block_of<G>()) sandwich_bwd_kernel(const SandwichArgs p) {
     constexpr int RPB = block_of<G>() / G;
-    extern __shared__ float sums[];  // [warps][cols] when G <= 32
+    using Stream = RowStream<T, VEC, NV, 5, block_of<G>()>;
+    constexpr int S = Stream::kStages;
+    extern __shared__ __align__(16) uint8_t staged[];
+    float* const sums = reinterpret_cast<float*>(staged + Stream::kBytes);  // [warps][cols] when G <= 32
     __shared__ float red[32];
     grid_release();
     grid_wait();
+    const Stream stream(staged);
     const int g = threadIdx.x % G, sub = threadIdx.x / G, cols = (int)p.cols;
     const bool own_gate = p.gate && p.shared == 1, kept_gate = p.gate && p.shared > 1 && (p.dgate || p.part_g);
     Pack<T, VEC> w[NV], wn[NV];
@@ -258,20 +329,56 @@ __global__ void __launch_bounds__(block_of<G>()) sandwich_bwd_kernel(const Sandw
         const int64_t group = unit / p.parts, part = unit - group * p.parts;
         const int64_t first = group * group_rows + min(group_rows, part * p.per_part);
         const int64_t last = group * group_rows + min(group_rows, (part + 1) * p.per_part);
+        auto row_of = [&](int64_t base) { return min(base + sub, last - 1); };
+        auto fetch = [&](int64_t base, int stage) {
+            if (base < last) {
+                const int64_t row = row_of(base), off = row * p.cols, goff = p.shared == 1 ? off : group * p.cols;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int c = (i * G + g) * VEC;
+                    if (c < cols) {
+                        stream.copy(stage, 0, i, (const T*)p.x + off + c);
+                        if (p.dy) stream.copy(stage, 1, i, (const T*)p.s + off + c), stream.copy(stage, 2, i, (const T*)p.dy + off + c);
+                        if (p.ds) stream.copy(stage, 3, i, (const T*)p.ds + off + c);
+                        if (p.gate) stream.copy(stage, 4, i, (const T*)p.gate + goff + c);
+                    }
+                }
+            }
+            copies_committed();
+        };
+        if constexpr (S > 0) {
+#pragma unroll
+            for (int k = 0; k + 1 < S; ++k) fetch(first + k * RPB, k);
+        }
+        int stage = 0;
+        float rx_next = 0.f, rt_next = 0.f;
+        if (first < last) rx_next = p.rstd[row_of(first)], rt_next = p.wn ? p.rstd[p.rows + row_of(first)] : 0.f;
         for (int64_t base = first; base < last; base += RPB) {
             const bool live = base + sub < last;
-            const int64_t row = live ? base + sub : last - 1, off = row * p.cols;
-            const int64_t goff = p.shared == 1 ? off : group * p.cols;
+            const int64_t row = row_of(base), off = row * p.cols;
+            const float rx = rx_next, rt = rt_next;
+            const int64_t after = row_of(base + RPB);
+            rx_next = p.rstd[after], rt_next = p.wn ? p.rstd[p.rows + after] : 0.f;
             Pack<T, VEC> x[NV], s[NV], dy[NV], ds[NV], ga[NV];
-            const float rx = p.rstd[row], rt = p.wn ? p.rstd[p.rows + row] : 0.f;
+            if constexpr (S > 0) {
+                copies_but<(S > 1 ? S - 2 : 0)>();
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * G + g) * VEC;
-                if (c < cols) {
-                    x[i] = load_pack<T, VEC>((const T*)p.x + off + c);
-                    if (p.dy) s[i] = load_pack<T, VEC>((const T*)p.s + off + c), dy[i] = load_pack<T, VEC>((const T*)p.dy + off + c);
-                    if (p.ds) ds[i] = load_pack<T, VEC>((const T*)p.ds + off + c);
-                    if (p.gate) ga[i] = load_pack<T, VEC>((const T*)p.gate + goff + c);
+                for (int i = 0; i < NV; ++i)
+                    x[i] = stream.get(stage, 0, i), s[i] = stream.get(stage, 1, i), dy[i] = stream.get(stage, 2, i), ds[i] = stream.get(stage, 3, i),
+                    ga[i] = stream.get(stage, 4, i);
+                fetch(base + (S - 1) * RPB, stage == 0 ? S - 1 : stage - 1);
+                stage = stage + 1 == S ? 0 : stage + 1;
+            } else {
+                const int64_t goff = p.shared == 1 ? off : group * p.cols;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int c = (i * G + g) * VEC;
+                    if (c < cols) {
+                        x[i] = load_pack<T, VEC>((const T*)p.x + off + c);
+                        if (p.dy) s[i] = load_pack<T, VEC>((const T*)p.s + off + c), dy[i] = load_pack<T, VEC>((const T*)p.dy + off + c);
+                        if (p.ds) ds[i] = load_pack<T, VEC>((const T*)p.ds + off + c);
+                        if (p.gate) ga[i] = load_pack<T, VEC>((const T*)p.gate + goff + c);
+                    }
                 }
             }
             float dot = 0.f, mean = 0.f;
@@ -339,6 +446,7 @@ __global__ void __launch_bounds__(block_of<G>()) sandwich_bwd_kernel(const Sandw
                 }
             }
         }
+        if constexpr (S > 0) copies_but<0>();  // (rows past the unit's end were not copied: the groups that are left are empty)
         if (kept_gate) {
             if (p.part_g) put_sums<float, VEC, NV, G>(dg, p.part_g + unit * p.cols, cols, sums);
             else put_sums<T, VEC, NV, G>(dg, (T*)p.dgate + group * p.cols, cols, sums);
@@ -429,7 +537,7 @@ __global__ void __launch_bounds__(1024) sandwich_join_kernel(const JoinArgs p) {
     const float* part = p.part[job] + row * n * p.cols;
     float t = 0.f;
     if (c < p.cols)
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t b = k; b < n; b += 32) t += part[b * p.cols + c];
     sh[k][lane] = t;
     __syncthreads();
@@ -440,14 +548,26 @@ __global__ void __launch_bounds__(1024) sandwich_join_kernel(const JoinArgs p) {
     }
 }
 
+// resident_blocks() of a kernel that may take more than 48 KB of shared memory.
+template <auto Kernel>
+int resident_with(int block, int smem) {
+    static std::once_flag once[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::call_once(once[dev & 63], [&] { cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    return resident_blocks<Kernel>(block, smem);
+}
+
 template <typename T>
 void launch_sandwich_fwd(const SandwichArgs& a, bool vec, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     bool long_rows = false;
-#define LFB_CALL(TT, VV, NV, G)                                                                                              \
-    launch_early(sandwich_fwd_kernel<TT, VV, NV, G>,                                                                         \
-                 row_blocks(a.rows, block_of<G>() / G, resident_blocks<sandwich_fwd_kernel<TT, VV, NV, G>>(block_of<G>(), 0)), \
-                 block_of<G>(), 0, 1, st, a)
+#define LFB_CALL(TT, VV, NV, G)                                                                                   \
+    {                                                                                                             \
+        constexpr int smem = RowStream<TT, VV, NV, 3, block_of<G>()>::kBytes;                                     \
+        const int slots = resident_with<sandwich_fwd_kernel<TT, VV, NV, G>>(block_of<G>(), smem);                 \
+        launch_early(sandwich_fwd_kernel<TT, VV, NV, G>, row_blocks(a.rows, block_of<G>() / G, slots), block_of<G>(), smem, 1, st, a); \
+    }
     LFB_NORM_FWD(T, V, a.cols, vec, LFB_CALL)
 #undef LFB_CALL
     if (long_rows)
@@ -481,10 +601,12 @@ void launch_sandwich_bwd(const SandwichArgs& a, bool vec, int64_t most, int* blo
         return (unsigned)*blocks;
     };
     // Shared memory of the largest width that a warp-per-row group takes, so that residency does not depend on cols.
-#define LFB_CALL(TT, VV, NV, G)                                                                                              \
-    launch_early(sandwich_bwd_kernel<TT, VV, NV, G>,                                                                         \
-                 grid(resident_blocks<sandwich_bwd_kernel<TT, VV, NV, G>>(block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0)),   \
-                 block_of<G>(), G <= 32 ? G * NV * VV * 32 : 0, 1, st, a)
+#define LFB_CALL(TT, VV, NV, G)                                                                                   \
+    {                                                                                                             \
+        constexpr int smem = RowStream<TT, VV, NV, 5, block_of<G>()>::kBytes + (G <= 32 ? G * NV * VV * 32 : 0);  \
+        const int slots = resident_with<sandwich_bwd_kernel<TT, VV, NV, G>>(block_of<G>(), smem);                 \
+        launch_early(sandwich_bwd_kernel<TT, VV, NV, G>, grid(slots), block_of<G>(), smem, 1, st, a);             \
+    }
     LFB_NORM_BWD(T, V, a.cols, vec, LFB_CALL)
 #undef LFB_CALL
     if (long_rows) launch_early(sandwich_bwd_long_kernel<T>, grid(resident_blocks<sandwich_bwd_long_kernel<T>>(512, 0)), 512, 0, 1, st, a);
@@ -519,6 +641,7 @@ SandwichArgs sandwich_args(const lf_sandwich_norm_t* a) {
     p.x = a->x, p.w = a->weight, p.r = a->residual, p.gate = a->gate, p.wn = a->next_weight, p.s = a->s, p.y = a->y, p.rstd = a->rstd;
     p.dy = a->dy, p.ds = a->ds, p.dx = a->dx, p.dr = a->d_residual, p.dgate = a->d_gate;
     p.rows = a->rows, p.cols = a->cols, p.shared = a->gate ? a->rows_per_gate : 1;
+    if (p.shared > 1) p.per_gate = Divisor((uint32_t)p.shared);
     p.alpha = (float)a->scale, p.eps = (float)a->eps, p.act = a->activation;
     return p;
 }
