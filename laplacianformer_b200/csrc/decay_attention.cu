@@ -60,6 +60,7 @@ struct alignas(64) MixArgs {
     int64_t o_sb, o_sh, o_st;
     int heads, t, da, dc, chunks, nseg, per_seg, items;
     int unit, units;         // chunks per unit, units per segment
+    int joined;              // a segment finds the state before it in the slot of its unit that is first in time
     int g0_row, g0_col;      // strides within a state matrix (transposed for dq and dk)
     float scale, g0_scale, gout_scale;
     int ksteps, nb;          // 16-column steps of da; dc rounded up to 16
@@ -95,7 +96,7 @@ __device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 // mbar_wait() for waits that are mostly short: the clock is read only after a run of tries, so that waiting warps take few
-// issue slots from the working ones (they took more than half: 4096 tokens of 128 heads 78 us with mbar_wait, XX with this).
+// issue slots from the working ones (with mbar_wait they took more than half of them).
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
     const uint32_t addr = smem_u32(bar);
     uint64_t t0 = 0;
@@ -243,7 +244,7 @@ template <typename T, int W, bool REV>
 __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W, kTiles = kEndsRing<W>;
     extern __shared__ uint8_t raw[];
-    uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const ring = raw + (-smem_u32(raw) & 1023u);  // (keeps the pointer one to shared memory)
     uint8_t* const lows = ring + kTiles * kTile;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(lows + 2 * kTile);
     uint64_t *full = bars, *empty = bars + kTiles, *ready = empty + kTiles, *used = ready + 2, *done = used + 2, *read = done + 1, *drain = done + 2;
@@ -387,6 +388,50 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
     if (warp == 9) tmem_dealloc(tmem, 128);
 }
 
+// From the units' sums the state before each segment, in the slot of its unit that is first in time: four elements of a head's
+// state per thread, its units read eight at a time and joined in the order of time.  (Segments that summed their
+// predecessors' units themselves read up to 34 x 64 KB each before their first chunk.)
+template <int W, bool REV>
+__global__ void __launch_bounds__(256) decay_join_kernel(const __grid_constant__ MixArgs p) {
+    constexpr int kState = 64 * W, kQuads = kState * kState / 4;
+    grid_release();
+    grid_wait();
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int bh = (int)(at / kQuads), b = bh / p.heads;
+    const float g = p.log_decay[bh - b * p.heads];
+    const int64_t len = tokens_in(p, b);
+    const int active = (int)((len + kChunk - 1) / kChunk), total = p.nseg * p.units;
+    float4* const slots = reinterpret_cast<float4*>(p.ends) + (int64_t)bh * total * kQuads + at % kQuads;
+    // Units are counted in time; the first chunk of one, its chunks (before another), whether its sum was made.
+    auto place = [&](int i) { return REV ? total - 1 - i : i; };
+    auto first = [&](int u) { return u / p.units * p.per_seg + u % p.units * p.unit; };
+    auto length = [&](int u) { return min(p.unit, p.per_seg - u % p.units * p.unit); };
+    auto there = [&](int u) {
+        const int seg = u / p.units, from = first(u);
+        return REV ? seg > 0 && from < active : seg < p.nseg - 1 && (int64_t)(from + length(u)) * kChunk <= len;
+    };
+    const float wu = power(g, (int64_t)p.unit * kChunk), wl = power(g, (int64_t)length(p.units - 1) * kChunk);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool any = false;  // (a power that overflows meets no 0)
+    for (int i0 = 0; i0 < total; i0 += 8) {
+        float4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i0 + j < total && there(place(i0 + j))) x[j] = slots[(int64_t)place(i0 + j) * kQuads];
+            else x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int u = place(i0 + j), v = u % p.units;
+            if (i0 + j >= total) break;
+            if (v == (REV ? p.units - 1 : 0)) slots[(int64_t)u * kQuads] = acc;  // (its own sum is in x)
+            if (!there(u)) continue;
+            const float w = !any ? 0.f : v == p.units - 1 ? wl : wu;
+            acc.x = __fmaf_rn(w, acc.x, x[j].x), acc.y = __fmaf_rn(w, acc.y, x[j].y), acc.z = __fmaf_rn(w, acc.z, x[j].z), acc.w = __fmaf_rn(w, acc.w, x[j].w);
+            any = true;
+        }
+    }
+}
+
 // W: 64-column blocks per operand row (head sizes up to 64 W).  REV: backwards
 // in time.
 template <typename T, int W, bool REV>
@@ -395,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     constexpr int kO = 128, kKv = 128 + 64 * W, kCols = W == 1 ? 256 : 512;   // tensor memory columns; scores from 0 on
     constexpr bool F16 = std::is_same<T, __half>::value;
     extern __shared__ uint8_t raw[];
-    uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const ring = raw + (-smem_u32(raw) & 1023u);  // (keeps the pointer one to shared memory)
     uint8_t* const low = ring + kRing * kTile;
     uint8_t* const gop = low + kTile;                                         // [state row][dc], 64 columns a block
     float* const pw = reinterpret_cast<float*>(gop + kState * 128 * W);       // l^n, n = 0..128
@@ -420,7 +465,6 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     tc_fence_after();
     grid_wait();
     const uint32_t tmem = *tmem_ptr;
-    constexpr int kTiles = 3;
     bool ok = true;
 
     if (warp == 8) {  // copies
@@ -430,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 const Item t = item_of(p, i);
                 for (int k = 0; ok && k < t.n; ++k) {
                     const int t0 = (REV ? t.first + t.n - 1 - k : t.first + k) * kChunk;
-                    for (int j = 3 - kTiles; j < 3; ++j) {
+                    for (int j = 0; j < 3; ++j) {
                         const int s = n % kRing;
                         if (!(ok = wait_for(&empty[s], (n / kRing & 1) ^ 1))) break;
                         expect(&full[s], kTile);
@@ -449,58 +493,50 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
         int n = 0, cc = 0;
         for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
             const Item t = item_of(p, i);
-            for (int k = 0; k < t.n; ++k, ++cc, n += kTiles) {
-                const int na = n, nk = n + kTiles - 2, nv = nk + 1;
+            for (int k = 0; k < t.n; ++k, ++cc, n += 3) {
+                const int na = n, nk = n + 1, nv = n + 2;
                 const uint32_t sk = smem_u32(ring + nk % kRing * kTile), sv = smem_u32(ring + nv % kRing * kTile);
                 if (!(ok = wait_for(&full[nk % kRing], nk / kRing & 1))) break;
-                bool has_g = k > 0;  // there is a state before this chunk
-                {
-                    const int first = REV ? (t.active - 1) / p.per_seg : 0;  // the segment that the sequence starts with
-                    has_g = k > 0 || p.g0 || t.seg != first;
-                    const uint32_t sa = smem_u32(ring + na % kRing * kTile);
-                    if (!(ok = wait_for(&full[na % kRing], na / kRing & 1))) break;
-                    if (cc > 0 && !(ok = wait_for(o_full, (cc - 1) & 1))) break;  // the scores' columns hold its operand
-                    tc_fence_after();
-                    const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sk, 16, 1024);
+                const int first = REV ? (t.active - 1) / p.per_seg : 0;  // the segment that the sequence starts with
+                const bool has_g = k > 0 || p.g0 || t.seg != first;      // there is a state before this chunk
+                const uint32_t sa = smem_u32(ring + na % kRing * kTile);
+                if (!(ok = wait_for(&full[na % kRing], na / kRing & 1))) break;
+                if (cc > 0 && !(ok = wait_for(o_full, (cc - 1) & 1))) break;  // the scores' columns hold its operand
+                tc_fence_after();
+                const uint64_t da = make_desc(sa, 16, 1024), db = make_desc(sk, 16, 1024);
 #pragma unroll
-                    for (int s = 0; s < 4 * W; ++s) {  // (unrolled: an address that the loop computes costs more than the product)
-                        const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
-                        if (s < p.ksteps) mma_f16(tmem, da + at, db + at, p.id_qk, s > 0 ? 1u : 0u, go);
-                    }
-                    if (go) mma_commit(s_full);
-                    if (!(ok = wait_for(g_ready, cc & 1))) break;
-                    tc_fence_after();
-                    if (has_g) {
-                        const uint64_t dg = make_desc(smem_u32(gop), kState * 128, 1024);
-#pragma unroll
-                        for (int s = 0; s < 4 * W; ++s) {
-                            const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
-                            if (s < p.ksteps) mma_f16(tmem + kO, da + at, dg + (uint64_t)(s * 128), p.id_qg, s > 0 ? 1u : 0u, go);
-                        }
-                        if (go) mma_commit(qg_full);
-                    }
-                    if (go) mma_commit(&empty[na % kRing]);
+                for (int s = 0; s < 4 * W; ++s) {  // (unrolled: an address that the loop computes costs more than the product)
+                    const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
+                    if (s < p.ksteps) mma_f16(tmem, da + at, db + at, p.id_qk, s > 0 ? 1u : 0u, go);
                 }
+                if (go) mma_commit(s_full);
+                if (!(ok = wait_for(g_ready, cc & 1))) break;
+                tc_fence_after();
+                if (has_g) {
+                    const uint64_t dg = make_desc(smem_u32(gop), kState * 128, 1024);
+#pragma unroll
+                    for (int s = 0; s < 4 * W; ++s) {
+                        const uint64_t at = (uint64_t)((s >> 2) * (kBlock >> 4) + (s & 3) * 2);
+                        if (s < p.ksteps) mma_f16(tmem + kO, da + at, dg + (uint64_t)(s * 128), p.id_qg, s > 0 ? 1u : 0u, go);
+                    }
+                    if (go) mma_commit(qg_full);
+                }
+                if (go) mma_commit(&empty[na % kRing]);
                 if (!(ok = wait_for(k_ready, cc & 1) && wait_for(&full[nv % kRing], nv / kRing & 1))) break;
                 tc_fence_after();
-                {
-                    const uint64_t dh = make_desc(sk, kBlock, 1024), dl = make_desc(smem_u32(low), kBlock, 1024);
-                    const uint64_t dv = make_desc(sv, kBlock, 1024);
+                const uint64_t dh = make_desc(sk, kBlock, 1024), dl = make_desc(smem_u32(low), kBlock, 1024);
+                const uint64_t dv = make_desc(sv, kBlock, 1024);
 #pragma unroll
-                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, has_g || s > 0 ? 1u : 0u, go);
+                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, has_g || s > 0 ? 1u : 0u, go);
 #pragma unroll
-                    for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, 1u, go);
-                    if (go) mma_commit(kv_full), mma_commit(&empty[nk % kRing]);
-                    {
-                        if (!(ok = wait_for(p_ready, cc & 1))) break;
-                        tc_fence_after();
+                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, 1u, go);
+                if (go) mma_commit(kv_full), mma_commit(&empty[nk % kRing]);
+                if (!(ok = wait_for(p_ready, cc & 1))) break;
+                tc_fence_after();
 #pragma unroll
-                        for (int s = 0; s < 8; ++s)  // scores of columns 64 on lie 64 columns further
-                            mma_f16_ts(tmem + kO, tmem + (s >> 2) * 64 + (s & 3) * 8, dv + (uint64_t)(s * 128), p.id_pv, has_g || s > 0 ? 1u : 0u, go);
-                        if (go) mma_commit(o_full);
-                    }
-                    if (go) mma_commit(&empty[nv % kRing]);
-                }
+                for (int s = 0; s < 8; ++s)  // scores of columns 64 on lie 64 columns further
+                    mma_f16_ts(tmem + kO, tmem + (s >> 2) * 64 + (s & 3) * 8, dv + (uint64_t)(s * 128), p.id_pv, has_g || s > 0 ? 1u : 0u, go);
+                if (go) mma_commit(o_full), mma_commit(&empty[nv % kRing]);
             }
         }
         if (!ok) {  // products in flight end before the tensor memory is freed
@@ -535,34 +571,32 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             // G before chunk k: as an operand (rows of dc columns, in fp16 times a power of two that keeps the largest in
             // range), and decayed over the chunk to where the products add to it.
             auto put_state = [&](int k) {
-                {
-                    float s = 1.f;
-                    if constexpr (F16) {
-                        float m = 0.f;
+                float s = 1.f;
+                if constexpr (F16) {
+                    float m = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 32 * W; ++j) m = fmaxf(m, fabsf(G[j]));
-                        const uint32_t wm = __reduce_max_sync(0xffffffffu, live ? __float_as_uint(m) : 0u);
-                        const int slot = puts++ & 1;
-                        if (lane == 0) atomicMax(&gmax[slot], wm);
-                        epi_sync(true);
-                        s = range_scale(gmax[slot]);
-                        if (tid == 0) gmax[slot ^ 1] = 0;
-                        unscale = 1.f / s;
-                    }
-                    if (live) {
-                        uint8_t* const dst = gop + (W == 2 ? half * kState * 128 : 0) + srow * 128;
-#pragma unroll
-                        for (int j = 0; j < 4 * W; ++j) {
-                            const float* v = &G[8 * j];
-                            const int ch = (W == 1 ? half * 4 : 0) + j;
-                            const uint4 o = F16 ? make_uint4(pack2<T>(v[0] * s, v[1] * s), pack2<T>(v[2] * s, v[3] * s), pack2<T>(v[4] * s, v[5] * s),
-                                                             pack2<T>(v[6] * s, v[7] * s))
-                                                : make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-                            sts16(dst + ((ch ^ (srow & 7)) << 4), o);
-                        }
-                    }
-                    fence_async_smem();
+                    for (int j = 0; j < 32 * W; ++j) m = fmaxf(m, fabsf(G[j]));
+                    const uint32_t wm = __reduce_max_sync(0xffffffffu, live ? __float_as_uint(m) : 0u);
+                    const int slot = puts++ & 1;
+                    if (lane == 0) atomicMax(&gmax[slot], wm);
+                    epi_sync(true);
+                    s = range_scale(gmax[slot]);
+                    if (tid == 0) gmax[slot ^ 1] = 0;
+                    unscale = 1.f / s;
                 }
+                if (live) {
+                    uint8_t* const dst = gop + (W == 2 ? half * kState * 128 : 0) + srow * 128;
+#pragma unroll
+                    for (int j = 0; j < 4 * W; ++j) {
+                        const float* v = &G[8 * j];
+                        const int ch = (W == 1 ? half * 4 : 0) + j;
+                        const uint4 o = F16 ? make_uint4(pack2<T>(v[0] * s, v[1] * s), pack2<T>(v[2] * s, v[3] * s), pack2<T>(v[4] * s, v[5] * s),
+                                                         pack2<T>(v[6] * s, v[7] * s))
+                                            : make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+                        sts16(dst + ((ch ^ (srow & 7)) << 4), o);
+                    }
+                }
+                fence_async_smem();
                 const float w = pw[tokens_of(k) - last_of(k)];
                 const uint64_t w2 = pk2(w, w);
 #pragma unroll
@@ -595,12 +629,16 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     for (int j = 0; j < 32 * W; ++j)
                         if (col0 + j < p.dc) G[j] = w * src[(int64_t)(col0 + j) * p.g0_col];
                 }
-                if (t.n > 0)
-                    for (int u = REV ? t.seg + 1 : 0; REV ? u <= first_seg : u < t.seg; ++u) {
-                        // its units, of p.unit chunks each (forwards to the segment's end, backwards to the last token)
-                        const int from = u * p.per_seg, to = min(from + p.per_seg, REV ? t.active : p.chunks), here = REV ? t.first + t.n : t.first;
-                        for (int v = 0; from + v * p.unit < to; ++v) {
-                            const float w = power(g, (int64_t)(REV ? from + v * p.unit - here : here - min(from + (v + 1) * p.unit, to)) * kChunk);
+                if (t.n > 0 && t.seg != first_seg) {
+                    // The sums of the units before this segment (forwards to its start, backwards from the last token), or what
+                    // they were joined to.
+                    const int here = REV ? t.first + t.n : t.first, mine = REV ? p.units - 1 : 0;
+                    const int u0 = p.joined ? t.seg : REV ? t.seg + 1 : 0, u1 = p.joined ? t.seg : REV ? first_seg : t.seg - 1;
+                    for (int u = u0; u <= u1; ++u) {
+                        const int from = u * p.per_seg, to = min(from + p.per_seg, REV ? t.active : p.chunks);
+                        for (int v = p.joined ? mine : 0; p.joined ? v == mine : from + v * p.unit < to; ++v) {
+                            const int64_t after = REV ? from + v * p.unit - here : here - min(from + (v + 1) * p.unit, to);
+                            const float w = p.joined ? 1.f : power(g, after * kChunk);
                             const float4* e = reinterpret_cast<const float4*>(p.ends + ((((int64_t)t.bh * p.nseg + u) * p.units + v) * kState + srow) * kState + col0);
 #pragma unroll
                             for (int j = 0; j < 8 * W; ++j) {
@@ -610,18 +648,16 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                             }
                         }
                     }
-            }
-            epi_sync(true);  // the tables are written
-            {
-                if (t.n > 0) {
-                    if (has_g) put_state(0);
-                    arrive(g_ready);
                 }
             }
+            epi_sync(true);  // the tables are written
+            if (t.n > 0) {
+                if (has_g) put_state(0);
+                arrive(g_ready);
+            }
             // ---- chunks
-            for (int k = 0; k < t.n; ++k, ++cc, n += kTiles) {
-                const int chunk = chunk_of(k), L = tokens_of(k), e = last_of(k);
-                const int nk = n + kTiles - 2, nv = nk + 1;
+            for (int k = 0; k < t.n; ++k, ++cc, n += 3) {
+                const int chunk = chunk_of(k), L = tokens_of(k), e = last_of(k), nk = n + 1, nv = n + 2;
                 // ---- b_j times its power of l, in two parts
                 uint8_t *hi = ring + nk % kRing * kTile + kr * 128, *lo = low + kr * 128;
                 if (W == 2) hi += kpart * kBlock, lo += kpart * kBlock;
@@ -639,11 +675,9 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 };
                 ok = wait_for(&full[nk % kRing], nk / kRing & 1) && ok;
                 fetch(0);
-                {
-                    ok = wait_for(s_full, cc & 1) && ok;  // the scores are done: b may be overwritten
-                    if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    if (!(ok = epi_sync(ok))) break;      // and the last output has left the staging
-                }
+                ok = wait_for(s_full, cc & 1) && ok;  // the scores are done: b may be overwritten
+                if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                if (!(ok = epi_sync(ok))) break;      // and the last output has left the staging
                 tc_fence_after();
 #pragma unroll
                 for (int j0 = 0; j0 < 4 * W; j0 += 4) {
@@ -679,58 +713,56 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 }
                 fence_async_smem();
                 arrive(k_ready);
-                {
-                    // ---- weighted scores: row `row`, columns 64 half on, in blocks of 32
+                // ---- weighted scores: row `row`, columns 64 half on, in blocks of 32
 #pragma unroll 1
-                    for (int bl = 0; bl < 2; ++bl) {
-                        const int blk = half * 2 + bl;
-                        uint32_t u[16];
-                        if (REV ? blk < quad : blk > quad) {
+                for (int bl = 0; bl < 2; ++bl) {
+                    const int blk = half * 2 + bl;
+                    uint32_t u[16];
+                    if (REV ? blk < quad : blk > quad) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) u[j] = 0u;
-                        } else {
+                        for (int j = 0; j < 16; ++j) u[j] = 0u;
+                    } else {
+                        float v[32];
+                        tmem_ld32(tq + blk * 32, v);
+                        const float2* f = reinterpret_cast<const float2*>(frow + blk * 32);
+                        tmem_wait_ld();
+                        reg_fence(v);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float2 c = f[j];
+                            float a, b;
+                            upk2(mul2(pk2(v[2 * j], v[2 * j + 1]), pk2(c.x, c.y)), a, b);
+                            u[j] = pack2<T>(a, b);
+                        }
+                        if (L < kChunk) {  // (a product with what lies past the sequence may not be finite)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) u[j] &= keep_low(16 * (L - blk * 32) - 32 * j);
+                        }
+                    }
+                    tmem_st16(tq + half * 64 + bl * 16, u);
+                }
+                if (has_g) {  // what the state gives, times the row's power
+                    ok = wait_for(qg_full, qg++ & 1) && ok;
+                    tc_fence_after();
+                    const int d = REV ? L - 1 - row : row;
+                    const float w = (d >= 0 ? pw[d] : 0.f) * p.scale * unscale;
+                    const uint64_t w2 = pk2(w, w);
+#pragma unroll
+                    for (int c = 0; c < W; ++c) {
+                        if (col0 + 32 * c < p.nb) {
                             float v[32];
-                            tmem_ld32(tq + blk * 32, v);
-                            const float2* f = reinterpret_cast<const float2*>(frow + blk * 32);
+                            tmem_ld32(tq + kO + col0 + 32 * c, v);
                             tmem_wait_ld();
                             reg_fence(v);
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const float2 c = f[j];
-                                float a, b;
-                                upk2(mul2(pk2(v[2 * j], v[2 * j + 1]), pk2(c.x, c.y)), a, b);
-                                u[j] = pack2<T>(a, b);
-                            }
-                            if (L < kChunk) {  // (a product with what lies past the sequence may not be finite)
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) u[j] &= keep_low(16 * (L - blk * 32) - 32 * j);
-                            }
-                        }
-                        tmem_st16(tq + half * 64 + bl * 16, u);
-                    }
-                    if (has_g) {  // what the state gives, times the row's power
-                        ok = wait_for(qg_full, qg++ & 1) && ok;
-                        tc_fence_after();
-                        const int d = REV ? L - 1 - row : row;
-                        const float w = (d >= 0 ? pw[d] : 0.f) * p.scale * unscale;
-                        const uint64_t w2 = pk2(w, w);
-#pragma unroll
-                        for (int c = 0; c < W; ++c) {
-                            if (col0 + 32 * c < p.nb) {
-                                float v[32];
-                                tmem_ld32(tq + kO + col0 + 32 * c, v);
-                                tmem_wait_ld();
-                                reg_fence(v);
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) upk2(mul2(pk2(v[2 * j], v[2 * j + 1]), w2), v[2 * j], v[2 * j + 1]);
-                                tmem_st32(tq + kO + col0 + 32 * c, v);
-                            }
+                            for (int j = 0; j < 16; ++j) upk2(mul2(pk2(v[2 * j], v[2 * j + 1]), w2), v[2 * j], v[2 * j + 1]);
+                            tmem_st32(tq + kO + col0 + 32 * c, v);
                         }
                     }
-                    tmem_wait_st();
-                    tc_fence_before();
-                    arrive(p_ready);
                 }
+                tmem_wait_st();
+                tc_fence_before();
+                arrive(p_ready);
                 // ---- the state after this chunk
                 ok = wait_for(kv_full, cc & 1) && ok;
                 tc_fence_after();
@@ -748,7 +780,6 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 }
                 has_g = true;
                 if (k + 1 < t.n) put_state(k + 1);
-                
                 // ---- the output
                 ok = wait_for(o_full, cc & 1) && ok;
                 tc_fence_after();
@@ -790,21 +821,19 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 }
             }
             if (!ok) break;
-            {
-                // ---- rows past the sequence in this segment's whole chunks
-                const int end = min(t.first + p.per_seg, p.chunks);
-                const int64_t z0 = (int64_t)max(t.first + t.n, t.first) * kChunk, z1 = min((int64_t)end * kChunk, (int64_t)p.t);
-                T* const o = (T*)p.o + t.b * p.o_sb + t.h * p.o_sh;
-                for (int64_t r = z0 + warp; r < z1; r += kEpi / 32)
-                    for (int c = lane; c < p.dc; c += 32) o[r * p.o_st + c] = Elem<T>::store(0.f);
-                // ---- the state at the end, from the segment that got there (without tokens: as it was)
-                const bool mine = t.active == 0 ? t.seg == 0 : REV ? t.seg == 0 : t.n > 0 && t.first + t.n == t.active;
-                if (p.gout && mine && live && srow < p.da) {
-                    float* const dst = p.gout + (int64_t)t.bh * p.da * p.dc + (int64_t)srow * p.dc;
+            // ---- rows past the sequence in this segment's whole chunks
+            const int end = min(t.first + p.per_seg, p.chunks);
+            const int64_t z0 = (int64_t)max(t.first + t.n, t.first) * kChunk, z1 = min((int64_t)end * kChunk, (int64_t)p.t);
+            T* const o = (T*)p.o + t.b * p.o_sb + t.h * p.o_sh;
+            for (int64_t r = z0 + warp; r < z1; r += kEpi / 32)
+                for (int c = lane; c < p.dc; c += 32) o[r * p.o_st + c] = Elem<T>::store(0.f);
+            // ---- the state at the end, from the segment that got there (without tokens: as it was)
+            const bool mine = t.active == 0 ? t.seg == 0 : REV ? t.seg == 0 : t.n > 0 && t.first + t.n == t.active;
+            if (p.gout && mine && live && srow < p.da) {
+                float* const dst = p.gout + (int64_t)t.bh * p.da * p.dc + (int64_t)srow * p.dc;
 #pragma unroll
-                    for (int j = 0; j < 32 * W; ++j)
-                        if (col0 + j < p.dc) dst[col0 + j] = G[j] * p.gout_scale;
-                }
+                for (int j = 0; j < 32 * W; ++j)
+                    if (col0 + j < p.dc) dst[col0 + j] = G[j] * p.gout_scale;
             }
         }
         if (tid == 0 && p.tma_out) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -954,6 +983,11 @@ bool encode_heads(CUtensorMap* map, const Heads& x, const Sizes& z, int dtype) {
                         x.d > 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B);  // (a row, not its neighbours')
 }
 
+// Sums before a head's last segment (of 16 KB) from which a launch of their own joins them: at 6 (64 heads of 3136 tokens)
+// the three launches of a training step cost more than the segments' own loops, 208 against 200 us; at 136 (8 heads of
+// 65536 tokens, size 128) they save, 277 -> 225 us.
+constexpr int kJoinFrom = 16;
+
 int blocks_of(int64_t da, int64_t dc) { return da <= 64 && dc <= 64 ? 1 : 2; }
 
 // Segments per sequence, and units of the sums that segments need of those before them.
@@ -1008,6 +1042,8 @@ void launch_mix(MixArgs a, int64_t bh, cudaStream_t st) {
         allow_smem<sums>(ends_smem<W>());
         a.items = (int)(bh * (a.nseg - 1) * a.units);
         launch_early(sums, (unsigned)std::min(a.items, slots), kThreads, ends_smem<W>(), 1, st, a);
+        constexpr auto join = decay_join_kernel<W, REV>;
+        if (a.joined) launch_early(join, (unsigned)(bh * (4 * W * W)), 256, 0, 1, st, a);
     }
     constexpr auto kernel = decay_mix_kernel<T, W, REV>;
     allow_smem<kernel>(mix_smem<W>());
@@ -1033,6 +1069,7 @@ int run_mix(const Mix& m, const Sizes& z, const float* log_decay, const int64_t*
     p.chunks = (int)((z.t + kChunk - 1) / kChunk);
     const Deal d = deal(z, w);
     p.nseg = d.nseg, p.per_seg = d.per_seg, p.unit = d.unit, p.units = d.units;
+    p.joined = (d.nseg - 1) * d.units * w * w > kJoinFrom;
     p.g0_row = m.transposed ? 1 : p.dc, p.g0_col = m.transposed ? p.da : 1;
     p.scale = (float)scale, p.g0_scale = m.rev ? (float)(1.0 / scale) : 1.f, p.gout_scale = m.rev ? (float)scale : 1.f;
     p.ksteps = (p.da + 15) / 16, p.nb = (p.dc + 15) / 16 * 16;
