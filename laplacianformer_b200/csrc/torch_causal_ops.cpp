@@ -224,8 +224,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
                                  const c10::optional<at::Tensor>& positions, int64_t offset, bool interleaved, double magnitude) {
         at::AutoDispatchBelowADInplaceOrView below;
         auto [y, z] = Rotary_forward(q, opt(k), frequencies, opt(positions), offset, interleaved, magnitude, false);
-        ctx->save_for_backward({opt(positions)});
-        ctx->saved_data["frequencies"] = frequencies;
+        ctx->save_for_backward({opt(positions), frequencies});
         ctx->saved_data["offset"] = offset;
         ctx->saved_data["interleaved"] = interleaved;
         ctx->saved_data["magnitude"] = magnitude;
@@ -236,12 +235,12 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         first_order("rotary");
-        const at::Tensor positions = ctx->get_saved_variables()[0];
+        const auto s = ctx->get_saved_variables();
         const bool k = ctx->saved_data["k"].toBool();
         at::Tensor dq = ctx->needs_input_grad(0) ? g[0] : at::Tensor(), dk = k && ctx->needs_input_grad(1) ? g[1] : at::Tensor();
         const bool nq = dq.defined(), nk = dk.defined();
         if (nq || nk) {
-            auto [a, b] = Rotary_forward(nq ? dq : dk, nq ? dk : at::Tensor(), ctx->saved_data["frequencies"].toTensor(), positions,
+            auto [a, b] = Rotary_forward(nq ? dq : dk, nq ? dk : at::Tensor(), s[1], s[0],
                                          ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(),
                                          ctx->saved_data["magnitude"].toDouble(), true);
             if (nq) dq = a, dk = b;

@@ -349,6 +349,15 @@ def test_attention_training_step_captured():
     assert all(torch.equal(a, c) for a, c in zip(out, step()))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("t, dk, dv, lengths", [(5000, 64, 48, [5000, 2111]), (4000, 128, 128, [1, 2500]), (3840, 64, 64, [3839, 0])])
+def test_attention_many_segments(t, dk, dv, lengths, dtype):
+    """Few heads of long sequences, dealt to many blocks whose sums are joined before them."""
+    g = gen(t)
+    check_attention(heads(g, 2, 1, t, dk, dtype), heads(g, 2, 1, t, dk, dtype), heads(g, 2, 1, t, dv, dtype), torch.tensor([-0.003], device="cuda"),
+                    state=rand(g, 2, 1, dk, dv, scale=3.0), lengths=torch.tensor(lengths, device="cuda"))
+
+
 def test_attention_many_sequences_long_offsets():
     """Elements past 2^31: the last sequences of a large batch are their own calls' results."""
     b, h, t, d = 530, 8, 8192, 64
