@@ -61,6 +61,7 @@ struct alignas(64) MixArgs {
     int heads, t, da, dc, chunks, nseg, per_seg, items;
     int unit, units;         // chunks per unit, units per segment
     int joined;              // a segment finds the state before it in the slot of its unit that is first in time
+    int turned;              // the sums are there already, transposed
     int g0_row, g0_col;      // strides within a state matrix (transposed for dq and dk)
     float scale, g0_scale, gout_scale;
     int ksteps, nb;          // 16-column steps of da; dc rounded up to 16
@@ -146,6 +147,12 @@ template <typename T> __device__ __forceinline__ uint32_t fma16x2(uint32_t a, ui
     uint32_t r;
     if constexpr (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     else asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// (The hardware's power of two, about 2 units in the last place, for factors that meet a 16-bit rounding.)
+__device__ __forceinline__ float exp2_of(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 // The lowest n bits (none below 0, all from 32 on).
@@ -237,6 +244,11 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int thread, 
     }
 }
 
+// Whether nothing is left of unit u of a segment where the next segment (in time) begins: such units are neither summed nor read.
+__device__ __forceinline__ bool forgotten(const MixArgs& p, float g, int u, bool rev) {
+    return power(g, (int64_t)(rev ? u * p.unit : max(0, p.per_seg - (u + 1) * p.unit)) * kChunk) == 0.f;
+}
+
 // What units of chunks add to the state, for the segments that go on after them: sum_j l^(n-j) b_j c_j^T with all weights
 // taken to the unit's end, so that the products of its chunks follow one another on one accumulator (weights that
 // underflow are of tokens that do not matter any more).  Two warps copy and multiply, eight scale b.
@@ -279,6 +291,7 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
         const int end = min(min(x.first + p.unit, (seg + 1) * p.per_seg), p.chunks), active = (int)((x.len + kChunk - 1) / kChunk);
         // Forwards only whole units are asked for.
         x.n = REV ? max(0, min(end, active) - x.first) : end > x.first && (int64_t)end * kChunk <= x.len ? end - x.first : 0;
+        if (forgotten(p, p.log_decay[x.h], u, REV)) x.n = 0;
         return x;
     };
     const int count = p.items;
@@ -408,6 +421,7 @@ __global__ void __launch_bounds__(256) decay_join_kernel(const __grid_constant__
     auto length = [&](int u) { return min(p.unit, p.per_seg - u % p.units * p.unit); };
     auto there = [&](int u) {
         const int seg = u / p.units, from = first(u);
+        if (forgotten(p, g, u % p.units, REV)) return false;
         return REV ? seg > 0 && from < active : seg < p.nseg - 1 && (int64_t)(from + length(u)) * kChunk <= len;
     };
     const float wu = power(g, (int64_t)p.unit * kChunk), wl = power(g, (int64_t)length(p.units - 1) * kChunk);
@@ -444,9 +458,8 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     uint8_t* const low = ring + kRing * kTile;
     uint8_t* const gop = low + kTile;                                         // [state row][dc], 64 columns a block
     float* const pw = reinterpret_cast<float*>(gop + kState * 128 * W);       // l^n, n = 0..128
-    float* const factors = pw + 132;                                          // of the scores, see there: two copies, 176 apart
-    uint32_t* const gmax = reinterpret_cast<uint32_t*>(factors + 340);
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 474);
+    uint32_t* const gmax = reinterpret_cast<uint32_t*>(pw + 132);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 134);
     uint64_t *full = bars, *empty = bars + kRing, *s_full = bars + 2 * kRing, *k_ready = s_full + 1, *p_ready = s_full + 2,
              *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7;
     uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 8);
@@ -553,14 +566,11 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
         const bool live = W == 2 || lane < 16;
         const int col0 = half * 32 * W;                           // this thread's columns of the state and of the output
         const int kr = tid >> 1, kpart = tid & 1;                 // the row of b, and half of it, that this thread scales
-        // Factors scale l^(i-j) of this thread's row i, from column 0 on: pairs of them are 8-byte loads from the copy
-        // that has them on that boundary (half a warp's loads meet no bank twice).  Past the diagonal they are 0.
-        const int f0 = REV ? 32 - row : 127 - row;
-        const float* const frow = factors + (f0 & 1 ? 177 : 0) + f0;
         int n = 0, cc = 0, qg = 0, puts = 0;
         for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
             const Item t = item_of(p, i);
             const float g = p.log_decay[t.h];
+            const float g2 = fmaxf(g, -1e30f) * 1.44269504f, l1 = exp2_of(g2);  // (times 0 steps: 0)
             const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
             bool has_g = (p.g0 || (t.n > 0 && t.seg != first_seg));
             float G[32 * W], unscale = 1.f;
@@ -612,10 +622,6 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             };
             epi_sync(true);  // the tables' last readers are done
             if (tid <= kChunk) pw[tid] = power(g, tid);
-            if (tid < 160) {
-                const int d = REV ? tid - 32 : 127 - tid;
-                factors[tid] = factors[176 + tid + 1] = d < 0 ? 0.f : power(g, d) * p.scale;
-            }
             // ---- the state before this segment
 #pragma unroll
             for (int j = 0; j < 32 * W; ++j) G[j] = 0.f;
@@ -639,12 +645,18 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                         for (int v = p.joined ? mine : 0; p.joined ? v == mine : from + v * p.unit < to; ++v) {
                             const int64_t after = REV ? from + v * p.unit - here : here - min(from + (v + 1) * p.unit, to);
                             const float w = p.joined ? 1.f : power(g, after * kChunk);
-                            const float4* e = reinterpret_cast<const float4*>(p.ends + ((((int64_t)t.bh * p.nseg + u) * p.units + v) * kState + srow) * kState + col0);
+                            if (w == 0.f) continue;  // forgotten: not summed either
+                            const float* const e = p.ends + (((int64_t)t.bh * p.nseg + u) * p.units + v) * (kState * kState);
+                            if (p.turned) {
 #pragma unroll
-                            for (int j = 0; j < 8 * W; ++j) {
-                                const float4 x = e[j];
-                                G[4 * j] = __fmaf_rn(w, x.x, G[4 * j]), G[4 * j + 1] = __fmaf_rn(w, x.y, G[4 * j + 1]);
-                                G[4 * j + 2] = __fmaf_rn(w, x.z, G[4 * j + 2]), G[4 * j + 3] = __fmaf_rn(w, x.w, G[4 * j + 3]);
+                                for (int j = 0; j < 32 * W; ++j) G[j] = __fmaf_rn(w, e[(col0 + j) * kState + srow], G[j]);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 8 * W; ++j) {
+                                    const float4 x = reinterpret_cast<const float4*>(e + srow * kState + col0)[j];
+                                    G[4 * j] = __fmaf_rn(w, x.x, G[4 * j]), G[4 * j + 1] = __fmaf_rn(w, x.y, G[4 * j + 1]);
+                                    G[4 * j + 2] = __fmaf_rn(w, x.z, G[4 * j + 2]), G[4 * j + 3] = __fmaf_rn(w, x.w, G[4 * j + 3]);
+                                }
                             }
                         }
                     }
@@ -713,7 +725,10 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 }
                 fence_async_smem();
                 arrive(k_ready);
-                // ---- weighted scores: row `row`, columns 64 half on, in blocks of 32
+                // ---- weighted scores: row `row`, columns 64 half on, in blocks of 32.  Their factors scale l^(i-j) are made
+                // here: loads from a table in shared memory wait for the products' operands, which go first (a block of 32
+                // columns took 1100 cycles so, 700 now; 8 heads of 65536 tokens, size 128: 228 -> 217 us; with two blocks
+                // per SM, which wait in turn, no difference).
 #pragma unroll 1
                 for (int bl = 0; bl < 2; ++bl) {
                     const int blk = half * 2 + bl;
@@ -724,16 +739,34 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     } else {
                         float v[32];
                         tmem_ld32(tq + blk * 32, v);
-                        const float2* f = reinterpret_cast<const float2*>(frow + blk * 32);
                         tmem_wait_ld();
                         reg_fence(v);
+                        // Two factors at once, of columns 16 apart, from the furthest columns on: each is l times the last, and
+                        // scale on the diagonal (0 before it).
+                        const int d = REV ? blk * 32 - row : row - blk * 32 - 15;  // steps to the first of the two columns
+                        const int d2 = REV ? d + 16 : d - 16;
+                        const float x0 = exp2_of((float)max(d, 0) * g2) * p.scale, y0 = exp2_of((float)max(d2, 0) * g2) * p.scale;
+                        uint64_t f = pk2(d >= 0 ? x0 : 0.f, d2 >= 0 ? y0 : 0.f);
+                        if (blk == quad) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const float2 c = f[j];
-                            float a, b;
-                            upk2(mul2(pk2(v[2 * j], v[2 * j + 1]), pk2(c.x, c.y)), a, b);
-                            u[j] = pack2<T>(a, b);
+                            for (int i = 0; i < 16; ++i) {
+                                const int j = REV ? i : 15 - i;
+                                upk2(mul2(pk2(v[j], v[j + 16]), f), v[j], v[j + 16]);
+                                float x, y;
+                                upk2(mul2(f, pk2(l1, l1)), x, y);
+                                const int next = REV ? j + 1 : j - 1;
+                                f = pk2(lane == next ? p.scale : x, lane == next + 16 ? p.scale : y);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int j = REV ? i : 15 - i;
+                                upk2(mul2(pk2(v[j], v[j + 16]), f), v[j], v[j + 16]);
+                                f = mul2(f, pk2(l1, l1));
+                            }
                         }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) u[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
                         if (L < kChunk) {  // (a product with what lies past the sequence may not be finite)
 #pragma unroll
                             for (int j = 0; j < 16; ++j) u[j] &= keep_low(16 * (L - blk * 32) - 32 * j);
@@ -1037,7 +1070,7 @@ void allow_smem(int bytes) {
 template <typename T, int W, bool REV>
 void launch_mix(MixArgs a, int64_t bh, cudaStream_t st) {
     const int slots = num_sms() * (W == 1 ? 2 : 1);
-    if (a.nseg > 1) {
+    if (a.nseg > 1 && !a.turned) {
         constexpr auto sums = decay_ends_kernel<T, W, REV>;
         allow_smem<sums>(ends_smem<W>());
         a.items = (int)(bh * (a.nseg - 1) * a.units);
@@ -1057,6 +1090,7 @@ struct Mix {
     float* gout = nullptr;
     bool transposed = false;  // the state matrices are [dc][da]
     bool rev = false;
+    bool turned = false;      // a call before has left the sums of c_j b_j^T
 };
 
 int run_mix(const Mix& m, const Sizes& z, const float* log_decay, const int64_t* lengths, double scale, int dtype, float* ends,
@@ -1069,6 +1103,7 @@ int run_mix(const Mix& m, const Sizes& z, const float* log_decay, const int64_t*
     p.chunks = (int)((z.t + kChunk - 1) / kChunk);
     const Deal d = deal(z, w);
     p.nseg = d.nseg, p.per_seg = d.per_seg, p.unit = d.unit, p.units = d.units;
+    p.turned = m.turned;
     p.joined = (d.nseg - 1) * d.units * w * w > kJoinFrom;
     p.g0_row = m.transposed ? 1 : p.dc, p.g0_col = m.transposed ? p.da : 1;
     p.scale = (float)scale, p.g0_scale = m.rev ? (float)(1.0 / scale) : 1.f, p.gout_scale = m.rev ? (float)scale : 1.f;
@@ -1203,17 +1238,19 @@ extern "C" int lf_decay_attention_bwd(const lf_decay_attention_t* a, void* works
     const Heads k = addressable(heads_of(a->k, a->k_strides, a->key_size), z, at, st);
     const Heads v = addressable(heads_of(a->v, a->v_strides, a->value_size), z, at, st);
     const Heads g = addressable(heads_of(a->d_o, a->do_strides, a->value_size), z, at, st);
-    auto mix = [&](const Heads& x, const Heads& y, const Heads& w, void* out, const float* g0, float* gout, bool transposed, bool rev) {
+    auto mix = [&](const Heads& x, const Heads& y, const Heads& w, void* out, const float* g0, float* gout, bool transposed, bool rev,
+                   bool turned) {
         Mix m;
-        m.a = x, m.b = y, m.c = w, m.out = dense_heads(out, z, w.d), m.g0 = g0, m.gout = gout, m.transposed = transposed, m.rev = rev;
+        m.a = x, m.b = y, m.c = w, m.out = dense_heads(out, z, w.d), m.g0 = g0, m.gout = gout, m.transposed = transposed, m.rev = rev, m.turned = turned;
         return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, (float*)at, st);
     };
     if (a->dq)
-        if (int rc = mix(g, v, k, a->dq, a->state, nullptr, true, false)) return rc;
+        if (int rc = mix(g, v, k, a->dq, a->state, nullptr, true, false, false)) return rc;
     if (a->dk)
-        if (int rc = mix(v, g, q, a->dk, a->d_state_out, nullptr, true, true)) return rc;
+        if (int rc = mix(v, g, q, a->dk, a->d_state_out, nullptr, true, true, false)) return rc;
     if (a->dv)
-        if (int rc = mix(k, q, g, a->dv, a->d_state_out, a->d_state, false, true)) return rc;
+        // (dk has left the sums of do q^T)
+        if (int rc = mix(k, q, g, a->dv, a->d_state_out, a->d_state, false, true, a->dk != nullptr)) return rc;
     return LF_OK;
 }
 
