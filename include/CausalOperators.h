@@ -13,15 +13,15 @@
 
 namespace laplace {
 
-// (o, state after the last token, or undefined).
+// (o, state after the last token, or undefined).  sums: filled for the backward, which then sums less (may stay undefined).
 std::tuple<at::Tensor, at::Tensor> DecayAttention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                           const at::Tensor& log_decay, const at::Tensor& state, const at::Tensor& lengths,
-                                                          double scale, bool want_state);
+                                                          double scale, bool want_state, at::Tensor* sums = nullptr);
 // (dq, dk, dv, d_state) from d_o and the gradient d_state of the last state (may be undefined).
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> DecayAttention_backward(
     const at::Tensor& d_o, const at::Tensor& d_state, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& log_decay, const at::Tensor& state, const at::Tensor& lengths, double scale, bool need_q, bool need_k, bool need_v,
-    bool need_state);
+    bool need_state, const at::Tensor& sums = {});
 // One token: heads are [batch, heads, size]; `state` is updated in place.
 at::Tensor DecayAttention_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
                                const at::Tensor& state, double scale);

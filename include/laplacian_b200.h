@@ -480,7 +480,10 @@ LF_API int lf_clip_grad_norm(const void* const* grads, void* const* outs, const 
    backward) are operands of a second product in dtype: in fp16 they become
    infinite beyond 65504.  A value that is not finite reaches all outputs of its
    128-token chunk.  Workspaces are 256-byte aligned; their sizes depend on the
-   sizes, strides and pointers: ask with the struct that will run. */
+   sizes, strides and pointers: ask with the struct that will run.
+   sums: NULL, or lf_decay_attention_sums_size() bytes, 256-byte aligned, which
+   the forward fills and the backward of the same call reads, instead of summing
+   keys and values again for dq. */
 typedef struct lf_decay_attention {
     const void *q, *k, *v;
     const float *log_decay, *state;
@@ -490,13 +493,14 @@ typedef struct lf_decay_attention {
     const void* d_o;
     const float* d_state_out;
     void *dq, *dk, *dv;
-    float* d_state;
+    float *d_state, *sums;
     int64_t q_strides[3], k_strides[3], v_strides[3], do_strides[3];
     int64_t b, h, t, key_size, value_size;
     double scale;
     int32_t dtype;
 } lf_decay_attention_t;
 
+LF_API size_t lf_decay_attention_sums_size(const lf_decay_attention_t* args);
 LF_API size_t lf_decay_attention_fwd_workspace_size(const lf_decay_attention_t* args);
 LF_API int lf_decay_attention_fwd(const lf_decay_attention_t* args, void* workspace, size_t workspace_bytes, lf_stream_t stream);
 LF_API size_t lf_decay_attention_bwd_workspace_size(const lf_decay_attention_t* args);

@@ -50,7 +50,7 @@ class DecayAttention(ctypes.Structure):
     """lf_decay_attention_t: causal linear attention with a decay per head, and its gradients."""
 
     _fields_ = ([(n, _P) for n in ("q", "k", "v", "log_decay", "state", "lengths", "o", "state_out", "d_o", "d_state_out", "dq", "dk",
-                                   "dv", "d_state")]
+                                   "dv", "d_state", "sums")]
                 + [(n, _I64 * 3) for n in ("q_strides", "k_strides", "v_strides", "do_strides")]
                 + [(n, _I64) for n in ("b", "h", "t", "key_size", "value_size")] + [("scale", _D), ("dtype", ctypes.c_int32)])
 
@@ -134,6 +134,7 @@ SIGNATURES = {
     "lf_gated_ffn_bwd": (_I, [_FFN, _P, _SZ, _P]),
     "lf_clip_grad_norm_workspace_size": (_SZ, [_P, _I64]),
     "lf_clip_grad_norm": (_I, [_P, _P, _P, _P, _I64, _D, _P, _P, _SZ, _P]),
+    "lf_decay_attention_sums_size": (_SZ, [_DEC]),
     "lf_decay_attention_fwd_workspace_size": (_SZ, [_DEC]),
     "lf_decay_attention_fwd": (_I, [_DEC, _P, _SZ, _P]),
     "lf_decay_attention_bwd_workspace_size": (_SZ, [_DEC]),

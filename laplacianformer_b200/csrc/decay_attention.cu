@@ -19,6 +19,20 @@
 // scores (once), the state that q meets (once; fp16: scaled by a power of two
 // into its range), and l^(n-j) b_j, which goes in as two 16-bit parts so that
 // the state keeps about 17 bits (bf16) or 22 (fp16) of each term.
+//
+// What bounds it.  Sequences are cut into segments until every block slot has
+// one (two slots per SM for heads up to 64); the state before a segment comes
+// from a launch that reads b and c of the segments before.  Where heads fill the
+// slots without cuts the main launch is memory bound: 296 heads of 7168 tokens,
+// bf16, size 64: 208 us, 5.2 TB/s.  8x16x16384x64: 240 us and 45 us for the
+// sums, since 256 segments leave 40 slots empty.  A training step is four mixes
+// and two sums (dq takes the forward's, dv those of dk, transposed): 1.21 ms; with
+// four sums 1.36.  Few chunks per slot (32x2x3136x32 172 us, 128x8x196x64 148 us
+// a training step) are bound by a chunk's chain: products, weights, products,
+// output, about 5200 cycles for a pair of blocks.
+// Between 64 and 128 one block fits an SM and waits on that chain alone: 8 heads
+// of 65536 tokens, size 128: 210 us, 2.6 TB/s.
+// A token at a time only the state matters: 192x16 heads of 64: 15 us, 6.7 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -61,7 +75,7 @@ struct alignas(64) MixArgs {
     int heads, t, da, dc, chunks, nseg, per_seg, items;
     int unit, units;         // chunks per unit, units per segment
     int joined;              // a segment finds the state before it in the slot of its unit that is first in time
-    int turned;              // the sums are there already, transposed
+    int turned;              // the sums are there already, transposed (of b and c the other way round)
     int g0_row, g0_col;      // strides within a state matrix (transposed for dq and dk)
     float scale, g0_scale, gout_scale;
     int ksteps, nb;          // 16-column steps of da; dc rounded up to 16
@@ -1160,6 +1174,7 @@ int check_attention(const char* what, const lf_decay_attention_t* a, bool bwd) {
                           (const void*)a->d_state})
         if (!aligned(p, 4)) return refuse(what, "a pointer is not aligned to its elements");
     if (!aligned(a->lengths, 8)) return refuse(what, "a pointer is not aligned to its elements");
+    if (!aligned(a->sums, 256)) return refuse(what, "sums must be 256-byte aligned");
     if (a->b == 0 || a->h == 0) return LF_OK;
     if (!a->log_decay) return refuse(what, "log_decay is required");
     if (a->t > 0 && (!a->q || !a->k || !a->v || (!bwd && !a->o) || (bwd && !a->d_o))) return refuse(what, "q, k, v and the output or its gradient are required");
@@ -1182,11 +1197,16 @@ int pass_state(const char* what, const float* from, float* to, size_t bytes, cud
 
 using namespace lfb;
 
+extern "C" size_t lf_decay_attention_sums_size(const lf_decay_attention_t* a) {
+    if (!a || check_sizes("lf_decay_attention_sums_size", a->b, a->h, a->t, a->key_size, a->value_size) || a->b == 0 || a->h == 0 || a->t == 0) return 0;
+    return ends_bytes({a->b, a->h, a->t}, blocks_of(a->key_size, a->value_size));
+}
+
 extern "C" size_t lf_decay_attention_fwd_workspace_size(const lf_decay_attention_t* a) {
     if (!a || check_attention("lf_decay_attention_fwd", a, false) || a->b == 0 || a->h == 0 || a->t == 0) return 0;
     const Sizes z{a->b, a->h, a->t};
     return packed_bytes(heads_of(a->q, a->q_strides, a->key_size), z) + packed_bytes(heads_of(a->k, a->k_strides, a->key_size), z) +
-           packed_bytes(heads_of(a->v, a->v_strides, a->value_size), z) + ends_bytes(z, blocks_of(a->key_size, a->value_size));
+           packed_bytes(heads_of(a->v, a->v_strides, a->value_size), z) + (a->sums ? 0 : ends_bytes(z, blocks_of(a->key_size, a->value_size)));
 }
 
 extern "C" int lf_decay_attention_fwd(const lf_decay_attention_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
@@ -1209,7 +1229,7 @@ extern "C" int lf_decay_attention_fwd(const lf_decay_attention_t* a, void* works
     m.c = addressable(heads_of(a->v, a->v_strides, a->value_size), z, at, st);
     m.out = dense_heads(a->o, z, a->value_size);
     m.g0 = a->state, m.gout = a->state_out;
-    return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, (float*)at, st);
+    return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, a->sums ? a->sums : (float*)at, st);
 }
 
 extern "C" size_t lf_decay_attention_bwd_workspace_size(const lf_decay_attention_t* a) {
@@ -1242,14 +1262,14 @@ extern "C" int lf_decay_attention_bwd(const lf_decay_attention_t* a, void* works
                    bool turned) {
         Mix m;
         m.a = x, m.b = y, m.c = w, m.out = dense_heads(out, z, w.d), m.g0 = g0, m.gout = gout, m.transposed = transposed, m.rev = rev, m.turned = turned;
-        return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, (float*)at, st);
+        return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, turned && !rev ? a->sums : (float*)at, st);
     };
+    // The segments' sums for dq are the forward's, those for dv are dk's, transposed.
     if (a->dq)
-        if (int rc = mix(g, v, k, a->dq, a->state, nullptr, true, false, false)) return rc;
+        if (int rc = mix(g, v, k, a->dq, a->state, nullptr, true, false, a->sums != nullptr)) return rc;
     if (a->dk)
         if (int rc = mix(v, g, q, a->dk, a->d_state_out, nullptr, true, true, false)) return rc;
     if (a->dv)
-        // (dk has left the sums of do q^T)
         if (int rc = mix(k, q, g, a->dv, a->d_state_out, a->d_state, false, true, a->dk != nullptr)) return rc;
     return LF_OK;
 }

@@ -518,33 +518,40 @@ __global__ void __launch_bounds__(512) sandwich_bwd_long_kernel(const SandwichAr
     }
 }
 
-// Rows of sums from their partial rows, joined in order: dw, dwn and the gate's
-// rows (blockIdx.y), 32 columns per block and 32 strided partial sums per column.
+// Rows of sums from their partial rows, joined in order, 32 columns per block: dw and dwn by all 32 warps, and four of
+// the gate's rows at a time by 8 warps each (their partial rows are few; there may be more of them than a grid is high).
 struct JoinArgs {
     const float* part[3];
     void* out[3];
-    int64_t cols, parts[3];
+    int64_t cols, parts[3], gates;
 };
+constexpr int kGateWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(1024) sandwich_join_kernel(const JoinArgs p) {
     __shared__ float sh[32][33];
     grid_release();
     grid_wait();
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const int job = min(2, (int)blockIdx.y);
-    const int64_t row = job == 2 ? blockIdx.y - 2 : 0, c = (int64_t)blockIdx.x * 32 + lane, n = p.parts[job];
+    const int job = min(2, (int)blockIdx.y), warps = job == 2 ? kGateWarps : 32;
     if (!p.out[job]) return;
-    const float* part = p.part[job] + row * n * p.cols;
-    float t = 0.f;
-    if (c < p.cols)
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane, n = p.parts[job], rows = job == 2 ? p.gates : 1;
+    const int per = 32 / warps, stride = ((int)gridDim.y - 2) * per;
+    for (int64_t row0 = job == 2 ? ((int)blockIdx.y - 2) * per : 0; row0 < rows; row0 += stride) {
+        const int64_t row = row0 + k / warps;
+        const bool in = c < p.cols && row < rows;
+        const float* part = p.part[job] + row * n * p.cols;
+        float t = 0.f;
+        if (in)
 #pragma unroll 8
-        for (int64_t b = k; b < n; b += 32) t += part[b * p.cols + c];
-    sh[k][lane] = t;
-    __syncthreads();
-    if (k == 0 && c < p.cols) {
-#pragma unroll
-        for (int i = 1; i < 32; ++i) t += sh[i][lane];
-        ((T*)p.out[job])[row * p.cols + c] = Elem<T>::store(t);
+            for (int64_t b = k % warps; b < n; b += warps) t += part[b * p.cols + c];
+        sh[k][lane] = t;
+        __syncthreads();
+        if (in && k % warps == 0) {
+            for (int i = 1; i < warps; ++i) t += sh[k + i][lane];
+            ((T*)p.out[job])[row * p.cols + c] = Elem<T>::store(t);
+        }
+        if (job != 2) return;
+        __syncthreads();
     }
 }
 
@@ -721,8 +728,8 @@ extern "C" int lf_sandwich_norm_bwd(const lf_sandwich_norm_t* a, void* workspace
     else if (a->dtype == LF_F16) launch_sandwich_bwd<__half>(p, vec, most, &blocks, st);
     else launch_sandwich_bwd<__nv_bfloat16>(p, vec, most, &blocks, st);
     if (p.part_w || p.part_wn || p.part_g) {
-        JoinArgs j{{p.part_w, p.part_wn, p.part_g}, {a->d_weight, a->d_next_weight, p.part_g ? a->d_gate : nullptr}, p.cols, {blocks, blocks, u.parts}};
-        const dim3 grid((unsigned)((p.cols + 31) / 32), (unsigned)(p.part_g ? 2 + u.groups : 2));
+        JoinArgs j{{p.part_w, p.part_wn, p.part_g}, {a->d_weight, a->d_next_weight, p.part_g ? a->d_gate : nullptr}, p.cols, {blocks, blocks, u.parts}, u.groups};
+        const dim3 grid((unsigned)((p.cols + 31) / 32), (unsigned)(p.part_g ? 2 + std::min<int64_t>((u.groups * kGateWarps + 31) / 32, 65000) : 2));
         if (a->dtype == LF_F32) launch_early(sandwich_join_kernel<float>, grid, 1024, 0, 1, st, j);
         else if (a->dtype == LF_F16) launch_early(sandwich_join_kernel<__half>, grid, 1024, 0, 1, st, j);
         else launch_early(sandwich_join_kernel<__nv_bfloat16>, grid, 1024, 0, 1, st, j);

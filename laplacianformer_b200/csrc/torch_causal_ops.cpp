@@ -66,10 +66,14 @@ DecayCall decay_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
 
 std::tuple<at::Tensor, at::Tensor> DecayAttention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                           const at::Tensor& log_decay, const at::Tensor& state, const at::Tensor& lengths,
-                                                          double scale, bool want_state) {
+                                                          double scale, bool want_state, at::Tensor* sums) {
     need_cuda(q, "q");
     c10::cuda::CUDAGuard guard(q.device());
     DecayCall c = decay_call(q, k, v, log_decay, state, lengths, scale);
+    if (sums) {
+        *sums = workspace(lf_decay_attention_sums_size(&c.a), q);
+        c.a.sums = (float*)mut(*sums);
+    }
     at::Tensor o = fresh_heads(q, c.a.value_size), out;
     if (want_state) out = fresh({c.a.b, c.a.h, c.a.key_size, c.a.value_size}, at::kFloat, q);
     c.a.o = mut(o), c.a.state_out = (float*)mut(out);
@@ -82,10 +86,11 @@ std::tuple<at::Tensor, at::Tensor> DecayAttention_forward(const at::Tensor& q, c
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> DecayAttention_backward(
     const at::Tensor& d_o_, const at::Tensor& d_state_, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& log_decay, const at::Tensor& state, const at::Tensor& lengths, double scale, bool need_q, bool need_k, bool need_v,
-    bool need_state) {
+    bool need_state, const at::Tensor& sums) {
     need_cuda(q, "q");
     c10::cuda::CUDAGuard guard(q.device());
     DecayCall c = decay_call(q, k, v, log_decay, state, lengths, scale);
+    if (sums.defined()) c.a.sums = (float*)sums.data_ptr();
     check_operand(d_o_, q, "d_o");
     check_shape(d_o_, v.sizes(), "d_o");
     if (d_state_.defined()) check_state(d_state_, q, c.a.key_size, c.a.value_size, "d_state");
@@ -141,8 +146,9 @@ struct DecayAttentionNode : torch::autograd::Function<DecayAttentionNode> {
                                  const at::Tensor& log_decay, const c10::optional<at::Tensor>& state,
                                  const c10::optional<at::Tensor>& lengths, double scale, bool want_state) {
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [o, out] = DecayAttention_forward(q, k, v, log_decay, opt(state), opt(lengths), scale, want_state);
-        ctx->save_for_backward({q, k, v, log_decay, opt(state), opt(lengths)});
+        at::Tensor sums;  // (a few matrices per head, where sequences are long and heads few)
+        auto [o, out] = DecayAttention_forward(q, k, v, log_decay, opt(state), opt(lengths), scale, want_state, q.requires_grad() ? &sums : nullptr);
+        ctx->save_for_backward({q, k, v, log_decay, opt(state), opt(lengths), sums});
         ctx->saved_data["scale"] = scale;
         ctx->set_materialize_grads(false);
         if (want_state) return {o, out};
@@ -159,7 +165,7 @@ struct DecayAttentionNode : torch::autograd::Function<DecayAttentionNode> {
         if (g[0].defined() || d_state.defined()) {
             const at::Tensor d_o = g[0].defined() ? g[0] : at::zeros_like(s[2]);  // only the state was used
             std::tie(dq, dk, dv, ds) = DecayAttention_backward(d_o, d_state, s[0], s[1], s[2], s[3], s[4], s[5],
-                                                               ctx->saved_data["scale"].toDouble(), nq, nk, nv, ns);
+                                                               ctx->saved_data["scale"].toDouble(), nq, nk, nv, ns, s[6]);
         }
         return {dq, dk, dv, at::Tensor(), ds, at::Tensor(), at::Tensor(), at::Tensor()};
     }

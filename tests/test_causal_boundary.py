@@ -45,6 +45,13 @@ def test_attention_workspaces():
     assert L.lf_decay_attention_fwd_workspace_size(odd) == (2 * 100 * 3 * 40 * 2 + 255) // 256 * 256
     assert L.lf_decay_attention_fwd(odd, None, 0, None) == capi.LF_ERR_INVALID and b"workspace" in L.lf_last_error()
     assert L.lf_decay_attention_fwd(odd, P + 16, 1 << 30, None) == capi.LF_ERR_INVALID
+    long = attention(t=5000, **{n + "_strides": strides(3, 5000, d) for n, d in (("q", 64), ("k", 64), ("v", 32))})
+    need = L.lf_decay_attention_sums_size(long)  # of the segments that a sequence is cut into, 64x64 floats each
+    assert need > 0 and need % (64 * 64 * 4) == 0 and L.lf_decay_attention_fwd_workspace_size(long) == need
+    long.sums = P
+    assert L.lf_decay_attention_fwd_workspace_size(long) == 0
+    assert L.lf_decay_attention_fwd(attention(sums=P + 16), None, 0, None) == capi.LF_ERR_INVALID and b"sums" in L.lf_last_error()
+    assert L.lf_decay_attention_sums_size(attention()) == 0 and L.lf_decay_attention_sums_size(None) == 0
     assert L.lf_decay_attention_bwd(attention(), None, 0, None) == capi.LF_ERR_INVALID  # no d_o
     assert L.lf_decay_attention_bwd(attention(d_o=P, d_state=P), None, 0, None) == capi.LF_ERR_INVALID  # the state's gradient without dv
 
