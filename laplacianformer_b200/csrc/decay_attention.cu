@@ -27,7 +27,7 @@
 // bf16, size 64: 208 us, 5.2 TB/s.  8x16x16384x64: 240 us and 45 us for the
 // sums, since 256 segments leave 40 slots empty.  A training step is four mixes
 // and two sums (dq takes the forward's, dv those of dk, transposed): 1.21 ms; with
-// four sums 1.36.  Few chunks per slot (32x2x3136x32 172 us, 128x8x196x64 148 us
+// four sums 1.36.  Few chunks per slot (32x2x3136x32 180 us, 128x8x196x64 150 us
 // a training step) are bound by a chunk's chain: products, weights, products,
 // output, about 5200 cycles for a pair of blocks.
 // Between 64 and 128 one block fits an SM and waits on that chain alone: 8 heads
@@ -265,7 +265,9 @@ __device__ __forceinline__ bool forgotten(const MixArgs& p, float g, int u, bool
 
 // What units of chunks add to the state, for the segments that go on after them: sum_j l^(n-j) b_j c_j^T with all weights
 // taken to the unit's end, so that the products of its chunks follow one another on one accumulator (weights that
-// underflow are of tokens that do not matter any more).  Two warps copy and multiply, eight scale b.
+// underflow are of tokens that do not matter any more).  Two warps copy and multiply, eight scale b.  The products of the
+// second parts have an accumulator of their own: a product cuts its sum off at the accumulator's last bit, and those sums
+// are small.
 template <typename T, int W, bool REV>
 __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W, kTiles = kEndsRing<W>;
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
         mbar_init(done, 1), mbar_init(read, kEpi / 2), mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) tmem_alloc(tmem_ptr, 128);
+    if (warp == 9) tmem_alloc(tmem_ptr, 2 * kState);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
 #pragma unroll
                 for (int s = 0; s < 8; ++s) mma_f16(tmem, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, k > 0 || s > 0 ? 1u : 0u, go);
 #pragma unroll
-                for (int s = 0; s < 8; ++s) mma_f16(tmem, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, 1u, go);
+                for (int s = 0; s < 8; ++s) mma_f16(tmem + kState, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, k > 0 || s > 0 ? 1u : 0u, go);
                 if (go) mma_commit(&empty[nb]), mma_commit(&empty[nc]), mma_commit(&used[m & 1]);
             }
             if (!ok) break;
@@ -393,10 +395,14 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
                 float* const dst = p.ends + (x.slot * kState + (W == 1 ? quad * 16 + lane : quad * 32 + lane)) * kState;
 #pragma unroll
                 for (int c = 0; c < kState; c += 16) {
-                    float v[16];
+                    float v[16], l[16];
                     tmem_ld16(tq + c, v);
+                    tmem_ld16(tq + kState + c, l);
                     tmem_wait_ld();
                     reg_fence(v);
+                    reg_fence(l);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] += l[j];
                     if (W == 2 || lane < 16)
 #pragma unroll
                         for (int j = 0; j < 16; j += 4)
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 9) tmem_dealloc(tmem, 128);
+    if (warp == 9) tmem_dealloc(tmem, 2 * kState);
 }
 
 // From the units' sums the state before each segment, in the slot of its unit that is first in time: four elements of a head's
@@ -466,6 +472,12 @@ template <typename T, int W, bool REV>
 __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W;                        // state rows
     constexpr int kO = 128, kKv = 128 + 64 * W, kCols = W == 1 ? 256 : 512;   // tensor memory columns; scores from 0 on
+    // Products that add to a state cut it off at its last bit 16 times a chunk, always downwards: 1.2e-5 of a slow head's
+    // state, which 16-bit outputs do not see.  Where the state is an output, a chunk's products start from 0 and are added
+    // to the decayed state in registers (8x16x16384x64 takes 8 % longer so); it waits in columns of its own, or, since the
+    // accumulators of 64 rows leave lanes 16 to 31 of each quarter free, there.
+    const bool exact = p.gout != nullptr;
+    const int kOld = W == 1 || !exact ? kKv : kKv + 128;
     constexpr bool F16 = std::is_same<T, __half>::value;
     extern __shared__ uint8_t raw[];
     uint8_t* const ring = raw + (-smem_u32(raw) & 1023u);  // (keeps the pointer one to shared memory)
@@ -554,9 +566,9 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 const uint64_t dh = make_desc(sk, kBlock, 1024), dl = make_desc(smem_u32(low), kBlock, 1024);
                 const uint64_t dv = make_desc(sv, kBlock, 1024);
 #pragma unroll
-                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, has_g || s > 0 ? 1u : 0u, go);
+                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, (has_g && !exact) || s > 0 ? 1u : 0u, go);
 #pragma unroll
-                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, 1u, go);
+                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, 1u, go);
                 if (go) mma_commit(kv_full), mma_commit(&empty[nk % kRing]);
                 if (!(ok = wait_for(p_ready, cc & 1))) break;
                 tc_fence_after();
@@ -593,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             auto tokens_of = [&](int k) { return (int)min((int64_t)kChunk, t.len - (int64_t)chunk_of(k) * kChunk); };
             auto last_of = [&](int k) { return !REV && p.gout && chunk_of(k) == t.active - 1 ? 1 : 0; };
             // G before chunk k: as an operand (rows of dc columns, in fp16 times a power of two that keeps the largest in
-            // range), and decayed over the chunk to where the products add to it.
+            // range), and decayed over the chunk to where the chunk's products, or their sum, add to it.
             auto put_state = [&](int k) {
                 float s = 1.f;
                 if constexpr (F16) {
@@ -629,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                         float v[16];
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) upk2(mul2(pk2(G[16 * c + j], G[16 * c + j + 1]), w2), v[j], v[j + 1]);
-                        tmem_st16(tq + kKv + col0 + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v));
+                        tmem_st16(tq + kOld + col0 + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v));
                     }
                 tmem_wait_st();
                 tc_fence_before();
@@ -678,7 +690,12 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             }
             epi_sync(true);  // the tables are written
             if (t.n > 0) {
-                if (has_g) put_state(0);
+                if (has_g) {
+                    if (W == 1 && exact)  // (the other lanes are 0)
+#pragma unroll
+                        for (int j = 0; j < 32 * W; ++j) G[j] += __shfl_xor_sync(0xffffffffu, G[j], 16);
+                    put_state(0);
+                }
                 arrive(g_ready);
             }
             // ---- chunks
@@ -818,6 +835,26 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     if (col0 + 32 * c < p.nb) tmem_ld32(tq + kKv + col0 + 32 * c, reinterpret_cast<float(&)[32]>(G[32 * c]));
                 tmem_wait_ld();
                 reg_fence(G);
+                if (exact) {
+                    if constexpr (W == 1) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float x = has_g || lane < 16 ? G[j] : 0.f;
+                            G[j] = x + __shfl_xor_sync(0xffffffffu, x, 16);
+                        }
+                    } else if (has_g) {
+#pragma unroll
+                        for (int c = 0; c < W; ++c)
+                            if (col0 + 32 * c < p.nb) {
+                                float v[32];
+                                tmem_ld32(tq + kOld + col0 + 32 * c, v);
+                                tmem_wait_ld();
+                                reg_fence(v);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) G[32 * c + j] += v[j];
+                            }
+                    }
+                }
                 if (p.nb & 16) {  // the last columns of 32 are nobody's
 #pragma unroll
                     for (int j = 16; j < 32 * W; j += 32)

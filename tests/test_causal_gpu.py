@@ -349,6 +349,24 @@ def test_attention_training_step_captured():
     assert all(torch.equal(a, c) for a, c in zip(out, step()))
 
 
+@pytest.mark.parametrize("b, d", [(296, 32), (148, 128), (3, 64)])
+def test_attention_states_of_slow_heads(b, d):
+    """States that remember 4096 tokens, over 64 chunks in one block or over segments.  In units of E of the state: a chunk's sum is
+    cut off at most 8 times by 2 (its products of the second parts are small), added with a rounding to a state that remembers 32
+    chunks, whose weights l^128 are off by at most 3 each: 16 + 32 + 96, besides u^2 of each term."""
+    g, t, dtype = gen(4), 8192, F16
+    q, k, v, do = (heads(g, b, 1, t, d, dtype) for _ in range(4))
+    dec = torch.full((1,), -(2.0**-12), device="cuda")
+    state = torch.zeros(b, 1, d, d, device="cuda").requires_grad_()
+    o, end = ops.decay_attention(q, k, v, dec, state, return_state=True)
+    (ds,) = torch.autograd.grad(o, state, do)
+    i = torch.arange(t, device="cuda").double()
+    want = torch.stack([(k[j].double() * torch.exp(-(2.0**-12) * (t - 1 - i))[:, None]).mT @ v[j].double() for j in range(b)])
+    want_ds = torch.stack([(q[j].double() * torch.exp(-(2.0**-12) * (i + 1))[:, None]).mT @ do[j].double() for j in range(b)]) * d**-0.5
+    u = U[dtype]
+    assert rel(end, want) <= u * u + 144 * E and rel(ds, want_ds) <= u * u + 144 * E
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("t, dk, dv, lengths", [(5000, 64, 48, [5000, 2111]), (4000, 128, 128, [1, 2500]), (3840, 64, 64, [3839, 0])])
 def test_attention_many_segments(t, dk, dv, lengths, dtype):
