@@ -27,7 +27,7 @@
 // bf16, size 64: 208 us, 5.2 TB/s.  8x16x16384x64: 240 us and 45 us for the
 // sums, since 256 segments leave 40 slots empty.  A training step is four mixes
 // and two sums (dq takes the forward's, dv those of dk, transposed): 1.21 ms; with
-// four sums 1.36.  Few chunks per slot (32x2x3136x32 180 us, 128x8x196x64 150 us
+// four sums 1.36.  Few chunks per slot (32x2x3136x32 172 us, 128x8x196x64 148 us
 // a training step) are bound by a chunk's chain: products, weights, products,
 // output, about 5200 cycles for a pair of blocks.
 // Between 64 and 128 one block fits an SM and waits on that chain alone: 8 heads
@@ -467,17 +467,17 @@ __global__ void __launch_bounds__(256) decay_join_kernel(const __grid_constant__
 }
 
 // W: 64-column blocks per operand row (head sizes up to 64 W).  REV: backwards
-// in time.
-template <typename T, int W, bool REV>
+// in time.  EXACT: the state is an output.  Products that add to a state cut it
+// off at its last bit 16 times a chunk, always downwards: 1.2e-5 of a slow head's
+// state, which 16-bit outputs do not see.  With EXACT a chunk's products start
+// from 0 and are added to the decayed state in registers (8x16x16384x64 takes 8 %
+// longer so); it waits in columns of its own, or, since the accumulators of 64
+// rows leave lanes 16 to 31 of each quarter free, there.
+template <typename T, int W, bool REV, bool EXACT>
 __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W;                        // state rows
     constexpr int kO = 128, kKv = 128 + 64 * W, kCols = W == 1 ? 256 : 512;   // tensor memory columns; scores from 0 on
-    // Products that add to a state cut it off at its last bit 16 times a chunk, always downwards: 1.2e-5 of a slow head's
-    // state, which 16-bit outputs do not see.  Where the state is an output, a chunk's products start from 0 and are added
-    // to the decayed state in registers (8x16x16384x64 takes 8 % longer so); it waits in columns of its own, or, since the
-    // accumulators of 64 rows leave lanes 16 to 31 of each quarter free, there.
-    const bool exact = p.gout != nullptr;
-    const int kOld = W == 1 || !exact ? kKv : kKv + 128;
+    constexpr int kOld = W == 1 || !EXACT ? kKv : kKv + 128;                  // the decayed state
     constexpr bool F16 = std::is_same<T, __half>::value;
     extern __shared__ uint8_t raw[];
     uint8_t* const ring = raw + (-smem_u32(raw) & 1023u);  // (keeps the pointer one to shared memory)
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 const uint64_t dh = make_desc(sk, kBlock, 1024), dl = make_desc(smem_u32(low), kBlock, 1024);
                 const uint64_t dv = make_desc(sv, kBlock, 1024);
 #pragma unroll
-                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, (has_g && !exact) || s > 0 ? 1u : 0u, go);
+                for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, (has_g && !EXACT) || s > 0 ? 1u : 0u, go);
 #pragma unroll
                 for (int s = 0; s < 8; ++s) mma_f16(tmem + kKv, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, 1u, go);
                 if (go) mma_commit(kv_full), mma_commit(&empty[nk % kRing]);
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             epi_sync(true);  // the tables are written
             if (t.n > 0) {
                 if (has_g) {
-                    if (W == 1 && exact)  // (the other lanes are 0)
+                    if (W == 1 && EXACT)  // (the other lanes are 0)
 #pragma unroll
                         for (int j = 0; j < 32 * W; ++j) G[j] += __shfl_xor_sync(0xffffffffu, G[j], 16);
                     put_state(0);
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     if (col0 + 32 * c < p.nb) tmem_ld32(tq + kKv + col0 + 32 * c, reinterpret_cast<float(&)[32]>(G[32 * c]));
                 tmem_wait_ld();
                 reg_fence(G);
-                if (exact) {
+                if constexpr (EXACT) {
                     if constexpr (W == 1) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
@@ -1129,10 +1129,13 @@ void launch_mix(MixArgs a, int64_t bh, cudaStream_t st) {
         constexpr auto join = decay_join_kernel<W, REV>;
         if (a.joined) launch_early(join, (unsigned)(bh * (4 * W * W)), 256, 0, 1, st, a);
     }
-    constexpr auto kernel = decay_mix_kernel<T, W, REV>;
-    allow_smem<kernel>(mix_smem<W>());
     a.items = (int)(bh * a.nseg);
-    launch_early(kernel, (unsigned)std::min(a.items, slots), kThreads, mix_smem<W>(), 1, st, a);
+    auto mix = [&](auto exact) {
+        constexpr auto kernel = decay_mix_kernel<T, W, REV, decltype(exact)::value>;
+        allow_smem<kernel>(mix_smem<W>());
+        launch_early(kernel, (unsigned)std::min(a.items, slots), kThreads, mix_smem<W>(), 1, st, a);
+    };
+    a.gout ? mix(std::true_type()) : mix(std::false_type());
 }
 
 struct Mix {
