@@ -81,7 +81,7 @@ FORWARD, BACKWARD = 20, 80
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("B, N, dim, heads, kw", [(3, 150, 64, 2, {}), (2, 131, 96, 3, {"rotary_dim": 20, "residual_scale": 0.5}), (1, 1, 64, 1, {}),
-                                                  (2, 40, 192, 2, {"decays": [1.0, 0.5]})])
+                                                  (2, 40, 192, 2, {"decays": [1.0, 0.5]}), (2, 33, 48, 3, {"rotary_dim": 0})])
 def test_block_forward_backward(B, N, dim, heads, kw, dtype):
     g, b = gen(N), block(dim, heads, dtype, **kw)
     x, dy = (rand(g, B, N, dim, dtype=dtype) for _ in range(2))
