@@ -51,7 +51,7 @@ __device__ __forceinline__ float sigmoid_of(float z) {
 // thread copies its packs of the next rows (K operands) to places of its own in
 // shared memory, asynchronously: that takes no registers and no barriers (bf16,
 // 131072x1024, a gate per token: forward 414 -> 212 us, backward 739 -> 380).
-// Rows without 16-byte packs (fp32 6304x771: 29 us so, 26 without) and rows of
+// Rows without 16-byte packs (fp32 6304x771: 29 us so, 25 without) and rows of
 // very wide groups, which do not fit, are loaded when their turn comes.
 template <typename T, int VEC, int NV, int K, int BLOCK>
 struct RowStream {
