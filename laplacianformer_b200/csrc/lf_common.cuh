@@ -9,6 +9,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include "divisor.h"
 #include "laplacian_b200.h"
 
 namespace lfb {
@@ -54,17 +55,6 @@ cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next kernel's blocks be placed as soon as there is room.
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery 1994).
-struct Divisor {
-    uint32_t d, mul, shift;
-    Divisor() = default;
-    explicit Divisor(uint32_t v) : d(v), shift(0) {
-        while ((1u << shift) < d) ++shift;
-        mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
-};
 
 // Element traits: storage type -> accumulation type, conversions.
 template <typename T> struct Elem;

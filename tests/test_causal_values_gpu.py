@@ -1,0 +1,30 @@
+"""The causal operators at small, large and far values: fp16 operands and gradients far from 1, decays that are NaN, wide gates,
+far positions, more than 2^31 rows.
+
+Tolerances as in test_causal_gpu.py: u half a step of the type, E of fp32, 1.25 u of the norm for an attention output."""
+import pytest
+import torch
+
+from laplacianformer_b200 import ops
+from test_causal_gpu import BF16, E, U, gen, rand, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ more rows than 32 bits count
+
+
+@pytest.mark.parametrize("groups, shared, c", [(33846154, 65, 1), (1, (1 << 31) + 5, 1), (2, (1 << 31) + 5, 1), (4200000, 524, 4)])
+def test_sandwich_rows_past_32_bits(groups, shared, c):
+    """A gate row serves its own rows, past the 2^31st and the 2^32nd too."""
+    rows = groups * shared
+    if torch.cuda.mem_get_info()[0] < rows * c * 2 * 3 + (8 << 30):
+        pytest.skip("needs %d GB" % (rows * c * 6 >> 30))
+    g = gen(1)
+    x = torch.empty(groups, shared, c, dtype=BF16, device="cuda").normal_(generator=g)
+    gate, w = torch.empty(groups, 1, c, dtype=BF16, device="cuda").normal_(generator=g), rand(g, c, dtype=BF16)
+    s = ops.sandwich_norm(x, w, x, gate, None, "none", 0.5).view(rows, c)
+    at = torch.cat((torch.arange(0, rows, max(1, rows // 5000), device="cuda"), torch.arange(rows - 1000, rows, device="cuda")))
+    y = x.view(rows, c)[at].double()
+    want = y + 0.5 * gate.view(groups, c)[at // shared].double() * y / torch.sqrt((y * y).mean(-1, keepdim=True) + 1e-6) * w.double()
+    within(s[at], want, U[BF16] * want.abs() + 24 * E * (y.abs() + (want - y).abs()), "s")
