@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
         for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
             const Item t = item_of(p, i);
             const float g = p.log_decay[t.h];
-            const float g2 = fmaxf(g, -1e30f) * 1.44269504f, l1 = exp2_of(g2);  // (times 0 steps: 0)
+            const float g2 = (g < -1e30f ? -1e30f : g) * 1.44269504f, l1 = exp2_of(g2);  // (times 0 steps: 0; NaN stays)
             const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
             bool has_g = (p.g0 || (t.n > 0 && t.seg != first_seg));
             float G[32 * W], unscale = 1.f;

@@ -6,9 +6,32 @@ import pytest
 import torch
 
 from laplacianformer_b200 import ops
-from test_causal_gpu import BF16, E, U, gen, rand, within
+from test_causal_gpu import BF16, E, F16, U, decays, gen, heads, rand, within
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ decays that are NaN
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("t, with_state", [(2, False), (100, False), (128, True), (300, False)])
+def test_attention_nan_decay(t, with_state, dtype):
+    """A head whose decay is NaN gives NaN (the first token has met no decay yet), and its gradients are NaN; no other head's are."""
+    g, b, h, d = gen(t), 2, 3, 64
+    q, k, v, do = (heads(g, b, h, t, d, dtype) for _ in range(4))
+    state = rand(g, b, h, d, d) if with_state else None
+    good, bad = torch.tensor([-0.1, -0.5, -0.01], device="cuda"), torch.tensor([-0.1, float("nan"), -0.01], device="cuda")
+    out = []
+    for dec in (good, bad):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        o, end = ops.decay_attention(*leaves, dec, state, return_state=True)
+        out.append((o, *torch.autograd.grad(o, leaves, do), end))
+    for a, c in zip(*out):
+        assert torch.equal(a[:, ::2], c[:, ::2])
+    o, dq, dk, dv, end = out[1]
+    assert torch.isnan(end[:, 1]).all() and torch.isnan(o[:, 1, 1:]).all() and torch.isnan(dq[:, 1, 1:]).all()
+    assert torch.isnan(dk[:, 1, :-1]).all() and torch.isnan(dv[:, 1, :-1]).all()
 
 
 # ------------------------------------------------------------------ more rows than 32 bits count
