@@ -29,16 +29,30 @@ struct Divisor {
     }
 };
 
-// The group of row r where each takes `each` of `rows` rows in turn: by the multiplication while rows are counted in 31 bits
-// (its d is 0 otherwise), else by a 64-bit division.
-struct RowGroups {
-    Divisor by;
-    int64_t each;
-    RowGroups() = default;
-    RowGroups(int64_t rows, int64_t each_) : by{}, each(each_) {
-        if (rows <= INT32_MAX && each <= rows && each > 0) by = Divisor((uint32_t)each);
+// r / d for 0 <= r < 2^40 and 0 < d < 2^40: with 2^s >= d > 2^(s-1) and m = floor(2^(40+s) / d) + 1, m d exceeds 2^(40+s) by
+// at most 2^s, so r m / 2^(40+s) has r / d for its floor (the same paper).  r 2^23 and m fit 64 bits.
+struct LongDivisor {
+    uint64_t mul;
+    uint32_t shift;  // s - 1
+    LongDivisor() = default;
+    explicit LongDivisor(int64_t d) {
+        uint32_t s = 1;
+        while (((int64_t)1 << s) < d) ++s;
+        uint64_t q = 0, rest = 1;  // 2^(40+s) / d bit by bit: the dividend may not fit 64 bits
+        for (uint32_t i = 0; i < 40 + s; ++i) {
+            rest *= 2, q *= 2;
+            if (rest >= (uint64_t)d) rest -= (uint64_t)d, ++q;
+        }
+        mul = q + 1, shift = s - 1;
     }
-    LFB_DIVISOR_CALL int64_t of(int64_t r) const { return by.d ? (int64_t)by.of((int)r) : r / each; }
+    LFB_DIVISOR_CALL int64_t of(int64_t r) const {
+#ifdef __CUDA_ARCH__
+        const uint64_t high = __umul64hi((uint64_t)r << 23, mul);
+#else
+        const uint64_t high = (uint64_t)(((unsigned __int128)((uint64_t)r << 23) * mul) >> 64);
+#endif
+        return (int64_t)(high >> shift);
+    }
 };
 
 }  // namespace lfb

@@ -33,7 +33,7 @@ struct SandwichArgs {
     float *part_w, *part_wn; // [gridDim.x][cols]
     float* part_g;           // [groups][parts][cols] where several blocks share a gate row, else null
     int64_t rows, cols, shared;   // rows per gate row
-    RowGroups gates;
+    LongDivisor per_gate;
     int64_t groups, parts, per_part;  // the backward's units: `parts` runs of at most per_part rows in each group of rows
     float alpha, eps;
     int act;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(block_of<G>()) sandwich_fwd_kernel(const Sandw
     // The row index is clamped, not skipped, so that every lane takes part in the shuffles.
     const int64_t step = (int64_t)gridDim.x * RPB, first = (int64_t)blockIdx.x * RPB;
     auto row_of = [&](int64_t base) { return min(base + sub, p.rows - 1); };
-    auto gate_of = [&](int64_t row) { return (p.shared == 1 ? row : p.gates.of(row)) * p.cols; };
+    auto gate_of = [&](int64_t row) { return (p.shared == 1 ? row : p.per_gate.of(row)) * p.cols; };
     auto fetch = [&](int64_t base, int stage) {
         if (base < p.rows) {
             const int64_t row = row_of(base), off = row * p.cols, goff = p.gate ? gate_of(row) : 0;
@@ -640,6 +640,10 @@ int check_sandwich(const char* what, const lf_sandwich_norm_t* a) {
         set_error("%s: rows must be a multiple of rows_per_gate", what);
         return LF_ERR_INVALID;
     }
+    if (a->gate && a->rows_per_gate > 1 && a->rows >= (int64_t)1 << 40) {
+        set_error("%s: a gate row for several rows is supported for less than 2^40 rows", what);
+        return LF_ERR_UNSUPPORTED;
+    }
     return LF_OK;
 }
 
@@ -648,7 +652,7 @@ SandwichArgs sandwich_args(const lf_sandwich_norm_t* a) {
     p.x = a->x, p.w = a->weight, p.r = a->residual, p.gate = a->gate, p.wn = a->next_weight, p.s = a->s, p.y = a->y, p.rstd = a->rstd;
     p.dy = a->dy, p.ds = a->ds, p.dx = a->dx, p.dr = a->d_residual, p.dgate = a->d_gate;
     p.rows = a->rows, p.cols = a->cols, p.shared = a->gate ? a->rows_per_gate : 1;
-    p.gates = RowGroups(p.rows, p.shared);
+    p.per_gate = LongDivisor(p.shared);
     p.alpha = (float)a->scale, p.eps = (float)a->eps, p.act = a->activation;
     return p;
 }

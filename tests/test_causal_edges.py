@@ -4,36 +4,45 @@ import subprocess
 
 import pytest
 
+from laplacianformer_b200 import capi
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 GROUPS = r"""
 #include <stdio.h>
 #include <stdlib.h>
 #include "divisor.h"
-int main(int argc, char** argv) {  // rows, rows per group, then row numbers
-    const lfb::RowGroups g(atoll(argv[1]), atoll(argv[2]));
-    for (int i = 3; i < argc; ++i) printf("%lld\n", (long long)g.of(atoll(argv[i])));
+int main(int argc, char** argv) {  // rows per group, then row numbers
+    const lfb::LongDivisor g(atoll(argv[1]));
+    for (int i = 2; i < argc; ++i) printf("%lld\n", (long long)g.of(atoll(argv[i])));
 }
 """
 
 
 @pytest.fixture(scope="module")
 def groups(tmp_path_factory):
-    """RowGroups, which says which gate row serves a row, compiled for the host."""
+    """LongDivisor, which says which gate row serves a row, compiled for the host."""
     d = tmp_path_factory.mktemp("groups")
     (d / "groups.cpp").write_text(GROUPS)
     subprocess.run(["g++", "-O1", "-std=c++17", "-I", os.path.join(ROOT, "laplacianformer_b200", "csrc"), str(d / "groups.cpp"), "-o", str(d / "groups")],
                    check=True)
 
-    def run(rows, each, at):
-        out = subprocess.run([str(d / "groups"), str(rows), str(each), *map(str, at)], check=True, capture_output=True, text=True, timeout=20)
+    def run(each, at):
+        out = subprocess.run([str(d / "groups"), str(each), *map(str, at)], check=True, capture_output=True, text=True, timeout=20)
         return [int(x) for x in out.stdout.split()]
 
     return run
 
 
 @pytest.mark.parametrize("rows, each", [(1, 1), (12, 1), (12, 5), (12, 12), ((1 << 31) - 1, 65), ((1 << 31) - 1, (1 << 31) - 1), ((1 << 31) - 1, 3), (1 << 31, 1 << 31),
-                                        (2200000000, 65), (4000000100, 197), ((1 << 32) + 5, (1 << 32) + 5), (3 << 32, 1 << 32), (1 << 33, 7), (1 << 32, (1 << 31) + 1)])
+                                        (2200000000, 65), (4000000100, 197), ((1 << 32) + 5, (1 << 32) + 5), (3 << 32, 1 << 32), (1 << 33, 7), (1 << 32, (1 << 31) + 1),
+                                        (1 << 40, 3), (1 << 40, 1), (1 << 40, 2), (1 << 40, (1 << 39) + 1), (1 << 40, (1 << 40) - 1)])
 def test_rows_of_a_shared_gate(groups, rows, each):
     at = sorted({r for base in (0, each, 2 * each, rows, 2200000000, 1 << 31, 1 << 32, rows // 2) for r in range(base - 2, base + 3) if 0 <= r < rows})
-    assert groups(rows, each, at) == [r // each for r in at]
+    assert groups(each, at) == [r // each for r in at]
+
+
+def test_rows_that_no_memory_holds_are_refused():
+    a = capi.SandwichNorm(x=1 << 20, weight=1 << 20, residual=1 << 20, s=1 << 20, gate=1 << 20, rows=1 << 40, cols=1, rows_per_gate=2, scale=1.0, eps=1e-6,
+                          dtype=capi.LF_BF16)
+    assert capi.lib().lf_sandwich_norm_fwd(a, None) == capi.LF_ERR_UNSUPPORTED
