@@ -530,8 +530,8 @@ LF_API int lf_decay_attention_step(const lf_decay_step_t* args, lf_stream_t stre
    x[i]: heads[i] heads of `size` contiguous elements, strides in elements of
    sequences, heads and tokens; y[i] dense [b, t, heads, size], which may be x[i]
    where that is dense.  positions: int64, position_stride apart between
-   sequences (0: shared), or NULL: offset + token.  The angle is formed in 64
-   bits.  F32, F16 or BF16. */
+   sequences (0: shared), or NULL: offset + token.  Angles are exact to fp32 at
+   positions up to 2^53.  F32, F16 or BF16. */
 typedef struct lf_rotary {
     const void* x[2];
     void* y[2];

@@ -324,7 +324,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, frequencies: torch.Tensor, p
     q [B, H, N, D] and k [B, Hk, N, D] (or None), fp32, fp16 or bf16, with any strides; frequencies from
     :func:`rotary_frequencies` (at most 128 pairs; channels past the pairs are copied).  Pairs are channels (i, i + pairs),
     or (2i, 2i + 1) if interleaved.  positions: int64 [N] or [B, N] on the GPU, or None: offset, offset + 1 and so on.
-    Angles are formed in 64 bits, so far positions lose nothing.
+    Angles are exact to fp32 at positions up to 2^53.
 
     Returns (q, k) turned, or q alone without k, in memory [B, N, H, D].  First order, reverse mode only."""
     y, z = ext().Rotary(q, k, frequencies, positions, offset, interleaved, magnitude)

@@ -2,11 +2,13 @@
 far positions, more than 2^31 rows.
 
 Tolerances as in test_causal_gpu.py: u half a step of the type, E of fp32, 1.25 u of the norm for an attention output."""
+from fractions import Fraction
+
 import pytest
 import torch
 
 from laplacianformer_b200 import ops
-from test_causal_gpu import BF16, E, F16, U, decays, gen, heads, rand, within
+from test_causal_gpu import BF16, E, F16, F32, U, decays, gen, heads, rand, within
 
 pytestmark = pytest.mark.gpu
 
@@ -32,6 +34,30 @@ def test_attention_nan_decay(t, with_state, dtype):
     o, dq, dk, dv, end = out[1]
     assert torch.isnan(end[:, 1]).all() and torch.isnan(o[:, 1, 1:]).all() and torch.isnan(dq[:, 1, 1:]).all()
     assert torch.isnan(dk[:, 1, :-1]).all() and torch.isnan(dv[:, 1, :-1]).all()
+
+
+# ------------------------------------------------------------------ far positions
+
+PI = Fraction(314159265358979323846264338327950288419716939937510582097494459230781640628620899862803482534211706798, 10**101)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("start", [0, 1000003, (1 << 31) - 3, (1 << 40) + 1, (1 << 47) + 12345, (1 << 53) - 8, -(1 << 52) - 1])
+def test_rotary_far_positions(start, interleaved):
+    """Angles at any position that 53 bits hold: the turns are formed here with 100 digits.  16 E of a pair's length, as for near ones."""
+    g, b, h, t, d = gen(1), 1, 2, 4, 32
+    q = heads(g, b, h, t, d, F32)
+    f = torch.cat((ops.rotary_frequencies(d)[:8], torch.tensor([1.0, 3.0, 0.7, 100.0, 1e-3, 2.5, 1.0 / 3, 6.283185307179586], dtype=torch.float64)))
+    at = [start + i for i in range(t)]
+    turns = [[Fraction(p) * Fraction(float(x)) / (2 * PI) for x in f] for p in at]
+    angle = torch.tensor([[float((y - round(y)) * 2 * PI) for y in row] for row in turns], dtype=torch.float64, device="cuda")
+    z = q.double()
+    z = torch.complex(z[..., ::2], z[..., 1::2]) if interleaved else torch.complex(z[..., : d // 2], z[..., d // 2 :])
+    y = z * torch.polar(torch.ones_like(angle), angle)
+    for got in (ops.rotary(q, None, f, torch.tensor(at, device="cuda"), interleaved=interleaved), ops.rotary(q, None, f, offset=start, interleaved=interleaved)):
+        got = got.double()
+        a = torch.complex(got[..., ::2], got[..., 1::2]) if interleaved else torch.complex(got[..., : d // 2], got[..., d // 2 :])
+        assert ((a - y).abs() <= 16 * E * z.abs()).all(), float(((a - y).abs() / z.abs()).max() / E)
 
 
 # ------------------------------------------------------------------ more rows than 32 bits count
