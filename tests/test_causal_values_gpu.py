@@ -36,6 +36,45 @@ def test_attention_nan_decay(t, with_state, dtype):
     assert torch.isnan(dk[:, 1, :-1]).all() and torch.isnan(dv[:, 1, :-1]).all()
 
 
+# ------------------------------------------------------------------ gates
+
+
+def gate64(z, act):
+    """(value, slope, the size of the slope's terms) in 64 bits without cancellation."""
+    q, p = torch.sigmoid(z), torch.sigmoid(-z)
+    if act == "sigmoid":
+        return q, q * p, q * p
+    if act == "silu":
+        return z * q, q * (1 + z * p), q * (1 + z.abs() * p)
+    return torch.tanh(z), 4 * torch.sigmoid(2 * z) * torch.sigmoid(-2 * z), 4 * torch.sigmoid(2 * z) * torch.sigmoid(-2 * z)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "tanh"])
+@pytest.mark.parametrize("rows, c, shared", [(40, 128, False), (30, 77, False), (20, 96, True), (2, 20001, False)])
+def test_gates_far_from_zero(rows, c, shared, act, dtype):
+    """Gates and their slopes are as good relative to themselves where they are saturated as elsewhere.  Roundings in units of E:
+    rx 8 and its products 3, the exponential 4 (of 2 z for tanh: its argument is exact), a sum and a quotient 2, products 3, the
+    scale 2: below 24; the slope takes two such quotients.  16-bit gates take the hardware's exponential, off by 2 + 1.173 |z| ulps
+    of 2 E: 192 E at 80."""
+    g, u, fast = gen(c), U[dtype], 192 * E * (dtype != F32)
+    x, w, ds = rand(g, rows, c, dtype=dtype), rand(g, c, dtype=dtype), rand(g, rows, c, dtype=dtype)
+    r = torch.zeros(rows, c, dtype=dtype, device="cuda")
+    lim = 80.0 if act != "tanh" else 40.0
+    z = (torch.rand(1 if shared else rows, c, generator=g, device="cuda") * 2 * lim - lim).to(dtype).requires_grad_()
+    s = ops.sandwich_norm(x, w, r, z[0] if shared else z, None, act, 0.7)
+    (dz,) = torch.autograd.grad(s, z, ds)
+    x64, z64 = x.double(), z.detach().double()
+    p = 0.7 * x64 / torch.sqrt((x64 * x64).mean(-1, keepdim=True) + 1e-6) * w.double()
+    val, slope, size = gate64(z64, act)
+    floor = {F32: 2.0**-126, BF16: 2.0**-126, F16: 2.0**-25}[dtype]
+    within(s, p * val, (u + 24 * E + fast) * (p * val).abs() + floor, "s")
+    want, most = ds.double() * p * slope, (ds.double() * p).abs() * size
+    if shared:
+        want, most = want.sum(0, keepdim=True), most.sum(0, keepdim=True)
+    within(dz, want, u * want.abs() + (60 * E + 2 * fast) * most + floor, "dgate")
+
+
 # ------------------------------------------------------------------ far positions
 
 PI = Fraction(314159265358979323846264338327950288419716939937510582097494459230781640628620899862803482534211706798, 10**101)
