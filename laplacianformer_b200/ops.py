@@ -306,7 +306,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", f
         raise ValueError("base and factor must be positive")
     if scaling == "base" and dim > 2:
         base = base * factor ** (dim / (dim - 2))
-    f = torch.pow(torch.tensor(base, dtype=torch.float64), torch.arange(0, dim, 2, dtype=torch.float64) / -max(dim, 1))
+    host = {"dtype": torch.float64, "device": "cpu"}  # (whatever the default device is)
+    f = torch.pow(torch.tensor(base, **host), torch.arange(0, dim, 2, **host) / -max(dim, 1))
     if scaling == "linear":
         f = f / factor
     elif scaling == "by_parts":

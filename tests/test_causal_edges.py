@@ -1,10 +1,12 @@
-"""CPU-side checks of the causal operators' edges: row numbers past 32 bits."""
+"""CPU-side checks of the causal operators' edges: row numbers past 32 bits, tensors that stay on the host."""
 import os
 import subprocess
 
 import pytest
+import torch
 
-from laplacianformer_b200 import capi
+from laplacianformer_b200 import capi, ops
+from laplacianformer_b200.block import DecayBlock
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -46,3 +48,14 @@ def test_rows_that_no_memory_holds_are_refused():
     a = capi.SandwichNorm(x=1 << 20, weight=1 << 20, residual=1 << 20, s=1 << 20, gate=1 << 20, rows=1 << 40, cols=1, rows_per_gate=2, scale=1.0, eps=1e-6,
                           dtype=capi.LF_BF16)
     assert capi.lib().lf_sandwich_norm_fwd(a, None) == capi.LF_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("scaling", ops.ROTARY_SCALINGS)
+def test_frequencies_are_on_the_host(scaling):
+    """Whatever the default device is: rotary() takes them from there."""
+    want = ops.rotary_frequencies(16, scaling=scaling, factor=2.0, original_length=64)
+    with torch.device("meta"):
+        f = ops.rotary_frequencies(16, scaling=scaling, factor=2.0, original_length=64)
+        block = DecayBlock(32, 2)
+    assert f.device.type == "cpu" and torch.equal(f, want)
+    assert block.frequencies.device.type == "cpu" and block.log_decay.device.type == "meta"
