@@ -61,6 +61,7 @@ constexpr int kRing = 5;              // operand tiles in flight: the chunk's th
 constexpr int kEpi = 256;             // threads that turn accumulators into operands and outputs
 constexpr int kThreads = kEpi + 64;   // and a warp for copies, a warp for products
 constexpr int kBlock = kChunk * 128;  // bytes of 128 rows of 64 columns
+constexpr int kCutChunks = 64;        // chunks whose products may follow one another on a state: with 16 cuts of 2^-23 at most, 2^-13
 constexpr uint32_t kNegateA = 1u << 13;  // of an instruction descriptor: the product with -A
 
 struct alignas(64) MixArgs {
@@ -467,9 +468,11 @@ __global__ void __launch_bounds__(256) decay_join_kernel(const __grid_constant__
 }
 
 // W: 64-column blocks per operand row (head sizes up to 64 W).  REV: backwards
-// in time.  EXACT: the state is an output.  Products that add to a state cut it
-// off at its last bit 16 times a chunk, always downwards: 1.2e-5 of a slow head's
-// state, which 16-bit outputs do not see.  With EXACT a chunk's products start
+// in time.  EXACT: the state is an output, or a segment is longer than kCutChunks.
+// Products that add to a state cut it off at its last bit 16 times a chunk, always
+// downwards: 1.2e-5 of a slow head's state, which 16-bit outputs do not see; but
+// in a head that forgets nothing the cuts add up (65536 tokens in one segment:
+// outputs 4.2e-4 too small, an fp16 rounding).  With EXACT a chunk's products start
 // from 0 and are added to the decayed state in registers (8x16x16384x64 takes 8 %
 // longer so); it waits in columns of its own, or, since the accumulators of 64
 // rows leave lanes 16 to 31 of each quarter free, there.
@@ -1135,7 +1138,7 @@ void launch_mix(MixArgs a, int64_t bh, cudaStream_t st) {
         allow_smem<kernel>(mix_smem<W>());
         launch_early(kernel, (unsigned)std::min(a.items, slots), kThreads, mix_smem<W>(), 1, st, a);
     };
-    a.gout ? mix(std::true_type()) : mix(std::false_type());
+    a.gout || a.per_seg > kCutChunks ? mix(std::true_type()) : mix(std::false_type());
 }
 
 struct Mix {
