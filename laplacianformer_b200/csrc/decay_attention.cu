@@ -264,26 +264,26 @@ __device__ __forceinline__ bool forgotten(const MixArgs& p, float g, int u, bool
     return power(g, (int64_t)(rev ? u * p.unit : max(0, p.per_seg - (u + 1) * p.unit)) * kChunk) == 0.f;
 }
 
-// What units of chunks add to the state, for the segments that go on after them: sum_j l^(n-j) b_j c_j^T with all weights
-// taken to the unit's end, so that the products of its chunks follow one another on one accumulator (weights that
-// underflow are of tokens that do not matter any more).  Two warps copy and multiply, eight scale b.  The products of the
-// second parts have an accumulator of their own: a product cuts its sum off at the accumulator's last bit, and those sums
-// are small.
+// What units of chunks add to the state, for the segments that go on after them: sum_j l^(n-j) b_j c_j^T.  A chunk's products
+// start from 0, with weights to the chunk's end, and are added to the unit's sum in registers while the next chunk's run: a
+// product cuts its sum off at the accumulator's last bit, so that sums of many chunks on one accumulator would lose more the
+// longer a unit is (units of 111 chunks: 7e-5 of the state; 2e-6 so, for 3 % of a prompt of 8 heads of 65536 tokens, size 128).
+// Two warps copy and multiply, eight scale b and add up.
 template <typename T, int W, bool REV>
-__global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_constant__ MixArgs p) {
+__global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_ends_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W, kTiles = kEndsRing<W>;
     extern __shared__ uint8_t raw[];
     uint8_t* const ring = raw + (-smem_u32(raw) & 1023u);  // (keeps the pointer one to shared memory)
     uint8_t* const lows = ring + kTiles * kTile;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(lows + 2 * kTile);
-    uint64_t *full = bars, *empty = bars + kTiles, *ready = empty + kTiles, *used = ready + 2, *done = used + 2, *read = done + 1, *drain = done + 2;
+    uint64_t *full = bars, *empty = bars + kTiles, *ready = empty + kTiles, *used = ready + 2, *read = used + 2, *drain = read + 2;
     uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_release();
     if (tid == 0) {
         for (int i = 0; i < kTiles; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&ready[i], kEpi), mbar_init(&used[i], 1);
-        mbar_init(done, 1), mbar_init(read, kEpi / 2), mbar_init(drain, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&ready[i], kEpi), mbar_init(&used[i], 1), mbar_init(&read[i], kEpi);
+        mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) tmem_alloc(tmem_ptr, 2 * kState);
@@ -332,26 +332,23 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
         __syncwarp();
     } else if (warp == 9) {
         const uint32_t go = elect_one() ? 1u : 0u;
-        int m = 0, items = 0;
+        int m = 0;
         for (int i = blockIdx.x; ok && i < count; i += gridDim.x) {
             const Unit x = unit_of(i);
-            if (x.n == 0) continue;
-            if (items > 0 && !(ok = wait_for(read, (items - 1) & 1))) break;  // the last sum has been read
             for (int k = 0; k < x.n; ++k, ++m) {
                 const int nb = 2 * m % kTiles, nc = (2 * m + 1) % kTiles;
                 if (!(ok = wait_for(&full[nc], (2 * m + 1) / kTiles & 1) && wait_for(&ready[m & 1], m >> 1 & 1))) break;
+                if (m > 1 && !(ok = wait_for(&read[m & 1], (m >> 1 & 1) ^ 1))) break;  // the sum before the last has been read
                 tc_fence_after();
                 const uint64_t dh = make_desc(smem_u32(ring + nb * kTile), kBlock, 1024), dl = make_desc(smem_u32(lows + (m & 1) * kTile), kBlock, 1024);
                 const uint64_t dv = make_desc(smem_u32(ring + nc * kTile), kBlock, 1024);
+                const uint32_t sum = tmem + (m & 1) * kState;
 #pragma unroll
-                for (int s = 0; s < 8; ++s) mma_f16(tmem, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, k > 0 || s > 0 ? 1u : 0u, go);
+                for (int s = 0; s < 8; ++s) mma_f16(sum, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, s > 0 ? 1u : 0u, go);
 #pragma unroll
-                for (int s = 0; s < 8; ++s) mma_f16(tmem + kState, dl + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv | kNegateA, k > 0 || s > 0 ? 1u : 0u, go);
+                for (int s = 0; s < 8; ++s) mma_f16(sum, dh + (uint64_t)(s * 128), dv + (uint64_t)(s * 128), p.id_kv, 1u, go);
                 if (go) mma_commit(&empty[nb]), mma_commit(&empty[nc]), mma_commit(&used[m & 1]);
             }
-            if (!ok) break;
-            if (go) mma_commit(done);
-            ++items;
         }
         if (!ok) {
             if (go) mma_commit(drain);
@@ -359,26 +356,45 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
         }
         __syncwarp();
     } else {
-        const int quad = warp & 3;
+        const int quad = warp & 3, half = warp >> 2, col0 = half * 32 * W;
         const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16);
-        int m = 0, items = 0;
+        int m = 0;
         for (int i = blockIdx.x; i < count; i += gridDim.x) {
             const Unit x = unit_of(i);
             if (x.n == 0) continue;
-            const float g = p.log_decay[x.h];
+            const float g = p.log_decay[x.h], whole = power(g, kChunk);
+            uint32_t wh[2][2], wl[2][2];  // of the 16 rows of this warp
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = warp * 16 + (j >> 1) * 8 + (j & 1) * 4 + (lane >> 3);
+                spread(split_weight<T>(power(g, REV ? r + 1 : kChunk - r)), wh[j >> 1][j & 1], wl[j >> 1][j & 1]);
+            }
+            float acc[32 * W];
+#pragma unroll
+            for (int j = 0; j < 32 * W; ++j) acc[j] = 0.f;
+            // Chunk k of the unit, the mk-th of this block.  (A power that overflows meets no 0.)
+            auto add = [&](int k, int mk) {
+                ok = ok && wait_for(&used[mk & 1], mk >> 1 & 1);
+                tc_fence_after();
+                const float w = REV ? power(g, (int64_t)k * kChunk) : k == 0 ? 0.f : whole;
+#pragma unroll
+                for (int c = 0; c < W; ++c)
+                    if (col0 + 32 * c < p.nb) {
+                        float v[32];
+                        tmem_ld32(tq + (mk & 1) * kState + col0 + 32 * c, v);
+                        tmem_wait_ld();
+                        reg_fence(v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) acc[32 * c + j] = REV ? __fmaf_rn(w, v[j], acc[32 * c + j]) : __fmaf_rn(w, acc[32 * c + j], v[j]);
+                    }
+                tc_fence_before();
+                arrive(&read[mk & 1]);
+            };
             for (int k = 0; k < x.n; ++k, ++m) {
                 const int nb = 2 * m % kTiles, nc = (2 * m + 1) % kTiles;
                 const int L = (int)min((int64_t)kChunk, x.len - (int64_t)(x.first + k) * kChunk);
-                uint32_t wh[2][2], wl[2][2];  // of the 16 rows of this warp
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = warp * 16 + (i >> 1) * 8 + (i & 1) * 4 + (lane >> 3);
-                    const int64_t n = REV ? (int64_t)k * kChunk + r + 1 : (int64_t)(x.n - k) * kChunk - r;
-                    spread(split_weight<T>(power(g, n)), wh[i >> 1][i & 1], wl[i >> 1][i & 1]);
-                }
-                uint8_t* const low = lows + (m & 1) * kTile;
+                uint8_t* const low = lows + (m & 1) * kTile;  // (its last products' sum has been read)
                 ok = ok && wait_for(&full[nb], 2 * m / kTiles & 1);
-                ok = ok && wait_for(&used[m & 1], (m >> 1 & 1) ^ 1);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) scale_rows<T, W>(ring + nb * kTile, low, warp * 16 + u * 8, lane, wh[u], wl[u]);
                 if (L < kChunk) {
@@ -388,31 +404,17 @@ __global__ void __launch_bounds__(kThreads) decay_ends_kernel(const __grid_const
                 }
                 fence_async_smem();
                 arrive(&ready[m & 1]);
+                if (k > 0) add(k - 1, m - 1);
             }
-            if (warp < 4) {
-                ok = ok && wait_for(done, items & 1);
-                tc_fence_after();
-                // The accumulators of 64 rows are 16 in each quarter of the lanes.
-                float* const dst = p.ends + (x.slot * kState + (W == 1 ? quad * 16 + lane : quad * 32 + lane)) * kState;
+            add(x.n - 1, m - 1);
+            // The accumulators of 64 rows are 16 in each quarter of the lanes.
+            if (W == 2 || lane < 16) {
+                float* const dst = p.ends + (x.slot * kState + (W == 1 ? quad * 16 + lane : quad * 32 + lane)) * kState + col0;
 #pragma unroll
-                for (int c = 0; c < kState; c += 16) {
-                    float v[16], l[16];
-                    tmem_ld16(tq + c, v);
-                    tmem_ld16(tq + kState + c, l);
-                    tmem_wait_ld();
-                    reg_fence(v);
-                    reg_fence(l);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] += l[j];
-                    if (W == 2 || lane < 16)
-#pragma unroll
-                        for (int j = 0; j < 16; j += 4)
-                            *reinterpret_cast<float4*>(dst + c + j) = c < p.nb ? make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-                tc_fence_before();
-                arrive(read);
+                for (int j = 0; j < 32 * W; j += 4)
+                    *reinterpret_cast<float4*>(dst + j) =
+                        col0 + j < p.nb ? make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            ++items;
         }
     }
     if (!ok) atomicExch(&g_decay_status, (int)LF_ERR_TIMEOUT);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from laplacianformer_b200 import ops
-from test_causal_gpu import E, F16, U, attention64, gen, rel
+from test_causal_gpu import E, F16, U, attention64, gen, heads, rel
 
 pytestmark = pytest.mark.gpu
 
@@ -17,6 +17,26 @@ def pieces64(q, k, v, g, state, scale=None, absolute=False):
         o, state = attention64(q[:, :, t : t + 512], k[:, :, t : t + 512], v[:, :, t : t + 512], g, state, None, scale, absolute)
         parts.append(o)
     return torch.cat(parts, 2), state
+
+
+@pytest.mark.parametrize("b, t, d, memory", [(8, 1 << 20, 64, 10), (128, 16384, 64, 6), (8, 65536, 128, 6)])
+def test_states_after_long_units(b, t, d, memory):
+    """States that are outputs, of heads that remember 2^memory chunks, where segments sum 15 to 111 chunks of their predecessors at
+    once.  In units of E of the state: a chunk's sum is cut off at most 8 times by 2 (16); weights l^n are off by 3 (two ulps, and E of
+    the exponent, which is below 1 where the weight counts), at most twice for a term (6); and each chunk remembered is added with a
+    rounding, up or down, that many times: sqrt(2^memory), five of them."""
+    g, u = gen(b), U[F16]
+    q, k, v, do = (heads(g, b, 1, t, d, F16).abs() for _ in range(4))  # (sums that grow: a cut that is always downwards shows)
+    g0 = -(2.0 ** (-7 - memory))
+    dec = torch.full((1,), g0, device="cuda")
+    state = torch.zeros(b, 1, d, d, device="cuda").requires_grad_()
+    o, end = ops.decay_attention(q, k, v, dec, state, scale=2.0**-12, return_state=True)
+    (ds,) = torch.autograd.grad(o, state, do)
+    i, bound = torch.arange(t, device="cuda").double(), u * u + (22 + 5 * 2.0 ** (memory / 2)) * E
+    for j in (0, b - 1):
+        want = (k[j, 0].double() * torch.exp(g0 * (t - 1 - i))[:, None]).mT @ v[j, 0].double()
+        want_ds = (q[j, 0].double() * torch.exp(g0 * (i + 1))[:, None]).mT @ do[j, 0].double() * 2.0**-12
+        assert rel(end[j, 0], want) <= bound and rel(ds[j, 0], want_ds) <= bound, (rel(end[j, 0], want) / E, rel(ds[j, 0], want_ds) / E)
 
 
 @pytest.mark.parametrize("b, t, d", [(296, 65536, 32), (296, 12000, 64), (148, 30000, 128), (296, 8192, 64)])
