@@ -477,10 +477,10 @@ LF_API int lf_clip_grad_norm(const void* const* grads, void* const* outs, const 
    state_out (may be NULL): the state after the last token.
    The backward takes d_o and (NULL: 0) d_state_out and writes the gradients that
    are not NULL; d_state needs dv.  Scores (scale q k^T, and scale d_o v^T in the
-   backward) are operands of a second product in dtype: in fp16 they become
-   infinite beyond 65504.  A value that is not finite reaches all outputs of its
-   128-token chunk.  Workspaces are 256-byte aligned; their sizes depend on the
-   sizes, strides and pointers: ask with the struct that will run.
+   backward) are operands of a second product in dtype, in fp16 scaled into its
+   range.  A value that is not finite reaches all outputs of its 128-token chunk.
+   Workspaces are 256-byte aligned; their sizes depend on the sizes, strides and
+   pointers: ask with the struct that will run.
    sums: NULL, or lf_decay_attention_sums_size() bytes, 256-byte aligned, which
    the forward fills and the backward of the same call reads, instead of summing
    keys and values again for dq. */

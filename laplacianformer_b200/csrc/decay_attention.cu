@@ -16,9 +16,15 @@
 // Every power of l is taken of a difference of positions and is at most 1 for
 // a decay: nothing is divided by a small power.  Sums and states are fp32.
 // Rounded to 16 bits as operands of products, besides the inputs: the weighted
-// scores (once), the state that q meets (once; fp16: scaled by a power of two
-// into its range), and l^(n-j) b_j, which goes in as two 16-bit parts so that
-// the state keeps about 17 bits (bf16) or 22 (fp16) of each term.
+// scores (once), the state that q meets (once), and l^(n-j) b_j, which goes in as
+// two 16-bit parts so that the state keeps about 17 bits (bf16) or 22 (fp16) of
+// each term.  In fp16, whose range is narrow (gradients of 1e-6 would be
+// subnormal, products of large ones infinite), powers of two bring these operands
+// into it and are taken out of the sums: one per row of scores, from the largest
+// sizes in the row of a and in the chunk of b, which the copying warp looks up
+// beside its copies; one per chunk of b, at most 2^14 (of a term 2^-39 of the
+// chunk's largest b, or of 1, is lost); one per state.  (32x2x3136x32 training
+// takes 195 us so, 170 without; by the threads that scale b 213.)
 //
 // What bounds it.  Sequences are cut into segments until every block slot has
 // one (two slots per SM for heads up to 64); the state before a segment comes
@@ -211,6 +217,32 @@ __device__ __forceinline__ float range_scale(uint32_t bits) {
     return __uint_as_float((uint32_t)max(1, min(127 + 141 - e, 254)) << 23);
 }
 
+// fp16 operands of products are brought into fp16's range by powers of two, which the products' sums are freed of again.
+// The largest size among 16-bit pairs, in bits (a NaN's are the largest), and of the first `packs` packs of 8 in a tile's row.
+__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <int W>
+__device__ __forceinline__ uint32_t largest16(const uint8_t* tile, int row, int from, int packs) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4 * W; ++j) {
+        const int c = from + j;
+        if (c < packs) {
+            const uint4 x = *reinterpret_cast<const uint4*>(tile + (c >> 3) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+            m = max16x2(max16x2(m, max16x2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu)), max16x2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+        }
+    }
+    return max(m & 0xffffu, m >> 16);
+}
+// 1 / s of a power of two between 2^-126 and 2^126.
+__device__ __forceinline__ float inverse2(float s) { return __uint_as_float(0x7f000000u - __float_as_uint(s)); }
+__device__ __forceinline__ float size16(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+// For b of sizes up to `top` whose weights are up to `grow`: the weights times it, and b times them, stay below 2^15.
+__device__ __forceinline__ float weight_scale(float top, float grow) { return range_scale(__float_as_uint(fmaxf(top, 1.f) * fmaxf(grow, 1.f))); }
+
 // Scales rows of a tile of b, 8 at a time (eight lanes to a row, so that no bank is met twice): b w in two parts, the
 // first in place, the second negated in `low`; w0 and w1 are a row's weight in two parts, for the rows 4 apart.
 //   high = b w0 rounded;  b w0 - high is exact (it has no more bits than b), and b w1 joins it with one rounding
@@ -272,18 +304,21 @@ __device__ __forceinline__ bool forgotten(const MixArgs& p, float g, int u, bool
 template <typename T, int W, bool REV>
 __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_ends_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W, kTiles = kEndsRing<W>;
+    constexpr bool F16 = std::is_same<T, __half>::value;
     extern __shared__ uint8_t raw[];
     uint8_t* const ring = raw + (-smem_u32(raw) & 1023u);  // (keeps the pointer one to shared memory)
     uint8_t* const lows = ring + kTiles * kTile;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(lows + 2 * kTile);
     uint64_t *full = bars, *empty = bars + kTiles, *ready = empty + kTiles, *used = ready + 2, *read = used + 2, *drain = read + 2;
     uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
+    uint32_t* const tops = tmem_ptr + 1;  // largest size in a chunk of b; three in turn
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_release();
     if (tid == 0) {
         for (int i = 0; i < kTiles; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&ready[i], kEpi), mbar_init(&used[i], 1), mbar_init(&read[i], kEpi);
         mbar_init(drain, 1);
+        tops[0] = tops[1] = tops[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) tmem_alloc(tmem_ptr, 2 * kState);
@@ -358,25 +393,29 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_ends_kernel(co
     } else {
         const int quad = warp & 3, half = warp >> 2, col0 = half * 32 * W;
         const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16);
-        int m = 0;
+        int m = 0, turn = 0;
         for (int i = blockIdx.x; i < count; i += gridDim.x) {
             const Unit x = unit_of(i);
             if (x.n == 0) continue;
             const float g = p.log_decay[x.h], whole = power(g, kChunk);
+            float w[4], scale = 1.f, held = 1.f;  // fp16: the scale of b, and, forwards, of what `acc` holds
             uint32_t wh[2][2], wl[2][2];  // of the 16 rows of this warp
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = warp * 16 + (j >> 1) * 8 + (j & 1) * 4 + (lane >> 3);
-                spread(split_weight<T>(power(g, REV ? r + 1 : kChunk - r)), wh[j >> 1][j & 1], wl[j >> 1][j & 1]);
+                w[j] = power(g, REV ? r + 1 : kChunk - r);
+                spread(split_weight<T>(w[j]), wh[j >> 1][j & 1], wl[j >> 1][j & 1]);
             }
             float acc[32 * W];
 #pragma unroll
             for (int j = 0; j < 32 * W; ++j) acc[j] = 0.f;
-            // Chunk k of the unit, the mk-th of this block.  (A power that overflows meets no 0.)
-            auto add = [&](int k, int mk) {
+            // Chunk k of the unit, the mk-th of this block, whose b was scaled by s.  (A power that overflows meets no 0.)
+            auto add = [&](int k, int mk, float s) {
                 ok = ok && wait_for(&used[mk & 1], mk >> 1 & 1);
                 tc_fence_after();
-                const float w = REV ? power(g, (int64_t)k * kChunk) : k == 0 ? 0.f : whole;
+                float w = REV ? power(g, (int64_t)k * kChunk) : k == 0 ? 0.f : whole;
+                if constexpr (F16) w *= REV ? inverse2(s) : s * inverse2(held);
+                held = s;
 #pragma unroll
                 for (int c = 0; c < W; ++c)
                     if (col0 + 32 * c < p.nb) {
@@ -394,7 +433,18 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_ends_kernel(co
                 const int nb = 2 * m % kTiles, nc = (2 * m + 1) % kTiles;
                 const int L = (int)min((int64_t)kChunk, x.len - (int64_t)(x.first + k) * kChunk);
                 uint8_t* const low = lows + (m & 1) * kTile;  // (its last products' sum has been read)
+                const float last = scale;
                 ok = ok && wait_for(&full[nb], 2 * m / kTiles & 1);
+                if constexpr (F16) {
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, (tid >> 1) < L ? largest16<W>(ring + nb * kTile, tid >> 1, (tid & 1) * 4 * W, 8 * W) : 0u);
+                    if (lane == 0) atomicMax(&tops[turn], top);
+                    epi_sync(true);
+                    scale = weight_scale(size16(tops[turn]), whole);
+                    if (tid == 0) tops[turn == 0 ? 2 : turn - 1] = 0;  // (read before this barrier, written after the next)
+                    turn = turn == 2 ? 0 : turn + 1;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) spread(split_weight<T>(w[j] * scale), wh[j >> 1][j & 1], wl[j >> 1][j & 1]);
+                }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) scale_rows<T, W>(ring + nb * kTile, low, warp * 16 + u * 8, lane, wh[u], wl[u]);
                 if (L < kChunk) {
@@ -404,9 +454,12 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_ends_kernel(co
                 }
                 fence_async_smem();
                 arrive(&ready[m & 1]);
-                if (k > 0) add(k - 1, m - 1);
+                if (k > 0) add(k - 1, m - 1, last);
             }
-            add(x.n - 1, m - 1);
+            add(x.n - 1, m - 1, scale);
+            if constexpr (F16 && !REV)
+#pragma unroll
+                for (int j = 0; j < 32 * W; ++j) acc[j] *= inverse2(held);
             // The accumulators of 64 rows are 16 in each quarter of the lanes.
             if (W == 2 || lane < 16) {
                 float* const dst = p.ends + (x.slot * kState + (W == 1 ? quad * 16 + lane : quad * 32 + lane)) * kState + col0;
@@ -489,17 +542,20 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     uint8_t* const low = ring + kRing * kTile;
     uint8_t* const gop = low + kTile;                                         // [state row][dc], 64 columns a block
     float* const pw = reinterpret_cast<float*>(gop + kState * 128 * W);       // l^n, n = 0..128
-    uint32_t* const gmax = reinterpret_cast<uint32_t*>(pw + 132);
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 134);
+    uint32_t* const gmax = reinterpret_cast<uint32_t*>(pw + 132);             // largest size in the state, and in a chunk of b;
+    uint32_t* const bmax = gmax + 2;                                          // two each, in turn (of the chunks)
+    uint16_t* const amax = reinterpret_cast<uint16_t*>(pw + 136);             // [2][128], largest size in each row of a
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 264);
     uint64_t *full = bars, *empty = bars + kRing, *s_full = bars + 2 * kRing, *k_ready = s_full + 1, *p_ready = s_full + 2,
-             *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7;
-    uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 8);
+             *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7, *measured = s_full + 8;
+    uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 10);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_release();
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         mbar_init(s_full, 1), mbar_init(kv_full, 1), mbar_init(o_full, 1), mbar_init(qg_full, 1), mbar_init(drain, 1);
         mbar_init(k_ready, kEpi), mbar_init(p_ready, kEpi), mbar_init(g_ready, kEpi);
+        mbar_init(&measured[0], 1), mbar_init(&measured[1], 1);
         gmax[0] = gmax[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -511,26 +567,49 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     const uint32_t tmem = *tmem_ptr;
     bool ok = true;
 
-    if (warp == 8) {  // copies
-        if (elect_one()) {
-            int n = 0;
+    if (warp == 8) {  // copies, and in fp16 how large a's rows and b are
+        const bool one = elect_one();
+        int n = 0, cc = 0;
+        if (F16 || one)
             for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
                 const Item t = item_of(p, i);
-                for (int k = 0; ok && k < t.n; ++k) {
-                    const int t0 = (REV ? t.first + t.n - 1 - k : t.first + k) * kChunk;
+                for (int k = 0; ok && k < t.n; ++k, ++cc) {
+                    const int chunk = REV ? t.first + t.n - 1 - k : t.first + k, t0 = chunk * kChunk;
                     for (int j = 0; j < 3; ++j) {
                         const int s = n % kRing;
                         if (!(ok = wait_for(&empty[s], (n / kRing & 1) ^ 1))) break;
-                        expect(&full[s], kTile);
-                        const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
-                        for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
+                        if (one) {
+                            expect(&full[s], kTile);
+                            const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
+                            for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
+                        }
                         ++n;
+                    }
+                    if constexpr (F16) {
+                        // The places of two chunks ago are free: their readers have let go of that chunk's b, whose place a has.
+                        ok = ok && wait_for(&full[(n - 3) % kRing], (n - 3) / kRing & 1) && wait_for(&full[(n - 2) % kRing], (n - 2) / kRing & 1);
+                        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                        const uint8_t *ta = ring + (n - 3) % kRing * kTile, *tb = ring + (n - 2) % kRing * kTile;
+                        const int L = (int)min((int64_t)kChunk, t.len - (int64_t)t0), packs = (p.da + 7) / 8;
+                        uint32_t top = 0;
+#pragma unroll 2
+                        for (int i = 0; i < kChunk / 32; ++i) {
+                            const int r = i * 32 + lane;
+                            uint32_t ma = largest16<W>(ta, r, 0, packs), mb = largest16<W>(tb, r, 0, packs);
+                            if (packs > 4 * W) ma = max(ma, largest16<W>(ta, r, 4 * W, packs)), mb = max(mb, largest16<W>(tb, r, 4 * W, packs));
+                            if (r >= L) ma = mb = 0;
+                            amax[(cc & 1) * kChunk + r] = (uint16_t)ma;
+                            top = max(top, mb);
+                        }
+                        top = __reduce_max_sync(0xffffffffu, top);
+                        if (lane == 0) bmax[cc & 1] = top;
+                        __syncwarp();
+                        if (lane == 0) arrive(&measured[cc & 1]);
                     }
                 }
             }
-            if (!ok)  // a wait ran out: let the copies in flight land
-                for (int k = max(0, n - kRing); k < n; ++k) mbar_wait(&full[k % kRing], k / kRing & 1, 100000000ull);
-        }
+        if (one && !ok)  // a wait ran out: let the copies in flight land
+            for (int k = max(0, n - kRing); k < n; ++k) mbar_wait(&full[k % kRing], k / kRing & 1, 100000000ull);
         __syncwarp();
     } else if (warp == 9) {  // products
         const uint32_t go = elect_one() ? 1u : 0u;
@@ -604,11 +683,19 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             const float g2 = (g < -1e30f ? -1e30f : g) * 1.44269504f, l1 = exp2_of(g2);  // (times 0 steps: 0; NaN stays)
             const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
             bool has_g = (p.g0 || (t.n > 0 && t.seg != first_seg));
-            float G[32 * W], unscale = 1.f;
+            float G[32 * W], unscale = 1.f;      // fp16: one over the scale of the state's operand,
+            float bscale = 1.f, btop = 0.f;      // the scale of b, and the largest size that a weight can give one of b's;
+            float held = 1.f;                    // without EXACT G is as the scaled products left it: this times too large
             // Chunk k of the item, its tokens, and 1 where the state shall not be decayed past its last token.
             auto chunk_of = [&](int k) { return REV ? t.first + t.n - 1 - k : t.first + k; };
             auto tokens_of = [&](int k) { return (int)min((int64_t)kChunk, t.len - (int64_t)chunk_of(k) * kChunk); };
             auto last_of = [&](int k) { return !REV && p.gout && chunk_of(k) == t.active - 1 ? 1 : 0; };
+            // fp16: the scale of the block's c-th chunk's b.
+            auto measure = [&](int c) {
+                ok = wait_for(&measured[c & 1], c >> 1 & 1) && ok;
+                const float grow = pw[kChunk];
+                btop = size16(bmax[c & 1]), bscale = weight_scale(btop, grow), btop *= fmaxf(grow, 1.f);
+            };
             // G before chunk k: as an operand (rows of dc columns, in fp16 times a power of two that keeps the largest in
             // range), and decayed over the chunk to where the chunk's products, or their sum, add to it.
             auto put_state = [&](int k) {
@@ -623,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     epi_sync(true);
                     s = range_scale(gmax[slot]);
                     if (tid == 0) gmax[slot ^ 1] = 0;
-                    unscale = 1.f / s;
+                    unscale = inverse2(s) * inverse2(held);
                 }
                 if (live) {
                     uint8_t* const dst = gop + (W == 2 ? half * kState * 128 : 0) + srow * 128;
@@ -638,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     }
                 }
                 fence_async_smem();
-                const float w = pw[tokens_of(k) - last_of(k)];
+                const float w = pw[tokens_of(k) - last_of(k)] * (F16 && !EXACT ? bscale * inverse2(held) : 1.f);
                 const uint64_t w2 = pk2(w, w);
 #pragma unroll
                 for (int c = 0; c < 2 * W; ++c)
@@ -695,6 +782,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             }
             epi_sync(true);  // the tables are written
             if (t.n > 0) {
+                if constexpr (F16) measure(cc);
                 if (has_g) {
                     if (W == 1 && EXACT)  // (the other lanes are 0)
 #pragma unroll
@@ -711,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 if (W == 2) hi += kpart * kBlock, lo += kpart * kBlock;
                 uint4 x[4];
                 int at[4];
-                const float w = kr >= L ? 0.f : REV ? pw[kr + 1] : pw[L - e - kr];
+                const float w = kr >= L ? 0.f : (REV ? pw[kr + 1] : pw[L - e - kr]) * bscale;
                 const T w0 = Elem<T>::store(w);
                 const uint32_t wh = pack2<T>(w, w), nh = wh ^ 0x80008000u, nl = pack2<T>(Elem<T>::load(w0) - w, Elem<T>::load(w0) - w);
                 auto fetch = [&](int j0) {
@@ -721,6 +809,10 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                         x[j] = *reinterpret_cast<const uint4*>(hi + at[j]);
                     }
                 };
+                // The scores' scale: in fp16 a power of two by which the largest that this row can have stays in range, and the
+                // output's to undo it.
+                const float unit = F16 ? fminf(range_scale(__float_as_uint((float)p.da * size16(amax[(cc & 1) * kChunk + row]) * btop)), 0x1p40f) : p.scale;
+                const float back = F16 ? p.scale * inverse2(unit) : 1.f;
                 ok = wait_for(&full[nk % kRing], nk / kRing & 1) && ok;
                 fetch(0);
                 ok = wait_for(s_full, cc & 1) && ok;  // the scores are done: b may be overwritten
@@ -777,11 +869,11 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                         tmem_ld32(tq + blk * 32, v);
                         tmem_wait_ld();
                         reg_fence(v);
-                        // Two factors at once, of columns 16 apart, from the furthest columns on: each is l times the last, and
-                        // scale on the diagonal (0 before it).
+                        // Two factors at once, of columns 16 apart, from the nearest columns on (so that one which underflows takes
+                        // none of a nearer column along): each is l times the last, and `unit` on the diagonal (0 before it).
                         const int d = REV ? blk * 32 - row : row - blk * 32 - 15;  // steps to the first of the two columns
                         const int d2 = REV ? d + 16 : d - 16;
-                        const float x0 = exp2_of((float)max(d, 0) * g2) * p.scale, y0 = exp2_of((float)max(d2, 0) * g2) * p.scale;
+                        const float x0 = exp2_of((float)max(d, 0) * g2) * unit, y0 = exp2_of((float)max(d2, 0) * g2) * unit;
                         uint64_t f = pk2(d >= 0 ? x0 : 0.f, d2 >= 0 ? y0 : 0.f);
                         if (blk == quad) {
 #pragma unroll
@@ -791,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                                 float x, y;
                                 upk2(mul2(f, pk2(l1, l1)), x, y);
                                 const int next = REV ? j + 1 : j - 1;
-                                f = pk2(lane == next ? p.scale : x, lane == next + 16 ? p.scale : y);
+                                f = pk2(lane == next ? unit : x, lane == next + 16 ? unit : y);
                             }
                         } else {
 #pragma unroll
@@ -814,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     ok = wait_for(qg_full, qg++ & 1) && ok;
                     tc_fence_after();
                     const int d = REV ? L - 1 - row : row;
-                    const float w = (d >= 0 ? pw[d] : 0.f) * p.scale * unscale;
+                    const float w = (d >= 0 ? pw[d] : 0.f) * unit * unscale;
                     const uint64_t w2 = pk2(w, w);
 #pragma unroll
                     for (int c = 0; c < W; ++c) {
@@ -840,11 +932,16 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     if (col0 + 32 * c < p.nb) tmem_ld32(tq + kKv + col0 + 32 * c, reinterpret_cast<float(&)[32]>(G[32 * c]));
                 tmem_wait_ld();
                 reg_fence(G);
+                if constexpr (F16 && !EXACT) held = bscale;
+                const float un = EXACT ? inverse2(bscale) : 1.f;
+                if constexpr (F16 && EXACT && W == 2)
+#pragma unroll
+                    for (int j = 0; j < 32 * W; ++j) G[j] *= un;
                 if constexpr (EXACT) {
                     if constexpr (W == 1) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float x = has_g || lane < 16 ? G[j] : 0.f;
+                            const float x = has_g || lane < 16 ? (F16 && lane < 16 ? G[j] * un : G[j]) : 0.f;
                             G[j] = x + __shfl_xor_sync(0xffffffffu, x, 16);
                         }
                     } else if (has_g) {
@@ -868,7 +965,10 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                             if (col0 + j >= p.nb) G[j + m] = 0.f;
                 }
                 has_g = true;
-                if (k + 1 < t.n) put_state(k + 1);
+                if (k + 1 < t.n) {
+                    if constexpr (F16) measure(cc + 1);
+                    put_state(k + 1);
+                }
                 // ---- the output
                 ok = wait_for(o_full, cc & 1) && ok;
                 tc_fence_after();
@@ -879,6 +979,9 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                         tmem_ld32(tq + kO + col0 + 32 * c, v);
                         tmem_wait_ld();
                         reg_fence(v);
+                        if constexpr (F16)
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) upk2(mul2(pk2(v[j], v[j + 1]), pk2(back, back)), v[j], v[j + 1]);
                         uint8_t* const dst = low + (W == 2 ? half * kBlock : 0) + row * 128;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {

@@ -275,7 +275,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     Returns o [B, H, N, Dv] (in memory [B, N, H, Dv], so that o.transpose(1, 2).reshape(B, N, H * Dv) copies nothing), or
     (o, state after the last token) with return_state, for the next piece of a prompt or :func:`decay_attention_step`.
     Work is linear in N, by chunks of 128 tokens on the tensor cores; a value that is not finite reaches its whole chunk.
-    In fp16 the scores become infinite beyond 65504.  First order, reverse mode only."""
+    fp16 operands are scaled inside, so that small gradients keep their digits.  First order, reverse mode only."""
     o, s = ext().DecayAttention(q, k, v, log_decay, state, lengths, q.shape[-1] ** -0.5 if scale is None else scale, return_state)
     return (o, s) if return_state else o
 

@@ -8,9 +8,93 @@ import pytest
 import torch
 
 from laplacianformer_b200 import ops
-from test_causal_gpu import BF16, E, F16, F32, U, decays, gen, heads, rand, within
+from test_causal_gpu import BF16, E, F16, F32, TINY, U, attention64, decays, gen, heads, rand, rel, within
 
 pytestmark = pytest.mark.gpu
+
+
+def off(a, b, dtype):
+    """Whether a is further from b than 1.25 u of its norm and half a smallest step per value, which its own rounding takes."""
+    d = (a.detach().double() - b.detach().double()).norm()
+    return not float(d) <= 1.25 * U[dtype] * float(b.norm()) + TINY[dtype] * b.numel() ** 0.5
+
+
+# ------------------------------------------------------------------ attention in fp16 far from 1
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("t, d", [(100, 64), (700, 64), (5000, 32), (600, 128), (150, 50)])
+@pytest.mark.parametrize("sizes", [
+    # binary exponents of q, k, v and do
+    (0, 6, 0, -20), (6, 0, 0, -22), (3, 3, 0, -16), (-18, 0, 9, 0), (0, -14, 6, -8), (-14, 0, 6, 4), (8, 8, -9, 0), (9, 9, -14, -10), (0, 0, 8, 8)])
+def test_attention_far_from_one(t, d, sizes, dtype):
+    """Small gradients (and small keys, queries and values) keep their digits beside large operands that bring the results into
+    range; products of large ones do not overflow."""
+    g, b, h = gen(t), 2, 3
+    q, k, v, do = (heads(g, b, h, t, d, dtype, 2.0**s) for s in sizes)
+    dec = torch.tensor([-0.05, -0.004, 0.0], device="cuda")
+    state = rand(g, b, h, d, d, scale=2.0 ** (sizes[1] + sizes[2]))
+    leaves = [x.requires_grad_() for x in (q, k, v, state)]
+    o, end = ops.decay_attention(q, k, v, dec, state, return_state=True)
+    dend = rand(g, b, h, d, d, scale=2.0 ** (sizes[0] + sizes[3]))
+    got = torch.autograd.grad((o, end), leaves, (do, dend))
+    l64 = [x.detach().double().requires_grad_() for x in leaves]
+    o64, end64 = attention64(*l64[:3], dec, l64[3])
+    want = torch.autograd.grad((o64, end64), l64, (do.double(), dend.double()))
+    u = U[dtype]
+    for j in range(h):
+        for name, a, c in zip(("o", "dq", "dk", "dv"), (o, *got), (o64, *want)):
+            a, c = a[:, j], c[:, j]
+            if float(c.abs().max()) < 60000 or dtype == BF16:  # (else the result itself is out of fp16's range)
+                assert not off(a, c, dtype), (name, j, rel(a, c) / u)
+        # States: u^2 of each term's size in two parts, whose last bit in fp16 is 2^-25 of 2^15 / its largest (2^-22 = u^2 at 2^-14).
+        assert rel(end[:, j], end64[:, j]) <= 1.5 * u * u + 60 * E, (j, rel(end[:, j], end64[:, j]))
+        assert rel(got[3][:, j], want[3][:, j]) <= 1.5 * u * u + 60 * E, (j, rel(got[3][:, j], want[3][:, j]))
+
+
+@pytest.mark.parametrize("t", [96, 1000])
+def test_attention_rows_of_unlike_sizes_fp16(t):
+    """Each token's outputs are as good as its own operands are, beside others a million times larger (queries, gradients), and
+    sums of unlike terms are as good as their largest."""
+    g, b, h, d = gen(t), 1, 3, 64
+    q, k, v, do = heads(g, b, h, t, d, F32), heads(g, b, h, t, d, F16), heads(g, b, h, t, d, F16), heads(g, b, h, t, d, F32)
+    size = torch.where(torch.arange(t, device="cuda") % 3 == 0, 1.0, 2.0**-20)[:, None]
+    q, do, k = (q * size).to(F16), (do * size).to(F16), (k * 64).to(F16)
+    dec = torch.tensor([-0.05, -0.004, 0.0], device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o = ops.decay_attention(*leaves, dec)
+    got = torch.autograd.grad(o, leaves, do)
+    l64 = [x.detach().double().requires_grad_() for x in leaves]
+    o64, _ = attention64(*l64, dec)
+    want = torch.autograd.grad(o64, l64, do.double())
+    big = size[:, 0] == 1
+    for name, a, c in zip(("o", "dq"), (o, got[0]), (o64, want[0])):
+        for j in range(h):
+            for rows in (big, ~big):
+                assert not off(a[0, j, rows], c[0, j, rows], F16), (name, j, rel(a[0, j, rows], c[0, j, rows]) / U[F16])
+    for name, a, c in zip(("dk", "dv"), got[1:], want[1:]):
+        for j in range(h):
+            assert not off(a[0, j], c[0, j], F16), (name, j)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_of_growing_heads(dtype):
+    """log_decay a little above 0: weights above 1 go the same way."""
+    g, b, t, d = gen(1), 2, 300, 64
+    q, k, v, do = (heads(g, b, 2, t, d, dtype) for _ in range(4))
+    dec = torch.tensor([0.01, 0.03], device="cuda")
+    do = do * torch.exp(dec.view(1, 2, 1, 1) * (torch.arange(t, device="cuda").view(1, 1, t, 1) - t)).to(dtype)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o, end = ops.decay_attention(*leaves, dec, return_state=True)
+    got = torch.autograd.grad(o, leaves, do)
+    l64 = [x.detach().double().requires_grad_() for x in leaves]
+    o64, end64 = attention64(*l64, dec)
+    want = torch.autograd.grad(o64, l64, do.double())
+    for j in range(2):
+        for a, c in zip((o, *got), (o64, *want)):
+            if float(c[:, j].abs().max()) < 60000 or dtype == BF16:  # (else the result itself is out of fp16's range)
+                assert not off(a[:, j], c[:, j], dtype)
+        assert rel(end[:, j], end64[:, j]) <= 1.5 * U[dtype] ** 2 + 60 * E
 
 
 # ------------------------------------------------------------------ decays that are NaN
