@@ -299,10 +299,11 @@ __device__ __forceinline__ bool forgotten(const MixArgs& p, float g, int u, bool
 // What units of chunks add to the state, for the segments that go on after them: sum_j l^(n-j) b_j c_j^T.  A chunk's products
 // start from 0, with weights to the chunk's end, and are added to the unit's sum in registers while the next chunk's run: a
 // product cuts its sum off at the accumulator's last bit, so that sums of many chunks on one accumulator would lose more the
-// longer a unit is (units of 111 chunks: 7e-5 of the state; 2e-6 so, for 3 % of a prompt of 8 heads of 65536 tokens, size 128).
-// Two warps copy and multiply, eight scale b and add up.
+// longer a unit is (units of 111 chunks: 7e-5 of the state, 6e-7 so).  Two warps copy and multiply, eight scale b and add up.
+// Blocks for heads above 64 take at most 144 registers a thread (as 448 threads would), so that the join's blocks are placed
+// beside them (8 heads of 65536 tokens, size 128: 216 us, 225 without).
 template <typename T, int W, bool REV>
-__global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_ends_kernel(const __grid_constant__ MixArgs p) {
+__global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay_ends_kernel(const __grid_constant__ MixArgs p) {
     constexpr int kTile = W * kBlock, kState = 64 * W, kTiles = kEndsRing<W>;
     constexpr bool F16 = std::is_same<T, __half>::value;
     extern __shared__ uint8_t raw[];
@@ -417,14 +418,14 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_ends_kernel(co
                 if constexpr (F16) w *= REV ? inverse2(s) : s * inverse2(held);
                 held = s;
 #pragma unroll
-                for (int c = 0; c < W; ++c)
-                    if (col0 + 32 * c < p.nb) {
-                        float v[32];
-                        tmem_ld32(tq + (mk & 1) * kState + col0 + 32 * c, v);
+                for (int c = 0; c < 32 * W; c += 16)
+                    if (col0 + c < p.nb) {
+                        float v[16];
+                        tmem_ld16(tq + (mk & 1) * kState + col0 + c, v);
                         tmem_wait_ld();
                         reg_fence(v);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) acc[32 * c + j] = REV ? __fmaf_rn(w, v[j], acc[32 * c + j]) : __fmaf_rn(w, acc[32 * c + j], v[j]);
+                        for (int j = 0; j < 16; ++j) acc[c + j] = REV ? __fmaf_rn(w, v[j], acc[c + j]) : __fmaf_rn(w, acc[c + j], v[j]);
                     }
                 tc_fence_before();
                 arrive(&read[mk & 1]);
