@@ -21,10 +21,10 @@
 // each term.  In fp16, whose range is narrow (gradients of 1e-6 would be
 // subnormal, products of large ones infinite), powers of two bring these operands
 // into it and are taken out of the sums: one per row of scores, from the largest
-// sizes in the row of a and in the chunk of b, which the copying warp looks up
-// beside its copies; one per chunk of b, at most 2^14 (of a term 2^-39 of the
-// chunk's largest b, or of 1, is lost); one per state.  (32x2x3136x32 training
-// takes 195 us so, 170 without; by the threads that scale b 213.)
+// size in the row of a and the largest that the row sees of b, which the copying
+// warp looks up beside its copies; one per chunk of weighted b, at most 2^14 (of
+// a term 2^-39 of the largest, or of 1, is lost); one per state.  (32x2x3136x32 training
+// takes 196 us so, 170 without; by the threads that scale b 213.)
 //
 // What bounds it.  Sequences are cut into segments until every block slot has
 // one (two slots per SM for heads up to 64); the state before a segment comes
@@ -240,7 +240,7 @@ __device__ __forceinline__ uint32_t largest16(const uint8_t* tile, int row, int 
 // 1 / s of a power of two between 2^-126 and 2^126.
 __device__ __forceinline__ float inverse2(float s) { return __uint_as_float(0x7f000000u - __float_as_uint(s)); }
 __device__ __forceinline__ float size16(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
-// For b of sizes up to `top` whose weights are up to `grow`: the weights times it, and b times them, stay below 2^15.
+// For weighted b of sizes up to `top` whose weights are up to `grow`: the weights times it, and b times them, stay below 2^15.
 __device__ __forceinline__ float weight_scale(float top, float grow) { return range_scale(__float_as_uint(fmaxf(top, 1.f) * fmaxf(grow, 1.f))); }
 
 // Scales rows of a tile of b, 8 at a time (eight lanes to a row, so that no bank is met twice): b w in two parts, the
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay
     uint64_t* const bars = reinterpret_cast<uint64_t*>(lows + 2 * kTile);
     uint64_t *full = bars, *empty = bars + kTiles, *ready = empty + kTiles, *used = ready + 2, *read = used + 2, *drain = read + 2;
     uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
-    uint32_t* const tops = tmem_ptr + 1;  // largest size in a chunk of b; three in turn
+    uint32_t* const tops = tmem_ptr + 1;  // largest size in a chunk of weighted b; three in turn
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_release();
     if (tid == 0) {
@@ -407,6 +407,7 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay
                 w[j] = power(g, REV ? r + 1 : kChunk - r);
                 spread(split_weight<T>(w[j]), wh[j >> 1][j & 1], wl[j >> 1][j & 1]);
             }
+            const float mine = F16 ? power(g, REV ? (tid >> 1) + 1 : kChunk - (tid >> 1)) : 0.f;  // of the row that this thread measures
             float acc[32 * W];
 #pragma unroll
             for (int j = 0; j < 32 * W; ++j) acc[j] = 0.f;
@@ -437,10 +438,11 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay
                 const float last = scale;
                 ok = ok && wait_for(&full[nb], 2 * m / kTiles & 1);
                 if constexpr (F16) {
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, (tid >> 1) < L ? largest16<W>(ring + nb * kTile, tid >> 1, (tid & 1) * 4 * W, 8 * W) : 0u);
+                    const float size = (tid >> 1) < L ? size16(largest16<W>(ring + nb * kTile, tid >> 1, (tid & 1) * 4 * W, 8 * W)) * mine : 0.f;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
                     if (lane == 0) atomicMax(&tops[turn], top);
                     epi_sync(true);
-                    scale = weight_scale(size16(tops[turn]), whole);
+                    scale = weight_scale(__uint_as_float(tops[turn]), whole);
                     if (tid == 0) tops[turn == 0 ? 2 : turn - 1] = 0;  // (read before this barrier, written after the next)
                     turn = turn == 2 ? 0 : turn + 1;
 #pragma unroll
@@ -543,10 +545,10 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     uint8_t* const low = ring + kRing * kTile;
     uint8_t* const gop = low + kTile;                                         // [state row][dc], 64 columns a block
     float* const pw = reinterpret_cast<float*>(gop + kState * 128 * W);       // l^n, n = 0..128
-    uint32_t* const gmax = reinterpret_cast<uint32_t*>(pw + 132);             // largest size in the state, and in a chunk of b;
-    uint32_t* const bmax = gmax + 2;                                          // two each, in turn (of the chunks)
-    uint16_t* const amax = reinterpret_cast<uint16_t*>(pw + 136);             // [2][128], largest size in each row of a
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 264);
+    uint32_t* const gmax = reinterpret_cast<uint32_t*>(pw + 132);             // largest size in the state; two in turn
+    float* const bmax = pw + 134;                                             // of a chunk's weighted b, and [2][128] of each
+    float* const most = pw + 136;                                             // row's scores at most; two in turn
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 392);
     uint64_t *full = bars, *empty = bars + kRing, *s_full = bars + 2 * kRing, *k_ready = s_full + 1, *p_ready = s_full + 2,
              *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7, *measured = s_full + 8;
     uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 10);
@@ -568,44 +570,77 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     const uint32_t tmem = *tmem_ptr;
     bool ok = true;
 
-    if (warp == 8) {  // copies, and in fp16 how large a's rows and b are
+    if (warp == 8) {  // copies, and in fp16 how large scores and weighted rows of b can be
         const bool one = elect_one();
         int n = 0, cc = 0;
         if (F16 || one)
             for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
                 const Item t = item_of(p, i);
+                float l[6];
+                if constexpr (F16)
+                    for (int j = 0; j < 6; ++j) l[j] = power(p.log_decay[t.h], j == 0 ? 1 : 2 << j);  // 1, 4, 8, 16, 32 and 64 rows
                 for (int k = 0; ok && k < t.n; ++k, ++cc) {
                     const int chunk = REV ? t.first + t.n - 1 - k : t.first + k, t0 = chunk * kChunk;
-                    for (int j = 0; j < 3; ++j) {
-                        const int s = n % kRing;
-                        if (!(ok = wait_for(&empty[s], (n / kRing & 1) ^ 1))) break;
-                        if (one) {
-                            expect(&full[s], kTile);
-                            const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
-                            for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
+                    auto copy = [&](int from, int to) {
+                        for (int j = from; ok && j < to; ++j) {
+                            const int s = n % kRing;
+                            if (!(ok = wait_for(&empty[s], (n / kRing & 1) ^ 1))) break;
+                            if (one) {
+                                expect(&full[s], kTile);
+                                const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
+                                for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
+                            }
+                            ++n;
                         }
-                        ++n;
-                    }
-                    if constexpr (F16) {
+                    };
+                    if constexpr (!F16) copy(0, 3);
+                    else {
+                        // c's place comes free later than a's and b's, and it is needed later: it waits until they have been measured, but
+                        // for the first one.
+                        const int na = n, nk = n + 1;
+                        copy(0, cc == 0 ? 3 : 2);
                         // The places of two chunks ago are free: their readers have let go of that chunk's b, whose place a has.
-                        ok = ok && wait_for(&full[(n - 3) % kRing], (n - 3) / kRing & 1) && wait_for(&full[(n - 2) % kRing], (n - 2) / kRing & 1);
+                        ok = ok && wait_for(&full[na % kRing], na / kRing & 1) && wait_for(&full[nk % kRing], nk / kRing & 1);
                         if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                        const uint8_t *ta = ring + (n - 3) % kRing * kTile, *tb = ring + (n - 2) % kRing * kTile;
+                        const uint8_t *ta = ring + na % kRing * kTile, *tb = ring + nk % kRing * kTile;
                         const int L = (int)min((int64_t)kChunk, t.len - (int64_t)t0), packs = (p.da + 7) / 8;
-                        uint32_t top = 0;
-#pragma unroll 2
-                        for (int i = 0; i < kChunk / 32; ++i) {
-                            const int r = i * 32 + lane;
+                        float* const mine = most + (cc & 1) * kChunk;
+                        float size[kChunk / 32];  // of a's rows
+#pragma unroll
+                        for (int q = 0; q < kChunk / 32; ++q) {
+                            const int r = q * 32 + lane;
                             uint32_t ma = largest16<W>(ta, r, 0, packs), mb = largest16<W>(tb, r, 0, packs);
                             if (packs > 4 * W) ma = max(ma, largest16<W>(ta, r, 4 * W, packs)), mb = max(mb, largest16<W>(tb, r, 4 * W, packs));
-                            if (r >= L) ma = mb = 0;
-                            amax[(cc & 1) * kChunk + r] = (uint16_t)ma;
-                            top = max(top, mb);
+                            size[q] = r < L ? size16(ma) : 0.f, mine[r] = r < L ? size16(mb) : 0.f;
                         }
-                        top = __reduce_max_sync(0xffffffffu, top);
-                        if (lane == 0) bmax[cc & 1] = top;
+                        __syncwarp();
+                        // The largest of b that a row sees, weighted as it sees it: of four rows by each lane, then of lanes 1, 2, 4, 8 and
+                        // 16 apart.
+                        float4 v = reinterpret_cast<float4*>(mine)[lane];
+                        if constexpr (REV) v.z = fmaxf(v.z, v.w * l[0]), v.y = fmaxf(v.y, v.z * l[0]), v.x = fmaxf(v.x, v.y * l[0]);
+                        else v.y = fmaxf(v.y, v.x * l[0]), v.z = fmaxf(v.z, v.y * l[0]), v.w = fmaxf(v.w, v.z * l[0]);
+                        float top = REV ? v.x : v.w;
+#pragma unroll
+                        for (int j = 0; j < 5; ++j) {
+                            const float x = REV ? __shfl_down_sync(0xffffffffu, top, 1 << j) : __shfl_up_sync(0xffffffffu, top, 1 << j);
+                            if (REV ? lane + (1 << j) < 32 : lane >= 1 << j) top = fmaxf(top, x * l[j + 1]);
+                        }
+                        float x = REV ? __shfl_down_sync(0xffffffffu, top, 1) : __shfl_up_sync(0xffffffffu, top, 1);
+                        if (lane == (REV ? 31 : 0)) x = 0.f;
+                        if constexpr (REV) {
+                            v.w = fmaxf(v.w, x *= l[0]), v.z = fmaxf(v.z, x *= l[0]), v.y = fmaxf(v.y, x *= l[0]), v.x = top;
+                            if (lane == 0) bmax[cc & 1] = top;
+                        } else {
+                            v.x = fmaxf(v.x, x *= l[0]), v.y = fmaxf(v.y, x *= l[0]), v.z = fmaxf(v.z, x *= l[0]), v.w = top;
+                            if (lane == (L - 1) >> 2) bmax[cc & 1] = (L & 3) == 1 ? v.x : (L & 3) == 2 ? v.y : (L & 3) == 3 ? v.z : v.w;
+                        }
+                        reinterpret_cast<float4*>(mine)[lane] = v;
+                        __syncwarp();
+#pragma unroll
+                        for (int q = 0; q < kChunk / 32; ++q) mine[q * 32 + lane] *= (float)p.da * size[q];
                         __syncwarp();
                         if (lane == 0) arrive(&measured[cc & 1]);
+                        if (cc > 0) copy(2, 3);
                     }
                 }
             }
@@ -685,8 +720,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
             bool has_g = (p.g0 || (t.n > 0 && t.seg != first_seg));
             float G[32 * W], unscale = 1.f;      // fp16: one over the scale of the state's operand,
-            float bscale = 1.f, btop = 0.f;      // the scale of b, and the largest size that a weight can give one of b's;
-            float held = 1.f;                    // without EXACT G is as the scaled products left it: this times too large
+            float bscale = 1.f, held = 1.f;      // the scale of b; without EXACT G is as the scaled products left it: `held` times too large
             // Chunk k of the item, its tokens, and 1 where the state shall not be decayed past its last token.
             auto chunk_of = [&](int k) { return REV ? t.first + t.n - 1 - k : t.first + k; };
             auto tokens_of = [&](int k) { return (int)min((int64_t)kChunk, t.len - (int64_t)chunk_of(k) * kChunk); };
@@ -694,8 +728,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             // fp16: the scale of the block's c-th chunk's b.
             auto measure = [&](int c) {
                 ok = wait_for(&measured[c & 1], c >> 1 & 1) && ok;
-                const float grow = pw[kChunk];
-                btop = size16(bmax[c & 1]), bscale = weight_scale(btop, grow), btop *= fmaxf(grow, 1.f);
+                bscale = weight_scale(bmax[c & 1], pw[kChunk]);
             };
             // G before chunk k: as an operand (rows of dc columns, in fp16 times a power of two that keeps the largest in
             // range), and decayed over the chunk to where the chunk's products, or their sum, add to it.
@@ -812,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 };
                 // The scores' scale: in fp16 a power of two by which the largest that this row can have stays in range, and the
                 // output's to undo it.
-                const float unit = F16 ? fminf(range_scale(__float_as_uint((float)p.da * size16(amax[(cc & 1) * kChunk + row]) * btop)), 0x1p40f) : p.scale;
+                const float unit = F16 ? fminf(range_scale(__float_as_uint(most[(cc & 1) * kChunk + row])), 0x1p40f) : p.scale;
                 const float back = F16 ? p.scale * inverse2(unit) : 1.f;
                 ok = wait_for(&full[nk % kRing], nk / kRing & 1) && ok;
                 fetch(0);

@@ -77,6 +77,32 @@ def test_attention_rows_of_unlike_sizes_fp16(t):
             assert not off(a[0, j], c[0, j], F16), (name, j)
 
 
+@pytest.mark.parametrize("t, at", [(128, 64), (300, 190)])
+def test_attention_beside_outliers_fp16(t, at):
+    """A token 2^27 times larger than the others costs those that do not see it (before it, or where it is forgotten) nothing."""
+    g, b, h, d = gen(t), 2, 3, 64
+    q, k, v, do = (heads(g, b, h, t, d, F16, s) for s in (1.0, 2.0**-12, 2.0**8, 2.0**-12))
+    q, k, v, do = (x.clone() for x in (q, k, v, do))
+    k[:, :, at, 3], do[:, :, at, 5] = 2.0**15, 2.0**15
+    dec = torch.tensor([-1.5, -0.004, 0.0], device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o, end = ops.decay_attention(*leaves, dec, return_state=True)
+    got = torch.autograd.grad(o, leaves, do)
+    l64 = [x.detach().double().requires_grad_() for x in leaves]
+    o64, end64 = attention64(*l64, dec)
+    want = torch.autograd.grad(o64, l64, do.double())
+    for j in range(h):
+        # o and dq look back, dk and dv ahead; after 30 tokens the first head has e^-45 of it left.
+        before, after = slice(0, at), slice(at + 1, t)
+        for name, a, c, rows in (("o", o, o64, before), ("dq", got[0], want[0], before), ("dk", got[1], want[1], after), ("dv", got[2], want[2], after)):
+            assert not off(a[:, j, rows], c[:, j, rows], F16), (name, j, rel(a[:, j, rows], c[:, j, rows]) / U[F16])
+        if j == 0:
+            before, after = slice(0, at - 30), slice(at + 30, t)
+            for name, a, c, rows in (("o", o, o64, after), ("dq", got[0], want[0], after), ("dk", got[1], want[1], before), ("dv", got[2], want[2], before)):
+                assert not off(a[:, j, rows], c[:, j, rows], F16), (name, j, rel(a[:, j, rows], c[:, j, rows]) / U[F16])
+            assert rel(end[:, j], end64[:, j]) <= 1.5 * U[F16] ** 2 + 60 * E
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_attention_of_growing_heads(dtype):
     """log_decay a little above 0: weights above 1 go the same way."""
