@@ -474,7 +474,8 @@ LF_API int lf_clip_grad_norm(const void* const* grads, void* const* outs, const 
    value_size].  log_decay: h floats, meant to be at most 0 (-inf: a token sees
    itself alone).  lengths: NULL, or tokens of each sequence (taken as 0 to t):
    later tokens are not read into any result, and their rows of the outputs are 0.
-   state_out (may be NULL): the state after the last token.
+   state_out (may be NULL): the state after the last token; it may be `state`, and
+   d_state may be d_state_out.
    The backward takes d_o and (NULL: 0) d_state_out and writes the gradients that
    are not NULL; d_state needs dv.  Scores (scale q k^T, and scale d_o v^T in the
    backward) are operands of a second product in dtype, in fp16 scaled into its

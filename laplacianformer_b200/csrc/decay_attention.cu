@@ -41,6 +41,7 @@
 // A token at a time only the state matters: 192x16 heads of 64: 15 us, 6.7 TB/s.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "tc_ptx.cuh"
 #include "tma_map.h"
@@ -1358,10 +1359,30 @@ int check_attention(const char* what, const lf_decay_attention_t* a, bool bwd) {
     if (!aligned(a->lengths, 8)) return refuse(what, "a pointer is not aligned to its elements");
     if (!aligned(a->sums, 256)) return refuse(what, "sums must be 256-byte aligned");
     if (a->b == 0 || a->h == 0) return LF_OK;
+    const uintptr_t n = (uintptr_t)(a->b * a->h * a->key_size * a->value_size) * 4;
+    for (const auto& x : {std::make_pair(a->state, a->state_out), std::make_pair(a->d_state_out, a->d_state)}) {
+        const uintptr_t from = (uintptr_t)x.first, to = (uintptr_t)x.second;
+        if (from && to && from != to && from < to + n && to < from + n) return refuse(what, "a state and the one that is written overlap without being the same");
+    }
     if (!a->log_decay) return refuse(what, "log_decay is required");
     if (a->t > 0 && (!a->q || !a->k || !a->v || (!bwd && !a->o) || (bwd && !a->d_o))) return refuse(what, "q, k, v and the output or its gradient are required");
     if (bwd && a->t > 0 && a->d_state && !a->dv) return refuse(what, "the state's gradient comes with dv");
     return LF_OK;
+}
+
+// A state updated in place where a sequence is cut: several blocks read what one of them writes, so they read a copy.
+size_t state_bytes(const lf_decay_attention_t* a) { return (size_t)(a->b * a->h * a->key_size * a->value_size) * 4; }
+size_t copy_bytes(const lf_decay_attention_t* a, const float* from, const float* to) {
+    return from && from == to && deal({a->b, a->h, a->t}, blocks_of(a->key_size, a->value_size)).nseg > 1 ? (state_bytes(a) + 255) / 256 * 256 : 0;
+}
+// `from`, or its copy at `at` (moved on).
+const float* read_apart(const lf_decay_attention_t* a, const float* from, const float* to, uint8_t*& at, cudaStream_t st) {
+    const size_t n = copy_bytes(a, from, to);
+    if (n == 0) return from;
+    cudaMemcpyAsync(at, from, state_bytes(a), cudaMemcpyDeviceToDevice, st);
+    const float* const copy = (const float*)at;
+    at += n;
+    return copy;
 }
 
 Heads heads_of(const void* p, const int64_t* s, int64_t d) { return {p, s[0], s[1], s[2], d}; }
@@ -1369,7 +1390,7 @@ Heads dense_heads(void* p, const Sizes& z, int64_t d) { return {p, z.t * z.h * d
 
 // T = 0: the state passes through.
 int pass_state(const char* what, const float* from, float* to, size_t bytes, cudaStream_t st) {
-    if (to && (from ? cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(to, 0, bytes, st)) != cudaSuccess)
+    if (to && to != from && (from ? cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(to, 0, bytes, st)) != cudaSuccess)
         return check_launch(what);
     return LF_OK;
 }
@@ -1388,7 +1409,8 @@ extern "C" size_t lf_decay_attention_fwd_workspace_size(const lf_decay_attention
     if (!a || check_attention("lf_decay_attention_fwd", a, false) || a->b == 0 || a->h == 0 || a->t == 0) return 0;
     const Sizes z{a->b, a->h, a->t};
     return packed_bytes(heads_of(a->q, a->q_strides, a->key_size), z) + packed_bytes(heads_of(a->k, a->k_strides, a->key_size), z) +
-           packed_bytes(heads_of(a->v, a->v_strides, a->value_size), z) + (a->sums ? 0 : ends_bytes(z, blocks_of(a->key_size, a->value_size)));
+           packed_bytes(heads_of(a->v, a->v_strides, a->value_size), z) + copy_bytes(a, a->state, a->state_out) +
+           (a->sums ? 0 : ends_bytes(z, blocks_of(a->key_size, a->value_size)));
 }
 
 extern "C" int lf_decay_attention_fwd(const lf_decay_attention_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
@@ -1397,7 +1419,7 @@ extern "C" int lf_decay_attention_fwd(const lf_decay_attention_t* a, void* works
     if (int rc = check_attention(what, a, false)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     if (a->b == 0 || a->h == 0) return LF_OK;
-    if (a->t == 0) return pass_state(what, a->state, a->state_out, (size_t)(a->b * a->h * a->key_size * a->value_size) * 4, st);
+    if (a->t == 0) return pass_state(what, a->state, a->state_out, state_bytes(a), st);
     const size_t need = lf_decay_attention_fwd_workspace_size(a);
     if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) {
         set_error("%s: needs %zu bytes of 256-byte aligned workspace, got %zu", what, need, workspace ? workspace_bytes : (size_t)0);
@@ -1410,7 +1432,7 @@ extern "C" int lf_decay_attention_fwd(const lf_decay_attention_t* a, void* works
     m.b = addressable(heads_of(a->k, a->k_strides, a->key_size), z, at, st);
     m.c = addressable(heads_of(a->v, a->v_strides, a->value_size), z, at, st);
     m.out = dense_heads(a->o, z, a->value_size);
-    m.g0 = a->state, m.gout = a->state_out;
+    m.g0 = read_apart(a, a->state, a->state_out, at, st), m.gout = a->state_out;
     return run_mix(m, z, a->log_decay, a->lengths, a->scale, a->dtype, a->sums ? a->sums : (float*)at, st);
 }
 
@@ -1419,7 +1441,7 @@ extern "C" size_t lf_decay_attention_bwd_workspace_size(const lf_decay_attention
     const Sizes z{a->b, a->h, a->t};
     return packed_bytes(heads_of(a->q, a->q_strides, a->key_size), z) + packed_bytes(heads_of(a->k, a->k_strides, a->key_size), z) +
            packed_bytes(heads_of(a->v, a->v_strides, a->value_size), z) + packed_bytes(heads_of(a->d_o, a->do_strides, a->value_size), z) +
-           ends_bytes(z, blocks_of(a->key_size, a->value_size));
+           copy_bytes(a, a->d_state_out, a->d_state) + ends_bytes(z, blocks_of(a->key_size, a->value_size));
 }
 
 extern "C" int lf_decay_attention_bwd(const lf_decay_attention_t* a, void* workspace, size_t workspace_bytes, lf_stream_t stream) {
@@ -1428,7 +1450,7 @@ extern "C" int lf_decay_attention_bwd(const lf_decay_attention_t* a, void* works
     if (int rc = check_attention(what, a, true)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     if (a->b == 0 || a->h == 0) return LF_OK;
-    if (a->t == 0) return pass_state(what, a->d_state_out, a->d_state, (size_t)(a->b * a->h * a->key_size * a->value_size) * 4, st);
+    if (a->t == 0) return pass_state(what, a->d_state_out, a->d_state, state_bytes(a), st);
     const size_t need = lf_decay_attention_bwd_workspace_size(a);
     if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) {
         set_error("%s: needs %zu bytes of 256-byte aligned workspace, got %zu", what, need, workspace ? workspace_bytes : (size_t)0);
@@ -1440,6 +1462,7 @@ extern "C" int lf_decay_attention_bwd(const lf_decay_attention_t* a, void* works
     const Heads k = addressable(heads_of(a->k, a->k_strides, a->key_size), z, at, st);
     const Heads v = addressable(heads_of(a->v, a->v_strides, a->value_size), z, at, st);
     const Heads g = addressable(heads_of(a->d_o, a->do_strides, a->value_size), z, at, st);
+    const float* const d_state_out = read_apart(a, a->d_state_out, a->d_state, at, st);
     auto mix = [&](const Heads& x, const Heads& y, const Heads& w, void* out, const float* g0, float* gout, bool transposed, bool rev,
                    bool turned) {
         Mix m;
@@ -1450,9 +1473,9 @@ extern "C" int lf_decay_attention_bwd(const lf_decay_attention_t* a, void* works
     if (a->dq)
         if (int rc = mix(g, v, k, a->dq, a->state, nullptr, true, false, a->sums != nullptr)) return rc;
     if (a->dk)
-        if (int rc = mix(v, g, q, a->dk, a->d_state_out, nullptr, true, true, false)) return rc;
+        if (int rc = mix(v, g, q, a->dk, d_state_out, nullptr, true, true, false)) return rc;
     if (a->dv)
-        if (int rc = mix(k, q, g, a->dv, a->d_state_out, a->d_state, false, true, a->dk != nullptr)) return rc;
+        if (int rc = mix(k, q, g, a->dv, d_state_out, a->d_state, false, true, a->dk != nullptr)) return rc;
     return LF_OK;
 }
 

@@ -1,4 +1,5 @@
-"""CPU-side checks of the causal operators' edges: row numbers past 32 bits, tensors that stay on the host."""
+"""CPU-side checks of the causal operators' edges: row numbers past 32 bits, tensors that stay on the host, states in place."""
+import ctypes
 import os
 import subprocess
 
@@ -8,6 +9,8 @@ import torch
 from laplacianformer_b200 import capi, ops
 from laplacianformer_b200.block import DecayBlock
 
+L = capi.lib()
+P = 1 << 20  # stands for a device pointer: nothing here gets as far as using it
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 GROUPS = r"""
@@ -59,3 +62,22 @@ def test_frequencies_are_on_the_host(scaling):
         block = DecayBlock(32, 2)
     assert f.device.type == "cpu" and torch.equal(f, want)
     assert block.frequencies.device.type == "cpu" and block.log_decay.device.type == "meta"
+
+
+def attention(t, **kw):
+    s = (ctypes.c_int64 * 3)(t * 2 * 64, 64, 2 * 64)
+    return capi.DecayAttention(**{"q": P, "k": P, "v": P, "log_decay": P, "o": P, "b": 1, "h": 2, "t": t, "key_size": 64, "value_size": 64, "scale": 0.125,
+                                  "dtype": capi.LF_BF16, "q_strides": s, "k_strides": s, "v_strides": s, "do_strides": s} | kw)
+
+
+def test_states_in_place_are_read_from_a_copy():
+    """Where a sequence is cut, several blocks read the state that one of them writes."""
+    fwd, bwd, n = L.lf_decay_attention_fwd_workspace_size, L.lf_decay_attention_bwd_workspace_size, 2 * 64 * 64 * 4
+    assert fwd(attention(100, state=P, state_out=P)) == 0  # one block reads and writes it
+    assert fwd(attention(5000, state=P, state_out=P)) == fwd(attention(5000, state=P, state_out=2 * P)) + n
+    back = {"d_o": P, "dv": P, "d_state_out": P}
+    assert bwd(attention(5000, d_state=P, **back)) == bwd(attention(5000, d_state=2 * P, **back)) + n
+    for near in (P + 4, P + n - 4, P - 4, P - n + 4):
+        assert L.lf_decay_attention_fwd(attention(100, state=P, state_out=near), None, 0, None) == capi.LF_ERR_INVALID and b"overlap" in L.lf_last_error()
+        assert L.lf_decay_attention_bwd(attention(100, d_state=near, **back), None, 0, None) == capi.LF_ERR_INVALID and b"overlap" in L.lf_last_error()
+    assert fwd(attention(5000, state=P, state_out=P + n)) == fwd(attention(5000, state=P, state_out=2 * P))

@@ -2,12 +2,13 @@
 far positions, more than 2^31 rows.
 
 Tolerances as in test_causal_gpu.py: u half a step of the type, E of fp32, 1.25 u of the norm for an attention output."""
+import ctypes
 from fractions import Fraction
 
 import pytest
 import torch
 
-from laplacianformer_b200 import ops
+from laplacianformer_b200 import capi, ops
 from test_causal_gpu import BF16, E, F16, F32, TINY, U, attention64, decays, gen, heads, rand, rel, within
 
 pytestmark = pytest.mark.gpu
@@ -144,6 +145,37 @@ def test_attention_nan_decay(t, with_state, dtype):
     o, dq, dk, dv, end = out[1]
     assert torch.isnan(end[:, 1]).all() and torch.isnan(o[:, 1, 1:]).all() and torch.isnan(dq[:, 1, 1:]).all()
     assert torch.isnan(dk[:, 1, :-1]).all() and torch.isnan(dv[:, 1, :-1]).all()
+
+
+# ------------------------------------------------------------------ states in place
+
+
+@pytest.mark.parametrize("b, h, t, d", [(2, 3, 100, 64), (1, 2, 5000, 64), (3, 1, 2000, 128), (7, 50, 1500, 32), (2, 2, 0, 16)])
+def test_attention_states_in_place(b, h, t, d):
+    """C callers may have the state, and its gradient, written over the one that is read."""
+    g = gen(t)
+    q, k, v, do = (heads(g, b, h, t, d, BF16) for _ in range(4))
+    state, dec = rand(g, b, h, d, d).requires_grad_(), torch.tensor([-0.01, -0.5, -0.0001], device="cuda").repeat(20)[:h].clone()
+    o, end = ops.decay_attention(q, k, v, dec, state, return_state=True)
+    dend = rand(g, b, h, d, d)
+    (want,) = torch.autograd.grad((o, end), state, (do, dend))
+    ptr = lambda x: x.data_ptr() or None  # noqa: E731
+    mine, out, grad, dv = state.detach().clone(), torch.empty(b, t, h, d, dtype=BF16, device="cuda"), dend.clone(), torch.empty(b, t, h, d, dtype=BF16, device="cuda")
+    s = (ctypes.c_int64 * 3)(t * h * d, d, h * d)
+    a = capi.DecayAttention(q=ptr(q), k=ptr(k), v=ptr(v), log_decay=ptr(dec), state=ptr(mine), state_out=ptr(mine), o=ptr(out), q_strides=s, k_strides=s, v_strides=s,
+                            do_strides=s, b=b, h=h, t=t, key_size=d, value_size=d, scale=d**-0.5, dtype=capi.LF_BF16)
+    L, stream = capi.lib(), torch.cuda.current_stream().cuda_stream
+
+    def call(size, run):
+        n = size(a)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        assert run(a, ptr(ws), n, stream) == capi.LF_OK, L.lf_last_error()
+
+    call(L.lf_decay_attention_fwd_workspace_size, L.lf_decay_attention_fwd)
+    assert torch.equal(mine, end) and torch.equal(out.transpose(1, 2), o)
+    a.state, a.state_out, a.d_o, a.d_state_out, a.d_state, a.dv = ptr(state), None, ptr(do), ptr(grad), ptr(grad), ptr(dv)
+    call(L.lf_decay_attention_bwd_workspace_size, L.lf_decay_attention_bwd)
+    assert torch.equal(grad, want)
 
 
 # ------------------------------------------------------------------ gates
