@@ -20,11 +20,13 @@
 // two 16-bit parts so that the state keeps about 17 bits (bf16) or 22 (fp16) of
 // each term.  In fp16, whose range is narrow (gradients of 1e-6 would be
 // subnormal, products of large ones infinite), powers of two bring these operands
-// into it and are taken out of the sums: one per row of scores, from the largest
-// size in the row of a and the largest that the row sees of b, which the copying
-// warp looks up beside its copies; one per chunk of weighted b, at most 2^14 (of
-// a term 2^-39 of the largest, or of 1, is lost); one per state.  (32x2x3136x32 training
-// takes 196 us so, 170 without; by the threads that scale b 213.)
+// into it and are taken out of the sums: one per row of scores, by its largest
+// weighted score; one per chunk of b, by its largest weighted row, at most 2^14 (of
+// a term 2^-30 of the largest is lost, or 2^-39); one per state.  What it takes to
+// find them: 32x2x3136x32 training 170 -> 201 us, 8x16x16384x64 training 1.39 ->
+// 1.56 ms, 8 heads of 65536 tokens, size 128, 231 -> 268 us.  (Bounds by the sizes
+// of a's rows and b, looked up by the copying warp: 196 us, 1.71 ms, 402 us; by a
+// launch of their own: 215 us, 1.93 ms, 335 us.)
 //
 // What bounds it.  Sequences are cut into segments until every block slot has
 // one (two slots per SM for heads up to 64); the state before a segment comes
@@ -219,57 +221,54 @@ __device__ __forceinline__ float range_scale(uint32_t bits) {
 }
 
 // fp16 operands of products are brought into fp16's range by powers of two, which the products' sums are freed of again.
-// The largest size among 16-bit pairs, in bits (a NaN's are the largest), and of the first `packs` packs of 8 in a tile's row.
-__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-template <int W>
-__device__ __forceinline__ uint32_t largest16(const uint8_t* tile, int row, int from, int packs) {
-    uint32_t m = 0;
+// The largest size among fp16 pairs (NaN only where all are).
+template <int N>
+__device__ __forceinline__ float largest16(const uint4 (&x)[N]) {
+    __half2 m = __half2half2(__ushort_as_half(0));
 #pragma unroll
-    for (int j = 0; j < 4 * W; ++j) {
-        const int c = from + j;
-        if (c < packs) {
-            const uint4 x = *reinterpret_cast<const uint4*>(tile + (c >> 3) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4));
-            m = max16x2(max16x2(m, max16x2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu)), max16x2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-        }
+    for (int j = 0; j < N; ++j) {
+        const uint32_t v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&v[q])));
     }
-    return max(m & 0xffffu, m >> 16);
+    return fmaxf(__low2float(m), __high2float(m));
 }
 // 1 / s of a power of two between 2^-126 and 2^126.
 __device__ __forceinline__ float inverse2(float s) { return __uint_as_float(0x7f000000u - __float_as_uint(s)); }
-__device__ __forceinline__ float size16(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+__device__ __forceinline__ float largest8(const float* p) {
+    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+    return fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+}
 // For weighted b of sizes up to `top` whose weights are up to `grow`: the weights times it, and b times them, stay below 2^15.
 __device__ __forceinline__ float weight_scale(float top, float grow) { return range_scale(__float_as_uint(fmaxf(top, 1.f) * fmaxf(grow, 1.f))); }
 
 // Scales rows of a tile of b, 8 at a time (eight lanes to a row, so that no bank is met twice): b w in two parts, the
 // first in place, the second negated in `low`; w0 and w1 are a row's weight in two parts, for the rows 4 apart.
 //   high = b w0 rounded;  b w0 - high is exact (it has no more bits than b), and b w1 joins it with one rounding
+__device__ __forceinline__ int row_pack(int w, int r, int ch) { return w * kBlock + r * 128 + ((ch ^ (r & 7)) << 4); }
+template <int W>
+__device__ __forceinline__ void fetch_rows(const uint8_t* tile, int row0, int lane, uint4 (&x)[2][W]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[i][w] = *reinterpret_cast<const uint4*>(tile + row_pack(w, row0 + (lane >> 3) + 4 * i, lane & 7));
+}
 template <typename T, int W>
-__device__ __forceinline__ void scale_rows(uint8_t* tile, uint8_t* low, int row0, int lane, const uint32_t (&wh)[2], const uint32_t (&wl)[2]) {
-    const int r = row0 + (lane >> 3), ch = lane & 7;
+__device__ __forceinline__ void scale_rows(uint8_t* tile, uint8_t* low, int row0, int lane, const uint4 (&x)[2][W], const uint32_t (&wh)[2], const uint32_t (&wl)[2]) {
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-        uint4 x[2];
-        int at[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            at[i] = w * kBlock + (r + 4 * i) * 128 + ((ch ^ ((r + 4 * i) & 7)) << 4);
-            x[i] = *reinterpret_cast<const uint4*>(tile + at[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            const uint32_t v[4] = {x[i][w].x, x[i][w].y, x[i][w].z, x[i][w].w};
             uint32_t h[4], l[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 h[q] = mul16x2<T>(v[q], wh[i]);
                 l[q] = fma16x2<T>(v[q], wl[i] ^ 0x80008000u, fma16x2<T>(v[q], wh[i] ^ 0x80008000u, h[q]));
             }
-            sts16(tile + at[i], make_uint4(h[0], h[1], h[2], h[3]));
-            sts16(low + at[i], make_uint4(l[0], l[1], l[2], l[3]));
+            const int at = row_pack(w, row0 + (lane >> 3) + 4 * i, lane & 7);
+            sts16(tile + at, make_uint4(h[0], h[1], h[2], h[3]));
+            sts16(low + at, make_uint4(l[0], l[1], l[2], l[3]));
         }
     }
 }
@@ -313,14 +312,13 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay
     uint64_t* const bars = reinterpret_cast<uint64_t*>(lows + 2 * kTile);
     uint64_t *full = bars, *empty = bars + kTiles, *ready = empty + kTiles, *used = ready + 2, *read = used + 2, *drain = read + 2;
     uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
-    uint32_t* const tops = tmem_ptr + 1;  // largest size in a chunk of weighted b; three in turn
+    float* const tops = reinterpret_cast<float*>(drain + 2);  // [2][8], largest weighted b that a warp has seen
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_release();
     if (tid == 0) {
         for (int i = 0; i < kTiles; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&ready[i], kEpi), mbar_init(&used[i], 1), mbar_init(&read[i], kEpi);
         mbar_init(drain, 1);
-        tops[0] = tops[1] = tops[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) tmem_alloc(tmem_ptr, 2 * kState);
@@ -395,7 +393,7 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay
     } else {
         const int quad = warp & 3, half = warp >> 2, col0 = half * 32 * W;
         const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16);
-        int m = 0, turn = 0;
+        int m = 0;
         for (int i = blockIdx.x; i < count; i += gridDim.x) {
             const Unit x = unit_of(i);
             if (x.n == 0) continue;
@@ -408,7 +406,6 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay
                 w[j] = power(g, REV ? r + 1 : kChunk - r);
                 spread(split_weight<T>(w[j]), wh[j >> 1][j & 1], wl[j >> 1][j & 1]);
             }
-            const float mine = F16 ? power(g, REV ? (tid >> 1) + 1 : kChunk - (tid >> 1)) : 0.f;  // of the row that this thread measures
             float acc[32 * W];
 #pragma unroll
             for (int j = 0; j < 32 * W; ++j) acc[j] = 0.f;
@@ -438,19 +435,28 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 448, W == 1 ? 2 : 1) decay
                 uint8_t* const low = lows + (m & 1) * kTile;  // (its last products' sum has been read)
                 const float last = scale;
                 ok = ok && wait_for(&full[nb], 2 * m / kTiles & 1);
+                uint4 rows[2][2][W];
                 if constexpr (F16) {
-                    const float size = (tid >> 1) < L ? size16(largest16<W>(ring + nb * kTile, tid >> 1, (tid & 1) * 4 * W, 8 * W)) * mine : 0.f;
+                    float size = 0.f;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        fetch_rows<W>(ring + nb * kTile, warp * 16 + u * 8, lane, rows[u]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (warp * 16 + u * 8 + (lane >> 3) + 4 * i < L) size = fmaxf(size, largest16(rows[u][i]) * w[2 * u + i]);
+                    }
                     const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
-                    if (lane == 0) atomicMax(&tops[turn], top);
+                    if (lane == 0) tops[(m & 1) * 8 + warp] = __uint_as_float(top);
                     epi_sync(true);
-                    scale = weight_scale(__uint_as_float(tops[turn]), whole);
-                    if (tid == 0) tops[turn == 0 ? 2 : turn - 1] = 0;  // (read before this barrier, written after the next)
-                    turn = turn == 2 ? 0 : turn + 1;
+                    scale = weight_scale(largest8(tops + (m & 1) * 8), whole);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) spread(split_weight<T>(w[j] * scale), wh[j >> 1][j & 1], wl[j >> 1][j & 1]);
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) scale_rows<T, W>(ring + nb * kTile, low, warp * 16 + u * 8, lane, wh[u], wl[u]);
+                for (int u = 0; u < 2; ++u) {
+                    if constexpr (!F16) fetch_rows<W>(ring + nb * kTile, warp * 16 + u * 8, lane, rows[u]);
+                    scale_rows<T, W>(ring + nb * kTile, low, warp * 16 + u * 8, lane, rows[u], wh[u], wl[u]);
+                }
                 if (L < kChunk) {
                     ok = ok && wait_for(&full[nc], (2 * m + 1) / kTiles & 1);
                     epi_sync(true);  // (the rows that others scaled)
@@ -547,19 +553,18 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     uint8_t* const gop = low + kTile;                                         // [state row][dc], 64 columns a block
     float* const pw = reinterpret_cast<float*>(gop + kState * 128 * W);       // l^n, n = 0..128
     uint32_t* const gmax = reinterpret_cast<uint32_t*>(pw + 132);             // largest size in the state; two in turn
-    float* const bmax = pw + 134;                                             // of a chunk's weighted b, and [2][128] of each
-    float* const most = pw + 136;                                             // row's scores at most; two in turn
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 392);
+    float* const tops = pw + 136;                                             // largest weighted b that a warp has seen
+    float* const most = pw + 144;                                             // [2][128], largest score in each half of a row
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(pw + 400);
     uint64_t *full = bars, *empty = bars + kRing, *s_full = bars + 2 * kRing, *k_ready = s_full + 1, *p_ready = s_full + 2,
-             *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7, *measured = s_full + 8;
-    uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 10);
+             *kv_full = s_full + 3, *o_full = s_full + 4, *g_ready = s_full + 5, *qg_full = s_full + 6, *drain = s_full + 7;
+    uint32_t* const tmem_ptr = reinterpret_cast<uint32_t*>(s_full + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_release();
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         mbar_init(s_full, 1), mbar_init(kv_full, 1), mbar_init(o_full, 1), mbar_init(qg_full, 1), mbar_init(drain, 1);
         mbar_init(k_ready, kEpi), mbar_init(p_ready, kEpi), mbar_init(g_ready, kEpi);
-        mbar_init(&measured[0], 1), mbar_init(&measured[1], 1);
         gmax[0] = gmax[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -571,82 +576,26 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
     const uint32_t tmem = *tmem_ptr;
     bool ok = true;
 
-    if (warp == 8) {  // copies, and in fp16 how large scores and weighted rows of b can be
-        const bool one = elect_one();
-        int n = 0, cc = 0;
-        if (F16 || one)
+    if (warp == 8) {  // copies
+        if (elect_one()) {
+            int n = 0;
             for (int i = blockIdx.x; ok && i < p.items; i += gridDim.x) {
                 const Item t = item_of(p, i);
-                float l[6];
-                if constexpr (F16)
-                    for (int j = 0; j < 6; ++j) l[j] = power(p.log_decay[t.h], j == 0 ? 1 : 2 << j);  // 1, 4, 8, 16, 32 and 64 rows
-                for (int k = 0; ok && k < t.n; ++k, ++cc) {
-                    const int chunk = REV ? t.first + t.n - 1 - k : t.first + k, t0 = chunk * kChunk;
-                    auto copy = [&](int from, int to) {
-                        for (int j = from; ok && j < to; ++j) {
-                            const int s = n % kRing;
-                            if (!(ok = wait_for(&empty[s], (n / kRing & 1) ^ 1))) break;
-                            if (one) {
-                                expect(&full[s], kTile);
-                                const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
-                                for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
-                            }
-                            ++n;
-                        }
-                    };
-                    if constexpr (!F16) copy(0, 3);
-                    else {
-                        // c's place comes free later than a's and b's, and it is needed later: it waits until they have been measured, but
-                        // for the first one.
-                        const int na = n, nk = n + 1;
-                        copy(0, cc == 0 ? 3 : 2);
-                        // The places of two chunks ago are free: their readers have let go of that chunk's b, whose place a has.
-                        ok = ok && wait_for(&full[na % kRing], na / kRing & 1) && wait_for(&full[nk % kRing], nk / kRing & 1);
-                        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                        const uint8_t *ta = ring + na % kRing * kTile, *tb = ring + nk % kRing * kTile;
-                        const int L = (int)min((int64_t)kChunk, t.len - (int64_t)t0), packs = (p.da + 7) / 8;
-                        float* const mine = most + (cc & 1) * kChunk;
-                        float size[kChunk / 32];  // of a's rows
-#pragma unroll
-                        for (int q = 0; q < kChunk / 32; ++q) {
-                            const int r = q * 32 + lane;
-                            uint32_t ma = largest16<W>(ta, r, 0, packs), mb = largest16<W>(tb, r, 0, packs);
-                            if (packs > 4 * W) ma = max(ma, largest16<W>(ta, r, 4 * W, packs)), mb = max(mb, largest16<W>(tb, r, 4 * W, packs));
-                            size[q] = r < L ? size16(ma) : 0.f, mine[r] = r < L ? size16(mb) : 0.f;
-                        }
-                        __syncwarp();
-                        // The largest of b that a row sees, weighted as it sees it: of four rows by each lane, then of lanes 1, 2, 4, 8 and
-                        // 16 apart.
-                        float4 v = reinterpret_cast<float4*>(mine)[lane];
-                        if constexpr (REV) v.z = fmaxf(v.z, v.w * l[0]), v.y = fmaxf(v.y, v.z * l[0]), v.x = fmaxf(v.x, v.y * l[0]);
-                        else v.y = fmaxf(v.y, v.x * l[0]), v.z = fmaxf(v.z, v.y * l[0]), v.w = fmaxf(v.w, v.z * l[0]);
-                        float top = REV ? v.x : v.w;
-#pragma unroll
-                        for (int j = 0; j < 5; ++j) {
-                            const float x = REV ? __shfl_down_sync(0xffffffffu, top, 1 << j) : __shfl_up_sync(0xffffffffu, top, 1 << j);
-                            if (REV ? lane + (1 << j) < 32 : lane >= 1 << j) top = fmaxf(top, x * l[j + 1]);
-                        }
-                        float x = REV ? __shfl_down_sync(0xffffffffu, top, 1) : __shfl_up_sync(0xffffffffu, top, 1);
-                        if (lane == (REV ? 31 : 0)) x = 0.f;
-                        if constexpr (REV) {
-                            v.w = fmaxf(v.w, x *= l[0]), v.z = fmaxf(v.z, x *= l[0]), v.y = fmaxf(v.y, x *= l[0]), v.x = top;
-                            if (lane == 0) bmax[cc & 1] = top;
-                        } else {
-                            v.x = fmaxf(v.x, x *= l[0]), v.y = fmaxf(v.y, x *= l[0]), v.z = fmaxf(v.z, x *= l[0]), v.w = top;
-                            if (lane == (L - 1) >> 2) bmax[cc & 1] = (L & 3) == 1 ? v.x : (L & 3) == 2 ? v.y : (L & 3) == 3 ? v.z : v.w;
-                        }
-                        reinterpret_cast<float4*>(mine)[lane] = v;
-                        __syncwarp();
-#pragma unroll
-                        for (int q = 0; q < kChunk / 32; ++q) mine[q * 32 + lane] *= (float)p.da * size[q];
-                        __syncwarp();
-                        if (lane == 0) arrive(&measured[cc & 1]);
-                        if (cc > 0) copy(2, 3);
+                for (int k = 0; ok && k < t.n; ++k) {
+                    const int t0 = (REV ? t.first + t.n - 1 - k : t.first + k) * kChunk;
+                    for (int j = 0; j < 3; ++j) {
+                        const int s = n % kRing;
+                        if (!(ok = wait_for(&empty[s], (n / kRing & 1) ^ 1))) break;
+                        expect(&full[s], kTile);
+                        const CUtensorMap* m = j == 0 ? &p.a : j == 1 ? &p.b : &p.c;
+                        for (int w = 0; w < W; ++w) load4d(ring + s * kTile + w * kBlock, m, &full[s], w * 64, t.h, t0, t.b);
+                        ++n;
                     }
                 }
             }
-        if (one && !ok)  // a wait ran out: let the copies in flight land
-            for (int k = max(0, n - kRing); k < n; ++k) mbar_wait(&full[k % kRing], k / kRing & 1, 100000000ull);
+            if (!ok)  // a wait ran out: let the copies in flight land
+                for (int k = max(0, n - kRing); k < n; ++k) mbar_wait(&full[k % kRing], k / kRing & 1, 100000000ull);
+        }
         __syncwarp();
     } else if (warp == 9) {  // products
         const uint32_t go = elect_one() ? 1u : 0u;
@@ -721,16 +670,12 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             const int first_seg = REV ? (t.active - 1) / p.per_seg : 0;
             bool has_g = (p.g0 || (t.n > 0 && t.seg != first_seg));
             float G[32 * W], unscale = 1.f;      // fp16: one over the scale of the state's operand,
-            float bscale = 1.f, held = 1.f;      // the scale of b; without EXACT G is as the scaled products left it: `held` times too large
+            float bscale = 1.f;                  // and b's scale, which without EXACT the state has too
+            const float grow = F16 ? fmaxf(exp2_of(15.f * g2), 1.f) : 1.f;
             // Chunk k of the item, its tokens, and 1 where the state shall not be decayed past its last token.
             auto chunk_of = [&](int k) { return REV ? t.first + t.n - 1 - k : t.first + k; };
             auto tokens_of = [&](int k) { return (int)min((int64_t)kChunk, t.len - (int64_t)chunk_of(k) * kChunk); };
             auto last_of = [&](int k) { return !REV && p.gout && chunk_of(k) == t.active - 1 ? 1 : 0; };
-            // fp16: the scale of the block's c-th chunk's b.
-            auto measure = [&](int c) {
-                ok = wait_for(&measured[c & 1], c >> 1 & 1) && ok;
-                bscale = weight_scale(bmax[c & 1], pw[kChunk]);
-            };
             // G before chunk k: as an operand (rows of dc columns, in fp16 times a power of two that keeps the largest in
             // range), and decayed over the chunk to where the chunk's products, or their sum, add to it.
             auto put_state = [&](int k) {
@@ -745,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     epi_sync(true);
                     s = range_scale(gmax[slot]);
                     if (tid == 0) gmax[slot ^ 1] = 0;
-                    unscale = inverse2(s) * inverse2(held);
+                    unscale = inverse2(s) * (EXACT ? 1.f : inverse2(bscale));
                 }
                 if (live) {
                     uint8_t* const dst = gop + (W == 2 ? half * kState * 128 : 0) + srow * 128;
@@ -760,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     }
                 }
                 fence_async_smem();
-                const float w = pw[tokens_of(k) - last_of(k)] * (F16 && !EXACT ? bscale * inverse2(held) : 1.f);
+                const float w = pw[tokens_of(k) - last_of(k)];
                 const uint64_t w2 = pk2(w, w);
 #pragma unroll
                 for (int c = 0; c < 2 * W; ++c)
@@ -817,7 +762,6 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
             }
             epi_sync(true);  // the tables are written
             if (t.n > 0) {
-                if constexpr (F16) measure(cc);
                 if (has_g) {
                     if (W == 1 && EXACT)  // (the other lanes are 0)
 #pragma unroll
@@ -834,9 +778,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 if (W == 2) hi += kpart * kBlock, lo += kpart * kBlock;
                 uint4 x[4];
                 int at[4];
-                const float w = kr >= L ? 0.f : (REV ? pw[kr + 1] : pw[L - e - kr]) * bscale;
-                const T w0 = Elem<T>::store(w);
-                const uint32_t wh = pack2<T>(w, w), nh = wh ^ 0x80008000u, nl = pack2<T>(Elem<T>::load(w0) - w, Elem<T>::load(w0) - w);
+                const float wj = kr >= L ? 0.f : REV ? pw[kr + 1] : pw[L - e - kr];
                 auto fetch = [&](int j0) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -844,16 +786,46 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                         x[j] = *reinterpret_cast<const uint4*>(hi + at[j]);
                     }
                 };
-                // The scores' scale: in fp16 a power of two by which the largest that this row can have stays in range, and the
-                // output's to undo it.
-                const float unit = F16 ? fminf(range_scale(__float_as_uint(most[(cc & 1) * kChunk + row])), 0x1p40f) : p.scale;
-                const float back = F16 ? p.scale * inverse2(unit) : 1.f;
                 ok = wait_for(&full[nk % kRing], nk / kRing & 1) && ok;
-                fetch(0);
+                if constexpr (F16) {
+                    float m = 0.f;
+                    if (W == 2) fetch(4), m = largest16(x);
+                    fetch(0), m = fmaxf(m, largest16(x));
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, kr < L ? __float_as_uint(m * wj) : 0u);
+                    if (lane == 0) tops[warp] = __uint_as_float(top);
+                } else {
+                    fetch(0);
+                }
                 ok = wait_for(s_full, cc & 1) && ok;  // the scores are done: b may be overwritten
                 if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 if (!(ok = epi_sync(ok))) break;      // and the last output has left the staging
                 tc_fence_after();
+                if constexpr (F16) {
+                    // b's scale stays while its weighted rows are between 2^5 and 2^15; a state that has it follows a new one.
+                    const float top = largest8(tops);
+                    if (top > 0.f && !(top * bscale >= 32.f && top * bscale < 32768.f)) {
+                        const float s = weight_scale(top, pw[kChunk]);
+                        if (!EXACT && has_g && s != bscale) {
+                            const float f = s * inverse2(bscale);
+                            for (int c = 0; c < 32 * W; c += 16)
+                                if (col0 + c < p.nb) {
+                                    float v[16];
+                                    tmem_ld16(tq + kOld + col0 + c, v);
+                                    tmem_wait_ld();
+                                    reg_fence(v);
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) v[j] *= f;
+                                    tmem_st16(tq + kOld + col0 + c, reinterpret_cast<const uint32_t(&)[16]>(v));
+                                }
+                            tmem_wait_st();
+                            tc_fence_before();
+                        }
+                        bscale = s;
+                    }
+                }
+                const float w = wj * bscale;
+                const T w0 = Elem<T>::store(w);
+                const uint32_t wh = pack2<T>(w, w), nh = wh ^ 0x80008000u, nl = pack2<T>(Elem<T>::load(w0) - w, Elem<T>::load(w0) - w);
 #pragma unroll
                 for (int j0 = 0; j0 < 4 * W; j0 += 4) {
                     if (j0 > 0) fetch(j0);
@@ -892,6 +864,36 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                 // here: loads from a table in shared memory wait for the products' operands, which go first (a block of 32
                 // columns took 1100 cycles so, 700 now; 8 heads of 65536 tokens, size 128: 228 -> 217 us; with two blocks
                 // per SM, which wait in turn, no difference).
+                float unit = p.scale, back = 1.f;
+                if constexpr (F16) {
+                    // The row's scale: its largest score, each 16 columns weighted as the nearest (for weights above 1: the furthest) of
+                    // them, goes to between 2^14 and 2^15; the output's undoes it.  The other half of the row is another warp's.
+                    float m = 0.f;
+#pragma unroll 1
+                    for (int bl = 0; bl < 2; ++bl) {
+                        const int blk = half * 2 + bl;
+                        if (REV ? blk < quad : blk > quad) continue;
+                        float v[32];
+                        tmem_ld32(tq + blk * 32, v);
+                        tmem_wait_ld();
+                        reg_fence(v);
+                        if (blk == quad || L < kChunk) {
+                            const uint32_t seen = (blk != quad ? 0xffffffffu : REV ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane)) & keep_low(L - blk * 32);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!(seen & 1u << j)) v[j] = 0.f;
+                        }
+                        float near = 0.f, far = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) near = fmaxf(near, fabsf(v[j])), far = fmaxf(far, fabsf(v[j + 16]));
+                        const int d = REV ? blk * 32 - row : row - blk * 32 - 15, d2 = REV ? d + 16 : d - 16;
+                        m = fmaxf(m, fmaxf(near * exp2_of((float)max(d, 0) * g2), far * exp2_of((float)max(d2, 0) * g2)));
+                    }
+                    most[half * kChunk + row] = m * grow;
+                    asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + quad) : "memory");
+                    m = fmaxf(most[row], most[kChunk + row]);
+                    unit = fminf(range_scale(__float_as_uint(m)), 0x1p40f), back = p.scale * inverse2(unit);
+                }
 #pragma unroll 1
                 for (int bl = 0; bl < 2; ++bl) {
                     const int blk = half * 2 + bl;
@@ -967,7 +969,6 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                     if (col0 + 32 * c < p.nb) tmem_ld32(tq + kKv + col0 + 32 * c, reinterpret_cast<float(&)[32]>(G[32 * c]));
                 tmem_wait_ld();
                 reg_fence(G);
-                if constexpr (F16 && !EXACT) held = bscale;
                 const float un = EXACT ? inverse2(bscale) : 1.f;
                 if constexpr (F16 && EXACT && W == 2)
 #pragma unroll
@@ -1000,10 +1001,7 @@ __global__ void __launch_bounds__(kThreads, W == 1 ? 2 : 1) decay_mix_kernel(con
                             if (col0 + j >= p.nb) G[j + m] = 0.f;
                 }
                 has_g = true;
-                if (k + 1 < t.n) {
-                    if constexpr (F16) measure(cc + 1);
-                    put_state(k + 1);
-                }
+                if (k + 1 < t.n) put_state(k + 1);
                 // ---- the output
                 ok = wait_for(o_full, cc & 1) && ok;
                 tc_fence_after();

@@ -104,6 +104,32 @@ def test_attention_beside_outliers_fp16(t, at):
             assert rel(end[:, j], end64[:, j]) <= 1.5 * U[F16] ** 2 + 60 * E
 
 
+@pytest.mark.parametrize("b, t, d", [(2, 900, 64), (1, 900, 128), (60, 1100, 32), (100, 1100, 128)])
+@pytest.mark.parametrize("with_state", [False, True])
+def test_attention_of_chunks_of_unlike_sizes_fp16(b, t, d, with_state):
+    """Keys, values and gradients that grow and shrink from one chunk to the next: a state goes on through all of them."""
+    g, h = gen(t + d), 3
+    size = torch.tensor([1.0, 2.0**-9, 2.0**6, 0.0, 2.0**-6, 2.0**7, 2.0**-12, 1.0, 2.0**3], device="cuda").repeat_interleave(128)[:t, None]
+    q, k, v, do = (heads(g, b, h, t, d, F32) for _ in range(4))
+    q, k, v, do = q.to(F16), (k * size).to(F16), (v * size.flip(0)).to(F16), (do * size * 2.0**-4).to(F16)
+    dec = torch.tensor([-0.05, -0.004, 0.0], device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = ops.decay_attention(*leaves, dec, return_state=with_state)
+    o, end = out if with_state else (out, None)
+    got = torch.autograd.grad(o, leaves, do)
+    l64 = [x.detach().double().requires_grad_() for x in leaves]
+    o64, end64 = attention64(*l64, dec)
+    want = torch.autograd.grad(o64, l64, do.double())
+    for j in range(h):
+        for name, a, c in zip(("o", "dq", "dk", "dv"), (o, *got), (o64, *want)):
+            for n in range(0, t, 128):
+                a_, c_ = a[:, j, n : n + 128], c[:, j, n : n + 128]
+                if float(c_.abs().max()) < 60000:  # (else the result itself is out of fp16's range)
+                    assert not off(a_, c_, F16), (name, j, n, rel(a_, c_) / U[F16])
+        if with_state:
+            assert rel(end[:, j], end64[:, j]) <= 1.5 * U[F16] ** 2 + 60 * E
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_attention_of_growing_heads(dtype):
     """log_decay a little above 0: weights above 1 go the same way."""
