@@ -39,15 +39,16 @@ struct SandwichArgs {
     int act;
 };
 
-// The sigmoids of |z| and -|z|: neither is a difference, so that both keep their digits however far z is from 0.
-// (expf is good to 2 units in the last place, the hardware's reciprocal of a number from 1 to 2 to 1.  The hardware's
-// exponential is off by 2 + 1.17 |z| of them, 1.1e-5 at 80, below a 30th of a 16-bit rounding and hence good enough for 16-bit
-// gates: 131072x1024 training 623 us, 653 with expf.)
+// The sigmoids q of z and p of -z: neither is a difference, so that both keep their digits however far z is from 0.  (Where e^-z
+// overflows, below -88, q is 0 and p only has to be finite.)
+// (expf is good to 2 units in the last place, the hardware's reciprocal to 1.  The hardware's exponential is off by 2 + 1.17 |z|
+// of them, 1.1e-5 at 80, below a 30th of a 16-bit rounding and hence good enough for 16-bit gates: 131072x1024 training 604-615
+// us, 653 with expf of -|z|.)
 template <typename T>
-__device__ __forceinline__ void sigmoids(float z, float& above, float& below) {
-    const float e = sizeof(T) == 2 ? __expf(-fabsf(z)) : expf(-fabsf(z));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(above) : "f"(1.f + e));
-    below = e * above;
+__device__ __forceinline__ void sigmoids(float z, float& q, float& p) {
+    const float e = sizeof(T) == 2 ? __expf(-z) : expf(-z);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
+    p = fminf(e, 3e38f) * q;
 }
 
 // Rows on their way.  A row's two reductions follow one another, so a group
@@ -79,26 +80,25 @@ __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group
 // act(g), and with SLOPE its derivative in d: q(z) q(-z) for the sigmoid q, q(z) (1 + z q(-z)), and 4 q(2z) q(-2z) for tanh.
 template <typename T, bool SLOPE, int N>
 __device__ __forceinline__ void gate_values(float (&v)[N], float (&d)[N], int act) {
-    float above, below;
+    float q, p;
     if (act == LF_GATE_SIGMOID) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            sigmoids<T>(v[j], above, below);
-            if (SLOPE) d[j] = above * below;
-            v[j] = v[j] < 0.f ? below : above;
+            sigmoids<T>(v[j], q, p);
+            if (SLOPE) d[j] = q * p;
+            v[j] = q;
         }
     } else if (act == LF_GATE_SILU) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            sigmoids<T>(v[j], above, below);
-            const float q = v[j] < 0.f ? below : above;
-            if (SLOPE) d[j] = q * __fmaf_rn(v[j], v[j] < 0.f ? above : below, 1.f);
+            sigmoids<T>(v[j], q, p);
+            if (SLOPE) d[j] = q * __fmaf_rn(v[j], p, 1.f);
             v[j] *= q;
         }
     } else if (act == LF_GATE_TANH) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            if (SLOPE) sigmoids<T>(2.f * v[j], above, below), d[j] = 4.f * above * below;
+            if (SLOPE) sigmoids<T>(2.f * v[j], q, p), d[j] = 4.f * q * p;
             v[j] = tanhf(v[j]);
         }
     } else if (SLOPE) {
