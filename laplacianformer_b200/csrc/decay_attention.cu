@@ -35,11 +35,11 @@
 // bf16, size 64: 208 us, 5.2 TB/s.  8x16x16384x64: 240 us and 45 us for the
 // sums, since 256 segments leave 40 slots empty.  A training step is four mixes
 // and two sums (dq takes the forward's, dv those of dk, transposed): 1.21 ms; with
-// four sums 1.36.  Few chunks per slot (32x2x3136x32 172 us, 128x8x196x64 148 us
-// a training step) are bound by a chunk's chain: products, weights, products,
+// four sums 1.36.  Few chunks per slot (32x2x3136x32 fp16 201 us, 128x8x196x64 bf16
+// 150 us a training step) are bound by a chunk's chain: products, weights, products,
 // output, about 5200 cycles for a pair of blocks.
 // Between 64 and 128 one block fits an SM and waits on that chain alone: 8 heads
-// of 65536 tokens, size 128: 210 us, 2.6 TB/s.
+// of 65536 tokens, size 128: 216 us, 2.5 TB/s.
 // A token at a time only the state matters: 192x16 heads of 64: 15 us, 6.7 TB/s.
 #include <algorithm>
 #include <type_traits>

@@ -12,7 +12,7 @@
 // where all digits are gone at 2^53); then the sine and cosine of the fraction
 // in 32 bits.
 //
-// Measured, bf16, queries and keys of 8x16x16384x64: 213 us a pass, 5.0 TB/s
+// Measured, bf16, queries and keys of 8x16x16384x64: 215 us a pass, 5.0 TB/s
 // (the copies of the next two tiles are in flight while one is turned; with
 // loads when a tile's turn came 330 us).
 #include <math.h>
