@@ -104,12 +104,12 @@ def test_attention_beside_outliers_fp16(t, at):
             assert rel(end[:, j], end64[:, j]) <= 1.5 * U[F16] ** 2 + 60 * E
 
 
-@pytest.mark.parametrize("b, t, d", [(2, 900, 64), (1, 900, 128), (60, 1100, 32), (100, 1100, 128)])
+@pytest.mark.parametrize("b, t, d", [(2, 900, 64), (1, 900, 128), (60, 1100, 32), (100, 1100, 128), (20, 2000, 64), (10, 2000, 128)])
 @pytest.mark.parametrize("with_state", [False, True])
 def test_attention_of_chunks_of_unlike_sizes_fp16(b, t, d, with_state):
     """Keys, values and gradients that grow and shrink from one chunk to the next: a state goes on through all of them."""
     g, h = gen(t + d), 3
-    size = torch.tensor([1.0, 2.0**-9, 2.0**6, 0.0, 2.0**-6, 2.0**7, 2.0**-12, 1.0, 2.0**3], device="cuda").repeat_interleave(128)[:t, None]
+    size = torch.tensor([1.0, 2.0**-9, 2.0**6, 0.0, 2.0**-6, 2.0**7, 2.0**-12, 1.0, 2.0**3], device="cuda").repeat(2).repeat_interleave(128)[:t, None]
     q, k, v, do = (heads(g, b, h, t, d, F32) for _ in range(4))
     q, k, v, do = q.to(F16), (k * size).to(F16), (v * size.flip(0)).to(F16), (do * size * 2.0**-4).to(F16)
     dec = torch.tensor([-0.05, -0.004, 0.0], device="cuda")
